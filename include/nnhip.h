@@ -654,6 +654,99 @@ nnhip_status nnhip_argmax_cols(nnhip_ctx* ctx, const float* logits, size_t V, si
  * ids (the embedding gather that read them ran earlier on the stream). */
 nnhip_status nnhip_argmax_rows(nnhip_ctx* ctx, const float* logits, size_t V, size_t B, int32_t* ids, int32_t* pos);
 
+/* ---- paged KV cache: sequences of unlike lengths whose keys and values lie in pages of a common
+ *      pool. No counterpart in the reference, which gives every sequence a cache of its own length
+ *      (compute_layer_gpt.hpp:764-765); for servers that start and end sequences at any step. ---- */
+
+/* One layer's paged cache. k / v: pools (num_pages, Hkv, page_size, dk) of f32, or f16 bit patterns when
+ * f16 != 0 (compute = F16), 16-byte aligned; page_size a power of two in [1, 1024]. table: DEVICE
+ * (B, table_stride) int32, entry (b, i) = the page that holds positions [i * page_size, (i + 1) *
+ * page_size) of sequence b; entries past a sequence's length may be anything. Sequences may share pages
+ * that no call writes. Every id that a call uses is checked on the device: one outside [0, num_pages)
+ * is never followed (each entry point says what its sequence gets). dk in {64, 128, 256} (the prompt
+ * attention: 64 or 128); num_pages * Hkv * page_size < 2^31. */
+typedef struct nnhip_kv_pages
+{
+    void* k;
+    void* v;
+    const int32_t* table;
+    size_t num_pages, page_size, table_stride, Hkv, dk;
+    int f16;
+} nnhip_kv_pages;
+
+/* Write the keys and values of packed prompts: k / v (Hkv*dk, M) feature-major, columns cu[b] ..
+ * cu[b+1] - 1 = the new tokens of sequence b (cu: DEVICE (B + 1) int32, not falling, cu[B] <= M), token t at
+ * position pos0[b] + t (pos0: DEVICE (B) int32, or NULL for 0). Keys are rotated at their positions with
+ * rope_cos / rope_sin (rope_len, dk/2) from nnhip_rope_table (both NULL: no position encoding), bit for
+ * bit as nnhip_kv_cache_fill's; f16 pools get the nearest f16. Not written: columns of no sequence
+ * (cu[B] and on), positions at or past table_stride * page_size or rope_len, pages outside the pool.
+ * Two tokens of one call at one place of the pool leave either there. The paged form of
+ * nnhip_kv_cache_fill (compute_layer_attention.hpp:1040-1060). */
+nnhip_status nnhip_kv_pages_fill(nnhip_ctx* ctx, const nnhip_kv_pages* cache, const float* k, const float* v,
+                                 size_t M, const int32_t* cu, const int32_t* pos0, size_t B, const float* rope_cos,
+                                 const float* rope_sin, size_t rope_len);
+
+/* nnhip_attention_decode over a paged cache: one new token for each of B sequences. q (H*dk, B), k / v
+ * (Hkv*dk, B) and out (H*dk, B), or token-major (B, H*dk), (B, Hkv*dk) with tokens != 0; pos (B) int32,
+ * DEVICE: the new token's position. Its rotated key and its value are written to their page and take
+ * part in the attention as the pool's type holds them. Scores of query head h and position j:
+ *   s = scale * rot(q_h) . K_j;  softcap > 0: s = softcap * tanh(s / softcap) (0: off);
+ *   slopes (DEVICE (H), or NULL): s += slopes[h] * (j - pos[b]);  out = softmax(s) . V over j <= pos[b].
+ * Any H / Hkv; a row all of whose scores are -infinity gives zeros.
+ * pos[b] < 0: an empty slot, out zeros, nothing written; pos[b] >= len_bound: out NaN, nothing written;
+ * a page outside the pool among positions [0, pos[b]]: out NaN. len_bound <= table_stride * page_size
+ * and (with tables) rope_len. Two sequences of one call whose new tokens fall on one place of the pool
+ * leave either there. Sums and softmax are f32 in an order of the kernel's own, the same in every call
+ * of the same sizes (compute_layer_attention.hpp:1022-1083). */
+nnhip_status nnhip_attention_pages_decode(nnhip_ctx* ctx, const nnhip_kv_pages* cache, const float* q, const float* k,
+                                          const float* v, size_t B, size_t H, const int32_t* pos, size_t len_bound,
+                                          const float* rope_cos, const float* rope_sin, size_t rope_len, float scale,
+                                          float softcap, const float* slopes, int tokens, float* out);
+
+/* Scratch that nnhip_attention_pages_decode (nnhip_logits_adjust_rows) of these sizes uses. The context
+ * keeps one for each stream that it was set to, grown on demand and freed with the context only, so that a
+ * captured call stays valid; a call that would have to grow it during a capture fails with
+ * NNHIP_ERR_UNSUPPORTED (call once before, on the capture's stream). Captured calls of one stream share
+ * its scratch: their replays must not overlap. */
+size_t nnhip_attention_pages_workspace_bytes(nnhip_ctx* ctx, size_t B, size_t H, size_t Hkv, size_t dk,
+                                             size_t len_bound);
+size_t nnhip_logits_workspace_bytes(nnhip_ctx* ctx, size_t V, size_t B);
+
+/* What is done to a batch's logits before the choice; every pointer is DEVICE memory and may be NULL.
+ * For token v of sequence b, with c = counts[b][v] (values below 0 count as 0), in this order, each step
+ * rounded to f32:
+ *   c > 0: x = x > 0 ? x / repeat[b] : x * repeat[b];  x -= frequency[b] * c;  x -= presence[b];
+ *   x += bias[b][v];  a clear bit v of allowed[b]: x = -infinity.
+ * counts (B, V) int32; repeat, frequency, presence (B) f32, used with counts only; bias and allowed: row b
+ * at bias + b * bias_stride (V floats) and allowed + b * allowed_stride (ceil(V / 32) words, bit v % 32 of
+ * word v / 32), stride 0: one row for all. count_choice != 0: counts[b][ids[b]] += 1 after the choice. */
+typedef struct nnhip_logit_rules
+{
+    int32_t* counts;
+    const float* repeat;
+    const float* presence;
+    const float* frequency;
+    const float* bias;
+    size_t bias_stride;
+    const uint32_t* allowed;
+    size_t allowed_stride;
+    int count_choice;
+} nnhip_logit_rules;
+
+/* Adjust token-major logits (B, V) by the rules and choose greedily: ids[b] = nnhip_argmax_rows's choice
+ * among the allowed tokens (best = the first allowed one, then every larger value replaces it); -1 where
+ * no token is allowed, whose counts and pos stay. out (B, V), or NULL: the adjusted logits (may be the
+ * logits themselves). pos, or NULL: pos[b] += 1 after a choice. ids may be NULL where out is given (then
+ * counts and pos must not be changed: count_choice == 0, pos NULL). The greedy rule of the reference
+ * (compute_layer_base.hpp:1152-1160) behind rules that it does not have. */
+nnhip_status nnhip_logits_adjust_rows(nnhip_ctx* ctx, const float* logits, size_t V, size_t B,
+                                      const nnhip_logit_rules* rules, float* out, int32_t* ids, int32_t* pos);
+
+/* counts[b][ids[m]] += 1 for the tokens m in [cu[b], cu[b+1]) of each sequence (ids (M), cu (B + 1), DEVICE;
+ * ids outside [0, V) are left out): the counts of a prompt. */
+nnhip_status nnhip_token_counts_add(nnhip_ctx* ctx, const int32_t* ids, size_t M, const int32_t* cu, size_t B,
+                                    size_t V, int32_t* counts);
+
 /* Y = res + the gated block of nnhip_ffn_glu_i8 on X (res (d, M) f32, must not alias Y): the second
  * residual add of GPTBlock::forward_step in fc2's launch (decode GEMV or prefill GEMM epilogue). Same bits as
  * nnhip_ffn_glu_i8 then nnhip_add(res, Y) (compute_layer_gpt.hpp:212-218). */

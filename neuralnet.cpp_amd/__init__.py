@@ -52,6 +52,16 @@ class GemvDesc(ctypes.Structure):
                 ("M", ctypes.c_uint64)]
 
 
+class _KVPagesDesc(ctypes.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("table", _vp), ("num_pages", _sz), ("page_size", _sz),
+                ("table_stride", _sz), ("Hkv", _sz), ("dk", _sz), ("f16", _st)]
+
+
+class _LogitRulesDesc(ctypes.Structure):
+    _fields_ = [("counts", _vp), ("repeat", _vp), ("presence", _vp), ("frequency", _vp), ("bias", _vp),
+                ("bias_stride", _sz), ("allowed", _vp), ("allowed_stride", _sz), ("count_choice", _st)]
+
+
 # name -> (restype, argtypes); every nnhip_* symbol of include/nnhip.h
 SIGNATURES = {
     "nnhip_last_error": (ctypes.c_char_p, []),
@@ -153,6 +163,13 @@ SIGNATURES = {
     "nnhip_embedding_gather_tokens": (_st, [_vp, _vp, _vp, _sz, _sz, _sz, _vp]),
     "nnhip_argmax_cols": (_st, [_vp, _vp, _sz, _sz, _vp]),
     "nnhip_argmax_rows": (_st, [_vp, _vp, _sz, _sz, _vp, _vp]),
+    "nnhip_kv_pages_fill": (_st, [_vp, _vp, _vp, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _sz]),
+    "nnhip_attention_pages_decode": (_st, [_vp, _vp, _vp, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _vp, _sz, _f, _f, _vp,
+                                           _st, _vp]),
+    "nnhip_attention_pages_workspace_bytes": (_sz, [_vp, _sz, _sz, _sz, _sz, _sz]),
+    "nnhip_logits_workspace_bytes": (_sz, [_vp, _sz, _sz]),
+    "nnhip_logits_adjust_rows": (_st, [_vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp]),
+    "nnhip_token_counts_add": (_st, [_vp, _vp, _sz, _vp, _sz, _sz, _vp]),
 }
 
 ACT_SWIGLU, ACT_RELU2GLU = 0, 1
@@ -233,6 +250,75 @@ def device_name(device: int = 0) -> str:
 
 def kp(K: int) -> int:
     return (K + TILE_K - 1) // TILE_K * TILE_K
+
+
+def _device_args(named):
+    """Checks (name, tensor or None, dtypes, shape or None) tuples: device, contiguity, type and shape, all
+    on one device."""
+    dev = None
+    for name, t, dtypes, shape in named:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise NNHipError(1, f"{name} must be a device tensor")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise NNHipError(1, f"{name} is on {t.device}, other operands on {dev}")
+        if not t.is_contiguous():
+            raise NNHipError(1, f"{name} must be contiguous")
+        if t.dtype not in dtypes:
+            raise NNHipError(1, f"{name} has dtype {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
+        if shape is not None and tuple(t.shape) != shape:
+            raise NNHipError(1, f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    return dev
+
+
+class KVPages:
+    """One layer's paged KV cache (nnhip_kv_pages): pools k, v (num_pages, Hkv, page_size, dk), float32 or
+    float16, and the page table (B, pages per sequence) int32, whose rows the sequences of a call are. The
+    tensors' contents may change between calls (the table's too); the tensors themselves stay."""
+
+    def __init__(self, k, v, table):
+        import torch
+        if k.dim() != 4 or table.dim() != 2:
+            raise NNHipError(1, "pools must be (num_pages, Hkv, page_size, dk), the table (B, pages)")
+        self.device = _device_args([("k", k, (torch.float32, torch.float16), None), ("v", v, (k.dtype,), tuple(k.shape)),
+                                    ("table", table, (torch.int32,), None)])
+        self.k, self.v, self.table = k, v, table
+        self.num_pages, self.Hkv, self.page_size, self.dk = k.shape
+        self.rows, self.max_pages = table.shape
+        self.desc = _KVPagesDesc(k.data_ptr(), v.data_ptr(), table.data_ptr(), self.num_pages, self.page_size,
+                                 self.max_pages, self.Hkv, self.dk, int(k.dtype == torch.float16))
+        self.ref = ctypes.addressof(self.desc)
+
+
+class LogitRules:
+    """What nnhip_logits_adjust_rows does to a batch's logits over a vocabulary of V (nnhip_logit_rules): counts
+    (B, V) int32, repeat / presence / frequency (B) float32, bias (B, V) or (1, V) float32, allowed
+    (B, ceil(V/32)) or (1, ceil(V/32)) int32 words of a bit per token; each may be None. With count_choice the
+    chosen tokens are counted. The tensors' contents may change between calls."""
+
+    def __init__(self, V: int, counts=None, repeat=None, presence=None, frequency=None, bias=None, allowed=None,
+                 count_choice: bool = False):
+        import torch
+        f32, i32, words = (torch.float32,), (torch.int32,), (V + 31) // 32
+        rows = [t.shape[0] for t in (counts, repeat, presence, frequency) if t is not None]
+        rows += [t.shape[0] for t in (bias, allowed) if t is not None and t.shape[0] != 1]
+        if any(r != rows[0] for r in rows):
+            raise NNHipError(1, f"the rules' rows differ: {rows}")
+        self.rows, self.V = rows[0] if rows else None, V  # rows: None fits any batch
+        self.device = _device_args(
+            [("counts", counts, i32, (self.rows, V)), ("repeat", repeat, f32, (self.rows,)),
+             ("presence", presence, f32, (self.rows,)), ("frequency", frequency, f32, (self.rows,)),
+             ("bias", bias, f32, None if bias is None else (bias.shape[0], V)),
+             ("allowed", allowed, i32, None if allowed is None else (allowed.shape[0], words))])
+        self.tensors = (counts, repeat, presence, frequency, bias, allowed)
+        p = [None if t is None else t.data_ptr() for t in self.tensors]
+        self.desc = _LogitRulesDesc(p[0], p[1], p[2], p[3], p[4], V if bias is not None and bias.shape[0] > 1 else 0,
+                                    p[5], words if allowed is not None and allowed.shape[0] > 1 else 0,
+                                    int(count_choice))
+        self.ref = ctypes.addressof(self.desc)
 
 
 class Context:
@@ -824,6 +910,112 @@ class Context:
                                        self._dev(out, torch.int32, "out"), self._dev(pos, torch.int32, "pos")),
                "nnhip_argmax_rows")
         return out
+
+    # -- paged KV cache, adjusted logits
+    def _arg(self, t, dtype, shape, name):
+        """The device address of t (None: null) after its checks: this context's device, contiguous, type, shape."""
+        if t is None:
+            return None
+        if t.device != self._device:
+            raise NNHipError(1, f"{name} is on {t.device}, the context on {self._device}")
+        if not t.is_contiguous():
+            raise NNHipError(1, f"{name} must be contiguous")
+        if t.dtype is not dtype:
+            raise NNHipError(1, f"{name} has dtype {t.dtype}, expected {dtype}")
+        if t.shape != shape:
+            raise NNHipError(1, f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+        return t.data_ptr()
+
+    def _rope(self, cos, sin, dk: int):
+        """Addresses and rows of the rope tables (None, None, 0 without)."""
+        if cos is None and sin is None:
+            return None, None, 0
+        if cos is None or sin is None:
+            raise NNHipError(1, "cos and sin go together")
+        shape = (cos.shape[0], dk // 2)
+        f32 = self._torch.float32
+        return self._arg(cos, f32, shape, "cos"), self._arg(sin, f32, shape, "sin"), shape[0]
+
+    def _packed(self, cache, cu, pos0):
+        """The sequences of a packed call (cu (B + 1), pos0 (B) or None): B and both addresses."""
+        if cache.device != self._device:
+            raise NNHipError(1, f"the cache is on {cache.device}, the context on {self._device}")
+        B, i32 = cu.shape[0] - 1, self._torch.int32
+        if B < 0 or B > cache.rows:
+            raise NNHipError(1, f"cu must hold B + 1 offsets, B at most the page table's {cache.rows} rows")
+        return B, self._arg(cu, i32, (B + 1,), "cu"), self._arg(pos0, i32, (B,), "pos0")
+
+    def kv_pages_fill(self, cache, k, v, cu, pos0=None, cos=None, sin=None) -> None:
+        """The keys and values k / v (Hkv*dk, M) of packed prompts (sequence b: columns cu[b] .. cu[b+1] - 1,
+        positions pos0[b] on) rotated into the pages of cache, a KVPages."""
+        B, cu_p, pos0_p = self._packed(cache, cu, pos0)
+        f32, M = self._torch.float32, k.shape[-1]
+        cs, sn, rows = self._rope(cos, sin, cache.dk)
+        shape = (cache.Hkv * cache.dk, M)
+        self._bind_stream()
+        _check(lib().nnhip_kv_pages_fill(self.h, cache.ref, self._arg(k, f32, shape, "k"), self._arg(v, f32, shape, "v"),
+                                         M, cu_p, pos0_p, B, cs, sn, rows), "nnhip_kv_pages_fill")
+
+    def attention_pages_decode(self, cache, q, k, v, H: int, pos, len_bound: int, scale: float, cos=None, sin=None,
+                               softcap: float = 0.0, slopes=None, out=None, tokens: bool = False):
+        """Attention of one new token per sequence over the pages of cache (a KVPages, whose table has B rows),
+        which also get its key and value: q (H*dk, B), k / v (Hkv*dk, B), or token-major (B, ...) with tokens;
+        pos (B) int32 device, below 0 for an empty slot. softcap > 0 caps the scores, slopes (H) bias them by
+        distance. Returns out like q."""
+        if cache.device != self._device:
+            raise NNHipError(1, f"the cache is on {cache.device}, the context on {self._device}")
+        f32, dk, B = self._torch.float32, cache.dk, pos.shape[0]
+        if B > cache.rows:
+            raise NNHipError(1, f"{B} sequences, the page table has {cache.rows} rows")
+        qs, ks = ((B, H * dk), (B, cache.Hkv * dk)) if tokens else ((H * dk, B), (cache.Hkv * dk, B))
+        if out is None:
+            out = self._empty(qs, f32)
+        cs, sn, rows = self._rope(cos, sin, dk)
+        self._bind_stream()
+        _check(lib().nnhip_attention_pages_decode(
+            self.h, cache.ref, self._arg(q, f32, qs, "q"), self._arg(k, f32, ks, "k"), self._arg(v, f32, ks, "v"), B, H,
+            self._arg(pos, self._torch.int32, (B,), "pos"), len_bound, cs, sn, rows, scale, softcap,
+            self._arg(slopes, f32, (H,), "slopes"), int(tokens), self._arg(out, f32, qs, "out")),
+            "nnhip_attention_pages_decode")
+        return out
+
+    def attention_pages_workspace_bytes(self, B: int, H: int, Hkv: int, dk: int, len_bound: int) -> int:
+        return int(lib().nnhip_attention_pages_workspace_bytes(self.h, B, H, Hkv, dk, len_bound))
+
+    def logits_workspace_bytes(self, V: int, B: int) -> int:
+        return int(lib().nnhip_logits_workspace_bytes(self.h, V, B))
+
+    def logits_adjust_rows(self, logits, rules=None, ids=None, out=None, pos=None):
+        """Token-major logits (B, V) adjusted by rules (a LogitRules, or None) and the greedy choice among the
+        allowed tokens into ids (B) int32 (-1: nothing is allowed), made when neither ids nor out is given. out
+        (B, V), when given, gets the adjusted logits (it may be logits itself); pos (B) int32 is advanced by one
+        after a choice. Returns ids."""
+        B, V = logits.shape
+        f32, i32 = self._torch.float32, self._torch.int32
+        if rules is not None:
+            if rules.V != V or rules.rows not in (None, B):
+                raise NNHipError(1, f"rules for {(rules.rows, rules.V)}, logits of {(B, V)}")
+            if rules.device not in (None, self._device):
+                raise NNHipError(1, f"the rules are on {rules.device}, the context on {self._device}")
+        if ids is None and out is None:
+            ids = self._empty((B,), i32)
+        self._bind_stream()
+        _check(lib().nnhip_logits_adjust_rows(
+            self.h, self._arg(logits, f32, (B, V), "logits"), V, B, None if rules is None else rules.ref,
+            self._arg(out, f32, (B, V), "out"), self._arg(ids, i32, (B,), "ids"), self._arg(pos, i32, (B,), "pos")),
+            "nnhip_logits_adjust_rows")
+        return ids
+
+    def token_counts_add(self, ids, cu, counts):
+        """counts (B, V) int32 [b, ids[m]] += 1 for the tokens m of each packed sequence (cu (B + 1))."""
+        i32 = self._torch.int32
+        B, V = counts.shape
+        M = ids.shape[0]
+        self._bind_stream()
+        _check(lib().nnhip_token_counts_add(self.h, self._arg(ids, i32, (M,), "ids"), M,
+                                            self._arg(cu, i32, (B + 1,), "cu"), B, V,
+                                            self._arg(counts, i32, (B, V), "counts")), "nnhip_token_counts_add")
+        return counts
 
     # -- gated feed-forward block
     def glu(self, Y1, act: int = ACT_SWIGLU):

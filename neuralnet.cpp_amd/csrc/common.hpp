@@ -381,4 +381,21 @@ hipError_t launch_embed(hipStream_t st, const float* table, const int32_t* ids, 
 hipError_t launch_argmax(hipStream_t st, const float* L, size_t V, size_t B, int32_t* ids, bool rows = false,
                          int32_t* pos = nullptr);
 
+// ---- paged KV cache (k_pages.hip; the prompt attention k_prefill.hip), logits (k_logits.hip)
+size_t pages_chunk(size_t B, size_t Hkv, size_t R, size_t len_bound, size_t num_cus);
+size_t pages_workspace_bytes(size_t B, size_t H, size_t Hkv, size_t dk, size_t len_bound, size_t num_cus);
+hipError_t launch_pages_attn(hipStream_t st, const nnhip_kv_pages& kv, const float* q, const float* k, const float* v,
+                             size_t B, size_t H, const int32_t* pos, size_t len_bound, const float* cosT,
+                             const float* sinT, float scale, float softcap, const float* slopes, bool tokens,
+                             float* part, float* out, size_t num_cus);
+hipError_t launch_pages_fill(hipStream_t st, const nnhip_kv_pages& kv, const float* k, const float* v, size_t M,
+                             const int32_t* cu, const int32_t* pos0, size_t B, const float* cosT, const float* sinT,
+                             size_t limit);
+size_t logits_slices(size_t V, size_t B, size_t num_cus);
+size_t logits_workspace_bytes(size_t V, size_t B, size_t num_cus);
+hipError_t launch_logits_adjust(hipStream_t st, const float* logits, size_t V, size_t B, const nnhip_logit_rules& rules,
+                                float* out, int32_t* ids, int32_t* pos, void* ws, size_t num_cus);
+hipError_t launch_token_counts(hipStream_t st, const int32_t* ids, size_t M, const int32_t* cu, size_t B, size_t V,
+                               int32_t* counts);
+
 }  // namespace nnhip

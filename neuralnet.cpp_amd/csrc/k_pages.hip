@@ -1,0 +1,740 @@
+// k_pages.hip — the paged KV cache: keys and values of sequences of unlike lengths in pages of a
+// common pool, found through a page table. Here its fill from packed prompts and the attention of
+// one new token per sequence; the attention of packed prompts is k_prefill.hip's.
+//
+// Layouts (device):
+//   pools   (num_pages, Hkv, page_size, dk) f32 or f16, keys and values apart: a page holds page_size
+//           consecutive positions of one sequence, and one head's rows of a page lie in one run
+//   table   (B, table_stride) int32: entry (b, i) = the page of positions [i * page_size, (i + 1) *
+//           page_size) of sequence b. Entries past a sequence's length are never read.
+//   q, out  (H*dk, n) or token-major (n, H*dk); k, v the same with Hkv heads
+//
+// No id of the table is followed before it is checked against num_pages: a sequence with a bad one
+// among its positions gets NaN outputs, and a bad page is never written.
+#include "common.hpp"
+#include "pages_index.hpp"
+
+#include <cmath>
+#include <type_traits>
+#include <utility>
+
+namespace nnhip
+{
+namespace
+{
+
+constexpr int kPgThreads = 256;  // 4 waves
+constexpr int kPgWaves = kPgThreads / kWave;
+constexpr int kPgU = 4;          // rows of a group of 16 lanes in flight together
+constexpr int kPgTile = 16;      // rows of a wave's tile: 4 groups x kPgU
+constexpr int kPgMaxR = 8;       // query heads of a work-group
+constexpr int kPgRec = 16;       // tail of a record: maximum[8], sum[8]
+constexpr int kPgMaxChunk = 1024;
+constexpr float kPgLazy = 8.0f;  // log2 growth of a maximum before its sums are rescaled
+
+struct PagesArgs
+{
+    const float* q;
+    const float* k;
+    const float* v;
+    const int32_t* pos;
+    const float* cosT;
+    const float* sinT;
+    void* kc;
+    void* vc;
+    const int32_t* table;
+    const float* slopes;
+    float* part;
+    float* out;
+    int B, H, Hkv, R, groups, RG;  // R = H / Hkv heads of a KV head, in `groups` groups of at most RG
+    int shift;                     // log2(page_size)
+    int table_stride, num_pages, len_bound, chunk, nchunk;
+    float scale2;  // scale * log2(e)
+    float capi;    // scale / softcap
+    float cap2;    // softcap * log2(e), 0 without a cap
+    int tokens;
+};
+
+// Two rounded products and a rounded sum per output, as the contiguous cache's append rotates.
+__device__ __forceinline__ void pg_rope(float x0, float x1, float cs, float sn, float& y0, float& y1)
+{
+    y0 = __fadd_rn(__fmul_rn(x0, cs), __fmul_rn(-x1, sn));
+    y1 = __fadd_rn(__fmul_rn(x1, cs), __fmul_rn(x0, sn));
+}
+
+template <typename F, int... I>
+__device__ __forceinline__ void static_for_each(F&& f, std::integer_sequence<int, I...>)
+{
+    (f(std::integral_constant<int, I>{}), ...);
+}
+
+// f(0), ..., f(N - 1) with constants
+template <int N, typename F>
+__device__ __forceinline__ void static_for(F&& f)
+{
+    static_for_each(f, std::make_integer_sequence<int, N>{});
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x)
+{
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, true));
+}
+constexpr int kDppXor1 = 0xB1, kDppXor2 = 0x4E, kDppHalfMirror = 0x141, kDppMirror = 0x140, kDppRor4 = 0x124,
+              kDppRor8 = 0x128, kDppBcast = 0x150;  // kDppBcast + n: lane n of each row of 16
+
+// The sums over 16 lanes of N values per lane, spread over the lanes: a level halves the lanes that
+// share a value, and while there are two values or more each lane passes one half of them on and
+// keeps the other. Lane 8 b3 + 4 b2 + 2 b1 + b0 ends with the values (16 / N of them, at least one)
+// from index N b3 / 2 + N b2 / 4 + ... on. 3 (N - 1) instructions against 4 N for every sum in every lane.
+template <int A, int CTRL, int BIT, int N>
+__device__ __forceinline__ void fold_level(float (&x)[N], int lane)
+{
+    if constexpr (A >= 2)
+    {
+        const bool up = (lane & BIT) != 0;
+#pragma unroll
+        for (int i = 0; i < A / 2; ++i)
+        {
+            const float send = up ? x[i] : x[i + A / 2], keep = up ? x[i + A / 2] : x[i];
+            x[i] = keep + dpp<CTRL>(send);
+        }
+    }
+    else x[0] += dpp<CTRL>(x[0]);
+}
+
+constexpr int half_of(int n) { return n > 1 ? n / 2 : 1; }
+
+template <int N>
+__device__ __forceinline__ void fold16(float (&x)[N], int lane)
+{
+    constexpr int N1 = half_of(N), N2 = half_of(N1), N3 = half_of(N2);
+    fold_level<N, kDppMirror, 8>(x, lane);
+    fold_level<N1, kDppHalfMirror, 4>(x, lane);
+    fold_level<N2, kDppXor2, 2>(x, lane);
+    fold_level<N3, kDppXor1, 1>(x, lane);
+}
+
+template <int LANE>
+__device__ __forceinline__ float bcast16(float x)
+{
+    return dpp<kDppBcast + LANE>(x);
+}
+
+// a's upper half of the lanes (odd rows of 16) against b's lower half (even rows), then their sum
+__device__ __forceinline__ float fold32(float a, float b)
+{
+    const auto z = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
+    const uint32_t x = z[0], y = z[1];  // (a bit cast of a vector's element takes the first one)
+    return __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y);
+}
+__device__ __forceinline__ float fold16_rows(float a, float b)
+{
+    const auto z = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
+    const uint32_t x = z[0], y = z[1];
+    return __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y);
+}
+
+// E elements of a cache row as a lane loads them: loads of W elements, 16 lanes side by side
+template <int DK, typename CT>
+struct PagesRow
+{
+    static constexpr int E = DK / 16;
+    static constexpr int W = sizeof(CT) == 4 ? 4 : (E < 8 ? E : 8);
+    static constexpr int N = E / W;               // loads
+    static constexpr int WORDS = W * (int)sizeof(CT) / 4;
+    typedef uint32_t Vec __attribute__((ext_vector_type(WORDS)));
+    Vec x[N];
+    static __device__ __forceinline__ int dim(int e, int j) { return 16 * W * (e / W) + W * j + e % W; }
+    __device__ __forceinline__ void load(const CT* row, int j)
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(row + 16 * W * i + W * j));
+    }
+    __device__ __forceinline__ void zero()
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = Vec(0u);
+    }
+    __device__ __forceinline__ float get(int e) const
+    {
+        constexpr int H = sizeof(CT) == 4 ? 1 : 2;  // elements in a word
+        const uint32_t word = x[e / W][e % W / H];
+        if constexpr (H == 1) return __builtin_bit_cast(float, word);
+        else
+        {
+            typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+            return (float)__builtin_bit_cast(h2, word)[e & 1];
+        }
+    }
+};
+
+// tanh to about 1e-7 of itself: the odd series below 0.3 (its next term is 2e-9), else from exp
+__device__ __forceinline__ float pg_tanh(float x)
+{
+    const float a = fabsf(x), z = x * x;
+    float s = -8.8632355e-3f;  // -1382 / 155925
+    s = __builtin_fmaf(s, z, 2.1869489e-2f);
+    s = __builtin_fmaf(s, z, -5.3968254e-2f);
+    s = __builtin_fmaf(s, z, 0.13333333f);
+    s = __builtin_fmaf(s, z, -0.33333333f);
+    const float small = __builtin_fmaf(x * z, s, x);
+    const float big = copysignf(1.0f - 2.0f / (__builtin_amdgcn_exp2f(a * 2.8853900f) + 1.0f), x);
+    return a < 0.3f ? small : big;
+}
+
+// Attention of one new token per sequence. Work-group = (chunk of `chunk` positions, KV head and group
+// of at most 8 of its query heads, sequence); a group of 16 lanes takes one row of dk at a time, 4 rows
+// on their way together, so a wave's tile is 16 rows; its four waves take the chunk's tiles in turn.
+// No wave waits for another before the chunk's end: each group of 16 lanes keeps running maxima, sums
+// and weighted values of its own rows. q stays in registers (each lane the elements of its columns).
+//   scores   each lane multiplies its columns, the sums over 16 lanes come out spread over them
+//            (fold16): lane 4u + s holds row u's score of head(s) s, so that the cap, the bias and the
+//            exponential are computed once per score;
+//   values   the probability of (row u, head h) is broadcast within the 16 lanes by a DPP move.
+// A head's reference maximum moves only when it has grown by 2^8.
+// The chunk that holds the new position writes its rotated key and its value to the page (no other
+// work-group reads that row) and starts the first group's sums with them.
+template <int DK, int RT, bool kFinal, typename CT>
+__global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
+{
+    using Row = PagesRow<DK, CT>;
+    constexpr int E = Row::E, HALF = DK / 2, NV = RT / 4 > 1 ? RT / 4 : 1;  // scores per lane
+    constexpr int NS = kPgU * RT;
+    __shared__ __align__(16) float q_s[RT * DK];
+    __shared__ float new_s[2][DK];
+    __shared__ int page_s[kPgMaxChunk];
+    __shared__ float ml_s[2][kPgWaves * 4][RT];
+    __shared__ float red_s[kPgWaves][RT * DK];
+
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, j = lane & 15, grp = lane >> 4;
+    const int c = blockIdx.x, b = blockIdx.z;
+    const int g = blockIdx.y / a.groups, hg = blockIdx.y - g * a.groups;
+    const int h0 = g * a.R + hg * a.RG;            // first query head
+    const int R = min(a.RG, a.R - hg * a.RG);      // query heads here (<= RT)
+    const int p = a.pos[b];
+    const size_t out_step = a.tokens ? 1 : (size_t)a.B;
+    float* const out = a.out + (a.tokens ? ((size_t)b * a.H + h0) * DK : (size_t)h0 * DK * a.B + b);
+    if (p < 0 || p >= a.len_bound)
+    {
+        // no token: zeros; a position past the bound: NaN
+        if (c == 0)
+            for (int e = tid; e < R * DK; e += kPgThreads) out[e * out_step] = p < 0 ? 0.0f : __builtin_nanf("");
+        return;
+    }
+    const int t0 = c * a.chunk;
+    if (t0 > p) return;
+    const int n = min(a.chunk, p - t0);            // cached rows here
+    const bool has_new = p - t0 < a.chunk;
+
+    // ---- rotated queries, the page of each of the chunk's pages, the new key and value
+    const size_t in_step = a.tokens ? 1 : (size_t)a.B;
+    for (int e = tid; e < RT * HALF; e += kPgThreads)
+    {
+        const int r = e / HALF, i = e - r * HALF;
+        float y0 = 0.0f, y1 = 0.0f;
+        if (r < R)
+        {
+            const float* q = a.q + (a.tokens ? ((size_t)b * a.H + h0 + r) * DK : (size_t)(h0 + r) * DK * a.B + b);
+            y0 = q[i * in_step], y1 = q[(i + HALF) * in_step];
+            if (a.cosT) pg_rope(y0, y1, a.cosT[(size_t)p * HALF + i], a.sinT[(size_t)p * HALF + i], y0, y1);
+        }
+        q_s[r * DK + i] = y0;
+        q_s[r * DK + i + HALF] = y1;
+    }
+    const int page0 = t0 >> a.shift;
+    const int pages = page_entries(t0, t0 + n - (has_new ? 0 : 1), a.shift);
+    const int32_t* table = a.table + (size_t)b * a.table_stride + page0;
+    bool bad = false;
+    for (int e = tid; e < pages; e += kPgThreads)
+    {
+        const int id = table[e];
+        const bool in = page_ok(id, a.num_pages);
+        bad |= !in;
+        page_s[e] = in ? id : 0;
+    }
+    if (has_new && tid < HALF)
+    {
+        const size_t at = a.tokens ? ((size_t)b * a.Hkv + g) * DK : (size_t)g * DK * a.B + b;
+        const float* k = a.k + at;
+        const float* v = a.v + at;
+        float y0 = k[tid * in_step], y1 = k[(tid + HALF) * in_step];
+        if (a.cosT) pg_rope(y0, y1, a.cosT[(size_t)p * HALF + tid], a.sinT[(size_t)p * HALF + tid], y0, y1);
+        // as the cache holds them (f16: rounded to nearest)
+        new_s[0][tid] = (float)(CT)y0;
+        new_s[0][tid + HALF] = (float)(CT)y1;
+        new_s[1][tid] = (float)(CT)v[tid * in_step];
+        new_s[1][tid + HALF] = (float)(CT)v[(tid + HALF) * in_step];
+    }
+    bad = __syncthreads_or(bad) != 0;
+    const int slot_mask = (1 << a.shift) - 1;
+    const CT* const kc = static_cast<const CT*>(a.kc);
+    const CT* const vc = static_cast<const CT*>(a.vc);
+    if (has_new && hg == 0 && !bad)
+    {
+        const size_t at = page_row(page_s[pages - 1], g, p & slot_mask, a.Hkv, a.shift) * DK;
+        for (int i = tid; i < 2 * DK; i += kPgThreads)
+            const_cast<CT*>(i < DK ? kc : vc)[at + (size_t)(i & (DK - 1))] = (CT)new_s[i / DK][i & (DK - 1)];
+    }
+
+    float q[RT][E];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int e = 0; e < E; ++e) q[r][e] = q_s[r * DK + Row::dim(e, j)];
+    // this lane's scores: row (lane / 4) % 4, heads hs .. hs + NV - 1
+    const int hs = RT >= 4 ? (j & 3) * NV : RT == 2 ? (j & 3) >> 1 : 0, ur = j >> 2;
+    float slope2[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) slope2[i] = a.slopes && hs + i < R ? a.slopes[h0 + hs + i] * 1.44269504f : 0.0f;
+    auto shape = [&](float dot, int i, int t) {
+        float x = a.cap2 > 0.0f ? a.cap2 * pg_tanh(dot * a.capi) : dot * a.scale2;
+        if (a.slopes) x = __builtin_fmaf(slope2[i], (float)(t - p), x);
+        return x;
+    };
+
+    float acc[RT][E], m[NV], l[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) m[i] = -__builtin_inff(), l[i] = 0.0f;
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[r][e] = 0.0f;
+
+    auto tile = [&](int base, auto full) {
+        constexpr bool kFull = decltype(full)::value;
+        Row kr[kPgU], vr[kPgU];
+        size_t at[kPgU];
+#pragma unroll
+        for (int u = 0; u < kPgU; ++u)
+        {
+            // rows behind the chunk's last read its first page's first row (their score is -inf)
+            int t = t0 + base + 4 * u + grp;
+            if (!kFull && base + 4 * u + grp >= n) t = t0;
+            at[u] = page_row(page_s[(t >> a.shift) - page0], g, t & slot_mask, a.Hkv, a.shift) * DK;
+            kr[u].load(kc + at[u], j);
+        }
+#pragma unroll
+        for (int u = 0; u < kPgU; ++u) vr[u].load(vc + at[u], j);
+        float s[NS];
+#pragma unroll
+        for (int u = 0; u < kPgU; ++u)
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+            {
+                float d = kr[u].get(0) * q[r][0];
+#pragma unroll
+                for (int e = 1; e < E; ++e) d = __builtin_fmaf(kr[u].get(e), q[r][e], d);
+                s[u * RT + r] = d;
+            }
+        fold16(s, lane);
+        float x[NV], top[NV];
+        bool grown = false;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+        {
+            const int tl = base + 4 * ur + grp;
+            x[i] = shape(s[i], i, t0 + tl);
+            if (!kFull && tl >= n) x[i] = -__builtin_inff();
+            top[i] = fmaxf(x[i], dpp<kDppRor8>(x[i]));
+            top[i] = fmaxf(top[i], dpp<kDppRor4>(top[i]));
+            grown |= top[i] > m[i] + kPgLazy;
+        }
+        if (__builtin_amdgcn_ballot_w64(grown) != 0)
+        {
+            float corr[NV];
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+            {
+                const float to = top[i] > m[i] + kPgLazy ? top[i] : m[i];
+                corr[i] = m[i] == to ? 1.0f : __builtin_amdgcn_exp2f(m[i] - to);
+                l[i] *= corr[i];
+                m[i] = to;
+            }
+            static_for<RT>([&](auto r) {
+                constexpr int h = decltype(r)::value;
+                const float f = bcast16<RT >= 4 ? h / NV : 2 * h>(corr[h % NV]);
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[h][e] *= f;
+            });
+        }
+        float pr[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+        {
+            // no score above -inf yet: nothing to add (and no -inf - -inf)
+            pr[i] = x[i] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x[i] - m[i]);
+            l[i] += pr[i];
+        }
+        static_for<kPgU>([&](auto uu) {
+            constexpr int u = decltype(uu)::value;
+            if (!kFull && base + 4 * u + grp >= n) vr[u].zero();  // whatever is there: 0 * it has to be 0
+            static_for<RT>([&](auto r) {
+                constexpr int h = decltype(r)::value;
+                const float f = bcast16<4 * u + (RT >= 4 ? h / NV : 2 * h)>(pr[h % NV]);
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[h][e] = __builtin_fmaf(f, vr[u].get(e), acc[h][e]);
+            });
+        });
+    };
+    int base = w * kPgTile;
+    for (; base + kPgTile <= n; base += kPgWaves * kPgTile) tile(base, std::true_type{});
+    if (base < n) tile(base, std::false_type{});
+
+    // ---- the new position: one more row of the first group of the first wave
+    if (has_new && w == 0)
+    {
+        float s[NS];
+#pragma unroll
+        for (int u = 0; u < kPgU; ++u)
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+            {
+                float d = 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) d = __builtin_fmaf(new_s[0][Row::dim(e, j)], q[r][e], d);
+                s[u * RT + r] = d;
+            }
+        fold16(s, lane);
+        float corr[NV], pr[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+        {
+            const float x = grp == 0 ? shape(s[i], i, p) : -__builtin_inff();
+            const float to = x > m[i] ? x : m[i];
+            corr[i] = m[i] == to ? 1.0f : __builtin_amdgcn_exp2f(m[i] - to);
+            pr[i] = x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x - to);
+            // every row of lanes holds the same score: it counts once
+            l[i] = l[i] * corr[i] + (ur == 0 ? pr[i] : 0.0f);
+            m[i] = to;
+        }
+        static_for<RT>([&](auto r) {
+            constexpr int h = decltype(r)::value;
+            const float f = bcast16<RT >= 4 ? h / NV : 2 * h>(corr[h % NV]);
+            const float y = bcast16<RT >= 4 ? h / NV : 2 * h>(pr[h % NV]);
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                acc[h][e] = __builtin_fmaf(y, grp == 0 ? new_s[1][Row::dim(e, j)] : 0.0f, acc[h][e] * f);
+        });
+    }
+
+    // ---- join: maxima and sums of the 16 groups of lanes, then their weighted values
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+    {
+        l[i] += dpp<kDppRor8>(l[i]);
+        l[i] += dpp<kDppRor4>(l[i]);
+        if (ur == 0)
+        {
+            ml_s[0][4 * w + grp][hs + i] = m[i];
+            ml_s[1][4 * w + grp][hs + i] = l[i];
+        }
+    }
+    __syncthreads();
+    constexpr int N = RT * E;
+    float y[N];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+    {
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < 4 * kPgWaves; ++i) top = fmaxf(top, ml_s[0][i][r]);
+        const float own = ml_s[0][4 * w + grp][r];
+        // (a NaN among the scores leaves its sum and values NaN, not the maximum)
+        const float f = own == top ? 1.0f : __builtin_amdgcn_exp2f(own - top);
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[r * E + e] = acc[r][e] * f;
+    }
+    // over the wave's four groups: each swap exchanges halves of two registers between halves of the
+    // lanes, and their sum holds one value in each half
+    static_assert(N % 4 == 0, "a quarter of the values per group of lanes");
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) y[i] = fold32(y[i], y[i + N / 2]);
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i)
+    {
+        const int at = i + (grp >> 1) * (N / 2) + (grp & 1) * (N / 4);
+        red_s[w][at / E * DK + Row::dim(at % E, j)] = fold16_rows(y[i], y[i + N / 4]);
+    }
+    __syncthreads();
+    float* const rec = a.part + ((((size_t)b * a.Hkv + g) * a.groups + hg) * a.nchunk + c) * (size_t)(a.RG * DK + kPgRec);
+    for (int e = tid; e < R * DK; e += kPgThreads)
+    {
+        const int r = e / DK;
+        float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4 * kPgWaves; ++i) top = fmaxf(top, ml_s[0][i][r]);
+#pragma unroll
+        for (int i = 0; i < 4 * kPgWaves; ++i)
+        {
+            const float mi = ml_s[0][i][r];
+            sum += ml_s[1][i][r] * (mi == top ? 1.0f : __builtin_amdgcn_exp2f(mi - top));
+        }
+        float v = red_s[0][e];
+#pragma unroll
+        for (int i = 1; i < kPgWaves; ++i) v += red_s[i][e];
+        if (bad) sum = __builtin_nanf("");
+        if constexpr (kFinal) out[e * out_step] = sum == 0.0f ? 0.0f : v / sum;
+        else
+        {
+            rec[e] = v;
+            if (e % DK == 0)
+            {
+                rec[a.RG * DK + r] = top;
+                rec[a.RG * DK + 8 + r] = sum;
+            }
+        }
+    }
+}
+
+// out of one (sequence, head) from its chunks' records: sum_c 2^(m_c - m) acc_c / sum_c 2^(m_c - m) l_c
+template <int DK>
+__global__ __launch_bounds__(kPgThreads) void k_pages_join(PagesArgs a)
+{
+    constexpr int L = DK / 4, G = kPgThreads / L;  // lanes of a record's row, records side by side
+    __shared__ float4 acc_s[G][L];
+    __shared__ float m_s[G], l_s[G];
+    const int h = blockIdx.x, b = blockIdx.y;
+    const int p = a.pos[b];
+    if (p < 0 || p >= a.len_bound) return;  // the chunks' kernel wrote those
+    const int g = h / a.R, r0 = h - g * a.R, hg = r0 / a.RG, r = r0 - hg * a.RG;
+    const int nch = p / a.chunk + 1;
+    const size_t step = (size_t)(a.RG * DK + kPgRec);
+    const float* rec = a.part + (((size_t)b * a.Hkv + g) * a.groups + hg) * a.nchunk * step;
+    const int tid = threadIdx.x, i = tid % L, gr = tid / L;
+    float m = -__builtin_inff(), l = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    constexpr int U = 4;  // records on their way together
+    for (int c0 = gr; c0 < nch; c0 += U * G)
+    {
+        float mc[U], lc[U];
+        float4 x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+        {
+            const int c = c0 + u * G;
+            const float* at = rec + (size_t)(c < nch ? c : c0) * step;
+            mc[u] = at[a.RG * DK + r];
+            lc[u] = at[a.RG * DK + 8 + r];
+            x[u] = reinterpret_cast<const float4*>(at + r * DK)[i];
+            if (c >= nch) mc[u] = -__builtin_inff(), lc[u] = 0.0f, x[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        float to = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u) to = fmaxf(to, mc[u]);
+        const float f = m == to ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+        l *= f, acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+        {
+            const float e = mc[u] == to ? 1.0f : __builtin_amdgcn_exp2f(mc[u] - to);
+            l = __builtin_fmaf(e, lc[u], l);
+            acc.x = __builtin_fmaf(e, x[u].x, acc.x), acc.y = __builtin_fmaf(e, x[u].y, acc.y);
+            acc.z = __builtin_fmaf(e, x[u].z, acc.z), acc.w = __builtin_fmaf(e, x[u].w, acc.w);
+        }
+        m = to;
+    }
+    acc_s[gr][i] = acc;
+    if (i == 0) m_s[gr] = m, l_s[gr] = l;
+    __syncthreads();
+    if (gr != 0) return;
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int k = 0; k < G; ++k) top = fmaxf(top, m_s[k]);
+    float sum = 0.0f;
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < G; ++k)
+    {
+        const float e = m_s[k] == top ? 1.0f : __builtin_amdgcn_exp2f(m_s[k] - top);
+        const float4 x = acc_s[k][i];
+        sum = __builtin_fmaf(e, l_s[k], sum);
+        y.x = __builtin_fmaf(e, x.x, y.x), y.y = __builtin_fmaf(e, x.y, y.y);
+        y.z = __builtin_fmaf(e, x.z, y.z), y.w = __builtin_fmaf(e, x.w, y.w);
+    }
+    const size_t st = a.tokens ? 1 : (size_t)a.B;
+    float* o = a.out + (a.tokens ? ((size_t)b * a.H + h) * DK + 4 * i : ((size_t)h * DK + 4 * i) * a.B + b);
+    const float inv = sum == 0.0f ? 1.0f : sum;
+    o[0] = y.x / inv, o[st] = y.y / inv, o[2 * st] = y.z / inv, o[3 * st] = y.w / inv;
+}
+
+template <int DK, int RT, typename CT>
+hipError_t launch_pages_rt(hipStream_t st, const PagesArgs& a)
+{
+    const dim3 grid((unsigned)a.nchunk, (unsigned)(a.Hkv * a.groups), (unsigned)a.B);
+    if (a.nchunk == 1)
+    {
+        k_pages_attn<DK, RT, true, CT><<<grid, kPgThreads, 0, st>>>(a);
+        return hipGetLastError();
+    }
+    k_pages_attn<DK, RT, false, CT><<<grid, kPgThreads, 0, st>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    k_pages_join<DK><<<dim3((unsigned)a.H, (unsigned)a.B), kPgThreads, 0, st>>>(a);
+    return hipGetLastError();
+}
+
+template <int DK, typename CT>
+hipError_t launch_pages_dk(hipStream_t st, const PagesArgs& a)
+{
+    if (a.RG == 1) return launch_pages_rt<DK, 1, CT>(st, a);
+    if (a.RG == 2) return launch_pages_rt<DK, 2, CT>(st, a);
+    if (a.RG <= 4) return launch_pages_rt<DK, 4, CT>(st, a);
+    return launch_pages_rt<DK, 8, CT>(st, a);
+}
+
+// ------------------------------------------------------------------ fill from packed prompts
+
+constexpr int kPfTok = 32;  // tokens of a work-group
+
+struct FillArgs
+{
+    const float* k;
+    const float* v;
+    const int32_t* cu;
+    const int32_t* pos0;
+    const float* cosT;
+    const float* sinT;
+    void* kc;
+    void* vc;
+    const int32_t* table;
+    int M, B, Hkv, shift, table_stride, num_pages, limit;  // limit: positions from here on are not written
+};
+
+// Work-group = (32 tokens, KV head, keys or values): the head's dk feature rows of those tokens read
+// along tokens, turned through LDS and written as rows of pages, keys rotated at their positions.
+// Where a token goes (its sequence by bisection in cu, its page) is found while its features are on
+// their way. Tokens of no sequence, positions outside the table or the rope tables and pages outside
+// the pool are not written.
+template <int DK, typename CT>
+__global__ __launch_bounds__(256) void k_pages_fill(FillArgs a)
+{
+    constexpr int HALF = DK / 2, NR = 256 / kPfTok, U = DK / NR;
+    __shared__ float x_s[DK][kPfTok + 1];
+    __shared__ int row_s[kPfTok], pos_s[kPfTok];
+    const int tid = threadIdx.x, g = blockIdx.y;
+    const bool keys = blockIdx.z == 0;
+    const int m0 = blockIdx.x * kPfTok;
+    const int c = tid % kPfTok, i0 = tid / kPfTok;
+    const float* src = (keys ? a.k : a.v) + (size_t)(g * DK + i0) * (size_t)a.M + (size_t)min(m0 + c, a.M - 1);
+    float x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = src[(size_t)(NR * u) * (size_t)a.M];
+    if (tid < kPfTok)
+    {
+        const int m = m0 + tid;
+        const int b = m < a.M ? packed_sequence(a.cu, a.B, m) : -1;
+        const int pos = b < 0 ? -1 : packed_position(a.cu, a.pos0, b, m, a.limit);
+        int row = -1;
+        if (pos >= 0)
+        {
+            const int id = a.table[(size_t)b * a.table_stride + (pos >> a.shift)];
+            if (page_ok(id, a.num_pages)) row = (int)page_row(id, g, pos & ((1 << a.shift) - 1), a.Hkv, a.shift);
+        }
+        row_s[tid] = row;
+        pos_s[tid] = pos;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) x_s[i0 + NR * u][c] = x[u];
+    __syncthreads();
+    // a thread stores features (j, j + 1) and (j + dk / 2, j + 1 + dk / 2) of its tokens
+    constexpr int J = HALF / 2, NT = 256 / J;
+    const int j = 2 * (tid % J), c0 = tid / J;
+    typedef CT v2 __attribute__((ext_vector_type(2)));
+    CT* const dst = static_cast<CT*>(keys ? a.kc : a.vc);
+#pragma unroll
+    for (int cn = c0; cn < kPfTok; cn += NT)
+    {
+        const int row = row_s[cn];
+        if (row < 0) continue;
+        float y[2][2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+        {
+            const float x0 = x_s[j + e][cn], x1 = x_s[j + e + HALF][cn];
+            y[0][e] = x0, y[1][e] = x1;
+            if (keys && a.cosT)
+            {
+                const size_t at = (size_t)pos_s[cn] * HALF + (size_t)(j + e);
+                pg_rope(x0, x1, a.cosT[at], a.sinT[at], y[0][e], y[1][e]);
+            }
+        }
+        CT* o = dst + (size_t)row * DK + j;
+        *reinterpret_cast<v2*>(o) = v2{(CT)y[0][0], (CT)y[0][1]};
+        *reinterpret_cast<v2*>(o + HALF) = v2{(CT)y[1][0], (CT)y[1][1]};
+    }
+}
+
+template <typename CT>
+hipError_t launch_pages_fill_ct(hipStream_t st, const FillArgs& a, size_t dk)
+{
+    const dim3 grid((unsigned)ceil_div(a.M, kPfTok), (unsigned)a.Hkv, 2);
+    if (dk == 64) k_pages_fill<64, CT><<<grid, 256, 0, st>>>(a);
+    else if (dk == 128) k_pages_fill<128, CT><<<grid, 256, 0, st>>>(a);
+    else if (dk == 256) k_pages_fill<256, CT><<<grid, 256, 0, st>>>(a);
+    else return hipErrorInvalidValue;
+    return hipGetLastError();
+}
+
+int log2_of(size_t v)
+{
+    int n = 0;
+    while ((size_t(1) << n) < v) ++n;
+    return n;
+}
+
+}  // namespace
+
+// Query heads of a KV head in groups of at most kPgMaxR, as even as they go
+static size_t pages_groups(size_t R) { return ceil_div(R, (size_t)kPgMaxR); }
+
+size_t pages_chunk(size_t B, size_t Hkv, size_t R, size_t len_bound, size_t num_cus)
+{
+    size_t chunk = 128;
+    while (chunk < kPgMaxChunk && B * Hkv * pages_groups(R) * ceil_div(len_bound, chunk) > 8 * num_cus) chunk *= 2;
+    return chunk;
+}
+
+size_t pages_workspace_bytes(size_t B, size_t H, size_t Hkv, size_t dk, size_t len_bound, size_t num_cus)
+{
+    const size_t R = H / Hkv, groups = pages_groups(R);
+    const size_t nchunk = ceil_div(len_bound, pages_chunk(B, Hkv, R, len_bound, num_cus));
+    return nchunk <= 1 ? 0 : B * Hkv * groups * nchunk * (ceil_div(R, groups) * dk + kPgRec) * sizeof(float);
+}
+
+hipError_t launch_pages_attn(hipStream_t st, const nnhip_kv_pages& kv, const float* q, const float* k, const float* v,
+                             size_t B, size_t H, const int32_t* pos, size_t len_bound, const float* cosT,
+                             const float* sinT, float scale, float softcap, const float* slopes, bool tokens,
+                             float* part, float* out, size_t num_cus)
+{
+    constexpr double kLog2e = 1.4426950408889634;
+    const size_t R = H / kv.Hkv, groups = pages_groups(R);
+    const size_t chunk = pages_chunk(B, kv.Hkv, R, len_bound, num_cus);
+    const bool cap = softcap > 0.0f;
+    PagesArgs a{q, k, v, pos, cosT, sinT, kv.k, kv.v, kv.table, slopes, part, out, (int)B, (int)H, (int)kv.Hkv, (int)R,
+                (int)groups, (int)ceil_div(R, groups), log2_of(kv.page_size), (int)kv.table_stride, (int)kv.num_pages,
+                (int)len_bound, (int)chunk, (int)ceil_div(len_bound, chunk), (float)(scale * kLog2e),
+                cap ? scale / softcap : 0.0f, cap ? (float)(softcap * kLog2e) : 0.0f, tokens ? 1 : 0};
+    if (kv.f16)
+    {
+        if (kv.dk == 64) return launch_pages_dk<64, _Float16>(st, a);
+        if (kv.dk == 128) return launch_pages_dk<128, _Float16>(st, a);
+        if (kv.dk == 256) return launch_pages_dk<256, _Float16>(st, a);
+        return hipErrorInvalidValue;
+    }
+    if (kv.dk == 64) return launch_pages_dk<64, float>(st, a);
+    if (kv.dk == 128) return launch_pages_dk<128, float>(st, a);
+    if (kv.dk == 256) return launch_pages_dk<256, float>(st, a);
+    return hipErrorInvalidValue;
+}
+
+hipError_t launch_pages_fill(hipStream_t st, const nnhip_kv_pages& kv, const float* k, const float* v, size_t M,
+                             const int32_t* cu, const int32_t* pos0, size_t B, const float* cosT, const float* sinT,
+                             size_t limit)
+{
+    FillArgs a{k, v, cu, pos0, cosT, sinT, kv.k, kv.v, kv.table, (int)M, (int)B, (int)kv.Hkv, log2_of(kv.page_size),
+               (int)kv.table_stride, (int)kv.num_pages, (int)limit};
+    return kv.f16 ? launch_pages_fill_ct<_Float16>(st, a, kv.dk) : launch_pages_fill_ct<float>(st, a, kv.dk);
+}
+
+}  // namespace nnhip

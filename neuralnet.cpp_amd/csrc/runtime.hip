@@ -42,6 +42,17 @@ struct nnhip_ctx
     size_t ones_bytes_ = 0;
     // ranges that the next per-token quantizer call reads in extra blocks (nnhip_ctx_prefetch_next)
     Prefetch pf{};
+    // scratch of the paged attention and the logits' choice: one buffer for each stream that calls
+    // came on, so that calls on two streams share none. Outgrown buffers stay until the context
+    // goes, because a captured call may replay into them (sizes double: all of them together are
+    // smaller than the last).
+    struct StreamWs
+    {
+        hipStream_t stream;
+        std::vector<void*> bufs;  // the last one is in use
+        size_t bytes;
+    };
+    std::vector<StreamWs> stream_ws;
 };
 
 namespace
@@ -179,6 +190,69 @@ nnhip_status ensure_ws(nnhip_ctx* ctx, size_t bytes, const char* fn)
     if (ensure_buf(ctx, ctx->ws, ctx->ws_bytes, round_up(bytes, step), fn, "workspace") == NNHIP_OK)
         return NNHIP_OK;
     return ensure_buf(ctx, ctx->ws, ctx->ws_bytes, bytes, fn, "workspace");
+}
+
+// Scratch of at least `bytes` on the context's current stream (nullptr for 0 bytes)
+nnhip_status ensure_stream_ws(nnhip_ctx* ctx, size_t bytes, const char* fn, void** out)
+{
+    *out = nullptr;
+    if (bytes == 0) return NNHIP_OK;
+    nnhip_ctx::StreamWs* ws = nullptr;
+    for (auto& w : ctx->stream_ws)
+        if (w.stream == ctx->stream) ws = &w;
+    if (!ws)
+    {
+        ctx->stream_ws.push_back({ctx->stream, {}, 0});
+        ws = &ctx->stream_ws.back();
+    }
+    if (ws->bytes < bytes)
+    {
+        hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(ctx->stream, &cs) != hipSuccess)
+        {
+            (void)hipGetLastError();
+            cs = hipStreamCaptureStatusNone;
+        }
+        if (cs != hipStreamCaptureStatusNone)
+            return fail(NNHIP_ERR_UNSUPPORTED, fn,
+                        "the workspace would grow during a capture: make one call of this size before, on this stream");
+        const size_t want = std::max(round_up(bytes, size_t(1) << 20), 2 * ws->bytes);
+        void* p = nullptr;
+        size_t got = want;
+        hipError_t e = hipMalloc(&p, want);
+        if (e != hipSuccess && want > bytes)
+        {
+            (void)hipGetLastError();
+            got = bytes;
+            e = hipMalloc(&p, bytes);
+        }
+        if (e != hipSuccess)
+        {
+            (void)hipGetLastError();
+            return fail(NNHIP_ERR_OOM, fn, "workspace allocation of " + std::to_string(bytes) + " bytes failed");
+        }
+        ws->bufs.push_back(p);
+        ws->bytes = got;
+    }
+    *out = ws->bufs.back();
+    return NNHIP_OK;
+}
+
+// The host's checks of a paged cache, with the rows of the rope tables (0 without)
+nnhip_status check_pages(const char* fn, const nnhip_kv_pages* c, const float* rope_cos, const float* rope_sin)
+{
+    NNHIP_REQUIRE(c && c->k && c->v && c->table, fn, "null cache, pool or page table");
+    NNHIP_REQUIRE((rope_cos == nullptr) == (rope_sin == nullptr), fn, "rope_cos and rope_sin go together");
+    NNHIP_REQUIRE(c->dk == 64 || c->dk == 128 || c->dk == 256, fn, "dk must be 64, 128 or 256");
+    NNHIP_REQUIRE(c->page_size >= 1 && c->page_size <= 1024 && (c->page_size & (c->page_size - 1)) == 0, fn,
+                  "page_size must be a power of two in [1, 1024]");
+    NNHIP_REQUIRE(c->Hkv >= 1 && c->Hkv <= 65535 && c->num_pages >= 1 && c->num_pages <= kMaxDim &&
+                      c->num_pages <= kMaxDim / (c->Hkv * c->page_size), fn,
+                  "num_pages * Hkv * page_size must be in [1, 2^31)");
+    NNHIP_REQUIRE(c->table_stride >= 1 && c->table_stride <= (size_t(1) << 30) / c->page_size, fn,
+                  "table_stride * page_size must be in [1, 2^30]");
+    NNHIP_REQUIRE(aligned16(c->k) && aligned16(c->v), fn, "pools must be 16-byte aligned");
+    return NNHIP_OK;
 }
 
 nnhip_status check_matmul_shape(const char* fn, size_t N, size_t K, size_t M)
@@ -324,6 +398,8 @@ nnhip_status nnhip_ctx_destroy(nnhip_ctx* ctx)
     if (ctx->ws) (void)hipFree(ctx->ws);
     if (ctx->attn_ws) (void)hipFree(ctx->attn_ws);
     if (ctx->ones) (void)hipFree(ctx->ones);
+    for (auto& w : ctx->stream_ws)
+        for (void* p : w.bufs) (void)hipFree(p);
     if (ctx->own) (void)hipStreamDestroy(ctx->own);
     delete ctx;
     if (e != hipSuccess) return hip_fail(fn, "hipStreamSynchronize", e);
@@ -1973,6 +2049,94 @@ nnhip_status nnhip_argmax_rows(nnhip_ctx* ctx, const float* logits, size_t V, si
     NNHIP_REQUIRE(logits && ids, fn, "null pointer");
     NNHIP_REQUIRE(V >= 1 && V <= kMaxDim && B <= kMaxDim && mul_ok(V, B), fn, "size out of range");
     NNHIP_LAUNCH(fn, launch_argmax(ctx->stream, logits, V, B, ids, true, pos));
+    return NNHIP_OK;
+}
+
+nnhip_status nnhip_kv_pages_fill(nnhip_ctx* ctx, const nnhip_kv_pages* cache, const float* k, const float* v,
+                                 size_t M, const int32_t* cu, const int32_t* pos0, size_t B, const float* rope_cos,
+                                 const float* rope_sin, size_t rope_len)
+{
+    const char* fn = "nnhip_kv_pages_fill";
+    NNHIP_CHECK_CTX(fn);
+    const nnhip_status st = check_pages(fn, cache, rope_cos, rope_sin);
+    if (st != NNHIP_OK) return st;
+    if (M == 0 || B == 0) return NNHIP_OK;
+    NNHIP_REQUIRE(k && v && cu, fn, "null pointer");
+    NNHIP_REQUIRE(B < kMaxDim && M < kMaxDim - 64, fn, "M or B too large");
+    size_t limit = cache->table_stride * cache->page_size;
+    if (rope_cos) limit = std::min(limit, rope_len);
+    NNHIP_LAUNCH(fn, launch_pages_fill(ctx->stream, *cache, k, v, M, cu, pos0, B, rope_cos, rope_sin, limit));
+    return NNHIP_OK;
+}
+
+size_t nnhip_attention_pages_workspace_bytes(nnhip_ctx* ctx, size_t B, size_t H, size_t Hkv, size_t dk, size_t len_bound)
+{
+    if (!ctx || Hkv == 0 || H == 0 || H % Hkv != 0 || B == 0 || len_bound == 0) return 0;
+    return pages_workspace_bytes(B, H, Hkv, dk, len_bound, (size_t)ctx->num_cus);
+}
+
+nnhip_status nnhip_attention_pages_decode(nnhip_ctx* ctx, const nnhip_kv_pages* cache, const float* q, const float* k,
+                                          const float* v, size_t B, size_t H, const int32_t* pos, size_t len_bound,
+                                          const float* rope_cos, const float* rope_sin, size_t rope_len, float scale,
+                                          float softcap, const float* slopes, int tokens, float* out)
+{
+    const char* fn = "nnhip_attention_pages_decode";
+    NNHIP_CHECK_CTX(fn);
+    nnhip_status st = check_pages(fn, cache, rope_cos, rope_sin);
+    if (st != NNHIP_OK) return st;
+    if (B == 0) return NNHIP_OK;
+    NNHIP_REQUIRE(q && k && v && pos && out, fn, "null pointer");
+    NNHIP_REQUIRE(H >= cache->Hkv && H % cache->Hkv == 0 && H <= 65535, fn,
+                  "H must be a multiple of Hkv, at most 65535");
+    NNHIP_REQUIRE(B <= 65535, fn, "B must be at most 65535");
+    NNHIP_REQUIRE(len_bound >= 1 && len_bound <= cache->table_stride * cache->page_size, fn,
+                  "len_bound must be in [1, table_stride * page_size]");
+    NNHIP_REQUIRE(!rope_cos || len_bound <= rope_len, fn, "len_bound must not exceed the rows of the rope tables");
+    NNHIP_REQUIRE(softcap >= 0.0f && softcap <= 3.0e38f, fn, "softcap must be finite and not negative");
+    void* ws = nullptr;
+    st = ensure_stream_ws(ctx, pages_workspace_bytes(B, H, cache->Hkv, cache->dk, len_bound, (size_t)ctx->num_cus), fn, &ws);
+    if (st != NNHIP_OK) return st;
+    NNHIP_LAUNCH(fn, launch_pages_attn(ctx->stream, *cache, q, k, v, B, H, pos, len_bound, rope_cos, rope_sin, scale,
+                                       softcap, slopes, tokens != 0, static_cast<float*>(ws), out, (size_t)ctx->num_cus));
+    return NNHIP_OK;
+}
+
+size_t nnhip_logits_workspace_bytes(nnhip_ctx* ctx, size_t V, size_t B)
+{
+    return !ctx || V == 0 ? 0 : logits_workspace_bytes(V, B, (size_t)ctx->num_cus);
+}
+
+nnhip_status nnhip_logits_adjust_rows(nnhip_ctx* ctx, const float* logits, size_t V, size_t B,
+                                      const nnhip_logit_rules* rules, float* out, int32_t* ids, int32_t* pos)
+{
+    const char* fn = "nnhip_logits_adjust_rows";
+    NNHIP_CHECK_CTX(fn);
+    if (B == 0) return NNHIP_OK;
+    const nnhip_logit_rules r = rules ? *rules : nnhip_logit_rules{};
+    NNHIP_REQUIRE(logits && (out || ids), fn, "null pointer");
+    NNHIP_REQUIRE(V >= 1 && V < (size_t(1) << 30) && B <= 65535, fn, "V must be in [1, 2^30), B at most 65535");
+    NNHIP_REQUIRE(ids || (!r.count_choice && !pos), fn, "counting the choice and advancing pos need ids");
+    NNHIP_REQUIRE(!r.count_choice || r.counts, fn, "counting the choice needs counts");
+    NNHIP_REQUIRE(r.counts || (!r.repeat && !r.presence && !r.frequency), fn, "penalties need counts");
+    NNHIP_REQUIRE(r.bias_stride == 0 || r.bias_stride >= V, fn, "bias_stride must be 0 or at least V");
+    NNHIP_REQUIRE(r.allowed_stride == 0 || r.allowed_stride >= ceil_div(V, 32), fn,
+                  "allowed_stride must be 0 or at least ceil(V / 32)");
+    void* ws = nullptr;
+    const nnhip_status st = ensure_stream_ws(ctx, logits_workspace_bytes(V, B, (size_t)ctx->num_cus), fn, &ws);
+    if (st != NNHIP_OK) return st;
+    NNHIP_LAUNCH(fn, launch_logits_adjust(ctx->stream, logits, V, B, r, out, ids, pos, ws, (size_t)ctx->num_cus));
+    return NNHIP_OK;
+}
+
+nnhip_status nnhip_token_counts_add(nnhip_ctx* ctx, const int32_t* ids, size_t M, const int32_t* cu, size_t B,
+                                    size_t V, int32_t* counts)
+{
+    const char* fn = "nnhip_token_counts_add";
+    NNHIP_CHECK_CTX(fn);
+    if (M == 0 || B == 0) return NNHIP_OK;
+    NNHIP_REQUIRE(ids && cu && counts, fn, "null pointer");
+    NNHIP_REQUIRE(V >= 1 && V <= kMaxDim && B < kMaxDim && M < kMaxDim - 256, fn, "size out of range");
+    NNHIP_LAUNCH(fn, launch_token_counts(ctx->stream, ids, M, cu, B, V, counts));
     return NNHIP_OK;
 }
 
