@@ -659,7 +659,7 @@ nnhip_status nnhip_argmax_rows(nnhip_ctx* ctx, const float* logits, size_t V, si
  *      (compute_layer_gpt.hpp:764-765); for servers that start and end sequences at any step. ---- */
 
 /* One layer's paged cache. k / v: pools (num_pages, Hkv, page_size, dk) of f32, or f16 bit patterns when
- * f16 != 0 (compute = F16), 16-byte aligned; page_size a power of two in [1, 1024]. table: DEVICE
+ * f16 != 0 (compute = F16), 16-byte aligned; page_size a power of two in [8, 1024]. table: DEVICE
  * (B, table_stride) int32, entry (b, i) = the page that holds positions [i * page_size, (i + 1) *
  * page_size) of sequence b; entries past a sequence's length may be anything. Sequences may share pages
  * that no call writes. Every id that a call uses is checked on the device: one outside [0, num_pages)
@@ -702,6 +702,23 @@ nnhip_status nnhip_attention_pages_decode(nnhip_ctx* ctx, const nnhip_kv_pages* 
                                           const float* v, size_t B, size_t H, const int32_t* pos, size_t len_bound,
                                           const float* rope_cos, const float* rope_sin, size_t rope_len, float scale,
                                           float softcap, const float* slopes, int tokens, float* out);
+
+/* Attention of packed prompts over pages that hold the keys and values of all their positions (after
+ * nnhip_kv_pages_fill): q and out (H*dk, M) feature-major, columns cu[b] .. cu[b+1] - 1 = the tokens of
+ * sequence b at positions pos0[b] + t (cu, pos0 as nnhip_kv_pages_fill's; pos0 may be NULL); t_bound bounds
+ * every sequence's tokens (it sizes the launch). A token at position i sees its own sequence's positions
+ * j <= i, and with prefix (DEVICE (B) int32, or NULL) also every j < prefix[b] that the sequence has;
+ * nothing of another sequence. Scores, softcap and slopes as nnhip_attention_pages_decode (j - i is above
+ * 0 inside a prefix); products, sums, errors and the f32 products' cases as nnhip_attention_prefill. dk in
+ * {64, 128}, any H / Hkv, H * dk * M < 2^29. Columns of no sequence are not written. NaN: a sequence with
+ * more than t_bound tokens, columns outside [0, M) or positions at or past table_stride * page_size or
+ * rope_len; a query that sees a position whose page is outside the pool (other queries of its sequence
+ * may be NaN then, too). The paged form of nnhip_attention_prefill
+ * (compute_layer_attention.hpp:1022-1083). */
+nnhip_status nnhip_attention_pages_prefill(nnhip_ctx* ctx, const nnhip_kv_pages* cache, const float* q, size_t M,
+                                           const int32_t* cu, const int32_t* pos0, size_t B, size_t t_bound, size_t H,
+                                           const float* rope_cos, const float* rope_sin, size_t rope_len, float scale,
+                                           float softcap, const float* slopes, const int32_t* prefix, float* out);
 
 /* Scratch that nnhip_attention_pages_decode (nnhip_logits_adjust_rows) of these sizes uses. The context
  * keeps one for each stream that it was set to, grown on demand and freed with the context only, so that a

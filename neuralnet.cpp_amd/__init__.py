@@ -166,6 +166,8 @@ SIGNATURES = {
     "nnhip_kv_pages_fill": (_st, [_vp, _vp, _vp, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _sz]),
     "nnhip_attention_pages_decode": (_st, [_vp, _vp, _vp, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _vp, _sz, _f, _f, _vp,
                                            _st, _vp]),
+    "nnhip_attention_pages_prefill": (_st, [_vp, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _vp, _vp, _sz, _f, _f, _vp,
+                                            _vp, _vp]),
     "nnhip_attention_pages_workspace_bytes": (_sz, [_vp, _sz, _sz, _sz, _sz, _sz]),
     "nnhip_logits_workspace_bytes": (_sz, [_vp, _sz, _sz]),
     "nnhip_logits_adjust_rows": (_st, [_vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp]),
@@ -977,6 +979,24 @@ class Context:
             self._arg(pos, self._torch.int32, (B,), "pos"), len_bound, cs, sn, rows, scale, softcap,
             self._arg(slopes, f32, (H,), "slopes"), int(tokens), self._arg(out, f32, qs, "out")),
             "nnhip_attention_pages_decode")
+        return out
+
+    def attention_pages_prefill(self, cache, q, cu, t_bound: int, H: int, scale: float, pos0=None, cos=None, sin=None,
+                                softcap: float = 0.0, slopes=None, prefix=None, out=None):
+        """Attention of packed prompts q (H*dk, M) (sequence b: columns cu[b] .. cu[b+1] - 1, at most t_bound of them,
+        positions pos0[b] on) over the pages of cache, which hold all their positions: causal, and bidirectional
+        over the first prefix[b] positions (prefix (B) int32, or None). Returns out (H*dk, M)."""
+        B, cu_p, pos0_p = self._packed(cache, cu, pos0)
+        f32, M = self._torch.float32, q.shape[-1]
+        shape = (H * cache.dk, M)
+        if out is None:
+            out = self._empty(shape, f32)
+        cs, sn, rows = self._rope(cos, sin, cache.dk)
+        self._bind_stream()
+        _check(lib().nnhip_attention_pages_prefill(
+            self.h, cache.ref, self._arg(q, f32, shape, "q"), M, cu_p, pos0_p, B, t_bound, H, cs, sn, rows, scale,
+            softcap, self._arg(slopes, f32, (H,), "slopes"), self._arg(prefix, self._torch.int32, (B,), "prefix"),
+            self._arg(out, f32, shape, "out")), "nnhip_attention_pages_prefill")
         return out
 
     def attention_pages_workspace_bytes(self, B: int, H: int, Hkv: int, dk: int, len_bound: int) -> int:

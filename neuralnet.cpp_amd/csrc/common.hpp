@@ -381,6 +381,20 @@ hipError_t launch_embed(hipStream_t st, const float* table, const int32_t* ids, 
 hipError_t launch_argmax(hipStream_t st, const float* L, size_t V, size_t B, int32_t* ids, bool rows = false,
                          int32_t* pos = nullptr);
 
+// tanh to about 1e-7 of itself: the odd series below 0.3 (its next term is 2e-9), else from exp
+__device__ __forceinline__ float shape_tanh(float x)
+{
+    const float a = fabsf(x), z = x * x;
+    float s = -8.8632355e-3f;  // -1382 / 155925
+    s = __builtin_fmaf(s, z, 2.1869489e-2f);
+    s = __builtin_fmaf(s, z, -5.3968254e-2f);
+    s = __builtin_fmaf(s, z, 0.13333333f);
+    s = __builtin_fmaf(s, z, -0.33333333f);
+    const float small = __builtin_fmaf(x * z, s, x);
+    const float big = copysignf(__builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(a * 2.8853900f) + 1.0f), 1.0f), x);
+    return a < 0.3f ? small : big;
+}
+
 // ---- paged KV cache (k_pages.hip; the prompt attention k_prefill.hip), logits (k_logits.hip)
 size_t pages_chunk(size_t B, size_t Hkv, size_t R, size_t len_bound, size_t num_cus);
 size_t pages_workspace_bytes(size_t B, size_t H, size_t Hkv, size_t dk, size_t len_bound, size_t num_cus);
@@ -391,6 +405,10 @@ hipError_t launch_pages_attn(hipStream_t st, const nnhip_kv_pages& kv, const flo
 hipError_t launch_pages_fill(hipStream_t st, const nnhip_kv_pages& kv, const float* k, const float* v, size_t M,
                              const int32_t* cu, const int32_t* pos0, size_t B, const float* cosT, const float* sinT,
                              size_t limit);
+hipError_t launch_pages_prefill(hipStream_t st, const nnhip_kv_pages& kv, const float* q, size_t M, const int32_t* cu,
+                                const int32_t* pos0, size_t B, size_t t_bound, size_t H, const float* cosT,
+                                const float* sinT, size_t limit, float scale, float softcap, const float* slopes,
+                                const int32_t* prefix, float* out);
 size_t logits_slices(size_t V, size_t B, size_t num_cus);
 size_t logits_workspace_bytes(size_t V, size_t B, size_t num_cus);
 hipError_t launch_logits_adjust(hipStream_t st, const float* logits, size_t V, size_t B, const nnhip_logit_rules& rules,

@@ -169,20 +169,6 @@ struct PagesRow
     }
 };
 
-// tanh to about 1e-7 of itself: the odd series below 0.3 (its next term is 2e-9), else from exp
-__device__ __forceinline__ float pg_tanh(float x)
-{
-    const float a = fabsf(x), z = x * x;
-    float s = -8.8632355e-3f;  // -1382 / 155925
-    s = __builtin_fmaf(s, z, 2.1869489e-2f);
-    s = __builtin_fmaf(s, z, -5.3968254e-2f);
-    s = __builtin_fmaf(s, z, 0.13333333f);
-    s = __builtin_fmaf(s, z, -0.33333333f);
-    const float small = __builtin_fmaf(x * z, s, x);
-    const float big = copysignf(1.0f - 2.0f / (__builtin_amdgcn_exp2f(a * 2.8853900f) + 1.0f), x);
-    return a < 0.3f ? small : big;
-}
-
 // Attention of one new token per sequence. Work-group = (chunk of `chunk` positions, KV head and group
 // of at most 8 of its query heads, sequence); a group of 16 lanes takes one row of dk at a time, 4 rows
 // on their way together, so a wave's tile is 16 rows; its four waves take the chunk's tiles in turn.
@@ -203,7 +189,7 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
     constexpr int NS = kPgU * RT;
     __shared__ __align__(16) float q_s[RT * DK];
     __shared__ float new_s[2][DK];
-    __shared__ int page_s[kPgMaxChunk];
+    __shared__ int page_s[kPgMaxChunk / 8];  // a page holds 8 positions or more
     __shared__ float ml_s[2][kPgWaves * 4][RT];
     __shared__ float red_s[kPgWaves][RT * DK];
 
@@ -288,7 +274,7 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
 #pragma unroll
     for (int i = 0; i < NV; ++i) slope2[i] = a.slopes && hs + i < R ? a.slopes[h0 + hs + i] * 1.44269504f : 0.0f;
     auto shape = [&](float dot, int i, int t) {
-        float x = a.cap2 > 0.0f ? a.cap2 * pg_tanh(dot * a.capi) : dot * a.scale2;
+        float x = a.cap2 > 0.0f ? a.cap2 * shape_tanh(dot * a.capi) : dot * a.scale2;
         if (a.slopes) x = __builtin_fmaf(slope2[i], (float)(t - p), x);
         return x;
     };

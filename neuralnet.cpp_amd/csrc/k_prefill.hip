@@ -51,6 +51,7 @@
 // Caches of f16 elements (compute = F16): the fill rounds the rotated keys and the values to the
 // nearest f16 (ties to even), as the decode append does.
 #include "common.hpp"
+#include "pages_index.hpp"
 
 #include <cmath>
 
@@ -208,6 +209,16 @@ struct PrefillArgs
     float scale;
     float scale2;  // |scale| * log2(e)
     int f32;       // 1: the f32 products throughout (a scale outside [2^-20, 2^20])
+    int M;         // columns of q and out (paged; otherwise B * T)
+    int groups;    // work-groups that share a KV head's queries: R heads each
+    // paged: B packed sequences of at most T tokens, whose keys and values lie in pages
+    const int32_t* table;
+    const int32_t* cu;      // columns cu[b] .. cu[b + 1] - 1 are sequence b's
+    const int32_t* starts;  // position of its first token, or null for 0
+    const int32_t* prefix;  // positions before prefix[b] are visible to all its queries, or null
+    const float* slopes;
+    int table_stride, num_pages, shift, limit;  // limit: positions from here on have no place
+    float cap2, capi2;      // softcap * log2(e) and its inverse, 0 without
 };
 
 template <int DK, typename CT>
@@ -276,21 +287,48 @@ struct PrefillWave
     bool live;  // the wave has queries
 };
 
+// What depends on the sequence: its tokens, its first column and position, the columns of q, the last key
+// that the lane's query sees and the last ones that all and any of the wave's queries see. Equal prompts
+// at one position have it in the arguments.
+template <bool kPaged>
+struct PrefillSeq
+{
+    __device__ __forceinline__ int n(const PrefillArgs& a) const { return a.T; }
+    __device__ __forceinline__ int col0(const PrefillArgs& a, const PrefillWave& w) const { return w.b * a.T; }
+    __device__ __forceinline__ int pos0(const PrefillArgs& a) const { return a.pos0; }
+    __device__ __forceinline__ int cols(const PrefillArgs& a) const { return a.B * a.T; }
+    __device__ __forceinline__ int sight(const PrefillWave& w) const { return w.qpos; }
+    __device__ __forceinline__ int from(const PrefillArgs& a, const PrefillWave& w) const { return a.pos0 + w.t0; }
+    __device__ __forceinline__ int to(const PrefillArgs& a, const PrefillWave& w) const { return a.pos0 + w.t0 + kPQ - 1; }
+};
+template <>
+struct PrefillSeq<true>
+{
+    int n_, col0_, pos0_, pre;  // pre: keys that every query sees
+    __device__ __forceinline__ int n(const PrefillArgs&) const { return n_; }
+    __device__ __forceinline__ int col0(const PrefillArgs&, const PrefillWave&) const { return col0_; }
+    __device__ __forceinline__ int pos0(const PrefillArgs&) const { return pos0_; }
+    __device__ __forceinline__ int cols(const PrefillArgs& a) const { return a.M; }
+    __device__ __forceinline__ int sight(const PrefillWave& w) const { return max(w.qpos, pre - 1); }
+    __device__ __forceinline__ int from(const PrefillArgs&, const PrefillWave& w) const { return max(pos0_ + w.t0, pre - 1); }
+    __device__ __forceinline__ int to(const PrefillArgs&, const PrefillWave& w) const { return max(pos0_ + w.t0 + kPQ - 1, pre - 1); }
+};
+
 // The lane's rotated query value pairs, f(c, e, value, value of the dimension DK/2 further) for its
 // dimensions 2Gc + Gh + e below DK/2. The cos / sin rows of 32 queries are 32 lines apart, so they
 // are read four at a time. Lanes past the last token repeat it (they are never stored).
-template <int DK, int G, typename F>
-__device__ __forceinline__ void load_query(const PrefillArgs& a, const PrefillWave& w, int h, F&& f)
+template <int DK, int G, bool kPaged, typename F>
+__device__ __forceinline__ void load_query(const PrefillArgs& a, const PrefillWave& w, const PrefillSeq<kPaged>& seq, int h, F&& f)
 {
     constexpr int HALF = DK / 2, NG = HALF / (2 * G);
-    const int M = a.B * a.T;
+    const int M = seq.cols(a);
     const __amdgpu_buffer_rsrc_t rq = pf_rsrc(a.q, (uint32_t)((size_t)a.H * DK * (size_t)M * 4u));
-    const uint32_t rope_bytes = a.cosT ? (uint32_t)((size_t)a.max_len * HALF * 4u) : 0u;
+    const uint32_t rope_bytes = a.cosT ? (uint32_t)((size_t)a.max_len * HALF * 4u) : 0u;  // (paged: max_len = limit)
     const __amdgpu_buffer_rsrc_t rc = pf_rsrc(a.cosT ? a.cosT : a.q, rope_bytes);
     const __amdgpu_buffer_rsrc_t rs = pf_rsrc(a.cosT ? a.sinT : a.q, rope_bytes);
-    const int qt = min(w.qt, a.T - 1);
-    const uint32_t q_at = (uint32_t)(((size_t)(w.head * DK + G * h) * (size_t)M + (size_t)(w.b * a.T + qt)) * 4u);
-    const uint32_t r_at = (uint32_t)(((size_t)(a.pos0 + qt) * HALF + (size_t)(G * h)) * 4u);
+    const int qt = min(w.qt, seq.n(a) - 1);
+    const uint32_t q_at = (uint32_t)(((size_t)(w.head * DK + G * h) * (size_t)M + (size_t)(seq.col0(a, w) + qt)) * 4u);
+    const uint32_t r_at = (uint32_t)(((size_t)(seq.pos0(a) + qt) * HALF + (size_t)(G * h)) * 4u);
 #pragma unroll
     for (int c = 0; c < NG; ++c)
     {
@@ -321,16 +359,42 @@ __device__ __forceinline__ void load_query(const PrefillArgs& a, const PrefillWa
 
 // out[head*DK + i][m] = y(d, v) for the lane's query: element v of block d belongs to row
 // r = 8(v/4) + 4h + v%4 of the block; dim(d, r) is its dimension
-template <int DK, typename D, typename Y>
-__device__ __forceinline__ void store_out(const PrefillArgs& a, const PrefillWave& w, int h, D&& dim, Y&& y)
+template <int DK, bool kPaged, typename D, typename Y>
+__device__ __forceinline__ void store_out(const PrefillArgs& a, const PrefillWave& w, const PrefillSeq<kPaged>& seq, int h,
+                                          D&& dim, Y&& y)
 {
-    if (w.qt >= a.T) return;
-    const int M = a.B * a.T, m = w.b * a.T + w.qt;
+    if (w.qt >= seq.n(a)) return;
+    const int M = seq.cols(a), m = seq.col0(a, w) + w.qt;
 #pragma unroll
     for (int d = 0; d < DK / 32; ++d)
 #pragma unroll
         for (int v = 0; v < 16; ++v)
             a.out[(size_t)(w.head * DK + dim(d, 8 * (v >> 2) + 4 * h + (v & 3))) * (size_t)M + (size_t)m] = y(d, v);
+}
+
+// Four elements of a cache row as floats
+template <typename CT>
+__device__ __forceinline__ float4 widen4(const CT* p)
+{
+    if constexpr (sizeof(CT) == 4) return *reinterpret_cast<const float4*>(p);
+    else
+    {
+        const v4h x = *reinterpret_cast<const v4h*>(p);
+        return make_float4((float)x[0], (float)x[1], (float)x[2], (float)x[3]);
+    }
+}
+
+// Paged: the pool's row of position t of the wave's sequence and KV head; a page outside the pool sets
+// `bad` and gives page 0's
+__device__ __forceinline__ size_t paged_row(const PrefillArgs& a, const PrefillWave& w, int t, bool& bad)
+{
+    int id = a.table[(size_t)w.b * a.table_stride + (t >> a.shift)];
+    if (!page_ok(id, a.num_pages))
+    {
+        bad = true;
+        id = 0;
+    }
+    return page_row(id, w.g, t & ((1 << a.shift) - 1), a.Hkv, a.shift);
 }
 
 // The work-group's attention on the fp32 MFMA (v_mfma_f32_32x32x2_f32), for inputs that the f16
@@ -339,16 +403,20 @@ __device__ __forceinline__ void store_out(const PrefillArgs& a, const PrefillWav
 // 8(v/4) + 4(l/32) + v%4 of its 16 elements v: the B operand of the P . V products when the keys of
 // product s are taken in that order. The sum over the head dimension takes product s = 4c + e over
 // dimensions 8c + e and 8c + 4 + e (the two lane halves).
-template <int DK, typename CT>
-__device__ void attend_f32(const PrefillArgs& a, const PrefillWave& w, int last_key, __amdgpu_buffer_rsrc_t rk,
-                           __amdgpu_buffer_rsrc_t rv, float* ks)
+// Paged: a NaN or an infinity among the values of a key that one query sees and another does not must
+// not reach the other, whose probability of 0 a matrix product would multiply with it; tiles that reach
+// past some query's sight therefore add their values key by key.
+template <int DK, bool kPaged, bool kShaped, typename CT>
+__device__ void attend_f32(const PrefillArgs& a, const PrefillWave& w, const PrefillSeq<kPaged>& seq, int last_key,
+                           __amdgpu_buffer_rsrc_t rk, __amdgpu_buffer_rsrc_t rv, float* ks, int tid)
 {
     constexpr int NC = DK / 8, ND = DK / 32, KROW = PrefillTile<DK, CT>::KROW;
-    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
+    const int lane = tid & 63, h = lane >> 5, l32 = lane & 31;
     const int row = a.Hkv * DK;
     float* vs = ks + kPK * KROW;
+    bool bad = false;  // a page outside the pool
     float qv[DK / 2];  // qv[4c + e] = rotated query value of dimension 8c + 4h + e
-    load_query<DK, 4>(a, w, h, [&](int c, int e, float y0, float y1) {
+    load_query<DK, 4>(a, w, seq, h, [&](int c, int e, float y0, float y1) {
         qv[4 * c + e] = y0;
         qv[4 * (c + NC / 2) + e] = y1;
     });
@@ -362,12 +430,26 @@ __device__ void attend_f32(const PrefillArgs& a, const PrefillWave& w, int last_
         for (int u = tid; u < kPK * DK / 4; u += kPThreads)
         {
             const int key = u / (DK / 4), c4 = u % (DK / 4);
+            if constexpr (kPaged)
+            {
+                const int t = kb * kPK + key;
+                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
+                if (t <= last_key)
+                {
+                    const size_t at = paged_row(a, w, t, bad) * DK + 4 * c4;
+                    x = widen4<CT>(static_cast<const CT*>(a.kc) + at);
+                    y = widen4<CT>(static_cast<const CT*>(a.vc) + at);
+                }
+                *reinterpret_cast<float4*>(ks + key * KROW + 4 * c4) = x;
+                *reinterpret_cast<float4*>(vs + key * KROW + 4 * c4) = y;
+                continue;
+            }
             const uint32_t off = (uint32_t)(((size_t)(kb * kPK + key) * (size_t)row + (size_t)w.g * DK + 4 * c4) * sizeof(CT));
             *reinterpret_cast<float4*>(ks + key * KROW + 4 * c4) = ld_c4<CT>(rk, off);
             *reinterpret_cast<float4*>(vs + key * KROW + 4 * c4) = ld_c4<CT>(rv, off);
         }
         __syncthreads();
-        if (!w.live || kb * kPK > a.pos0 + w.t0 + kPQ - 1) continue;
+        if (!w.live || kb * kPK > seq.to(a, w)) continue;
         v16f s = v16f{};
 #pragma unroll
         for (int c = 0; c < NC; ++c)
@@ -384,8 +466,13 @@ __device__ void attend_f32(const PrefillArgs& a, const PrefillWave& w, int last_
         for (int v = 0; v < 16; ++v)
         {
             const int key = kb * kPK + 8 * (v >> 2) + 4 * h + (v & 3);
-            const float x = s[v] * a.scale;
-            sc[v] = key <= w.qpos ? x : -__builtin_inff();
+            float x = s[v] * a.scale;
+            if constexpr (kShaped)
+            {
+                if (a.cap2 > 0.0f) x = a.cap2 * 0.69314718f * shape_tanh(x * (a.capi2 * 1.44269504f));
+                if (a.slopes) x += a.slopes[w.head] * (float)(key - w.qpos);
+            }
+            sc[v] = key <= seq.sight(w) ? x : -__builtin_inff();
             mx = fmaxf(mx, sc[v]);
         }
         mx = fmaxf(mx, __shfl_xor(mx, 32));
@@ -410,6 +497,36 @@ __device__ void attend_f32(const PrefillArgs& a, const PrefillWave& w, int last_
 #pragma unroll
                 for (int v = 0; v < 16; ++v) o[d][v] *= corr;
         }
+        if constexpr (kPaged)
+        {
+            if (kb * kPK + kPK - 1 > seq.from(a, w))
+            {
+#pragma unroll 1
+                for (int n = 0; n < 16; ++n)
+                {
+                    float own = 0.0f;
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) own = v == n ? sc[v] : own;
+                    const float other = __shfl_xor(own, 32);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+                    {
+                        const float pr = half == h ? own : other;
+                        const int key = 8 * (n >> 2) + 4 * half + (n & 3);
+                        const bool seen = kb * kPK + key <= seq.sight(w);
+#pragma unroll
+                        for (int d = 0; d < ND; ++d)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                            {
+                                const float x = vs[key * KROW + 32 * d + 8 * (i >> 2) + 4 * h + (i & 3)];
+                                o[d][i] = __builtin_fmaf(pr, seen ? x : 0.0f, o[d][i]);
+                            }
+                    }
+                }
+                continue;
+            }
+        }
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -419,11 +536,64 @@ __device__ void attend_f32(const PrefillArgs& a, const PrefillWave& w, int last_
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vs[key * KROW + 32 * d + l32], sc[sp], o[d], 0, 0, 0);
             }
     }
+    if constexpr (kPaged)
+    {
+        // nothing visible above -infinity: 0; a page outside the pool: NaN
+        bad = __syncthreads_or(bad) != 0;
+        if (bad) l_run = __builtin_nanf("");
+        else if (l_run == 0.0f) l_run = 1.0f;
+    }
     if (w.live)
-        store_out<DK>(a, w, h, [](int d, int r) { return 32 * d + r; }, [&](int d, int v) { return o[d][v] / l_run; });
+        store_out<DK>(a, w, seq, h, [](int d, int r) { return 32 * d + r; }, [&](int d, int v) { return o[d][v] / l_run; });
 }
 
-template <int DK, typename CT>
+// The place of thread tid of work-group `block`, and the last key that the work-group sees; false if it
+// has nothing to do (paged: or its sequence does not fit, see store_nan). Heaviest items first: the last
+// queries attend over the most keys.
+template <bool kPaged>
+__device__ __forceinline__ bool find_place(const PrefillArgs& a, int block, int tid, PrefillWave& w, PrefillSeq<kPaged>& seq,
+                                           int& last_key)
+{
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int groups = kPaged ? a.groups : 1;
+    const int per_qb = a.B * a.Hkv * groups;
+    const int qb = a.nqb - 1 - block / per_qb;
+    const int bg = block % per_qb;
+    w.b = bg / (a.Hkv * groups);
+    w.g = bg / groups % a.Hkv;
+    w.head = (w.g * groups + bg % groups) * a.R + wave % a.R;
+    const int qn = kPQ * (kPWaves / a.R);  // queries of the work-group
+    w.t0 = qb * qn + wave / a.R * kPQ;
+    w.qt = w.t0 + (tid & 31);
+    if constexpr (kPaged)
+    {
+        const int col0 = a.cu[w.b], pos0 = a.starts ? a.starts[w.b] : 0;
+        const int64_t n = (int64_t)a.cu[w.b + 1] - col0;
+        if (col0 < 0 || col0 + n > a.M || n > a.T || pos0 < 0 || pos0 >= a.limit || n > a.limit - pos0 || qb * qn >= n) return false;
+        seq = {(int)n, col0, pos0, a.prefix ? max(0, min(a.prefix[w.b], pos0 + (int)n)) : 0};
+    }
+    w.qpos = seq.pos0(a) + w.qt;
+    w.live = w.t0 < seq.n(a);
+    last_key = seq.pos0(a) + min(qb * qn + qn, seq.n(a)) - 1;
+    if constexpr (kPaged) last_key = max(last_key, seq.pre - 1);
+    return true;
+}
+
+// A packed sequence that does not fit its bounds: NaN in the columns that are there
+template <int DK>
+__device__ void store_nan(const PrefillArgs& a, int block, int tid)
+{
+    const int per_qb = a.B * a.Hkv * a.groups, bg = block % per_qb, b = bg / (a.Hkv * a.groups);
+    const int first = (bg / a.groups % a.Hkv * a.groups + bg % a.groups) * a.R;
+    const int col0 = a.cu[b], pos0 = a.starts ? a.starts[b] : 0;
+    const int64_t n = (int64_t)a.cu[b + 1] - col0;
+    if (col0 >= 0 && col0 + n <= a.M && n <= a.T && pos0 >= 0 && pos0 < a.limit && n <= a.limit - pos0) return;
+    const int64_t c1 = min(col0 + n, (int64_t)a.M);
+    for (int64_t c = max(col0, 0) + (int64_t)(a.nqb - 1 - block / per_qb) * kPThreads + tid; c < c1; c += (int64_t)a.nqb * kPThreads)
+        for (int i = 0; i < a.R * DK; ++i) a.out[(size_t)(first * DK + i) * (size_t)a.M + (size_t)c] = __builtin_nanf("");
+}
+
+template <int DK, bool kPaged, bool kShaped, typename CT>
 __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
 {
     using Tile = PrefillTile<DK, CT>;
@@ -440,27 +610,21 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
 
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // heaviest items first: the last queries attend over the most keys
-    const int per_qb = a.B * a.Hkv;
-    const int qb = a.nqb - 1 - (int)blockIdx.x / per_qb;
-    const int bg = (int)blockIdx.x % per_qb;
     PrefillWave w;
-    w.b = bg / a.Hkv;
-    w.g = bg % a.Hkv;
-    w.head = w.g * a.R + wave % a.R;
-    const int qn = kPQ * (kPWaves / a.R);  // queries of the work-group
-    w.t0 = qb * qn + wave / a.R * kPQ;
-    w.qt = w.t0 + l32;
-    w.qpos = a.pos0 + w.qt;
-    w.live = w.t0 < a.T;
+    PrefillSeq<kPaged> seq;
+    int last_key;
+    if (!find_place(a, (int)blockIdx.x, tid, w, seq, last_key))
+    {
+        if constexpr (kPaged) store_nan<DK>(a, (int)blockIdx.x, tid);
+        return;
+    }
     const int row = a.Hkv * DK;
-    const int valid = a.pos0 + a.T;  // cache rows [0, valid) hold keys / values
-    const int last_key = a.pos0 + min(qb * qn + qn, a.T) - 1;
+    const int valid = seq.pos0(a) + seq.n(a);  // cache rows [0, valid) hold keys / values
     const int nkb = last_key / kPK + 1;
-    const size_t seq_off = (size_t)w.b * (size_t)a.max_len * (size_t)row;
+    const size_t seq_off = kPaged ? 0 : (size_t)w.b * (size_t)a.max_len * (size_t)row;
     // rows at or past `valid` read as zeros: their scores are masked and their zero values keep
     // 0 * v finite
-    const uint32_t seq_bytes = (uint32_t)((size_t)min(valid, a.max_len) * (size_t)row * sizeof(CT));
+    const uint32_t seq_bytes = kPaged ? 0u : (uint32_t)((size_t)min(valid, a.max_len) * (size_t)row * sizeof(CT));
     const __amdgpu_buffer_rsrc_t rk = pf_rsrc(static_cast<const CT*>(a.kc) + seq_off, seq_bytes);
     const __amdgpu_buffer_rsrc_t rv = pf_rsrc(static_cast<const CT*>(a.vc) + seq_off, seq_bytes);
 
@@ -486,7 +650,84 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
     }
     const uint32_t tile_bytes = (uint32_t)(kPK * row) * (uint32_t)sizeof(CT);
     const CT* const kvb = (is_v ? static_cast<const CT*>(a.vc) : static_cast<const CT*>(a.kc)) + seq_off;
+    // paged: the page(s) of the thread's keys in the tile to be loaded next, read from the table a tile ahead so
+    // that no load waits for its address. A page holds 8 positions or more: the four keys of a V thread lie in
+    // one. Keys past the last that the work-group sees are read where that one is (trim() makes them zeros).
+    int ids[KU];
+    bool bad = false;
+    auto key_at = [&](int kb, int i) {
+        return is_v ? min(kb * kPK + 4 * vq, last_key & ~3) : min(kb * kPK + (u + 256 * i) / CH, last_key);
+    };
+    auto load_ids = [&](int kb) {
+        if constexpr (kPaged)
+        {
+#pragma unroll
+            for (int i = 0; i < KU; ++i)
+                if (i == 0 || !is_v) ids[i] = a.table[(size_t)w.b * a.table_stride + (key_at(kb, i) >> a.shift)];
+        }
+    };
+    auto load_paged = [&](int kb) {
+        const uint8_t* at[KU];
+#pragma unroll
+        for (int i = 0; i < KU; ++i)
+            if (i == 0 || !is_v)
+            {
+                const bool in = page_ok(ids[i], a.num_pages);
+                bad |= !in;
+                const uint32_t r = (uint32_t)page_row(in ? ids[i] : 0, w.g, key_at(kb, i) & ((1 << a.shift) - 1), a.Hkv, a.shift);
+                at[i] = reinterpret_cast<const uint8_t*>(kvb) + (uint64_t)r * (uint32_t)(DK * sizeof(CT)) +
+                        (is_v ? ND * vg : 8 * ((u + 256 * i) % CH)) * (int)sizeof(CT);
+            }
+        if (is_v)
+        {
+            constexpr int W = ND * (int)sizeof(CT) / 4;  // words per key
+            typedef uint32_t VWord __attribute__((ext_vector_type(W)));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+            {
+                const VWord x = *reinterpret_cast<const VWord*>(at[0] + i * DK * (int)sizeof(CT));
+#pragma unroll
+                for (int e = 0; e < W; ++e) raw[W * i + e] = x[e];
+            }
+        }
+        else
+        {
+#pragma unroll
+            for (int j = 0; j < KU; ++j)
+#pragma unroll
+                for (int q = 0; q < (F32C ? 2 : 1); ++q)
+                {
+                    const u32x4 x = reinterpret_cast<const u32x4*>(at[j])[q];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) raw[(F32C ? 8 : 4) * j + 4 * q + e] = x[e];
+                }
+        }
+        if (kb + 1 < nkb) load_ids(kb + 1);
+    };
+    // paged: what was read for keys behind the last becomes 0, as buffer loads past their range give
+    auto trim = [&](int kb) {
+        if constexpr (kPaged)
+        {
+            if (kb * kPK + kPK - 1 <= last_key) return;
+            constexpr int VK = F32C ? ND : ND / 2;  // words of a V thread's key
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < VK; ++e)
+                    if (is_v && kb * kPK + 4 * vq + i > last_key) raw[VK * i + e] = 0u;
+#pragma unroll
+            for (int j = 0; j < KU; ++j)
+#pragma unroll
+                for (int e = 0; e < (F32C ? 8 : 4); ++e)
+                    if (!is_v && kb * kPK + (u + 256 * j) / CH > last_key) raw[(F32C ? 8 : 4) * j + e] = 0u;
+        }
+    };
     auto load_raw = [&](int kb) {
+        if constexpr (kPaged)
+        {
+            load_paged(kb);
+            return;
+        }
         const uint64_t before = (uint64_t)kb * tile_bytes;
         const __amdgpu_buffer_rsrc_t rt = pf_rsrc(reinterpret_cast<const uint8_t*>(kvb) + before,
                                                   before < seq_bytes ? seq_bytes - (uint32_t)before : 0u);
@@ -642,6 +883,7 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
         }
     };
 
+    load_ids(0);
     load_raw(0);
 
     // ---- the lane's rotated query in halves: step c holds dimensions 16c + 8h + 0..7, scaled by 2^eq
@@ -651,7 +893,7 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
         float qv[DK / 2];
         uint32_t mx = 0;
         const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
-        load_query<DK, 8>(a, w, h, [&](int c, int e, float y0, float y1) {
+        load_query<DK, 8>(a, w, seq, h, [&](int c, int e, float y0, float y1) {
             qv[8 * c + e] = y0;
             qv[8 * (c + NC / 2) + e] = y1;
             mx = max(mx, max(__builtin_bit_cast(uint32_t, y0) & 0x7FFFFFFFu, __builtin_bit_cast(uint32_t, y1) & 0x7FFFFFFFu));
@@ -679,6 +921,7 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
     for (int d = 0; d < ND; ++d) o[d] = v16f{};
     float m_ref = -__builtin_inff(), l_run = 0.0f;  // log2 units; l_run: this lane half's keys
 
+    trim(0);
     post_max(0);
     if constexpr (!F32C)
     {
@@ -697,6 +940,7 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
     if (nkb > 1)
     {
         load_raw(1);
+        trim(1);
         post_max(1);
     }
     bool fallback = false;
@@ -719,7 +963,7 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
             convert(kb + 1, sflag + ((kb + 1) & 1));
             if (kb + 2 < nkb) load_raw(kb + 2);  // in flight during this tile's products
         }
-        if (w.live && kb * kPK <= a.pos0 + w.t0 + kPQ - 1)
+        if (w.live && kb * kPK <= seq.to(a, w))
         {
             // S^T = K . Q^T: the products of the halves but low x low (at most 2^-22 of a term)
             v16f s = v16f{};
@@ -743,12 +987,25 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
             }
             // scores in log2 units are s * f; the causal mask only where the tile reaches past the
             // wave's first query
-            const float f = F32C ? eqf * pow2(-ek_now) : eqf;
-            if (kb * kPK + kPK - 1 > a.pos0 + w.t0)
+            float f = F32C ? eqf * pow2(-ek_now) : eqf;
+            if constexpr (kShaped)
+            {
+                const float slope2 = a.slopes ? a.slopes[w.head] * 1.44269504f : 0.0f;
+                const float away = (float)(kb * kPK + 4 * h - w.qpos);
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                {
+                    float x = s[v] * f;
+                    if (a.cap2 > 0.0f) x = a.cap2 * shape_tanh(x * a.capi2);
+                    s[v] = __builtin_fmaf(slope2, away + (float)(8 * (v >> 2) + (v & 3)), x);
+                }
+                f = 1.0f;
+            }
+            if (kb * kPK + kPK - 1 > seq.from(a, w))
             {
 #pragma unroll
                 for (int v = 0; v < 16; ++v)
-                    if (kb * kPK + 8 * (v >> 2) + 4 * h + (v & 3) > w.qpos) s[v] = -__builtin_inff();
+                    if (kb * kPK + 8 * (v >> 2) + 4 * h + (v & 3) > seq.sight(w)) s[v] = -__builtin_inff();
             }
             float mx = s[0];
 #pragma unroll
@@ -807,47 +1064,64 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
             }
             o[ND - 1] += sum[(ND - 1) & 1];
         }
-        if (kb + 2 < nkb) post_max(kb + 2);
+        if (kb + 2 < nkb)
+        {
+            trim(kb + 2);
+            post_max(kb + 2);
+        }
     }
     // V is not looked through for infinities and NaN: any that matters is in the sums. Nor for values whose smallest part would lie below bf16's range: their output is tiny then.
     l_run += __shfl_xor(l_run, 32);
-    bool bad = !(l_run < __builtin_inff());
+    bool lost = !(l_run < __builtin_inff());
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int v = 0; v < 16; ++v)
         {
             const float y = fabsf(o[d][v]);
-            bad |= !(y < __builtin_inff()) || (y < l_run * kPTiny && y != 0.0f);
+            lost |= !(y < __builtin_inff()) || (y < l_run * kPTiny && y != 0.0f);
         }
-    if (__syncthreads_or(!fallback && w.live && bad) || fallback)
+    if (__syncthreads_or(!fallback && w.live && lost) || fallback)
     {
-        attend_f32<DK, CT>(a, w, last_key, rk, rv, reinterpret_cast<float*>(smem));
+        if constexpr (kPaged)
+        {
+            // everything from scratch: kept alive across the loop above, it would push that into spills
+            int t2 = threadIdx.x, block = blockIdx.x;
+            asm volatile("" : "+v"(t2), "+s"(block));
+            PrefillWave w2;
+            PrefillSeq<true> seq2;
+            int last2;
+            find_place(a, block, t2, w2, seq2, last2);
+            attend_f32<DK, kPaged, kShaped, CT>(a, w2, seq2, last2, rk, rv, reinterpret_cast<float*>(smem), t2);
+        }
+        else attend_f32<DK, kPaged, kShaped, CT>(a, w, seq, last_key, rk, rv, reinterpret_cast<float*>(smem), tid);
         return;
     }
+    if constexpr (kPaged)
+        if (__syncthreads_or(bad)) l_run = __builtin_nanf("");
     if (!w.live) return;
     // o / l, correctly rounded but for the last step's double rounding: the residual is exact
     const float r = 1.0f / l_run;
-    store_out<DK>(a, w, h, [](int d, int i) { return ND * i + d; }, [&](int d, int v) {
+    store_out<DK>(a, w, seq, h, [](int d, int i) { return ND * i + d; }, [&](int d, int v) {
         const float q = o[d][v] * r;
         return __builtin_fmaf(__builtin_fmaf(-q, l_run, o[d][v]), r, q);
     });
 }
 
-template <int DK, typename CT>
+template <int DK, bool kPaged, bool kShaped, typename CT>
 hipError_t launch_prefill_dk(hipStream_t st, const PrefillArgs& a)
 {
     constexpr int lds = PrefillTile<DK, CT>::kBytes;
     static bool attr_set = false;
     if (!attr_set)
     {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_attn_prefill<DK, CT>),
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_attn_prefill<DK, kPaged, kShaped, CT>),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
         attr_set = true;
     }
-    const unsigned blocks = (unsigned)(a.nqb * a.B * a.Hkv);
-    hipLaunchKernelGGL((k_attn_prefill<DK, CT>), dim3(blocks), dim3(kPThreads), lds, st, a);
+    const unsigned blocks = (unsigned)(a.nqb * a.B * a.Hkv * a.groups);
+    hipLaunchKernelGGL((k_attn_prefill<DK, kPaged, kShaped, CT>), dim3(blocks), dim3(kPThreads), lds, st, a);
     return hipGetLastError();
 }
 
@@ -892,16 +1166,43 @@ hipError_t launch_attn_prefill(hipStream_t st, const float* q, const void* kc, c
     const float mag = std::fabs(scale);
     const bool f32 = !(mag >= 0x1p-20f && mag <= 0x1p20f);
     PrefillArgs a{q, kc, vc, cosT, sinT, out, (int)B, (int)T, (int)H, (int)Hkv, (int)R, (int)pos0,
-                  (int)max_len, (int)ceil_div(T, kPQ * (kPWaves / R)), scale, (float)(mag * 1.4426950408889634), f32 ? 1 : 0};
+                  (int)max_len, (int)ceil_div(T, kPQ * (kPWaves / R)), scale, (float)(mag * 1.4426950408889634), f32 ? 1 : 0,
+                  (int)(B * T), 1};
     if (cache_f16)
     {
-        if (dk == 64) return launch_prefill_dk<64, _Float16>(st, a);
-        if (dk == 128) return launch_prefill_dk<128, _Float16>(st, a);
+        if (dk == 64) return launch_prefill_dk<64, false, false, _Float16>(st, a);
+        if (dk == 128) return launch_prefill_dk<128, false, false, _Float16>(st, a);
         return hipErrorInvalidValue;
     }
-    if (dk == 64) return launch_prefill_dk<64, float>(st, a);
-    if (dk == 128) return launch_prefill_dk<128, float>(st, a);
+    if (dk == 64) return launch_prefill_dk<64, false, false, float>(st, a);
+    if (dk == 128) return launch_prefill_dk<128, false, false, float>(st, a);
     return hipErrorInvalidValue;
+}
+
+hipError_t launch_pages_prefill(hipStream_t st, const nnhip_kv_pages& kv, const float* q, size_t M, const int32_t* cu,
+                                const int32_t* pos0, size_t B, size_t t_bound, size_t H, const float* cosT,
+                                const float* sinT, size_t limit, float scale, float softcap, const float* slopes,
+                                const int32_t* prefix, float* out)
+{
+    // a KV head's R query heads in work-groups of 8, 4, 2 or 1
+    const size_t heads = H / kv.Hkv, R = heads % 8 == 0 ? 8 : heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
+    const float mag = std::fabs(scale);
+    const bool f32 = !(mag >= 0x1p-20f && mag <= 0x1p20f);
+    const double cap2 = softcap * 1.4426950408889634;
+    PrefillArgs a{q, kv.k, kv.v, cosT, sinT, out, (int)B, (int)t_bound, (int)H, (int)kv.Hkv, (int)R, 0,
+                  (int)limit, (int)ceil_div(t_bound, kPQ * (kPWaves / R)), scale, (float)(mag * 1.4426950408889634), f32 ? 1 : 0,
+                  (int)M, (int)(heads / R), kv.table, cu, pos0, prefix, slopes, (int)kv.table_stride, (int)kv.num_pages,
+                  0, (int)limit, (float)cap2, softcap > 0.0f ? (float)(1.0 / cap2) : 0.0f};
+    while ((size_t(1) << a.shift) < kv.page_size) ++a.shift;
+    if (cap2 > 0.0 || slopes)
+    {
+        if (kv.f16)
+            return kv.dk == 64 ? launch_prefill_dk<64, true, true, _Float16>(st, a) : launch_prefill_dk<128, true, true, _Float16>(st, a);
+        return kv.dk == 64 ? launch_prefill_dk<64, true, true, float>(st, a) : launch_prefill_dk<128, true, true, float>(st, a);
+    }
+    if (kv.f16)
+        return kv.dk == 64 ? launch_prefill_dk<64, true, false, _Float16>(st, a) : launch_prefill_dk<128, true, false, _Float16>(st, a);
+    return kv.dk == 64 ? launch_prefill_dk<64, true, false, float>(st, a) : launch_prefill_dk<128, true, false, float>(st, a);
 }
 
 }  // namespace nnhip

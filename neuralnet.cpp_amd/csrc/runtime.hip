@@ -244,8 +244,8 @@ nnhip_status check_pages(const char* fn, const nnhip_kv_pages* c, const float* r
     NNHIP_REQUIRE(c && c->k && c->v && c->table, fn, "null cache, pool or page table");
     NNHIP_REQUIRE((rope_cos == nullptr) == (rope_sin == nullptr), fn, "rope_cos and rope_sin go together");
     NNHIP_REQUIRE(c->dk == 64 || c->dk == 128 || c->dk == 256, fn, "dk must be 64, 128 or 256");
-    NNHIP_REQUIRE(c->page_size >= 1 && c->page_size <= 1024 && (c->page_size & (c->page_size - 1)) == 0, fn,
-                  "page_size must be a power of two in [1, 1024]");
+    NNHIP_REQUIRE(c->page_size >= 8 && c->page_size <= 1024 && (c->page_size & (c->page_size - 1)) == 0, fn,
+                  "page_size must be a power of two in [8, 1024]");
     NNHIP_REQUIRE(c->Hkv >= 1 && c->Hkv <= 65535 && c->num_pages >= 1 && c->num_pages <= kMaxDim &&
                       c->num_pages <= kMaxDim / (c->Hkv * c->page_size), fn,
                   "num_pages * Hkv * page_size must be in [1, 2^31)");
@@ -2092,12 +2092,42 @@ nnhip_status nnhip_attention_pages_decode(nnhip_ctx* ctx, const nnhip_kv_pages* 
     NNHIP_REQUIRE(len_bound >= 1 && len_bound <= cache->table_stride * cache->page_size, fn,
                   "len_bound must be in [1, table_stride * page_size]");
     NNHIP_REQUIRE(!rope_cos || len_bound <= rope_len, fn, "len_bound must not exceed the rows of the rope tables");
-    NNHIP_REQUIRE(softcap >= 0.0f && softcap <= 3.0e38f, fn, "softcap must be finite and not negative");
+    NNHIP_REQUIRE(softcap >= 0.0f && softcap <= 1.0e30f && (softcap == 0.0f || softcap >= 1.0e-30f), fn,
+                  "softcap must be 0 or in [1e-30, 1e30]");
     void* ws = nullptr;
     st = ensure_stream_ws(ctx, pages_workspace_bytes(B, H, cache->Hkv, cache->dk, len_bound, (size_t)ctx->num_cus), fn, &ws);
     if (st != NNHIP_OK) return st;
     NNHIP_LAUNCH(fn, launch_pages_attn(ctx->stream, *cache, q, k, v, B, H, pos, len_bound, rope_cos, rope_sin, scale,
                                        softcap, slopes, tokens != 0, static_cast<float*>(ws), out, (size_t)ctx->num_cus));
+    return NNHIP_OK;
+}
+
+nnhip_status nnhip_attention_pages_prefill(nnhip_ctx* ctx, const nnhip_kv_pages* cache, const float* q, size_t M,
+                                           const int32_t* cu, const int32_t* pos0, size_t B, size_t t_bound, size_t H,
+                                           const float* rope_cos, const float* rope_sin, size_t rope_len, float scale,
+                                           float softcap, const float* slopes, const int32_t* prefix, float* out)
+{
+    const char* fn = "nnhip_attention_pages_prefill";
+    NNHIP_CHECK_CTX(fn);
+    const nnhip_status st = check_pages(fn, cache, rope_cos, rope_sin);
+    if (st != NNHIP_OK) return st;
+    if (!prefill_dk_supported(cache->dk)) return fail(NNHIP_ERR_UNSUPPORTED, fn, "dk must be 64 or 128");
+    if (M == 0 || B == 0 || t_bound == 0) return NNHIP_OK;
+    NNHIP_REQUIRE(q && cu && out, fn, "null pointer");
+    NNHIP_REQUIRE(H >= cache->Hkv && H % cache->Hkv == 0 && H <= 65535, fn,
+                  "H must be a multiple of Hkv, at most 65535");
+    NNHIP_REQUIRE(M < (size_t(1) << 29) && H * cache->dk * M < (size_t(1) << 29), fn,
+                  "q / out must be below 2^29 elements");
+    NNHIP_REQUIRE(softcap >= 0.0f && softcap <= 1.0e30f && (softcap == 0.0f || softcap >= 1.0e-30f), fn,
+                  "softcap must be 0 or in [1e-30, 1e30]");
+    NNHIP_REQUIRE(t_bound <= M, fn, "t_bound must not exceed M");
+    size_t limit = cache->table_stride * cache->page_size;
+    if (rope_cos) limit = std::min(limit, rope_len);
+    NNHIP_REQUIRE(!rope_cos || limit * cache->dk < (size_t(1) << 30), fn, "rope tables must be below 2 GiB");
+    NNHIP_REQUIRE(mul_ok(B, H) && mul_ok(B * H, ceil_div(t_bound, 32)) && B * H * ceil_div(t_bound, 32) < (size_t(1) << 22), fn,
+                  "B * H * ceil(t_bound / 32) must be below 2^22");
+    NNHIP_LAUNCH(fn, launch_pages_prefill(ctx->stream, *cache, q, M, cu, pos0, B, t_bound, H, rope_cos, rope_sin, limit,
+                                          scale, softcap, slopes, prefix, out));
     return NNHIP_OK;
 }
 

@@ -17,7 +17,7 @@ int main()
     long wrong = 0, seen = 0;
     for (int round = 0; round < 3000; ++round)
     {
-        const int shift = pick(0, 10), Hkv = pick(1, 9), num_pages = pick(1, 40), stride = pick(1, 30);
+        const int shift = pick(3, 10), Hkv = pick(1, 9), num_pages = pick(1, 40), stride = pick(1, 30);
         const long rows = (long)num_pages * Hkv << shift;
         const int capacity = stride << shift;
         std::vector<int32_t> table(stride);
@@ -30,7 +30,7 @@ int main()
             const int n = std::min(chunk, p - t0);
             const bool has_new = p - t0 < chunk;
             const int entries = page_entries(t0, t0 + n - (has_new ? 0 : 1), shift), e0 = t0 >> shift;
-            wrong += entries < 1 || entries > 1024 || e0 + entries > stride;
+            wrong += entries < 1 || entries > 1024 / 8 || e0 + entries > stride;
             for (int t = t0; t < t0 + n + (has_new ? 1 : 0); ++t)
             {
                 const int e = (t >> shift) - e0;

@@ -137,7 +137,7 @@ def test_decode_head_layouts(ctx, nnhip, H, Hkv, dk, f16):
     check_decode(ctx, nnhip, 3, H, Hkv, dk, 16, [0, 37, 300], f16, seed=1)
 
 
-@pytest.mark.parametrize("page", [1, 2, 8, 64, 1024])
+@pytest.mark.parametrize("page", [8, 16, 64, 1024])
 @pytest.mark.parametrize("f16", [False, True])
 def test_decode_page_sizes(ctx, nnhip, page, f16):
     # lengths on and beside the edges of tiles (16), waves' turns (64), chunks (128) and pages
@@ -258,6 +258,196 @@ def test_fill_matches_contiguous_fill(ctx, nnhip):
         assert same(got, host(ref)[:, :T])
 
 
+# ------------------------------------------------------------------------------------------ prompts
+
+# The prompt attention's products are sums of f16 and bf16 parts (or f32 products) that hold f32 operands to
+# 2^-22 of a term, so its outputs are held to the decode form's bound with 4 u for each u of a product.
+
+def check_prompt(ctx, nnhip, lens, pos0, H, Hkv, dk, page, f16, rope=True, cap=0.0, slopes=False, prefix=None, seed=0,
+                 spread=1.0, t_bound=None, edit=None):
+    print(f"prompt lens={lens} pos0={pos0} H={H} Hkv={Hkv} dk={dk} page={page} f16={f16} cap={cap} slopes={slopes} "
+          f"prefix={prefix}", flush=True)
+    rng = np.random.default_rng(seed + 7 * dk + H)
+    B, M = len(lens), sum(lens) + 3
+    cu = np.concatenate(([0], np.cumsum(lens))).astype(np.int32)
+    c = Cache(rng, [p + n for p, n in zip(pos0, lens)], Hkv, page, dk, f16)
+    q = (spread * rng.standard_normal((H, dk, M))).astype(np.float32)
+    if edit is not None:
+        edit(c, q)
+    cos, sin = nnhip.rope_table(dk, max(p + n for p, n in zip(pos0, lens))) if rope else (None, None)
+    sl = (2.0 ** (-8.0 * (np.arange(H) + 1) / H)).astype(np.float32) if slopes else None
+    scale = float(np.float32(1 / math.sqrt(dk)))
+    out = dev(np.full((H * dk, M), 77.0, np.float32))
+    ctx.attention_pages_prefill(c.on_device(nnhip), dev(q.reshape(H * dk, M)), dev(cu), t_bound or max(lens), H, scale,
+                                pos0=dev(np.array(pos0, np.int32)), cos=None if cos is None else dev(cos),
+                                sin=None if sin is None else dev(sin), softcap=cap, slopes=None if sl is None else dev(sl),
+                                prefix=None if prefix is None else dev(np.array(prefix, np.int32)), out=out)
+    out = host(out).astype(np.float64).reshape(H, dk, M)
+    assert np.all(out[:, :, cu[-1]:] == 77.0), "columns of no sequence were written"
+    worst = 0.0
+    for b, n in enumerate(lens):
+        if n == 0:
+            continue
+        K, V = c.rows(b, pos0[b] + n)
+        at = np.arange(pos0[b] + n)
+        for t in range(n):
+            i, m = pos0[b] + t, cu[b] + t
+            see = at <= i
+            if prefix is not None:
+                see |= at < prefix[b]
+            qr = rotate(q[:, :, m].astype(np.float64), cos, sin, i)
+            for h in range(H):
+                ref, tol = attend64(qr[h], K[:, h // (H // Hkv)], V[:, h // (H // Hkv)], scale, cap,
+                                    0.0 if sl is None else float(sl[h]), at - float(i), see)
+                got = out[h, :, m]
+                nan = np.isnan(ref)
+                assert np.array_equal(nan, np.isnan(got)), f"b={b} t={t} h={h}: NaN"
+                off = np.abs(got - ref)[~nan] / tol[~nan]
+                if off.size:
+                    worst = max(worst, float(off.max()))
+                    assert worst <= 4, f"b={b} t={t} h={h}: {worst} times the bound"
+    print(f"  {worst:.3f} of the bound", flush=True)
+    return out
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("dk", [64, 128])
+@pytest.mark.parametrize("H,Hkv", [(1, 1), (4, 2), (4, 1), (8, 1), (6, 2), (12, 1)])
+def test_prompt_head_layouts(ctx, nnhip, H, Hkv, dk, f16):
+    check_prompt(ctx, nnhip, [1, 37, 0, 65], [0, 0, 5, 11], H, Hkv, dk, 16, f16, seed=20)
+
+
+@pytest.mark.parametrize("page", [8, 64, 1024])
+@pytest.mark.parametrize("f16", [False, True])
+def test_prompt_page_sizes(ctx, nnhip, page, f16):
+    # lengths and starts on and beside the edges of tiles (32) and pages
+    check_prompt(ctx, nnhip, [31, 32, 33, 8, 7, 1], [0, 32, 31, 56, 1, 127], 2, 1, 64, page, f16, seed=21)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("cap,slopes,prefix", [(20.0, False, None), (0.0, True, None), (5.0, True, [40, 0, 200]),
+                                               (0.0, False, [200, 33, 1])])
+def test_prompt_shaped_scores(ctx, nnhip, cap, slopes, prefix, f16):
+    check_prompt(ctx, nnhip, [70, 45, 33], [0, 20, 100], 4, 2, 128, 32, f16, cap=cap, slopes=slopes, prefix=prefix, seed=22,
+                 spread=3.0)
+
+
+def test_prompt_bounds_and_no_rope(ctx, nnhip):
+    check_prompt(ctx, nnhip, [5, 90], [0, 0], 4, 4, 64, 16, False, rope=False, seed=23, t_bound=93)
+    check_prompt(ctx, nnhip, [3], [700], 4, 1, 64, 16, True, seed=24)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("cap", [0.0, 10.0])
+def test_prompt_nonfinite(ctx, nnhip, f16, cap):
+    """A NaN or an infinity in a key or a value reaches the queries that see it, and no other of the same
+    tile, work-group or sequence; scores of f32 range take the f32 products."""
+    def values(c, q):
+        c.v[c.table[0, 2], 0, 3, 5] = np.nan        # position 35
+        c.v[c.table[1, 0], 0, 9, 6] = np.inf        # position 9: infinite where it is seen
+        c.k[c.table[2, 1], 0, 4] = np.nan           # position 20
+
+    rng_lens = [60, 40, 50]
+    out = check_prompt_nonfinite(ctx, nnhip, rng_lens, f16, cap, values)
+    nan = np.isnan(out)
+    assert nan[:, 5, 35:60].all() and not nan[:, :, :35].any() and not nan[:, :5, 35:60].any()
+    assert np.isinf(out[:, 6, 69:100]).all() and np.isfinite(out[:, :, 60:69]).all()
+    assert nan[:, :, 120:150].all() and not nan[:, :, 100:120].any()
+    assert np.all(np.isfinite(out[:, 7, 60:100]))
+
+    def large(c, q):
+        q *= 1e4
+    if not f16:
+        check_prompt(ctx, nnhip, [40], [3], 2, 1, 64, 16, f16, cap=cap, seed=26, edit=large)
+
+
+def check_prompt_nonfinite(ctx, nnhip, lens, f16, cap, edit):
+    rng = np.random.default_rng(25)
+    H, dk, page = 2, 64, 16
+    c = Cache(rng, lens, 1, page, dk, f16)
+    M = sum(lens)
+    q = rng.standard_normal((H * dk, M)).astype(np.float32)
+    edit(c, q)
+    cu = np.concatenate(([0], np.cumsum(lens))).astype(np.int32)
+    return host(ctx.attention_pages_prefill(c.on_device(nnhip), dev(q), dev(cu), max(lens), H, 0.125, softcap=cap)).reshape(H, dk, M)
+
+
+def test_prompt_bad_sequences(ctx, nnhip):
+    """Sequences that do not fit get NaN in the columns that are there; a page outside the pool shows in
+    the queries that see it; the others keep their outputs."""
+    rng = np.random.default_rng(27)
+    H, Hkv, dk, page = 2, 1, 64, 16
+    lens = [40, 40, 40, 20]
+    c = Cache(rng, lens, Hkv, page, dk, False)
+    M = 140
+    q = dev(rng.standard_normal((H * dk, M)).astype(np.float32))
+    cu = np.concatenate(([0], np.cumsum(lens))).astype(np.int32)
+
+    def run(cu=cu, t_bound=40, pos0=None, table=None):
+        cache = nnhip.KVPages(dev(c.k), dev(c.v), dev(c.table if table is None else table))
+        return host(ctx.attention_pages_prefill(cache, q, dev(np.array(cu, np.int32)), t_bound, H, 0.125,
+                                                pos0=None if pos0 is None else dev(np.array(pos0, np.int32))))
+
+    ref = run()
+    assert np.all(np.isfinite(ref))
+    got = run(t_bound=39)
+    assert np.isnan(got[:, :120]).all() and np.array_equal(got[:, 120:], ref[:, 120:])
+    got = run(pos0=[0, 9, -1, 0])  # the second ends past its table's 48 positions
+    assert np.array_equal(got[:, :40], ref[:, :40]) and np.isnan(got[:, 40:120]).all()
+    got = run(cu=[0, 40, 80, 120, 200], t_bound=80)
+    assert np.array_equal(got[:, :120], ref[:, :120]) and np.isnan(got[:, 120:]).all()
+    for bad in (-1, c.k.shape[0], 2 ** 31 - 1):
+        t = c.table.copy()
+        t[1, 2] = bad  # positions 32 .. 39
+        t[3, 2] = bad  # past its length
+        got = run(table=t)
+        assert np.isnan(got[:, 72:80]).all()
+        keep = [m for m in range(M) if not 40 <= m < 80]
+        assert np.array_equal(got[:, keep], ref[:, keep])
+
+
+def test_prompt_matches_contiguous_prefill(ctx, nnhip):
+    """Equal prompts over pages against nnhip_attention_prefill on contiguous caches: the same arithmetic."""
+    rng = np.random.default_rng(28)
+    for f16 in (False, True):
+        B, T, H, Hkv, dk, page, past = 2, 70, 8, 2, 128, 16, 26
+        dt = np.float16 if f16 else np.float32
+        kc, vc = (rng.standard_normal((B, 96, Hkv * dk)).astype(dt) for _ in range(2))
+        q = dev(rng.standard_normal((H * dk, B * T)).astype(np.float32))
+        cos, sin = (dev(x) for x in nnhip.rope_table(dk, 96))
+        want = ctx.attention_prefill(q, dev(kc), dev(vc), B, T, H, Hkv, dk, past, 0.1, cos, sin)
+        table = rng.permutation(B * 6).astype(np.int32).reshape(B, 6)
+        pools = []
+        for x in (kc, vc):
+            pool = np.zeros((B * 6, Hkv, page, dk), dt)
+            pool[table] = x.reshape(B, 6, page, Hkv, dk).transpose(0, 1, 3, 2, 4)
+            pools.append(dev(pool))
+        got = ctx.attention_pages_prefill(nnhip.KVPages(*pools, dev(table)), q, dev(np.arange(B + 1, dtype=np.int32) * T), T, H,
+                                          0.1, pos0=dev(np.full(B, past, np.int32)), cos=cos, sin=sin)
+        assert same(host(got), host(want))
+
+
+def test_prompt_then_decode(ctx, nnhip):
+    """A prompt in one call and its last token alone by the decode form agree; fill, prompt and decode in turn."""
+    rng = np.random.default_rng(29)
+    H, Hkv, dk, page, lens = 8, 2, 64, 16, [50, 7, 33]
+    B, M = len(lens), sum(lens)
+    cu = np.concatenate(([0], np.cumsum(lens))).astype(np.int32)
+    table = dev(rng.permutation(B * 5).astype(np.int32).reshape(B, 5))
+    cache = nnhip.KVPages(*(dev(np.zeros((B * 5, Hkv, page, dk), np.float32)) for _ in range(2)), table)
+    q, k, v = (dev(rng.standard_normal((n * dk, M)).astype(np.float32)) for n in (H, Hkv, Hkv))
+    cos, sin = (dev(x) for x in nnhip.rope_table(dk, 80))
+    ctx.kv_pages_fill(cache, k, v, dev(cu), cos=cos, sin=sin)
+    before = host(cache.k)
+    out = host(ctx.attention_pages_prefill(cache, q, dev(cu), 50, H, 0.125, cos=cos, sin=sin))
+    last = [int(x) - 1 for x in cu[1:]]
+    one = host(ctx.attention_pages_decode(cache, q[:, last].contiguous(), k[:, last].contiguous(), v[:, last].contiguous(),
+                                          H, dev(np.array(lens, np.int32) - 1), 50, 0.125, cos=cos, sin=sin))
+    assert same(host(cache.k), before)  # the same rows again
+    # both within a few roundings of the same value: scores up to about 4, 50 terms
+    assert np.max(np.abs(one - out[:, last])) <= 64 * U * np.max(np.abs(host(v)))
+
+
 def test_refusals(ctx, nnhip):
     import torch
     f = dict(dtype=torch.float32, device="cuda")
@@ -277,7 +467,7 @@ def test_refusals(ctx, nnhip):
                dict(out=torch.zeros(2, 256, **f).t()), dict(q=q.cpu())):
         with pytest.raises(nnhip.NNHipError):
             decode(**kw)
-    for shape in ((4, 2, 16, 96), (4, 2, 24, 64), (4, 2, 2048, 64)):
+    for shape in ((4, 2, 16, 96), (4, 2, 24, 64), (4, 2, 4, 64), (4, 2, 2048, 64)):
         p = torch.zeros(shape, **f)
         with pytest.raises(nnhip.NNHipError):
             decode(cache=nnhip.KVPages(p, p.clone(), table))
@@ -295,6 +485,16 @@ def test_refusals(ctx, nnhip):
     with pytest.raises(nnhip.NNHipError):
         ctx.kv_pages_fill(c, kk, kk, cu, pos0=torch.zeros(2, **i))
     ctx.kv_pages_fill(c, kk[:, :0], kk[:, :0], cu)  # no columns: nothing to do
+    qq = torch.zeros(256, 3, **f)
+    ctx.attention_pages_prefill(c, qq, cu, 3, 4, 0.125)
+    for a, kw in (((qq, cu, 4, 4), {}), ((qq, cu, 3, 3), {}), ((qq, cu, 3, 2), {}), ((qq.half(), cu, 3, 4), {}),
+                  ((qq, cu, 3, 4), dict(softcap=-1.0)), ((qq, cu, 3, 4), dict(prefix=torch.zeros(2, **i))),
+                  ((qq, cu, 3, 4), dict(out=qq.t().contiguous())), ((qq, cu, 3, 4), dict(cos=torch.zeros(3, 32, **f)))):
+        with pytest.raises(nnhip.NNHipError):
+            ctx.attention_pages_prefill(c, *a, 0.125, **kw)
+    wide = torch.zeros(2, 1, 16, 256, **f)
+    with pytest.raises(nnhip.NNHipError, match="64 or 128"):
+        ctx.attention_pages_prefill(nnhip.KVPages(wide, wide.clone(), table), torch.zeros(256, 3, **f), cu, 3, 1, 0.1)
     ctx.sync()
 
 
