@@ -396,7 +396,6 @@ __device__ __forceinline__ float shape_tanh(float x)
 }
 
 // ---- paged KV cache (k_pages.hip; the prompt attention k_prefill.hip), logits (k_logits.hip)
-size_t pages_chunk(size_t B, size_t Hkv, size_t R, size_t len_bound, size_t num_cus);
 size_t pages_workspace_bytes(size_t B, size_t H, size_t Hkv, size_t dk, size_t len_bound, size_t num_cus);
 hipError_t launch_pages_attn(hipStream_t st, const nnhip_kv_pages& kv, const float* q, const float* k, const float* v,
                              size_t B, size_t H, const int32_t* pos, size_t len_bound, const float* cosT,

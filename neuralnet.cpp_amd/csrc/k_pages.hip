@@ -29,7 +29,11 @@ constexpr int kPgU = 4;          // rows of a group of 16 lanes in flight togeth
 constexpr int kPgTile = 16;      // rows of a wave's tile: 4 groups x kPgU
 constexpr int kPgMaxR = 8;       // query heads of a work-group
 constexpr int kPgRec = 16;       // tail of a record: maximum[8], sum[8]
-constexpr int kPgMaxChunk = 1024;
+#ifndef NNHIP_PG_MIN_CHUNK
+#define NNHIP_PG_MIN_CHUNK 128
+#endif
+constexpr int kPgMinChunk = NNHIP_PG_MIN_CHUNK;  // positions of a work-group at least (a multiple of 64)
+constexpr int kPgEvenB = 1024;   // sequences up to which the chunks are sized by the lengths
 constexpr float kPgLazy = 8.0f;  // log2 growth of a maximum before its sums are rescaled
 
 struct PagesArgs
@@ -48,7 +52,9 @@ struct PagesArgs
     float* out;
     int B, H, Hkv, R, groups, RG;  // R = H / Hkv heads of a KV head, in `groups` groups of at most RG
     int shift;                     // log2(page_size)
-    int table_stride, num_pages, len_bound, chunk, nchunk;
+    int table_stride, num_pages, len_bound;
+    int chunk, nchunk;             // even == 0: chunks of every sequence
+    int even;                      // > 0: chunks sized by the lengths (see find_item), about `even` of them
     float scale2;  // scale * log2(e)
     float capi;    // scale / softcap
     float cap2;    // softcap * log2(e), 0 without a cap
@@ -169,9 +175,66 @@ struct PagesRow
     }
 };
 
-// Attention of one new token per sequence. Work-group = (chunk of `chunk` positions, KV head and group
-// of at most 8 of its query heads, sequence); a group of 16 lanes takes one row of dk at a time, 4 rows
-// on their way together, so a wave's tile is 16 rows; its four waves take the chunk's tiles in turn.
+// A barrier for LDS data only: loads of the pools stay in flight across it
+__device__ __forceinline__ void lds_barrier()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // vmcnt and expcnt at their maxima, lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// Where a work-group works: chunk c of `chunk` positions of sequence b, whose new token has position p;
+// `first` = the sequence's first record. b < 0: nothing to do.
+struct PagesItem
+{
+    int b, c, chunk, first, p;
+};
+
+__device__ __forceinline__ int pages_len(const PagesArgs& a, int p) { return p < 0 || p >= a.len_bound ? 0 : p + 1; }
+
+// Item `item` of a call (with seq >= 0: the first of that sequence). With lengths spread from 1 to 16 K,
+// chunks of one size for len_bound leave a few long work-groups and thousands of empty ones (37 sequences
+// of 1 .. 16384 over 2 KV heads: 63 us against 26), so every wave sizes the chunks by the lengths
+// themselves: with D = a.even the smallest multiple of 64 that is at least sum(len) / D, which makes at
+// most D + B chunks. Every work-group of the call and the join find the same ones; nothing is kept.
+__device__ __forceinline__ PagesItem find_item(const PagesArgs& a, int item, int seq)
+{
+    const int lane = threadIdx.x & 63;
+    uint32_t total = 0;  // below 2^31
+    for (int b = lane; b < a.B; b += kWave) total += (uint32_t)pages_len(a, a.pos[b]);
+    for (int off = 1; off < min(a.B, kWave); off <<= 1) total += (uint32_t)__shfl_xor((int)total, off, kWave);
+    total = (uint32_t)__builtin_amdgcn_readfirstlane((int)total);
+    const int chunk = max(kPgMinChunk, (int)(64 * (((total + 63) / 64 + (uint32_t)a.even - 1) / (uint32_t)a.even)));
+    int before = 0;
+    for (int b0 = 0; b0 < a.B; b0 += kWave)
+    {
+        const int b = b0 + lane, p = b < a.B ? a.pos[b] : -1;
+        const int n = b < a.B ? max(1, (int)(((uint32_t)pages_len(a, p) + (uint32_t)chunk - 1) / (uint32_t)chunk)) : 0;
+        const int live = min(a.B - b0, kWave);
+        int incl = n;
+        for (int off = 1; off < live; off <<= 1)
+        {
+            const int x = __shfl_up(incl, off, kWave);
+            if (lane >= off) incl += x;
+        }
+        const int sum = __builtin_amdgcn_readlane(incl, live - 1);
+        const unsigned long long here = __builtin_amdgcn_ballot_w64(b < a.B && (seq >= 0 ? b == seq : before + incl > item));
+        if (here != 0)
+        {
+            const int l = __builtin_ctzll(here);
+            const int first = before + __builtin_amdgcn_readlane(incl - n, l);
+            return {b0 + l, item - first, chunk, first, __builtin_amdgcn_readlane(p, l)};
+        }
+        before += sum;
+    }
+    return {-1, 0, chunk, 0, -1};
+}
+
+// Attention of one new token per sequence. Work-group = (chunk of positions, KV head and group of at most 8
+// of its query heads, sequence); a group of 16 lanes takes one row of dk at a time, 4 rows on their way
+// together, so a wave's tile is 16 rows; its four waves take the chunk's tiles in turn. A tile lies in one
+// page, or in two of 8 rows: its addresses are the wave's.
 // No wave waits for another before the chunk's end: each group of 16 lanes keeps running maxima, sums
 // and weighted values of its own rows. q stays in registers (each lane the elements of its columns).
 //   scores   each lane multiplies its columns, the sums over 16 lanes come out spread over them
@@ -186,19 +249,36 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
 {
     using Row = PagesRow<DK, CT>;
     constexpr int E = Row::E, HALF = DK / 2, NV = RT / 4 > 1 ? RT / 4 : 1;  // scores per lane
-    constexpr int NS = kPgU * RT;
+    constexpr int NS = kPgU * RT, QI = (RT * HALF + kPgThreads - 1) / kPgThreads;  // query pairs per thread
     __shared__ __align__(16) float q_s[RT * DK];
     __shared__ float new_s[2][DK];
-    __shared__ int page_s[kPgMaxChunk / 8];  // a page holds 8 positions or more
     __shared__ float ml_s[2][kPgWaves * 4][RT];
     __shared__ float red_s[kPgWaves][RT * DK];
+    __shared__ float tot_s[2][RT];
+    __shared__ int bad_s[kPgWaves];
 
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, j = lane & 15, grp = lane >> 4;
-    const int c = blockIdx.x, b = blockIdx.z;
-    const int g = blockIdx.y / a.groups, hg = blockIdx.y - g * a.groups;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 15, grp = lane >> 4;
+    const int HG = a.Hkv * a.groups;
+    const int gh = blockIdx.x % HG, item = blockIdx.x / HG;
+    const int g = gh / a.groups, hg = gh - g * a.groups;
+    const PagesItem it = !kFinal && a.even ? find_item(a, item, -1)
+                                           : PagesItem{item / a.nchunk, item % a.nchunk, a.chunk, item - item % a.nchunk,
+                                                       a.pos[item / a.nchunk]};
+    if (it.b < 0) return;
+    const int b = it.b, c = it.c, p = it.p;
     const int h0 = g * a.R + hg * a.RG;            // first query head
     const int R = min(a.RG, a.R - hg * a.RG);      // query heads here (<= RT)
-    const int p = a.pos[b];
+    // the query pairs, on their way while the rest finds its place
+    const size_t in_step = a.tokens ? 1 : (size_t)a.B;
+    float qx[QI][2];
+#pragma unroll
+    for (int u = 0; u < QI; ++u)
+    {
+        const int e = tid + u * kPgThreads, r = min(e / HALF, R - 1), i = e % HALF;
+        const float* q = a.q + (a.tokens ? ((size_t)b * a.H + h0 + r) * DK : (size_t)(h0 + r) * DK * a.B + b);
+        qx[u][0] = q[i * in_step];
+        qx[u][1] = q[(i + HALF) * in_step];
+    }
     const size_t out_step = a.tokens ? 1 : (size_t)a.B;
     float* const out = a.out + (a.tokens ? ((size_t)b * a.H + h0) * DK : (size_t)h0 * DK * a.B + b);
     if (p < 0 || p >= a.len_bound)
@@ -208,36 +288,57 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
             for (int e = tid; e < R * DK; e += kPgThreads) out[e * out_step] = p < 0 ? 0.0f : __builtin_nanf("");
         return;
     }
-    const int t0 = c * a.chunk;
+    const int t0 = c * it.chunk;
     if (t0 > p) return;
-    const int n = min(a.chunk, p - t0);            // cached rows here
-    const bool has_new = p - t0 < a.chunk;
+    const int n = min(it.chunk, p - t0);           // cached rows here
+    const bool has_new = p - t0 < it.chunk;
 
-    // ---- rotated queries, the page of each of the chunk's pages, the new key and value
-    const size_t in_step = a.tokens ? 1 : (size_t)a.B;
-    for (int e = tid; e < RT * HALF; e += kPgThreads)
-    {
-        const int r = e / HALF, i = e - r * HALF;
-        float y0 = 0.0f, y1 = 0.0f;
-        if (r < R)
-        {
-            const float* q = a.q + (a.tokens ? ((size_t)b * a.H + h0 + r) * DK : (size_t)(h0 + r) * DK * a.B + b);
-            y0 = q[i * in_step], y1 = q[(i + HALF) * in_step];
-            if (a.cosT) pg_rope(y0, y1, a.cosT[(size_t)p * HALF + i], a.sinT[(size_t)p * HALF + i], y0, y1);
-        }
-        q_s[r * DK + i] = y0;
-        q_s[r * DK + i + HALF] = y1;
-    }
-    const int page0 = t0 >> a.shift;
-    const int pages = page_entries(t0, t0 + n - (has_new ? 0 : 1), a.shift);
-    const int32_t* table = a.table + (size_t)b * a.table_stride + page0;
+    // ---- the wave's first tile: its page ids
+    const int32_t* const table = a.table + (size_t)b * a.table_stride;
     bool bad = false;
-    for (int e = tid; e < pages; e += kPgThreads)
+    int ids[2];
+    auto load_ids = [&](int base) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) ids[i] = table[(t0 + min(base + 8 * i, max(n - 1, 0))) >> a.shift];
+    };
+    load_ids(w * kPgTile);
+    const int new_id = has_new ? table[p >> a.shift] : 0;
+    const int slot_mask = (1 << a.shift) - 1;
+    const CT* const kc = static_cast<const CT*>(a.kc);
+    const CT* const vc = static_cast<const CT*>(a.vc);
+    Row kr[kPgU], vr[kPgU];
+    auto load = [&](int base) {
+        size_t at[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+        {
+            const int id = __builtin_amdgcn_readfirstlane(ids[i]);
+            const bool in = page_ok(id, a.num_pages);
+            bad |= !in;
+            // rows 8 i .. 8 i + 7 of the tile; those behind the chunk's last row are in the same page as its
+            // last 8 rows, or read those (their score is -inf)
+            at[i] = page_row(in ? id : 0, g, (t0 + min(base + 8 * i, (n - 1) & ~7)) & slot_mask, a.Hkv, a.shift) * DK;
+        }
+        load_ids(base + kPgWaves * kPgTile);
+#pragma unroll
+        for (int u = 0; u < kPgU; ++u) kr[u].load(kc + at[u / 2] + (4 * (u & 1) + grp) * DK, j);
+#pragma unroll
+        for (int u = 0; u < kPgU; ++u) vr[u].load(vc + at[u / 2] + (4 * (u & 1) + grp) * DK, j);
+    };
+
+    // ---- rotated queries, the new key and value
+#pragma unroll
+    for (int u = 0; u < QI; ++u)
     {
-        const int id = table[e];
-        const bool in = page_ok(id, a.num_pages);
-        bad |= !in;
-        page_s[e] = in ? id : 0;
+        const int e = tid + u * kPgThreads, r = e / HALF, i = e % HALF;
+        float y0 = qx[u][0], y1 = qx[u][1];
+        if (a.cosT) pg_rope(y0, y1, a.cosT[(size_t)p * HALF + i], a.sinT[(size_t)p * HALF + i], y0, y1);
+        if (e < RT * HALF)
+        {
+            // (heads past R stay 0)
+            q_s[r * DK + i] = r < R ? y0 : 0.0f;
+            q_s[r * DK + i + HALF] = r < R ? y1 : 0.0f;
+        }
     }
     if (has_new && tid < HALF)
     {
@@ -252,15 +353,18 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
         new_s[1][tid] = (float)(CT)v[tid * in_step];
         new_s[1][tid + HALF] = (float)(CT)v[(tid + HALF) * in_step];
     }
-    bad = __syncthreads_or(bad) != 0;
-    const int slot_mask = (1 << a.shift) - 1;
-    const CT* const kc = static_cast<const CT*>(a.kc);
-    const CT* const vc = static_cast<const CT*>(a.vc);
-    if (has_new && hg == 0 && !bad)
+    if (w * kPgTile < n) load(w * kPgTile);  // the first tile, on its way during the rest
+    lds_barrier();
+    if (has_new)
     {
-        const size_t at = page_row(page_s[pages - 1], g, p & slot_mask, a.Hkv, a.shift) * DK;
-        for (int i = tid; i < 2 * DK; i += kPgThreads)
-            const_cast<CT*>(i < DK ? kc : vc)[at + (size_t)(i & (DK - 1))] = (CT)new_s[i / DK][i & (DK - 1)];
+        const bool in = page_ok(new_id, a.num_pages);
+        bad |= !in;
+        if (hg == 0 && in)
+        {
+            const size_t at = page_row(new_id, g, p & slot_mask, a.Hkv, a.shift) * DK;
+            for (int i = tid; i < 2 * DK; i += kPgThreads)
+                const_cast<CT*>(i < DK ? kc : vc)[at + (size_t)(i & (DK - 1))] = (CT)new_s[i / DK][i & (DK - 1)];
+        }
     }
 
     float q[RT][E];
@@ -287,21 +391,8 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[r][e] = 0.0f;
 
-    auto tile = [&](int base, auto full) {
-        constexpr bool kFull = decltype(full)::value;
-        Row kr[kPgU], vr[kPgU];
-        size_t at[kPgU];
-#pragma unroll
-        for (int u = 0; u < kPgU; ++u)
-        {
-            // rows behind the chunk's last read its first page's first row (their score is -inf)
-            int t = t0 + base + 4 * u + grp;
-            if (!kFull && base + 4 * u + grp >= n) t = t0;
-            at[u] = page_row(page_s[(t >> a.shift) - page0], g, t & slot_mask, a.Hkv, a.shift) * DK;
-            kr[u].load(kc + at[u], j);
-        }
-#pragma unroll
-        for (int u = 0; u < kPgU; ++u) vr[u].load(vc + at[u], j);
+    auto tile = [&](int base) {
+        const bool part = base + kPgTile > n;  // rows behind the chunk's last one
         float s[NS];
 #pragma unroll
         for (int u = 0; u < kPgU; ++u)
@@ -321,7 +412,7 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
         {
             const int tl = base + 4 * ur + grp;
             x[i] = shape(s[i], i, t0 + tl);
-            if (!kFull && tl >= n) x[i] = -__builtin_inff();
+            if (part && tl >= n) x[i] = -__builtin_inff();
             top[i] = fmaxf(x[i], dpp<kDppRor8>(x[i]));
             top[i] = fmaxf(top[i], dpp<kDppRor4>(top[i]));
             grown |= top[i] > m[i] + kPgLazy;
@@ -352,9 +443,12 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
             pr[i] = x[i] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x[i] - m[i]);
             l[i] += pr[i];
         }
+        if (part)  // whatever is there: 0 * it has to be 0
+#pragma unroll
+            for (int u = 0; u < kPgU; ++u)
+                if (base + 4 * u + grp >= n) vr[u].zero();
         static_for<kPgU>([&](auto uu) {
             constexpr int u = decltype(uu)::value;
-            if (!kFull && base + 4 * u + grp >= n) vr[u].zero();  // whatever is there: 0 * it has to be 0
             static_for<RT>([&](auto r) {
                 constexpr int h = decltype(r)::value;
                 const float f = bcast16<4 * u + (RT >= 4 ? h / NV : 2 * h)>(pr[h % NV]);
@@ -363,12 +457,16 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
             });
         });
     };
-    int base = w * kPgTile;
-    for (; base + kPgTile <= n; base += kPgWaves * kPgTile) tile(base, std::true_type{});
-    if (base < n) tile(base, std::false_type{});
+    // (the next tile's rows on their way during a tile, in registers of their own, changed nothing: the other
+    // waves' are)
+    for (int base = w * kPgTile; base < n; base += kPgWaves * kPgTile)
+    {
+        if (base != w * kPgTile) load(base);
+        tile(base);
+    }
 
-    // ---- the new position: one more row of the first group of the first wave
-    if (has_new && w == 0)
+    // ---- the new position: one more row, of the first group of the wave whose turn it is
+    if (has_new && w == (n + kPgTile - 1) / kPgTile % kPgWaves)
     {
         float s[NS];
 #pragma unroll
@@ -416,16 +514,29 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
             ml_s[1][4 * w + grp][hs + i] = l[i];
         }
     }
+    if (lane == 0) bad_s[w] = bad;
     __syncthreads();
     constexpr int N = RT * E;
     float y[N];
 #pragma unroll
     for (int r = 0; r < RT; ++r)
     {
-        float top = -__builtin_inff();
-#pragma unroll
-        for (int i = 0; i < 4 * kPgWaves; ++i) top = fmaxf(top, ml_s[0][i][r]);
-        const float own = ml_s[0][4 * w + grp][r];
+        // lane j of every 16: group j's maximum and sum
+        const float mj = ml_s[0][j][r], own = ml_s[0][4 * w + grp][r];
+        float top = mj;
+        top = fmaxf(top, dpp<kDppRor8>(top));
+        top = fmaxf(top, dpp<kDppRor4>(top));
+        top = fmaxf(top, dpp<kDppXor2>(top));
+        top = fmaxf(top, dpp<kDppXor1>(top));
+        if (w == r % kPgWaves)
+        {
+            float sum = ml_s[1][j][r] * (mj == top ? 1.0f : __builtin_amdgcn_exp2f(mj - top));
+            sum += dpp<kDppRor8>(sum);
+            sum += dpp<kDppRor4>(sum);
+            sum += dpp<kDppXor2>(sum);
+            sum += dpp<kDppXor1>(sum);
+            if (lane == 0) tot_s[0][r] = top, tot_s[1][r] = sum;
+        }
         // (a NaN among the scores leaves its sum and values NaN, not the maximum)
         const float f = own == top ? 1.0f : __builtin_amdgcn_exp2f(own - top);
 #pragma unroll
@@ -443,30 +554,20 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
         red_s[w][at / E * DK + Row::dim(at % E, j)] = fold16_rows(y[i], y[i + N / 4]);
     }
     __syncthreads();
-    float* const rec = a.part + ((((size_t)b * a.Hkv + g) * a.groups + hg) * a.nchunk + c) * (size_t)(a.RG * DK + kPgRec);
+    bad = (bad_s[0] | bad_s[1] | bad_s[2] | bad_s[3]) != 0;
+    float* const rec = a.part + ((size_t)(it.first + c) * HG + gh) * (size_t)(a.RG * DK + kPgRec);
     for (int e = tid; e < R * DK; e += kPgThreads)
     {
         const int r = e / DK;
-        float top = -__builtin_inff(), sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4 * kPgWaves; ++i) top = fmaxf(top, ml_s[0][i][r]);
-#pragma unroll
-        for (int i = 0; i < 4 * kPgWaves; ++i)
-        {
-            const float mi = ml_s[0][i][r];
-            sum += ml_s[1][i][r] * (mi == top ? 1.0f : __builtin_amdgcn_exp2f(mi - top));
-        }
-        float v = red_s[0][e];
-#pragma unroll
-        for (int i = 1; i < kPgWaves; ++i) v += red_s[i][e];
-        if (bad) sum = __builtin_nanf("");
+        const float sum = bad ? __builtin_nanf("") : tot_s[1][r];
+        const float v = (red_s[0][e] + red_s[1][e]) + (red_s[2][e] + red_s[3][e]);
         if constexpr (kFinal) out[e * out_step] = sum == 0.0f ? 0.0f : v / sum;
         else
         {
             rec[e] = v;
             if (e % DK == 0)
             {
-                rec[a.RG * DK + r] = top;
+                rec[a.RG * DK + r] = tot_s[0][r];
                 rec[a.RG * DK + 8 + r] = sum;
             }
         }
@@ -481,12 +582,13 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_join(PagesArgs a)
     __shared__ float4 acc_s[G][L];
     __shared__ float m_s[G], l_s[G];
     const int h = blockIdx.x, b = blockIdx.y;
-    const int p = a.pos[b];
+    const PagesItem it = a.even ? find_item(a, 0, b) : PagesItem{b, 0, a.chunk, b * a.nchunk, a.pos[b]};
+    const int p = it.p;
     if (p < 0 || p >= a.len_bound) return;  // the chunks' kernel wrote those
     const int g = h / a.R, r0 = h - g * a.R, hg = r0 / a.RG, r = r0 - hg * a.RG;
-    const int nch = p / a.chunk + 1;
-    const size_t step = (size_t)(a.RG * DK + kPgRec);
-    const float* rec = a.part + (((size_t)b * a.Hkv + g) * a.groups + hg) * a.nchunk * step;
+    const int nch = p / it.chunk + 1, HG = a.Hkv * a.groups;
+    const size_t step = (size_t)HG * (a.RG * DK + kPgRec);
+    const float* rec = a.part + ((size_t)it.first * HG + g * a.groups + hg) * (size_t)(a.RG * DK + kPgRec);
     const int tid = threadIdx.x, i = tid % L, gr = tid / L;
     float m = -__builtin_inff(), l = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -544,10 +646,17 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_join(PagesArgs a)
     o[0] = y.x / inv, o[st] = y.y / inv, o[2 * st] = y.z / inv, o[3 * st] = y.w / inv;
 }
 
+// Chunks of a call at most, over all sequences
+size_t pages_items(size_t B, size_t len_bound, size_t chunk, size_t even)
+{
+    const size_t all = B * ceil_div(len_bound, chunk);
+    return even && even + B < all ? even + B : all;
+}
+
 template <int DK, int RT, typename CT>
 hipError_t launch_pages_rt(hipStream_t st, const PagesArgs& a)
 {
-    const dim3 grid((unsigned)a.nchunk, (unsigned)(a.Hkv * a.groups), (unsigned)a.B);
+    const dim3 grid((unsigned)(pages_items(a.B, a.len_bound, a.chunk, a.even) * a.Hkv * a.groups));
     if (a.nchunk == 1)
     {
         k_pages_attn<DK, RT, true, CT><<<grid, kPgThreads, 0, st>>>(a);
@@ -565,8 +674,8 @@ hipError_t launch_pages_dk(hipStream_t st, const PagesArgs& a)
 {
     if (a.RG == 1) return launch_pages_rt<DK, 1, CT>(st, a);
     if (a.RG == 2) return launch_pages_rt<DK, 2, CT>(st, a);
-    if (a.RG <= 4) return launch_pages_rt<DK, 4, CT>(st, a);
-    return launch_pages_rt<DK, 8, CT>(st, a);
+    if (DK == 256 || a.RG <= 4) return launch_pages_rt<DK, 4, CT>(st, a);
+    if constexpr (DK != 256) return launch_pages_rt<DK, 8, CT>(st, a);
 }
 
 // ------------------------------------------------------------------ fill from packed prompts
@@ -671,21 +780,36 @@ int log2_of(size_t v)
 
 }  // namespace
 
-// Query heads of a KV head in groups of at most kPgMaxR, as even as they go
-static size_t pages_groups(size_t R) { return ceil_div(R, (size_t)kPgMaxR); }
+// Query heads of a KV head in groups of at most 8 (dk = 256: 4, whose registers are as many), as even as they go
+static size_t pages_groups(size_t R, size_t dk) { return ceil_div(R, (size_t)(dk == 256 ? 4 : kPgMaxR)); }
 
-size_t pages_chunk(size_t B, size_t Hkv, size_t R, size_t len_bound, size_t num_cus)
+// How a call is cut: chunks of `chunk` positions (nchunk to a sequence), or with even > 0 about `even` of a
+// size that the kernels find
+struct PagesCut
 {
-    size_t chunk = 128;
-    while (chunk < kPgMaxChunk && B * Hkv * pages_groups(R) * ceil_div(len_bound, chunk) > 8 * num_cus) chunk *= 2;
-    return chunk;
+    size_t chunk, nchunk, even;
+};
+
+static PagesCut pages_cut(size_t B, size_t Hkv, size_t R, size_t dk, size_t len_bound, size_t num_cus)
+{
+    const size_t HG = Hkv * pages_groups(R, dk);
+#ifndef NNHIP_PG_PER_CU
+#define NNHIP_PG_PER_CU 2
+#endif
+    const size_t want = ceil_div(NNHIP_PG_PER_CU * num_cus, HG);  // chunks that fill the GPU
+    if (len_bound <= kPgMinChunk) return {kPgMinChunk, 1, 0};
+    if (B <= kPgEvenB && B * len_bound < (size_t(1) << 31)) return {kPgMinChunk, 0, want > 2 * B ? want - B : B};
+    size_t chunk = kPgMinChunk;
+    while (B * ceil_div(len_bound, chunk) > 2 * want && chunk < len_bound) chunk *= 2;
+    return {chunk, ceil_div(len_bound, chunk), 0};
 }
 
 size_t pages_workspace_bytes(size_t B, size_t H, size_t Hkv, size_t dk, size_t len_bound, size_t num_cus)
 {
-    const size_t R = H / Hkv, groups = pages_groups(R);
-    const size_t nchunk = ceil_div(len_bound, pages_chunk(B, Hkv, R, len_bound, num_cus));
-    return nchunk <= 1 ? 0 : B * Hkv * groups * nchunk * (ceil_div(R, groups) * dk + kPgRec) * sizeof(float);
+    const size_t R = H / Hkv, groups = pages_groups(R, dk);
+    const PagesCut cut = pages_cut(B, Hkv, R, dk, len_bound, num_cus);
+    if (cut.nchunk == 1) return 0;
+    return pages_items(B, len_bound, cut.chunk, cut.even) * Hkv * groups * (ceil_div(R, groups) * dk + kPgRec) * sizeof(float);
 }
 
 hipError_t launch_pages_attn(hipStream_t st, const nnhip_kv_pages& kv, const float* q, const float* k, const float* v,
@@ -694,12 +818,12 @@ hipError_t launch_pages_attn(hipStream_t st, const nnhip_kv_pages& kv, const flo
                              float* part, float* out, size_t num_cus)
 {
     constexpr double kLog2e = 1.4426950408889634;
-    const size_t R = H / kv.Hkv, groups = pages_groups(R);
-    const size_t chunk = pages_chunk(B, kv.Hkv, R, len_bound, num_cus);
+    const size_t R = H / kv.Hkv, dk = kv.dk, groups = pages_groups(R, dk);
+    const PagesCut cut = pages_cut(B, kv.Hkv, R, dk, len_bound, num_cus);
     const bool cap = softcap > 0.0f;
     PagesArgs a{q, k, v, pos, cosT, sinT, kv.k, kv.v, kv.table, slopes, part, out, (int)B, (int)H, (int)kv.Hkv, (int)R,
                 (int)groups, (int)ceil_div(R, groups), log2_of(kv.page_size), (int)kv.table_stride, (int)kv.num_pages,
-                (int)len_bound, (int)chunk, (int)ceil_div(len_bound, chunk), (float)(scale * kLog2e),
+                (int)len_bound, (int)cut.chunk, (int)cut.nchunk, (int)cut.even, (float)(scale * kLog2e),
                 cap ? scale / softcap : 0.0f, cap ? (float)(softcap * kLog2e) : 0.0f, tokens ? 1 : 0};
     if (kv.f16)
     {

@@ -2088,7 +2088,7 @@ nnhip_status nnhip_attention_pages_decode(nnhip_ctx* ctx, const nnhip_kv_pages* 
     NNHIP_REQUIRE(q && k && v && pos && out, fn, "null pointer");
     NNHIP_REQUIRE(H >= cache->Hkv && H % cache->Hkv == 0 && H <= 65535, fn,
                   "H must be a multiple of Hkv, at most 65535");
-    NNHIP_REQUIRE(B <= 65535, fn, "B must be at most 65535");
+    NNHIP_REQUIRE(B <= 65535 && B * H < (size_t(1) << 22), fn, "B must be at most 65535, B * H below 2^22");
     NNHIP_REQUIRE(len_bound >= 1 && len_bound <= cache->table_stride * cache->page_size, fn,
                   "len_bound must be in [1, table_stride * page_size]");
     NNHIP_REQUIRE(!rope_cos || len_bound <= rope_len, fn, "len_bound must not exceed the rows of the rope tables");
