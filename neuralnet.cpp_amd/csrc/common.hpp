@@ -381,18 +381,25 @@ hipError_t launch_embed(hipStream_t st, const float* table, const int32_t* ids, 
 hipError_t launch_argmax(hipStream_t st, const float* L, size_t V, size_t B, int32_t* ids, bool rows = false,
                          int32_t* pos = nullptr);
 
-// tanh to about 1e-7 of itself: the odd series below 0.3 (its next term is 2e-9), else from exp
-__device__ __forceinline__ float shape_tanh(float x)
+// tanh to 1e-7 of itself, for |x| <= 1 (an odd polynomial through the Chebyshev points, 2e-8 off before
+// rounding) and for any x (from exp beyond 1)
+__device__ __forceinline__ float tanh_below1(float x)
 {
-    const float a = fabsf(x), z = x * x;
-    float s = -8.8632355e-3f;  // -1382 / 155925
-    s = __builtin_fmaf(s, z, 2.1869489e-2f);
-    s = __builtin_fmaf(s, z, -5.3968254e-2f);
-    s = __builtin_fmaf(s, z, 0.13333333f);
-    s = __builtin_fmaf(s, z, -0.33333333f);
-    const float small = __builtin_fmaf(x * z, s, x);
-    const float big = copysignf(__builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(a * 2.8853900f) + 1.0f), 1.0f), x);
-    return a < 0.3f ? small : big;
+    const float z = x * x;
+    float s = -4.206954909e-04f;
+    s = __builtin_fmaf(s, z, 2.510459395e-03f);
+    s = __builtin_fmaf(s, z, -8.218921721e-03f);
+    s = __builtin_fmaf(s, z, 2.166011557e-02f);
+    s = __builtin_fmaf(s, z, -5.393479019e-02f);
+    s = __builtin_fmaf(s, z, 1.333312839e-01f);
+    s = __builtin_fmaf(s, z, -3.333333135e-01f);
+    return __builtin_fmaf(x * z, s, x);
+}
+__device__ __forceinline__ float tanh_any(float x)
+{
+    const float a = fabsf(x);
+    const float far = copysignf(__builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(a * 2.8853900f) + 1.0f), 1.0f), x);
+    return a > 1.0f ? far : tanh_below1(x);
 }
 
 // ---- paged KV cache (k_pages.hip; the prompt attention k_prefill.hip), logits (k_logits.hip)

@@ -6,13 +6,13 @@
 #include "common.hpp"
 #include "pages_index.hpp"
 
+#include <algorithm>
+
 namespace nnhip
 {
 namespace
 {
 
-constexpr int kLgThreads = 1024;
-constexpr int kLgU = 4;       // groups of 4 logits in flight per thread
 constexpr int kLgSlices = 64; // at most, of a row
 
 // What a slice of a row found: its best value (index -1: none), and its first allowed token as
@@ -74,9 +74,10 @@ __device__ __forceinline__ void choose(const LogitArgs& a, int b, const LogitBes
 
 // Work-group = a slice of row b in groups of 4 logits. Bound by HBM: logits, counts, biases and masks
 // read once, the adjusted logits written once.
-__global__ __launch_bounds__(kLgThreads) void k_logits_adjust(LogitArgs a)
+template <int T, int U>
+__global__ __launch_bounds__(T) void k_logits_adjust(LogitArgs a)
 {
-    __shared__ LogitBest best_s[kLgThreads / kWave];
+    __shared__ LogitBest best_s[T / kWave];
     const int b = blockIdx.y, tid = threadIdx.x, V = a.V;
     const int groups = (V + 3) / 4;
     const int per = (groups + a.slices - 1) / a.slices;
@@ -109,17 +110,17 @@ __global__ __launch_bounds__(kLgThreads) void k_logits_adjust(LogitArgs a)
         return y;
     };
 
-    for (int base = i0 + tid; base < i1; base += kLgThreads * kLgU)
+    for (int base = i0 + tid; base < i1; base += T * U)
     {
-        f32x4u xv[kLgU], bv[kLgU];
-        i32x4u cv[kLgU];
-        uint32_t word[kLgU];
+        f32x4u xv[U], bv[U];
+        i32x4u cv[U];
+        uint32_t word[U];
 #pragma unroll
-        for (int u = 0; u < kLgU; ++u)
+        for (int u = 0; u < U; ++u)
         {
-            const int v = 4 * (base + u * kLgThreads);
+            const int v = 4 * (base + u * T);
             xv[u] = f32x4u(0.0f), bv[u] = f32x4u(0.0f), cv[u] = i32x4u(0), word[u] = 0xFFFFFFFFu;
-            if (base + u * kLgThreads >= i1) continue;
+            if (base + u * T >= i1) continue;
             if (v + 4 <= V)
             {
                 xv[u] = *reinterpret_cast<const f32x4u*>(x + v);
@@ -137,17 +138,17 @@ __global__ __launch_bounds__(kLgThreads) void k_logits_adjust(LogitArgs a)
             if (allowed) word[u] = allowed[v >> 5] >> (v & 31);
         }
 #pragma unroll
-        for (int u = 0; u < kLgU; ++u)
+        for (int u = 0; u < U; ++u)
         {
-            const int v = 4 * (base + u * kLgThreads);
-            if (base + u * kLgThreads >= i1) continue;
+            const int v = 4 * (base + u * T);
+            if (base + u * T >= i1) continue;
             f32x4u y;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (v + e < V) y[e] = one(xv[u][e], cv[u][e], bv[u][e], (word[u] >> e) & 1u, v + e);
             if (out)
             {
-                if (v + 4 <= V) *reinterpret_cast<f32x4u*>(out + v) = y;
+                if (v + 4 <= V) __builtin_nontemporal_store(y, reinterpret_cast<f32x4u*>(out + v));
                 else
                     for (int e = 0; e < 4; ++e)
                         if (v + e < V) out[v + e] = y[e];
@@ -159,7 +160,7 @@ __global__ __launch_bounds__(kLgThreads) void k_logits_adjust(LogitArgs a)
     if ((tid & 63) == 0) best_s[tid >> 6] = best;
     __syncthreads();
     if (tid >= kWave) return;
-    best = tid < kLgThreads / kWave ? best_s[tid] : LogitBest{-__builtin_inff(), -1, 0xFFFFFFFFu, 0u};
+    best = tid < T / kWave ? best_s[tid] : LogitBest{-__builtin_inff(), -1, 0xFFFFFFFFu, 0u};
     best = wave_best(best);
     if (tid != 0) return;
     if (a.slices == 1) choose(a, b, best);
@@ -187,13 +188,19 @@ __global__ __launch_bounds__(256) void k_token_counts(const int32_t* ids, int M,
 
 }  // namespace
 
+// Rows of up to 16384 logits: one work-group of 1024 threads with 4 groups of 4 logits each on their way,
+// so that a row is one round trip and one launch (10000 logits with every rule: 6.4 us a call, 7.8 with the
+// kernel of long rows). Longer ones: slices of 4096 or more, up to 16 work-groups of 512 threads to a CU
+// (256 rows of 131071: 4 to a CU 91.9 us, 8 86.7, 16 83.1; 1024 threads and 4 groups, one to a CU, 94), and a
+// second launch that joins them.
+constexpr size_t kLgRow = 16384;
+constexpr size_t kLgPerCu = 16;
+
 size_t logits_slices(size_t V, size_t B, size_t num_cus)
 {
-    // a work-group's threads have kLgU groups each in flight: a shorter slice leaves threads without work
-    const size_t most = ceil_div(V, (size_t)4 * kLgU * kLgThreads);
-    size_t s = 1;
-    while (s < most && s < kLgSlices && B * s < 2 * num_cus) ++s;
-    return s;
+    if (V <= kLgRow) return 1;
+    const size_t most = std::min<size_t>(kLgSlices, V / 4096);
+    return std::max<size_t>(1, std::min(most, kLgPerCu * num_cus / B));
 }
 
 size_t logits_workspace_bytes(size_t V, size_t B, size_t num_cus)
@@ -207,7 +214,8 @@ hipError_t launch_logits_adjust(hipStream_t st, const float* logits, size_t V, s
 {
     const size_t s = logits_slices(V, B, num_cus);
     LogitArgs a{logits, rules, out, ids, pos, static_cast<LogitBest*>(ws), (int)V, (int)s};
-    k_logits_adjust<<<dim3((unsigned)s, (unsigned)B), kLgThreads, 0, st>>>(a);
+    if (V <= kLgRow) k_logits_adjust<1024, 4><<<dim3((unsigned)s, (unsigned)B), 1024, 0, st>>>(a);
+    else k_logits_adjust<512, 2><<<dim3((unsigned)s, (unsigned)B), 512, 0, st>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || s == 1 || !ids) return e;
     k_logits_choose<<<dim3((unsigned)B), kWave, 0, st>>>(a);

@@ -29,10 +29,7 @@ constexpr int kPgU = 4;          // rows of a group of 16 lanes in flight togeth
 constexpr int kPgTile = 16;      // rows of a wave's tile: 4 groups x kPgU
 constexpr int kPgMaxR = 8;       // query heads of a work-group
 constexpr int kPgRec = 16;       // tail of a record: maximum[8], sum[8]
-#ifndef NNHIP_PG_MIN_CHUNK
-#define NNHIP_PG_MIN_CHUNK 128
-#endif
-constexpr int kPgMinChunk = NNHIP_PG_MIN_CHUNK;  // positions of a work-group at least (a multiple of 64)
+constexpr int kPgMinChunk = 128;  // positions of a work-group at least (a multiple of 64)
 constexpr int kPgEvenB = 1024;   // sequences up to which the chunks are sized by the lengths
 constexpr float kPgLazy = 8.0f;  // log2 growth of a maximum before its sums are rescaled
 
@@ -378,7 +375,7 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
 #pragma unroll
     for (int i = 0; i < NV; ++i) slope2[i] = a.slopes && hs + i < R ? a.slopes[h0 + hs + i] * 1.44269504f : 0.0f;
     auto shape = [&](float dot, int i, int t) {
-        float x = a.cap2 > 0.0f ? a.cap2 * shape_tanh(dot * a.capi) : dot * a.scale2;
+        float x = a.cap2 > 0.0f ? a.cap2 * tanh_any(dot * a.capi) : dot * a.scale2;
         if (a.slopes) x = __builtin_fmaf(slope2[i], (float)(t - p), x);
         return x;
     };
@@ -680,7 +677,7 @@ hipError_t launch_pages_dk(hipStream_t st, const PagesArgs& a)
 
 // ------------------------------------------------------------------ fill from packed prompts
 
-constexpr int kPfTok = 32;  // tokens of a work-group
+constexpr int kPfTok = 64;  // tokens of a work-group (16 x 1111 .. 2048 tokens, 5 heads of 128, f16: 46.5 us, 32: 50.4)
 
 struct FillArgs
 {
@@ -696,65 +693,101 @@ struct FillArgs
     int M, B, Hkv, shift, table_stride, num_pages, limit;  // limit: positions from here on are not written
 };
 
-// Work-group = (32 tokens, KV head, keys or values): the head's dk feature rows of those tokens read
-// along tokens, turned through LDS and written as rows of pages, keys rotated at their positions.
-// Where a token goes (its sequence by bisection in cu, its page) is found while its features are on
-// their way. Tokens of no sequence, positions outside the table or the rope tables and pages outside
-// the pool are not written.
+// The sequence of column m0 + lane, or -1:
+// packed_sequence's in two round trips for up to 64 sequences, for the wave at once.
+__device__ __forceinline__ int wave_sequence(const int32_t* cu, int B, int M, int m0, int lane)
+{
+    // the first b with cu[b + 1] > m0, by 64ths
+    int lo = 0, n = B;
+    while (n > 0)
+    {
+        const int step = (n + kWave - 1) / kWave;
+        const int at = lo + min((lane + 1) * step, n) - 1;
+        const unsigned long long above = __builtin_amdgcn_ballot_w64(cu[at + 1] > m0);
+        if (above == 0)
+        {
+            lo += n;
+            break;
+        }
+        const int k = __builtin_ctzll(above) * step;
+        lo += k;
+        if (step == 1) break;
+        n = min(step, n - k);
+    }
+    const int m = m0 + (lane & (kPfTok - 1));
+    if (lo >= B || m >= M) return -1;
+    // the ends of the sequences from there on that lie in the block
+    const int end = lo + 1 + lane <= B ? cu[lo + 1 + lane] : 0x7FFFFFFF;
+    const int ends = __builtin_popcountll(__builtin_amdgcn_ballot_w64(end <= m0 + kPfTok - 1));
+    if (ends == kWave) return packed_sequence(cu, B, m);  // (64 sequences without a token among them)
+    int b = lo;
+    for (int i = 0; i < ends; ++i) b += __builtin_amdgcn_readlane(end, i) <= m ? 1 : 0;
+    return b < B && cu[b] >= 0 && cu[b] <= m && cu[b + 1] > m ? b : -1;
+}
+
+// Work-group = (64 tokens, KV head, keys or values): the head's dk feature rows of those tokens read
+// along tokens, turned through LDS and written as rows of pages, keys rotated at their positions. Bound by
+// HBM; a work-group lives for its chain of round trips, so the features are on their way while the chain
+// sequence -> position -> page and rotation is followed, the same in each wave.
+// Tokens of no sequence, positions outside the table or the rope tables and pages outside the pool are
+// not written.
 template <int DK, typename CT>
 __global__ __launch_bounds__(256) void k_pages_fill(FillArgs a)
 {
     constexpr int HALF = DK / 2, NR = 256 / kPfTok, U = DK / NR;
+    constexpr int J = HALF / 2, NT = 256 / J, N = kPfTok / NT;  // threads of a token, tokens at a time, times
     __shared__ float x_s[DK][kPfTok + 1];
-    __shared__ int row_s[kPfTok], pos_s[kPfTok];
-    const int tid = threadIdx.x, g = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 63, g = blockIdx.y;
     const bool keys = blockIdx.z == 0;
     const int m0 = blockIdx.x * kPfTok;
     const int c = tid % kPfTok, i0 = tid / kPfTok;
     const float* src = (keys ? a.k : a.v) + (size_t)(g * DK + i0) * (size_t)a.M + (size_t)min(m0 + c, a.M - 1);
+    const int b = wave_sequence(a.cu, a.B, a.M, m0, lane);
+    const int at = b < 0 ? -1 : packed_position(a.cu, a.pos0, b, m0 + (lane & (kPfTok - 1)), a.limit);
     float x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) x[u] = src[(size_t)(NR * u) * (size_t)a.M];
-    if (tid < kPfTok)
+    int to = -1;
+    if (at >= 0)
     {
-        const int m = m0 + tid;
-        const int b = m < a.M ? packed_sequence(a.cu, a.B, m) : -1;
-        const int pos = b < 0 ? -1 : packed_position(a.cu, a.pos0, b, m, a.limit);
-        int row = -1;
-        if (pos >= 0)
+        const int id = a.table[(size_t)b * a.table_stride + (at >> a.shift)];
+        if (page_ok(id, a.num_pages)) to = (int)page_row(id, g, at & ((1 << a.shift) - 1), a.Hkv, a.shift);
+    }
+    // a thread stores features (j, j + 1) and (j + dk / 2, j + 1 + dk / 2) of its tokens
+    const int j = 2 * (tid % J), c0 = tid / J;
+    typedef float v2f __attribute__((ext_vector_type(2), aligned(4)));
+    v2f cs[N], sn[N];
+    int row[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+    {
+        row[n] = __shfl(to, c0 + NT * n, kWave);
+        const size_t r = (size_t)max(__shfl(at, c0 + NT * n, kWave), 0) * HALF + (size_t)j;
+        if (keys && a.cosT)
         {
-            const int id = a.table[(size_t)b * a.table_stride + (pos >> a.shift)];
-            if (page_ok(id, a.num_pages)) row = (int)page_row(id, g, pos & ((1 << a.shift) - 1), a.Hkv, a.shift);
+            cs[n] = *reinterpret_cast<const v2f*>(a.cosT + r);
+            sn[n] = *reinterpret_cast<const v2f*>(a.sinT + r);
         }
-        row_s[tid] = row;
-        pos_s[tid] = pos;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) x_s[i0 + NR * u][c] = x[u];
     __syncthreads();
-    // a thread stores features (j, j + 1) and (j + dk / 2, j + 1 + dk / 2) of its tokens
-    constexpr int J = HALF / 2, NT = 256 / J;
-    const int j = 2 * (tid % J), c0 = tid / J;
     typedef CT v2 __attribute__((ext_vector_type(2)));
     CT* const dst = static_cast<CT*>(keys ? a.kc : a.vc);
 #pragma unroll
-    for (int cn = c0; cn < kPfTok; cn += NT)
+    for (int n = 0; n < N; ++n)
     {
-        const int row = row_s[cn];
-        if (row < 0) continue;
+        const int cn = c0 + NT * n;
+        if (row[n] < 0) continue;
         float y[2][2];
 #pragma unroll
         for (int e = 0; e < 2; ++e)
         {
             const float x0 = x_s[j + e][cn], x1 = x_s[j + e + HALF][cn];
             y[0][e] = x0, y[1][e] = x1;
-            if (keys && a.cosT)
-            {
-                const size_t at = (size_t)pos_s[cn] * HALF + (size_t)(j + e);
-                pg_rope(x0, x1, a.cosT[at], a.sinT[at], y[0][e], y[1][e]);
-            }
+            if (keys && a.cosT) pg_rope(x0, x1, cs[n][e], sn[n][e], y[0][e], y[1][e]);
         }
-        CT* o = dst + (size_t)row * DK + j;
+        CT* o = dst + (size_t)row[n] * DK + j;
         *reinterpret_cast<v2*>(o) = v2{(CT)y[0][0], (CT)y[0][1]};
         *reinterpret_cast<v2*>(o + HALF) = v2{(CT)y[1][0], (CT)y[1][1]};
     }
@@ -793,10 +826,10 @@ struct PagesCut
 static PagesCut pages_cut(size_t B, size_t Hkv, size_t R, size_t dk, size_t len_bound, size_t num_cus)
 {
     const size_t HG = Hkv * pages_groups(R, dk);
-#ifndef NNHIP_PG_PER_CU
-#define NNHIP_PG_PER_CU 2
-#endif
-    const size_t want = ceil_div(NNHIP_PG_PER_CU * num_cus, HG);  // chunks that fill the GPU
+    // chunks that fill the GPU: two work-groups to a CU, and not one more, which a CU would take as a third (4
+    // sequences of 128 K over 8 KV heads: 512 work-groups 234 us, 528 269, 768 241, 256 302; 1 x 32768 over 5
+    // heads 23.4, 25.2 with 768)
+    const size_t want = 2 * num_cus / HG;
     if (len_bound <= kPgMinChunk) return {kPgMinChunk, 1, 0};
     if (B <= kPgEvenB && B * len_bound < (size_t(1) << 31)) return {kPgMinChunk, 0, want > 2 * B ? want - B : B};
     size_t chunk = kPgMinChunk;

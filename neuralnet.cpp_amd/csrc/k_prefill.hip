@@ -469,7 +469,7 @@ __device__ void attend_f32(const PrefillArgs& a, const PrefillWave& w, const Pre
             float x = s[v] * a.scale;
             if constexpr (kShaped)
             {
-                if (a.cap2 > 0.0f) x = a.cap2 * 0.69314718f * shape_tanh(x * (a.capi2 * 1.44269504f));
+                if (a.cap2 > 0.0f) x = a.cap2 * 0.69314718f * tanh_any(x * (a.capi2 * 1.44269504f));
                 if (a.slopes) x += a.slopes[w.head] * (float)(key - w.qpos);
             }
             sc[v] = key <= seq.sight(w) ? x : -__builtin_inff();
@@ -558,7 +558,9 @@ __device__ __forceinline__ bool find_place(const PrefillArgs& a, int block, int 
     const int groups = kPaged ? a.groups : 1;
     const int per_qb = a.B * a.Hkv * groups;
     const int qb = a.nqb - 1 - block / per_qb;
-    const int bg = block % per_qb;
+    // (paged: a step further per block of queries, or a long sequence's work-groups, per_qb apart, would all
+    // fall on one or two of the 8 XCDs)
+    const int bg = kPaged ? (block + block / per_qb) % per_qb : block % per_qb;
     w.b = bg / (a.Hkv * groups);
     w.g = bg / groups % a.Hkv;
     w.head = (w.g * groups + bg % groups) * a.R + wave % a.R;
@@ -583,7 +585,7 @@ __device__ __forceinline__ bool find_place(const PrefillArgs& a, int block, int 
 template <int DK>
 __device__ void store_nan(const PrefillArgs& a, int block, int tid)
 {
-    const int per_qb = a.B * a.Hkv * a.groups, bg = block % per_qb, b = bg / (a.Hkv * a.groups);
+    const int per_qb = a.B * a.Hkv * a.groups, bg = (block + block / per_qb) % per_qb, b = bg / (a.Hkv * a.groups);
     const int first = (bg / a.groups % a.Hkv * a.groups + bg % a.groups) * a.R;
     const int col0 = a.cu[b], pos0 = a.starts ? a.starts[b] : 0;
     const int64_t n = (int64_t)a.cu[b + 1] - col0;
@@ -992,13 +994,31 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
             {
                 const float slope2 = a.slopes ? a.slopes[w.head] * 1.44269504f : 0.0f;
                 const float away = (float)(kb * kPK + 4 * h - w.qpos);
+                // scores rarely reach the cap: the polynomial alone where none does (16 exponentials and
+                // reciprocals less)
+                const float g = a.cap2 > 0.0f ? f * a.capi2 : f;
+                bool far = false;
 #pragma unroll
                 for (int v = 0; v < 16; ++v)
                 {
-                    float x = s[v] * f;
-                    if (a.cap2 > 0.0f) x = a.cap2 * shape_tanh(x * a.capi2);
-                    s[v] = __builtin_fmaf(slope2, away + (float)(8 * (v >> 2) + (v & 3)), x);
+                    s[v] *= g;
+                    far |= !(fabsf(s[v]) <= 1.0f);
                 }
+                if (a.cap2 > 0.0f)
+                {
+                    if (__builtin_amdgcn_ballot_w64(far) == 0)
+                    {
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) s[v] = a.cap2 * tanh_below1(s[v]);
+                    }
+                    else
+                    {
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) s[v] = a.cap2 * tanh_any(s[v]);
+                    }
+                }
+#pragma unroll
+                for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(slope2, away + (float)(8 * (v >> 2) + (v & 3)), s[v]);
                 f = 1.0f;
             }
             if (kb * kPK + kPK - 1 > seq.from(a, w))
