@@ -67,7 +67,7 @@ __device__ __forceinline__ void choose(const LogitArgs& a, int b, const LogitBes
 {
     const int id = best.first == 0xFFFFFFFFu ? -1 : (best.first & 1u) ? (int)(best.first >> 1) : best.i;
     a.ids[b] = id;
-    if (id < 0) return;
+    if (id < 0 || (a.pos && a.pos[b] < 0)) return;
     if (a.r.count_choice && a.r.counts) a.r.counts[(size_t)b * a.V + id] += 1;
     if (a.pos) a.pos[b] += 1;
 }

@@ -20,6 +20,12 @@ columns: the GEMM path, nnhip_kv_cache_fill and the causal nnhip_attention_prefi
 token the result of its own step() (the reference fills the cache with one forward_step per
 context token, compute_layer_gpt.hpp:774-794), and the logits and greedy ids of each sequence's
 last token.
+
+With paged caches (Decoder(caches=[KVPages, ...]), one per block, which may share a page table) the
+sequences of a batch start, end and grow apart: Decoder.prefill_packed takes prompts of unlike lengths
+packed one behind another (nnhip_kv_pages_fill, nnhip_attention_pages_prefill), and step() runs
+nnhip_attention_pages_decode, for which a position below 0 marks an empty slot. The choice of the next
+token can go through rules (step(rules=LogitRules), nnhip_logits_adjust_rows).
 """
 from __future__ import annotations
 
@@ -108,6 +114,7 @@ class Decoder:
             caches = [(torch.zeros((B, cfg.max_len, Hkv * dk), **cdt), torch.zeros((B, cfg.max_len, Hkv * dk), **cdt))
                       for _ in blocks]
         self.caches = caches
+        self.paged = bool(caches) and isinstance(caches[0], _pkg().KVPages)
         if cfg.rope:
             c, s = _pkg().rope_table(dk, cfg.max_len)
             self.cos, self.sin = torch.from_numpy(c).to(dev), torch.from_numpy(s).to(dev)
@@ -195,7 +202,23 @@ class Decoder:
         block's q / k / v / attention output / block output (tests). Returns (logits (vocab, B), greedy
         ids (B,)) of each sequence's last token."""
         cfg, ctx, B = self.cfg, self.ctx, self.B
+        if self.paged:
+            raise _pkg().NNHipError(1, "paged caches take prompts through prefill_packed")
         M = B * T
+        pf = self._prefill_buffers(M)
+
+        def attend(i):
+            kc, vc = self.caches[i]
+            ctx.kv_cache_fill(pf["k"], pf["v"], B, T, cfg.Hkv, cfg.dk, pos0, kc, vc, self.cos, self.sin)
+            ctx.attention_prefill(pf["q"], kc, vc, B, T, cfg.H, cfg.Hkv, cfg.dk, pos0, cfg.scale, self.cos, self.sin,
+                                  out=pf["a"])
+
+        ctx.copy_columns(self._prefill_blocks(ids, M, attend, hook), T - 1, T, B, out=self.x)
+        return self._prefill_head()
+
+    def _prefill_blocks(self, ids, M: int, attend, hook):
+        """Every block over the M tokens ids; attend(i) turns block i's q, k, v into its attention output."""
+        cfg, ctx = self.cfg, self.ctx
         pf = self._prefill_buffers(M)
         outs = (pf["xi"], pf["s"], pf["rs"])
         x, r = pf["x"], pf["r"]
@@ -216,10 +239,7 @@ class Decoder:
             mm(blk.q, pf["q"])
             mm(blk.k, pf["k"])
             mm(blk.v, pf["v"])
-            kc, vc = self.caches[i]
-            ctx.kv_cache_fill(pf["k"], pf["v"], B, T, cfg.Hkv, cfg.dk, pos0, kc, vc, self.cos, self.sin)
-            ctx.attention_prefill(pf["q"], kc, vc, B, T, cfg.H, cfg.Hkv, cfg.dk, pos0, cfg.scale, self.cos, self.sin,
-                                  out=pf["a"])
+            attend(i)
             if hook is not None:
                 for name in ("q", "k", "v", "a"):
                     hook(i, name, pf[name])
@@ -230,12 +250,38 @@ class Decoder:
                                blk.fc2.tau, blk.fc2.bias, r, cfg.act, out=x, gamma_sub=blk.g_ffn_sub, eps_sub=cfg.eps)
             if hook is not None:
                 hook(i, "x", x)
-        ctx.copy_columns(x, T - 1, T, B, out=self.x)
+        return x
+
+    def _prefill_head(self):
+        """Logits and greedy ids of the last tokens in self.x."""
         self._quant(self.x, self.g_final)
         self._mm(self.head, self._logits_cols)
-        ctx.argmax_cols(self._logits_cols, out=self.ids)
+        self.ctx.argmax_cols(self._logits_cols, out=self.ids)
         self._logits = self._logits_cols
         return self._logits, self.ids
+
+    def prefill_packed(self, ids, cu, t_bound: int, pos0=None, hook=None):
+        """Prompts of unlike lengths into paged caches: ids (M,) int32 holds the tokens of sequence b in
+        ids[cu[b] .. cu[b+1] - 1] (cu (B + 1,) int32 device; every sequence has at least one and at most t_bound), at
+        positions pos0[b] on (pos0 (B,) int32 device, None: 0). Every token gets the result of its own step(). hook
+        as prefill(). Returns (logits (vocab, B), greedy ids (B,)) of each sequence's last token."""
+        import torch
+        cfg, ctx = self.cfg, self.ctx
+        if not self.paged:
+            raise _pkg().NNHipError(1, "prefill_packed needs paged caches")
+        if tuple(cu.shape) != (self.B + 1,):
+            raise _pkg().NNHipError(1, f"cu must have shape ({self.B + 1},)")
+        pf = self._prefill_buffers(ids.shape[0])
+
+        def attend(i):
+            cache = self.caches[i]
+            ctx.kv_pages_fill(cache, pf["k"], pf["v"], cu, pos0=pos0, cos=self.cos, sin=self.sin)
+            ctx.attention_pages_prefill(cache, pf["q"], cu, t_bound, cfg.H, cfg.scale, pos0=pos0, cos=self.cos,
+                                        sin=self.sin, out=pf["a"])
+
+        x = self._prefill_blocks(ids, ids.shape[0], attend, hook)
+        torch.index_select(x, 1, (cu[1:] - 1).long(), out=self.x)
+        return self._prefill_head()
 
     def _mm(self, lin: Linear, out):
         return self.ctx.ternary_matmul(lin.rp, lin.tau, self.xi, self.s, self.rs, lin.N, lin.K, self.B,
@@ -254,6 +300,16 @@ class Decoder:
         if kind in self.prefetch:
             self.ctx.prefetch_next([lin.rp for lin in lins])
 
+    def _attend(self, i: int, q, k, v, pos, len_bound: int, out, tokens: bool = False):
+        """Block i's attention of the step's tokens over its cache."""
+        cfg, cache = self.cfg, self.caches[i]
+        if self.paged:
+            self.ctx.attention_pages_decode(cache, q, k, v, cfg.H, pos, len_bound, cfg.scale, cos=self.cos, sin=self.sin,
+                                            out=out, tokens=tokens)
+        else:
+            self.ctx.attention_decode(q, k, v, cfg.H, cfg.Hkv, cfg.dk, pos, len_bound, cache[0], cache[1], cfg.scale,
+                                      self.cos, self.sin, out=out, tokens=tokens)
+
     def _quant(self, x, gamma):
         outs = (self.xi, self.s, self.rs)
         if gamma is None:
@@ -269,9 +325,7 @@ class Decoder:
                               (blk.k.rp, blk.k.tau, blk.k.bias, blk.k.N, self.k),
                               (blk.v.rp, blk.v.tau, blk.v.bias, blk.v.N, self.v)],
                              self.xi, self.s, self.rs, blk.q.K, self.B)
-        kc, vc = self.caches[i]
-        ctx.attention_decode(self.q, self.k, self.v, cfg.H, cfg.Hkv, cfg.dk, pos, len_bound, kc, vc, cfg.scale,
-                             self.cos, self.sin, out=self.a)
+        self._attend(i, self.q, self.k, self.v, pos, len_bound, self.a)
         if attn_hook is not None:
             attn_hook(i, self.a)
         self._quant(self.a, blk.g_attn_sub)
@@ -362,18 +416,15 @@ class Decoder:
         cfg, blk, ctx, B, d = self.cfg, self.blocks[i], self.ctx, self.B, self.cfg.d
         outs = (self.xi, self.s, self.rs)
         self._qkv(blk, self._tok)
-        kc, vc = self.caches[i]
         o = blk.o
         if self._tok:
-            ctx.attention_decode(self.q_t, self.k_t, self.v_t, cfg.H, cfg.Hkv, cfg.dk, pos, len_bound, kc, vc,
-                                 cfg.scale, self.cos, self.sin, out=self.a_t, tokens=True)
+            self._attend(i, self.q_t, self.k_t, self.v_t, pos, len_bound, self.a_t, tokens=True)
             if attn_hook is not None:
                 attn_hook(i, self.a_t.t())
             self._prefetch("o", o)
             ctx.rmsnorm_quant_i8_tokens(self.a_t, blk.g_attn_sub, cfg.eps, outs=outs)
         else:
-            ctx.attention_decode(self.q, self.k, self.v, cfg.H, cfg.Hkv, cfg.dk, pos, len_bound, kc, vc, cfg.scale,
-                                 self.cos, self.sin, out=self.a)
+            self._attend(i, self.q, self.k, self.v, pos, len_bound, self.a)
             if attn_hook is not None:
                 attn_hook(i, self.a)
             self._prefetch("o", o)
@@ -410,10 +461,12 @@ class Decoder:
             ctx.partial_residual_quant_i8(pf, f2.tau, self.s, self.rs, d, B, self.x, res=self.r, bias=f2.bias,
                                           gamma=g_next, eps=cfg.eps, outs=outs)
 
-    def step(self, ids, pos, len_bound: int, attn_hook=None, advance: bool = False):
+    def step(self, ids, pos, len_bound: int, attn_hook=None, advance: bool = False, rules=None):
         """ids / pos: (B,) int32 device tensors. Returns (logits (vocab, B), greedy ids (B,)).
         advance: the greedy ids are written into ids itself and every pos is advanced by one, so
-        that the next call continues the generation (a captured step then replays as is)."""
+        that the next call continues the generation (a captured step then replays as is); paged
+        caches: a pos below 0 (an empty slot) stays. rules: a LogitRules for the choice (the logits
+        returned are those before it)."""
         ctx = self.ctx
         fused = self.fused_ok()
         if fused and self._tok:
@@ -441,10 +494,18 @@ class Decoder:
             h = self.head
             ctx.ternary_matmul_n([(h.rp, h.tau, h.bias, h.N, self.logits_t)], self.xi, self.s, self.rs, h.K, self.B,
                                  tokens=True)
-            ctx.argmax_rows(self.logits_t, out=out_ids, pos=pos if advance else None)
+            if rules is not None or self.paged:
+                ctx.logits_adjust_rows(self.logits_t, rules, ids=out_ids, pos=pos if advance else None)
+            else:
+                ctx.argmax_rows(self.logits_t, out=out_ids, pos=pos if advance else None)
             self._logits = self.logits_t.t()
             return self._logits, out_ids
         self._mm(self.head, self._logits_cols)
+        if rules is not None or self.paged:
+            rows = self._logits_cols.t().contiguous()
+            ctx.logits_adjust_rows(rows, rules, ids=out_ids, pos=pos if advance else None)
+            self._logits = self._logits_cols
+            return self._logits, out_ids
         ctx.argmax_cols(self._logits_cols, out=out_ids)
         if advance:
             pos.add_(1)
