@@ -219,6 +219,8 @@ struct PrefillArgs
     const float* slopes;
     int table_stride, num_pages, shift, limit;  // limit: positions from here on have no place
     float cap2, capi2;      // softcap * log2(e) and its inverse, 0 without
+    float* part;            // spans: records of the items that several work-groups share
+    int spans;              // work-groups that take spans of all tiles (see PromptPlan); 0: one item each
 };
 
 template <int DK, typename CT>
@@ -372,6 +374,23 @@ __device__ __forceinline__ void store_out(const PrefillArgs& a, const PrefillWav
             a.out[(size_t)(w.head * DK + dim(d, 8 * (v >> 2) + 4 * h + (v & 3))) * (size_t)M + (size_t)m] = y(d, v);
 }
 
+// A record (prompt_record) of the wave's part of an item: y(d, v) as store_out's, the lane's reference maximum and
+// sum. Lanes l and l + 32 hold other dimensions of one query.
+template <int DK, typename D, typename Y>
+__device__ __forceinline__ void store_record(float* rec, int tid, D&& dim, Y&& y, float m, float l)
+{
+    const int h = (tid >> 5) & 1, row = (tid >> 6) * 32 + (tid & 31);
+#pragma unroll
+    for (int d = 0; d < DK / 32; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) rec[(size_t)dim(d, 8 * (v >> 2) + 4 * h + (v & 3)) * (32 * kPWaves) + row] = y(d, v);
+    if (h == 0)
+    {
+        rec[(size_t)DK * (32 * kPWaves) + row] = m;
+        rec[(size_t)(DK + 1) * (32 * kPWaves) + row] = l;
+    }
+}
+
 // Four elements of a cache row as floats
 template <typename CT>
 __device__ __forceinline__ float4 widen4(const CT* p)
@@ -408,7 +427,7 @@ __device__ __forceinline__ size_t paged_row(const PrefillArgs& a, const PrefillW
 // past some query's sight therefore add their values key by key.
 template <int DK, bool kPaged, bool kShaped, typename CT>
 __device__ void attend_f32(const PrefillArgs& a, const PrefillWave& w, const PrefillSeq<kPaged>& seq, int last_key,
-                           __amdgpu_buffer_rsrc_t rk, __amdgpu_buffer_rsrc_t rv, float* ks, int tid)
+                           int k0, int k1, float* rec, __amdgpu_buffer_rsrc_t rk, __amdgpu_buffer_rsrc_t rv, float* ks, int tid)
 {
     constexpr int NC = DK / 8, ND = DK / 32, KROW = PrefillTile<DK, CT>::KROW;
     const int lane = tid & 63, h = lane >> 5, l32 = lane & 31;
@@ -424,7 +443,7 @@ __device__ void attend_f32(const PrefillArgs& a, const PrefillWave& w, const Pre
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = v16f{};
     float m_run = -__builtin_inff(), l_run = 0.0f;
-    for (int kb = 0; kb <= last_key / kPK; ++kb)
+    for (int kb = kPaged ? k0 : 0; kb < (kPaged ? k1 : last_key / kPK + 1); ++kb)
     {
         __syncthreads();  // every wave is done with the previous tile
         for (int u = tid; u < kPK * DK / 4; u += kPThreads)
@@ -541,62 +560,218 @@ __device__ void attend_f32(const PrefillArgs& a, const PrefillWave& w, const Pre
         // nothing visible above -infinity: 0; a page outside the pool: NaN
         bad = __syncthreads_or(bad) != 0;
         if (bad) l_run = __builtin_nanf("");
-        else if (l_run == 0.0f) l_run = 1.0f;
+        if (rec)
+        {
+            // the reference in log2 units, as records hold it, and what its rounding left out as a factor
+            const float m2 = m_run * 1.44269504f;
+            const float left = __builtin_fmaf(m_run, 1.44269504f, -m2) + m_run * 1.92596299e-8f;
+            const float f = m_run == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(left);
+            store_record<DK>(rec, tid, [](int d, int r) { return 32 * d + r; }, [&](int d, int v) { return o[d][v] * f; }, m2, l_run * f);
+            return;
+        }
+        if (l_run == 0.0f) l_run = 1.0f;
     }
     if (w.live)
         store_out<DK>(a, w, seq, h, [](int d, int r) { return 32 * d + r; }, [&](int d, int v) { return o[d][v] / l_run; });
 }
 
-// The place of thread tid of work-group `block`, and the last key that the work-group sees; false if it
-// has nothing to do (paged: or its sequence does not fit, see store_nan). Heaviest items first: the last
-// queries attend over the most keys.
+// What a work-group works on: a block of qn = 32 (8 / R) queries of R heads (from `first`, of KV head g) of
+// sequence b. Paged: with the sequence.
+struct PrefillItem
+{
+    int b, g, first, qb;
+    PrefillSeq<true> seq;
+};
+
+// The place of thread tid in an item, and the last key that the item sees
 template <bool kPaged>
-__device__ __forceinline__ bool find_place(const PrefillArgs& a, int block, int tid, PrefillWave& w, PrefillSeq<kPaged>& seq,
-                                           int& last_key)
+__device__ __forceinline__ void seat(const PrefillArgs& a, const PrefillItem& it, int tid, PrefillWave& w,
+                                     PrefillSeq<kPaged>& seq, int& last_key)
 {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int groups = kPaged ? a.groups : 1;
-    const int per_qb = a.B * a.Hkv * groups;
-    const int qb = a.nqb - 1 - block / per_qb;
-    // (paged: a step further per block of queries, or a long sequence's work-groups, per_qb apart, would all
-    // fall on one or two of the 8 XCDs)
-    const int bg = kPaged ? (block + block / per_qb) % per_qb : block % per_qb;
-    w.b = bg / (a.Hkv * groups);
-    w.g = bg / groups % a.Hkv;
-    w.head = (w.g * groups + bg % groups) * a.R + wave % a.R;
     const int qn = kPQ * (kPWaves / a.R);  // queries of the work-group
-    w.t0 = qb * qn + wave / a.R * kPQ;
+    w.b = it.b;
+    w.g = it.g;
+    w.head = it.first + wave % a.R;
+    w.t0 = it.qb * qn + wave / a.R * kPQ;
     w.qt = w.t0 + (tid & 31);
-    if constexpr (kPaged)
-    {
-        const int col0 = a.cu[w.b], pos0 = a.starts ? a.starts[w.b] : 0;
-        const int64_t n = (int64_t)a.cu[w.b + 1] - col0;
-        if (col0 < 0 || col0 + n > a.M || n > a.T || pos0 < 0 || pos0 >= a.limit || n > a.limit - pos0 || qb * qn >= n) return false;
-        seq = {(int)n, col0, pos0, a.prefix ? max(0, min(a.prefix[w.b], pos0 + (int)n)) : 0};
-    }
+    if constexpr (kPaged) seq = it.seq;
     w.qpos = seq.pos0(a) + w.qt;
     w.live = w.t0 < seq.n(a);
-    last_key = seq.pos0(a) + min(qb * qn + qn, seq.n(a)) - 1;
+    last_key = seq.pos0(a) + min(it.qb * qn + qn, seq.n(a)) - 1;
     if constexpr (kPaged) last_key = max(last_key, seq.pre - 1);
+}
+
+// ---- paged: packed sequences
+
+// Sequence b as its arguments say; false if it does not fit them (it gets NaN)
+__device__ __forceinline__ bool packed_seq(const PrefillArgs& a, int b, PrefillSeq<true>& seq)
+{
+    const int col0 = a.cu[b], pos0 = a.starts ? a.starts[b] : 0;
+    const int64_t n = (int64_t)a.cu[b + 1] - col0;
+    if (col0 < 0 || col0 + n > a.M || n > a.T || pos0 < 0 || pos0 >= a.limit || n > a.limit - pos0) return false;
+    seq = {(int)n, col0, pos0, a.prefix ? max(0, min(a.prefix[b], pos0 + (int)n)) : 0};
     return true;
 }
 
-// A packed sequence that does not fit its bounds: NaN in the columns that are there
+// NaN in the columns that are there of the heads from `first` on, by thread `at` of `step`
 template <int DK>
-__device__ void store_nan(const PrefillArgs& a, int block, int tid)
+__device__ void store_nan(const PrefillArgs& a, int b, int first, int heads, int at, int step)
 {
-    const int per_qb = a.B * a.Hkv * a.groups, bg = (block + block / per_qb) % per_qb, b = bg / (a.Hkv * a.groups);
-    const int first = (bg / a.groups % a.Hkv * a.groups + bg % a.groups) * a.R;
-    const int col0 = a.cu[b], pos0 = a.starts ? a.starts[b] : 0;
-    const int64_t n = (int64_t)a.cu[b + 1] - col0;
-    if (col0 >= 0 && col0 + n <= a.M && n <= a.T && pos0 >= 0 && pos0 < a.limit && n <= a.limit - pos0) return;
-    const int64_t c1 = min(col0 + n, (int64_t)a.M);
-    for (int64_t c = max(col0, 0) + (int64_t)(a.nqb - 1 - block / per_qb) * kPThreads + tid; c < c1; c += (int64_t)a.nqb * kPThreads)
-        for (int i = 0; i < a.R * DK; ++i) a.out[(size_t)(first * DK + i) * (size_t)a.M + (size_t)c] = __builtin_nanf("");
+    const int64_t c1 = min((int64_t)a.cu[b + 1], (int64_t)a.M);
+    for (int64_t c = (int64_t)max(a.cu[b], 0) + at; c < c1; c += step)
+        for (int i = 0; i < heads * DK; ++i) a.out[(size_t)(first * DK + i) * (size_t)a.M + (size_t)c] = __builtin_nanf("");
 }
 
+// Work of the whole call in tiles of 32 keys, for work-groups that take equal spans of it: blocks of queries
+// differ in their keys by any factor, and a chunk of a long prompt has fewer of them than the GPU has CUs
+// (4 x 1024 queries of 20 heads: 270 for 256 CUs, the last 14 of which took as long as all others). The order
+// is (head group, sequence, block of queries, tile); an item counts kOver tiles more than it has, which
+// its queries and outputs cost. A cut within the first or last kSnap tiles of an item moves to its edge, and
+// where no item has more than kShort tiles, to its start. Every work-group finds the cuts for itself.
+struct PromptPlan
+{
+    int64_t per, head, total;  // tiles of a span, of a head group, of all
+    int snap;
+};
+struct PromptCut
+{
+    int gh, b, qb, t;
+};
+constexpr int kOver = 3, kSnap = 4, kShort = 16, kSpanMin = 8;
+
+__device__ __forceinline__ int prompt_blocks(const PrefillArgs& a, int n)
+{
+    const int qn = kPQ * (kPWaves / a.R);
+    return (n + qn - 1) / qn;
+}
+
+// Tiles of block qb
+__device__ __forceinline__ int prompt_tiles(const PrefillArgs& a, const PrefillSeq<true>& q, int qb)
+{
+    const int qn = kPQ * (kPWaves / a.R);
+    return (max(q.pos0_ + min(qb * qn + qn, q.n_), q.pre) + kPK - 1) / kPK;
+}
+
+// Tiles of blocks 0 .. qb - 1 with kOver each: A + j u for block j - 1, but at least P, and the last block's own
+__device__ __forceinline__ int64_t prompt_before(const PrefillArgs& a, const PrefillSeq<true>& q, int qb)
+{
+    const int nq = prompt_blocks(a, q.n_), u = kPWaves / a.R, A = (q.pos0_ + kPK - 1) / kPK, P = (q.pre + kPK - 1) / kPK;
+    const int64_t full = min(qb, nq - 1);
+    const int64_t k = max((int64_t)0, min(full, (int64_t)((P - A + u - 1) / u - 1)));
+    int64_t f = k * P + (full - k) * A + u * (full * (full + 1) / 2 - k * (k + 1) / 2) + kOver * full;
+    if (qb == nq && nq > 0) f += prompt_tiles(a, q, nq - 1) + kOver;
+    return f;
+}
+
+// Work of sequence b (0 past the last, or if it does not fit)
+__device__ __forceinline__ int64_t prompt_work(const PrefillArgs& a, int b, int& most)
+{
+    PrefillSeq<true> q;
+    most = 0;
+    if (b >= a.B || !packed_seq(a, b, q) || q.n_ <= 0) return 0;
+    const int nq = prompt_blocks(a, q.n_);
+    most = prompt_tiles(a, q, nq - 1);
+    return prompt_before(a, q, nq);
+}
+
+__device__ __forceinline__ int64_t read_lane64(int64_t x, int l)
+{
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, l);
+    return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)x >> 32), l) << 32) | lo);
+}
+
+__device__ __forceinline__ PromptPlan prompt_plan(const PrefillArgs& a, int spans)
+{
+    const int lane = threadIdx.x & 63;
+    int64_t sum = 0;
+    int most = 0;
+    for (int b = lane; b < a.B; b += kWave)
+    {
+        int m;
+        sum += prompt_work(a, b, m);
+        most = max(most, m);
+    }
+    for (int off = 1; off < min(a.B, kWave); off <<= 1)
+    {
+        sum += __shfl_xor(sum, off, kWave);
+        most = max(most, __shfl_xor(most, off, kWave));
+    }
+    PromptPlan p;
+    p.head = read_lane64(sum, 0);
+    most = __builtin_amdgcn_readfirstlane(most);
+    p.total = p.head * (a.Hkv * a.groups);
+    p.per = (p.total + spans - 1) / spans;
+    p.snap = kSnap;
+    if (most <= kShort) p.snap = 1 << 30;
+    else p.per = max(p.per, (int64_t)max(kSpanMin + kOver, (most + kOver) / 32));  // at most about 32 spans to an item
+    return p;
+}
+
+// Where tile x of the call lies
+__device__ __forceinline__ PromptCut prompt_cut(const PrefillArgs& a, const PromptPlan& p, int64_t x)
+{
+    if (x >= p.total) return {a.Hkv * a.groups, 0, 0, 0};
+    const int lane = threadIdx.x & 63, gh = (int)(x / p.head);
+    int64_t y = x - gh * p.head;
+    for (int b0 = 0; b0 < a.B; b0 += kWave)
+    {
+        int m;
+        const int64_t own = prompt_work(a, b0 + lane, m);
+        int64_t incl = own;
+        const int live = min(a.B - b0, kWave);
+        for (int off = 1; off < live; off <<= 1)
+        {
+            const int64_t t = __shfl_up(incl, off, kWave);
+            if (lane >= off) incl += t;
+        }
+        const unsigned long long here = __builtin_amdgcn_ballot_w64(lane < live && incl > y);
+        if (here == 0)
+        {
+            y -= read_lane64(incl, live - 1);
+            continue;
+        }
+        const int l = __builtin_ctzll(here), b = b0 + l;
+        y -= read_lane64(incl - own, l);
+        PrefillSeq<true> q;
+        packed_seq(a, b, q);
+        int lo = 0, hi = prompt_blocks(a, q.n_) - 1;  // the last block whose tiles begin at or before y
+        while (lo < hi)
+        {
+            const int mid = (lo + hi + 1) >> 1;
+            if (prompt_before(a, q, mid) <= y) lo = mid;
+            else hi = mid - 1;
+        }
+        const int tiles = prompt_tiles(a, q, lo);
+        int t = (int)(y - prompt_before(a, q, lo)) - kOver;
+        if (t < p.snap) t = 0;
+        else if (tiles - t < p.snap) return {gh, b, lo + 1, 0};
+        return {gh, b, lo, t};
+    }
+    return {a.Hkv * a.groups, 0, 0, 0};
+}
+
+__device__ __forceinline__ bool cut_before(const PromptCut& x, const PromptCut& y)
+{
+    if (x.gh != y.gh) return x.gh < y.gh;
+    if (x.b != y.b) return x.b < y.b;
+    return x.qb != y.qb ? x.qb < y.qb : x.t < y.t;
+}
+
+__device__ __forceinline__ bool cut_same_item(const PromptCut& x, const PromptCut& y) { return x.gh == y.gh && x.b == y.b && x.qb == y.qb; }
+
+// Record `slot` of span g: an item's outputs before the division, as [dk][256] by dimension and lane of a work-group's
+// waves, then its reference maxima and its sums [256] each. Slot 0: the span's first item, begun by another
+// span; slot 1: its last, begun here.
+template <int DK>
+__device__ __forceinline__ float* prompt_record(const PrefillArgs& a, int g, int slot)
+{
+    return a.part + ((size_t)g * 2 + slot) * (size_t)((DK + 2) * 32 * kPWaves);
+}
+
+// Attention of an item over its tiles k0 .. k1 - 1; rec: into a record instead of the output
 template <int DK, bool kPaged, bool kShaped, typename CT>
-__global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
+__device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& item, uint8_t* smem, int k0, int k1, float* rec)
 {
     using Tile = PrefillTile<DK, CT>;
     constexpr bool F32C = sizeof(CT) == 4;
@@ -604,25 +779,24 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
     constexpr int ND = DK / 32;  // 32-row blocks of O^T, and dimensions per lane when staging V
     constexpr int CH = DK / 8;   // 16-byte chunks of a K row
     constexpr int KU = CH * kPK / 256;  // chunks a thread stages
-    extern __shared__ __align__(16) uint8_t smem[];
     uint32_t* smax = reinterpret_cast<uint32_t*>(smem + Tile::kMain);  // [2][4]: per tile parity and K wave; f16 caches: [8] per wave
     // set to send the work-group to the f32 products: written in iteration kb (or before the loop) into
     // [(kb + 1) & 1] and read after the barrier of iteration kb + 1, so all waves read the same value
     int* sflag = reinterpret_cast<int*>(smem + Tile::kMain + 32);
 
-    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
+    // (paged: opaque per item, so that no thread-index arithmetic stays alive across the items)
+    int tid = threadIdx.x;
+    if constexpr (kPaged) asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, h = lane >> 5, l32 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     PrefillWave w;
     PrefillSeq<kPaged> seq;
     int last_key;
-    if (!find_place(a, (int)blockIdx.x, tid, w, seq, last_key))
-    {
-        if constexpr (kPaged) store_nan<DK>(a, (int)blockIdx.x, tid);
-        return;
-    }
+    seat(a, item, tid, w, seq, last_key);
     const int row = a.Hkv * DK;
     const int valid = seq.pos0(a) + seq.n(a);  // cache rows [0, valid) hold keys / values
-    const int nkb = last_key / kPK + 1;
+    const int nkb = kPaged ? k1 : last_key / kPK + 1;
+    const int kb0 = kPaged ? k0 : 0;
     const size_t seq_off = kPaged ? 0 : (size_t)w.b * (size_t)a.max_len * (size_t)row;
     // rows at or past `valid` read as zeros: their scores are masked and their zero values keep
     // 0 * v finite
@@ -630,7 +804,7 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
     const __amdgpu_buffer_rsrc_t rk = pf_rsrc(static_cast<const CT*>(a.kc) + seq_off, seq_bytes);
     const __amdgpu_buffer_rsrc_t rv = pf_rsrc(static_cast<const CT*>(a.vc) + seq_off, seq_bytes);
 
-    if (tid < 2) sflag[tid] = tid == 0 ? a.f32 : 0;
+    if (tid < 2) sflag[tid] = tid == (kb0 & 1) ? a.f32 : 0;
     __syncthreads();
 
     // ---- staging, 16 elements per thread: waves 0-3 take V (thread = 4 keys x ND dimensions), waves
@@ -885,8 +1059,8 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
         }
     };
 
-    load_ids(0);
-    load_raw(0);
+    load_ids(kb0);
+    load_raw(kb0);
 
     // ---- the lane's rotated query in halves: step c holds dimensions 16c + 8h + 0..7, scaled by 2^eq
     v8h qh[NC], ql[NC];
@@ -903,7 +1077,7 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
         mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32, kWave));
         int eq = f16_exp(mx);
         const bool far = abs(eq) > kPExpMax;
-        if (__builtin_amdgcn_ballot_w64(far) != 0 && lane == 0) sflag[0] = 1;
+        if (__builtin_amdgcn_ballot_w64(far) != 0 && lane == 0) sflag[kb0 & 1] = 1;
         if (far) eq = 0;
         const float sq = sign * pow2(eq);
         eqf = a.scale2 * pow2(-eq);
@@ -923,8 +1097,8 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
     for (int d = 0; d < ND; ++d) o[d] = v16f{};
     float m_ref = -__builtin_inff(), l_run = 0.0f;  // log2 units; l_run: this lane half's keys
 
-    trim(0);
-    post_max(0);
+    trim(kb0);
+    post_max(kb0);
     if constexpr (!F32C)
     {
         const uint32_t mx = wave_max(__builtin_bit_cast(uint32_t, eqf));  // not negative
@@ -938,15 +1112,15 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
         for (int i = 0; i < kPWaves; ++i) mx = max(mx, smax[i]);
         klim = kPReach / (DK * 0x1p15f) / __builtin_bit_cast(float, mx);  // |q| 2^eq is at most 2^15
     }
-    convert(0, sflag);
-    if (nkb > 1)
+    convert(kb0, sflag + (kb0 & 1));
+    if (kb0 + 1 < nkb)
     {
-        load_raw(1);
-        trim(1);
-        post_max(1);
+        load_raw(kb0 + 1);
+        trim(kb0 + 1);
+        post_max(kb0 + 1);
     }
     bool fallback = false;
-    for (int kb = 0; kb < nkb; ++kb)
+    for (int kb = kb0; kb < nkb; ++kb)
     {
         __syncthreads();  // tile kb is in LDS, the maxima of tile kb + 1 too; buffer (kb + 1) & 1 is free
         if (sflag[kb & 1])
@@ -1036,7 +1210,8 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
             if (__builtin_amdgcn_ballot_w64(grown) != 0)
             {
                 const float m_new = grown ? mx : m_ref;
-                const float corr = __builtin_amdgcn_exp2f(m_ref - m_new);  // 0 on the first tile
+                // 0 on the first tile (a query may have seen no key yet where a span begins within its item)
+                const float corr = kPaged && !grown ? 1.0f : __builtin_amdgcn_exp2f(m_ref - m_new);
                 l_run *= corr;
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
@@ -1044,12 +1219,13 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
                     for (int v = 0; v < 16; ++v) o[d][v] *= corr;
                 m_ref = m_new;
             }
+            const float ref = kPaged && m_ref == -__builtin_inff() ? 0.0f : m_ref;
             v8b p[3][2];
 #pragma unroll
             for (int v = 0; v < 16; v += 2)
             {
-                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], f, -m_ref));
-                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v + 1], f, -m_ref));
+                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], f, -ref));
+                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v + 1], f, -ref));
                 l_run += p0;
                 l_run += p1;
                 v2b x[3];
@@ -1103,22 +1279,26 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
         }
     if (__syncthreads_or(!fallback && w.live && lost) || fallback)
     {
-        if constexpr (kPaged)
-        {
-            // everything from scratch: kept alive across the loop above, it would push that into spills
-            int t2 = threadIdx.x, block = blockIdx.x;
-            asm volatile("" : "+v"(t2), "+s"(block));
-            PrefillWave w2;
-            PrefillSeq<true> seq2;
-            int last2;
-            find_place(a, block, t2, w2, seq2, last2);
-            attend_f32<DK, kPaged, kShaped, CT>(a, w2, seq2, last2, rk, rv, reinterpret_cast<float*>(smem), t2);
-        }
-        else attend_f32<DK, kPaged, kShaped, CT>(a, w, seq, last_key, rk, rv, reinterpret_cast<float*>(smem), tid);
+        // everything from scratch: kept alive across the loop above, it would push that into spills
+        int t2 = threadIdx.x;
+        if constexpr (kPaged) asm volatile("" : "+v"(t2));
+        PrefillWave w2;
+        PrefillSeq<kPaged> seq2;
+        int last2;
+        if constexpr (kPaged) seat(a, item, t2, w2, seq2, last2);
+        else w2 = w, seq2 = seq, last2 = last_key;
+        attend_f32<DK, kPaged, kShaped, CT>(a, w2, seq2, last2, k0, k1, rec, rk, rv, reinterpret_cast<float*>(smem), kPaged ? t2 : tid);
         return;
     }
     if constexpr (kPaged)
+    {
         if (__syncthreads_or(bad)) l_run = __builtin_nanf("");
+        if (rec)
+        {
+            store_record<DK>(rec, tid, [](int d, int i) { return ND * i + d; }, [&](int d, int v) { return o[d][v]; }, m_ref, l_run);
+            return;
+        }
+    }
     if (!w.live) return;
     // o / l, correctly rounded but for the last step's double rounding: the residual is exact
     const float r = 1.0f / l_run;
@@ -1126,6 +1306,119 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
         const float q = o[d][v] * r;
         return __builtin_fmaf(__builtin_fmaf(-q, l_run, o[d][v]), r, q);
     });
+}
+
+template <int DK, bool kPaged, bool kShaped, typename CT>
+__global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
+{
+    extern __shared__ __align__(16) uint8_t smem[];
+    PrefillItem it;
+    const int groups = kPaged ? a.groups : 1, HG = a.Hkv * groups;
+    // one item each, heaviest first: the last queries attend over the most keys. (Paged: a step further per block
+    // of queries, or a long sequence's work-groups, per_qb apart, would all fall on one or two of the 8 XCDs.)
+    const int per_qb = a.B * HG, back = (int)blockIdx.x / per_qb;
+    const int bg = kPaged ? ((int)blockIdx.x + back) % per_qb : (int)blockIdx.x % per_qb;
+    if constexpr (!kPaged)
+    {
+        it.b = bg / a.Hkv;
+        it.g = bg % a.Hkv;
+        it.first = it.g * a.R;
+        it.qb = a.nqb - 1 - back;
+        attend<DK, kPaged, kShaped, CT>(a, it, smem, 0, 0, nullptr);
+    }
+    else
+    {
+        const int g = blockIdx.x;
+        PromptCut at, end;
+        if (a.spans)
+        {
+            for (int b = g; b < a.B; b += gridDim.x)
+                if (!packed_seq(a, b, it.seq)) store_nan<DK>(a, b, 0, a.H, threadIdx.x, kPThreads);
+            const PromptPlan plan = prompt_plan(a, gridDim.x);
+            at = prompt_cut(a, plan, g * plan.per);
+            end = prompt_cut(a, plan, (g + 1) * plan.per);
+        }
+        else
+        {
+            at = {bg % HG, bg / HG, a.nqb - 1 - back, 0};
+            if (!packed_seq(a, at.b, it.seq))
+            {
+                store_nan<DK>(a, at.b, at.gh * a.R, a.R, at.qb * kPThreads + (int)threadIdx.x, a.nqb * kPThreads);
+                return;
+            }
+            if (at.qb >= prompt_blocks(a, it.seq.n_)) return;
+            end = {at.gh, at.b, at.qb + 1, 0};
+        }
+        while (cut_before(at, end))
+        {
+            // the next sequence with a block left
+            const bool there = at.b < a.B;
+            if (!there || !packed_seq(a, at.b, it.seq) || at.qb >= prompt_blocks(a, it.seq.n_))
+            {
+                at = there ? PromptCut{at.gh, at.b + 1, 0, 0} : PromptCut{at.gh + 1, 0, 0, 0};
+                continue;
+            }
+            const int tiles = prompt_tiles(a, it.seq, at.qb), to = cut_same_item(at, end) ? end.t : tiles;
+            it.b = at.b;
+            it.g = at.gh / groups;
+            it.first = at.gh * a.R;
+            it.qb = at.qb;
+            float* rec = at.t == 0 && to == tiles ? nullptr : prompt_record<DK>(a, g, at.t > 0 ? 0 : 1);
+            attend<DK, kPaged, kShaped, CT>(a, it, smem, at.t, to, rec);
+            at = {at.gh, at.b, at.qb + 1, 0};
+        }
+    }
+}
+
+// The items that several spans share: work-group g joins the one that the cut before span g is the first to
+// fall into, from its records: sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, 16 dimensions of its 256 queries
+template <int DK>
+__global__ __launch_bounds__(32 * kPWaves) void k_prompt_join(PrefillArgs a, int spans)
+{
+    constexpr int N = 16;
+    const int g = blockIdx.x + 1, d0 = blockIdx.y * N, row = threadIdx.x;
+    const PromptPlan plan = prompt_plan(a, spans);
+    const PromptCut at = prompt_cut(a, plan, g * plan.per);
+    if (at.gh >= a.Hkv * a.groups || at.t == 0) return;
+    const PromptCut last = prompt_cut(a, plan, (g - 1) * plan.per);
+    if (cut_same_item(at, last) && last.t > 0) return;
+    PrefillSeq<true> q;
+    packed_seq(a, at.b, q);
+    // the spans from g on that begin within the item (their cuts are plan.per apart)
+    int64_t until = at.gh * plan.head;
+    for (int b0 = 0; b0 < at.b; b0 += kWave)
+    {
+        int m;
+        int64_t x = b0 + (int)(threadIdx.x & 63) < at.b ? prompt_work(a, b0 + (int)(threadIdx.x & 63), m) : 0;
+        for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off, kWave);
+        until += read_lane64(x, 0);
+    }
+    const int tiles = prompt_tiles(a, q, at.qb);
+    until += prompt_before(a, q, at.qb) + kOver + tiles - plan.snap;  // the last cut that does not move to the item's end
+    const int n = (int)((until - g * plan.per) / plan.per) + 2;       // records: span g - 1's, then those of g ..
+    const int wave = row >> 5, qt = at.qb * kPQ * (kPWaves / a.R) + wave / a.R * kPQ + (row & 31);
+    float top = -__builtin_inff(), den = 0.0f, y[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] = 0.0f;
+    for (int s = 0; s < n; ++s)
+    {
+        const float* rec = prompt_record<DK>(a, g - 1 + s, s == 0 ? 1 : 0) + row;
+        float x[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = rec[(size_t)(d0 + i) * (32 * kPWaves)];
+        const float m = rec[(size_t)DK * (32 * kPWaves)], l = rec[(size_t)(DK + 1) * (32 * kPWaves)];
+        const float to = fmaxf(top, m);
+        const float old = top == to ? 1.0f : __builtin_amdgcn_exp2f(top - to);
+        const float now = m == to ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+        den = __builtin_fmaf(l, now, den * old);
+#pragma unroll
+        for (int i = 0; i < N; ++i) y[i] = __builtin_fmaf(x[i], now, y[i] * old);
+        top = to;
+    }
+    if (qt >= q.n_) return;
+    float* out = a.out + (size_t)((at.gh * a.R + wave % a.R) * DK + d0) * (size_t)a.M + (size_t)(q.col0_ + qt);
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[(size_t)i * (size_t)a.M] = den == 0.0f ? 0.0f : y[i] / den;
 }
 
 template <int DK, bool kPaged, bool kShaped, typename CT>
@@ -1140,8 +1433,15 @@ hipError_t launch_prefill_dk(hipStream_t st, const PrefillArgs& a)
         if (e != hipSuccess) return e;
         attr_set = true;
     }
-    const unsigned blocks = (unsigned)(a.nqb * a.B * a.Hkv * a.groups);
+    const unsigned blocks = kPaged && a.spans ? (unsigned)a.spans : (unsigned)(a.nqb * a.B * a.Hkv * a.groups);
     hipLaunchKernelGGL((k_attn_prefill<DK, kPaged, kShaped, CT>), dim3(blocks), dim3(kPThreads), lds, st, a);
+    if constexpr (kPaged)
+        if (a.spans > 1)
+        {
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+            k_prompt_join<DK><<<dim3((unsigned)a.spans - 1, DK / 16), 32 * kPWaves, 0, st>>>(a, a.spans);
+        }
     return hipGetLastError();
 }
 
@@ -1199,10 +1499,18 @@ hipError_t launch_attn_prefill(hipStream_t st, const float* q, const void* kc, c
     return hipErrorInvalidValue;
 }
 
+// Spans of a call: one work-group to a CU (its registers allow no more), unless no sequence can be long enough to be cut
+size_t pages_prefill_spans(size_t limit, size_t num_cus) { return limit <= (size_t)kShort * kPK ? 0 : num_cus; }
+
+size_t pages_prefill_workspace_bytes(size_t dk, size_t limit, size_t num_cus)
+{
+    return pages_prefill_spans(limit, num_cus) * 2 * (dk + 2) * 32 * kPWaves * sizeof(float);
+}
+
 hipError_t launch_pages_prefill(hipStream_t st, const nnhip_kv_pages& kv, const float* q, size_t M, const int32_t* cu,
                                 const int32_t* pos0, size_t B, size_t t_bound, size_t H, const float* cosT,
                                 const float* sinT, size_t limit, float scale, float softcap, const float* slopes,
-                                const int32_t* prefix, float* out)
+                                const int32_t* prefix, float* out, void* ws, size_t num_cus)
 {
     // a KV head's R query heads in work-groups of 8, 4, 2 or 1
     const size_t heads = H / kv.Hkv, R = heads % 8 == 0 ? 8 : heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
@@ -1212,7 +1520,8 @@ hipError_t launch_pages_prefill(hipStream_t st, const nnhip_kv_pages& kv, const 
     PrefillArgs a{q, kv.k, kv.v, cosT, sinT, out, (int)B, (int)t_bound, (int)H, (int)kv.Hkv, (int)R, 0,
                   (int)limit, (int)ceil_div(t_bound, kPQ * (kPWaves / R)), scale, (float)(mag * 1.4426950408889634), f32 ? 1 : 0,
                   (int)M, (int)(heads / R), kv.table, cu, pos0, prefix, slopes, (int)kv.table_stride, (int)kv.num_pages,
-                  0, (int)limit, (float)cap2, softcap > 0.0f ? (float)(1.0 / cap2) : 0.0f};
+                  0, (int)limit, (float)cap2, softcap > 0.0f ? (float)(1.0 / cap2) : 0.0f,
+                  static_cast<float*>(ws), (int)pages_prefill_spans(limit, num_cus)};
     while ((size_t(1) << a.shift) < kv.page_size) ++a.shift;
     if (cap2 > 0.0 || slopes)
     {

@@ -2109,7 +2109,7 @@ nnhip_status nnhip_attention_pages_prefill(nnhip_ctx* ctx, const nnhip_kv_pages*
 {
     const char* fn = "nnhip_attention_pages_prefill";
     NNHIP_CHECK_CTX(fn);
-    const nnhip_status st = check_pages(fn, cache, rope_cos, rope_sin);
+    nnhip_status st = check_pages(fn, cache, rope_cos, rope_sin);
     if (st != NNHIP_OK) return st;
     if (!prefill_dk_supported(cache->dk)) return fail(NNHIP_ERR_UNSUPPORTED, fn, "dk must be 64 or 128");
     if (M == 0 || B == 0 || t_bound == 0) return NNHIP_OK;
@@ -2126,8 +2126,11 @@ nnhip_status nnhip_attention_pages_prefill(nnhip_ctx* ctx, const nnhip_kv_pages*
     NNHIP_REQUIRE(!rope_cos || limit * cache->dk < (size_t(1) << 30), fn, "rope tables must be below 2 GiB");
     NNHIP_REQUIRE(mul_ok(B, H) && mul_ok(B * H, ceil_div(t_bound, 32)) && B * H * ceil_div(t_bound, 32) < (size_t(1) << 22), fn,
                   "B * H * ceil(t_bound / 32) must be below 2^22");
+    void* ws = nullptr;
+    st = ensure_stream_ws(ctx, pages_prefill_workspace_bytes(cache->dk, limit, (size_t)ctx->num_cus), fn, &ws);
+    if (st != NNHIP_OK) return st;
     NNHIP_LAUNCH(fn, launch_pages_prefill(ctx->stream, *cache, q, M, cu, pos0, B, t_bound, H, rope_cos, rope_sin, limit,
-                                          scale, softcap, slopes, prefix, out));
+                                          scale, softcap, slopes, prefix, out, ws, (size_t)ctx->num_cus));
     return NNHIP_OK;
 }
 

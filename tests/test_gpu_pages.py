@@ -264,7 +264,7 @@ def test_fill_matches_contiguous_fill(ctx, nnhip):
 # 2^-22 of a term, so its outputs are held to the decode form's bound with 4 u for each u of a product.
 
 def check_prompt(ctx, nnhip, lens, pos0, H, Hkv, dk, page, f16, rope=True, cap=0.0, slopes=False, prefix=None, seed=0,
-                 spread=1.0, t_bound=None, edit=None):
+                 spread=1.0, t_bound=None, edit=None, sample=None):
     print(f"prompt lens={lens} pos0={pos0} H={H} Hkv={Hkv} dk={dk} page={page} f16={f16} cap={cap} slopes={slopes} "
           f"prefix={prefix}", flush=True)
     rng = np.random.default_rng(seed + 7 * dk + H)
@@ -290,7 +290,7 @@ def check_prompt(ctx, nnhip, lens, pos0, H, Hkv, dk, page, f16, rope=True, cap=0
             continue
         K, V = c.rows(b, pos0[b] + n)
         at = np.arange(pos0[b] + n)
-        for t in range(n):
+        for t in range(n) if sample is None else sorted({0, n - 1, *rng.integers(0, n, sample).tolist()}):
             i, m = pos0[b] + t, cu[b] + t
             see = at <= i
             if prefix is not None:
@@ -370,6 +370,151 @@ def check_prompt_nonfinite(ctx, nnhip, lens, f16, cap, edit):
     edit(c, q)
     cu = np.concatenate(([0], np.cumsum(lens))).astype(np.int32)
     return host(ctx.attention_pages_prefill(c.on_device(nnhip), dev(q), dev(cu), max(lens), H, 0.125, softcap=cap)).reshape(H, dk, M)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("H,Hkv,dk", [(4, 1, 128), (8, 1, 64), (2, 2, 64), (12, 1, 128)])
+def test_prompt_shared_items(ctx, nnhip, H, Hkv, dk, f16):
+    """Few queries over long caches: work-groups share the keys of a block of queries and join, at every number of
+    them to a block, beside sequences of one tile and an empty one."""
+    check_prompt(ctx, nnhip, [5, 1, 0, 40, 70], [3000, 1023, 9, 4090, 0], H, Hkv, dk, 64, f16, seed=30, sample=3)
+    check_prompt(ctx, nnhip, [1], [9000], H, Hkv, dk, 64, f16, seed=31)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_prompt_shared_items_shaped(ctx, nnhip, f16):
+    check_prompt(ctx, nnhip, [300, 33, 2], [400, 2000, 5], 4, 2, 64, 16, f16, cap=8.0, slopes=True, prefix=[650, 0, 7], seed=32,
+                 spread=3.0, sample=6)
+    check_prompt(ctx, nnhip, [700], [0], 8, 4, 64, 16, f16, seed=33, prefix=[512], sample=12)
+
+
+def test_prompt_shared_items_many_sequences(ctx, nnhip):
+    """More sequences than a wave has lanes, most of them of a token or none."""
+    rng = np.random.default_rng(34)
+    lens = [int(x) for x in rng.integers(0, 3, 150)]
+    lens[70], lens[149] = 900, 65
+    check_prompt(ctx, nnhip, lens, [int(x) for x in rng.integers(0, 40, 150)], 2, 1, 64, 16, True, seed=34, sample=4)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_prompt_shared_items_nonfinite(ctx, nnhip, f16):
+    """What one work-group of an item meets (a NaN, an infinity, keys of f32 range, a page outside the pool) and
+    the others do not."""
+    rng = np.random.default_rng(35)
+    H, dk, page, n, past = 4, 64, 16, 40, 3000
+    total = past + n
+    q = rng.standard_normal((H * dk, n)).astype(np.float32)
+
+    def run(edit):
+        c = Cache(np.random.default_rng(36), [total], 1, page, dk, f16)
+        edit(c)
+        return host(ctx.attention_pages_prefill(c.on_device(nnhip), dev(q), dev(np.array([0, n], np.int32)), n, H, 0.125,
+                                                pos0=dev(np.array([past], np.int32)))).reshape(H, dk, n)
+
+    def at(c, t):
+        return c.table[0, t // page], t % page
+
+    ref = run(lambda c: None)
+
+    def v_nan(c):
+        i, s = at(c, 1500)
+        c.v[i, 0, s, 5] = np.nan
+
+    def v_late(c):
+        i, s = at(c, past + 20)
+        c.v[i, 0, s, 5] = np.inf
+
+    def k_nan(c):
+        i, s = at(c, past + 20)
+        c.k[i, 0, s, 0] = np.nan
+
+    def bad(c):
+        c.table[0, 1500 // page] = c.k.shape[0]
+
+    got = run(v_nan)
+    assert np.isnan(got[:, 5]).all() and np.isfinite(np.delete(got, 5, 1)).all()
+    got = run(v_late)
+    assert np.isinf(got[:, 5, 20:]).all() and np.isfinite(got[:, 5, :20]).all()
+    got = run(k_nan)
+    assert np.isnan(got[:, :, 20:]).all() and np.isfinite(got[:, :, :20]).all()
+    assert np.isnan(run(bad)).all()
+
+    # keys so large that one work-group takes the f32 products; their scores decide the softmax
+    def large(c):
+        for t in range(1500, 1510):
+            i, s = at(c, t)
+            c.k[i, 0, s] *= 2.0 ** 9
+    c = Cache(np.random.default_rng(36), [total], 1, page, dk, f16)
+    large(c)
+    got = run(large).astype(np.float64)
+    K, V = c.rows(0, total)
+    for t in (0, 17, 39):
+        see = np.arange(total) <= past + t
+        for h in range(H):
+            r, tol = attend64(q.reshape(H, dk, n)[h, :, t].astype(np.float64), K[:, 0], V[:, 0], 0.125, 0.0, 0.0,
+                              np.arange(total) - float(past + t), see)
+            assert np.all(np.abs(got[h, :, t] - r) <= 4 * tol)
+    assert np.isfinite(ref).all()
+
+
+def test_prompt_bad_sequences_in_spans(ctx, nnhip):
+    """As test_prompt_bad_sequences where work-groups share items: room for 3000 positions in the table."""
+    rng = np.random.default_rng(37)
+    H, dk, page, lens = 2, 64, 16, [40, 900, 20]
+    c = Cache(rng, lens, 1, page, dk, False, width=200)
+    M = sum(lens) + 5
+    q = dev(rng.standard_normal((H * dk, M)).astype(np.float32))
+
+    def run(cu, t_bound, pos0=None):
+        return host(ctx.attention_pages_prefill(c.on_device(nnhip), q, dev(np.array(cu, np.int32)), t_bound, H, 0.125,
+                                                pos0=None if pos0 is None else dev(np.array(pos0, np.int32)),
+                                                out=dev(np.full((H * dk, M), 7.0, np.float32))))
+
+    ref = run([0, 40, 940, 960], 900)
+    assert np.isfinite(ref).all() and np.all(ref[:, 960:] == 7.0)
+    got = run([0, 40, 940, 960], 899)
+    assert np.isnan(got[:, 40:940]).all() and np.array_equal(got[:, :40], ref[:, :40]) and np.array_equal(got[:, 940:], ref[:, 940:])
+    got = run([0, 40, 940, 960], 900, [0, 0, 3190])
+    assert np.isnan(got[:, 940:960]).all() and np.array_equal(got[:, :940], ref[:, :940])
+    got = run([0, 0, 0, 0], 900)
+    assert np.all(got == 7.0)
+
+
+def test_prompt_captured_in_spans(nnhip):
+    """A captured prompt call replays with new lengths (the work-groups find their shares on the device)."""
+    import torch
+    ctx = nnhip.Context(0)
+    rng = np.random.default_rng(38)
+    H, dk, page = 4, 64, 16
+    c = Cache(rng, [2000, 2000], 1, page, dk, True)
+    cache = c.on_device(nnhip)
+    q = dev(rng.standard_normal((H * dk, 300)).astype(np.float32))
+    cu, pos0 = dev(np.array([0, 100, 300], np.int32)), dev(np.array([1500, 0], np.int32))
+    out = torch.zeros_like(q)
+    side = torch.cuda.Stream()
+
+    def call():
+        ctx.attention_pages_prefill(cache, q, cu, 300, H, 0.125, pos0=pos0, out=out)
+
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        call()
+    for a, b, p in ((100, 1500, 0), (7, 1993, 1700), (290, 0, 30), (0, 5, 1000)):
+        cu.copy_(torch.tensor([0, a, 300], dtype=torch.int32))
+        pos0.copy_(torch.tensor([b, p], dtype=torch.int32))
+        torch.cuda.synchronize()
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        out.zero_()
+        call()
+        torch.cuda.synchronize()
+        assert torch.equal(got, out) and bool(torch.isfinite(out).all())
+    ctx.close()
 
 
 def test_prompt_bad_sequences(ctx, nnhip):
