@@ -918,15 +918,15 @@ class Context:
         """The device address of t (None: null) after its checks: this context's device, contiguous, type, shape."""
         if t is None:
             return None
-        if t.device != self._device:
+        if t.get_device() == self.device and t.dtype is dtype and t.shape == shape and t.is_contiguous():
+            return t.data_ptr()
+        if t.get_device() != self.device:
             raise NNHipError(1, f"{name} is on {t.device}, the context on {self._device}")
-        if not t.is_contiguous():
-            raise NNHipError(1, f"{name} must be contiguous")
         if t.dtype is not dtype:
             raise NNHipError(1, f"{name} has dtype {t.dtype}, expected {dtype}")
         if t.shape != shape:
             raise NNHipError(1, f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-        return t.data_ptr()
+        raise NNHipError(1, f"{name} must be contiguous")
 
     def _rope(self, cos, sin, dk: int):
         """Addresses and rows of the rope tables (None, None, 0 without)."""

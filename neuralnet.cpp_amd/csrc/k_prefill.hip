@@ -957,8 +957,7 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
     float eqf = 0.0f;  // the lane's query: 2^-eq |scale| log2(e)
     float klim = 0.0f; // f16 caches: the largest key element within kPReach of every query of the work-group
     // K's exponent, then raw as f16 halves (K) and bf16 parts (V) into buffer kb & 1
-    auto convert = [&](int kb, int* flag) {
-        uint8_t* buf = smem + (kb & 1) * Tile::kBuf;
+    auto find_scale = [&](int kb, int* flag) {
         if constexpr (F32C)
         {
             const uint32_t* sm = smax + (kb & 1) * 4;
@@ -979,6 +978,10 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
             const uint16_t top = max(m[0], m[1]);
             if (__builtin_amdgcn_ballot_w64(!((float)__builtin_bit_cast(_Float16, top) <= klim)) != 0 && lane == 0) *flag = 1;
         }
+    };
+    // raw as f16 halves (K, scaled by 2^ek) and bf16 parts (V) into buffer kb & 1
+    auto convert = [&](int kb) {
+        uint8_t* buf = smem + (kb & 1) * Tile::kBuf;
         const float sk = F32C ? pow2(ek) : 1.0f;
         if (is_v)
         {
@@ -1112,7 +1115,8 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
         for (int i = 0; i < kPWaves; ++i) mx = max(mx, smax[i]);
         klim = kPReach / (DK * 0x1p15f) / __builtin_bit_cast(float, mx);  // |q| 2^eq is at most 2^15
     }
-    convert(kb0, sflag + (kb0 & 1));
+    find_scale(kb0, sflag + (kb0 & 1));
+    convert(kb0);
     if (kb0 + 1 < nkb)
     {
         load_raw(kb0 + 1);
@@ -1136,8 +1140,12 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
         __builtin_amdgcn_sched_barrier(0);
         if (kb + 1 < nkb)
         {
-            convert(kb + 1, sflag + ((kb + 1) & 1));
-            if (kb + 2 < nkb) load_raw(kb + 2);  // in flight during this tile's products
+            find_scale(kb + 1, sflag + ((kb + 1) & 1));
+            if (!is_v)
+            {
+                convert(kb + 1);
+                if (kb + 2 < nkb) load_raw(kb + 2);  // in flight during this tile's products
+            }
         }
         if (w.live && kb * kPK <= seq.to(a, w))
         {
@@ -1260,7 +1268,15 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
             }
             o[ND - 1] += sum[(ND - 1) & 1];
         }
-        if (kb + 2 < nkb)
+        // V's waves convert behind their products, K's before them: each SIMD has one of both, whose VALU and MFMA
+        // phases then fall together
+        if (is_v && kb + 1 < nkb)
+        {
+            trim(kb + 1);
+            convert(kb + 1);
+            if (kb + 2 < nkb) load_raw(kb + 2);
+        }
+        if (!is_v && kb + 2 < nkb)
         {
             trim(kb + 2);
             post_max(kb + 2);
