@@ -195,6 +195,8 @@ constexpr float kPLazy = 8.0f;         // log2 growth of a query's maximum befor
 // Largest dk max|q| max|k| |scale| log2(e) of a query and a tile: a score's parts below the halves' range
 // (2^-40 of the largest value) add up to less than 2^-21, and no score rounds a reference maximum by 2^-5.
 constexpr float kPReach = 0x1p18f;
+constexpr float kPUp = 7.0f;           // f16 parts of probabilities: the reference lies 2^7 below the maximum
+constexpr float kPDeep = 14.0f;        // ... and two of them hold what is above 2^-14
 constexpr float kPTiny = 0x1p-100f;    // outputs below this (but for 0) may have lost bits of a bf16 part
 
 struct PrefillArgs
@@ -223,11 +225,12 @@ struct PrefillArgs
     int spans;              // work-groups that take spans of all tiles (see PromptPlan); 0: one item each
 };
 
-template <int DK, typename CT>
+// kHalf: V as it is in f16 caches, for products with probabilities in f16 parts
+template <int DK, typename CT, bool kHalf = false>
 struct PrefillTile
 {
     static constexpr int kKPlanes = sizeof(CT) == 4 ? 2 : 1;  // K: high and low f16 halves of f32 values
-    static constexpr int kVPlanes = sizeof(CT) == 4 ? 3 : 2;  // V: bf16 parts of f32 / f16 values
+    static constexpr int kVPlanes = kHalf ? 1 : sizeof(CT) == 4 ? 3 : 2;  // V: bf16 parts of f32 / f16 values, or f16
     // rows are padded by 16 bytes: 16 lanes' reads of consecutive rows fall on all banks, and every
     // chunk is at a constant offset from a lane's first
     static constexpr int kKPitch = DK * 2 + 16, kVPitch = kPK * 2 + 16;
@@ -250,6 +253,17 @@ __device__ __forceinline__ void split2(float x0, float x1, v2h& hi, v2h& lo)
     asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(l0) : "v"(u), "v"(x0));
     asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(l1) : "v"(u), "v"(x1));
     lo = __builtin_convertvector(v2f{l0, l1}, v2h);
+}
+
+// x = hi + lo / up, up = 2^11: two halves that hold 22 bits of what is from 2^-14 on
+__device__ __forceinline__ void split2_up(float x0, float x1, float up, v2h& hi, v2h& lo)
+{
+    hi = __builtin_convertvector(v2f{x0, x1}, v2h);
+    const uint32_t u = __builtin_bit_cast(uint32_t, hi);
+    float l0, l1;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(l0) : "v"(u), "v"(x0));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(l1) : "v"(u), "v"(x1));
+    lo = __builtin_convertvector(v2f{l0 * up, l1 * up}, v2h);
 }
 
 // The first N bf16 parts of two values: x = sum of parts, exactly, for f32 values (N = 3) and widened f16
@@ -773,8 +787,9 @@ __device__ __forceinline__ float* prompt_record(const PrefillArgs& a, int g, int
 template <int DK, bool kPaged, bool kShaped, typename CT>
 __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& item, uint8_t* smem, int k0, int k1, float* rec)
 {
-    using Tile = PrefillTile<DK, CT>;
     constexpr bool F32C = sizeof(CT) == 4;
+    constexpr bool kHalf = kPaged && !F32C;
+    using Tile = PrefillTile<DK, CT, kHalf>;
     constexpr int NC = DK / 16;  // MFMA steps over the head dimension
     constexpr int ND = DK / 32;  // 32-row blocks of O^T, and dimensions per lane when staging V
     constexpr int CH = DK / 8;   // 16-byte chunks of a K row
@@ -993,6 +1008,15 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
             {
                 const int r = 32 * e + vg;
                 uint8_t* dst = buf + Tile::kV + r * Tile::kVPitch + 32 * s + 16 * hh + 8 * ah;
+                if constexpr (kHalf)
+                {
+                    // the halves of dimension e of the four keys
+                    const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+                    const uint32_t k01 = __builtin_amdgcn_perm(raw[ND / 2 + e / 2], raw[e / 2], sel);
+                    const uint32_t k23 = __builtin_amdgcn_perm(raw[ND / 2 * 3 + e / 2], raw[ND / 2 * 2 + e / 2], sel);
+                    *reinterpret_cast<u32x2*>(dst) = u32x2{k01, k23};
+                    continue;
+                }
                 float x[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -1040,7 +1064,7 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
     // group g of K holds steps GK g .., group g of V^T (block, half) pairs GV g .., each with its planes.
     constexpr int PK = Tile::kKPlanes, PV = Tile::kVPlanes, GK = 4 / PK, GV = 4 / PV;
     constexpr int GKN = NC / GK, GVN = 2 * ND / GV;  // groups
-    static_assert(NC % GK == 0 && (2 * ND) % GV == 0, "whole groups");
+    static_assert(NC % GK == 0 && (2 * ND) % GV == 0 && (!kHalf || GV == 4), "whole groups");
     const uint32_t k_at = (uint32_t)(l32 * Tile::kKPitch + 16 * h), v_at = (uint32_t)(Tile::kV + l32 * Tile::kVPitch + 16 * h);
     auto read_k = [&](u32x4(&f)[4], uint32_t par, int g) {
         const uint8_t* p = smem + (par + k_at);
@@ -1203,6 +1227,13 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
                 for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(slope2, away + (float)(8 * (v >> 2) + (v & 3)), s[v]);
                 f = 1.0f;
             }
+            float low = 0.0f;  // kHalf: the lane's lowest score (masked ones, too)
+            if constexpr (kHalf)
+            {
+                low = s[0];
+#pragma unroll
+                for (int v = 1; v < 16; ++v) low = fminf(low, s[v]);
+            }
             if (kb * kPK + kPK - 1 > seq.from(a, w))
             {
 #pragma unroll
@@ -1214,10 +1245,10 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
             for (int v = 1; v < 16; ++v) mx = fmaxf(mx, s[v]);
             mx = fmaxf(mx, __shfl_xor(mx, 32)) * f;
             // the reference of a query moves only when its maximum has grown by 2^8 (or is new)
-            const bool grown = mx > m_ref + kPLazy;
+            const bool grown = mx > m_ref + (kHalf ? kPLazy + kPUp : kPLazy);
             if (__builtin_amdgcn_ballot_w64(grown) != 0)
             {
-                const float m_new = grown ? mx : m_ref;
+                const float m_new = grown ? (kHalf ? mx - kPUp : mx) : m_ref;
                 // 0 on the first tile (a query may have seen no key yet where a span begins within its item)
                 const float corr = kPaged && !grown ? 1.0f : __builtin_amdgcn_exp2f(m_ref - m_new);
                 l_run *= corr;
@@ -1228,6 +1259,88 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
                 m_ref = m_new;
             }
             const float ref = kPaged && m_ref == -__builtin_inff() ? 0.0f : m_ref;
+            if constexpr (kHalf)
+            {
+                // p = a + b 2^-11 to 2^-22 of it for p from 2^-14 on; in [2^7, 2^15] at the largest
+                v8h pa[2], pb[2];
+#pragma unroll
+                for (int v = 0; v < 16; v += 2)
+                {
+                    s[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], f, -ref));
+                    s[v + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v + 1], f, -ref));
+                    l_run += s[v];
+                    l_run += s[v + 1];
+                    v2h x, y;
+                    split2_up(s[v], s[v + 1], 0x1p11f, x, y);
+                    pa[v >> 3][v & 7] = x[0], pa[v >> 3][(v & 7) + 1] = x[1];
+                    pb[v >> 3][v & 7] = y[0], pb[v >> 3][(v & 7) + 1] = y[1];
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                // O^T += V^T . P^T, a tile summed from zero, the low parts first
+                v16f sum[2];
+#pragma unroll
+                for (int g = 0; g < GVN; ++g)
+                {
+                    const u32x4(&f4)[4] = fr[(GKN + g) & 1];
+                    if (g + 1 < GVN) read_v(fr[(GKN + g + 1) & 1], par, g + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                    {
+                        sum[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, f4[2 * e]), pb[0], v16f{}, 0, 0, 0);
+                        sum[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, f4[2 * e + 1]), pb[1], sum[e], 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                    {
+                        sum[e] *= 0x1p-11f;
+                        sum[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, f4[2 * e]), pa[0], sum[e], 0, 0, 0);
+                        sum[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, f4[2 * e + 1]), pa[1], sum[e], 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) o[2 * g + e] += sum[e];
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                // probabilities below 2^-14 have lost bits: what is left of all goes into further parts, 11 bits each,
+                // as many as the lowest needs down to 2^-80 (2^-87 of the largest)
+                const float deep = -kPDeep - __builtin_fmaf(low, f, -ref);  // > 0: below 2^-14
+                if (__builtin_amdgcn_ballot_w64(deep > 0.0f) != 0) [[unlikely]]
+                {
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        s[v] = s[v] - (float)pa[v >> 3][v & 7] - (float)pb[v >> 3][v & 7] * 0x1p-11f;
+                    float up = 0x1p22f, down = 0x1p-22f;
+#pragma unroll 1
+                    for (float left = fminf(deep, 66.0f); __builtin_amdgcn_ballot_w64(left > 0.0f) != 0;
+                         left -= 11.0f, up *= 0x1p11f, down *= 0x1p-11f)
+                    {
+                        v8h c[2];
+#pragma unroll
+                        for (int v = 0; v < 16; v += 2)
+                        {
+                            const v2h x = __builtin_convertvector(v2f{s[v] * up, s[v + 1] * up}, v2h);
+                            c[v >> 3][v & 7] = x[0], c[v >> 3][(v & 7) + 1] = x[1];
+                            s[v] -= (float)x[0] * down;
+                            s[v + 1] -= (float)x[1] * down;
+                        }
+#pragma unroll
+                        for (int g = 0; g < GVN; ++g)
+                        {
+                            u32x4 f4[4];
+                            read_v(f4, par, g);
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                            {
+                                v16f t = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, f4[2 * e]), c[0], v16f{}, 0, 0, 0);
+                                t = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, f4[2 * e + 1]), c[1], t, 0, 0, 0);
+                                o[2 * g + e] += t * down;
+                            }
+                        }
+                    }
+                }
+            }
+            else
+            {
             v8b p[3][2];
 #pragma unroll
             for (int v = 0; v < 16; v += 2)
@@ -1267,6 +1380,7 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
                 __builtin_amdgcn_sched_barrier(0);
             }
             o[ND - 1] += sum[(ND - 1) & 1];
+            }
         }
         // V's waves convert behind their products, K's before them: each SIMD has one of both, whose VALU and MFMA
         // phases then fall together
@@ -1440,7 +1554,7 @@ __global__ __launch_bounds__(32 * kPWaves) void k_prompt_join(PrefillArgs a, int
 template <int DK, bool kPaged, bool kShaped, typename CT>
 hipError_t launch_prefill_dk(hipStream_t st, const PrefillArgs& a)
 {
-    constexpr int lds = PrefillTile<DK, CT>::kBytes;
+    constexpr int lds = PrefillTile<DK, CT, kPaged && sizeof(CT) == 2>::kBytes;
     static bool attr_set = false;
     if (!attr_set)
     {
