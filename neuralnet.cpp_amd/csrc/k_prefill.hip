@@ -195,8 +195,7 @@ constexpr float kPLazy = 8.0f;         // log2 growth of a query's maximum befor
 // Largest dk max|q| max|k| |scale| log2(e) of a query and a tile: a score's parts below the halves' range
 // (2^-40 of the largest value) add up to less than 2^-21, and no score rounds a reference maximum by 2^-5.
 constexpr float kPReach = 0x1p18f;
-constexpr float kPUp = 7.0f;           // f16 parts of probabilities: the reference lies 2^7 below the maximum
-constexpr float kPDeep = 14.0f;        // ... and two of them hold what is above 2^-14
+constexpr float kPUp = 15.0f;          // f16 parts of probabilities: the largest of a tile is 2^15
 constexpr float kPTiny = 0x1p-100f;    // outputs below this (but for 0) may have lost bits of a bf16 part
 
 struct PrefillArgs
@@ -994,7 +993,8 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
             if (__builtin_amdgcn_ballot_w64(!((float)__builtin_bit_cast(_Float16, top) <= klim)) != 0 && lane == 0) *flag = 1;
         }
     };
-    // raw as f16 halves (K, scaled by 2^ek) and bf16 parts (V) into buffer kb & 1
+    u16x2 v_top = {0, 0};  // kHalf, V's waves: the largest value (bits)
+    // raw as f16 halves (K, scaled by 2^ek) and bf16 parts (V; kHalf: as it is) into buffer kb & 1
     auto convert = [&](int kb) {
         uint8_t* buf = smem + (kb & 1) * Tile::kBuf;
         const float sk = F32C ? pow2(ek) : 1.0f;
@@ -1010,6 +1010,9 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
                 uint8_t* dst = buf + Tile::kV + r * Tile::kVPitch + 32 * s + 16 * hh + 8 * ah;
                 if constexpr (kHalf)
                 {
+                    if (e == 0)
+#pragma unroll
+                        for (int i = 0; i < VW; ++i) v_top = __builtin_elementwise_max(v_top, __builtin_bit_cast(u16x2, raw[i] & 0x7FFF7FFFu));
                     // the halves of dimension e of the four keys
                     const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
                     const uint32_t k01 = __builtin_amdgcn_perm(raw[ND / 2 + e / 2], raw[e / 2], sel);
@@ -1123,6 +1126,7 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = v16f{};
     float m_ref = -__builtin_inff(), l_run = 0.0f;  // log2 units; l_run: this lane half's keys
+    bool deep = false;  // kHalf: the lane's query has seen a tile whose smallest weight has lost bits
 
     trim(kb0);
     post_max(kb0);
@@ -1245,10 +1249,11 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
             for (int v = 1; v < 16; ++v) mx = fmaxf(mx, s[v]);
             mx = fmaxf(mx, __shfl_xor(mx, 32)) * f;
             // the reference of a query moves only when its maximum has grown by 2^8 (or is new)
-            const bool grown = mx > m_ref + (kHalf ? kPLazy + kPUp : kPLazy);
+            if constexpr (kHalf) mx = __builtin_ceilf(mx);  // whole powers of two: every rescaling is exact
+            const bool grown = mx > m_ref + kPLazy;
             if (__builtin_amdgcn_ballot_w64(grown) != 0)
             {
-                const float m_new = grown ? (kHalf ? mx - kPUp : mx) : m_ref;
+                const float m_new = grown ? mx : m_ref;
                 // 0 on the first tile (a query may have seen no key yet where a span begins within its item)
                 const float corr = kPaged && !grown ? 1.0f : __builtin_amdgcn_exp2f(m_ref - m_new);
                 l_run *= corr;
@@ -1261,20 +1266,26 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
             const float ref = kPaged && m_ref == -__builtin_inff() ? 0.0f : m_ref;
             if constexpr (kHalf)
             {
-                // p = a + b 2^-11 to 2^-22 of it for p from 2^-14 on; in [2^7, 2^15] at the largest
+                // The tile's weights under a reference of its own, 2^15 at most: p = a + b 2^-11 to 2^-22 of it for p
+                // from 2^-14 on, and to 2^-36 below
+                const float own = mx == -__builtin_inff() ? 0.0f : mx - kPUp;
+                const float back = mx == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(own - ref);
+                deep |= __builtin_fmaf(low, f, -own) < -14.0f;
+                float l_tile = 0.0f;
                 v8h pa[2], pb[2];
 #pragma unroll
                 for (int v = 0; v < 16; v += 2)
                 {
-                    s[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], f, -ref));
-                    s[v + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v + 1], f, -ref));
-                    l_run += s[v];
-                    l_run += s[v + 1];
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], f, -own));
+                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v + 1], f, -own));
+                    l_tile += p0;
+                    l_tile += p1;
                     v2h x, y;
-                    split2_up(s[v], s[v + 1], 0x1p11f, x, y);
+                    split2_up(p0, p1, 0x1p11f, x, y);
                     pa[v >> 3][v & 7] = x[0], pa[v >> 3][(v & 7) + 1] = x[1];
                     pb[v >> 3][v & 7] = y[0], pb[v >> 3][(v & 7) + 1] = y[1];
                 }
+                l_run = __builtin_fmaf(l_tile, back, l_run);
                 __builtin_amdgcn_sched_barrier(0);
                 // O^T += V^T . P^T, a tile summed from zero, the low parts first
                 v16f sum[2];
@@ -1298,88 +1309,53 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
                         sum[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, f4[2 * e + 1]), pa[1], sum[e], 0, 0, 0);
                     }
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) o[2 * g + e] += sum[e];
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) o[2 * g + e][v] = __builtin_fmaf(sum[e][v], back, o[2 * g + e][v]);
                     __builtin_amdgcn_sched_barrier(0);
-                }
-                // probabilities below 2^-14 have lost bits: what is left of all goes into further parts, 11 bits each,
-                // as many as the lowest needs down to 2^-80 (2^-87 of the largest)
-                const float deep = -kPDeep - __builtin_fmaf(low, f, -ref);  // > 0: below 2^-14
-                if (__builtin_amdgcn_ballot_w64(deep > 0.0f) != 0) [[unlikely]]
-                {
-#pragma unroll
-                    for (int v = 0; v < 16; ++v)
-                        s[v] = s[v] - (float)pa[v >> 3][v & 7] - (float)pb[v >> 3][v & 7] * 0x1p-11f;
-                    float up = 0x1p22f, down = 0x1p-22f;
-#pragma unroll 1
-                    for (float left = fminf(deep, 66.0f); __builtin_amdgcn_ballot_w64(left > 0.0f) != 0;
-                         left -= 11.0f, up *= 0x1p11f, down *= 0x1p-11f)
-                    {
-                        v8h c[2];
-#pragma unroll
-                        for (int v = 0; v < 16; v += 2)
-                        {
-                            const v2h x = __builtin_convertvector(v2f{s[v] * up, s[v + 1] * up}, v2h);
-                            c[v >> 3][v & 7] = x[0], c[v >> 3][(v & 7) + 1] = x[1];
-                            s[v] -= (float)x[0] * down;
-                            s[v + 1] -= (float)x[1] * down;
-                        }
-#pragma unroll
-                        for (int g = 0; g < GVN; ++g)
-                        {
-                            u32x4 f4[4];
-                            read_v(f4, par, g);
-#pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                            {
-                                v16f t = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, f4[2 * e]), c[0], v16f{}, 0, 0, 0);
-                                t = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, f4[2 * e + 1]), c[1], t, 0, 0, 0);
-                                o[2 * g + e] += t * down;
-                            }
-                        }
-                    }
                 }
             }
             else
             {
-            v8b p[3][2];
+                v8b p[3][2];
 #pragma unroll
-            for (int v = 0; v < 16; v += 2)
-            {
-                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], f, -ref));
-                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v + 1], f, -ref));
-                l_run += p0;
-                l_run += p1;
-                v2b x[3];
-                split_bf16(p0, p1, x);
-#pragma unroll
-                for (int q = 0; q < 3; ++q) p[q][v >> 3][v & 7] = x[q][0], p[q][v >> 3][(v & 7) + 1] = x[q][1];
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            // O^T += V^T . P^T: the products of parts i and j with i + j <= 2, smallest first; the rest is
-            // at most 2^-24 of a term. A tile is summed from zero and added once: that rounds the running
-            // sum once in 32 keys. The add of a block runs beside the products of the next.
-            v16f sum[2];
-#pragma unroll
-            for (int g = 0; g < GVN; ++g)
-            {
-                const u32x4(&f4)[4] = fr[(GKN + g) & 1];
-                if (g + 1 < GVN) read_v(fr[(GKN + g + 1) & 1], par, g + 1);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int e = 0; e < GV; ++e)
+                for (int v = 0; v < 16; v += 2)
                 {
-                    const int d = (GV * g + e) >> 1, t = (GV * g + e) & 1;
-                    if (t == 0) sum[d & 1] = v16f{};
-                    if (t == 1 - (GV & 1) && d > 0) o[d - 1] += sum[(d - 1) & 1];
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], f, -ref));
+                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v + 1], f, -ref));
+                    l_run += p0;
+                    l_run += p1;
+                    v2b x[3];
+                    split_bf16(p0, p1, x);
 #pragma unroll
-                    for (int n = 2; n >= 0; --n)
-#pragma unroll
-                        for (int i = PV - 1 < n ? PV - 1 : n; i >= 0; --i)
-                            sum[d & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, f4[PV * e + i]), p[n - i][t], sum[d & 1], 0, 0, 0);
+                    for (int q = 0; q < 3; ++q) p[q][v >> 3][v & 7] = x[q][0], p[q][v >> 3][(v & 7) + 1] = x[q][1];
                 }
                 __builtin_amdgcn_sched_barrier(0);
-            }
-            o[ND - 1] += sum[(ND - 1) & 1];
+                // O^T += V^T . P^T: the products of parts i and j with i + j <= 2, smallest first; the rest is
+                // at most 2^-24 of a term. A tile is summed from zero and added once: that rounds the running
+                // sum once in 32 keys. The add of a block runs beside the products of the next.
+                v16f sum[2];
+#pragma unroll
+                for (int g = 0; g < GVN; ++g)
+                {
+                    const u32x4(&f4)[4] = fr[(GKN + g) & 1];
+                    if (g + 1 < GVN) read_v(fr[(GKN + g + 1) & 1], par, g + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int e = 0; e < GV; ++e)
+                    {
+                        const int d = (GV * g + e) >> 1, t = (GV * g + e) & 1;
+                        if (t == 0) sum[d & 1] = v16f{};
+                        if (t == 1 - (GV & 1) && d > 0) o[d - 1] += sum[(d - 1) & 1];
+#pragma unroll
+                        for (int n = 2; n >= 0; --n)
+#pragma unroll
+                            for (int i = PV - 1 < n ? PV - 1 : n; i >= 0; --i)
+                                sum[d & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, f4[PV * e + i]), p[n - i][t], sum[d & 1], 0, 0, 0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                o[ND - 1] += sum[(ND - 1) & 1];
             }
         }
         // V's waves convert behind their products, K's before them: each SIMD has one of both, whose VALU and MFMA
@@ -1399,13 +1375,27 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
     // V is not looked through for infinities and NaN: any that matters is in the sums. Nor for values whose smallest part would lie below bf16's range: their output is tiny then.
     l_run += __shfl_xor(l_run, 32);
     bool lost = !(l_run < __builtin_inff());
+    float faint = l_run * kPTiny;  // outputs below (but for 0) may have lost bits
+    if constexpr (kHalf)
+    {
+        // Weights below 2^-29 of the largest of their tile are held to 2^-51 of that one: nothing beside an output, unless
+        // the heavy keys' values are 0 where theirs are not. Such outputs are below 2^-32 of the largest value then,
+        // and come from the f32 products. (From 2^-27 on, a value that happens to be 0 sent a call in four there,
+        // at the cost of five tiles each.)
+        const uint32_t top = wave_max(max((uint32_t)v_top[0], (uint32_t)v_top[1]));
+        if (lane == 0) smax[wave] = is_v ? top : 0u;
+        __syncthreads();
+        const uint32_t most = max(max(smax[0], smax[1]), max(smax[2], smax[3]));
+        deep |= __shfl_xor((int)deep, 32) != 0;
+        faint = deep ? l_run * ((float)__builtin_bit_cast(_Float16, (uint16_t)most) * 0x1p-32f) : -1.0f;
+    }
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int v = 0; v < 16; ++v)
         {
             const float y = fabsf(o[d][v]);
-            lost |= !(y < __builtin_inff()) || (y < l_run * kPTiny && y != 0.0f);
+            lost |= !(y < __builtin_inff()) || (y < faint && (kHalf || y != 0.0f));
         }
     if (__syncthreads_or(!fallback && w.live && lost) || fallback)
     {
