@@ -697,7 +697,7 @@ nnhip_status nnhip_kv_pages_fill(nnhip_ctx* ctx, const nnhip_kv_pages* cache, co
  * a page outside the pool among positions [0, pos[b]]: out NaN. len_bound <= table_stride * page_size
  * and (with tables) rope_len. Two sequences of one call whose new tokens fall on one place of the pool
  * leave either there. Sums and softmax are f32 in an order of the kernel's own, the same in every call
- * of the same sizes (compute_layer_attention.hpp:1022-1083). */
+ * of the same sizes and positions (compute_layer_attention.hpp:1022-1083). */
 nnhip_status nnhip_attention_pages_decode(nnhip_ctx* ctx, const nnhip_kv_pages* cache, const float* q, const float* k,
                                           const float* v, size_t B, size_t H, const int32_t* pos, size_t len_bound,
                                           const float* rope_cos, const float* rope_sin, size_t rope_len, float scale,
@@ -709,7 +709,10 @@ nnhip_status nnhip_attention_pages_decode(nnhip_ctx* ctx, const nnhip_kv_pages* 
  * every sequence's tokens (it sizes the launch). A token at position i sees its own sequence's positions
  * j <= i, and with prefix (DEVICE (B) int32, or NULL) also every j < prefix[b] that the sequence has;
  * nothing of another sequence. Scores, softcap and slopes as nnhip_attention_pages_decode (j - i is above
- * 0 inside a prefix); products, sums, errors and the f32 products' cases as nnhip_attention_prefill. dk in
+ * 0 inside a prefix); products, sums, errors and the f32 products' cases as nnhip_attention_prefill, but for
+ * f16 pools, whose weights are held to 2^-22 of themselves down to 2^-29 of the largest in their run of 32
+ * keys and to 2^-51 of that one below (outputs so small that this could show take the f32 products). The
+ * sums' order depends on all sequences of the call. dk in
  * {64, 128}, any H / Hkv, H * dk * M < 2^29. Columns of no sequence are not written. NaN: a sequence with
  * more than t_bound tokens, columns outside [0, M) or positions at or past table_stride * page_size or
  * rope_len; a query that sees a position whose page is outside the pool (other queries of its sequence

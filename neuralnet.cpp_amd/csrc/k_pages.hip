@@ -240,7 +240,13 @@ __device__ __forceinline__ PagesItem find_item(const PagesArgs& a, int item, int
 //   values   the probability of (row u, head h) is broadcast within the 16 lanes by a DPP move.
 // A head's reference maximum moves only when it has grown by 2^8.
 // The chunk that holds the new position writes its rotated key and its value to the page (no other
-// work-group reads that row) and starts the first group's sums with them.
+// work-group reads that row) and adds them to its sums as one more row.
+// Bound by HBM where the caches are large (4 x 60000 .. 131072 positions, 8 heads of 128, f16: 231 us with the
+// join, 6.4 TB/s of the bytes it cannot do without; a large copy reaches 4.9 read and written together);
+// by the chain of round trips position -> page -> rows, about 7 us in the kernel and 4 in the join,
+// where they are small (16 x 2112, 5 heads of 128, f32: 34.3 us, 4.9 TB/s; 1 x 100: 7.5 us, one launch). With 8
+// heads to a KV head of 64 in f16 the 400 VALU instructions of a tile (256 multiply-adds, 90 of
+// the fold, 32 broadcasts) take as long as its bytes.
 template <int DK, int RT, bool kFinal, typename CT>
 __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
 {
@@ -571,7 +577,9 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
     }
 }
 
-// out of one (sequence, head) from its chunks' records: sum_c 2^(m_c - m) acc_c / sum_c 2^(m_c - m) l_c
+// out of one (sequence, head) from its chunks' records: sum_c 2^(m_c - m) acc_c / sum_c 2^(m_c - m) l_c, in the order
+// of the records: the same in every call of the same sizes and positions. A launch of its own: a join by the
+// last work-group to arrive would need the records written back from one XCD's L2 before another's reads.
 template <int DK>
 __global__ __launch_bounds__(kPgThreads) void k_pages_join(PagesArgs a)
 {
@@ -728,7 +736,8 @@ __device__ __forceinline__ int wave_sequence(const int32_t* cu, int B, int M, in
 // Work-group = (64 tokens, KV head, keys or values): the head's dk feature rows of those tokens read
 // along tokens, turned through LDS and written as rows of pages, keys rotated at their positions. Bound by
 // HBM; a work-group lives for its chain of round trips, so the features are on their way while the chain
-// sequence -> position -> page and rotation is followed, the same in each wave.
+// sequence -> position -> page and rotation is followed, the same in each wave (by bisection in each thread
+// behind the features 56.5 us, 44.4 so: 16 x 1111 .. 2048 tokens, 5 heads of 128, f16, 4.4 TB/s).
 // Tokens of no sequence, positions outside the table or the rope tables and pages outside the pool are
 // not written.
 template <int DK, typename CT>

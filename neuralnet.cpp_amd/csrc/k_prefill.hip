@@ -44,10 +44,28 @@
 // Softmax in log2 units with the hardware exp2; a query's reference maximum moves only when it has
 // grown by 2^8 (probabilities are at most 2^8), so the sums are rarely rescaled.
 // Work-groups are issued heaviest first (the last query blocks attend over the most keys).
-// Measured (calls back to back in a graph, us, f32 products / here): f32 caches 4 x 2048 tokens
+// V's four waves convert their part of the next tile behind their products, K's before them: every SIMD
+// has one wave of each, and one's VALU phases fall on the other's MFMA phases (4 x 2048 tokens f32 caches
+// 389 -> 367 us, f16 280 -> 273, back to back on one box).
+// Measured before that (calls back to back in a graph, us, f32 products / here): f32 caches 4 x 2048 tokens
 // 809 / 398, 3 x 1111 at 517 411 / 202, 16 x 2048 3088 / 1498, 1 x 64 22.5 / 17.7; f16 caches 817 / 293,
 // 421 / 146, 3153 / 1121, 22.7 / 15.9. Two f16 halves for P and V too (at the cost above) took 295 and
 // 198 us at 4 x 2048.
+//
+// Over pages (kPaged): packed sequences of unlike lengths, each at its own position, whose rows are found
+// through a page table read a tile ahead; a prefix that all queries see, a tanh cap and a distance bias on
+// the scores. Any H / Hkv: a KV head's heads go in groups of 8, 4, 2 or 1.
+//   * Work-groups take equal spans of all tiles of the call (PromptPlan) and join the blocks of queries
+//     they share; a plain work-group per block of queries left most CUs idle behind a long sequence, or
+//     behind the 14 blocks beyond 256 (4 x 700 .. 1024 tokens at 6144, f16: 1087 -> 754 us).
+//   * f16 caches: V as it is in f16 products with the weights in two f16 parts, p = a + b 2^-11, under a reference of
+//     the tile's own: every weight to 2^-22 of itself down to 2^-29 of the largest of its 32 keys, and to
+//     2^-51 of that one below; two MFMAs instead of five and no splitting of V (688 -> 579 us). Weights of
+//     one tile share an exponent with each other here, never with values; where heavy keys' values are 0, and
+//     lost bits could show, the f32 products run.
+// prompt of 4 x 700 .. 1024 tokens at position 6144, 20 heads over 5 of 128, f16: 579 us, 396 TFLOP/s of the
+// attention's own products; 8 x 77 .. 1900 tokens, 16 heads over 2 of 64, f32, capped and biased: 139 us.
+// Bound by the VALU and MFMA work of a tile, which two waves to a SIMD overlap in part.
 // Caches of f16 elements (compute = F16): the fill rounds the rotated keys and the values to the
 // nearest f16 (ties to even), as the decode append does.
 #include "common.hpp"
