@@ -680,7 +680,7 @@ typedef struct nnhip_kv_pages
  * rope_cos / rope_sin (rope_len, dk/2) from nnhip_rope_table (both NULL: no position encoding), bit for
  * bit as nnhip_kv_cache_fill's; f16 pools get the nearest f16. Not written: columns of no sequence
  * (cu[B] and on), positions at or past table_stride * page_size or rope_len, pages outside the pool.
- * Two tokens of one call at one place of the pool leave either there. The paged form of
+ * Two tokens of one call at one place of the pool leave there, for each element, either's. The paged form of
  * nnhip_kv_cache_fill (compute_layer_attention.hpp:1040-1060). */
 nnhip_status nnhip_kv_pages_fill(nnhip_ctx* ctx, const nnhip_kv_pages* cache, const float* k, const float* v,
                                  size_t M, const int32_t* cu, const int32_t* pos0, size_t B, const float* rope_cos,
@@ -696,7 +696,7 @@ nnhip_status nnhip_kv_pages_fill(nnhip_ctx* ctx, const nnhip_kv_pages* cache, co
  * pos[b] < 0: an empty slot, out zeros, nothing written; pos[b] >= len_bound: out NaN, nothing written;
  * a page outside the pool among positions [0, pos[b]]: out NaN. len_bound <= table_stride * page_size
  * and (with tables) rope_len. Two sequences of one call whose new tokens fall on one place of the pool
- * leave either there. Sums and softmax are f32 in an order of the kernel's own, the same in every call
+ * leave there, for each element, either's. Sums and softmax are f32 in an order of the kernel's own, the same in every call
  * of the same sizes and positions (compute_layer_attention.hpp:1022-1083). */
 nnhip_status nnhip_attention_pages_decode(nnhip_ctx* ctx, const nnhip_kv_pages* cache, const float* q, const float* k,
                                           const float* v, size_t B, size_t H, const int32_t* pos, size_t len_bound,
@@ -728,7 +728,8 @@ nnhip_status nnhip_attention_pages_prefill(nnhip_ctx* ctx, const nnhip_kv_pages*
  * more than 512 positions. The context keeps one for each stream that it was set to, grown on demand and freed with the context only, so that a
  * captured call stays valid; a call that would have to grow it during a capture fails with
  * NNHIP_ERR_UNSUPPORTED (call once before, on the capture's stream). Captured calls of one stream share
- * its scratch: their replays must not overlap. */
+ * its scratch, wherever they are replayed: their replays must overlap neither each other nor eager calls
+ * on that stream. */
 size_t nnhip_attention_pages_workspace_bytes(nnhip_ctx* ctx, size_t B, size_t H, size_t Hkv, size_t dk,
                                              size_t len_bound);
 size_t nnhip_logits_workspace_bytes(nnhip_ctx* ctx, size_t V, size_t B);

@@ -722,14 +722,15 @@ __device__ __forceinline__ int wave_sequence(const int32_t* cu, int B, int M, in
         if (step == 1) break;
         n = min(step, n - k);
     }
+    if (lo >= B) return -1;
     const int m = m0 + (lane & (kPfTok - 1));
-    if (lo >= B || m >= M) return -1;
-    // the ends of the sequences from there on that lie in the block
+    // the ends of the sequences from there on that lie in the block: of every lane, those behind column M too
     const int end = lo + 1 + lane <= B ? cu[lo + 1 + lane] : 0x7FFFFFFF;
     const int ends = __builtin_popcountll(__builtin_amdgcn_ballot_w64(end <= m0 + kPfTok - 1));
-    if (ends == kWave) return packed_sequence(cu, B, m);  // (64 sequences without a token among them)
     int b = lo;
     for (int i = 0; i < ends; ++i) b += __builtin_amdgcn_readlane(end, i) <= m ? 1 : 0;
+    if (m >= M) return -1;
+    if (ends == kWave) return packed_sequence(cu, B, m);  // (64 sequences that end here, and more maybe)
     return b < B && cu[b] >= 0 && cu[b] <= m && cu[b + 1] > m ? b : -1;
 }
 

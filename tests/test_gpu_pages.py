@@ -242,6 +242,24 @@ def test_fill(ctx, nnhip, dk, f16, rope):
     assert same(host(cache.k), c.k) and same(host(cache.v), c.v)
 
 
+@pytest.mark.parametrize("lens", [[1] + [0] * 8 + [4], [3] + [0] * 62 + [2], [1] + [0] * 63 + [5], [2] + [0] * 150 + [1, 0, 1],
+                                  [0] * 70 + [65] + [0] * 40 + [7] + [0] * 5])
+def test_fill_sequences_without_tokens(ctx, nnhip, lens):
+    """Runs of empty sequences between tokens of one block, no column behind the last token."""
+    rng = np.random.default_rng(12)
+    Hkv, dk, page = 2, 64, 8
+    cu = np.concatenate(([0], np.cumsum(lens))).astype(np.int32)
+    M = int(cu[-1])
+    c = Cache(rng, lens, Hkv, page, dk, False)
+    k, v = (rng.standard_normal((Hkv * dk, M)).astype(np.float32) for _ in range(2))
+    cache = c.on_device(nnhip)
+    ctx.kv_pages_fill(cache, dev(k), dev(v), dev(cu))
+    for b, n in enumerate(lens):
+        for t in range(n):
+            c.set(b, t, k[:, cu[b] + t].reshape(Hkv, dk), v[:, cu[b] + t].reshape(Hkv, dk))
+    assert same(host(cache.k), c.k) and same(host(cache.v), c.v)
+
+
 def test_fill_matches_contiguous_fill(ctx, nnhip):
     """Equal prompts into pages of 8 and into contiguous caches: the same bits."""
     rng = np.random.default_rng(11)
