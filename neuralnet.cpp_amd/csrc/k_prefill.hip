@@ -800,6 +800,13 @@ __device__ __forceinline__ float* prompt_record(const PrefillArgs& a, int g, int
     return a.part + ((size_t)g * 2 + slot) * (size_t)((DK + 2) * 32 * kPWaves);
 }
 
+// The cuts before each of the spans, behind their records
+template <int DK>
+__device__ __forceinline__ PromptCut* prompt_cuts(const PrefillArgs& a, int spans)
+{
+    return reinterpret_cast<PromptCut*>(prompt_record<DK>(a, spans, 0));
+}
+
 // Attention of an item over its tiles k0 .. k1 - 1; rec: into a record instead of the output
 template <int DK, bool kPaged, bool kShaped, typename CT>
 __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& item, uint8_t* smem, int k0, int k1, float* rec)
@@ -1475,6 +1482,7 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
             const PromptPlan plan = prompt_plan(a, gridDim.x);
             at = prompt_cut(a, plan, g * plan.per);
             end = prompt_cut(a, plan, (g + 1) * plan.per);
+            if (threadIdx.x == 0) prompt_cuts<DK>(a, a.spans)[g] = at;
         }
         else
         {
@@ -1509,31 +1517,20 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
 }
 
 // The items that several spans share: work-group g joins the one that the cut before span g is the first to
-// fall into, from its records: sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, 16 dimensions of its 256 queries
+// fall into, from its records: sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, 16 dimensions of its 256 queries.
+// Span g - 1 wrote slot 1, those from g on that begin within the item slot 0: fewer than 40 (PromptPlan's per).
 template <int DK>
-__global__ __launch_bounds__(32 * kPWaves) void k_prompt_join(PrefillArgs a, int spans)
+__global__ __launch_bounds__(32 * kPWaves) void k_prompt_join(PrefillArgs a)
 {
     constexpr int N = 16;
-    const int g = blockIdx.x + 1, d0 = blockIdx.y * N, row = threadIdx.x;
-    const PromptPlan plan = prompt_plan(a, spans);
-    const PromptCut at = prompt_cut(a, plan, g * plan.per);
-    if (at.gh >= a.Hkv * a.groups || at.t == 0) return;
-    const PromptCut last = prompt_cut(a, plan, (g - 1) * plan.per);
-    if (cut_same_item(at, last) && last.t > 0) return;
+    const int g = blockIdx.x + 1, d0 = blockIdx.y * N, row = threadIdx.x, lane = row & 63;
+    const PromptCut* const cuts = prompt_cuts<DK>(a, a.spans);
+    const PromptCut at = cuts[g], last = cuts[g - 1], later = cuts[min(g + lane, a.spans - 1)];
+    if (at.gh >= a.Hkv * a.groups || at.t == 0 || (cut_same_item(at, last) && last.t > 0)) return;
+    const unsigned long long within = __builtin_amdgcn_ballot_w64(g + lane < a.spans && cut_same_item(at, later));
+    const int n = 1 + __builtin_popcountll(within);
     PrefillSeq<true> q;
     packed_seq(a, at.b, q);
-    // the spans from g on that begin within the item (their cuts are plan.per apart)
-    int64_t until = at.gh * plan.head;
-    for (int b0 = 0; b0 < at.b; b0 += kWave)
-    {
-        int m;
-        int64_t x = b0 + (int)(threadIdx.x & 63) < at.b ? prompt_work(a, b0 + (int)(threadIdx.x & 63), m) : 0;
-        for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off, kWave);
-        until += read_lane64(x, 0);
-    }
-    const int tiles = prompt_tiles(a, q, at.qb);
-    until += prompt_before(a, q, at.qb) + kOver + tiles - plan.snap;  // the last cut that does not move to the item's end
-    const int n = (int)((until - g * plan.per) / plan.per) + 2;       // records: span g - 1's, then those of g ..
     const int wave = row >> 5, qt = at.qb * kPQ * (kPWaves / a.R) + wave / a.R * kPQ + (row & 31);
     float top = -__builtin_inff(), den = 0.0f, y[N];
 #pragma unroll
@@ -1578,7 +1575,7 @@ hipError_t launch_prefill_dk(hipStream_t st, const PrefillArgs& a)
         {
             const hipError_t e = hipGetLastError();
             if (e != hipSuccess) return e;
-            k_prompt_join<DK><<<dim3((unsigned)a.spans - 1, DK / 16), 32 * kPWaves, 0, st>>>(a, a.spans);
+            k_prompt_join<DK><<<dim3((unsigned)a.spans - 1, DK / 16), 32 * kPWaves, 0, st>>>(a);
         }
     return hipGetLastError();
 }
@@ -1642,7 +1639,7 @@ size_t pages_prefill_spans(size_t limit, size_t num_cus) { return limit <= (size
 
 size_t pages_prefill_workspace_bytes(size_t dk, size_t limit, size_t num_cus)
 {
-    return pages_prefill_spans(limit, num_cus) * 2 * (dk + 2) * 32 * kPWaves * sizeof(float);
+    return pages_prefill_spans(limit, num_cus) * (2 * (dk + 2) * 32 * kPWaves * sizeof(float) + sizeof(PromptCut));
 }
 
 hipError_t launch_pages_prefill(hipStream_t st, const nnhip_kv_pages& kv, const float* q, size_t M, const int32_t* cu,
