@@ -55,7 +55,7 @@
 // Over pages (kPaged): packed sequences of unlike lengths, each at its own position, whose rows are found
 // through a page table read a tile ahead; a prefix that all queries see, a tanh cap and a distance bias on
 // the scores. Any H / Hkv: a KV head's heads go in groups of 8, 4, 2 or 1.
-//   * Work-groups take equal spans of all tiles of the call (PromptPlan) and join the blocks of queries
+//   * Work-groups take equal spans of all tiles of the call (prompt_cut) and join the blocks of queries
 //     they share; a plain work-group per block of queries left most CUs idle behind a long sequence, or
 //     behind the 14 blocks beyond 256 (4 x 700 .. 1024 tokens at 6144, f16: 1087 -> 754 us).
 //   * f16 caches: V as it is in f16 products with the weights in two f16 parts, p = a + b 2^-11, under a reference of
@@ -208,6 +208,8 @@ typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kPWaves = 8;             // waves of a work-group: R heads x (8 / R) blocks of 32 queries
 constexpr int kPThreads = 64 * kPWaves;
+constexpr int kPWaveShift = 3, kPQShift = 5, kPKShift = 5;  // their logarithms
+static_assert(kPWaves == 1 << kPWaveShift && kPQ == 1 << kPQShift && kPK == 1 << kPKShift, "");
 constexpr int kPExpMax = 48;           // scalings beyond 2^+-48 take the f32 products
 constexpr float kPLazy = 8.0f;         // log2 growth of a query's maximum before its sums are rescaled
 // Largest dk max|q| max|k| |scale| log2(e) of a query and a tile: a score's parts below the halves' range
@@ -239,7 +241,7 @@ struct PrefillArgs
     int table_stride, num_pages, shift, limit;  // limit: positions from here on have no place
     float cap2, capi2;      // softcap * log2(e) and its inverse, 0 without
     float* part;            // spans: records of the items that several work-groups share
-    int spans;              // work-groups that take spans of all tiles (see PromptPlan); 0: one item each
+    int spans;              // work-groups that take spans of all tiles (see prompt_cut); 0: one item each
 };
 
 // kHalf: V as it is in f16 caches, for products with probabilities in f16 parts
@@ -606,6 +608,9 @@ __device__ void attend_f32(const PrefillArgs& a, const PrefillWave& w, const Pre
         store_out<DK>(a, w, seq, h, [](int d, int r) { return 32 * d + r; }, [&](int d, int v) { return o[d][v] / l_run; });
 }
 
+// log2 of the heads of a work-group, which are 1, 2, 4 or 8
+__device__ __forceinline__ int log2_heads(const PrefillArgs& a) { return __builtin_ctz(a.R); }
+
 // What a work-group works on: a block of qn = 32 (8 / R) queries of R heads (from `first`, of KV head g) of
 // sequence b. Paged: with the sequence.
 struct PrefillItem
@@ -620,11 +625,11 @@ __device__ __forceinline__ void seat(const PrefillArgs& a, const PrefillItem& it
                                      PrefillSeq<kPaged>& seq, int& last_key)
 {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int qn = kPQ * (kPWaves / a.R);  // queries of the work-group
+    const int rs = log2_heads(a), qn = kPQ << (kPWaveShift - rs);  // queries of the work-group
     w.b = it.b;
     w.g = it.g;
-    w.head = it.first + wave % a.R;
-    w.t0 = it.qb * qn + wave / a.R * kPQ;
+    w.head = it.first + (wave & (a.R - 1));
+    w.t0 = it.qb * qn + (wave >> rs) * kPQ;
     w.qt = w.t0 + (tid & 31);
     if constexpr (kPaged) seq = it.seq;
     w.qpos = seq.pos0(a) + w.qt;
@@ -659,12 +664,7 @@ __device__ void store_nan(const PrefillArgs& a, int b, int first, int heads, int
 // (4 x 1024 queries of 20 heads: 270 for 256 CUs, the last 14 of which took as long as all others). The order
 // is (head group, sequence, block of queries, tile); an item counts kOver tiles more than it has, which
 // its queries and outputs cost. A cut within the first or last kSnap tiles of an item moves to its edge, and
-// where no item has more than kShort tiles, to its start. Every work-group finds the cuts for itself.
-struct PromptPlan
-{
-    int64_t per, head, total;  // tiles of a span, of a head group, of all
-    int snap;
-};
+// where no item has more than kShort tiles, to its start. Every work-group finds its two cuts.
 struct PromptCut
 {
     int gh, b, qb, t;
@@ -673,24 +673,26 @@ constexpr int kOver = 3, kSnap = 4, kShort = 16, kSpanMin = 8;
 
 __device__ __forceinline__ int prompt_blocks(const PrefillArgs& a, int n)
 {
-    const int qn = kPQ * (kPWaves / a.R);
-    return (n + qn - 1) / qn;
+    const int qs = kPQShift + kPWaveShift - log2_heads(a);  // log2 of a block's queries
+    return (n + (1 << qs) - 1) >> qs;
 }
 
 // Tiles of block qb
 __device__ __forceinline__ int prompt_tiles(const PrefillArgs& a, const PrefillSeq<true>& q, int qb)
 {
-    const int qn = kPQ * (kPWaves / a.R);
-    return (max(q.pos0_ + min(qb * qn + qn, q.n_), q.pre) + kPK - 1) / kPK;
+    const int qs = kPQShift + kPWaveShift - log2_heads(a);
+    return (max(q.pos0_ + min((qb + 1) << qs, q.n_), q.pre) + kPK - 1) >> kPKShift;
 }
 
 // Tiles of blocks 0 .. qb - 1 with kOver each: A + j u for block j - 1, but at least P, and the last block's own
 __device__ __forceinline__ int64_t prompt_before(const PrefillArgs& a, const PrefillSeq<true>& q, int qb)
 {
-    const int nq = prompt_blocks(a, q.n_), u = kPWaves / a.R, A = (q.pos0_ + kPK - 1) / kPK, P = (q.pre + kPK - 1) / kPK;
-    const int64_t full = min(qb, nq - 1);
-    const int64_t k = max((int64_t)0, min(full, (int64_t)((P - A + u - 1) / u - 1)));
-    int64_t f = k * P + (full - k) * A + u * (full * (full + 1) / 2 - k * (k + 1) / 2) + kOver * full;
+    const int us = kPWaveShift - log2_heads(a);  // log2 of u
+    const int nq = prompt_blocks(a, q.n_), A = (q.pos0_ + kPK - 1) >> kPKShift, P = (q.pre + kPK - 1) >> kPKShift;
+    const int full = min(qb, nq - 1);
+    const int k = max(0, min(full, ((P - A + (1 << us) - 1) >> us) - 1));
+    int64_t f = (int64_t)k * P + (int64_t)(full - k) * (A + kOver) + (int64_t)k * kOver +
+                (((int64_t)full * (full + 1) - (int64_t)k * (k + 1)) >> 1 << us);
     if (qb == nq && nq > 0) f += prompt_tiles(a, q, nq - 1) + kOver;
     return f;
 }
@@ -712,15 +714,17 @@ __device__ __forceinline__ int64_t read_lane64(int64_t x, int l)
     return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)x >> 32), l) << 32) | lo);
 }
 
-__device__ __forceinline__ PromptPlan prompt_plan(const PrefillArgs& a, int spans)
+// The cut before span `span` of `spans` (or the call's end), found by a wave
+__device__ __forceinline__ PromptCut prompt_cut(const PrefillArgs& a, int spans, int span)
 {
     const int lane = threadIdx.x & 63;
-    int64_t sum = 0;
+    int64_t own = 0, sum = 0;
     int most = 0;
     for (int b = lane; b < a.B; b += kWave)
     {
         int m;
-        sum += prompt_work(a, b, m);
+        own = prompt_work(a, b, m);
+        sum += own;
         most = max(most, m);
     }
     for (int off = 1; off < min(a.B, kWave); off <<= 1)
@@ -728,27 +732,24 @@ __device__ __forceinline__ PromptPlan prompt_plan(const PrefillArgs& a, int span
         sum += __shfl_xor(sum, off, kWave);
         most = max(most, __shfl_xor(most, off, kWave));
     }
-    PromptPlan p;
-    p.head = read_lane64(sum, 0);
+    const int64_t head = read_lane64(sum, 0), total = head * (a.Hkv * a.groups);  // tiles of a head group, of all
     most = __builtin_amdgcn_readfirstlane(most);
-    p.total = p.head * (a.Hkv * a.groups);
-    p.per = (p.total + spans - 1) / spans;
-    p.snap = kSnap;
-    if (most <= kShort) p.snap = 1 << 30;
-    else p.per = max(p.per, (int64_t)max(kSpanMin + kOver, (most + kOver) / 32));  // at most about 32 spans to an item
-    return p;
-}
-
-// Where tile x of the call lies
-__device__ __forceinline__ PromptCut prompt_cut(const PrefillArgs& a, const PromptPlan& p, int64_t x)
-{
-    if (x >= p.total) return {a.Hkv * a.groups, 0, 0, 0};
-    const int lane = threadIdx.x & 63, gh = (int)(x / p.head);
-    int64_t y = x - gh * p.head;
+    int64_t per = (total + spans - 1) / spans;
+    int snap = 1 << 30;
+    if (most > kShort)
+    {
+        per = max(per, (int64_t)max(kSpanMin + kOver, (most + kOver) / 32));  // at most about 32 spans to an item
+        snap = kSnap;
+    }
+    // where tile x of the call lies
+    const int64_t x = span * per;
+    if (x >= total) return {a.Hkv * a.groups, 0, 0, 0};
+    const int gh = (int)(x / head);
+    int64_t y = x - gh * head;
     for (int b0 = 0; b0 < a.B; b0 += kWave)
     {
         int m;
-        const int64_t own = prompt_work(a, b0 + lane, m);
+        if (a.B > kWave) own = prompt_work(a, b0 + lane, m);
         int64_t incl = own;
         const int live = min(a.B - b0, kWave);
         for (int off = 1; off < live; off <<= 1)
@@ -766,20 +767,29 @@ __device__ __forceinline__ PromptCut prompt_cut(const PrefillArgs& a, const Prom
         y -= read_lane64(incl - own, l);
         PrefillSeq<true> q;
         packed_seq(a, b, q);
-        int lo = 0, hi = prompt_blocks(a, q.n_) - 1;  // the last block whose tiles begin at or before y
-        while (lo < hi)
+        // the last block whose tiles begin at or before y: of 64 candidates at a time
+        int qb = 0;
+        for (int n = prompt_blocks(a, q.n_); n > 1;)
         {
-            const int mid = (lo + hi + 1) >> 1;
-            if (prompt_before(a, q, mid) <= y) lo = mid;
-            else hi = mid - 1;
+            const int step = (n + kWave - 1) / kWave;
+            const bool at_or_before = lane * step < n && prompt_before(a, q, qb + lane * step) <= y;
+            const int k = step * (__builtin_popcountll(__builtin_amdgcn_ballot_w64(at_or_before)) - 1);
+            qb += k;
+            n = min(step, n - k);
         }
-        const int tiles = prompt_tiles(a, q, lo);
-        int t = (int)(y - prompt_before(a, q, lo)) - kOver;
-        if (t < p.snap) t = 0;
-        else if (tiles - t < p.snap) return {gh, b, lo + 1, 0};
-        return {gh, b, lo, t};
+        const int tiles = prompt_tiles(a, q, qb);
+        int t = (int)(y - prompt_before(a, q, qb)) - kOver;
+        if (t < snap) t = 0;
+        else if (tiles - t < snap) return {gh, b, qb + 1, 0};
+        return {gh, b, qb, t};
     }
     return {a.Hkv * a.groups, 0, 0, 0};
+}
+
+__device__ __forceinline__ PromptCut uniform(const PromptCut& x)
+{
+    return {__builtin_amdgcn_readfirstlane(x.gh), __builtin_amdgcn_readfirstlane(x.b), __builtin_amdgcn_readfirstlane(x.qb),
+            __builtin_amdgcn_readfirstlane(x.t)};
 }
 
 __device__ __forceinline__ bool cut_before(const PromptCut& x, const PromptCut& y)
@@ -1477,12 +1487,25 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
         PromptCut at, end;
         if (a.spans)
         {
-            for (int b = g; b < a.B; b += gridDim.x)
-                if (!packed_seq(a, b, it.seq)) store_nan<DK>(a, b, 0, a.H, threadIdx.x, kPThreads);
-            const PromptPlan plan = prompt_plan(a, gridDim.x);
-            at = prompt_cut(a, plan, g * plan.per);
-            end = prompt_cut(a, plan, (g + 1) * plan.per);
-            if (threadIdx.x == 0) prompt_cuts<DK>(a, a.spans)[g] = at;
+            // the span's two cuts by a wave each, while the others look for sequences that do not fit
+            const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+            PromptCut* const cuts = reinterpret_cast<PromptCut*>(smem);
+            if (wave < 2)
+            {
+                const PromptCut cut = prompt_cut(a, a.spans, g + wave);
+                if ((threadIdx.x & 63) == 0)
+                {
+                    cuts[wave] = cut;
+                    if (wave == 0) prompt_cuts<DK>(a, a.spans)[g] = cut;
+                }
+            }
+            else
+                for (int b = g; b < a.B; b += a.spans)
+                    if (PrefillSeq<true> any; !packed_seq(a, b, any)) store_nan<DK>(a, b, 0, a.H, (int)threadIdx.x - 2 * kWave, kPThreads - 2 * kWave);
+            __syncthreads();
+            at = uniform(cuts[0]);
+            end = uniform(cuts[1]);
+            __syncthreads();
         }
         else
         {
@@ -1518,7 +1541,7 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
 
 // The items that several spans share: work-group g joins the one that the cut before span g is the first to
 // fall into, from its records: sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, 16 dimensions of its 256 queries.
-// Span g - 1 wrote slot 1, those from g on that begin within the item slot 0: fewer than 40 (PromptPlan's per).
+// Span g - 1 wrote slot 1, those from g on that begin within the item slot 0: fewer than 40 (prompt_cut's per).
 template <int DK>
 __global__ __launch_bounds__(32 * kPWaves) void k_prompt_join(PrefillArgs a)
 {
