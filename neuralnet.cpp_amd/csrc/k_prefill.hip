@@ -259,7 +259,7 @@ struct PrefillTile
     static constexpr int KROW = DK + 4;                      // f32 products: padded row (floats)
     static constexpr int kF32 = 2 * kPK * KROW * 4;
     static constexpr int kMain = 2 * kBuf > kF32 ? 2 * kBuf : kF32;  // double-buffered
-    static constexpr int kBytes = kMain + 64;                // maxima of K in two tiles, the fallback flag
+    static constexpr int kBytes = kMain + 128;               // maxima of K in two tiles, the fallback flag, the waves' findings
 };
 
 // The two halves of two f32 values scaled into f16's range: x = hi + lo up to 2^-23 |x| or 2^-25
@@ -364,29 +364,38 @@ __device__ __forceinline__ void load_query(const PrefillArgs& a, const PrefillWa
     const int qt = min(w.qt, seq.n(a) - 1);
     const uint32_t q_at = (uint32_t)(((size_t)(w.head * DK + G * h) * (size_t)M + (size_t)(seq.col0(a, w) + qt)) * 4u);
     const uint32_t r_at = (uint32_t)(((size_t)(seq.pos0(a) + qt) * HALF + (size_t)(G * h)) * 4u);
+    // all elements on their way together, the tables' a group ahead of their use
+    float x[NG][2][G];
+    float4 cs[2][G / 4], sn[2][G / 4];
+    auto load_tables = [&](int c) {
+#pragma unroll
+        for (int e = 0; e < G / 4; ++e)
+        {
+            cs[c & 1][e] = ld_f4(rc, r_at + (uint32_t)(2 * G * c + 4 * e) * 4u);
+            sn[c & 1][e] = ld_f4(rs, r_at + (uint32_t)(2 * G * c + 4 * e) * 4u);
+        }
+    };
+    load_tables(0);
 #pragma unroll
     for (int c = 0; c < NG; ++c)
-    {
-        float x[2][G];
-        float4 cs[G / 4], sn[G / 4];
 #pragma unroll
         for (int e = 0; e < G; ++e)
 #pragma unroll
             for (int q = 0; q < 2; ++q)
-                x[q][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rq, q_at, (2 * G * c + e + HALF * q) * M * 4, 0));
+                x[c][q][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rq, q_at, (2 * G * c + e + HALF * q) * M * 4, 0));
 #pragma unroll
-        for (int e = 0; e < G / 4; ++e)
-        {
-            cs[e] = ld_f4(rc, r_at + (uint32_t)(2 * G * c + 4 * e) * 4u);
-            sn[e] = ld_f4(rs, r_at + (uint32_t)(2 * G * c + 4 * e) * 4u);
-        }
+    for (int c = 0; c < NG; ++c)
+    {
+        if (c + 1 < NG) load_tables(c + 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int e = 0; e < G; ++e)
         {
-            const float cv = e % 4 == 0 ? cs[e / 4].x : e % 4 == 1 ? cs[e / 4].y : e % 4 == 2 ? cs[e / 4].z : cs[e / 4].w;
-            const float sv = e % 4 == 0 ? sn[e / 4].x : e % 4 == 1 ? sn[e / 4].y : e % 4 == 2 ? sn[e / 4].z : sn[e / 4].w;
-            float y0 = x[0][e], y1 = x[1][e];
-            if (a.cosT) pf_rope(x[0][e], x[1][e], cv, sv, y0, y1);
+            const float4 c4 = cs[c & 1][e / 4], s4 = sn[c & 1][e / 4];
+            const float cv = e % 4 == 0 ? c4.x : e % 4 == 1 ? c4.y : e % 4 == 2 ? c4.z : c4.w;
+            const float sv = e % 4 == 0 ? s4.x : e % 4 == 1 ? s4.y : e % 4 == 2 ? s4.z : s4.w;
+            float y0 = x[c][0][e], y1 = x[c][1][e];
+            if (a.cosT) pf_rope(x[c][0][e], x[c][1][e], cv, sv, y0, y1);
             f(c, e, y0, y1);
         }
     }
@@ -832,6 +841,7 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
     // set to send the work-group to the f32 products: written in iteration kb (or before the loop) into
     // [(kb + 1) & 1] and read after the barrier of iteration kb + 1, so all waves read the same value
     int* sflag = reinterpret_cast<int*>(smem + Tile::kMain + 32);
+    int* sany = reinterpret_cast<int*>(smem + Tile::kMain + 64);  // [2][8]: what each wave has found at the end
 
     // (paged: opaque per item, so that no thread-index arithmetic stays alive across the items)
     int tid = threadIdx.x;
@@ -1410,6 +1420,7 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
     // V is not looked through for infinities and NaN: any that matters is in the sums. Nor for values whose smallest part would lie below bf16's range: their output is tiny then.
     l_run += __shfl_xor(l_run, 32);
     bool lost = !(l_run < __builtin_inff());
+    const int any_bad = kPaged && __builtin_amdgcn_ballot_w64(bad) != 0 ? 2 : 0;
     float faint = l_run * kPTiny;  // outputs below (but for 0) may have lost bits
     if constexpr (kHalf)
     {
@@ -1418,21 +1429,38 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
         // and come from the f32 products. (From 2^-27 on, a value that happens to be 0 sent a call in four there,
         // at the cost of five tiles each.)
         const uint32_t top = wave_max(max((uint32_t)v_top[0], (uint32_t)v_top[1]));
-        if (lane == 0) smax[wave] = is_v ? top : 0u;
+        if (lane == 0) smax[wave] = is_v ? top : 0u, sany[kPWaves + wave] = any_bad;
         __syncthreads();
         const uint32_t most = max(max(smax[0], smax[1]), max(smax[2], smax[3]));
         deep |= __shfl_xor((int)deep, 32) != 0;
         faint = deep ? l_run * ((float)__builtin_bit_cast(_Float16, (uint16_t)most) * 0x1p-32f) : -1.0f;
     }
+    {
+        // the lowest magnitude (but for zeros where those hold no lost bits), and NaN from an infinity or a NaN
+        float low = __builtin_inff(), odd = 0.0f;
+        uint32_t least = 0xFFFFFFFFu;
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+        for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int v = 0; v < 16; ++v)
-        {
-            const float y = fabsf(o[d][v]);
-            lost |= !(y < __builtin_inff()) || (y < faint && (kHalf || y != 0.0f));
-        }
-    if (__syncthreads_or(!fallback && w.live && lost) || fallback)
+            for (int v = 0; v < 16; ++v)
+            {
+                const float y = o[d][v];
+                odd = __builtin_fmaf(y, 0.0f, odd);
+                if constexpr (kHalf) low = fminf(low, fabsf(y));
+                else least = min(least, 2 * __builtin_bit_cast(uint32_t, y) - 1);
+            }
+        lost |= odd != odd;
+        if constexpr (kHalf) lost |= low < faint;
+        else lost |= faint > 0.0f && least < 2 * __builtin_bit_cast(uint32_t, faint) - 1;
+    }
+    const bool any_lost = __builtin_amdgcn_ballot_w64(!fallback && w.live && lost) != 0;
+    if (lane == 0) sany[wave] = any_lost | (kHalf ? 0 : any_bad);
+    __syncthreads();
+    int found = 0;
+#pragma unroll
+    for (int i = 0; i < (kHalf ? 2 : 1) * kPWaves; ++i) found |= sany[i];
+    found = __builtin_amdgcn_readfirstlane(found);
+    if ((found & 1) || fallback)
     {
         // everything from scratch: kept alive across the loop above, it would push that into spills
         int t2 = threadIdx.x;
@@ -1447,7 +1475,7 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
     }
     if constexpr (kPaged)
     {
-        if (__syncthreads_or(bad)) l_run = __builtin_nanf("");
+        if (found & 2) l_run = __builtin_nanf("");
         if (rec)
         {
             store_record<DK>(rec, tid, [](int d, int i) { return ND * i + d; }, [&](int d, int v) { return o[d][v]; }, m_ref, l_run);
