@@ -258,7 +258,10 @@ struct PrefillTile
     static constexpr int kBuf = kV + kVPlanes * kVPlane;
     static constexpr int KROW = DK + 4;                      // f32 products: padded row (floats)
     static constexpr int kF32 = 2 * kPK * KROW * 4;
-    static constexpr int kMain = 2 * kBuf > kF32 ? 2 * kBuf : kF32;  // double-buffered
+    static constexpr int kTPitch = DK * 2 + 16;              // rows of the cos / sin tables, before the first tile
+    static constexpr int kTables = 2 * 32 * kPWaves * kTPitch;
+    static constexpr int kMain = 2 * kBuf > kTables ? 2 * kBuf : kTables;  // double-buffered
+    static_assert(kF32 <= kMain, "");
     static constexpr int kBytes = kMain + 128;               // maxima of K in two tiles, the fallback flag, the waves' findings
 };
 
@@ -349,56 +352,54 @@ struct PrefillSeq<true>
     __device__ __forceinline__ int to(const PrefillArgs&, const PrefillWave& w) const { return max(pos0_ + w.t0 + kPQ - 1, pre - 1); }
 };
 
-// The lane's rotated query value pairs, f(c, e, value, value of the dimension DK/2 further) for its
-// dimensions 2Gc + Gh + e below DK/2. The cos / sin rows of 32 queries are 32 lines apart, so they
-// are read four at a time. Lanes past the last token repeat it (they are never stored).
-template <int DK, int G, bool kPaged, typename F>
-__device__ __forceinline__ void load_query(const PrefillArgs& a, const PrefillWave& w, const PrefillSeq<kPaged>& seq, int h, F&& f)
+// The lane's query: values x[c][0][e] of its dimensions 2Gc + Gh + e below DK/2 and x[c][1][e] of those DK/2
+// further. Lanes past the last token repeat it (they are never stored).
+template <int DK, int G>
+struct PrefillQuery
 {
-    constexpr int HALF = DK / 2, NG = HALF / (2 * G);
-    const int M = seq.cols(a);
-    const __amdgpu_buffer_rsrc_t rq = pf_rsrc(a.q, (uint32_t)((size_t)a.H * DK * (size_t)M * 4u));
-    const uint32_t rope_bytes = a.cosT ? (uint32_t)((size_t)a.max_len * HALF * 4u) : 0u;  // (paged: max_len = limit)
-    const __amdgpu_buffer_rsrc_t rc = pf_rsrc(a.cosT ? a.cosT : a.q, rope_bytes);
-    const __amdgpu_buffer_rsrc_t rs = pf_rsrc(a.cosT ? a.sinT : a.q, rope_bytes);
-    const int qt = min(w.qt, seq.n(a) - 1);
-    const uint32_t q_at = (uint32_t)(((size_t)(w.head * DK + G * h) * (size_t)M + (size_t)(seq.col0(a, w) + qt)) * 4u);
-    const uint32_t r_at = (uint32_t)(((size_t)(seq.pos0(a) + qt) * HALF + (size_t)(G * h)) * 4u);
-    // all elements on their way together, the tables' a group ahead of their use
+    static constexpr int HALF = DK / 2, NG = HALF / (2 * G);
     float x[NG][2][G];
-    float4 cs[2][G / 4], sn[2][G / 4];
-    auto load_tables = [&](int c) {
-#pragma unroll
-        for (int e = 0; e < G / 4; ++e)
-        {
-            cs[c & 1][e] = ld_f4(rc, r_at + (uint32_t)(2 * G * c + 4 * e) * 4u);
-            sn[c & 1][e] = ld_f4(rs, r_at + (uint32_t)(2 * G * c + 4 * e) * 4u);
-        }
-    };
-    load_tables(0);
-#pragma unroll
-    for (int c = 0; c < NG; ++c)
-#pragma unroll
-        for (int e = 0; e < G; ++e)
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-                x[c][q][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rq, q_at, (2 * G * c + e + HALF * q) * M * 4, 0));
-#pragma unroll
-    for (int c = 0; c < NG; ++c)
+    template <bool kPaged>
+    __device__ __forceinline__ void load(const PrefillArgs& a, const PrefillWave& w, const PrefillSeq<kPaged>& seq, int h)
     {
-        if (c + 1 < NG) load_tables(c + 1);
-        __builtin_amdgcn_sched_barrier(0);
+        const int M = seq.cols(a);
+        const __amdgpu_buffer_rsrc_t rq = pf_rsrc(a.q, (uint32_t)((size_t)a.H * DK * (size_t)M * 4u));
+        const int qt = min(w.qt, seq.n(a) - 1);
+        const uint32_t q_at = (uint32_t)(((size_t)(w.head * DK + G * h) * (size_t)M + (size_t)(seq.col0(a, w) + qt)) * 4u);
 #pragma unroll
-        for (int e = 0; e < G; ++e)
-        {
-            const float4 c4 = cs[c & 1][e / 4], s4 = sn[c & 1][e / 4];
-            const float cv = e % 4 == 0 ? c4.x : e % 4 == 1 ? c4.y : e % 4 == 2 ? c4.z : c4.w;
-            const float sv = e % 4 == 0 ? s4.x : e % 4 == 1 ? s4.y : e % 4 == 2 ? s4.z : s4.w;
-            float y0 = x[c][0][e], y1 = x[c][1][e];
-            if (a.cosT) pf_rope(x[c][0][e], x[c][1][e], cv, sv, y0, y1);
-            f(c, e, y0, y1);
-        }
+        for (int c = 0; c < NG; ++c)
+#pragma unroll
+            for (int e = 0; e < G; ++e)
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    x[c][q][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rq, q_at, (2 * G * c + e + HALF * q) * M * 4, 0));
     }
+    // f(c, e, rotated values), with cs(c, i) and sn(c, i) = the tables at dimensions 2Gc + Gh + 4i .. + 3
+    template <typename C, typename S, typename F>
+    __device__ __forceinline__ void rotate(const PrefillArgs& a, C&& cs, S&& sn, F&& f) const
+    {
+#pragma unroll
+        for (int c = 0; c < NG; ++c)
+#pragma unroll
+            for (int i = 0; i < G / 4; ++i)
+            {
+                float4 c4 = make_float4(1.0f, 1.0f, 1.0f, 1.0f), s4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (a.cosT) c4 = cs(c, i), s4 = sn(c, i);
+                const float cv[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                {
+                    float y0 = x[c][0][4 * i + e], y1 = x[c][1][4 * i + e];
+                    if (a.cosT) pf_rope(y0, y1, cv[e], sv[e], y0, y1);
+                    f(c, 4 * i + e, y0, y1);
+                }
+            }
+    }
+};
+
+__device__ __forceinline__ uint32_t rope_bytes(const PrefillArgs& a, int half)
+{
+    return a.cosT ? (uint32_t)((size_t)a.max_len * half * 4u) : 0u;  // (paged: max_len = limit)
 }
 
 // out[head*DK + i][m] = y(d, v) for the lane's query: element v of block d belongs to row
@@ -477,7 +478,14 @@ __device__ void attend_f32(const PrefillArgs& a, const PrefillWave& w, const Pre
     float* vs = ks + kPK * KROW;
     bool bad = false;  // a page outside the pool
     float qv[DK / 2];  // qv[4c + e] = rotated query value of dimension 8c + 4h + e
-    load_query<DK, 4>(a, w, seq, h, [&](int c, int e, float y0, float y1) {
+    PrefillQuery<DK, 4> query;
+    query.load(a, w, seq, h);
+    const __amdgpu_buffer_rsrc_t rc = pf_rsrc(a.cosT ? a.cosT : a.q, rope_bytes(a, DK / 2));
+    const __amdgpu_buffer_rsrc_t rs = pf_rsrc(a.cosT ? a.sinT : a.q, rope_bytes(a, DK / 2));
+    const uint32_t r_at = (uint32_t)(((size_t)(seq.pos0(a) + min(w.qt, seq.n(a) - 1)) * (DK / 2) + (size_t)(4 * h)) * 4u);
+    auto table = [&](__amdgpu_buffer_rsrc_t r, int c, int i) { return ld_f4(r, r_at + (uint32_t)(8 * c + 4 * i) * 4u); };
+    query.rotate(a, [&](int c, int i) { return table(rc, c, i); }, [&](int c, int i) { return table(rs, c, i); },
+                 [&](int c, int e, float y0, float y1) {
         qv[4 * c + e] = y0;
         qv[4 * (c + NC / 2) + e] = y1;
     });
@@ -863,9 +871,6 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
     const __amdgpu_buffer_rsrc_t rk = pf_rsrc(static_cast<const CT*>(a.kc) + seq_off, seq_bytes);
     const __amdgpu_buffer_rsrc_t rv = pf_rsrc(static_cast<const CT*>(a.vc) + seq_off, seq_bytes);
 
-    if (tid < 2) sflag[tid] = tid == (kb0 & 1) ? a.f32 : 0;
-    __syncthreads();
-
     // ---- staging, 16 elements per thread: waves 0-3 take V (thread = 4 keys x ND dimensions), waves
     // 4-7 take K (thread = KU chunks of 8 dimensions of a key). raw holds them as loaded.
     constexpr int RW = F32C ? 16 : 8;  // words
@@ -1134,7 +1139,41 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
         }
     };
 
+    // ---- everything that the first tile waits for on its way together: rows of the cos / sin tables, page ids,
+    // queries, then (with the ids) keys and values. The tables' rows of the work-group's queries are one run; from
+    // registers a lane's row would be read in lines of its own, 16 bytes at a time, by every head again.
+    const int qn = kPQ << (kPWaveShift - log2_heads(a));
+    constexpr int TC = DK / 8, TU = 32 * kPWaves * TC / kPThreads;  // 16-byte chunks of a row, those of a thread at most
+    float4 tc[TU], ts[TU];
+    if (a.cosT)
+    {
+        const __amdgpu_buffer_rsrc_t rc = pf_rsrc(a.cosT, rope_bytes(a, DK / 2)), rs = pf_rsrc(a.sinT, rope_bytes(a, DK / 2));
+        const uint32_t t_at = (uint32_t)(seq.pos0(a) + item.qb * qn) * (uint32_t)(DK * 2) + (uint32_t)tid * 16u;
+#pragma unroll
+        for (int i = 0; i < TU; ++i)
+            if (i * kPThreads < qn * TC)
+            {
+                tc[i] = ld_f4(rc, t_at + (uint32_t)(i * kPThreads * 16));
+                ts[i] = ld_f4(rs, t_at + (uint32_t)(i * kPThreads * 16));
+            }
+    }
     load_ids(kb0);
+    PrefillQuery<DK, 8> query;
+    if (w.live) query.load(a, w, seq, h);
+    if (a.cosT)
+    {
+#pragma unroll
+        for (int i = 0; i < TU; ++i)
+        {
+            const int ct = tid + i * kPThreads;
+            if (ct >= qn * TC) break;
+            uint8_t* dst = smem + ct / TC * Tile::kTPitch + 16 * (ct % TC);
+            *reinterpret_cast<float4*>(dst) = tc[i];
+            *reinterpret_cast<float4*>(dst + qn * Tile::kTPitch) = ts[i];
+        }
+    }
+    if (tid < 2) sflag[tid] = tid == (kb0 & 1) ? a.f32 : 0;
+    __syncthreads();
     load_raw(kb0);
 
     // ---- the lane's rotated query in halves: step c holds dimensions 16c + 8h + 0..7, scaled by 2^eq
@@ -1144,7 +1183,10 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
         float qv[DK / 2];
         uint32_t mx = 0;
         const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
-        load_query<DK, 8>(a, w, seq, h, [&](int c, int e, float y0, float y1) {
+        const uint8_t* tab = smem + (min(w.qt, seq.n(a) - 1) - item.qb * qn) * Tile::kTPitch + 32 * h;
+        auto table = [&](const uint8_t* t, int c, int i) { return *reinterpret_cast<const float4*>(t + 64 * c + 16 * i); };
+        query.rotate(a, [&](int c, int i) { return table(tab, c, i); }, [&](int c, int i) { return table(tab + qn * Tile::kTPitch, c, i); },
+                     [&](int c, int e, float y0, float y1) {
             qv[8 * c + e] = y0;
             qv[8 * (c + NC / 2) + e] = y1;
             mx = max(mx, max(__builtin_bit_cast(uint32_t, y0) & 0x7FFFFFFFu, __builtin_bit_cast(uint32_t, y1) & 0x7FFFFFFFu));
