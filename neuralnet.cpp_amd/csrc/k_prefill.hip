@@ -1588,11 +1588,12 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
             if (at.qb >= prompt_blocks(a, it.seq.n_)) return;
             end = {at.gh, at.b, at.qb + 1, 0};
         }
+        bool known = a.spans == 0;  // it.seq is at.b's
         while (cut_before(at, end))
         {
             // the next sequence with a block left
             const bool there = at.b < a.B;
-            if (!there || !packed_seq(a, at.b, it.seq) || at.qb >= prompt_blocks(a, it.seq.n_))
+            if (!there || !(known || packed_seq(a, at.b, it.seq)) || at.qb >= prompt_blocks(a, it.seq.n_))
             {
                 at = there ? PromptCut{at.gh, at.b + 1, 0, 0} : PromptCut{at.gh + 1, 0, 0, 0};
                 continue;
@@ -1604,6 +1605,7 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
             it.qb = at.qb;
             float* rec = at.t == 0 && to == tiles ? nullptr : prompt_record<DK>(a, g, at.t > 0 ? 0 : 1);
             attend<DK, kPaged, kShaped, CT>(a, it, smem, at.t, to, rec);
+            known = false;
             at = {at.gh, at.b, at.qb + 1, 0};
         }
     }
