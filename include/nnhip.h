@@ -725,7 +725,7 @@ nnhip_status nnhip_attention_pages_prefill(nnhip_ctx* ctx, const nnhip_kv_pages*
 
 /* Scratch that nnhip_attention_pages_decode (nnhip_logits_adjust_rows) of these sizes uses;
  * nnhip_attention_pages_prefill uses 2 * (dk + 2) KiB and 16 bytes for each CU where the table (and the rope tables) hold
- * more than 512 positions. The context keeps one for each stream that it was set to, grown on demand and freed with the context only, so that a
+ * more than 128 positions. The context keeps one for each stream that it was set to, grown on demand and freed with the context only, so that a
  * captured call stays valid; a call that would have to grow it during a capture fails with
  * NNHIP_ERR_UNSUPPORTED (call once before, on the capture's stream). Captured calls of one stream share
  * its scratch, wherever they are replayed: their replays must overlap neither each other nor eager calls

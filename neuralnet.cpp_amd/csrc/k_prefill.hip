@@ -378,19 +378,26 @@ struct PrefillQuery
     template <typename C, typename S, typename F>
     __device__ __forceinline__ void rotate(const PrefillArgs& a, C&& cs, S&& sn, F&& f) const
     {
+        if (!a.cosT)
+        {
+#pragma unroll
+            for (int c = 0; c < NG; ++c)
+#pragma unroll
+                for (int e = 0; e < G; ++e) f(c, e, x[c][0][e], x[c][1][e]);
+            return;
+        }
 #pragma unroll
         for (int c = 0; c < NG; ++c)
 #pragma unroll
             for (int i = 0; i < G / 4; ++i)
             {
-                float4 c4 = make_float4(1.0f, 1.0f, 1.0f, 1.0f), s4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (a.cosT) c4 = cs(c, i), s4 = sn(c, i);
+                const float4 c4 = cs(c, i), s4 = sn(c, i);
                 const float cv[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                 {
-                    float y0 = x[c][0][4 * i + e], y1 = x[c][1][4 * i + e];
-                    if (a.cosT) pf_rope(y0, y1, cv[e], sv[e], y0, y1);
+                    float y0, y1;
+                    pf_rope(x[c][0][4 * i + e], x[c][1][4 * i + e], cv[e], sv[e], y0, y1);
                     f(c, 4 * i + e, y0, y1);
                 }
             }
@@ -686,7 +693,7 @@ struct PromptCut
 {
     int gh, b, qb, t;
 };
-constexpr int kOver = 3, kSnap = 4, kShort = 16, kSpanMin = 8;
+constexpr int kOver = 3, kSnap = 2, kShort = 4, kSpanMin = 2;
 
 __device__ __forceinline__ int prompt_blocks(const PrefillArgs& a, int n)
 {
@@ -1613,7 +1620,7 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
 
 // The items that several spans share: work-group g joins the one that the cut before span g is the first to
 // fall into, from its records: sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, 16 dimensions of its 256 queries.
-// Span g - 1 wrote slot 1, those from g on that begin within the item slot 0: fewer than 40 (prompt_cut's per).
+// Span g - 1 wrote slot 1, those from g on that begin within the item slot 0: fewer than 64 (prompt_cut's per).
 template <int DK>
 __global__ __launch_bounds__(32 * kPWaves) void k_prompt_join(PrefillArgs a)
 {
