@@ -1297,32 +1297,39 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
             if constexpr (kShaped)
             {
                 const float slope2 = a.slopes ? a.slopes[w.head] * 1.44269504f : 0.0f;
-                const float away = (float)(kb * kPK + 4 * h - w.qpos);
-                // scores rarely reach the cap: the polynomial alone where none does (16 exponentials and
-                // reciprocals less)
+                // scores rarely reach the cap: a polynomial alone where none does (16 exponentials and
+                // reciprocals less), of 3 terms where none is above a quarter of it
                 const float g = a.cap2 > 0.0f ? f * a.capi2 : f;
-                bool far = false;
+                float top = 0.0f;  // (a NaN does not show, and stays one in each form)
 #pragma unroll
                 for (int v = 0; v < 16; ++v)
                 {
                     s[v] *= g;
-                    far |= !(fabsf(s[v]) <= 1.0f);
+                    const float x = s[v];
+                    top = fmaxf(top, fabsf(x));
                 }
                 if (a.cap2 > 0.0f)
                 {
-                    if (__builtin_amdgcn_ballot_w64(far) == 0)
+                    if (__builtin_amdgcn_ballot_w64(top > 0.25f) == 0)
                     {
 #pragma unroll
-                        for (int v = 0; v < 16; ++v) s[v] = a.cap2 * tanh_below1(s[v]);
+                        for (int v = 0; v < 16; ++v) s[v] = tanh_below_quarter(s[v]);
+                    }
+                    else if (__builtin_amdgcn_ballot_w64(top > 1.0f) == 0)
+                    {
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) s[v] = tanh_below1(s[v]);
                     }
                     else
                     {
 #pragma unroll
-                        for (int v = 0; v < 16; ++v) s[v] = a.cap2 * tanh_any(s[v]);
+                        for (int v = 0; v < 16; ++v) s[v] = tanh_any(s[v]);
                     }
                 }
+                // (the distance of the tile's first key and the steps from there apart: a step costs one multiply-add)
+                const float unit = a.cap2 > 0.0f ? a.cap2 : 1.0f, away = slope2 * (float)(kb * kPK + 4 * h - w.qpos);
 #pragma unroll
-                for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(slope2, away + (float)(8 * (v >> 2) + (v & 3)), s[v]);
+                for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(s[v], unit, __builtin_fmaf(slope2, (float)(8 * (v >> 2) + (v & 3)), away));
                 f = 1.0f;
             }
             float low = 0.0f;  // kHalf: the lane's lowest score (masked ones, too)
