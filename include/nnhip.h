@@ -697,7 +697,9 @@ nnhip_status nnhip_kv_pages_fill(nnhip_ctx* ctx, const nnhip_kv_pages* cache, co
  * a page outside the pool among positions [0, pos[b]]: out NaN. len_bound <= table_stride * page_size
  * and (with tables) rope_len. Two sequences of one call whose new tokens fall on one place of the pool
  * leave there, for each element, either's. Sums and softmax are f32 in an order of the kernel's own, the same in every call
- * of the same sizes and positions (compute_layer_attention.hpp:1022-1083). */
+ * of the same sizes and positions; over f16 pools with more than 4 heads to a KV head (dk 64, 128) the
+ * rotated queries go into the products with 22 bits of every element down to 2^-29 of its head's largest
+ * (compute_layer_attention.hpp:1022-1083). */
 nnhip_status nnhip_attention_pages_decode(nnhip_ctx* ctx, const nnhip_kv_pages* cache, const float* q, const float* k,
                                           const float* v, size_t B, size_t H, const int32_t* pos, size_t len_bound,
                                           const float* rope_cos, const float* rope_sin, size_t rope_len, float scale,

@@ -31,6 +31,7 @@ constexpr int kPgMaxR = 8;       // query heads of a work-group
 constexpr int kPgRec = 16;       // tail of a record: maximum[8], sum[8]
 constexpr int kPgMinChunk = 128;  // positions of a work-group at least (a multiple of 64)
 constexpr int kPgEvenB = 1024;   // sequences up to which the chunks are sized by the lengths
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 constexpr float kPgLazy = 8.0f;  // log2 growth of a maximum before its sums are rescaled
 
 struct PagesArgs
@@ -172,6 +173,18 @@ struct PagesRow
     }
 };
 
+// Lanes of 16 that hold head h's maximum, and the weight of row u and head h (k_pages_attn)
+template <bool kDots, int RT>
+constexpr int head_lane(int h)
+{
+    return kDots ? h : RT >= 4 ? h / (RT / 4) : 2 * h;
+}
+template <bool kDots, int RT>
+constexpr int score_lane(int u, int h)
+{
+    return kDots ? 8 * (u / 2) + h : 4 * u + head_lane<false, RT>(h);
+}
+
 // A barrier for LDS data only: loads of the pools stay in flight across it
 __device__ __forceinline__ void lds_barrier()
 {
@@ -236,7 +249,11 @@ __device__ __forceinline__ PagesItem find_item(const PagesArgs& a, int item, int
 // and weighted values of its own rows. q stays in registers (each lane the elements of its columns).
 //   scores   each lane multiplies its columns, the sums over 16 lanes come out spread over them
 //            (fold16): lane 4u + s holds row u's score of head(s) s, so that the cap, the bias and the
-//            exponential are computed once per score;
+//            exponential are computed once per score. 8 heads over f16 pools: 16 keys by (8 queries in two
+//            f16 parts) is one 16x16x32 product for 32 dimensions, in place of 220 of 390 VALU
+//            instructions a tile of dk 64 (37 sequences of 1 .. 16384 over 2 KV heads of 64: 25.6 -> 21.7 us with the
+//            join). 4 heads fill half of it, and the rows in lines of 64 bytes cost more than the
+//            instructions (64 x 2000 over 5 heads of 128: 71 -> 77 us), so they stay with the VALU;
 //   values   the probability of (row u, head h) is broadcast within the 16 lanes by a DPP move.
 // A head's reference maximum moves only when it has grown by 2^8.
 // The chunk that holds the new position writes its rotated key and its value to the page (no other
@@ -244,14 +261,16 @@ __device__ __forceinline__ PagesItem find_item(const PagesArgs& a, int item, int
 // Bound by HBM where the caches are large (4 x 60000 .. 131072 positions, 8 heads of 128, f16: 231 us with the
 // join, 6.4 TB/s of the bytes it cannot do without; a large copy reaches 4.9 read and written together);
 // by the chain of round trips position -> page -> rows, about 7 us in the kernel and 4 in the join,
-// where they are small (16 x 2112, 5 heads of 128, f32: 34.3 us, 4.9 TB/s; 1 x 100: 7.5 us, one launch). With 8
-// heads to a KV head of 64 in f16 the 400 VALU instructions of a tile (256 multiply-adds, 90 of
-// the fold, 32 broadcasts) take as long as its bytes.
+// where they are small (16 x 2112, 5 heads of 128, f32: 34.6 us, 4.9 TB/s; 1 x 100: 7.5 us, one launch). 8 heads to a
+// KV head of 64: by both, and the VALU instructions of the values (128 multiply-adds a tile).
 template <int DK, int RT, bool kFinal, typename CT>
 __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
 {
     using Row = PagesRow<DK, CT>;
     constexpr int E = Row::E, HALF = DK / 2, NV = RT / 4 > 1 ? RT / 4 : 1;  // scores per lane
+    constexpr bool kDots = sizeof(CT) == 2 && RT == 8;   // scores by matrix products
+    constexpr int NM = kDots ? 1 : NV;                   // heads per lane
+    constexpr int KC = DK / 32;                          // kDots: steps of a score
     constexpr int NS = kPgU * RT, QI = (RT * HALF + kPgThreads - 1) / kPgThreads;  // query pairs per thread
     __shared__ __align__(16) float q_s[RT * DK];
     __shared__ float new_s[2][DK];
@@ -309,7 +328,8 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
     const int slot_mask = (1 << a.shift) - 1;
     const CT* const kc = static_cast<const CT*>(a.kc);
     const CT* const vc = static_cast<const CT*>(a.vc);
-    Row kr[kPgU], vr[kPgU];
+    Row kr[kDots ? 1 : kPgU], vr[kPgU];
+    v8h km[kDots ? KC : 1];
     auto load = [&](int base) {
         size_t at[2];
 #pragma unroll
@@ -323,10 +343,22 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
             at[i] = page_row(in ? id : 0, g, (t0 + min(base + 8 * i, (n - 1) & ~7)) & slot_mask, a.Hkv, a.shift) * DK;
         }
         load_ids(base + kPgWaves * kPgTile);
+        if constexpr (kDots)
+        {
+            const CT* k = kc + (j & 8 ? at[1] : at[0]) + (j & 7) * DK + 8 * grp;
+            const CT* v = vc + (grp & 2 ? at[1] : at[0]) + 4 * (grp & 1) * DK;
 #pragma unroll
-        for (int u = 0; u < kPgU; ++u) kr[u].load(kc + at[u / 2] + (4 * (u & 1) + grp) * DK, j);
+            for (int i = 0; i < KC; ++i) km[i] = __builtin_nontemporal_load(reinterpret_cast<const v8h*>(k + 32 * i));
 #pragma unroll
-        for (int u = 0; u < kPgU; ++u) vr[u].load(vc + at[u / 2] + (4 * (u & 1) + grp) * DK, j);
+            for (int u = 0; u < kPgU; ++u) vr[u].load(v + u * DK, j);
+        }
+        else
+        {
+#pragma unroll
+            for (int u = 0; u < kPgU; ++u) kr[u].load(kc + at[u / 2] + (4 * (u & 1) + grp) * DK, j);
+#pragma unroll
+            for (int u = 0; u < kPgU; ++u) vr[u].load(vc + at[u / 2] + (4 * (u & 1) + grp) * DK, j);
+        }
     };
 
     // ---- rotated queries, the new key and value
@@ -370,25 +402,89 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
         }
     }
 
-    float q[RT][E];
+    // This lane's scores: row (lane / 4) % 4 of its 16 lanes' four and heads hs .. hs + NV - 1; kDots: two rows from
+    // 2 (lane / 8 % 2) on, and head hs = lane % 8.
+    const int hs = kDots ? j & 7 : RT >= 4 ? (j & 3) * NV : RT == 2 ? (j & 3) >> 1 : 0, ur = j >> 2;
+    auto row_at = [&](int i) { return kDots ? 4 * grp + 2 * (j >> 3) + i : 4 * ur + grp; };  // in the tile
+    float q[kDots ? 1 : RT][kDots ? 1 : E];
+    // kDots: columns 0 .. 7 of the products are the heads' queries in f16, columns 8 .. 15 what that leaves,
+    // q = (hi + lo 2^-11) 2^(e - 14): 22 bits of every element down to 2^-29 of its head's largest, and of
+    // smaller ones what is above 2^-51 of that. The products of f16 keys with them are exact, their sums f32.
+    const bool lo_col = (j & 8) != 0;
+    v8h qm[kDots ? KC : 1];
+    float unit = 1.0f;
+    if constexpr (kDots)
+    {
+        float x[KC][8];
+        uint32_t mx = 0;
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
+        for (int c = 0; c < KC; ++c)
 #pragma unroll
-        for (int e = 0; e < E; ++e) q[r][e] = q_s[r * DK + Row::dim(e, j)];
-    // this lane's scores: row (lane / 4) % 4, heads hs .. hs + NV - 1
-    const int hs = RT >= 4 ? (j & 3) * NV : RT == 2 ? (j & 3) >> 1 : 0, ur = j >> 2;
-    float slope2[NV];
+            for (int i = 0; i < 8; ++i)
+            {
+                x[c][i] = q_s[hs * DK + 32 * c + 8 * grp + i];
+                mx = max(mx, __builtin_bit_cast(uint32_t, x[c][i]) & 0x7FFFFFFFu);
+            }
+        mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16, kWave));
+        mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32, kWave));
+        const int e = min(max((int)(mx >> 23) - 127, -85), 127);
+        const float up = __builtin_bit_cast(float, (uint32_t)(127 + 14 - e) << 23);  // the largest is below 2^15
+        unit = __builtin_bit_cast(float, (uint32_t)(127 - 14 + e) << 23);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) slope2[i] = a.slopes && hs + i < R ? a.slopes[h0 + hs + i] * 1.44269504f : 0.0f;
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+            {
+                const float y = x[c][i] * up;
+                const _Float16 hi = (_Float16)y;
+                const float rest = y - (float)hi;  // (NaN beside an infinity, which hi says)
+                qm[c][i] = lo_col ? (_Float16)(rest == rest ? rest * 0x1p11f : 0.0f) : hi;
+            }
+    }
+    else
+    {
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int e = 0; e < E; ++e) q[r][e] = q_s[r * DK + Row::dim(e, j)];
+    }
+    // 16 keys' products with the lane's column, of which it has four rows; then the scores of two of them: a hi
+    // lane and its lo lane exchange the others
+    auto dots = [&](const v8h(&k)[kDots ? KC : 1], float(&x)[NV]) {
+        typedef float v4f __attribute__((ext_vector_type(4)));
+        v4f d = v4f{};
+#pragma unroll
+        for (int c = 0; c < (kDots ? KC : 1); ++c) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[c], qm[c], d, 0, 0, 0);
+        const float y[4] = {d[0], d[1], d[2], d[3]};
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+        {
+            const float got = dpp<kDppRor8>(lo_col ? y[i] : y[2 + i]);
+            x[i] = lo_col ? __builtin_fmaf(y[2 + i], 0x1p-11f, got) : __builtin_fmaf(got, 0x1p-11f, y[i]);
+        }
+    };
+    // over the lanes of 16 that hold the same heads
+    auto same_max = [&](float x) {
+        x = fmaxf(x, dpp<kDppRor8>(x));
+        return kDots ? x : fmaxf(x, dpp<kDppRor4>(x));
+    };
+    auto same_sum = [&](float x) {
+        x += dpp<kDppRor8>(x);
+        return kDots ? x : x + dpp<kDppRor4>(x);
+    };
+    const float scale2 = a.scale2 * unit, capi = a.capi * unit;
+    float slope2[NM];
+#pragma unroll
+    for (int i = 0; i < NM; ++i) slope2[i] = a.slopes && hs + i < R ? a.slopes[h0 + hs + i] * 1.44269504f : 0.0f;
     auto shape = [&](float dot, int i, int t) {
-        float x = a.cap2 > 0.0f ? a.cap2 * tanh_any(dot * a.capi) : dot * a.scale2;
-        if (a.slopes) x = __builtin_fmaf(slope2[i], (float)(t - p), x);
+        float x = a.cap2 > 0.0f ? a.cap2 * tanh_any(dot * capi) : dot * scale2;
+        if (a.slopes) x = __builtin_fmaf(slope2[kDots ? 0 : i], (float)(t - p), x);
         return x;
     };
 
-    float acc[RT][E], m[NV], l[NV];
+    float acc[RT][E], m[NM], l[NM];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) m[i] = -__builtin_inff(), l[i] = 0.0f;
+    for (int i = 0; i < NM; ++i) m[i] = -__builtin_inff(), l[i] = 0.0f;
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -396,35 +492,46 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
 
     auto tile = [&](int base) {
         const bool part = base + kPgTile > n;  // rows behind the chunk's last one
-        float s[NS];
+        float x[NV], top[NM];
+        if constexpr (kDots) dots(km, x);
+        else
+        {
+            float s[NS];
 #pragma unroll
-        for (int u = 0; u < kPgU; ++u)
+            for (int u = 0; u < kPgU; ++u)
 #pragma unroll
-            for (int r = 0; r < RT; ++r)
-            {
-                float d = kr[u].get(0) * q[r][0];
+                for (int r = 0; r < RT; ++r)
+                {
+                    float d = kr[u].get(0) * q[r][0];
 #pragma unroll
-                for (int e = 1; e < E; ++e) d = __builtin_fmaf(kr[u].get(e), q[r][e], d);
-                s[u * RT + r] = d;
-            }
-        fold16(s, lane);
-        float x[NV], top[NV];
+                    for (int e = 1; e < E; ++e) d = __builtin_fmaf(kr[u].get(e), q[r][e], d);
+                    s[u * RT + r] = d;
+                }
+            fold16(s, lane);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) x[i] = s[i];
+        }
         bool grown = false;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
         {
-            const int tl = base + 4 * ur + grp;
-            x[i] = shape(s[i], i, t0 + tl);
+            const int tl = base + row_at(i);
+            x[i] = shape(x[i], i, t0 + tl);
             if (part && tl >= n) x[i] = -__builtin_inff();
-            top[i] = fmaxf(x[i], dpp<kDppRor8>(x[i]));
-            top[i] = fmaxf(top[i], dpp<kDppRor4>(top[i]));
+            if (kDots && i > 0) top[0] = fmaxf(top[0], x[i]);
+            else top[kDots ? 0 : i] = x[i];
+        }
+#pragma unroll
+        for (int i = 0; i < NM; ++i)
+        {
+            top[i] = same_max(top[i]);
             grown |= top[i] > m[i] + kPgLazy;
         }
         if (__builtin_amdgcn_ballot_w64(grown) != 0)
         {
-            float corr[NV];
+            float corr[NM];
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
+            for (int i = 0; i < NM; ++i)
             {
                 const float to = top[i] > m[i] + kPgLazy ? top[i] : m[i];
                 corr[i] = m[i] == to ? 1.0f : __builtin_amdgcn_exp2f(m[i] - to);
@@ -433,7 +540,7 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
             }
             static_for<RT>([&](auto r) {
                 constexpr int h = decltype(r)::value;
-                const float f = bcast16<RT >= 4 ? h / NV : 2 * h>(corr[h % NV]);
+                const float f = bcast16<head_lane<kDots, RT>(h)>(corr[h % NM]);
 #pragma unroll
                 for (int e = 0; e < E; ++e) acc[h][e] *= f;
             });
@@ -443,18 +550,18 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
         for (int i = 0; i < NV; ++i)
         {
             // no score above -inf yet: nothing to add (and no -inf - -inf)
-            pr[i] = x[i] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x[i] - m[i]);
-            l[i] += pr[i];
+            pr[i] = x[i] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x[i] - m[kDots ? 0 : i]);
+            l[kDots ? 0 : i] += pr[i];
         }
         if (part)  // whatever is there: 0 * it has to be 0
 #pragma unroll
             for (int u = 0; u < kPgU; ++u)
-                if (base + 4 * u + grp >= n) vr[u].zero();
+                if (base + (kDots ? 4 * grp + u : 4 * u + grp) >= n) vr[u].zero();
         static_for<kPgU>([&](auto uu) {
             constexpr int u = decltype(uu)::value;
             static_for<RT>([&](auto r) {
                 constexpr int h = decltype(r)::value;
-                const float f = bcast16<4 * u + (RT >= 4 ? h / NV : 2 * h)>(pr[h % NV]);
+                const float f = bcast16<score_lane<kDots, RT>(u, h)>(pr[kDots ? u % NV : h % NV]);
 #pragma unroll
                 for (int e = 0; e < E; ++e) acc[h][e] = __builtin_fmaf(f, vr[u].get(e), acc[h][e]);
             });
@@ -471,34 +578,49 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
     // ---- the new position: one more row, of the first group of the wave whose turn it is
     if (has_new && w == (n + kPgTile - 1) / kPgTile % kPgWaves)
     {
-        float s[NS];
-#pragma unroll
-        for (int u = 0; u < kPgU; ++u)
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-            {
-                float d = 0.0f;
-#pragma unroll
-                for (int e = 0; e < E; ++e) d = __builtin_fmaf(new_s[0][Row::dim(e, j)], q[r][e], d);
-                s[u * RT + r] = d;
-            }
-        fold16(s, lane);
-        float corr[NV], pr[NV];
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
+        float x[NV];
+        if constexpr (kDots)
         {
-            const float x = grp == 0 ? shape(s[i], i, p) : -__builtin_inff();
-            const float to = x > m[i] ? x : m[i];
+            v8h k[KC];
+#pragma unroll
+            for (int c = 0; c < KC; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) k[c][i] = (_Float16)new_s[0][32 * c + 8 * grp + i];
+            dots(k, x);
+        }
+        else
+        {
+            float s[NS];
+#pragma unroll
+            for (int u = 0; u < kPgU; ++u)
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+                {
+                    float d = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) d = __builtin_fmaf(new_s[0][Row::dim(e, j)], q[r][e], d);
+                    s[u * RT + r] = d;
+                }
+            fold16(s, lane);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) x[i] = s[i];
+        }
+        float corr[NM], pr[NM];
+#pragma unroll
+        for (int i = 0; i < NM; ++i)
+        {
+            x[i] = grp == 0 ? shape(x[i], i, p) : -__builtin_inff();
+            const float to = x[i] > m[i] ? x[i] : m[i];
             corr[i] = m[i] == to ? 1.0f : __builtin_amdgcn_exp2f(m[i] - to);
-            pr[i] = x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x - to);
+            pr[i] = x[i] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x[i] - to);
             // every row of lanes holds the same score: it counts once
-            l[i] = l[i] * corr[i] + (ur == 0 ? pr[i] : 0.0f);
+            l[i] = l[i] * corr[i] + ((kDots ? j < RT : ur == 0) ? pr[i] : 0.0f);
             m[i] = to;
         }
         static_for<RT>([&](auto r) {
             constexpr int h = decltype(r)::value;
-            const float f = bcast16<RT >= 4 ? h / NV : 2 * h>(corr[h % NV]);
-            const float y = bcast16<RT >= 4 ? h / NV : 2 * h>(pr[h % NV]);
+            const float f = bcast16<head_lane<kDots, RT>(h)>(corr[h % NM]);
+            const float y = bcast16<head_lane<kDots, RT>(h)>(pr[h % NM]);
 #pragma unroll
             for (int e = 0; e < E; ++e)
                 acc[h][e] = __builtin_fmaf(y, grp == 0 ? new_s[1][Row::dim(e, j)] : 0.0f, acc[h][e] * f);
@@ -507,11 +629,10 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
 
     // ---- join: maxima and sums of the 16 groups of lanes, then their weighted values
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NM; ++i)
     {
-        l[i] += dpp<kDppRor8>(l[i]);
-        l[i] += dpp<kDppRor4>(l[i]);
-        if (ur == 0)
+        l[i] = same_sum(l[i]);
+        if (kDots ? j < RT : ur == 0)
         {
             ml_s[0][4 * w + grp][hs + i] = m[i];
             ml_s[1][4 * w + grp][hs + i] = l[i];

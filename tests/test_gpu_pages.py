@@ -92,7 +92,7 @@ def attend64(q, K, V, scale, cap, slope, dist, see):
 
 
 def check_decode(ctx, nnhip, B, H, Hkv, dk, page, pos, f16, rope=True, cap=0.0, slopes=False, tokens=True, seed=0,
-                 len_bound=None, spread=1.0):
+                 len_bound=None, spread=1.0, edit=None):
     print(f"decode B={B} H={H} Hkv={Hkv} dk={dk} page={page} pos={list(pos)[:8]} f16={f16} cap={cap} slopes={slopes} "
           f"tokens={tokens}", flush=True)
     rng = np.random.default_rng(seed + 1000 * dk + H)
@@ -104,6 +104,8 @@ def check_decode(ctx, nnhip, B, H, Hkv, dk, page, pos, f16, rope=True, cap=0.0, 
             c.set(b, p, np.full((Hkv, dk), np.nan), np.full((Hkv, dk), np.nan))
     q = (spread * rng.standard_normal((B, H, dk))).astype(np.float32)
     k, v = (rng.standard_normal((B, Hkv, dk)).astype(np.float32) for _ in range(2))
+    if edit is not None:
+        edit(c, q, k)
     cos, sin = nnhip.rope_table(dk, bound) if rope else (None, None)
     sl = (2.0 ** (-8.0 * (np.arange(H) + 1) / H)).astype(np.float32) if slopes else None
     scale = float(np.float32(1 / math.sqrt(dk)))
@@ -161,6 +163,44 @@ def test_decode_large_scores(ctx, nnhip):
     """Scores of hundreds: the softmax is nearly a choice, the sums move their reference often."""
     check_decode(ctx, nnhip, 2, 4, 1, 128, 64, [200, 1500], True, seed=5, spread=60.0)
     check_decode(ctx, nnhip, 2, 4, 1, 128, 64, [200, 1500], False, seed=6, spread=60.0)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("H,Hkv,dk", [(8, 1, 64), (16, 2, 128), (6, 1, 64), (4, 1, 128)])
+def test_decode_query_range(ctx, nnhip, H, Hkv, dk, f16):
+    """Heads of all magnitudes, and in each an element far above the others where the keys are 0: the score is
+    that of the small elements, held to their own size (no term of the bound knows the large one)."""
+
+    def edit(c, q, k):
+        c.k[..., 0] *= 0  # (NaN stays where nothing is)
+        k[..., 0] = 0
+        q *= (10.0 ** np.linspace(-30, 1, H))[None, :, None].astype(np.float32)
+        q[..., 0] = 2.0 ** 18 * np.abs(q).max(-1)
+
+    check_decode(ctx, nnhip, 2, H, Hkv, dk, 16, [140, 517], f16, rope=False, seed=8, edit=edit)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_decode_infinite_query(ctx, nnhip, f16):
+    """An infinite element of a head's query against keys of one sign: all scores -infinity give zeros, all +infinity
+    NaN, and the other heads do not see it."""
+    import torch
+    rng = np.random.default_rng(9)
+    B, H, dk, n = 1, 8, 64, 300
+    c = Cache(rng, [n + 1], 1, 16, dk, f16)
+    c.k[..., 0] = np.abs(c.k[..., 0]) + c.dt(0.1)
+    q, k, v = (rng.standard_normal((B, h, dk)).astype(np.float32) for h in (H, 1, 1))
+    k[..., 0] = 1.0
+    ref = None
+    for q3, q5 in ((0.5, 0.5), (-np.inf, np.inf)):
+        q[0, 3, 0], q[0, 5, 0] = q3, q5
+        out = host(ctx.attention_pages_decode(c.on_device(nnhip), dev(q.reshape(B, -1)), dev(k.reshape(B, -1)),
+                                              dev(v.reshape(B, -1)), H, dev(np.array([n], np.int32)), n + 1, 0.125,
+                                              tokens=True)).reshape(H, dk)
+        if ref is None:
+            ref = out
+    rest = [h for h in range(H) if h not in (3, 5)]
+    assert np.all(out[3] == 0) and np.all(np.isnan(out[5])) and same(out[rest], ref[rest])
 
 
 def test_decode_long(ctx, nnhip):
