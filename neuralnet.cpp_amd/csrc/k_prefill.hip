@@ -46,7 +46,7 @@
 // Work-groups are issued heaviest first (the last query blocks attend over the most keys).
 // V's four waves convert their part of the next tile behind their products, K's before them: every SIMD
 // has one wave of each, and one's VALU phases fall on the other's MFMA phases (4 x 2048 tokens f32 caches
-// 389 -> 367 us, f16 280 -> 273, back to back on one box).
+// 389 -> 367 us, f16 280 -> 273, back to back on one box; 363 and 269 with the queries as below).
 // Measured before that (calls back to back in a graph, us, f32 products / here): f32 caches 4 x 2048 tokens
 // 809 / 398, 3 x 1111 at 517 411 / 202, 16 x 2048 3088 / 1498, 1 x 64 22.5 / 17.7; f16 caches 817 / 293,
 // 421 / 146, 3153 / 1121, 22.7 / 15.9. Two f16 halves for P and V too (at the cost above) took 295 and
@@ -63,8 +63,10 @@
 //     2^-51 of that one below; two MFMAs instead of five and no splitting of V (688 -> 579 us). Weights of
 //     one tile share an exponent with each other here, never with values; where heavy keys' values are 0, and
 //     lost bits could show, the f32 products run.
-// prompt of 4 x 700 .. 1024 tokens at position 6144, 20 heads over 5 of 128, f16: 579 us, 396 TFLOP/s of the
-// attention's own products; 8 x 77 .. 1900 tokens, 16 heads over 2 of 64, f32, capped and biased: 139 us.
+//   * A block of queries costs about four tiles besides its own: its queries (128 KB for dk 128, into one CU), their
+//     rotation and splitting, and the check at its end. What it waits for is on its way together.
+// 4 x 700 .. 1024 tokens at position 6144, 20 heads over 5 of 128, f16: 555 us with the join (20), 410 TFLOP/s of the
+// attention's own products; 8 x 77 .. 1900 tokens, 16 heads over 2 of 64, f32, capped and biased: 110 .. 120 us.
 // Bound by the VALU and MFMA work of a tile, which two waves to a SIMD overlap in part.
 // Caches of f16 elements (compute = F16): the fill rounds the rotated keys and the values to the
 // nearest f16 (ties to even), as the decode append does.
