@@ -262,15 +262,18 @@ class Decoder:
 
     def prefill_packed(self, ids, cu, t_bound: int, pos0=None, hook=None):
         """Prompts of unlike lengths into paged caches: ids (M,) int32 holds the tokens of sequence b in
-        ids[cu[b] .. cu[b+1] - 1] (cu (B + 1,) int32 device; every sequence has at least one and at most t_bound), at
-        positions pos0[b] on (pos0 (B,) int32 device, None: 0). Every token gets the result of its own step(). hook
-        as prefill(). Returns (logits (vocab, B), greedy ids (B,)) of each sequence's last token."""
+        ids[cu[b] .. cu[b+1] - 1] (cu (B + 1,) int32 device, at most t_bound each), at positions pos0[b] on (pos0 (B,)
+        int32 device, None: 0). Every token gets the result of its own step(). hook as prefill(). Returns (logits
+        (vocab, B), greedy ids (B,)) of each sequence's last token; those of a sequence without tokens (a slot
+        whose cache stays as it is) mean nothing."""
         import torch
         cfg, ctx = self.cfg, self.ctx
         if not self.paged:
             raise _pkg().NNHipError(1, "prefill_packed needs paged caches")
         if tuple(cu.shape) != (self.B + 1,):
             raise _pkg().NNHipError(1, f"cu must have shape ({self.B + 1},)")
+        if ids.shape[0] < 1:
+            raise _pkg().NNHipError(1, "prefill_packed needs a token")
         pf = self._prefill_buffers(ids.shape[0])
 
         def attend(i):
@@ -280,7 +283,8 @@ class Decoder:
                                         sin=self.sin, out=pf["a"])
 
         x = self._prefill_blocks(ids, ids.shape[0], attend, hook)
-        torch.index_select(x, 1, (cu[1:] - 1).long(), out=self.x)
+        # (an empty first sequence, or offsets past the tokens, would be an index outside x)
+        torch.index_select(x, 1, (cu[1:] - 1).clamp(0, ids.shape[0] - 1).long(), out=self.x)
         return self._prefill_head()
 
     def _mm(self, lin: Linear, out):

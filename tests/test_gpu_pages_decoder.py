@@ -130,6 +130,36 @@ def test_packed_prompts_then_steps(ctx, nnhip, B, f16, sub):
         m.same_pools()
 
 
+def test_packed_prompts_with_empty_slots(ctx, nnhip):
+    """Slots without new tokens (the first and the last among them) beside prompts: the prompts' logits, ids and
+    cached rows are those of a call of all slots, the empty slots' pages stay."""
+    import torch
+    from nnhip_py import decoder as dmod
+    rng = np.random.default_rng(77)
+    cfg = dmod.Config(d=256, H=4, Hkv=2, F=320, vocab=97, max_len=96, act=0, eps=1e-5)
+    B, L, lens = 5, 2, [7, 20, 3, 33, 1]
+    base = _gpu_model(ctx, nnhip, cfg, L, B, 0x9F, subln=True)[0]
+    ids = [rng.integers(0, cfg.vocab, n).astype(np.int32) for n in lens]
+    found = []
+    for live in ([0, 1, 2, 3, 4], [1, 3]):
+        m = Mirror(nnhip, cfg, L, B, 16, 6, False, np.random.default_rng(5))
+        dec = dmod.Decoder(ctx, cfg, base.blocks, base.emb, base.g_final, base.head, B, caches=m.caches)
+        n = [len(ids[b]) if b in live else 0 for b in range(B)]
+        cu = np.concatenate(([0], np.cumsum(n))).astype(np.int32)
+        logits, got = dec.prefill_packed(dev(np.concatenate([ids[b] for b in live])), dev(cu), max(n))
+        found.append((host(logits)[:, [1, 3]].copy(), host(got)[[1, 3]].copy(), [(host(c.k), host(c.v)) for c in m.caches]))
+    assert np.array_equal(found[0][0], found[1][0]) and np.array_equal(found[0][1], found[1][1])
+    for (k0, v0), (k1, v1) in zip(found[0][2], found[1][2]):
+        for b in range(B):
+            for t in range(lens[b]):
+                page, s = m.table[b, t // 16], t % 16
+                for x, y in ((k0, k1), (v0, v1)):
+                    if b in (1, 3):
+                        assert same(x[page, :, s], y[page, :, s])
+                    else:
+                        assert np.all(np.isnan(y[page, :, s]))
+
+
 def test_captured_step(nnhip):
     """A step over paged caches with its choice, captured once and replayed between eager work, continues as
     the eager steps do."""
