@@ -198,6 +198,25 @@ def test_unaligned_and_rows(ctx, nnhip):
     assert same(host(out), y) and np.array_equal(host(ids), want)
 
 
+def test_rows_past_32_bits(ctx, nnhip):
+    """More than 2^31 logits: the last rows' choices and adjusted logits."""
+    import torch
+    V, B = 131071, 16500
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.empty(B, V, dtype=torch.float32, device="cuda")
+    x.uniform_(-1, 1, generator=g)
+    bias = torch.zeros(1, V, dtype=torch.float32, device="cuda")
+    bias[0, ::2] = -3.0
+    ids = torch.empty(B, dtype=torch.int32, device="cuda")
+    ctx.logits_adjust_rows(x, nnhip.LogitRules(V, bias=bias), ids=ids, out=x)
+    tail = x[-300:]
+    assert torch.equal(ids[-300:].long(), tail.argmax(1)) and bool((ids % 2 == 1).all())
+    assert float(tail[:, ::2].max()) <= -2.0 and float(tail[:, ::2].min()) >= -4.0
+    assert float(tail[:, 1::2].min()) >= -1.0
+    del x, tail
+    torch.cuda.empty_cache()
+
+
 def test_token_counts(ctx, nnhip):
     rng = np.random.default_rng(11)
     lens, V = [0, 1, 700, 0, 33], 50

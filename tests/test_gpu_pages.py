@@ -673,6 +673,41 @@ def test_prompt_then_decode(ctx, nnhip):
     assert np.max(np.abs(one - out[:, last])) <= 64 * U * np.max(np.abs(host(v)))
 
 
+@pytest.mark.parametrize("f16", [False, True])
+def test_pools_past_32_bits(ctx, nnhip, f16):
+    """Pages whose elements lie past 2^31 and 2^32 of the pool's: the same bits as from a pool of those pages alone."""
+    import torch
+    rng = np.random.default_rng(52)
+    dt = torch.float16 if f16 else torch.float32
+    B, H, Hkv, dk, page, n = 2, 8, 2, 128, 64, 300
+    need = -(-(n + 1) // page)
+    many = 2 ** 32 // (Hkv * page * dk) + 2 * B * need
+    assert many * Hkv * page < 2 ** 31
+    few = rng.permutation(B * need).astype(np.int32).reshape(B, need)
+    places = (few * ((many - 1) // (B * need - 1))).astype(np.int32)  # from the first to the last of the pool
+    cu = dev(np.arange(B + 1, dtype=np.int32) * n)
+    q, k, v = (dev(rng.standard_normal((h * dk, B * n)).astype(np.float32)) for h in (H, Hkv, Hkv))
+    qd, kd, vd = (dev(rng.standard_normal((h * dk, B)).astype(np.float32)) for h in (H, Hkv, Hkv))
+    pos = dev(np.full(B, n, np.int32))
+    cos, sin = (dev(x) for x in nnhip.rope_table(dk, n + 1))
+    found = []
+    for pages, table in ((B * need, few), (many, places)):
+        pools = [torch.empty(pages, Hkv, page, dk, dtype=dt, device="cuda") for _ in range(2)]
+        cache = nnhip.KVPages(*pools, dev(table))
+        ctx.kv_pages_fill(cache, k, v, cu, cos=cos, sin=sin)
+        a = host(ctx.attention_pages_prefill(cache, q, cu, n, H, 0.09, cos=cos, sin=sin))
+        d = host(ctx.attention_pages_decode(cache, qd, kd, vd, H, pos, n + 1, 0.09, cos=cos, sin=sin))
+        rows = [host(p[torch.from_numpy(table.reshape(-1).astype(np.int64)).cuda()])[:, :, :] for p in pools]
+        last = (n + 1) % page or page
+        kept = [r.reshape(B, need, Hkv, page, dk) for r in rows]
+        found.append((a, d, [r[:, :-1] for r in kept], [r[:, -1, :, :last] for r in kept]))
+        del pools, cache
+    assert same(found[0][0], found[1][0]) and same(found[0][1], found[1][1])
+    for i in (2, 3):
+        for x, y in zip(found[0][i], found[1][i]):
+            assert same(np.ascontiguousarray(x), np.ascontiguousarray(y))
+
+
 def test_refusals(ctx, nnhip):
     import torch
     f = dict(dtype=torch.float32, device="cuda")
