@@ -251,7 +251,7 @@ __device__ __forceinline__ PagesItem find_item(const PagesArgs& a, int item, int
 //            (fold16): lane 4u + s holds row u's score of head(s) s, so that the cap, the bias and the
 //            exponential are computed once per score. 8 heads over f16 pools: 16 keys by (8 queries in two
 //            f16 parts) is one 16x16x32 product for 32 dimensions, in place of 220 of 390 VALU
-//            instructions a tile of dk 64 (37 sequences of 1 .. 16384 over 2 KV heads of 64: 25.6 -> 21.7 us with the
+//            instructions a tile of dk 64 (37 sequences of 1 .. 16384 over 2 KV heads of 64: 25.6 -> 21 us with the
 //            join). 4 heads fill half of it, and the rows in lines of 64 bytes cost more than the
 //            instructions (64 x 2000 over 5 heads of 128: 71 -> 77 us), so they stay with the VALU;
 //   values   the probability of (row u, head h) is broadcast within the 16 lanes by a DPP move.
@@ -490,7 +490,7 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[r][e] = 0.0f;
 
-    auto tile = [&](int base) {
+    auto tile = [&](int base, v8h(&km)[kDots ? KC : 1], Row(&vr)[kPgU]) {
         const bool part = base + kPgTile > n;  // rows behind the chunk's last one
         float x[NV], top[NM];
         if constexpr (kDots) dots(km, x);
@@ -567,12 +567,26 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
             });
         });
     };
-    // (the next tile's rows on their way during a tile, in registers of their own, changed nothing: the other
-    // waves' are)
+    // (kDots: the next tile's rows are on their way during a tile, 3 .. 7 % of the call; where a tile takes the VALU
+    // longer that changes nothing, since the other waves' are)
     for (int base = w * kPgTile; base < n; base += kPgWaves * kPgTile)
     {
-        if (base != w * kPgTile) load(base);
-        tile(base);
+        if constexpr (kDots)
+        {
+            v8h km_now[KC];
+            Row vr_now[kPgU];
+#pragma unroll
+            for (int i = 0; i < KC; ++i) km_now[i] = km[i];
+#pragma unroll
+            for (int u = 0; u < kPgU; ++u) vr_now[u] = vr[u];
+            if (base + kPgWaves * kPgTile < n) load(base + kPgWaves * kPgTile);
+            tile(base, km_now, vr_now);
+        }
+        else
+        {
+            if (base != w * kPgTile) load(base);
+            tile(base, km, vr);
+        }
     }
 
     // ---- the new position: one more row, of the first group of the wave whose turn it is
