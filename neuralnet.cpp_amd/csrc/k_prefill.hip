@@ -46,7 +46,7 @@
 // Work-groups are issued heaviest first (the last query blocks attend over the most keys).
 // V's four waves convert their part of the next tile behind their products, K's before them: every SIMD
 // has one wave of each, and one's VALU phases fall on the other's MFMA phases (4 x 2048 tokens f32 caches
-// 389 -> 367 us, f16 280 -> 273, back to back on one box; 363 and 269 with the queries as below).
+// 389 -> 367 us, f16 280 -> 273, back to back on one box; 350 and 269 with the steps below).
 // Measured before that (calls back to back in a graph, us, f32 products / here): f32 caches 4 x 2048 tokens
 // 809 / 398, 3 x 1111 at 517 411 / 202, 16 x 2048 3088 / 1498, 1 x 64 22.5 / 17.7; f16 caches 817 / 293,
 // 421 / 146, 3153 / 1121, 22.7 / 15.9. Two f16 halves for P and V too (at the cost above) took 295 and
@@ -66,7 +66,7 @@
 //   * A block of queries costs about four tiles besides its own: its queries (128 KB for dk 128, into one CU), their
 //     rotation and splitting, and the check at its end. What it waits for is on its way together.
 // 4 x 700 .. 1024 tokens at position 6144, 20 heads over 5 of 128, f16: 555 us with the join (20), 410 TFLOP/s of the
-// attention's own products; 8 x 77 .. 1900 tokens, 16 heads over 2 of 64, f32, capped and biased: 110 .. 120 us.
+// attention's own products; 8 x 77 .. 1900 tokens, 16 heads over 2 of 64, f32, capped and biased: 105 .. 114 us.
 // Bound by the VALU and MFMA work of a tile, which two waves to a SIMD overlap in part.
 // Caches of f16 elements (compute = F16): the fill rounds the rotated keys and the values to the
 // nearest f16 (ties to even), as the decode append does.
@@ -313,11 +313,28 @@ __device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, 
 // kPExpMax for all-zero values. Outside +-kPExpMax (infinities and NaN among it) the f32 products run.
 __device__ __forceinline__ int f16_exp(uint32_t mx) { return mx == 0 ? kPExpMax : 14 + 127 - (int)(mx >> 23); }
 
-// The wave's largest value
+// A lane's value and that of the lane 32 away
+__device__ __forceinline__ float max_halves(float x)
+{
+    const auto z = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+    const uint32_t a = z[0], b = z[1];
+    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+
+// The wave's largest value, by moves between registers (through LDS, 43 instructions and six round
+// trips a tile of f32 keys: 4 x 2048 tokens 360 us, 347 so)
 __device__ __forceinline__ uint32_t wave_max(uint32_t v)
 {
-    for (int off = 32; off >= 1; off >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, off, kWave));
-    return v;
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));   // lane ^ 1
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));   // lane ^ 2
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));  // 7 - lane of 8
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true));  // 15 - lane of 16
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    const uint32_t r0 = r[0], r1 = r[1];
+    v = max(r0, r1);
+    const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    const uint32_t h0 = h[0], h1 = h[1];
+    return max(h0, h1);
 }
 
 // Where a wave works: query head, first query, the lane's query
@@ -1350,7 +1367,8 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
             float mx = s[0];
 #pragma unroll
             for (int v = 1; v < 16; ++v) mx = fmaxf(mx, s[v]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32)) * f;
+            // (by registers 1 % faster with dk 64, 1 % slower with dk 128, where it takes two that are short)
+            mx = (DK == 64 ? max_halves(mx) : fmaxf(mx, __shfl_xor(mx, 32))) * f;
             // the reference of a query moves only when its maximum has grown by 2^8 (or is new)
             if constexpr (kHalf) mx = __builtin_ceilf(mx);  // whole powers of two: every rescaling is exact
             const bool grown = mx > m_ref + kPLazy;
