@@ -454,6 +454,20 @@ def test_prompt_shared_items_many_sequences(ctx, nnhip):
     check_prompt(ctx, nnhip, lens, [int(x) for x in rng.integers(0, 40, 150)], 2, 1, 64, 16, True, seed=34, sample=4)
 
 
+@pytest.mark.parametrize("seed", range(8))
+def test_prompt_random_packings(ctx, nnhip, seed):
+    """Spans of a few tiles: cuts at any tile of an item, beside empty sequences, prefixes and items of one tile."""
+    rng = np.random.default_rng(600 + seed)
+    B = int(rng.integers(1, 10))
+    lens = [int(x) for x in rng.integers(0, 120, B)]
+    lens[int(rng.integers(0, B))] = 33
+    pos0 = [int(x) for x in rng.integers(0, [1, 700, 700][seed % 3], B)]
+    H, Hkv, dk = [(20, 5, 128), (16, 2, 64), (4, 4, 64), (6, 3, 128)][seed % 4]
+    prefix = [int(x) for x in rng.integers(0, 300, B)] if seed % 3 == 1 else None
+    check_prompt(ctx, nnhip, lens, pos0, H, Hkv, dk, [8, 32, 64][seed % 3], seed % 2 == 0, cap=[0.0, 25.0][seed // 4],
+                 slopes=seed % 4 == 1, prefix=prefix, seed=600 + seed, sample=5)
+
+
 @pytest.mark.parametrize("f16", [False, True])
 def test_prompt_shared_items_nonfinite(ctx, nnhip, f16):
     """What one work-group of an item meets (a NaN, an infinity, keys of f32 range, a page outside the pool) and
