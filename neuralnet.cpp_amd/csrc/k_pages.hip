@@ -47,6 +47,7 @@ struct PagesArgs
     const int32_t* table;
     const float* slopes;
     float* part;
+    int2* places;  // even > 0: each sequence's first record and its chunks' size, for the join
     float* out;
     int B, H, Hkv, R, groups, RG;  // R = H / Hkv heads of a KV head, in `groups` groups of at most RG
     int shift;                     // log2(page_size)
@@ -203,12 +204,13 @@ struct PagesItem
 
 __device__ __forceinline__ int pages_len(const PagesArgs& a, int p) { return p < 0 || p >= a.len_bound ? 0 : p + 1; }
 
-// Item `item` of a call (with seq >= 0: the first of that sequence). With lengths spread from 1 to 16 K,
+// Item `item` of a call. With lengths spread from 1 to 16 K,
 // chunks of one size for len_bound leave a few long work-groups and thousands of empty ones (37 sequences
 // of 1 .. 16384 over 2 KV heads: 63 us against 26), so every wave sizes the chunks by the lengths
 // themselves: with D = a.even the smallest multiple of 64 that is at least sum(len) / D, which makes at
-// most D + B chunks. Every work-group of the call and the join find the same ones; nothing is kept.
-__device__ __forceinline__ PagesItem find_item(const PagesArgs& a, int item, int seq)
+// most D + B chunks. Every work-group of the call finds the same ones; the first of a sequence leaves its
+// place for the join.
+__device__ __forceinline__ PagesItem find_item(const PagesArgs& a, int item)
 {
     const int lane = threadIdx.x & 63;
     uint32_t total = 0;  // below 2^31
@@ -229,7 +231,7 @@ __device__ __forceinline__ PagesItem find_item(const PagesArgs& a, int item, int
             if (lane >= off) incl += x;
         }
         const int sum = __builtin_amdgcn_readlane(incl, live - 1);
-        const unsigned long long here = __builtin_amdgcn_ballot_w64(b < a.B && (seq >= 0 ? b == seq : before + incl > item));
+        const unsigned long long here = __builtin_amdgcn_ballot_w64(b < a.B && before + incl > item);
         if (here != 0)
         {
             const int l = __builtin_ctzll(here);
@@ -251,7 +253,7 @@ __device__ __forceinline__ PagesItem find_item(const PagesArgs& a, int item, int
 //            (fold16): lane 4u + s holds row u's score of head(s) s, so that the cap, the bias and the
 //            exponential are computed once per score. 8 heads over f16 pools: 16 keys by (8 queries in two
 //            f16 parts) is one 16x16x32 product for 32 dimensions, in place of 220 of 390 VALU
-//            instructions a tile of dk 64 (37 sequences of 1 .. 16384 over 2 KV heads of 64: 25.6 -> 21 us with the
+//            instructions a tile of dk 64 (37 sequences of 1 .. 16384 over 2 KV heads of 64: 25.6 -> 20.8 us with the
 //            join). 4 heads fill half of it, and the rows in lines of 64 bytes cost more than the
 //            instructions (64 x 2000 over 5 heads of 128: 71 -> 77 us), so they stay with the VALU;
 //   values   the probability of (row u, head h) is broadcast within the 16 lanes by a DPP move.
@@ -261,7 +263,7 @@ __device__ __forceinline__ PagesItem find_item(const PagesArgs& a, int item, int
 // Bound by HBM where the caches are large (4 x 60000 .. 131072 positions, 8 heads of 128, f16: 231 us with the
 // join, 6.4 TB/s of the bytes it cannot do without; a large copy reaches 4.9 read and written together);
 // by the chain of round trips position -> page -> rows, about 7 us in the kernel and 4 in the join,
-// where they are small (16 x 2112, 5 heads of 128, f32: 34.6 us, 4.9 TB/s; 1 x 100: 7.5 us, one launch). 8 heads to a
+// where they are small (16 x 2112, 5 heads of 128, f32: 34.0 us, 5 TB/s; 1 x 100: 7.5 us, one launch). 8 heads to a
 // KV head of 64: by both, and the VALU instructions of the values (128 multiply-adds a tile).
 template <int DK, int RT, bool kFinal, typename CT>
 __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
@@ -283,7 +285,7 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
     const int HG = a.Hkv * a.groups;
     const int gh = blockIdx.x % HG, item = blockIdx.x / HG;
     const int g = gh / a.groups, hg = gh - g * a.groups;
-    const PagesItem it = !kFinal && a.even ? find_item(a, item, -1)
+    const PagesItem it = !kFinal && a.even ? find_item(a, item)
                                            : PagesItem{item / a.nchunk, item % a.nchunk, a.chunk, item - item % a.nchunk,
                                                        a.pos[item / a.nchunk]};
     if (it.b < 0) return;
@@ -310,6 +312,7 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
             for (int e = tid; e < R * DK; e += kPgThreads) out[e * out_step] = p < 0 ? 0.0f : __builtin_nanf("");
         return;
     }
+    if (!kFinal && a.even && c == 0 && gh == 0 && tid == 0) a.places[b] = make_int2(it.first, it.chunk);
     const int t0 = c * it.chunk;
     if (t0 > p) return;
     const int n = min(it.chunk, p - t0);           // cached rows here
@@ -722,7 +725,8 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_join(PagesArgs a)
     __shared__ float4 acc_s[G][L];
     __shared__ float m_s[G], l_s[G];
     const int h = blockIdx.x, b = blockIdx.y;
-    const PagesItem it = a.even ? find_item(a, 0, b) : PagesItem{b, 0, a.chunk, b * a.nchunk, a.pos[b]};
+    const int2 place = a.even ? a.places[b] : make_int2(b * a.nchunk, a.chunk);
+    const PagesItem it{b, 0, place.y, place.x, a.pos[b]};
     const int p = it.p;
     if (p < 0 || p >= a.len_bound) return;  // the chunks' kernel wrote those
     const int g = h / a.R, r0 = h - g * a.R, hg = r0 / a.RG, r = r0 - hg * a.RG;
@@ -982,12 +986,18 @@ static PagesCut pages_cut(size_t B, size_t Hkv, size_t R, size_t dk, size_t len_
     return {chunk, ceil_div(len_bound, chunk), 0};
 }
 
+// Floats of a call's records
+static size_t pages_records(size_t B, size_t Hkv, size_t groups, size_t RG, size_t dk, size_t len_bound, const PagesCut& cut)
+{
+    return pages_items(B, len_bound, cut.chunk, cut.even) * Hkv * groups * (RG * dk + kPgRec);
+}
+
 size_t pages_workspace_bytes(size_t B, size_t H, size_t Hkv, size_t dk, size_t len_bound, size_t num_cus)
 {
     const size_t R = H / Hkv, groups = pages_groups(R, dk);
     const PagesCut cut = pages_cut(B, Hkv, R, dk, len_bound, num_cus);
     if (cut.nchunk == 1) return 0;
-    return pages_items(B, len_bound, cut.chunk, cut.even) * Hkv * groups * (ceil_div(R, groups) * dk + kPgRec) * sizeof(float);
+    return pages_records(B, Hkv, groups, ceil_div(R, groups), dk, len_bound, cut) * sizeof(float) + (cut.even ? B * sizeof(int2) : 0);
 }
 
 hipError_t launch_pages_attn(hipStream_t st, const nnhip_kv_pages& kv, const float* q, const float* k, const float* v,
@@ -999,7 +1009,9 @@ hipError_t launch_pages_attn(hipStream_t st, const nnhip_kv_pages& kv, const flo
     const size_t R = H / kv.Hkv, dk = kv.dk, groups = pages_groups(R, dk);
     const PagesCut cut = pages_cut(B, kv.Hkv, R, dk, len_bound, num_cus);
     const bool cap = softcap > 0.0f;
-    PagesArgs a{q, k, v, pos, cosT, sinT, kv.k, kv.v, kv.table, slopes, part, out, (int)B, (int)H, (int)kv.Hkv, (int)R,
+    PagesArgs a{q, k, v, pos, cosT, sinT, kv.k, kv.v, kv.table, slopes, part,
+                reinterpret_cast<int2*>(part + (cut.even ? pages_records(B, kv.Hkv, groups, ceil_div(R, groups), dk, len_bound, cut) : 0)),
+                out, (int)B, (int)H, (int)kv.Hkv, (int)R,
                 (int)groups, (int)ceil_div(R, groups), log2_of(kv.page_size), (int)kv.table_stride, (int)kv.num_pages,
                 (int)len_bound, (int)cut.chunk, (int)cut.nchunk, (int)cut.even, (float)(scale * kLog2e),
                 cap ? scale / softcap : 0.0f, cap ? (float)(softcap * kLog2e) : 0.0f, tokens ? 1 : 0};
