@@ -452,8 +452,9 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
             for (int e = 0; e < E; ++e) q[r][e] = q_s[r * DK + Row::dim(e, j)];
     }
     // 16 keys' products with the lane's column, of which it has four rows; then the scores of two of them: a hi
-    // lane and its lo lane exchange the others
-    auto dots = [&](const v8h(&k)[kDots ? KC : 1], float(&x)[NV]) {
+    // lane and its lo lane exchange the others. An infinite key times a part that is 0, or whose sign is not its
+    // element's, is not the score's: such scores of the tile's first `rows` come from the queries as they are.
+    auto dots = [&](const v8h(&k)[kDots ? KC : 1], float(&x)[NV], int rows) {
         typedef float v4f __attribute__((ext_vector_type(4)));
         v4f d = v4f{};
 #pragma unroll
@@ -464,6 +465,33 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
         {
             const float got = dpp<kDppRor8>(lo_col ? y[i] : y[2 + i]);
             x[i] = lo_col ? __builtin_fmaf(y[2 + i], 0x1p-11f, got) : __builtin_fmaf(got, 0x1p-11f, y[i]);
+        }
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) odd |= !__builtin_isfinite(x[i]);
+        if (__builtin_amdgcn_ballot_w64(odd) == 0) return;
+        odd = false;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) odd |= !__builtin_isfinite(x[i]) && row_at(i) < rows;
+        if (__builtin_amdgcn_ballot_w64(odd) == 0) return;
+        const float up = 1.0f / unit;  // a power of 2
+#pragma unroll 1
+        for (int r = 0; r < RT; ++r)
+        {
+            // lane j of every 16: row j's product with head r
+            float d = 0.0f;
+#pragma unroll
+            for (int c = 0; c < (kDots ? KC : 1); ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d = __builtin_fmaf((float)k[c][i], q_s[r * DK + 32 * c + 8 * grp + i], d);
+            d += __shfl_xor(d, 16, kWave);
+            d += __shfl_xor(d, 32, kWave);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+            {
+                const float at = __shfl(d, row_at(i), kWave);
+                if (r == hs && !__builtin_isfinite(x[i])) x[i] = at * up;
+            }
         }
     };
     // over the lanes of 16 that hold the same heads
@@ -496,7 +524,7 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
     auto tile = [&](int base, v8h(&km)[kDots ? KC : 1], Row(&vr)[kPgU]) {
         const bool part = base + kPgTile > n;  // rows behind the chunk's last one
         float x[NV], top[NM];
-        if constexpr (kDots) dots(km, x);
+        if constexpr (kDots) dots(km, x, n - base);
         else
         {
             float s[NS];
@@ -603,7 +631,7 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
             for (int c = 0; c < KC; ++c)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) k[c][i] = (_Float16)new_s[0][32 * c + 8 * grp + i];
-            dots(k, x);
+            dots(k, x, kPgTile);
         }
         else
         {

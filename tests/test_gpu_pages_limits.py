@@ -1,0 +1,86 @@
+"""Paged decode attention at the ends of what its inputs may hold: infinite keys (an f16 pool gets them from every
+key past 65504), queries and caps of extreme sizes. A score is the sum of its products as f32 adds them: an
+infinite key makes it infinite where the query's element is not 0, NaN where it is; a score of -infinity
+weighs nothing, +infinity and NaN make the head's output NaN. Finite outputs are held to the bound of
+test_gpu_pages.py over the keys that weigh something."""
+import numpy as np
+import pytest
+
+from test_gpu_pages import Cache, attend64, dev, host
+
+pytestmark = pytest.mark.gpu
+
+
+def scores_of(q, K):
+    """The products' sums with infinities, for (H, dk) queries of one KV head and (n, dk) keys."""
+    with np.errstate(invalid="ignore"):
+        return (q[:, None, :] * K[None, :, :]).sum(-1)
+
+
+def check_head(out, q, K, V, scale):
+    """One head's output against its formula; returns what became of it."""
+    s = scores_of(q[None], K)[0] * scale
+    if np.isnan(s).any() or (s == np.inf).any():
+        assert np.all(np.isnan(out)), out
+        return "nan"
+    see = s > -np.inf
+    if not see.any():
+        assert np.all(out == 0), out
+        return "zero"
+    ref, tol = attend64(q, K[see], V[see], scale, 0.0, 0.0, np.zeros(int(see.sum())), np.ones(int(see.sum()), bool))
+    off = np.abs(out - ref)
+    assert np.all(off <= tol), f"{np.max(off / tol)} times the bound"
+    return "finite"
+
+
+@pytest.mark.parametrize("new", [False, True])
+@pytest.mark.parametrize("exact", [False, True])
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("dk", [64, 128])
+@pytest.mark.parametrize("R", [2, 5, 8])
+def test_decode_infinite_keys(ctx, nnhip, R, dk, f16, exact, new):
+    """Infinite keys among the cached ones, or the new one, against queries of mixed signs, exact: ones that f16 holds
+    (nothing is left for a second part). Sequence 0: an infinity that some heads weigh -infinity and others +infinity;
+    1: one against query elements far below their head's largest; 2: every key, -infinity for heads of one
+    sign; 3: one against an element that is 0; 4: none."""
+    print(f"infinite keys R={R} dk={dk} f16={f16} exact={exact} new={new}", flush=True)
+    rng = np.random.default_rng(100 + R)
+    B, Hkv, page, n = 5, 2, 16, 300
+    H = R * Hkv
+    pos = np.full(B, n, np.int32)
+    c = Cache(rng, pos + 1, Hkv, page, dk, f16)
+    q = rng.standard_normal((B, H, dk)).astype(np.float32)
+    if exact:
+        q = (np.round(q * 64) / 64).astype(np.float32)
+    q[0, :, 5] = np.where(np.arange(H) % 2 == 0, -0.5, 0.75)
+    q[1, :, 9] = 2.0 ** -44 * np.where(np.arange(H) % 3 == 0, 1.0, -1.0)
+    q[2, :, 0] = np.where(np.arange(H) % 2 == 0, -1.0, 1.0)
+    q[3, :, 7] = np.where(np.arange(H) % 2 == 0, 0.0, -1.0)
+    k, v = (rng.standard_normal((B, Hkv, dk)).astype(np.float32) for _ in range(2))
+
+    def put(b, t, e):
+        if new and t == n:
+            k[b, :, e] = np.inf if not f16 else 1e6  # f16: past its largest
+        else:
+            c.k[c.table[b, t // page], :, t % page, e] = np.inf
+
+    put(0, n if new else 130, 5)
+    put(1, n if new else 17, 9)
+    for t in range(n + 1):
+        put(2, t, 0)
+    if not new:
+        k[2, :, 0] = np.inf
+    put(3, n if new else 299, 7)
+    out = host(ctx.attention_pages_decode(c.on_device(nnhip), dev(q.reshape(B, -1)), dev(k.reshape(B, -1)),
+                                          dev(v.reshape(B, -1)), H, dev(pos), n + 1, 0.125,
+                                          tokens=True)).astype(np.float64).reshape(B, H, dk)
+    found = set()
+    for b in range(B):
+        with np.errstate(over="ignore"):
+            c.set(b, n, k[b], v[b])
+        K, V = c.rows(b, n + 1)
+        for h in range(H):
+            g = h // R
+            found.add((b, check_head(out[b, h], q[b, h].astype(np.float64), K[:, g], V[:, g], 0.125)))
+    assert found == {(0, "finite"), (0, "nan"), (1, "finite"), (1, "nan"), (2, "zero"), (2, "nan"), (3, "nan"),
+                     (3, "finite"), (4, "finite")}
