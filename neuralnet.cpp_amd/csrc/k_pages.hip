@@ -503,7 +503,10 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
         x += dpp<kDppRor8>(x);
         return kDots ? x : x + dpp<kDppRor4>(x);
     };
-    const float scale2 = a.scale2 * unit, capi = a.capi * unit;
+    // (kDots: a product past f32's range would make a score of 0 NaN; any other score is past the cap, or the
+    // range, with the largest float, too)
+    auto held = [](float x) { return x > 3.40282347e38f ? 3.40282347e38f : x < -3.40282347e38f ? -3.40282347e38f : x; };
+    const float scale2 = held(a.scale2 * unit), capi = held(a.capi * unit);
     float slope2[NM];
 #pragma unroll
     for (int i = 0; i < NM; ++i) slope2[i] = a.slopes && hs + i < R ? a.slopes[h0 + hs + i] * 1.44269504f : 0.0f;

@@ -84,3 +84,33 @@ def test_decode_infinite_keys(ctx, nnhip, R, dk, f16, exact, new):
             found.add((b, check_head(out[b, h], q[b, h].astype(np.float64), K[:, g], V[:, g], 0.125)))
     assert found == {(0, "finite"), (0, "nan"), (1, "finite"), (1, "nan"), (2, "zero"), (2, "nan"), (3, "nan"),
                      (3, "finite"), (4, "finite")}
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("H,Hkv,dk", [(4, 2, 64), (8, 1, 64), (10, 2, 128), (8, 1, 256)])
+@pytest.mark.parametrize("size,cap,scale", [(1e15, 1e-30, 0.125), (1e30, 0.0, 1e20), (1e-30, 1e30, 0.125)])
+def test_decode_extreme_queries_and_caps(ctx, nnhip, H, Hkv, dk, f16, size, cap, scale):
+    """Queries, caps and scales whose quotient or product passes f32's range on the way: sequence 0's keys are 0, so all
+    its scores are, and its output is the mean of the values; under the smallest cap sequence 1's is, too (scores of
+    1e-30 at most), and under the largest its scores are those of queries of 1e-30."""
+    print(f"extreme H={H} Hkv={Hkv} dk={dk} f16={f16} size={size} cap={cap} scale={scale}", flush=True)
+    rng = np.random.default_rng(200 + dk)
+    B, page, n = 2, 16, 200
+    pos = np.full(B, n, np.int32)
+    c = Cache(rng, pos + 1, Hkv, page, dk, f16)
+    q = (size * rng.standard_normal((B, H, dk))).astype(np.float32)
+    k, v = (rng.standard_normal((B, Hkv, dk)).astype(np.float32) for _ in range(2))
+    k[0] = 0
+    for t in range(n):
+        c.k[c.table[0, t // page], :, t % page] = 0
+    out = host(ctx.attention_pages_decode(c.on_device(nnhip), dev(q.reshape(B, -1)), dev(k.reshape(B, -1)),
+                                          dev(v.reshape(B, -1)), H, dev(pos), n + 1, scale, softcap=cap,
+                                          tokens=True)).astype(np.float64).reshape(B, H, dk)
+    for b in range(1 if cap == 0 else 2):
+        c.set(b, n, k[b], v[b])
+        V = c.rows(b, n + 1)[1]
+        for h in range(H):
+            x = V[:, h // (H // Hkv)]
+            # equal weights (scores below 1e-28 change none): attend64's bound of the sums, nothing of the scores
+            tol = 2.0 ** -24 * (4 * np.sqrt(n + 1) + 40 + 16) * np.abs(x).mean(0)
+            assert np.all(np.abs(out[b, h] - x.mean(0)) <= tol), (b, h)
