@@ -759,7 +759,8 @@ typedef struct nnhip_logit_rules
 
 /* Adjust token-major logits (B, V) by the rules and choose greedily: ids[b] = nnhip_argmax_rows's choice
  * among the allowed tokens (best = the first allowed one, then every larger value replaces it); -1 where
- * no token is allowed, whose counts and pos stay. out (B, V), or NULL: the adjusted logits (may be the
+ * no token is allowed, whose counts and pos stay. (-1 is no input for the next step: the embedding
+ * of it is NaN, and that step would write it over the row at pos[b].) out (B, V), or NULL: the adjusted logits (may be the
  * logits themselves). pos, or NULL: pos[b] += 1 after a choice; a pos[b] below 0 (an empty slot of
  * nnhip_attention_pages_decode) stays, and nothing is counted for it. ids may be NULL where out is given (then
  * counts and pos must not be changed: count_choice == 0, pos NULL). The greedy rule of the reference

@@ -465,12 +465,25 @@ class Decoder:
             ctx.partial_residual_quant_i8(pf, f2.tau, self.s, self.rs, d, B, self.x, res=self.r, bias=f2.bias,
                                           gamma=g_next, eps=cfg.eps, outs=outs)
 
+    def _choose(self, rows, rules, ids, pos, advance: bool):
+        """The step's choice from token-major logits; returns it. With advance it goes into ids and pos moves on, but
+        where nothing is allowed (-1) both stay: -1 is no token to go on from."""
+        import torch
+        kept = advance and rules is not None and rules.masks
+        out = torch.empty_like(ids) if kept else ids if advance else self.ids
+        self.ctx.logits_adjust_rows(rows, rules, ids=out, pos=pos if advance else None)
+        if kept:
+            torch.where(out < 0, ids, out, out=ids)
+        return out
+
     def step(self, ids, pos, len_bound: int, attn_hook=None, advance: bool = False, rules=None):
         """ids / pos: (B,) int32 device tensors. Returns (logits (vocab, B), greedy ids (B,)).
         advance: the greedy ids are written into ids itself and every pos is advanced by one, so
         that the next call continues the generation (a captured step then replays as is); paged
         caches: a pos below 0 (an empty slot) stays. rules: a LogitRules for the choice (the logits
-        returned are those before it)."""
+        returned are those before it). Where its mask allows nothing the id returned is -1 (in a tensor of
+        its own: the next input is ids), and ids and pos keep that sequence's token and position: the next
+        call repeats it, the same key and value in the same place."""
         ctx = self.ctx
         fused = self.fused_ok()
         if fused and self._tok:
@@ -494,20 +507,20 @@ class Decoder:
                 self.block_step(i, pos, len_bound, attn_hook)
             self._quant(self.x, self.g_final)
         out_ids = ids if advance else self.ids
+        ruled = rules is not None or self.paged
         if fused and self.logits_t is not None:
             h = self.head
             ctx.ternary_matmul_n([(h.rp, h.tau, h.bias, h.N, self.logits_t)], self.xi, self.s, self.rs, h.K, self.B,
                                  tokens=True)
-            if rules is not None or self.paged:
-                ctx.logits_adjust_rows(self.logits_t, rules, ids=out_ids, pos=pos if advance else None)
+            if ruled:
+                out_ids = self._choose(self.logits_t, rules, ids, pos, advance)
             else:
                 ctx.argmax_rows(self.logits_t, out=out_ids, pos=pos if advance else None)
             self._logits = self.logits_t.t()
             return self._logits, out_ids
         self._mm(self.head, self._logits_cols)
-        if rules is not None or self.paged:
-            rows = self._logits_cols.t().contiguous()
-            ctx.logits_adjust_rows(rows, rules, ids=out_ids, pos=pos if advance else None)
+        if ruled:
+            out_ids = self._choose(self._logits_cols.t().contiguous(), rules, ids, pos, advance)
             self._logits = self._logits_cols
             return self._logits, out_ids
         ctx.argmax_cols(self._logits_cols, out=out_ids)

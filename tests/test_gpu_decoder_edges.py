@@ -1,0 +1,108 @@
+"""The decoder where the choice or the batch is at an edge, over paged and contiguous caches."""
+import numpy as np
+import pytest
+
+from test_gpu_logits import rules as apply_rules
+from test_gpu_pages import dev, host, same
+from test_gpu_pages_decoder import Mirror
+from test_gpu_prefill import _gpu_model
+
+pytestmark = pytest.mark.gpu
+
+
+def model(ctx, nnhip, B, seed, **kw):
+    from nnhip_py import decoder as dmod
+    cfg = dmod.Config(**{**dict(d=256, H=4, Hkv=2, F=320, vocab=97, max_len=96, act=0, eps=1e-5), **kw})
+    return cfg, _gpu_model(ctx, nnhip, cfg, 2, B, seed, subln=True)[0]
+
+
+def decoder(ctx, nnhip, cfg, base, B, paged=True, page=16, seed=5):
+    from nnhip_py import decoder as dmod
+    if not paged:
+        return dmod.Decoder(ctx, cfg, base.blocks, base.emb, base.g_final, base.head, B)
+    m = Mirror(nnhip, cfg, 2, B, page, -(-cfg.max_len // page), False, np.random.default_rng(seed))
+    return dmod.Decoder(ctx, cfg, base.blocks, base.emb, base.g_final, base.head, B, caches=m.caches)
+
+
+def cached(dec, b, n):
+    """The cached keys and values of sequence b's first n positions (one page's at most), block by block."""
+    if dec.paged:
+        return [np.ascontiguousarray(host(t)[host(c.table)[b, 0], :, :n]) for c in dec.caches for t in (c.k, c.v)]
+    return [host(t)[b, :n].copy() for c in dec.caches for t in c]
+
+
+@pytest.mark.parametrize("paged", [True, False])
+@pytest.mark.parametrize("B", [3, 18])
+def test_step_where_nothing_is_allowed(ctx, nnhip, B, paged):
+    """A sequence whose mask allows nothing gets the choice -1 and stays as it is, its input token too: the steps after
+    it find the same state (pools, logits and counts bit for bit), and it goes on once tokens are allowed. The
+    other sequences are not touched by it. B = 18 runs the unfused step."""
+    import torch
+    print(f"nothing allowed B={B} paged={paged}", flush=True)
+    cfg, base = model(ctx, nnhip, B, 0xB0 + B)
+    dec = decoder(ctx, nnhip, cfg, base, B, paged)
+    counts = torch.zeros(B, cfg.vocab, dtype=torch.int32, device="cuda")
+    words = torch.full((B, 4), -1, dtype=torch.int32, device="cuda")
+    rule = nnhip.LogitRules(cfg.vocab, counts=counts, repeat=dev(np.full(B, 1.2, np.float32)), allowed=words,
+                            count_choice=True)
+    ids = dev(np.arange(B, dtype=np.int32) + 1)
+    pos = torch.zeros(B, dtype=torch.int32, device="cuda")
+    for _ in range(3):
+        dec.step(ids, pos, cfg.max_len, advance=True, rules=rule)
+    words[1] = 0
+    start = host(ids).copy(), host(pos).copy(), host(counts).copy()
+    seen = []
+    for i in range(3):
+        before = host(ids).copy(), host(pos).copy()
+        logits, got = dec.step(ids, pos, cfg.max_len, advance=True, rules=rule)
+        got, rest = host(got), [b for b in range(B) if b != 1]
+        assert got[1] == -1 and np.all(got[rest] >= 0)
+        assert host(ids)[1] == start[0][1] and np.array_equal(host(ids)[rest], got[rest])
+        assert host(pos)[1] == 3 and np.array_equal(host(pos)[rest], before[1][rest] + 1)
+        assert np.array_equal(host(counts)[1], start[2][1])
+        seen.append((host(logits)[:, 1].copy(), cached(dec, 1, 4)))
+    for x, rows in seen:
+        assert np.all(np.isfinite(x)) and np.array_equal(x, seen[0][0])
+        assert all(np.all(np.isfinite(a)) and same(a, b) for a, b in zip(rows, seen[0][1]))
+    words[1] = -1
+    logits, got = dec.step(ids, pos, cfg.max_len, advance=True, rules=rule)
+    assert np.array_equal(host(logits)[:, 1], seen[0][0])
+    want = apply_rules(seen[0][0][None].copy(), counts=start[2][1:2], repeat=np.full(1, 1.2, np.float32))[1]
+    assert host(got)[1] == want[0] == host(ids)[1] and host(pos)[1] == 4
+
+
+def test_captured_step_where_nothing_is_allowed(nnhip):
+    """The same in a captured step, whose input is the ids it replays into."""
+    import torch
+    ctx = nnhip.Context(0)
+    cfg, base = model(ctx, nnhip, 3, 0xB7)
+    runs = []
+    for captured in (False, True):
+        dec = decoder(ctx, nnhip, cfg, base, 3)
+        words = torch.full((3, 4), -1, dtype=torch.int32, device="cuda")
+        rule = nnhip.LogitRules(cfg.vocab, allowed=words)
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            _, ids = dec.prefill_packed(dev(np.arange(9, dtype=np.int32)), dev(np.array([0, 2, 5, 9], np.int32)), 4)
+            pos = dev(np.array([2, 3, 4], np.int32))
+            _, got = dec.step(ids, pos, cfg.max_len, advance=True, rules=rule)
+        torch.cuda.synchronize()
+        if captured:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                _, got = dec.step(ids, pos, cfg.max_len, advance=True, rules=rule)
+        trace = []
+        for i in range(6):
+            words[2] = 0 if i in (1, 2, 4) else -1
+            torch.cuda.synchronize()
+            if captured:
+                g.replay()
+            else:
+                with torch.cuda.stream(side):
+                    _, got = dec.step(ids, pos, cfg.max_len, advance=True, rules=rule)
+            torch.cuda.synchronize()
+            assert (host(got)[2] == -1) == (i in (1, 2, 4))
+            trace.append(np.concatenate((host(got), host(ids), host(pos))))
+        runs.append(np.array(trace))
+    assert np.array_equal(*runs)
+    ctx.close()
