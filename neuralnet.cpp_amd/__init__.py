@@ -317,6 +317,7 @@ class LogitRules:
              ("allowed", allowed, i32, None if allowed is None else (allowed.shape[0], words))])
         self.tensors = (counts, repeat, presence, frequency, bias, allowed)
         self.masks = allowed is not None  # the choice may be -1
+        self.counts_choice = bool(count_choice)
         p = [None if t is None else t.data_ptr() for t in self.tensors]
         self.desc = _LogitRulesDesc(p[0], p[1], p[2], p[3], p[4], V if bias is not None and bias.shape[0] > 1 else 0,
                                     p[5], words if allowed is not None and allowed.shape[0] > 1 else 0,

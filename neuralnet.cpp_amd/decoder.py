@@ -471,7 +471,12 @@ class Decoder:
         import torch
         kept = advance and rules is not None and rules.masks
         out = torch.empty_like(ids) if kept else ids if advance else self.ids
-        self.ctx.logits_adjust_rows(rows, rules, ids=out, pos=pos if advance else None)
+        if not advance and rules is not None and rules.counts_choice:
+            # positions say which slots are empty, and nothing is counted for those; these ones are moved on
+            pos = torch.add(pos, 0)
+        elif not advance:
+            pos = None
+        self.ctx.logits_adjust_rows(rows, rules, ids=out, pos=pos)
         if kept:
             torch.where(out < 0, ids, out, out=ids)
         return out
@@ -480,8 +485,8 @@ class Decoder:
         """ids / pos: (B,) int32 device tensors. Returns (logits (vocab, B), greedy ids (B,)).
         advance: the greedy ids are written into ids itself and every pos is advanced by one, so
         that the next call continues the generation (a captured step then replays as is); paged
-        caches: a pos below 0 (an empty slot) stays. rules: a LogitRules for the choice (the logits
-        returned are those before it). Where its mask allows nothing the id returned is -1 (in a tensor of
+        caches: a pos below 0 (an empty slot) stays, and nothing is counted for it. rules: a LogitRules for
+        the choice (the logits returned are those before it). Where its mask allows nothing the id returned is -1 (in a tensor of
         its own: the next input is ids), and ids and pos keep that sequence's token and position: the next
         call repeats it, the same key and value in the same place."""
         ctx = self.ctx

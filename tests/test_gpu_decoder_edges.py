@@ -106,3 +106,24 @@ def test_captured_step_where_nothing_is_allowed(nnhip):
         runs.append(np.array(trace))
     assert np.array_equal(*runs)
     ctx.close()
+
+
+@pytest.mark.parametrize("advance", [False, True])
+@pytest.mark.parametrize("B", [3, 18])
+def test_empty_slot_is_not_counted(ctx, nnhip, B, advance):
+    """A step counts the choices of live sequences only, whether or not it advances them."""
+    import torch
+    print(f"empty slot B={B} advance={advance}", flush=True)
+    cfg, base = model(ctx, nnhip, B, 0xC0 + B)
+    dec = decoder(ctx, nnhip, cfg, base, B)
+    counts = torch.zeros(B, cfg.vocab, dtype=torch.int32, device="cuda")
+    rule = nnhip.LogitRules(cfg.vocab, counts=counts, repeat=dev(np.full(B, 1.2, np.float32)), count_choice=True)
+    pos = np.zeros(B, np.int32)
+    pos[[0, B - 1]] = -1, -5
+    pos_d, ids = dev(pos), dev(np.arange(B, dtype=np.int32))
+    _, got = dec.step(ids, pos_d, cfg.max_len, advance=advance, rules=rule)
+    want = np.zeros((B, cfg.vocab), np.int32)
+    live = np.flatnonzero(pos >= 0)
+    want[live, host(got)[live]] = 1
+    assert np.array_equal(host(counts), want)
+    assert np.array_equal(host(pos_d), np.where(pos >= 0, pos + advance, pos))
