@@ -43,16 +43,16 @@ struct nnhip_ctx
     // ranges that the next per-token quantizer call reads in extra blocks (nnhip_ctx_prefetch_next)
     Prefetch pf{};
     // scratch of the paged attention and the logits' choice: one buffer for each stream that calls
-    // came on, so that calls on two streams share none. Outgrown buffers stay until the context
-    // goes, because a captured call may replay into them (sizes double: all of them together are
-    // smaller than the last).
+    // came on, so that calls on two streams share none
     struct StreamWs
     {
         hipStream_t stream;
-        std::vector<void*> bufs;  // the last one is in use
+        void* buf;
         size_t bytes;
     };
     std::vector<StreamWs> stream_ws;
+    // buffers that those above outgrew (ensure_buf)
+    std::vector<void*> outgrown;
 };
 
 namespace
@@ -153,43 +153,58 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 bool mul_ok(size_t a, size_t b) { return a == 0 || b <= SIZE_MAX / a; }
 
-// Grow a context-owned device buffer to at least `bytes` (waits for queued work first, because
-// a kernel in flight may still use the old buffer).
-nnhip_status ensure_buf(nnhip_ctx* ctx, void*& buf, size_t& have, size_t bytes, const char* fn, const char* what)
+// Whether what is launched now is recorded into a graph
+bool capturing(nnhip_ctx* ctx)
+{
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(ctx->stream, &cs) == hipSuccess) return cs != hipStreamCaptureStatusNone;
+    (void)hipGetLastError();
+    return false;
+}
+
+nnhip_status fail_growth(const char* fn, const char* what)
+{
+    return fail(NNHIP_ERR_UNSUPPORTED, fn, std::string("the ") + what +
+                " would grow during a capture: make one call of this size before");
+}
+
+// A context-owned device buffer of at least `bytes`; a growth makes it twice as large at least, and
+// `least` bytes, where there is room. What it outgrows stays until the context goes, because a kernel in
+// flight or a captured call may use it; all of that together is smaller than what it grew to.
+nnhip_status ensure_buf(nnhip_ctx* ctx, void*& buf, size_t& have, size_t bytes, const char* fn, const char* what,
+                        size_t least = 0)
 {
     if (have >= bytes) return NNHIP_OK;
-    hipError_t e = hipStreamSynchronize(ctx->stream);
-    if (e != hipSuccess) return hip_fail(fn, "hipStreamSynchronize", e);
-    if (buf)
+    if (capturing(ctx)) return fail_growth(fn, what);
+    size_t got = std::max({bytes, least, 2 * have});
+    void* p = nullptr;
+    hipError_t e = hipMalloc(&p, got);
+    if (e != hipSuccess && got > bytes)
     {
-        e = hipFree(buf);
-        buf = nullptr;
-        have = 0;
-        if (e != hipSuccess) return hip_fail(fn, "hipFree", e);
+        (void)hipGetLastError();
+        got = bytes;
+        e = hipMalloc(&p, got);
     }
-    e = hipMalloc(&buf, bytes);
     if (e != hipSuccess)
     {
-        buf = nullptr;
         (void)hipGetLastError();
         return fail(NNHIP_ERR_OOM, fn, std::string(what) + " allocation of " + std::to_string(bytes) + " bytes failed");
     }
-    have = bytes;
+    if (buf) ctx->outgrown.push_back(buf);
+    buf = p;
+    have = got;
     return NNHIP_OK;
 }
 
-// The workspace grows to 1 MiB, then in 64 MiB steps where the device has room: a growth costs a wait, a free and
-// an allocation (about 0.4 ms), and a layer's calls differ in size (the two products of a training
-// step at 2048 tokens need 21 and 57 MB: first pass 824 us with two growths, 428 us with one).
+// The workspace grows to 1 MiB, then in 64 MiB steps: a layer's calls differ in size, and a growth costs an
+// allocation (the two products of a training step at 2048 tokens need 21 and 57 MB: first pass 824 us with
+// two growths, each with a wait and a free, too, 428 us with one).
 nnhip_status ensure_ws(nnhip_ctx* ctx, size_t bytes, const char* fn)
 {
-    if (ctx->ws_bytes >= bytes) return NNHIP_OK;
     // up to 1 MiB stays in one: the allocator serves that from memory it holds (0.9 us against 12-30 us
     // for 2 to 64 MiB, all the difference in a small call's first pass)
     const size_t step = bytes <= (size_t(1) << 20) ? size_t(1) << 20 : size_t(64) << 20;
-    if (ensure_buf(ctx, ctx->ws, ctx->ws_bytes, round_up(bytes, step), fn, "workspace") == NNHIP_OK)
-        return NNHIP_OK;
-    return ensure_buf(ctx, ctx->ws, ctx->ws_bytes, bytes, fn, "workspace");
+    return ensure_buf(ctx, ctx->ws, ctx->ws_bytes, bytes, fn, "workspace", round_up(bytes, step));
 }
 
 // Scratch of at least `bytes` on the context's current stream (nullptr for 0 bytes)
@@ -202,40 +217,12 @@ nnhip_status ensure_stream_ws(nnhip_ctx* ctx, size_t bytes, const char* fn, void
         if (w.stream == ctx->stream) ws = &w;
     if (!ws)
     {
-        ctx->stream_ws.push_back({ctx->stream, {}, 0});
+        ctx->stream_ws.push_back({ctx->stream, nullptr, 0});
         ws = &ctx->stream_ws.back();
     }
-    if (ws->bytes < bytes)
-    {
-        hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-        if (hipStreamIsCapturing(ctx->stream, &cs) != hipSuccess)
-        {
-            (void)hipGetLastError();
-            cs = hipStreamCaptureStatusNone;
-        }
-        if (cs != hipStreamCaptureStatusNone)
-            return fail(NNHIP_ERR_UNSUPPORTED, fn,
-                        "the workspace would grow during a capture: make one call of this size before, on this stream");
-        const size_t want = std::max(round_up(bytes, size_t(1) << 20), 2 * ws->bytes);
-        void* p = nullptr;
-        size_t got = want;
-        hipError_t e = hipMalloc(&p, want);
-        if (e != hipSuccess && want > bytes)
-        {
-            (void)hipGetLastError();
-            got = bytes;
-            e = hipMalloc(&p, bytes);
-        }
-        if (e != hipSuccess)
-        {
-            (void)hipGetLastError();
-            return fail(NNHIP_ERR_OOM, fn, "workspace allocation of " + std::to_string(bytes) + " bytes failed");
-        }
-        ws->bufs.push_back(p);
-        ws->bytes = got;
-    }
-    *out = ws->bufs.back();
-    return NNHIP_OK;
+    const nnhip_status st = ensure_buf(ctx, ws->buf, ws->bytes, bytes, fn, "workspace of this stream", round_up(bytes, size_t(1) << 20));
+    *out = ws->buf;
+    return st;
 }
 
 // The host's checks of a paged cache, with the rows of the rope tables (0 without)
@@ -399,7 +386,8 @@ nnhip_status nnhip_ctx_destroy(nnhip_ctx* ctx)
     if (ctx->attn_ws) (void)hipFree(ctx->attn_ws);
     if (ctx->ones) (void)hipFree(ctx->ones);
     for (auto& w : ctx->stream_ws)
-        for (void* p : w.bufs) (void)hipFree(p);
+        if (w.buf) (void)hipFree(w.buf);
+    for (void* p : ctx->outgrown) (void)hipFree(p);
     if (ctx->own) (void)hipStreamDestroy(ctx->own);
     delete ctx;
     if (e != hipSuccess) return hip_fail(fn, "hipStreamSynchronize", e);
@@ -1048,8 +1036,9 @@ static nnhip_status matmul_digits(nnhip_ctx* ctx, const char* fn, const void* rp
     {
         st = ensure_buf(ctx, reinterpret_cast<void*&>(ctx->ones), ctx->ones_bytes_, ones * 4, fn, "unit scales");
         if (st != NNHIP_OK) return st;
-        NNHIP_LAUNCH(fn, launch_fill_u32(ctx->stream, reinterpret_cast<uint32_t*>(ctx->ones), 0x3F800000u, ones));
-        ctx->ones_words = ones;
+        const size_t words = ctx->ones_bytes_ / 4;
+        NNHIP_LAUNCH(fn, launch_fill_u32(ctx->stream, reinterpret_cast<uint32_t*>(ctx->ones), 0x3F800000u, words));
+        ctx->ones_words = words;
     }
     uint8_t* w = static_cast<uint8_t*>(ctx->ws);
     int8_t* xi = reinterpret_cast<int8_t*>(w);

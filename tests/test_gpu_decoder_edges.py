@@ -127,3 +127,98 @@ def test_empty_slot_is_not_counted(ctx, nnhip, B, advance):
     want[live, host(got)[live]] = 1
     assert np.array_equal(host(counts), want)
     assert np.array_equal(host(pos_d), np.where(pos >= 0, pos + advance, pos))
+
+
+def scribble():
+    """NaN into whatever the allocators hand out next, small and large."""
+    import torch
+    return [torch.full((n,), float("nan"), device="cuda") for n in [1 << 8, 1 << 16, 1 << 18, 1 << 20, 1 << 24] * 4]
+
+
+@pytest.mark.parametrize("paged", [True, False])
+def test_captured_step_beside_larger_calls(nnhip, paged):
+    """A captured step of 18 sequences (whose feed-forward block uses the context's workspace) goes on as eager steps do
+    after eager prompts that outgrow that workspace: the captured calls keep theirs."""
+    import torch
+    print(f"captured step beside larger calls paged={paged}", flush=True)
+    ctx = nnhip.Context(0)
+    B = 18
+    cfg, base = model(ctx, nnhip, B, 0xF1, max_len=512)
+    assert nnhip.lib().nnhip_ffn_glu_workspace_bytes(cfg.d, cfg.F, 400 * B) > 1 << 20  # what it starts with
+    runs = []
+    for captured in (True, False):
+        dec, other = (decoder(ctx, nnhip, cfg, base, B, paged, seed=s) for s in (5, 6))
+        ids, pos = dev(np.arange(B, dtype=np.int32)), torch.zeros(B, dtype=torch.int32, device="cuda")
+        side = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            dec.step(ids, pos, cfg.max_len, advance=True)
+        torch.cuda.synchronize()
+        if captured:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                dec.step(ids, pos, cfg.max_len, advance=True)
+        trace, kept = [], []
+        for i in range(6):
+            if i in (1, 3):
+                T = 400 if i == 1 else 510
+                prompt = dev(np.arange(B * T, dtype=np.int32) % cfg.vocab)
+                if paged:
+                    other.prefill_packed(prompt, dev(np.arange(B + 1, dtype=np.int32) * T), T)
+                else:
+                    other.prefill(prompt, T)
+                torch.cuda.synchronize()
+                kept.append(scribble())
+            if captured:
+                g.replay()
+            else:
+                with torch.cuda.stream(side):
+                    dec.step(ids, pos, cfg.max_len, advance=True)
+            torch.cuda.synchronize()
+            trace.append(np.concatenate((host(ids), host(pos))))
+        runs.append(np.array(trace))
+    assert np.array_equal(*runs)
+    ctx.close()
+
+
+def test_captured_attention_beside_larger_calls(nnhip):
+    """The same for the scratch of the attention over contiguous caches; a capture that would have to grow a
+    workspace is refused, and the calls after it work."""
+    import torch
+    ctx = nnhip.Context(0)
+    H, Hkv, dk = 8, 2, 64
+
+    def problem(B, n):
+        x = [torch.randn(B, h * dk, device="cuda") for h in (H, Hkv, Hkv)]
+        caches = [torch.randn(B, n, Hkv * dk, device="cuda") for _ in range(2)]
+        return x, torch.full((B,), n - 1, dtype=torch.int32, device="cuda"), n, caches, torch.empty(B, H * dk, device="cuda")
+
+    def call(p):
+        x, pos, n, (kc, vc), out = p
+        return ctx.attention_decode(*x, H, Hkv, dk, pos, n, kc, vc, 0.125, None, None, out=out, tokens=True)
+
+    small, large = problem(2, 2000), problem(9, 9000)
+    assert 0 < nnhip.attention_workspace_bytes(2, H, Hkv, dk, 2000) < nnhip.attention_workspace_bytes(9, H, Hkv, dk, 9000)
+    fresh, g0 = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with pytest.raises(nnhip.NNHipError, match="capture"):
+        with torch.cuda.graph(g0, stream=fresh):
+            small[4].zero_()
+            call(small)
+    want = call(small).clone()
+    side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=side):
+        call(small)
+    kept = []
+    for i in range(4):
+        if i == 1:
+            call(large)
+            torch.cuda.synchronize()
+            kept.append(scribble())
+        small[4].zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(small[4], want)
+    ctx.close()
