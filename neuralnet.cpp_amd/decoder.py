@@ -143,6 +143,7 @@ class Decoder:
         self._logits = self._logits_cols
         self.logits_t = None    # token-major (B, vocab) logits of the step, when the head takes them
         self.ids = torch.empty((B,), dtype=torch.int32, device=dev)
+        self._pf_kept = []
         if self._tok and blocks:
             # the token-major q/k/v and o products run on the single-launch decode GEMV only: one
             # call of each on scratch tells whether this model's shapes are taken
@@ -176,23 +177,32 @@ class Decoder:
         token-major logits when the head produces those)."""
         return self._logits
 
+    # scratch of prompts: the buffers, the token columns that they hold, whether a captured prompt uses
+    # them, and their views for the last number of columns
+    _pf_flat, _pf_room, _pf_captured, _pf_M = {}, 0, False, None
+
     def _prefill_buffers(self, M: int):
-        """Scratch of a prefill over M = B*T token columns (allocated once per M)."""
+        """Scratch of a prefill over M token columns: views of buffers that grow to the largest M. Those that a captured
+        prompt uses stay as long as the decoder, beside what outgrows them."""
         import torch
-        if getattr(self, "_pf_M", None) == M:
-            return self._pf
-        cfg = self.cfg
-        dev = f"cuda:{self.ctx.device}"
-        f32 = dict(dtype=torch.float32, device=dev)
-        d, H, Hkv, dk = cfg.d, cfg.H, cfg.Hkv, cfg.dk
-        kpd = _pkg().kp
-        self._pf = dict(
-            x=torch.empty((d, M), **f32), r=torch.empty((d, M), **f32), q=torch.empty((H * dk, M), **f32),
-            k=torch.empty((Hkv * dk, M), **f32), v=torch.empty((Hkv * dk, M), **f32),
-            a=torch.empty((H * dk, M), **f32),
-            xi=torch.empty((M * kpd(max(d, H * dk)),), dtype=torch.int8, device=dev),
-            s=torch.empty((M,), **f32), rs=torch.empty((M,), dtype=torch.int32, device=dev))
-        self._pf_M = M
+        if M > self._pf_room:
+            for t in self._pf_flat.values():
+                t.record_stream(torch.cuda.current_stream(t.device))  # the last prompt may still be running there
+            if self._pf_captured:
+                self._pf_kept.append(self._pf_flat)
+            self._pf, self._pf_flat, self._pf_room, self._pf_captured, self._pf_M = None, {}, 0, False, None
+            cfg = self.cfg
+            d, Hdk, kv, f32 = cfg.d, cfg.H * cfg.dk, cfg.Hkv * cfg.dk, torch.float32
+            self._pf_flat = {name: torch.empty((n * M,), dtype=dt, device=f"cuda:{self.ctx.device}") for name, n, dt in (
+                ("x", d, f32), ("r", d, f32), ("q", Hdk, f32), ("k", kv, f32), ("v", kv, f32), ("a", Hdk, f32),
+                ("s", 1, f32), ("rs", 1, torch.int32), ("xi", _pkg().kp(max(d, Hdk)), torch.int8))}
+            self._pf_room = M
+        if torch.cuda.is_current_stream_capturing():
+            self._pf_captured = True
+        if self._pf_M != M:
+            self._pf = {name: t[:t.numel() // self._pf_room * M] for name, t in self._pf_flat.items()}
+            self._pf.update((name, self._pf[name].view(-1, M)) for name in ("x", "r", "q", "k", "v", "a"))
+            self._pf_M = M
         return self._pf
 
     def prefill(self, ids, T: int, pos0: int = 0, hook=None):

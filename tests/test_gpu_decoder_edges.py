@@ -222,3 +222,56 @@ def test_captured_attention_beside_larger_calls(nnhip):
         torch.cuda.synchronize()
         assert torch.equal(small[4], want)
     ctx.close()
+
+
+@pytest.mark.parametrize("paged", [True, False])
+def test_captured_prompt_beside_others(nnhip, paged):
+    """A captured prompt (the chunks of a server's loop) replays beside eager ones of fewer and of more tokens, which need
+    other views of the decoder's scratch, and larger ones: the logits, ids and cached rows of an eager run."""
+    import torch
+    print(f"captured prompt beside others paged={paged}", flush=True)
+    ctx = nnhip.Context(0)
+    B, T = 3, 40
+    cfg, base = model(ctx, nnhip, B, 0xF7, max_len=600)
+    runs = []
+    for captured in (True, False):
+        dec = decoder(ctx, nnhip, cfg, base, B, paged, page=64)
+
+        def prompt(ids, n, T):
+            if paged:
+                return dec.prefill_packed(ids, n, T)
+            return dec.prefill(ids, T)
+
+        ids = torch.zeros(B * T, dtype=torch.int32, device="cuda")
+        n = dev(np.array([0, 7, 40, B * T], np.int32))
+        bound = 80 if paged else T
+        side = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            prompt(ids, n, bound)
+        torch.cuda.synchronize()
+        if captured:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                logits, got = prompt(ids, n, bound)
+        trace, kept = [], []
+        for i, other in enumerate((None, 9, None, 200, 501, None, 300)):
+            if other:  # an eager prompt of other sizes
+                x = dev((np.arange(B * other, dtype=np.int32) * 5 + i) % cfg.vocab)
+                prompt(x, dev(np.arange(B + 1, dtype=np.int32) * other), other)
+                torch.cuda.synchronize()
+                kept.append(scribble())
+            ids.copy_(dev((np.arange(B * T, dtype=np.int32) * 3 + i) % cfg.vocab))
+            torch.cuda.synchronize()
+            if captured:
+                g.replay()
+            else:
+                with torch.cuda.stream(side):
+                    logits, got = prompt(ids, n, bound)
+            torch.cuda.synchronize()
+            trace.append((host(logits).copy(), host(got).copy(), cached(dec, 2, 40)))
+        runs.append(trace)
+    for (x0, i0, c0), (x1, i1, c1) in zip(*runs):
+        assert np.all(np.isfinite(x0)) and np.array_equal(x0, x1) and np.array_equal(i0, i1)
+        assert all(same(a, b) for a, b in zip(c0, c1))
+    ctx.close()
