@@ -2125,7 +2125,7 @@ nnhip_status nnhip_attention_pages_prefill(nnhip_ctx* ctx, const nnhip_kv_pages*
 
 size_t nnhip_logits_workspace_bytes(nnhip_ctx* ctx, size_t V, size_t B)
 {
-    return !ctx || V == 0 ? 0 : logits_workspace_bytes(V, B, (size_t)ctx->num_cus);
+    return !ctx || V == 0 || B == 0 ? 0 : logits_workspace_bytes(V, B, (size_t)ctx->num_cus);
 }
 
 nnhip_status nnhip_logits_adjust_rows(nnhip_ctx* ctx, const float* logits, size_t V, size_t B,

@@ -114,3 +114,18 @@ def test_decode_extreme_queries_and_caps(ctx, nnhip, H, Hkv, dk, f16, size, cap,
             # equal weights (scores below 1e-28 change none): attend64's bound of the sums, nothing of the scores
             tol = 2.0 ** -24 * (4 * np.sqrt(n + 1) + 40 + 16) * np.abs(x).mean(0)
             assert np.all(np.abs(out[b, h] - x.mean(0)) <= tol), (b, h)
+
+
+def test_workspace_queries(ctx, nnhip):
+    """Of no sequence, of short rows and short caches (nothing), of long ones (per sequence), of arguments that fit
+    nothing."""
+    for B in (0, 1, 64, 65535):
+        assert ctx.logits_workspace_bytes(0, B) == ctx.logits_workspace_bytes(10000, B) == 0
+        assert ctx.attention_pages_workspace_bytes(B, 8, 2, 64, 128) == 0
+        assert ctx.attention_pages_workspace_bytes(B, 8, 2, 64, 0) == ctx.attention_pages_workspace_bytes(B, 8, 3, 64, 999) == 0
+        assert ctx.attention_pages_workspace_bytes(B, 0, 2, 64, 999) == ctx.attention_pages_workspace_bytes(B, 8, 0, 64, 999) == 0
+    assert ctx.logits_workspace_bytes(131071, 0) == ctx.attention_pages_workspace_bytes(0, 8, 2, 64, 9999) == 0
+    for B in (1, 64, 1024):
+        assert ctx.logits_workspace_bytes(131071, B) >= 16 * B  # two slices a row at least
+        assert ctx.attention_pages_workspace_bytes(B, 8, 2, 64, 9999) >= B * 8 * 64 * 4  # a record a head at least
+    assert ctx.logits_workspace_bytes(131071, 65535) == 0  # a row a work-group
