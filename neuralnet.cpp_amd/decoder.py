@@ -205,12 +205,12 @@ class Decoder:
             self._pf_M = M
         return self._pf
 
-    def prefill(self, ids, T: int, pos0: int = 0, hook=None):
+    def prefill(self, ids, T: int, pos0: int = 0, hook=None, rules=None):
         """T tokens of each of the B sequences, at positions pos0 .. pos0 + T - 1, through every block
         in one pass: the caches get rows pos0 .. pos0 + T - 1 and every token the result of its own
         step(). ids: (B*T,) int32 device tensor, token column b*T + t. hook(i, name, tensor) sees each
         block's q / k / v / attention output / block output (tests). Returns (logits (vocab, B), greedy
-        ids (B,)) of each sequence's last token."""
+        ids (B,)) of each sequence's last token, chosen under rules (a LogitRules) as step() does."""
         cfg, ctx, B = self.cfg, self.ctx, self.B
         if self.paged:
             raise _pkg().NNHipError(1, "paged caches take prompts through prefill_packed")
@@ -224,7 +224,7 @@ class Decoder:
                                   out=pf["a"])
 
         ctx.copy_columns(self._prefill_blocks(ids, M, attend, hook), T - 1, T, B, out=self.x)
-        return self._prefill_head()
+        return self._prefill_head(rules)
 
     def _prefill_blocks(self, ids, M: int, attend, hook):
         """Every block over the M tokens ids; attend(i) turns block i's q, k, v into its attention output."""
@@ -262,20 +262,25 @@ class Decoder:
                 hook(i, "x", x)
         return x
 
-    def _prefill_head(self):
-        """Logits and greedy ids of the last tokens in self.x."""
+    def _prefill_head(self, rules=None, live=None):
+        """Logits and greedy ids of the last tokens in self.x; with rules, the choice under them (live: (B,) int32, below 0
+        for a sequence whose choice is not counted)."""
         self._quant(self.x, self.g_final)
         self._mm(self.head, self._logits_cols)
-        self.ctx.argmax_cols(self._logits_cols, out=self.ids)
+        if rules is None:
+            self.ctx.argmax_cols(self._logits_cols, out=self.ids)
+        else:
+            self.ctx.logits_adjust_rows(self._logits_cols.t().contiguous(), rules, ids=self.ids, pos=live)
         self._logits = self._logits_cols
         return self._logits, self.ids
 
-    def prefill_packed(self, ids, cu, t_bound: int, pos0=None, hook=None):
+    def prefill_packed(self, ids, cu, t_bound: int, pos0=None, hook=None, rules=None):
         """Prompts of unlike lengths into paged caches: ids (M,) int32 holds the tokens of sequence b in
         ids[cu[b] .. cu[b+1] - 1] (cu (B + 1,) int32 device, at most t_bound each), at positions pos0[b] on (pos0 (B,)
         int32 device, None: 0). Every token gets the result of its own step(). hook as prefill(). Returns (logits
         (vocab, B), greedy ids (B,)) of each sequence's last token; those of a sequence without tokens (a slot
-        whose cache stays as it is) mean nothing."""
+        whose cache stays as it is) mean nothing. rules: a LogitRules for the choice, as step()'s: -1 where
+        its mask allows nothing, the other choices counted (if it counts them) but for sequences without tokens."""
         import torch
         cfg, ctx = self.cfg, self.ctx
         if not self.paged:
@@ -295,7 +300,7 @@ class Decoder:
         x = self._prefill_blocks(ids, ids.shape[0], attend, hook)
         # (an empty first sequence, or offsets past the tokens, would be an index outside x)
         torch.index_select(x, 1, (cu[1:] - 1).clamp(0, ids.shape[0] - 1).long(), out=self.x)
-        return self._prefill_head()
+        return self._prefill_head(rules, None if rules is None else (cu[1:] > cu[:-1]).int() - 1)
 
     def _mm(self, lin: Linear, out):
         return self.ctx.ternary_matmul(lin.rp, lin.tau, self.xi, self.s, self.rs, lin.N, lin.K, self.B,

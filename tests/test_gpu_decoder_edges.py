@@ -275,3 +275,57 @@ def test_captured_prompt_beside_others(nnhip, paged):
         assert np.all(np.isfinite(x0)) and np.array_equal(x0, x1) and np.array_equal(i0, i1)
         assert all(same(a, b) for a, b in zip(c0, c1))
     ctx.close()
+
+
+def test_first_token_under_rules(ctx, nnhip):
+    """prefill_packed's choice under rules: penalties, bias and masks as step()'s, the chosen tokens counted,
+    nothing counted for a slot without tokens; the ids go on into steps."""
+    import torch
+    B = 5
+    cfg, base = model(ctx, nnhip, B, 0xD1)
+    lens = [7, 0, 20, 1, 0]
+    rng = np.random.default_rng(3)
+    cu = np.concatenate(([0], np.cumsum(lens))).astype(np.int32)
+    prompt = rng.integers(0, cfg.vocab, int(cu[-1])).astype(np.int32)
+    live = np.flatnonzero(lens)
+    counts = np.zeros((B, cfg.vocab), np.int32)
+    for b in range(B):
+        np.add.at(counts[b], prompt[cu[b]:cu[b + 1]], 1)
+    kw = dict(repeat=np.full(B, 1.5, np.float32), presence=np.full(B, 0.3, np.float32),
+              frequency=np.full(B, 0.2, np.float32), bias=rng.standard_normal((1, cfg.vocab)).astype(np.float32))
+    words = np.full((B, 4), 0xAAAAAAAA, np.uint32)
+    words[3] = 0  # nothing is allowed
+    dec = decoder(ctx, nnhip, cfg, base, B)
+    counts_d = torch.zeros(B, cfg.vocab, dtype=torch.int32, device="cuda")
+    ctx.token_counts_add(dev(prompt), dev(cu), counts_d)
+    words_d = dev(words.view(np.int32))
+    rule = nnhip.LogitRules(cfg.vocab, counts=counts_d, count_choice=True, allowed=words_d,
+                            **{k: dev(v) for k, v in kw.items()})
+    logits, ids = dec.prefill_packed(dev(prompt), dev(cu), 20, rules=rule)
+    want = apply_rules(host(logits).T.copy(), counts=counts, allowed=words, **kw)[1]
+    got = host(ids).copy()
+    assert np.array_equal(got[live], want[live]) and got[3] == -1 and np.all(got[[0, 2]] % 2 == 1)
+    for b in (0, 2):
+        counts[b, got[b]] += 1
+    assert np.array_equal(host(counts_d), counts)
+    plain = decoder(ctx, nnhip, cfg, base, B)
+    same_logits, free = plain.prefill_packed(dev(prompt), dev(cu), 20)
+    assert np.array_equal(host(same_logits)[:, live], host(logits)[:, live])
+    assert np.array_equal(host(free)[live], host(logits).argmax(0)[live])
+
+
+def test_first_token_under_rules_of_equal_prompts(ctx, nnhip):
+    """The same for prefill() into contiguous caches."""
+    import torch
+    B, T = 3, 11
+    cfg, base = model(ctx, nnhip, B, 0xD3)
+    prompt = np.random.default_rng(4).integers(0, cfg.vocab, (B, T)).astype(np.int32)
+    counts = np.stack([np.bincount(x, minlength=cfg.vocab) for x in prompt]).astype(np.int32)
+    words, repeat = np.full((1, 4), 0x55555555, np.uint32), np.full(B, 1.5, np.float32)
+    counts_d = dev(counts)
+    rule = nnhip.LogitRules(cfg.vocab, counts=counts_d, repeat=dev(repeat), allowed=dev(words.view(np.int32)), count_choice=True)
+    logits, ids = decoder(ctx, nnhip, cfg, base, B, paged=False).prefill(dev(prompt.reshape(-1)), T, rules=rule)
+    want = apply_rules(host(logits).T.copy(), counts=counts, repeat=repeat, allowed=words)[1]
+    assert np.array_equal(host(ids), want) and np.all(want % 2 == 0)
+    counts[np.arange(B), want] += 1
+    assert np.array_equal(host(counts_d), counts)
