@@ -707,8 +707,8 @@ nnhip_status nnhip_attention_pages_decode(nnhip_ctx* ctx, const nnhip_kv_pages* 
 
 /* Attention of packed prompts over pages that hold the keys and values of all their positions (after
  * nnhip_kv_pages_fill): q and out (H*dk, M) feature-major, columns cu[b] .. cu[b+1] - 1 = the tokens of
- * sequence b at positions pos0[b] + t (cu, pos0 as nnhip_kv_pages_fill's; pos0 may be NULL); t_bound bounds
- * every sequence's tokens (it sizes the launch). A token at position i sees its own sequence's positions
+ * sequence b at positions pos0[b] + t (cu, pos0 as nnhip_kv_pages_fill's; pos0 may be NULL); t_bound, at most M,
+ * bounds every sequence's tokens (it sizes the launch). A token at position i sees its own sequence's positions
  * j <= i, and with prefix (DEVICE (B) int32, or NULL) also every j < prefix[b] that the sequence has;
  * nothing of another sequence. Scores, softcap and slopes as nnhip_attention_pages_decode (j - i is above
  * 0 inside a prefix); products, sums, errors and the f32 products' cases as nnhip_attention_prefill, but for

@@ -985,8 +985,8 @@ class Context:
 
     def attention_pages_prefill(self, cache, q, cu, t_bound: int, H: int, scale: float, pos0=None, cos=None, sin=None,
                                 softcap: float = 0.0, slopes=None, prefix=None, out=None):
-        """Attention of packed prompts q (H*dk, M) (sequence b: columns cu[b] .. cu[b+1] - 1, at most t_bound of them,
-        positions pos0[b] on) over the pages of cache, which hold all their positions: causal, and bidirectional
+        """Attention of packed prompts q (H*dk, M) (sequence b: columns cu[b] .. cu[b+1] - 1, at most t_bound <= M of
+        them, positions pos0[b] on) over the pages of cache, which hold all their positions: causal, and bidirectional
         over the first prefix[b] positions (prefix (B) int32, or None). Returns out (H*dk, M)."""
         B, cu_p, pos0_p = self._packed(cache, cu, pos0)
         f32, M = self._torch.float32, q.shape[-1]

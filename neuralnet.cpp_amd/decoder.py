@@ -276,11 +276,12 @@ class Decoder:
 
     def prefill_packed(self, ids, cu, t_bound: int, pos0=None, hook=None, rules=None):
         """Prompts of unlike lengths into paged caches: ids (M,) int32 holds the tokens of sequence b in
-        ids[cu[b] .. cu[b+1] - 1] (cu (B + 1,) int32 device, at most t_bound each), at positions pos0[b] on (pos0 (B,)
-        int32 device, None: 0). Every token gets the result of its own step(). hook as prefill(). Returns (logits
-        (vocab, B), greedy ids (B,)) of each sequence's last token; those of a sequence without tokens (a slot
-        whose cache stays as it is) mean nothing. rules: a LogitRules for the choice, as step()'s: -1 where
-        its mask allows nothing, the other choices counted (if it counts them) but for sequences without tokens."""
+        ids[cu[b] .. cu[b+1] - 1] (cu (B + 1,) int32 device, at most t_bound each; the bound may be past M), at
+        positions pos0[b] on (pos0 (B,) int32 device, None: 0). Every token gets the result of its own step(). hook
+        as prefill(). Returns (logits (vocab, B), greedy ids (B,)) of each sequence's last token; those of a sequence
+        without tokens (a slot whose cache stays as it is) mean nothing. rules: a LogitRules for the choice, as
+        step()'s: -1 where its mask allows nothing, the other choices counted (if it counts them) but for sequences
+        without tokens."""
         import torch
         cfg, ctx = self.cfg, self.ctx
         if not self.paged:
@@ -290,6 +291,7 @@ class Decoder:
         if ids.shape[0] < 1:
             raise _pkg().NNHipError(1, "prefill_packed needs a token")
         pf = self._prefill_buffers(ids.shape[0])
+        t_bound = min(t_bound, ids.shape[0])
 
         def attend(i):
             cache = self.caches[i]

@@ -329,3 +329,12 @@ def test_first_token_under_rules_of_equal_prompts(ctx, nnhip):
     assert np.array_equal(host(ids), want) and np.all(want % 2 == 0)
     counts[np.arange(B), want] += 1
     assert np.array_equal(host(counts_d), counts)
+
+
+def test_prompt_bound_past_the_tokens(ctx, nnhip):
+    """t_bound only bounds the sequences' tokens: a constant one of a server is no error for a short packing."""
+    cfg, base = model(ctx, nnhip, 2, 0xE1)
+    ids, cu = dev(np.arange(5, dtype=np.int32)), dev(np.array([0, 2, 5], np.int32))
+    outs = [decoder(ctx, nnhip, cfg, base, 2).prefill_packed(ids, cu, t) for t in (3, 5, 6, 4096)]
+    for logits, got in outs[1:]:
+        assert np.array_equal(host(logits), host(outs[0][0])) and np.array_equal(host(got), host(outs[0][1]))
