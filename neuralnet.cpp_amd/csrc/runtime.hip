@@ -2101,7 +2101,7 @@ nnhip_status nnhip_attention_pages_prefill(nnhip_ctx* ctx, const nnhip_kv_pages*
     nnhip_status st = check_pages(fn, cache, rope_cos, rope_sin);
     if (st != NNHIP_OK) return st;
     if (!prefill_dk_supported(cache->dk)) return fail(NNHIP_ERR_UNSUPPORTED, fn, "dk must be 64 or 128");
-    if (M == 0 || B == 0 || t_bound == 0) return NNHIP_OK;
+    if (M == 0 || B == 0) return NNHIP_OK;
     NNHIP_REQUIRE(q && cu && out, fn, "null pointer");
     NNHIP_REQUIRE(H >= cache->Hkv && H % cache->Hkv == 0 && H <= 65535, fn,
                   "H must be a multiple of Hkv, at most 65535");

@@ -129,3 +129,21 @@ def test_workspace_queries(ctx, nnhip):
         assert ctx.logits_workspace_bytes(131071, B) >= 16 * B  # two slices a row at least
         assert ctx.attention_pages_workspace_bytes(B, 8, 2, 64, 9999) >= B * 8 * 64 * 4  # a record a head at least
     assert ctx.logits_workspace_bytes(131071, 65535) == 0  # a row a work-group
+
+
+@pytest.mark.parametrize("width", [8, 40])  # 128 positions: a work-group a block of queries; 640: equal spans
+@pytest.mark.parametrize("dk,f16", [(64, False), (128, True)])
+def test_prompt_bound_of_no_tokens(ctx, nnhip, width, dk, f16):
+    """t_bound = 0 over sequences without tokens: nothing is written; over sequences with some: theirs are NaN, as any
+    that has more than the bound."""
+    import torch
+    rng = np.random.default_rng(31)
+    H, Hkv, page, M = 4, 2, 16, 20
+    c = Cache(rng, [64, 64, 64], Hkv, page, dk, f16, width=width)
+    q = dev(rng.standard_normal((H * dk, M)).astype(np.float32))
+    for cu, bad in (([0, 0, 0, 0], []), ([3, 3, 4, 9], list(range(3, 9)))):
+        out = torch.full((H * dk, M), 7.0, device="cuda")
+        ctx.attention_pages_prefill(c.on_device(nnhip), q, dev(np.array(cu, np.int32)), 0, H, 0.125, out=out)
+        got = host(out)
+        rest = [m for m in range(M) if m not in bad]
+        assert np.all(np.isnan(got[:, bad])) and np.all(got[:, rest] == 7.0)
