@@ -710,20 +710,28 @@ nnhip_status nnhip_attention_pages_decode(nnhip_ctx* ctx, const nnhip_kv_pages* 
  * sequence b at positions pos0[b] + t (cu, pos0 as nnhip_kv_pages_fill's; pos0 may be NULL); t_bound, at most M,
  * bounds every sequence's tokens (it sizes the launch). A token at position i sees its own sequence's positions
  * j <= i, and with prefix (DEVICE (B) int32, or NULL) also every j < prefix[b] that the sequence has;
- * nothing of another sequence. Scores, softcap and slopes as nnhip_attention_pages_decode (j - i is above
- * 0 inside a prefix); products, sums, errors and the f32 products' cases as nnhip_attention_prefill, but for
- * f16 pools, whose weights are held to 2^-22 of themselves down to 2^-29 of the largest in their run of 32
- * keys and to 2^-51 of that one below (outputs so small that this could show take the f32 products). The
- * sums' order depends on all sequences of the call. dk in
- * {64, 128}, any H / Hkv, H * dk * M < 2^29. Columns of no sequence are not written. NaN: a sequence with
- * more than t_bound tokens, columns outside [0, M) or positions at or past table_stride * page_size or
- * rope_len; a query that sees a position whose page is outside the pool (other queries of its sequence
- * may be NaN then, too). The paged form of nnhip_attention_prefill
- * (compute_layer_attention.hpp:1022-1083). */
+ * nothing of another sequence. Scores, softcap and slopes as nnhip_attention_pages_decode: the bias is linear in
+ * the position, so keys ahead of the query, inside a prefix, gain by it (a model whose bias falls with the
+ * distance on both sides takes nnhip_attention_pages_prefill_distance). Products, sums, errors and the f32
+ * products' cases as nnhip_attention_prefill, but for f16 pools, whose weights are held to 2^-22 of themselves
+ * down to 2^-29 of the largest in their run of 32 keys and to 2^-51 of that one below (outputs so small that this
+ * could show take the f32 products). The sums' order depends on all sequences of the call. dk in {64, 128}, any
+ * H / Hkv, H * dk * M < 2^29. Columns of no sequence are not written. NaN: a sequence with more than t_bound
+ * tokens, columns outside [0, M) or positions at or past table_stride * page_size or rope_len; a query that sees
+ * a position whose page is outside the pool (other queries of its sequence may be NaN then, too). The paged form
+ * of nnhip_attention_prefill (compute_layer_attention.hpp:1022-1083). */
 nnhip_status nnhip_attention_pages_prefill(nnhip_ctx* ctx, const nnhip_kv_pages* cache, const float* q, size_t M,
                                            const int32_t* cu, const int32_t* pos0, size_t B, size_t t_bound, size_t H,
                                            const float* rope_cos, const float* rope_sin, size_t rope_len, float scale,
                                            float softcap, const float* slopes, const int32_t* prefix, float* out);
+
+/* nnhip_attention_pages_prefill with the bias of the distance, s -= slopes[h] * |j - i|, for keys on both sides of the
+ * query. Where prefix is NULL no key is ahead, and both give the same bits. */
+nnhip_status nnhip_attention_pages_prefill_distance(nnhip_ctx* ctx, const nnhip_kv_pages* cache, const float* q, size_t M,
+                                                    const int32_t* cu, const int32_t* pos0, size_t B, size_t t_bound,
+                                                    size_t H, const float* rope_cos, const float* rope_sin, size_t rope_len,
+                                                    float scale, float softcap, const float* slopes, const int32_t* prefix,
+                                                    float* out);
 
 /* Scratch that nnhip_attention_pages_decode (nnhip_logits_adjust_rows) of these sizes uses;
  * nnhip_attention_pages_prefill uses 2 * (dk + 2) KiB and 16 bytes for each CU where the table (and the rope tables) hold

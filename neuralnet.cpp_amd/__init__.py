@@ -168,6 +168,8 @@ SIGNATURES = {
                                            _st, _vp]),
     "nnhip_attention_pages_prefill": (_st, [_vp, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _vp, _vp, _sz, _f, _f, _vp,
                                             _vp, _vp]),
+    "nnhip_attention_pages_prefill_distance": (_st, [_vp, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _vp, _vp, _sz, _f, _f,
+                                                     _vp, _vp, _vp]),
     "nnhip_attention_pages_workspace_bytes": (_sz, [_vp, _sz, _sz, _sz, _sz, _sz]),
     "nnhip_logits_workspace_bytes": (_sz, [_vp, _sz, _sz]),
     "nnhip_logits_adjust_rows": (_st, [_vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp]),
@@ -984,10 +986,12 @@ class Context:
         return out
 
     def attention_pages_prefill(self, cache, q, cu, t_bound: int, H: int, scale: float, pos0=None, cos=None, sin=None,
-                                softcap: float = 0.0, slopes=None, prefix=None, out=None):
+                                softcap: float = 0.0, slopes=None, prefix=None, out=None, distance: bool = False):
         """Attention of packed prompts q (H*dk, M) (sequence b: columns cu[b] .. cu[b+1] - 1, at most t_bound <= M of
         them, positions pos0[b] on) over the pages of cache, which hold all their positions: causal, and bidirectional
-        over the first prefix[b] positions (prefix (B) int32, or None). Returns out (H*dk, M)."""
+        over the first prefix[b] positions (prefix (B) int32, or None). slopes (H) bias the scores by
+        slopes[h] * (j - i), or with distance by -slopes[h] * |j - i|: for keys ahead of the query, inside a prefix,
+        these differ. Returns out (H*dk, M)."""
         B, cu_p, pos0_p = self._packed(cache, cu, pos0)
         f32, M = self._torch.float32, q.shape[-1]
         shape = (H * cache.dk, M)
@@ -995,10 +999,11 @@ class Context:
             out = self._empty(shape, f32)
         cs, sn, rows = self._rope(cos, sin, cache.dk)
         self._bind_stream()
-        _check(lib().nnhip_attention_pages_prefill(
+        fn = "nnhip_attention_pages_prefill_distance" if distance else "nnhip_attention_pages_prefill"
+        _check(getattr(lib(), fn)(
             self.h, cache.ref, self._arg(q, f32, shape, "q"), M, cu_p, pos0_p, B, t_bound, H, cs, sn, rows, scale,
             softcap, self._arg(slopes, f32, (H,), "slopes"), self._arg(prefix, self._torch.int32, (B,), "prefix"),
-            self._arg(out, f32, shape, "out")), "nnhip_attention_pages_prefill")
+            self._arg(out, f32, shape, "out")), fn)
         return out
 
     def attention_pages_workspace_bytes(self, B: int, H: int, Hkv: int, dk: int, len_bound: int) -> int:

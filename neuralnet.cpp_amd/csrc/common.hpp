@@ -423,7 +423,7 @@ hipError_t launch_pages_fill(hipStream_t st, const nnhip_kv_pages& kv, const flo
 hipError_t launch_pages_prefill(hipStream_t st, const nnhip_kv_pages& kv, const float* q, size_t M, const int32_t* cu,
                                 const int32_t* pos0, size_t B, size_t t_bound, size_t H, const float* cosT,
                                 const float* sinT, size_t limit, float scale, float softcap, const float* slopes,
-                                const int32_t* prefix, float* out, void* ws, size_t num_cus);
+                                const int32_t* prefix, bool distance, float* out, void* ws, size_t num_cus);
 size_t pages_prefill_spans(size_t limit, size_t num_cus);
 size_t pages_prefill_workspace_bytes(size_t dk, size_t limit, size_t num_cus);
 size_t logits_slices(size_t V, size_t B, size_t num_cus);

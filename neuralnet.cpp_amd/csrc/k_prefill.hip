@@ -53,8 +53,8 @@
 // 198 us at 4 x 2048.
 //
 // Over pages (kPaged): packed sequences of unlike lengths, each at its own position, whose rows are found
-// through a page table read a tile ahead; a prefix that all queries see, a tanh cap and a distance bias on
-// the scores. Any H / Hkv: a KV head's heads go in groups of 8, 4, 2 or 1.
+// through a page table read a tile ahead; a prefix that all queries see, a tanh cap and a bias on the scores, linear in
+// the position or (kDistance: they differ for keys ahead of the query, inside a prefix) in the distance. Any H / Hkv: a KV head's heads go in groups of 8, 4, 2 or 1.
 //   * Work-groups take equal spans of all tiles of the call (prompt_cut) and join the blocks of queries
 //     they share; a plain work-group per block of queries left most CUs idle behind a long sequence, or
 //     behind the 14 blocks beyond 256 (4 x 700 .. 1024 tokens at 6144, f16: 1087 -> 754 us).
@@ -495,7 +495,7 @@ __device__ __forceinline__ size_t paged_row(const PrefillArgs& a, const PrefillW
 // Paged: a NaN or an infinity among the values of a key that one query sees and another does not must
 // not reach the other, whose probability of 0 a matrix product would multiply with it; tiles that reach
 // past some query's sight therefore add their values key by key.
-template <int DK, bool kPaged, bool kShaped, typename CT>
+template <int DK, bool kPaged, bool kShaped, bool kDistance, typename CT>
 __device__ void attend_f32(const PrefillArgs& a, const PrefillWave& w, const PrefillSeq<kPaged>& seq, int last_key,
                            int k0, int k1, float* rec, __amdgpu_buffer_rsrc_t rk, __amdgpu_buffer_rsrc_t rv, float* ks, int tid)
 {
@@ -566,7 +566,8 @@ __device__ void attend_f32(const PrefillArgs& a, const PrefillWave& w, const Pre
             if constexpr (kShaped)
             {
                 if (a.cap2 > 0.0f) x = a.cap2 * 0.69314718f * tanh_any(x * (a.capi2 * 1.44269504f));
-                if (a.slopes) x += a.slopes[w.head] * (float)(key - w.qpos);
+                const float away = (float)(key - w.qpos);
+                if (a.slopes) x += a.slopes[w.head] * (kDistance ? -fabsf(away) : away);
             }
             sc[v] = key <= seq.sight(w) ? x : -__builtin_inff();
             mx = fmaxf(mx, sc[v]);
@@ -862,7 +863,7 @@ __device__ __forceinline__ PromptCut* prompt_cuts(const PrefillArgs& a, int span
 }
 
 // Attention of an item over its tiles k0 .. k1 - 1; rec: into a record instead of the output
-template <int DK, bool kPaged, bool kShaped, typename CT>
+template <int DK, bool kPaged, bool kShaped, bool kDistance, typename CT>
 __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& item, uint8_t* smem, int k0, int k1, float* rec)
 {
     constexpr bool F32C = sizeof(CT) == 4;
@@ -1351,10 +1352,15 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
                         for (int v = 0; v < 16; ++v) s[v] = tanh_any(s[v]);
                     }
                 }
-                // (the distance of the tile's first key and the steps from there apart: a step costs one multiply-add)
-                const float unit = a.cap2 > 0.0f ? a.cap2 : 1.0f, away = slope2 * (float)(kb * kPK + 4 * h - w.qpos);
+                // (the distance of the tile's first key and the steps from there apart: a step costs one multiply-add; kDistance:
+                // and a change of sign, 107 us instead of 102 at 8 x 77 .. 1900 tokens, 16 heads over 2 of 64)
+                const float unit = a.cap2 > 0.0f ? a.cap2 : 1.0f, first = (float)(kb * kPK + 4 * h - w.qpos), away = slope2 * first;
 #pragma unroll
-                for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(s[v], unit, __builtin_fmaf(slope2, (float)(8 * (v >> 2) + (v & 3)), away));
+                for (int v = 0; v < 16; ++v)
+                {
+                    const float step = (float)(8 * (v >> 2) + (v & 3)), bias = __builtin_fmaf(slope2, step, away);
+                    s[v] = __builtin_fmaf(s[v], unit, kDistance && first + step > 0.0f ? -bias : bias);
+                }
                 f = 1.0f;
             }
             float low = 0.0f;  // kHalf: the lane's lowest score (masked ones, too)
@@ -1558,7 +1564,7 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
         int last2;
         if constexpr (kPaged) seat(a, item, t2, w2, seq2, last2);
         else w2 = w, seq2 = seq, last2 = last_key;
-        attend_f32<DK, kPaged, kShaped, CT>(a, w2, seq2, last2, k0, k1, rec, rk, rv, reinterpret_cast<float*>(smem), kPaged ? t2 : tid);
+        attend_f32<DK, kPaged, kShaped, kDistance, CT>(a, w2, seq2, last2, k0, k1, rec, rk, rv, reinterpret_cast<float*>(smem), kPaged ? t2 : tid);
         return;
     }
     if constexpr (kPaged)
@@ -1579,7 +1585,7 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
     });
 }
 
-template <int DK, bool kPaged, bool kShaped, typename CT>
+template <int DK, bool kPaged, bool kShaped, typename CT, bool kDistance = false>
 __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
 {
     extern __shared__ __align__(16) uint8_t smem[];
@@ -1595,7 +1601,7 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
         it.g = bg % a.Hkv;
         it.first = it.g * a.R;
         it.qb = a.nqb - 1 - back;
-        attend<DK, kPaged, kShaped, CT>(a, it, smem, 0, 0, nullptr);
+        attend<DK, kPaged, kShaped, kDistance, CT>(a, it, smem, 0, 0, nullptr);
     }
     else
     {
@@ -1650,7 +1656,7 @@ __global__ __launch_bounds__(kPThreads) void k_attn_prefill(PrefillArgs a)
             it.first = at.gh * a.R;
             it.qb = at.qb;
             float* rec = at.t == 0 && to == tiles ? nullptr : prompt_record<DK>(a, g, at.t > 0 ? 0 : 1);
-            attend<DK, kPaged, kShaped, CT>(a, it, smem, at.t, to, rec);
+            attend<DK, kPaged, kShaped, kDistance, CT>(a, it, smem, at.t, to, rec);
             known = false;
             at = {at.gh, at.b, at.qb + 1, 0};
         }
@@ -1697,20 +1703,20 @@ __global__ __launch_bounds__(32 * kPWaves) void k_prompt_join(PrefillArgs a)
     for (int i = 0; i < N; ++i) out[(size_t)i * (size_t)a.M] = den == 0.0f ? 0.0f : y[i] / den;
 }
 
-template <int DK, bool kPaged, bool kShaped, typename CT>
+template <int DK, bool kPaged, bool kShaped, typename CT, bool kDistance = false>
 hipError_t launch_prefill_dk(hipStream_t st, const PrefillArgs& a)
 {
     constexpr int lds = PrefillTile<DK, CT, kPaged && sizeof(CT) == 2>::kBytes;
     static bool attr_set = false;
     if (!attr_set)
     {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_attn_prefill<DK, kPaged, kShaped, CT>),
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_attn_prefill<DK, kPaged, kShaped, CT, kDistance>),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
         attr_set = true;
     }
     const unsigned blocks = kPaged && a.spans ? (unsigned)a.spans : (unsigned)(a.nqb * a.B * a.Hkv * a.groups);
-    hipLaunchKernelGGL((k_attn_prefill<DK, kPaged, kShaped, CT>), dim3(blocks), dim3(kPThreads), lds, st, a);
+    hipLaunchKernelGGL((k_attn_prefill<DK, kPaged, kShaped, CT, kDistance>), dim3(blocks), dim3(kPThreads), lds, st, a);
     if constexpr (kPaged)
         if (a.spans > 1)
         {
@@ -1786,7 +1792,7 @@ size_t pages_prefill_workspace_bytes(size_t dk, size_t limit, size_t num_cus)
 hipError_t launch_pages_prefill(hipStream_t st, const nnhip_kv_pages& kv, const float* q, size_t M, const int32_t* cu,
                                 const int32_t* pos0, size_t B, size_t t_bound, size_t H, const float* cosT,
                                 const float* sinT, size_t limit, float scale, float softcap, const float* slopes,
-                                const int32_t* prefix, float* out, void* ws, size_t num_cus)
+                                const int32_t* prefix, bool distance, float* out, void* ws, size_t num_cus)
 {
     // a KV head's R query heads in work-groups of 8, 4, 2 or 1
     const size_t heads = H / kv.Hkv, R = heads % 8 == 0 ? 8 : heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
@@ -1799,6 +1805,14 @@ hipError_t launch_pages_prefill(hipStream_t st, const nnhip_kv_pages& kv, const 
                   0, (int)limit, (float)cap2, softcap > 0.0f ? (float)(1.0 / cap2) : 0.0f,
                   static_cast<float*>(ws), (int)pages_prefill_spans(limit, num_cus)};
     while ((size_t(1) << a.shift) < kv.page_size) ++a.shift;
+    // (a key ahead of its query is inside a prefix: without one the two biases are the same)
+    if (slopes && prefix && distance)
+    {
+        if (kv.f16)
+            return kv.dk == 64 ? launch_prefill_dk<64, true, true, _Float16, true>(st, a)
+                               : launch_prefill_dk<128, true, true, _Float16, true>(st, a);
+        return kv.dk == 64 ? launch_prefill_dk<64, true, true, float, true>(st, a) : launch_prefill_dk<128, true, true, float, true>(st, a);
+    }
     if (cap2 > 0.0 || slopes)
     {
         if (kv.f16)

@@ -2091,12 +2091,12 @@ nnhip_status nnhip_attention_pages_decode(nnhip_ctx* ctx, const nnhip_kv_pages* 
     return NNHIP_OK;
 }
 
-nnhip_status nnhip_attention_pages_prefill(nnhip_ctx* ctx, const nnhip_kv_pages* cache, const float* q, size_t M,
-                                           const int32_t* cu, const int32_t* pos0, size_t B, size_t t_bound, size_t H,
-                                           const float* rope_cos, const float* rope_sin, size_t rope_len, float scale,
-                                           float softcap, const float* slopes, const int32_t* prefix, float* out)
+static nnhip_status attention_pages_prefill(nnhip_ctx* ctx, const char* fn, const nnhip_kv_pages* cache, const float* q, size_t M,
+                                            const int32_t* cu, const int32_t* pos0, size_t B, size_t t_bound, size_t H,
+                                            const float* rope_cos, const float* rope_sin, size_t rope_len, float scale,
+                                            float softcap, const float* slopes, const int32_t* prefix, bool distance,
+                                            float* out)
 {
-    const char* fn = "nnhip_attention_pages_prefill";
     NNHIP_CHECK_CTX(fn);
     nnhip_status st = check_pages(fn, cache, rope_cos, rope_sin);
     if (st != NNHIP_OK) return st;
@@ -2119,8 +2119,27 @@ nnhip_status nnhip_attention_pages_prefill(nnhip_ctx* ctx, const nnhip_kv_pages*
     st = ensure_stream_ws(ctx, pages_prefill_workspace_bytes(cache->dk, limit, (size_t)ctx->num_cus), fn, &ws);
     if (st != NNHIP_OK) return st;
     NNHIP_LAUNCH(fn, launch_pages_prefill(ctx->stream, *cache, q, M, cu, pos0, B, t_bound, H, rope_cos, rope_sin, limit,
-                                          scale, softcap, slopes, prefix, out, ws, (size_t)ctx->num_cus));
+                                          scale, softcap, slopes, prefix, distance, out, ws, (size_t)ctx->num_cus));
     return NNHIP_OK;
+}
+
+nnhip_status nnhip_attention_pages_prefill(nnhip_ctx* ctx, const nnhip_kv_pages* cache, const float* q, size_t M,
+                                           const int32_t* cu, const int32_t* pos0, size_t B, size_t t_bound, size_t H,
+                                           const float* rope_cos, const float* rope_sin, size_t rope_len, float scale,
+                                           float softcap, const float* slopes, const int32_t* prefix, float* out)
+{
+    return attention_pages_prefill(ctx, "nnhip_attention_pages_prefill", cache, q, M, cu, pos0, B, t_bound, H, rope_cos,
+                                   rope_sin, rope_len, scale, softcap, slopes, prefix, false, out);
+}
+
+nnhip_status nnhip_attention_pages_prefill_distance(nnhip_ctx* ctx, const nnhip_kv_pages* cache, const float* q, size_t M,
+                                                    const int32_t* cu, const int32_t* pos0, size_t B, size_t t_bound,
+                                                    size_t H, const float* rope_cos, const float* rope_sin, size_t rope_len,
+                                                    float scale, float softcap, const float* slopes, const int32_t* prefix,
+                                                    float* out)
+{
+    return attention_pages_prefill(ctx, "nnhip_attention_pages_prefill_distance", cache, q, M, cu, pos0, B, t_bound, H,
+                                   rope_cos, rope_sin, rope_len, scale, softcap, slopes, prefix, true, out);
 }
 
 size_t nnhip_logits_workspace_bytes(nnhip_ctx* ctx, size_t V, size_t B)

@@ -147,3 +147,65 @@ def test_prompt_bound_of_no_tokens(ctx, nnhip, width, dk, f16):
         got = host(out)
         rest = [m for m in range(M) if m not in bad]
         assert np.all(np.isnan(got[:, bad])) and np.all(got[:, rest] == 7.0)
+
+
+def distance_ref(c, b, q, i, n, slope, cap, scale, prefix):
+    at = np.arange(n)
+    K, V = c.rows(b, n)
+    return attend64(q, K[:, 0], V[:, 0], scale, cap, slope, -np.abs(at - float(i)), (at <= i) | (at < prefix))
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("dk", [64, 128])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+def test_prompt_distance_bias(ctx, nnhip, cap, dk, f16):
+    """Biases that fall with the distance on both sides of the query, inside prefixes longer and shorter than a tile, than
+    the sequence, and of none; the first query of a prefix weighs its far end least, not most."""
+    print(f"distance bias cap={cap} dk={dk} f16={f16}", flush=True)
+    rng = np.random.default_rng(300 + dk)
+    H, lens, pos0, prefix = 4, [300, 40, 90, 33], [0, 20, 0, 100], [256, 50, 1000, 0]
+    cu = np.concatenate(([0], np.cumsum(lens))).astype(np.int32)
+    M = int(cu[-1])
+    c = Cache(rng, [p + n for p, n in zip(pos0, lens)], 1, 16, dk, f16)
+    q = rng.standard_normal((H, dk, M)).astype(np.float32)
+    slopes = (2.0 ** -np.array([0.5, 2.0, 5.0, 8.0])).astype(np.float32)
+    scale = float(np.float32(1 / np.sqrt(dk)))
+
+    def run(prefix, distance):
+        return host(ctx.attention_pages_prefill(
+            c.on_device(nnhip), dev(q.reshape(H * dk, M)), dev(cu), max(lens), H, scale, pos0=dev(np.array(pos0, np.int32)),
+            softcap=cap, slopes=dev(slopes), prefix=None if prefix is None else dev(np.array(prefix, np.int32)),
+            distance=distance)).reshape(H, dk, M)
+
+    out = run(prefix, True).astype(np.float64)
+    worst = 0.0
+    for b, n in enumerate(lens):
+        for t in sorted({0, 1, 31, 32, n // 2, n - 1}):
+            for h in range(H):
+                ref, tol = distance_ref(c, b, q[h, :, cu[b] + t].astype(np.float64), pos0[b] + t, pos0[b] + n,
+                                        float(slopes[h]), cap, scale, prefix[b])
+                worst = max(worst, float(np.max(np.abs(out[h, :, cu[b] + t] - ref) / tol)))
+                assert worst <= 4, f"b={b} t={t} h={h}: {worst} times the bound"  # 4 u of a product, as the prompts' tests
+    for p in (None, [0, 0, 0, 0]):  # nothing is ahead: the linear bias, bit for bit
+        assert np.array_equal(run(p, True), run(p, False))
+    assert not np.array_equal(run(prefix, True), run(prefix, False))
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_prompt_distance_bias_f32_products(ctx, nnhip, f16):
+    """The same from the products that inputs beyond the parts' range take: a query of 1e16 against keys of 0 beside an
+    ordinary one."""
+    rng = np.random.default_rng(310)
+    dk, n, prefix = 64, 200, 150
+    c = Cache(rng, [n], 1, 16, dk, f16)
+    c.k[..., 3] *= 0
+    q = rng.standard_normal((1, dk, n)).astype(np.float32)
+    q[0, 3, ::7] = 1e16
+    out = host(ctx.attention_pages_prefill(c.on_device(nnhip), dev(q.reshape(dk, n)), dev(np.array([0, n], np.int32)), n, 1,
+                                           0.125, slopes=dev(np.array([0.3], np.float32)),
+                                           prefix=dev(np.array([prefix], np.int32)), distance=True)).astype(np.float64)
+    for t in (0, 7, 8, 70, 149, 150, 196, 199):
+        x = q[0, :, t].astype(np.float64)
+        x[3] = 0  # its keys are
+        ref, tol = distance_ref(c, 0, x, t, n, float(np.float32(0.3)), 0.0, 0.125, prefix)
+        assert np.all(np.abs(out[:, t] - ref) <= 4 * tol), t
