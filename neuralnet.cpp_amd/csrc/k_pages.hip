@@ -324,7 +324,7 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
     int ids[2];
     auto load_ids = [&](int base) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) ids[i] = table[(t0 + min(base + 8 * i, max(n - 1, 0))) >> a.shift];
+        for (int i = 0; i < 2; ++i) ids[i] = table[tile_lookup(t0, base + 8 * i, n) >> a.shift];
     };
     load_ids(w * kPgTile);
     const int new_id = has_new ? table[p >> a.shift] : 0;
@@ -343,7 +343,7 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn(PagesArgs a)
             bad |= !in;
             // rows 8 i .. 8 i + 7 of the tile; those behind the chunk's last row are in the same page as its
             // last 8 rows, or read those (their score is -inf)
-            at[i] = page_row(in ? id : 0, g, (t0 + min(base + 8 * i, (n - 1) & ~7)) & slot_mask, a.Hkv, a.shift) * DK;
+            at[i] = page_row(in ? id : 0, g, tile_rows(t0, base + 8 * i, n) & slot_mask, a.Hkv, a.shift) * DK;
         }
         load_ids(base + kPgWaves * kPgTile);
         if constexpr (kDots)

@@ -924,7 +924,7 @@ __device__ __forceinline__ void attend(const PrefillArgs& a, const PrefillItem& 
     int ids[KU];
     bool bad = false;
     auto key_at = [&](int kb, int i) {
-        return is_v ? min(kb * kPK + 4 * vq, last_key & ~3) : min(kb * kPK + (u + 256 * i) / CH, last_key);
+        return is_v ? seen_rows(kb * kPK + 4 * vq, last_key, 4) : seen_rows(kb * kPK + (u + 256 * i) / CH, last_key, 1);
     };
     auto load_ids = [&](int kb) {
         if constexpr (kPaged)

@@ -1,5 +1,6 @@
 // pages_index.hpp — where a position of a paged sequence lies. Plain arithmetic that the kernels share
-// with a CPU test (tests/cpp/pages_index_check.cpp), so that its bounds are checked without a GPU.
+// with CPU tests (tests/cpp/pages_index_check.cpp, pages_tiles_check.cpp), so that its bounds are checked
+// without a GPU.
 #pragma once
 
 #include <cstddef>
@@ -23,7 +24,28 @@ NNHIP_HD size_t page_row(int id, int g, int slot, int Hkv, int shift)
     return (((size_t)id * (size_t)Hkv + (size_t)g) << shift) + (size_t)slot;
 }
 
-// Table entries that positions [t0, last] of a sequence need, from entry t0 >> shift on
+// Position of a chunk (its first position t0, a multiple of 8, n > 0 cached rows) where the decode's tile of
+// rows at, at + 1, ... looks up its page: its own, or the chunk's last one (n == 0: the chunk's first).
+NNHIP_HD int tile_lookup(int t0, int at, int n) { return t0 + (at < n ? at : n > 0 ? n - 1 : 0); }
+
+// Position of the first of 8 rows that such a tile reads, which lie in that page: its own rows, or those that
+// hold the chunk's last one
+NNHIP_HD int tile_rows(int t0, int at, int n)
+{
+    const int last = (n - 1) & ~7;
+    return t0 + (at < last ? at : last);
+}
+
+// Position whose row(s) the prompt's tile reads for position t: its own, or, for t past the last one that is seen,
+// the run of `run` (a power of two, up to 8) positions with that one
+NNHIP_HD int seen_rows(int t, int last, int run)
+{
+    const int end = last & -run;
+    return t < end ? t : end;
+}
+
+// Table entries that positions [t0, last] of a sequence need, from entry t0 >> shift on (the kernels look theirs up
+// one at a time; a count for tests that walk chunks)
 NNHIP_HD int page_entries(int t0, int last, int shift) { return (last >> shift) - (t0 >> shift) + 1; }
 
 // The sequence of column m of a packed call: the first b with cu[b + 1] > m, or -1 if it has none
