@@ -664,7 +664,7 @@ nnhip_status nnhip_argmax_rows(nnhip_ctx* ctx, const float* logits, size_t V, si
  * page_size) of sequence b; entries past a sequence's length may be anything. Sequences may share pages
  * that no call writes. Every id that a call uses is checked on the device: one outside [0, num_pages)
  * is never followed (each entry point says what its sequence gets). dk in {64, 128, 256} (the prompt
- * attention: 64 or 128); num_pages * Hkv * page_size < 2^31. */
+ * attention: 64 or 128); Hkv <= 65535; num_pages * Hkv * page_size < 2^31; table_stride * page_size <= 2^30. */
 typedef struct nnhip_kv_pages
 {
     void* k;
@@ -692,7 +692,8 @@ nnhip_status nnhip_kv_pages_fill(nnhip_ctx* ctx, const nnhip_kv_pages* cache, co
  * part in the attention as the pool's type holds them. Scores of query head h and position j:
  *   s = scale * rot(q_h) . K_j;  softcap > 0: s = softcap * tanh(s / softcap) (0: off);
  *   slopes (DEVICE (H), or NULL): s += slopes[h] * (j - pos[b]);  out = softmax(s) . V over j <= pos[b].
- * Any H / Hkv; a row all of whose scores are -infinity gives zeros.
+ * Any H / Hkv, H and B <= 65535, B * H < 2^22, softcap 0 or in [1e-30, 1e30]; a row all of whose scores are
+ * -infinity gives zeros.
  * pos[b] < 0: an empty slot, out zeros, nothing written; pos[b] >= len_bound: out NaN, nothing written;
  * a page outside the pool among positions [0, pos[b]]: out NaN. len_bound <= table_stride * page_size
  * and (with tables) rope_len. Two sequences of one call whose new tokens fall on one place of the pool
@@ -716,7 +717,8 @@ nnhip_status nnhip_attention_pages_decode(nnhip_ctx* ctx, const nnhip_kv_pages* 
  * products' cases as nnhip_attention_prefill, but for f16 pools, whose weights are held to 2^-22 of themselves
  * down to 2^-29 of the largest in their run of 32 keys and to 2^-51 of that one below (outputs so small that this
  * could show take the f32 products). The sums' order depends on all sequences of the call. dk in {64, 128}, any
- * H / Hkv, H * dk * M < 2^29. Columns of no sequence are not written. NaN: a sequence with more than t_bound
+ * H / Hkv, H <= 65535, B * H < 2^22, H * dk * M < 2^29, with tables min(table_stride * page_size, rope_len) * dk
+ * < 2^30. Columns of no sequence are not written. NaN: a sequence with more than t_bound
  * tokens, columns outside [0, M) or positions at or past table_stride * page_size or rope_len; a query that sees
  * a position whose page is outside the pool (other queries of its sequence may be NaN then, too). The paged form
  * of nnhip_attention_prefill (compute_layer_attention.hpp:1022-1083). */
@@ -771,7 +773,7 @@ typedef struct nnhip_logit_rules
  * of it is NaN, and that step would write it over the row at pos[b].) out (B, V), or NULL: the adjusted logits (may be the
  * logits themselves). pos, or NULL: pos[b] += 1 after a choice; a pos[b] below 0 (an empty slot of
  * nnhip_attention_pages_decode) stays, and nothing is counted for it. ids may be NULL where out is given (then
- * counts and pos must not be changed: count_choice == 0, pos NULL). The greedy rule of the reference
+ * counts and pos must not be changed: count_choice == 0, pos NULL). V < 2^30, B <= 65535. The greedy rule of the reference
  * (compute_layer_base.hpp:1152-1160) behind rules that it does not have. */
 nnhip_status nnhip_logits_adjust_rows(nnhip_ctx* ctx, const float* logits, size_t V, size_t B,
                                       const nnhip_logit_rules* rules, float* out, int32_t* ids, int32_t* pos);

@@ -1800,7 +1800,7 @@ hipError_t launch_pages_prefill(hipStream_t st, const nnhip_kv_pages& kv, const 
     const bool f32 = !(mag >= 0x1p-20f && mag <= 0x1p20f);
     const double cap2 = softcap * 1.4426950408889634;
     PrefillArgs a{q, kv.k, kv.v, cosT, sinT, out, (int)B, (int)t_bound, (int)H, (int)kv.Hkv, (int)R, 0,
-                  (int)limit, (int)std::max<size_t>(1, ceil_div(t_bound, kPQ * (kPWaves / R))), scale, (float)(mag * 1.4426950408889634), f32 ? 1 : 0,
+                  (int)limit, (int)std::max<size_t>(1, ceil_div(std::min(t_bound, limit), kPQ * (kPWaves / R))), scale, (float)(mag * 1.4426950408889634), f32 ? 1 : 0,
                   (int)M, (int)(heads / R), kv.table, cu, pos0, prefix, slopes, (int)kv.table_stride, (int)kv.num_pages,
                   0, (int)limit, (float)cap2, softcap > 0.0f ? (float)(1.0 / cap2) : 0.0f,
                   static_cast<float*>(ws), (int)pages_prefill_spans(limit, num_cus)};

@@ -2113,8 +2113,7 @@ static nnhip_status attention_pages_prefill(nnhip_ctx* ctx, const char* fn, cons
     size_t limit = cache->table_stride * cache->page_size;
     if (rope_cos) limit = std::min(limit, rope_len);
     NNHIP_REQUIRE(!rope_cos || limit * cache->dk < (size_t(1) << 30), fn, "rope tables must be below 2 GiB");
-    NNHIP_REQUIRE(mul_ok(B, H) && mul_ok(B * H, ceil_div(t_bound, 32)) && B * H * ceil_div(t_bound, 32) < (size_t(1) << 22), fn,
-                  "B * H * ceil(t_bound / 32) must be below 2^22");
+    NNHIP_REQUIRE(B < (size_t(1) << 22) && B * H < (size_t(1) << 22), fn, "B * H must be below 2^22");
     void* ws = nullptr;
     st = ensure_stream_ws(ctx, pages_prefill_workspace_bytes(cache->dk, limit, (size_t)ctx->num_cus), fn, &ws);
     if (st != NNHIP_OK) return st;

@@ -81,3 +81,23 @@ def test_prompt_head_ratios(ctx, nnhip, H, Hkv, f16):
 def test_long_prompt_in_one_call(ctx, nnhip, H, Hkv, dk, slopes, f16):
     """One prompt of 12 K tokens behind another's 500 positions, a short one beside it."""
     check_prompt(ctx, nnhip, [12000, 5], [500, 3], H, Hkv, dk, 64, f16, slopes=slopes, seed=52, sample=12)
+
+
+@pytest.mark.parametrize("width", [8, 64])  # 128 positions: a work-group a block of queries; 1024: equal spans
+def test_prompt_constant_bound(ctx, nnhip, width):
+    """A server's constant bound of 32 K tokens with 64 slots and 64 heads, most of a packing's columns behind its last
+    sequence: the outputs of the tight bound, and the other columns as they were."""
+    import torch
+    print(f"constant bound width={width}", flush=True)
+    rng = np.random.default_rng(70)
+    B, H, Hkv, dk, page, M = 64, 64, 8, 64, 16, 1 << 15
+    lens = rng.integers(0, 5, B)
+    lens[[3, 40]] = 128, 77
+    cu = np.concatenate(([0], np.cumsum(lens))).astype(np.int32)
+    k, v = (torch.randn(B * width, Hkv, page, dk, device="cuda") for _ in range(2))
+    cache = nnhip.KVPages(k, v, dev(rng.permutation(B * width).astype(np.int32).reshape(B, width)))
+    q = torch.randn(H * dk, M, device="cuda")
+    n = int(cu[-1])
+    tight = ctx.attention_pages_prefill(cache, q[:, :n].contiguous(), dev(cu), 128, H, 0.125)
+    out = ctx.attention_pages_prefill(cache, q, dev(cu), M, H, 0.125, out=torch.full((H * dk, M), 7.0, device="cuda"))
+    assert torch.equal(out[:, :n], tight) and bool(torch.isfinite(tight).all()) and bool((out[:, n:] == 7.0).all())
