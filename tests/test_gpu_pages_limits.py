@@ -209,3 +209,79 @@ def test_prompt_distance_bias_f32_products(ctx, nnhip, f16):
         x[3] = 0  # its keys are
         ref, tol = distance_ref(c, 0, x, t, n, float(np.float32(0.3)), 0.0, 0.125, prefix)
         assert np.all(np.abs(out[:, t] - ref) <= 4 * tol), t
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("R,dk", [(2, 64), (5, 64), (8, 64), (8, 128)])
+def test_decode_infinite_keys_under_a_cap(ctx, nnhip, R, dk, f16):
+    """Under a cap an infinite score is the cap or its negative, and a key like any other: several of them among the cached
+    keys and the new one, with a distance bias. One against an element that is 0 leaves the head NaN."""
+    rng = np.random.default_rng(120 + R)
+    B, page, n, cap, scale = 4, 16, 300, 3.0, 0.125
+    H = R
+    pos = np.full(B, n, np.int32)
+    c = Cache(rng, pos + 1, 1, page, dk, f16)
+    q = rng.standard_normal((B, H, dk)).astype(np.float32)
+    q[:, :, 9] = 2.0 ** -44 * np.where(np.arange(H) % 3 == 0, 1.0, -1.0)
+    q[3, 0, 7] = 0
+    k, v = (rng.standard_normal((B, 1, dk)).astype(np.float32) for _ in range(2))
+
+    def put(b, t, e, x):
+        c.k[c.table[b, t // page], :, t % page, e] = x
+
+    for b, e in ((0, 5), (1, 9)):
+        for t in (3, 64, 65, 131, 280, 299):
+            put(b, t, e, np.inf if t % 2 else -np.inf)
+    k[0, 0, 5], k[1, 0, 9] = 1e6, -1e6  # f16: past its largest
+    put(3, 250, 7, np.inf)
+    slopes = np.linspace(0.001, 0.02, H).astype(np.float32)
+    out = host(ctx.attention_pages_decode(c.on_device(nnhip), dev(q.reshape(B, -1)), dev(k.reshape(B, -1)),
+                                          dev(v.reshape(B, -1)), H, dev(pos), n + 1, scale, softcap=cap,
+                                          slopes=dev(slopes), tokens=True)).astype(np.float64).reshape(B, H, dk)
+    dist = np.arange(n + 1) - float(n)
+    for b in range(B):
+        with np.errstate(over="ignore"):
+            c.set(b, n, k[b], v[b])
+        K, V = c.rows(b, n + 1)
+        for h in range(H):
+            x = q[b, h].astype(np.float64)
+            s = scores_of(x[None], K[:, 0])[0] * scale
+            if np.isnan(s).any():
+                assert b == 3 and h == 0 and np.all(np.isnan(out[b, h]))
+                continue
+            assert not (b == 3 and h == 0)
+            s = cap * np.tanh(s / cap) + float(slopes[h]) * dist
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            # attend64's bound; an infinite score's value is the cap itself
+            near = np.isfinite(K[:, 0]).all(1)
+            mag = 4 * np.sqrt(dk + 8) * np.max(np.abs(K[near, 0]) @ np.abs(x)) * scale
+            delta = 2.0 ** -24 * (mag + 8 * np.max(np.abs(s)) + 4 * cap + 2 * float(slopes[h]) * n + 8)
+            tol = (2 * delta + 2.0 ** -24 * (4 * np.sqrt(n + 1) + 40)) * (p @ np.abs(V[:, 0])) + 1e-30
+            off = np.abs(out[b, h] - p @ V[:, 0])
+            assert np.all(off <= tol), f"b={b} h={h}: {np.max(off / tol)} times the bound"
+
+
+def test_decode_infinite_keys_before_bad_pages(ctx, nnhip):
+    """An infinite key in an early tile, a page outside the pool in a later one: NaN for that sequence alone."""
+    rng = np.random.default_rng(140)
+    B, H, dk, page, n = 3, 8, 64, 16, 500
+    pos = np.full(B, n, np.int32)
+    c = Cache(rng, pos + 1, 1, page, dk, True)
+    q = rng.standard_normal((B, H, dk)).astype(np.float32)
+    q[:, :, 5] = -0.5
+    q[:, :, 9] = 2.0 ** -44
+    k, v = (dev(rng.standard_normal((B, dk)).astype(np.float32)) for _ in range(2))
+    for b in range(2):
+        for t in (0, 130, 270, 400):
+            c.k[c.table[b, t // page], 0, t % page, 5] = np.inf
+            c.k[c.table[b, t // page], 0, t % page, 9] = -np.inf
+    call = lambda t: host(ctx.attention_pages_decode(nnhip.KVPages(dev(c.k), dev(c.v), dev(t)), dev(q.reshape(B, -1)), k, v, H,
+                                                     dev(pos), n + 1, 0.125, tokens=True))
+    good = call(c.table)
+    assert np.all(np.isfinite(good))
+    for entry in (7, 15, 24, 30):
+        table = c.table.copy()
+        table[1, entry] = c.k.shape[0]
+        out = call(table)
+        assert np.all(np.isnan(out[1])) and np.array_equal(out[[0, 2]], good[[0, 2]])
