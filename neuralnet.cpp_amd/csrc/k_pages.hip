@@ -204,12 +204,11 @@ struct PagesItem
 
 __device__ __forceinline__ int pages_len(const PagesArgs& a, int p) { return p < 0 || p >= a.len_bound ? 0 : p + 1; }
 
-// Item `item` of a call. With lengths spread from 1 to 16 K,
-// chunks of one size for len_bound leave a few long work-groups and thousands of empty ones (37 sequences
-// of 1 .. 16384 over 2 KV heads: 63 us against 26), so every wave sizes the chunks by the lengths
-// themselves: with D = a.even the smallest multiple of 64 that is at least sum(len) / D, which makes at
-// most D + B chunks. Every work-group of the call finds the same ones; the first of a sequence leaves its
-// place for the join.
+// Item `item` of a call. With lengths spread from 1 to 16 K, chunks of one size for len_bound leave a few
+// long work-groups and thousands of empty ones (37 sequences of 1 .. 16384 over 2 KV heads: 63 us against 26
+// when this was measured, 19.4 now), so every wave sizes the chunks by the lengths themselves: with D = a.even
+// the smallest multiple of 64 that is at least sum(len) / D, which makes at most D + B chunks. Every
+// work-group of the call finds the same ones; the first of a sequence leaves its place for the join.
 __device__ __forceinline__ PagesItem find_item(const PagesArgs& a, int item)
 {
     const int lane = threadIdx.x & 63;
