@@ -53,8 +53,9 @@
 // 198 us at 4 x 2048.
 //
 // Over pages (kPaged): packed sequences of unlike lengths, each at its own position, whose rows are found
-// through a page table read a tile ahead; a prefix that all queries see, a tanh cap and a bias on the scores, linear in
-// the position or (kDistance: they differ for keys ahead of the query, inside a prefix) in the distance. Any H / Hkv: a KV head's heads go in groups of 8, 4, 2 or 1.
+// through a page table read a tile ahead; a prefix that all queries see, a tanh cap and a bias on the scores,
+// linear in the position or (kDistance; the two differ for keys ahead of the query, inside a prefix) in the
+// distance. Any H / Hkv: a KV head's heads go in groups of 8, 4, 2 or 1.
 //   * Work-groups take equal spans of all tiles of the call (prompt_cut) and join the blocks of queries
 //     they share; a plain work-group per block of queries left most CUs idle behind a long sequence, or
 //     behind the 14 blocks beyond 256 (4 x 700 .. 1024 tokens at 6144, f16: 1087 -> 754 us).

@@ -214,6 +214,8 @@ class Decoder:
         cfg, ctx, B = self.cfg, self.ctx, self.B
         if self.paged:
             raise _pkg().NNHipError(1, "paged caches take prompts through prefill_packed")
+        if T < 1:
+            raise _pkg().NNHipError(1, "prefill needs a token")
         M = B * T
         pf = self._prefill_buffers(M)
 
@@ -503,9 +505,9 @@ class Decoder:
         advance: the greedy ids are written into ids itself and every pos is advanced by one, so
         that the next call continues the generation (a captured step then replays as is); paged
         caches: a pos below 0 (an empty slot) stays, and nothing is counted for it. rules: a LogitRules for
-        the choice (the logits returned are those before it). Where its mask allows nothing the id returned is -1 (in a tensor of
-        its own: the next input is ids), and ids and pos keep that sequence's token and position: the next
-        call repeats it, the same key and value in the same place."""
+        the choice (the logits returned are those before it). Where its mask allows nothing the id returned
+        is -1 (in a tensor of its own: the next input is ids), and ids and pos keep that sequence's token and
+        position: the next call repeats it, the same key and value in the same place."""
         ctx = self.ctx
         fused = self.fused_ok()
         if fused and self._tok:

@@ -338,3 +338,12 @@ def test_prompt_bound_past_the_tokens(ctx, nnhip):
     outs = [decoder(ctx, nnhip, cfg, base, 2).prefill_packed(ids, cu, t) for t in (3, 5, 6, 4096)]
     for logits, got in outs[1:]:
         assert np.array_equal(host(logits), host(outs[0][0])) and np.array_equal(host(got), host(outs[0][1]))
+
+
+def test_prompts_without_tokens_are_refused(ctx, nnhip):
+    cfg, base = model(ctx, nnhip, 2, 0xE5)
+    none, cu = dev(np.zeros(0, np.int32)), dev(np.zeros(3, np.int32))
+    with pytest.raises(nnhip.NNHipError, match="token"):
+        decoder(ctx, nnhip, cfg, base, 2, paged=False).prefill(none, 0)
+    with pytest.raises(nnhip.NNHipError, match="token"):
+        decoder(ctx, nnhip, cfg, base, 2).prefill_packed(none, cu, 0)
