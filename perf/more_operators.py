@@ -327,8 +327,8 @@ def _run_own(s):
         q, k = ctx.qk_norm_rope(s["q"], s["k"], s["dk"], s["eps"], s["gq"], s["gk"], pos=s["pos"], cos=s["cos"],
                                 sin=s["sin"], q_out=s["q_out"], k_out=s["k_out"], tokens=s["tokens"])
         return {"q": q, "k": k}
-    ctx.pages_assign(s["table"], s["page"], s["free"], s["count"], s["lens"], s["add"], cu=s["cu"], pos0=s["pos0"])
-    ctx.pages_slots(s["table"], s["page"], s["free"].shape[0], s["cu"], s["pos0"], s["M"], pos=s["pos"], slots=s["slots"])
+    ctx.pages_assign(s["table"], s["page"], s["free"], s["count"], s["lens"], s["add"], cu=s["cu"], pos0=s["pos0"],
+                     pos=s["pos"], slots=s["slots"])
     ctx.pages_release(s["table"], s["page"], s["free"], s["count"], s["lens"], s["keep"])
     return _tables_out(s)
 
