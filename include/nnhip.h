@@ -735,9 +735,105 @@ nnhip_status nnhip_attention_pages_prefill_distance(nnhip_ctx* ctx, const nnhip_
                                                     float scale, float softcap, const float* slopes, const int32_t* prefix,
                                                     float* out);
 
-/* Scratch that nnhip_attention_pages_decode (nnhip_logits_adjust_rows) of these sizes uses;
+/* ---- the paged KV cache in 8 bits: int8 codes with an f32 scale for every block of positions of a head. No
+ *      counterpart in the reference (its caches are F32 or F16, compute_layer_gpt.hpp:764-765); about half the
+ *      memory of f16 pages, and half the bytes of each decode step's attention. ---- */
+
+/* One layer's paged cache in 8 bits. k / v: pools of num_pages * Hkv * page_size * dk int8 codes, 16-byte aligned, by
+ * pages as nnhip_kv_pages', but each 16 positions of a head as 16 * dk bytes of their own: keys (dk / 16, 16 positions, 16
+ * dimensions), values (dk, 16 positions). k_scale / v_scale: (num_pages, Hkv, page_size / block) f32. A code q of a
+ * block with scale s stands for fl(q * s). page_size a power of two in [16, 1024], block a power of two in [16, 64], at most page_size;
+ * the rest, and the table, as in nnhip_kv_pages. A new pool may hold anything: a block's scale is set by its first
+ * token, which is the token at the block's first position.
+ * What a write does: s = fl(m * fl(1/127)) with m the largest magnitude (NaN left out) among the call's tokens in the block,
+ * and q = round_half_away(clamp(fl(x / s), -127, 127)), 0 for NaN and where s is 0, as nnhip_quantize_i8. Where the block has older
+ * tokens (positions before the sequence's first one of the call), its scale is kept if it is at least s;
+ * otherwise their codes become those of the values that they stood for under s. An infinity makes a scale infinite, and
+ * its block's codes 0: they stand for NaN. */
+typedef struct nnhip_kv_pages_i8
+{
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    const int32_t* table;
+    size_t num_pages, page_size, block, table_stride, Hkv, dk;
+} nnhip_kv_pages_i8;
+
+/* nnhip_kv_pages_fill into a cache in 8 bits: the same arguments, the same tokens left out. A sequence's tokens are taken
+ * to be new: those at its positions from pos0[b] on and behind are written over, or mean nothing. Two sequences of one
+ * call that write into one block of the pool leave anything there. M <= 2^31 - 192. */
+nnhip_status nnhip_kv_pages_fill_i8(nnhip_ctx* ctx, const nnhip_kv_pages_i8* cache, const float* k, const float* v,
+                                    size_t M, const int32_t* cu, const int32_t* pos0, size_t B, const float* rope_cos,
+                                    const float* rope_sin, size_t rope_len);
+
+/* The values that a cache in 8 bits holds: k / v (Hkv*dk, M) feature-major get, in columns cu[b] .. cu[b+1] - 1, those of
+ * sequence b's positions pos0[b] on (pos0 may be NULL for 0); NaN for positions at or past table_stride * page_size and
+ * pages outside the pool. Columns of no sequence are not written. To move sequences to another cache, or to look at them. */
+nnhip_status nnhip_kv_pages_read_i8(nnhip_ctx* ctx, const nnhip_kv_pages_i8* cache, size_t M, const int32_t* cu,
+                                    const int32_t* pos0, size_t B, float* k, float* v);
+
+/* nnhip_attention_pages_decode over a cache in 8 bits: the same arguments, limits and empty slots; dk in {64, 128, 256}.
+ * The new key and value are written as nnhip_kv_pages_fill_i8 writes one token, and take part as the cache then holds
+ * them. k and v both NULL: nothing is written, the cache holds position pos[b] already (several calls may share pages then).
+ * Products with the codes are exact, of queries with 30 bits under their head's largest element and weights with 30 bits under
+ * the tile's; sums of tiles and softmax are f32. NaN: a head whose rotated query holds an infinity or a NaN, a
+ * sequence with a scale that is not finite among its positions. */
+nnhip_status nnhip_attention_pages_decode_i8(nnhip_ctx* ctx, const nnhip_kv_pages_i8* cache, const float* q, const float* k,
+                                             const float* v, size_t B, size_t H, const int32_t* pos, size_t len_bound,
+                                             const float* rope_cos, const float* rope_sin, size_t rope_len, float scale,
+                                             float softcap, const float* slopes, int tokens, float* out);
+
+/* nnhip_attention_pages_prefill over a cache in 8 bits: the same arguments and limits, dk in {64, 128}; distance != 0:
+ * the bias of nnhip_attention_pages_prefill_distance. The codes go into the products as they are, queries and weights
+ * in two f16 parts: queries to 2^-23 of each element and 2^-40 of the query's largest, weights to 2^-22 of each and 2^-31 of the largest
+ * before; sums and softmax are f32. NaN: a query that holds an infinity or a NaN, or sees a scale that is not finite. */
+nnhip_status nnhip_attention_pages_prefill_i8(nnhip_ctx* ctx, const nnhip_kv_pages_i8* cache, const float* q, size_t M,
+                                              const int32_t* cu, const int32_t* pos0, size_t B, size_t t_bound, size_t H,
+                                              const float* rope_cos, const float* rope_sin, size_t rope_len, float scale,
+                                              float softcap, const float* slopes, const int32_t* prefix, int distance,
+                                              float* out);
+
+/* RMSNorm of every head of queries and keys, and the rotation at each token's position: for each head of each token
+ *   y = (x * rinv) * gamma[f],  rinv = 1 / sqrt(sum_f x^2 * fl(1/dk) + eps);  (y[j], y[j + dk/2]) rotated at pos[m] as
+ * nnhip_attention_decode rotates (rope_cos / rope_sin (rope_len, dk/2), both NULL: no rotation). q (H*dk, M), k (Hkv*dk, M)
+ * feature-major, or with tokens != 0 (M, H*dk), (M, Hkv*dk); q_out, k_out like them (may be q and k themselves, no other overlap).
+ * q or k may be NULL (with its output); gamma_q, gamma_k (dk), NULL: a gain of 1. pos (M) int32, DEVICE, NULL without
+ * tables: a token with pos[m] < 0 is left as its output is, one at or past rope_len gets NaN. dk in {64, 128, 256}; M * (H + Hkv) < 2^31.
+ * The attention that follows takes no tables. No counterpart in the reference, whose attention has no such norms; per head the step of
+ * RMSNorm::forward (compute_layer_mlp.hpp:686-707) and of RotaryEmbedding (compute_position_encoding.hpp:150-166). */
+nnhip_status nnhip_qk_norm_rope(nnhip_ctx* ctx, const float* q, const float* k, size_t M, size_t H, size_t Hkv, size_t dk,
+                                const float* gamma_q, const float* gamma_k, float eps, const int32_t* pos,
+                                const float* rope_cos, const float* rope_sin, size_t rope_len, int tokens, float* q_out,
+                                float* k_out);
+
+/* Pages for new tokens, from a free list on the GPU. table (B, table_stride), lens (B): the sequences' pages and lengths;
+ * add (B): their new tokens; free_pages (num_pages) with free_count (1) entries in use, taken from the end; all DEVICE int32. In the
+ * order of the sequences, b gets the pages that its lens[b] + add[b] positions need beyond those it has, entries
+ * behind them in its row of the table, if the list holds those of every sequence up to b; one that needs no page is served in any case. Not
+ * served: lens[b] < 0 (an empty slot), add[b] <= 0, and what the table has no place for.
+ * cu (B + 1): offsets of the served tokens; pos0 (B): lens[b] of a served sequence, else -1 (nnhip_attention_pages_decode's empty
+ * slot, when each adds one token); lens[b] += add[b] where served. pos / slots (M), each or both NULL: of token m, in the order of
+ * cu, its position and page * page_size + position % page_size; -1 for tokens behind cu[B] (tokens past M are not written). num_pages * page_size < 2^31,
+ * page_size a power of two in [8, 1024], B <= 65535, table_stride * page_size <= 2^30. No counterpart in the reference. */
+nnhip_status nnhip_pages_assign(nnhip_ctx* ctx, int32_t* table, size_t table_stride, size_t page_size, size_t num_pages,
+                                size_t B, int32_t* free_pages, int32_t* free_count, int32_t* lens, const int32_t* add,
+                                int32_t* cu, int32_t* pos0, size_t M, int32_t* pos, int32_t* slots);
+
+/* Positions and slots, as nnhip_pages_assign's, of packed tokens: columns cu[b] .. cu[b+1] - 1 at positions pos0[b] on
+ * (pos0 NULL: 0). -1: a token of no sequence, a position at or past table_stride * page_size; the slot alone: a page outside [0, num_pages). */
+nnhip_status nnhip_pages_slots(nnhip_ctx* ctx, const int32_t* table, size_t table_stride, size_t page_size, size_t num_pages,
+                               const int32_t* cu, const int32_t* pos0, size_t B, size_t M, int32_t* pos, int32_t* slots);
+
+/* Pages back to the free list: sequence b keeps its first keep[b] positions (0: it is over; lens[b] or more: all; DEVICE
+ * int32), lens[b] becomes that, and the pages behind go back, the last sequence's last one first: a release of what
+ * nnhip_pages_assign has just given leaves the list as it was. Empty slots (lens[b] < 0) stay. Pages must be in one row of the table only. */
+nnhip_status nnhip_pages_release(nnhip_ctx* ctx, const int32_t* table, size_t table_stride, size_t page_size, size_t num_pages,
+                                 size_t B, int32_t* free_pages, int32_t* free_count, int32_t* lens, const int32_t* keep);
+
+/* Scratch that nnhip_attention_pages_decode (nnhip_logits_adjust_rows) of these sizes uses, over pages of any type;
  * nnhip_attention_pages_prefill uses 2 * (dk + 2) KiB and 16 bytes for each CU where the table (and the rope tables) hold
- * more than 128 positions. The context keeps one for each stream that it was set to, grown on demand and freed with the context only, so that a
+ * more than 128 positions, nnhip_pages_assign and nnhip_pages_release 16 bytes for each of more than 256 sequences. The context keeps one for each stream that it was set to, grown on demand and freed with the context only, so that a
  * captured call stays valid; a call that would have to grow it during a capture fails with
  * NNHIP_ERR_UNSUPPORTED (call once before, on the capture's stream). Captured calls of one stream share
  * its scratch, wherever they are replayed: their replays must overlap neither each other nor eager calls

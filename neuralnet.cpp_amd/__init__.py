@@ -57,6 +57,11 @@ class _KVPagesDesc(ctypes.Structure):
                 ("table_stride", _sz), ("Hkv", _sz), ("dk", _sz), ("f16", _st)]
 
 
+class _KVPagesI8Desc(ctypes.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("table", _vp), ("num_pages", _sz),
+                ("page_size", _sz), ("block", _sz), ("table_stride", _sz), ("Hkv", _sz), ("dk", _sz)]
+
+
 class _LogitRulesDesc(ctypes.Structure):
     _fields_ = [("counts", _vp), ("repeat", _vp), ("presence", _vp), ("frequency", _vp), ("bias", _vp),
                 ("bias_stride", _sz), ("allowed", _vp), ("allowed_stride", _sz), ("count_choice", _st)]
@@ -170,6 +175,16 @@ SIGNATURES = {
                                             _vp, _vp]),
     "nnhip_attention_pages_prefill_distance": (_st, [_vp, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _vp, _vp, _sz, _f, _f,
                                                      _vp, _vp, _vp]),
+    "nnhip_kv_pages_fill_i8": (_st, [_vp, _vp, _vp, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _sz]),
+    "nnhip_kv_pages_read_i8": (_st, [_vp, _vp, _sz, _vp, _vp, _sz, _vp, _vp]),
+    "nnhip_attention_pages_decode_i8": (_st, [_vp, _vp, _vp, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _vp, _sz, _f, _f, _vp,
+                                              _st, _vp]),
+    "nnhip_attention_pages_prefill_i8": (_st, [_vp, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _vp, _vp, _sz, _f, _f, _vp,
+                                               _vp, _st, _vp]),
+    "nnhip_qk_norm_rope": (_st, [_vp, _vp, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _f, _vp, _vp, _vp, _sz, _st, _vp, _vp]),
+    "nnhip_pages_assign": (_st, [_vp, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp]),
+    "nnhip_pages_slots": (_st, [_vp, _vp, _sz, _sz, _sz, _vp, _vp, _sz, _sz, _vp, _vp]),
+    "nnhip_pages_release": (_st, [_vp, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _vp]),
     "nnhip_attention_pages_workspace_bytes": (_sz, [_vp, _sz, _sz, _sz, _sz, _sz]),
     "nnhip_logits_workspace_bytes": (_sz, [_vp, _sz, _sz]),
     "nnhip_logits_adjust_rows": (_st, [_vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp]),
@@ -295,6 +310,43 @@ class KVPages:
         self.desc = _KVPagesDesc(k.data_ptr(), v.data_ptr(), table.data_ptr(), self.num_pages, self.page_size,
                                  self.max_pages, self.Hkv, self.dk, int(k.dtype == torch.float16))
         self.ref = ctypes.addressof(self.desc)
+
+
+class KVPagesI8:
+    """One layer's paged KV cache in 8 bits (nnhip_kv_pages_i8): codes k (num_pages, Hkv, page_size/16, dk/16, 16, 16) and v
+    (num_pages, Hkv, page_size/16, dk, 16) int8, keys by (16 positions, 16 dimensions) and values by (dimension, 16 positions);
+    scales k_scale, v_scale (num_pages, Hkv, page_size/block) float32, one for every `block` positions of a head; and
+    the page table as KVPages'. It is taken wherever KVPages is. empty() makes the tensors of a new cache."""
+
+    def __init__(self, k, v, k_scale, v_scale, table):
+        import torch
+        if k.dim() != 6 or tuple(k.shape[4:]) != (16, 16) or k_scale.dim() != 3 or table.dim() != 2:
+            raise NNHipError(1, "codes must be (num_pages, Hkv, page_size/16, dk/16, 16, 16) and (num_pages, Hkv, "
+                                "page_size/16, dk, 16), scales (num_pages, Hkv, page_size/block), the table (B, pages)")
+        pages, Hkv, groups, chunks = k.shape[:4]
+        i8, f32 = (torch.int8,), (torch.float32,)
+        self.device = _device_args([("k", k, i8, None), ("v", v, i8, (pages, Hkv, groups, 16 * chunks, 16)),
+                                    ("k_scale", k_scale, f32, (pages, Hkv, k_scale.shape[2])),
+                                    ("v_scale", v_scale, f32, tuple(k_scale.shape)), ("table", table, (torch.int32,), None)])
+        self.k, self.v, self.k_scale, self.v_scale, self.table = k, v, k_scale, v_scale, table
+        self.num_pages, self.Hkv, self.page_size, self.dk = pages, Hkv, 16 * groups, 16 * chunks
+        if k_scale.shape[2] < 1 or self.page_size % k_scale.shape[2]:
+            raise NNHipError(1, f"{k_scale.shape[2]} scales do not divide a page of {self.page_size} positions")
+        self.block = self.page_size // k_scale.shape[2]
+        self.rows, self.max_pages = table.shape
+        self.desc = _KVPagesI8Desc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), table.data_ptr(),
+                                   pages, self.page_size, self.block, self.max_pages, Hkv, self.dk)
+        self.ref = ctypes.addressof(self.desc)
+
+    @classmethod
+    def empty(cls, num_pages: int, Hkv: int, page_size: int, dk: int, block: int, table):
+        """A new cache on the table's device."""
+        import torch
+        if page_size < 16 or page_size % 16 or dk % 16 or block < 1 or page_size % block:
+            raise NNHipError(1, "page_size and dk must be multiples of 16, block a divisor of page_size")
+        new = lambda dt, *s: torch.zeros((num_pages, Hkv) + s, dtype=dt, device=table.device)  # noqa: E731
+        scales = [new(torch.float32, page_size // block) for _ in range(2)]
+        return cls(new(torch.int8, page_size // 16, dk // 16, 16, 16), new(torch.int8, page_size // 16, dk, 16), *scales, table)
 
 
 class LogitRules:
@@ -953,19 +1005,34 @@ class Context:
 
     def kv_pages_fill(self, cache, k, v, cu, pos0=None, cos=None, sin=None) -> None:
         """The keys and values k / v (Hkv*dk, M) of packed prompts (sequence b: columns cu[b] .. cu[b+1] - 1,
-        positions pos0[b] on) rotated into the pages of cache, a KVPages."""
+        positions pos0[b] on) rotated into the pages of cache, a KVPages or a KVPagesI8 (which holds them quantized)."""
         B, cu_p, pos0_p = self._packed(cache, cu, pos0)
         f32, M = self._torch.float32, k.shape[-1]
         cs, sn, rows = self._rope(cos, sin, cache.dk)
         shape = (cache.Hkv * cache.dk, M)
         self._bind_stream()
-        _check(lib().nnhip_kv_pages_fill(self.h, cache.ref, self._arg(k, f32, shape, "k"), self._arg(v, f32, shape, "v"),
-                                         M, cu_p, pos0_p, B, cs, sn, rows), "nnhip_kv_pages_fill")
+        fn = "nnhip_kv_pages_fill_i8" if type(cache) is KVPagesI8 else "nnhip_kv_pages_fill"
+        _check(getattr(lib(), fn)(self.h, cache.ref, self._arg(k, f32, shape, "k"), self._arg(v, f32, shape, "v"),
+                                  M, cu_p, pos0_p, B, cs, sn, rows), fn)
+
+    def kv_pages_read(self, cache, cu, M: int, pos0=None, k=None, v=None):
+        """The values that cache, a KVPagesI8, holds: k, v (Hkv*dk, M) get in columns cu[b] .. cu[b+1] - 1 those of sequence
+        b's positions pos0[b] on. Returns k, v."""
+        if type(cache) is not KVPagesI8:
+            raise NNHipError(1, "kv_pages_read takes a KVPagesI8 (the pools of a KVPages are its values)")
+        B, cu_p, pos0_p = self._packed(cache, cu, pos0)
+        f32, shape = self._torch.float32, (cache.Hkv * cache.dk, M)
+        k = self._empty(shape, f32) if k is None else k
+        v = self._empty(shape, f32) if v is None else v
+        self._bind_stream()
+        _check(lib().nnhip_kv_pages_read_i8(self.h, cache.ref, M, cu_p, pos0_p, B, self._arg(k, f32, shape, "k"),
+                                            self._arg(v, f32, shape, "v")), "nnhip_kv_pages_read_i8")
+        return k, v
 
     def attention_pages_decode(self, cache, q, k, v, H: int, pos, len_bound: int, scale: float, cos=None, sin=None,
                                softcap: float = 0.0, slopes=None, out=None, tokens: bool = False):
-        """Attention of one new token per sequence over the pages of cache (a KVPages, whose table has B rows),
-        which also get its key and value: q (H*dk, B), k / v (Hkv*dk, B), or token-major (B, ...) with tokens;
+        """Attention of one new token per sequence over the pages of cache (a KVPages or KVPagesI8, whose table has B rows),
+        which also get its key and value (k and v None, over a KVPagesI8: it holds position pos already): q (H*dk, B), k / v (Hkv*dk, B), or token-major (B, ...) with tokens;
         pos (B) int32 device, below 0 for an empty slot. softcap > 0 caps the scores, slopes (H) bias them by
         distance. Returns out like q."""
         if cache.device != self._device:
@@ -978,11 +1045,11 @@ class Context:
             out = self._empty(qs, f32)
         cs, sn, rows = self._rope(cos, sin, dk)
         self._bind_stream()
-        _check(lib().nnhip_attention_pages_decode(
+        fn = "nnhip_attention_pages_decode_i8" if type(cache) is KVPagesI8 else "nnhip_attention_pages_decode"
+        _check(getattr(lib(), fn)(
             self.h, cache.ref, self._arg(q, f32, qs, "q"), self._arg(k, f32, ks, "k"), self._arg(v, f32, ks, "v"), B, H,
             self._arg(pos, self._torch.int32, (B,), "pos"), len_bound, cs, sn, rows, scale, softcap,
-            self._arg(slopes, f32, (H,), "slopes"), int(tokens), self._arg(out, f32, qs, "out")),
-            "nnhip_attention_pages_decode")
+            self._arg(slopes, f32, (H,), "slopes"), int(tokens), self._arg(out, f32, qs, "out")), fn)
         return out
 
     def attention_pages_prefill(self, cache, q, cu, t_bound: int, H: int, scale: float, pos0=None, cos=None, sin=None,
@@ -999,12 +1066,98 @@ class Context:
             out = self._empty(shape, f32)
         cs, sn, rows = self._rope(cos, sin, cache.dk)
         self._bind_stream()
-        fn = "nnhip_attention_pages_prefill_distance" if distance else "nnhip_attention_pages_prefill"
+        more = ()
+        if type(cache) is KVPagesI8:
+            fn, more = "nnhip_attention_pages_prefill_i8", (int(distance),)
+        else:
+            fn = "nnhip_attention_pages_prefill_distance" if distance else "nnhip_attention_pages_prefill"
         _check(getattr(lib(), fn)(
             self.h, cache.ref, self._arg(q, f32, shape, "q"), M, cu_p, pos0_p, B, t_bound, H, cs, sn, rows, scale,
             softcap, self._arg(slopes, f32, (H,), "slopes"), self._arg(prefix, self._torch.int32, (B,), "prefix"),
-            self._arg(out, f32, shape, "out")), fn)
+            *more, self._arg(out, f32, shape, "out")), fn)
         return out
+
+    def qk_norm_rope(self, q, k, dk: int, eps: float, gamma_q=None, gamma_k=None, pos=None, cos=None, sin=None,
+                     q_out=None, k_out=None, tokens: bool = False):
+        """RMSNorm of every head (dk elements, gains gamma_q, gamma_k (dk) or None) of q (H*dk, M) and k (Hkv*dk, M), or
+        token-major with tokens, and their rotation at pos (M) int32 device (a token below 0 stays). q or k may be
+        None; q_out and k_out, made when not given, may be q and k. Returns them."""
+        torch = self._torch
+        f32 = torch.float32
+        if q is None and k is None:
+            raise NNHipError(1, "q or k must be given")
+        M = (k if q is None else q).shape[0 if tokens else 1]
+
+        def one(x, out, name):
+            if x is None:
+                if out is not None:
+                    raise NNHipError(1, f"{name}_out without {name}")
+                return 0, None, None, None
+            rows = x.shape[1 if tokens else 0]
+            if rows % dk:
+                raise NNHipError(1, f"{name} has {rows} features, heads of {dk}")
+            shape = (M, rows) if tokens else (rows, M)
+            if out is None:
+                out = self._empty(shape, f32)
+            return rows // dk, self._arg(x, f32, shape, name), self._arg(out, f32, shape, name + "_out"), out
+
+        H, q_p, qo_p, q_out = one(q, q_out, "q")
+        Hkv, k_p, ko_p, k_out = one(k, k_out, "k")
+        cs, sn, rows = self._rope(cos, sin, dk)
+        self._bind_stream()
+        _check(lib().nnhip_qk_norm_rope(
+            self.h, q_p, k_p, M, H, Hkv, dk, self._arg(gamma_q, f32, (dk,), "gamma_q"),
+            self._arg(gamma_k, f32, (dk,), "gamma_k"), eps, self._arg(pos, torch.int32, (M,), "pos"), cs, sn, rows,
+            int(tokens), qo_p, ko_p), "nnhip_qk_norm_rope")
+        return q_out, k_out
+
+    def _places(self, pos, slots):
+        """The capacity M of per-token outputs and their addresses."""
+        i32 = self._torch.int32
+        M = 0 if pos is None and slots is None else (slots if pos is None else pos).shape[0]
+        return M, self._arg(pos, i32, (M,), "pos"), self._arg(slots, i32, (M,), "slots")
+
+    def pages_assign(self, table, page_size: int, free_pages, free_count, lens, add, cu=None, pos0=None, pos=None, slots=None):
+        """Pages for add[b] new tokens of each sequence from the list free_pages (num_pages) with free_count (1) entries, into
+        its row of table (B, pages), behind the pages of its lens[b] positions; lens moves on (all int32 device tensors). cu
+        (B + 1): offsets of the tokens that got their places; pos0 (B): the first one's position, -1 for none; pos, slots
+        (M), when given: every token's position and slot, -1 behind the last. Returns cu, pos0."""
+        i32, (B, width) = self._torch.int32, table.shape
+        cu = self._empty((B + 1,), i32) if cu is None else cu
+        pos0 = self._empty((B,), i32) if pos0 is None else pos0
+        num_pages = free_pages.shape[0]
+        M, pos_p, slots_p = self._places(pos, slots)
+        self._bind_stream()
+        _check(lib().nnhip_pages_assign(
+            self.h, self._arg(table, i32, (B, width), "table"), width, page_size, num_pages, B,
+            self._arg(free_pages, i32, (num_pages,), "free_pages"), self._arg(free_count, i32, (1,), "free_count"),
+            self._arg(lens, i32, (B,), "lens"), self._arg(add, i32, (B,), "add"), self._arg(cu, i32, (B + 1,), "cu"),
+            self._arg(pos0, i32, (B,), "pos0"), M, pos_p, slots_p), "nnhip_pages_assign")
+        return cu, pos0
+
+    def pages_slots(self, table, page_size: int, num_pages: int, cu, pos0=None, pos=None, slots=None):
+        """Positions pos (M) and slots (M) of packed tokens (cu (B + 1), pos0 (B) or None), either of which may be None."""
+        i32, B = self._torch.int32, cu.shape[0] - 1
+        if B > table.shape[0]:
+            raise NNHipError(1, f"{B} sequences, the page table has {table.shape[0]} rows")
+        M, pos_p, slots_p = self._places(pos, slots)
+        self._bind_stream()
+        _check(lib().nnhip_pages_slots(
+            self.h, self._arg(table, i32, tuple(table.shape), "table"), table.shape[1], page_size, num_pages,
+            self._arg(cu, i32, (B + 1,), "cu"), self._arg(pos0, i32, (B,), "pos0"), B, M, pos_p, slots_p),
+            "nnhip_pages_slots")
+        return pos, slots
+
+    def pages_release(self, table, page_size: int, free_pages, free_count, lens, keep) -> None:
+        """Sequence b keeps its first keep[b] positions (0: none): lens[b] becomes that, and the pages behind go back to
+        the list, so that a release of what pages_assign has just given leaves the list as it was."""
+        i32, (B, width) = self._torch.int32, table.shape
+        num_pages = free_pages.shape[0]
+        self._bind_stream()
+        _check(lib().nnhip_pages_release(
+            self.h, self._arg(table, i32, (B, width), "table"), width, page_size, num_pages, B,
+            self._arg(free_pages, i32, (num_pages,), "free_pages"), self._arg(free_count, i32, (1,), "free_count"),
+            self._arg(lens, i32, (B,), "lens"), self._arg(keep, i32, (B,), "keep")), "nnhip_pages_release")
 
     def attention_pages_workspace_bytes(self, B: int, H: int, Hkv: int, dk: int, len_bound: int) -> int:
         return int(lib().nnhip_attention_pages_workspace_bytes(self.h, B, H, Hkv, dk, len_bound))

@@ -411,6 +411,22 @@ __device__ __forceinline__ float tanh_any(float x)
     return a > 1.0f ? far : tanh_below1(x);
 }
 
+// The wave's largest value, by moves between registers (through LDS, 43 instructions and six round
+// trips a tile of f32 keys: 4 x 2048 tokens 360 us, 347 so)
+__device__ __forceinline__ uint32_t wave_max(uint32_t v)
+{
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));   // lane ^ 1
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));   // lane ^ 2
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));  // 7 - lane of 8
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true));  // 15 - lane of 16
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    const uint32_t r0 = r[0], r1 = r[1];
+    v = max(r0, r1);
+    const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    const uint32_t h0 = h[0], h1 = h[1];
+    return max(h0, h1);
+}
+
 // ---- paged KV cache (k_pages.hip; the prompt attention k_prefill.hip), logits (k_logits.hip)
 size_t pages_workspace_bytes(size_t B, size_t H, size_t Hkv, size_t dk, size_t len_bound, size_t num_cus);
 hipError_t launch_pages_attn(hipStream_t st, const nnhip_kv_pages& kv, const float* q, const float* k, const float* v,
@@ -426,6 +442,32 @@ hipError_t launch_pages_prefill(hipStream_t st, const nnhip_kv_pages& kv, const 
                                 const int32_t* prefix, bool distance, float* out, void* ws, size_t num_cus);
 size_t pages_prefill_spans(size_t limit, size_t num_cus);
 size_t pages_prefill_workspace_bytes(size_t dk, size_t limit, size_t num_cus);
+// the same over pools in 8 bits (k_pages_i8.hip, k_prefill_i8.hip)
+hipError_t launch_pages_attn_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, const float* q, const float* k, const float* v,
+                                size_t B, size_t H, const int32_t* pos, size_t len_bound, const float* cosT,
+                                const float* sinT, float scale, float softcap, const float* slopes, bool tokens,
+                                float* part, float* out, size_t num_cus);
+hipError_t launch_pages_fill_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, const float* k, const float* v, size_t M,
+                                const int32_t* cu, const int32_t* pos0, size_t B, const float* cosT, const float* sinT,
+                                size_t limit);
+hipError_t launch_pages_read_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, size_t M, const int32_t* cu, const int32_t* pos0,
+                                size_t B, float* k, float* v);
+hipError_t launch_pages_prefill_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, const float* q, size_t M, const int32_t* cu,
+                                   const int32_t* pos0, size_t B, size_t t_bound, size_t H, const float* cosT,
+                                   const float* sinT, size_t limit, float scale, float softcap, const float* slopes,
+                                   const int32_t* prefix, bool distance, float* out, void* ws, size_t num_cus);
+// norms of queries and keys with the rotation (k_qk.hip); page tables (k_tables.hip)
+hipError_t launch_qk_norm_rope(hipStream_t st, const float* q, const float* k, size_t M, size_t H, size_t Hkv, size_t dk,
+                               const float* gq, const float* gk, float eps, const int32_t* pos, const float* cosT,
+                               const float* sinT, size_t rope_len, bool tokens, float* q_out, float* k_out, size_t num_cus);
+size_t tables_workspace_bytes(size_t B);
+hipError_t launch_pages_assign(hipStream_t st, int32_t* table, size_t table_stride, size_t page_size, size_t num_pages, size_t B,
+                               int32_t* free_pages, int32_t* free_count, int32_t* lens, const int32_t* add, int32_t* cu,
+                               int32_t* pos0, size_t M, int32_t* pos, int32_t* slots, void* ws);
+hipError_t launch_pages_slots(hipStream_t st, const int32_t* table, size_t table_stride, size_t page_size, size_t num_pages,
+                              const int32_t* cu, const int32_t* pos0, size_t B, size_t M, int32_t* pos, int32_t* slots);
+hipError_t launch_pages_release(hipStream_t st, const int32_t* table, size_t table_stride, size_t page_size, size_t num_pages,
+                                size_t B, int32_t* free_pages, int32_t* free_count, int32_t* lens, const int32_t* keep, void* ws);
 size_t logits_slices(size_t V, size_t B, size_t num_cus);
 size_t logits_workspace_bytes(size_t V, size_t B, size_t num_cus);
 hipError_t launch_logits_adjust(hipStream_t st, const float* logits, size_t V, size_t B, const nnhip_logit_rules& rules,

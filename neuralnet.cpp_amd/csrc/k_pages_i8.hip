@@ -1,0 +1,833 @@
+// k_pages_i8.hip — the paged KV cache in 8 bits: int8 codes and one f32 scale for every `block` positions of a head.
+// Its fill from packed prompts, the values read back, and the attention of one new token per sequence with the
+// append; the attention of packed prompts is k_prefill_i8.hip's.
+//
+// Layouts (device), as the pools of k_pages.hip by pages (num_pages, Hkv, page_size, dk), but for each 16 positions:
+//   keys    (dk / 16, 16 positions, 16 dimensions) bytes: a wave's 16-byte loads of 16 positions are one run, and
+//           each is an operand of the int8 MFMA as it stands (16 positions x 64 dimensions)
+//   values  (dk, 16 positions) bytes: 16 positions of a dimension are an operand of the product with the weights
+//   scales  (num_pages, Hkv, page_size / block) f32, keys and values apart
+//
+// A block's scale is s = fl(max|x| fl(1/127)) over its tokens and the head's dk dimensions, a code quantize_one(x, s)
+// (token_quant.hpp): the engine's activations are held the same way. A token that joins a block whose scale is smaller
+// raises it, and the older codes q become quantize_one(fl(q s_old), s): each time at most half a step of the new
+// scale is added to what they are off.
+#include "pages_split.hpp"
+#include "token_quant.hpp"
+
+#include <cmath>
+
+namespace nnhip
+{
+namespace
+{
+
+// The pools of a cache and their scales
+struct PoolsI8
+{
+    int8_t* k;
+    int8_t* v;
+    float* ks;
+    float* vs;
+    int bshift;  // log2(block)
+};
+
+typedef int32_t v4i __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v4fu __attribute__((ext_vector_type(4), aligned(4)));
+
+// The old codes of a block again under a larger scale: positions 0 .. n - 1 of the block that begins at row `row`,
+// piece (16 bytes) `at` of every `step`. Of values, only the bytes of those positions are written.
+__device__ __forceinline__ void requantize(int8_t* pool, size_t row, int n, int dk, bool keys, float s_old, float s_new,
+                                           int at, int step)
+{
+    u32x4* const pieces = reinterpret_cast<u32x4*>(pool + (row >> 4) * (size_t)(16 * dk));
+    const int groups = (n + 15) >> 4;
+    for (int i = at; i < groups * dk; i += step)
+    {
+        const int first = i / dk * 16;  // position of the piece's group
+        const int live = keys ? (first + (i & 15) < n ? 16 : 0) : min(16, n - first);
+        if (live == 0) continue;
+        u32x4 x = pieces[i];
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+        {
+            uint32_t y = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+            {
+                const int c = (int8_t)(x[w] >> (8 * e));
+                y |= (uint32_t)(uint8_t)quantize_one(__fmul_rn((float)c, s_old), s_new) << (8 * e);
+            }
+            x[w] = y;
+        }
+        if (live == 16) pieces[i] = x;
+        else
+        {
+            int8_t* const b = reinterpret_cast<int8_t*>(pieces + i);
+            for (int e = 0; e < live; ++e)
+            {
+                const uint32_t w = e < 8 ? (e < 4 ? x[0] : x[1]) : (e < 12 ? x[2] : x[3]);
+                b[e] = (int8_t)(w >> (8 * (e & 3)));
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ fill from packed prompts
+
+struct FillI8Args
+{
+    const float* k;
+    const float* v;
+    const int32_t* cu;
+    const int32_t* pos0;
+    const float* cosT;
+    const float* sinT;
+    PoolsI8 pools;
+    const int32_t* table;
+    int M, B, Hkv, shift, table_stride, num_pages, limit;  // limit: positions from here on are not written
+};
+
+// Work-group = (64 columns, KV head, keys or values) and the blocks whose first token of this call lies in them, the
+// last of which may end up to 63 columns further: each block's largest value is known to one work-group, and every
+// element is read once. Lane = column, wave = a quarter of the dimension pairs (j, j + dk / 2); the values stay in
+// registers between the search for the blocks' maxima and their codes. Keys are stored as 16-byte pieces (lanes side
+// by side), values through LDS as bytes, 16 positions of a dimension at a time. Bound by HBM.
+// Tokens of no sequence, positions outside the table or the rope tables and pages outside the pool are not written.
+template <int DK>
+__global__ __launch_bounds__(256) void k_pages_fill_i8(FillI8Args a)
+{
+    constexpr int HALF = DK / 2, NP = DK / 8;  // pairs of a thread
+    constexpr int kCols = 2 * kPfTok, kPitch = kCols + 4;
+    __shared__ uint32_t top_s[kPfTok];   // by the block's first column: its largest magnitude (bits)
+    __shared__ int row_s[kCols];         // row of a column's token, -1 if it is not this work-group's
+    __shared__ uint8_t head_s[kCols];    // columns that begin a group of 16 positions, in order
+    __shared__ __align__(16) uint8_t code_s[DK * kPitch];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = blockIdx.y;
+    const bool keys = blockIdx.z == 0;
+    const int m0 = blockIdx.x * kPfTok, block = 1 << a.pools.bshift;
+    if (tid < kPfTok) top_s[tid] = 0u;
+
+    // the lane's column and the one 64 further, which is part of this work-group where the last block goes on there
+    int pos[2], row[2] = {-1, -1}, first[2] = {-1, -1}, older[2] = {0, 0};
+    const int b = wave_sequence(a.cu, a.B, a.M, m0, lane);
+    pos[0] = b < 0 ? -1 : packed_position(a.cu, a.pos0, b, m0 + lane, a.limit);
+    if (pos[0] >= 0)
+    {
+        const int cu0 = a.cu[b], head = block_column(m0 + lane, cu0, pos[0], block);
+        if (head < m0) pos[0] = -1;
+        else
+        {
+            first[0] = head - m0;
+            older[0] = (pos[0] & (block - 1)) - (m0 + lane - head);  // positions of the block before the call's
+        }
+    }
+    const int b_last = __builtin_amdgcn_readlane(b, 63), pos_last = __builtin_amdgcn_readlane(pos[0], 63);
+    int more = 0;
+    if (b_last >= 0 && pos_last >= 0)
+    {
+        const int left = block - 1 - (pos_last & (block - 1));  // of the block, behind column 63
+        more = min(min(left, a.limit - 1 - pos_last), min(a.cu[b_last + 1], a.M) - (m0 + kPfTok));
+    }
+    pos[1] = lane < more ? pos_last + 1 + lane : -1;
+    first[1] = __builtin_amdgcn_readlane(first[0], 63);
+    older[1] = __builtin_amdgcn_readlane(older[0], 63);
+    const bool any[2] = {true, more > 0};
+
+    const float* const src = (keys ? a.k : a.v) + (size_t)(g * DK + w * NP) * (size_t)a.M;
+    float x[2][2][NP];
+    auto load = [&](int e) {
+        const int m = min(m0 + kPfTok * e + lane, a.M - 1);
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int i = 0; i < NP; ++i) x[e][q][i] = src[(size_t)(HALF * q + i) * (size_t)a.M + (size_t)m];
+    };
+    load(0);
+    if (any[1]) load(1);
+    float s_old[2] = {0.0f, 0.0f};
+    float* const scales = keys ? a.pools.ks : a.pools.vs;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (pos[e] >= 0)
+        {
+            const int id = a.table[(size_t)(e ? b_last : b) * a.table_stride + (pos[e] >> a.shift)];
+            if (page_ok(id, a.num_pages)) row[e] = (int)page_row(id, g, pos[e] & ((1 << a.shift) - 1), a.Hkv, a.shift);
+            if (row[e] >= 0 && older[e] > 0) s_old[e] = scales[row[e] >> a.pools.bshift];
+        }
+    __syncthreads();  // top_s is clear
+    float top[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+    {
+        if (!any[e]) break;
+        if (keys && a.cosT)
+        {
+            const size_t at = (size_t)max(pos[e], 0) * HALF + (size_t)(w * NP);
+#pragma unroll
+            for (int i = 0; i < NP; i += 4)
+            {
+                const v4fu c = *reinterpret_cast<const v4fu*>(a.cosT + at + i), s = *reinterpret_cast<const v4fu*>(a.sinT + at + i);
+#pragma unroll
+                for (int n = 0; n < 4; ++n) pg_rope(x[e][0][i + n], x[e][1][i + n], c[n], s[n], x[e][0][i + n], x[e][1][i + n]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NP; ++i) top[e] = fmaxf(top[e], fmaxf(fabsf(x[e][0][i]), fabsf(x[e][1][i])));
+        if (row[e] >= 0) atomicMax(&top_s[first[e]], __builtin_bit_cast(uint32_t, top[e]));
+        if (w == 0) row_s[kPfTok * e + lane] = row[e];
+    }
+    if (!any[1] && w == 0) row_s[kPfTok + lane] = -1;
+    __syncthreads();
+    float s[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (row[e] >= 0)
+        {
+            s[e] = __fmul_rn(__builtin_bit_cast(float, top_s[first[e]]), 1.0f / 127.0f);
+            if (older[e] > 0) s[e] = fmaxf(s[e], s_old[e]);
+            if (w == 0 && kPfTok * e + lane == first[e]) scales[row[e] >> a.pools.bshift] = s[e];
+        }
+    int8_t* const pool = keys ? a.pools.k : a.pools.v;
+
+    // ---- older codes of blocks whose scale has grown (each has its first token of this call in the first 64 columns)
+    for (unsigned long long grown = __builtin_amdgcn_ballot_w64(row[0] >= 0 && first[0] == lane && older[0] > 0 && s[0] > s_old[0]);
+         grown != 0; grown &= grown - 1)
+    {
+        const int l = __builtin_ctzll(grown), n = __builtin_amdgcn_readlane(older[0], l);
+        const float before = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s_old[0]), l));
+        const float after = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s[0]), l));
+        requantize(pool, (size_t)(__builtin_amdgcn_readlane(row[0], l) - n), n, DK, keys, before, after, tid, 256);
+    }
+
+    // ---- codes: 4 of a quarter's dimensions in a word
+    uint32_t code[2][2][NP / 4];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+    {
+        if (!any[e]) break;
+        const float r = quant_rcp(s[e]);
+        bool amb = false;
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int i = 0; i < NP; i += 4)
+            {
+                uint32_t y = 0;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) y |= (uint32_t)(uint8_t)quantize_code(x[e][q][i + n], r, amb) << (8 * n);
+                code[e][q][i / 4] = y;
+            }
+        if (amb && row[e] >= 0)
+        {
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int i = 0; i < NP; i += 4)
+                {
+                    uint32_t y = 0;
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) y |= (uint32_t)(uint8_t)quantize_one(x[e][q][i + n], s[e]) << (8 * n);
+                    code[e][q][i / 4] = y;
+                }
+        }
+    }
+    if (keys)
+    {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (any[e] && row[e] >= 0)
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int i = 0; i < NP; i += NP < 16 ? NP : 16)
+                    {
+                        int8_t* const to = pool + key_byte((size_t)row[e], HALF * q + w * NP + i, DK);
+                        if constexpr (NP < 16)
+                            *reinterpret_cast<uint2*>(to) = make_uint2(code[e][q][0], code[e][q][1]);
+                        else
+                            *reinterpret_cast<u32x4*>(to) =
+                                u32x4{code[e][q][i / 4], code[e][q][i / 4 + 1], code[e][q][i / 4 + 2], code[e][q][i / 4 + 3]};
+                    }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (any[e])
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int i = 0; i < NP; ++i)
+                    code_s[(HALF * q + w * NP + i) * kPitch + kPfTok * e + lane] = (uint8_t)(code[e][q][i / 4] >> (8 * (i & 3)));
+    // the columns that begin a group of 16 positions, listed by every wave alike
+    int heads = 0;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+    {
+        const int c = kPfTok * e + lane, before = c > 0 ? row_s[c - 1] : -1;
+        const bool head = row[e] >= 0 && !(before >= 0 && before == row[e] - 1 && (row[e] & 15) != 0);
+        const unsigned long long set = __builtin_amdgcn_ballot_w64(head);
+        if (w == 0 && head) head_s[heads + __builtin_popcountll(set & ((1ull << lane) - 1))] = (uint8_t)c;
+        heads += __builtin_popcountll(set);
+    }
+    __syncthreads();
+    for (int i = tid; i < heads * DK; i += 256)
+    {
+        const int c = head_s[i / DK], d = i % DK, at = row_s[c];
+        const uint8_t* const from = code_s + d * kPitch + c;
+        int8_t* const to = pool + value_byte((size_t)at, d, DK);
+        int n = 1;
+        while (n < 16 - (at & 15) && c + n < kCols && row_s[c + n] == at + n) ++n;
+        if (n == 16)
+        {
+            u32x4 y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                y[e] = from[4 * e] | (uint32_t)from[4 * e + 1] << 8 | (uint32_t)from[4 * e + 2] << 16 | (uint32_t)from[4 * e + 3] << 24;
+            *reinterpret_cast<u32x4*>(to) = y;
+        }
+        else
+            for (int e = 0; e < n; ++e) to[e] = (int8_t)from[e];
+    }
+}
+
+// ------------------------------------------------------------------ values read back
+
+struct ReadI8Args
+{
+    PoolsI8 pools;
+    const int32_t* table;
+    const int32_t* cu;
+    const int32_t* pos0;
+    float* k;
+    float* v;
+    int M, B, Hkv, shift, table_stride, num_pages, limit;
+};
+
+// Work-group = (64 columns, KV head, keys or values), lane = column, wave = a quarter of the dimensions: code * scale,
+// one rounded product. Bound by the f32 columns that it writes.
+template <int DK>
+__global__ __launch_bounds__(256) void k_pages_read_i8(ReadI8Args a)
+{
+    constexpr int ND = DK / 4;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = blockIdx.y;
+    const bool keys = blockIdx.z == 0;
+    const int m0 = blockIdx.x * kPfTok, m = m0 + lane;
+    const int b = wave_sequence(a.cu, a.B, a.M, m0, lane);
+    if (b < 0) return;
+    const int pos = packed_position(a.cu, a.pos0, b, m, a.limit);
+    size_t row = 0;
+    float s = __builtin_nanf("");  // a position that has no place
+    if (pos >= 0)
+    {
+        const int id = a.table[(size_t)b * a.table_stride + (pos >> a.shift)];
+        if (page_ok(id, a.num_pages))
+        {
+            row = page_row(id, g, pos & ((1 << a.shift) - 1), a.Hkv, a.shift);
+            s = (keys ? a.pools.ks : a.pools.vs)[row >> a.pools.bshift];
+        }
+    }
+    int8_t c[ND];
+    if (keys)
+    {
+#pragma unroll
+        for (int i = 0; i < ND; i += 16)
+        {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(a.pools.k + key_byte(row, w * ND + i, DK));
+#pragma unroll
+            for (int e = 0; e < 16; ++e) c[i + e] = (int8_t)(x[e / 4] >> (8 * (e & 3)));
+        }
+    }
+    else
+    {
+#pragma unroll
+        for (int i = 0; i < ND; ++i) c[i] = a.pools.v[value_byte(row, w * ND + i, DK)];
+    }
+    float* const out = (keys ? a.k : a.v) + (size_t)(g * DK + w * ND) * (size_t)a.M + (size_t)m;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) out[(size_t)i * (size_t)a.M] = __fmul_rn((float)c[i], s);
+}
+
+// ------------------------------------------------------------------ attention of one new token per sequence
+
+// The new token of a sequence into its page, by one wave: its rotated key and its value (element i at k[i * step]),
+// of KV head g at position p, whose page is `id`. Nothing is written for a page outside the pool.
+template <int DK>
+__device__ __forceinline__ void append_i8(const PoolsI8& pools, const float* k, const float* v, size_t step, const float* cosT,
+                                          const float* sinT, int p, int id, int num_pages, int g, int Hkv, int shift)
+{
+    constexpr int HALF = DK / 2, N = (HALF + 63) / 64;
+    const int lane = threadIdx.x & 63, into = p & ((1 << pools.bshift) - 1);
+    float x[2][2][N];  // keys, values; the halves
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+    {
+        const int i = min(lane + 64 * n, HALF - 1);
+        x[0][0][n] = k[i * step], x[0][1][n] = k[(i + HALF) * step];
+        x[1][0][n] = v[i * step], x[1][1][n] = v[(i + HALF) * step];
+    }
+    if (!page_ok(id, num_pages)) return;
+    const size_t row = page_row(id, g, p & ((1 << shift) - 1), Hkv, shift), at = row >> pools.bshift;
+    float s_old[2] = {0.0f, 0.0f};
+    if (into > 0) s_old[0] = pools.ks[at], s_old[1] = pools.vs[at];
+    if (cosT)
+    {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+        {
+            const size_t r = (size_t)p * HALF + (size_t)min(lane + 64 * n, HALF - 1);
+            pg_rope(x[0][0][n], x[0][1][n], cosT[r], sinT[r], x[0][0][n], x[0][1][n]);
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+    {
+        float top = 0.0f;
+#pragma unroll
+        for (int n = 0; n < N; ++n) top = fmaxf(top, fmaxf(fabsf(x[q][0][n]), fabsf(x[q][1][n])));
+        const uint32_t bits = wave_max(__builtin_bit_cast(uint32_t, top));
+        float s = __fmul_rn(__builtin_bit_cast(float, bits), 1.0f / 127.0f);
+        if (into > 0) s = fmaxf(s, s_old[q]);
+        int8_t* const pool = q ? pools.v : pools.k;
+        if (into > 0 && s > s_old[q]) requantize(pool, row - into, into, DK, q == 0, s_old[q], s, lane, 64);
+        if (lane == 0 && (into == 0 || s > s_old[q])) (q ? pools.vs : pools.ks)[at] = s;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            if (lane + 64 * n < HALF)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                {
+                    const int d = lane + 64 * n + HALF * h;
+                    pool[q ? value_byte(row, d, DK) : key_byte(row, d, DK)] = (int8_t)quantize_one(x[q][h][n], s);
+                }
+    }
+}
+
+// The append by itself, for calls whose attention reads a KV head by more than one work-group a chunk
+template <int DK>
+__global__ __launch_bounds__(64) void k_pages_append_i8(PagesArgs a, PoolsI8 pools)
+{
+    const int g = blockIdx.x, b = blockIdx.y, p = a.pos[b];
+    if (p < 0 || p >= a.len_bound) return;
+    const size_t at = a.tokens ? ((size_t)b * a.Hkv + g) * DK : (size_t)g * DK * a.B + b;
+    append_i8<DK>(pools, a.k + at, a.v + at, a.tokens ? 1 : (size_t)a.B, a.cosT, a.sinT, p,
+                  a.table[(size_t)b * a.table_stride + (p >> a.shift)], a.num_pages, g, a.Hkv, a.shift);
+}
+
+constexpr int kI8Tile = 64;       // positions of a wave's tile
+constexpr float kI8Room = 4.0f;   // log2 units between a new reference maximum and the largest score
+constexpr int kI8Pitch = 80;      // bytes of a row of weights' digits in LDS (64 positions)
+
+// X as four signed base-256 digits, X = sum d_i 256^i, the bytes of the result (|X| < 2^31 - 2^23.01)
+__device__ __forceinline__ uint32_t digits(uint32_t X) { return (X + 0x80808080u) ^ 0x80808080u; }
+
+__device__ __forceinline__ float pow2_field(int field) { return __builtin_bit_cast(float, (uint32_t)field << 23); }
+
+// Order between a wave's own LDS accesses of different lanes
+__device__ __forceinline__ void wave_lds_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Attention of one new token per sequence: work-groups as k_pages_attn's (a chunk of positions of a sequence, a KV head
+// and a group of at most 4 NS of its query heads; four waves take the chunk's tiles in turn), records and join the
+// same. Both products run on the int8 MFMA with the codes as they lie in the pools:
+//   scores  a head's rotated query as 30-bit fixed point under its largest element, |X| < 2^30, in four
+//           signed base-256 digits: rows 4 h + i of a 16 x 64 operand for four heads, against 16 positions' keys. Every
+//           partial sum is exact in int32, and a lane finds the four digit sums of one head and position in its
+//           registers; s = (256 a3 + a2) 2^16 + (256 a1 + a0) is rounded as an f32.
+//   values  the weights of a tile, times their blocks' scales over the tile's largest (a power of two above it), as
+//           30-bit fixed point in the same digits, through LDS to the columns of an operand; the digits' sums over
+//           the tile's 64 positions are exact, and each is added to an f32 sum of its own, joined at the end.
+// So neither codes are converted nor multiplied by their scales one by one: 190 VALU instructions a tile of 64
+// positions for 4 heads of 128, where multiply-adds on widened elements would take 1300.
+// A head's reference maximum moves when a score passes it, to 4 above that score (weights are 2^-4 at most then and
+// 1 at most later: none is held to less than 2^-26 of the largest).
+// The chunk that holds the new position first writes its key and value, by the wave that reads them; no other wave
+// reads that block.
+// A block whose scale is not finite (its tokens had an infinity) stands for NaN, and so does a query with one.
+template <int DK, int NS, bool kFinal>
+__global__ __launch_bounds__(kPgThreads) void k_pages_attn_i8(PagesArgs a, PoolsI8 pools, int append)
+{
+    constexpr int HALF = DK / 2, RT = 4 * NS, KC = DK / 64, ND = DK / 16;
+    constexpr int QI = (RT * HALF + kPgThreads - 1) / kPgThreads;  // query pairs per thread
+    __shared__ __align__(16) float q_s[RT * DK];
+    __shared__ __align__(16) uint8_t w_s[kPgWaves][NS][16 * kI8Pitch];
+    __shared__ float ml_s[2][kPgWaves][RT];
+    __shared__ __align__(16) float red_s[kPgWaves][RT * DK];
+    __shared__ int bad_s[kPgWaves];
+
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 15, grp = lane >> 4;
+    const int HG = a.Hkv * a.groups;
+    const int gh = blockIdx.x % HG, item = blockIdx.x / HG;
+    const int g = gh / a.groups, hg = gh - g * a.groups;
+    const PagesItem it = !kFinal && a.even ? find_item(a, item)
+                                           : PagesItem{item / a.nchunk, item % a.nchunk, a.chunk, item - item % a.nchunk,
+                                                       a.pos[item / a.nchunk]};
+    if (it.b < 0) return;
+    const int b = it.b, c = it.c, p = it.p;
+    const int h0 = g * a.R + hg * a.RG;        // first query head
+    const int R = min(a.RG, a.R - hg * a.RG);  // query heads here (<= RT)
+    const size_t io_step = a.tokens ? 1 : (size_t)a.B;
+    float qx[QI][2];
+#pragma unroll
+    for (int u = 0; u < QI; ++u)
+    {
+        const int e = tid + u * kPgThreads, r = min(e / HALF, R - 1), i = e % HALF;
+        const float* q = a.q + (a.tokens ? ((size_t)b * a.H + h0 + r) * DK : (size_t)(h0 + r) * DK * a.B + b);
+        qx[u][0] = q[i * io_step];
+        qx[u][1] = q[(i + HALF) * io_step];
+    }
+    float* const out = a.out + (a.tokens ? ((size_t)b * a.H + h0) * DK : (size_t)h0 * DK * a.B + b);
+    if (p < 0 || p >= a.len_bound)
+    {
+        // no token: zeros; a position past the bound: NaN
+        if (c == 0)
+            for (int e = tid; e < R * DK; e += kPgThreads) out[e * io_step] = p < 0 ? 0.0f : __builtin_nanf("");
+        return;
+    }
+    if (!kFinal && a.even && c == 0 && gh == 0 && tid == 0) a.places[b] = make_int2(it.first, it.chunk);
+    const int t0 = c * it.chunk;
+    if (t0 > p) return;
+    const int last = min(p, t0 + it.chunk - 1);  // the chunk's last position
+
+    // ---- the tiles: a lane looks up the page of group lane % 4 of 16 positions
+    const int32_t* const table = a.table + (size_t)b * a.table_stride;
+    const int slot_mask = (1 << a.shift) - 1;
+    bool bad = false;
+    int id;
+    auto load_id = [&](int t) { id = table[min(t + 16 * (lane & 3), last) >> a.shift]; };
+    u32x4 kf[4][KC], vf[ND];
+    float ks = 0.0f, vs = 0.0f;
+    auto load = [&](int t) {
+        const int at = t + 16 * (lane & 3);
+        const bool in = page_ok(id, a.num_pages);
+        bad |= !in;
+        // groups behind the last position read the last one's rows (their scores are -inf)
+        const int row = (int)(page_row(in ? id : 0, g, min(at, last & ~15) & slot_mask, a.Hkv, a.shift) >> 4);
+        ks = pools.ks[row >> (pools.bshift - 4)];
+        vs = pools.vs[row >> (pools.bshift - 4)];
+        if (at > last) ks = vs = 0.0f;
+        load_id(t + kPgWaves * kI8Tile);
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+        {
+            const u32x4* k = reinterpret_cast<const u32x4*>(pools.k + (size_t)__builtin_amdgcn_readlane(row, n) * (16 * DK)) + lane;
+#pragma unroll
+            for (int i = 0; i < KC; ++i) kf[n][i] = __builtin_nontemporal_load(k + 64 * i);
+        }
+        const u32x4* v = reinterpret_cast<const u32x4*>(pools.v + (size_t)__shfl(row, grp, kWave) * (16 * DK)) + j;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) vf[i] = __builtin_nontemporal_load(v + 16 * i);
+    };
+    const int first = t0 + w * kI8Tile;
+    load_id(first);
+    const int new_tile = p & -kI8Tile;
+    if (append && p == last && first <= new_tile && (new_tile - first) % (kPgWaves * kI8Tile) == 0)
+    {
+        const size_t at = a.tokens ? ((size_t)b * a.Hkv + g) * DK : (size_t)g * DK * a.B + b;
+        append_i8<DK>(pools, a.k + at, a.v + at, io_step, a.cosT, a.sinT, p, table[p >> a.shift], a.num_pages, g, a.Hkv, a.shift);
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
+    }
+    if (first <= last) load(first);  // on its way during the rest
+
+    // ---- rotated queries, as digits
+#pragma unroll
+    for (int u = 0; u < QI; ++u)
+    {
+        const int e = tid + u * kPgThreads, r = e / HALF, i = e % HALF;
+        float y0 = qx[u][0], y1 = qx[u][1];
+        if (a.cosT) pg_rope(y0, y1, a.cosT[(size_t)p * HALF + i], a.sinT[(size_t)p * HALF + i], y0, y1);
+        if (e < RT * HALF)
+        {
+            // (heads past R stay 0)
+            q_s[r * DK + i] = r < R ? y0 : 0.0f;
+            q_s[r * DK + i + HALF] = r < R ? y1 : 0.0f;
+        }
+    }
+    lds_barrier();
+    u32x4 qd[NS][KC];
+    float unit[NS], slope2[NS];  // of head 4 s + lane / 16
+    // (a product past f32's range would make a score of 0 NaN; any other score is past the cap, or the range, with the
+    // largest float, too)
+    auto held = [](float x) { return fminf(fmaxf(x, -3.40282347e38f), 3.40282347e38f); };
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+    {
+        const float* const q = q_s + (4 * s + (j >> 2)) * DK + 16 * grp;
+        uint32_t mx = 0;
+#pragma unroll
+        for (int i = 0; i < KC; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mx = max(mx, __builtin_bit_cast(uint32_t, q[64 * i + e]) & 0x7FFFFFFFu);
+        mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16, kWave));
+        mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32, kWave));
+        const int e0 = max((int)(mx >> 23), 30);  // the largest is below 2^(e0 - 126)
+        const float up = pow2_field(283 - e0);           // brings it below 2^30
+#pragma unroll
+        for (int i = 0; i < KC; ++i)
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+            {
+                uint32_t y = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                {
+                    const uint32_t d = digits((uint32_t)(int)__builtin_rintf(q[64 * i + 4 * n + e] * up));
+                    y |= (d >> (8 * (j & 3)) & 0xFFu) << (8 * e);
+                }
+                qd[s][i][n] = y;
+            }
+        // (1 / up is a power of two)
+        float own = mx >= 0x7F800000u ? __builtin_nanf("") : 1.0f / up;
+        own = __shfl(own, 4 * grp, kWave);
+        const float to = a.cap2 > 0.0f ? a.capi : a.scale2;
+        unit[s] = own == own ? held(own * to) : own;
+        slope2[s] = a.slopes && 4 * s + grp < R ? a.slopes[h0 + 4 * s + grp] * 1.44269504f : 0.0f;
+    }
+
+    v4f acc[NS][ND];
+    float m[NS], l[NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+    {
+        m[s] = -__builtin_inff(), l[s] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) acc[s][i] = v4f{};
+    }
+    auto tile = [&](int t, const u32x4(&kf)[4][KC], const u32x4(&vf)[ND], float ks, float vs) {
+        // a power of two above the tile's largest scale of values
+        float top_v = fmaxf(vs, dpp<kDppXor1>(vs));
+        top_v = fmaxf(top_v, dpp<kDppXor2>(top_v));
+        const bool odd = __builtin_amdgcn_ballot_w64(!(fabsf(vs) < __builtin_inff())) != 0;
+        const int ev = min(max(__builtin_amdgcn_readfirstlane((int)(__builtin_bit_cast(uint32_t, top_v) >> 23)), 31), 252);
+        const float down = odd ? 0.0f : pow2_field(253 - ev);                  // 2^(126 - ev) times a scale is at most 1
+        const float back = odd ? __builtin_nanf("") : pow2_field(ev - 29);     // 2^(ev - 126 - 30)
+        float kg[4], vg[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+        {
+            kg[n] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), n));
+            vg[n] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs), n)) * down;
+        }
+        const bool part = t + kI8Tile - 1 > last;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+        {
+            float x[4];
+            float top = -__builtin_inff();
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+            {
+                v4i d = v4i{};
+#pragma unroll
+                for (int i = 0; i < KC; ++i)
+                    d = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, qd[s][i]), __builtin_bit_cast(v4i, kf[n][i]), d, 0, 0, 0);
+                const int hi = (int)((uint32_t)d[3] << 8) + d[2], lo = (int)((uint32_t)d[1] << 8) + d[0];
+                float f = unit[s] * kg[n];
+                f = kg[n] < __builtin_inff() && f == f ? held(f) : __builtin_nanf("");
+                x[n] = __builtin_fmaf((float)hi, 65536.0f, (float)lo) * f;
+                if (a.cap2 > 0.0f) x[n] = a.cap2 * tanh_any(x[n]);
+                const int at = t + 16 * n + j;
+                if (a.slopes) x[n] = __builtin_fmaf(slope2[s], (float)(at - p), x[n]);
+                if (part && at > last) x[n] = -__builtin_inff();
+                top = fmaxf(top, x[n]);
+            }
+            top = fmaxf(top, dpp<kDppRor8>(top));
+            top = fmaxf(top, dpp<kDppRor4>(top));
+            top = fmaxf(top, dpp<kDppXor2>(top));
+            top = fmaxf(top, dpp<kDppXor1>(top));
+            if (__builtin_amdgcn_ballot_w64(top > m[s]) != 0)
+            {
+                const float to = top > m[s] ? top + kI8Room : m[s];
+                const float corr = m[s] == to ? 1.0f : __builtin_amdgcn_exp2f(m[s] - to);
+                l[s] *= corr;
+                m[s] = to;
+                const float f = __shfl(corr, (j >> 2) * 16, kWave);
+#pragma unroll
+                for (int i = 0; i < ND; ++i) acc[s][i] *= f;
+            }
+            uint8_t* const to = w_s[w][s] + 4 * grp * kI8Pitch + j;
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+            {
+                // no score above -inf yet: nothing to add (and no -inf - -inf)
+                const float pr = x[n] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x[n] - m[s]);
+                l[s] += pr;
+                const uint32_t d = digits((uint32_t)__builtin_fmaf(pr * vg[n], 0x1p30f, 0.5f));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) to[i * kI8Pitch + 16 * n] = (uint8_t)(d >> (8 * i));
+            }
+        }
+        wave_lds_fence();
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+        {
+            const v4i wd = *reinterpret_cast<const v4i*>(w_s[w][s] + j * kI8Pitch + 16 * grp);
+#pragma unroll
+            for (int i = 0; i < ND; ++i)
+            {
+                const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, vf[i]), wd, v4i{}, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[s][i][e] = __builtin_fmaf((float)d[e], back, acc[s][i][e]);
+            }
+        }
+        wave_lds_fence();
+    };
+    for (int t = first; t <= last; t += kPgWaves * kI8Tile)
+    {
+        u32x4 k_now[4][KC], v_now[ND];
+        const float ks_now = ks, vs_now = vs;
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int i = 0; i < KC; ++i) k_now[n][i] = kf[n][i];
+#pragma unroll
+        for (int i = 0; i < ND; ++i) v_now[i] = vf[i];
+        if (t + kPgWaves * kI8Tile <= last) load(t + kPgWaves * kI8Tile);
+        tile(t, k_now, v_now, ks_now, vs_now);
+    }
+
+    // ---- join of the four waves
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+    {
+        l[s] += dpp<kDppRor8>(l[s]);
+        l[s] += dpp<kDppRor4>(l[s]);
+        l[s] += dpp<kDppXor2>(l[s]);
+        l[s] += dpp<kDppXor1>(l[s]);
+        if (j == 0) ml_s[0][w][4 * s + grp] = m[s], ml_s[1][w][4 * s + grp] = l[s];
+    }
+    const bool any_bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+    if (lane == 0) bad_s[w] = any_bad;
+    __syncthreads();
+    const float digit = pow2_field(127 + 8 * (j & 3));
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+    {
+        const int h = 4 * s + (j >> 2);
+        const float own = ml_s[0][w][h], top = fmaxf(fmaxf(ml_s[0][0][h], ml_s[0][1][h]), fmaxf(ml_s[0][2][h], ml_s[0][3][h]));
+        const float f = (own == top ? 1.0f : __builtin_amdgcn_exp2f(own - top)) * digit;
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+        {
+            v4f y = acc[s][i] * f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+            {
+                y[e] += dpp<kDppXor1>(y[e]);
+                y[e] += dpp<kDppXor2>(y[e]);
+            }
+            if ((i & 3) == (j & 3)) *reinterpret_cast<v4f*>(&red_s[w][h * DK + 16 * i + 4 * grp]) = y;
+        }
+    }
+    __syncthreads();
+    const bool lost = (bad_s[0] | bad_s[1] | bad_s[2] | bad_s[3]) != 0;
+    float* const rec = a.part + ((size_t)(it.first + c) * HG + gh) * (size_t)(a.RG * DK + kPgRec);
+    for (int e = tid; e < R * DK; e += kPgThreads)
+    {
+        const int r = e / DK;
+        const float top = fmaxf(fmaxf(ml_s[0][0][r], ml_s[0][1][r]), fmaxf(ml_s[0][2][r], ml_s[0][3][r]));
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPgWaves; ++i)
+            sum += ml_s[1][i][r] * (ml_s[0][i][r] == top ? 1.0f : __builtin_amdgcn_exp2f(ml_s[0][i][r] - top));
+        if (lost) sum = __builtin_nanf("");
+        const float y = (red_s[0][e] + red_s[1][e]) + (red_s[2][e] + red_s[3][e]);
+        if constexpr (kFinal) out[e * io_step] = sum == 0.0f ? 0.0f : y / sum;
+        else
+        {
+            rec[e] = y;
+            if (e % DK == 0)
+            {
+                rec[a.RG * DK + r] = top;
+                rec[a.RG * DK + 8 + r] = sum;
+            }
+        }
+    }
+}
+
+template <int DK, int NS>
+hipError_t launch_attn_i8(hipStream_t st, const PagesArgs& a, const PoolsI8& pools)
+{
+    const bool alone = a.k && a.groups > 1;
+    if (alone)
+    {
+        k_pages_append_i8<DK><<<dim3((unsigned)a.Hkv, (unsigned)a.B), 64, 0, st>>>(a, pools);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    const int append = a.k && !alone;
+    const dim3 grid((unsigned)(pages_items(a.B, a.len_bound, a.chunk, a.even) * a.Hkv * a.groups));
+    if (a.nchunk == 1)
+    {
+        k_pages_attn_i8<DK, NS, true><<<grid, kPgThreads, 0, st>>>(a, pools, append);
+        return hipGetLastError();
+    }
+    k_pages_attn_i8<DK, NS, false><<<grid, kPgThreads, 0, st>>>(a, pools, append);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    k_pages_join<DK><<<dim3((unsigned)a.H, (unsigned)a.B), kPgThreads, 0, st>>>(a);
+    return hipGetLastError();
+}
+
+PoolsI8 pools_of(const nnhip_kv_pages_i8& kv)
+{
+    return {static_cast<int8_t*>(kv.k), static_cast<int8_t*>(kv.v), kv.k_scale, kv.v_scale, log2_of(kv.block)};
+}
+
+}  // namespace
+
+hipError_t launch_pages_attn_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, const float* q, const float* k, const float* v,
+                                size_t B, size_t H, const int32_t* pos, size_t len_bound, const float* cosT,
+                                const float* sinT, float scale, float softcap, const float* slopes, bool tokens,
+                                float* part, float* out, size_t num_cus)
+{
+    constexpr double kLog2e = 1.4426950408889634;
+    const size_t R = H / kv.Hkv, dk = kv.dk, groups = pages_groups(R, dk);
+    const PagesCut cut = pages_cut(B, kv.Hkv, R, dk, len_bound, num_cus);
+    const bool cap = softcap > 0.0f;
+    PagesArgs a{q, k, v, pos, cosT, sinT, kv.k, kv.v, kv.table, slopes, part,
+                reinterpret_cast<int2*>(part + (cut.even ? pages_records(B, kv.Hkv, groups, ceil_div(R, groups), dk, len_bound, cut) : 0)),
+                out, (int)B, (int)H, (int)kv.Hkv, (int)R,
+                (int)groups, (int)ceil_div(R, groups), log2_of(kv.page_size), (int)kv.table_stride, (int)kv.num_pages,
+                (int)len_bound, (int)cut.chunk, (int)cut.nchunk, (int)cut.even, (float)(scale * kLog2e),
+                cap ? scale / softcap : 0.0f, cap ? (float)(softcap * kLog2e) : 0.0f, tokens ? 1 : 0};
+    const PoolsI8 pools = pools_of(kv);
+    if (dk == 256) return launch_attn_i8<256, 1>(st, a, pools);
+    if (dk == 128) return a.RG <= 4 ? launch_attn_i8<128, 1>(st, a, pools) : launch_attn_i8<128, 2>(st, a, pools);
+    if (dk == 64) return a.RG <= 4 ? launch_attn_i8<64, 1>(st, a, pools) : launch_attn_i8<64, 2>(st, a, pools);
+    return hipErrorInvalidValue;
+}
+
+hipError_t launch_pages_fill_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, const float* k, const float* v, size_t M,
+                                const int32_t* cu, const int32_t* pos0, size_t B, const float* cosT, const float* sinT,
+                                size_t limit)
+{
+    const FillI8Args a{k, v, cu, pos0, cosT, sinT, pools_of(kv), kv.table, (int)M, (int)B, (int)kv.Hkv, log2_of(kv.page_size),
+                       (int)kv.table_stride, (int)kv.num_pages, (int)limit};
+    const dim3 grid((unsigned)ceil_div(M, kPfTok), (unsigned)kv.Hkv, 2);
+    if (kv.dk == 64) k_pages_fill_i8<64><<<grid, 256, 0, st>>>(a);
+    else if (kv.dk == 128) k_pages_fill_i8<128><<<grid, 256, 0, st>>>(a);
+    else if (kv.dk == 256) k_pages_fill_i8<256><<<grid, 256, 0, st>>>(a);
+    else return hipErrorInvalidValue;
+    return hipGetLastError();
+}
+
+hipError_t launch_pages_read_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, size_t M, const int32_t* cu, const int32_t* pos0,
+                                size_t B, float* k, float* v)
+{
+    const ReadI8Args a{pools_of(kv), kv.table, cu, pos0, k, v, (int)M, (int)B, (int)kv.Hkv, log2_of(kv.page_size),
+                       (int)kv.table_stride, (int)kv.num_pages, (int)(kv.table_stride * kv.page_size)};
+    const dim3 grid((unsigned)ceil_div(M, kPfTok), (unsigned)kv.Hkv, 2);
+    if (kv.dk == 64) k_pages_read_i8<64><<<grid, 256, 0, st>>>(a);
+    else if (kv.dk == 128) k_pages_read_i8<128><<<grid, 256, 0, st>>>(a);
+    else if (kv.dk == 256) k_pages_read_i8<256><<<grid, 256, 0, st>>>(a);
+    else return hipErrorInvalidValue;
+    return hipGetLastError();
+}
+
+}  // namespace nnhip

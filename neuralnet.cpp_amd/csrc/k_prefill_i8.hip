@@ -1,0 +1,512 @@
+// k_prefill_i8.hip — attention of packed prompts over a paged KV cache in 8 bits (k_pages_i8.hip's pools): unlike
+// lengths, positions and prefixes, a tanh cap and a bias on the scores, as k_prefill.hip's over f32 and f16 pages.
+//
+// A work-group = 8 waves = (R heads of a KV head) x (8 / R blocks of 32 queries); lane l holds query l % 32 of its wave
+// throughout. Tiles of 64 keys are staged in LDS (double buffered, one barrier a tile) as f16, which holds every code
+// as it is: keys as rows of dk, values as rows of 64 keys, in the order in which the weights of a query lie in its
+// lane. The codes are widened once for the 256 queries (5 instructions for 4 of them), and no code is multiplied by its scale:
+//   S^T = K . Q^T  with each query in two f16 parts, q 2^e = hi + lo to 2^-23 of it (and 2^-40 of the query's
+//                  largest): two v_mfma_f32_32x32x16_f16 a step, whose products are exact; a key's scale is a factor of
+//                  the 16 scores that share it, folded into the exponential's argument with the softmax scale;
+//   O^T += V^T . P^T  with the weights in two f16 parts, 2^6 .. 2^15 at their largest, the scale of the values folded into the
+//                  weights by its logarithm in the same argument. Parts hold 22 bits of every weight down to 2^-24 of the largest and
+//                  2^-40 of the largest below. So that no scale costs bits, O is kept in units of a power of two within
+//                  2^-6 .. 2 of the group's scale: where a group's leaves that range, O moves to another unit first.
+// O^T stays in the accumulators over all tiles; a query's reference maximum moves when its maximum has grown by
+// 2^8, by a whole power of two. Sums and softmax are f32. The next tile is converted by half of the waves before their
+// products and by the other half behind them, so that every SIMD has one of each.
+// Work-groups take equal spans of all tiles and join the items they share (prompt_spans.hpp).
+// A query that holds an infinity or a NaN gets NaN, and so does one that sees a block whose scale is not finite.
+#include "prompt_spans.hpp"
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+
+namespace nnhip
+{
+namespace
+{
+
+struct ScalesI8
+{
+    const float* k;
+    const float* v;
+    int bshift;  // log2(positions of a scale)
+};
+
+constexpr int kI8Keys = 64;      // keys of a tile, two halves of kPK
+constexpr float kI8Up = 6.0f;    // log2 of the largest weight when a reference maximum is new
+constexpr int kI8Low = 6;        // a group's scale of values is at most this many powers of two below O's unit
+
+template <int DK>
+struct TileI8
+{
+    // rows are padded by 16 bytes: 16 lanes' accesses of consecutive rows fall on all banks
+    static constexpr int kKPitch = DK * 2 + 16, kVPitch = kI8Keys * 2 + 16;
+    static constexpr int kV = kI8Keys * kKPitch, kBuf = kV + DK * kVPitch;
+    static constexpr int kTPitch = DK * 2 + 16;  // rows of the cos / sin tables, before the first tile
+    static constexpr int kTables = 2 * 32 * kPWaves * kTPitch;
+    static constexpr int kMain = 2 * kBuf > kTables ? 2 * kBuf : kTables;
+    static constexpr int kScales = kMain;          // [2][2][4]: per buffer, of keys and of values
+    static constexpr int kFound = kMain + 64;      // [8]
+    static constexpr int kBytes = kMain + 96;
+};
+
+// Four codes as f16: 1024 + 128 + code is the byte code + 128 under the exponent of 1024
+__device__ __forceinline__ u32x2 widen_codes(uint32_t x)
+{
+    const uint32_t u = x ^ 0x80808080u;
+    const v2h off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    const v2h a = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + off;
+    const v2h b = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + off;
+    return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+}
+
+// Attention of an item over its tiles of 32 keys k0 .. k1 - 1; rec: into a record instead of the output
+template <int DK, bool kShaped>
+__device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& sc, const PrefillItem& item, uint8_t* smem,
+                                          int k0, int k1, float* rec, bool distance)
+{
+    using Tile = TileI8<DK>;
+    constexpr int NC = DK / 16;  // MFMA steps over the head dimension
+    constexpr int ND = DK / 32;  // 32-row blocks of O^T
+    constexpr int NPC = 4 * DK;  // 16-byte pieces of a tile's keys, or values
+    float* const scales = reinterpret_cast<float*>(smem + Tile::kScales);
+    int* const found_s = reinterpret_cast<int*>(smem + Tile::kFound);
+
+    // (opaque per item, so that no thread-index arithmetic stays alive across the items)
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, h = lane >> 5, l32 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    PrefillWave w;
+    PrefillSeq<true> seq;
+    int last_key;
+    seat(a, item, tid, w, seq, last_key);
+    const int end_key = min(last_key, k1 * kPK - 1);  // the last key of these tiles
+
+    // ---- staging: a wave's pieces are of one group of 16 positions
+    const int group = wave * 64 % NPC / DK;
+    const bool has_k = DK == 128 || wave < 4, has_v = DK == 128 || wave >= 4;
+    const int piece = tid % DK;  // within its group
+    bool bad = false;
+    int id;
+    auto at_group = [&](int kb) { return min(kb * kPK + 16 * group, end_key & ~15); };
+    auto load_id = [&](int kb) { id = a.table[(size_t)w.b * a.table_stride + (at_group(kb) >> a.shift)]; };
+    u32x4 raw_k, raw_v;
+    float raw_s[2];
+    auto load_raw = [&](int kb) {
+        const int page = __builtin_amdgcn_readfirstlane(id);
+        const bool in = page_ok(page, a.num_pages);
+        bad |= !in;
+        const size_t row = page_row(in ? page : 0, w.g, at_group(kb) & ((1 << a.shift) - 1), a.Hkv, a.shift);
+        const size_t off = (row >> 4) * (size_t)(16 * DK) + (size_t)(16 * piece);
+        if (has_k) raw_k = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(a.kc) + off);
+        if (has_v) raw_v = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(a.vc) + off);
+        const bool there = kb * kPK + 16 * group <= end_key;  // (behind the last key: whatever is there)
+        raw_s[0] = there ? sc.k[row >> sc.bshift] : 0.0f;
+        raw_s[1] = there ? sc.v[row >> sc.bshift] : 0.0f;
+        if (kb + 2 < k1) load_id(kb + 2);
+    };
+    auto convert = [&](int par) {
+        uint8_t* const buf = smem + par * Tile::kBuf;
+        if (has_k)
+        {
+            // 16 dimensions (chunk piece / 16) of position piece % 16
+            uint8_t* const dst = buf + (16 * group + (piece & 15)) * Tile::kKPitch + 32 * (piece >> 4);
+            const u32x2 x = widen_codes(raw_k[0]), y = widen_codes(raw_k[1]), z = widen_codes(raw_k[2]), t = widen_codes(raw_k[3]);
+            *reinterpret_cast<u32x4*>(dst) = u32x4{x[0], x[1], y[0], y[1]};
+            *reinterpret_cast<u32x4*>(dst + 16) = u32x4{z[0], z[1], t[0], t[1]};
+        }
+        if (has_v)
+        {
+            // 16 positions of dimension `piece`, as S^T's accumulators hold them: 0..3 and 8..11, then 4..7 and 12..15
+            uint8_t* const dst = buf + Tile::kV + piece * Tile::kVPitch + 32 * group;
+            const u32x2 x = widen_codes(raw_v[0]), y = widen_codes(raw_v[1]), z = widen_codes(raw_v[2]), t = widen_codes(raw_v[3]);
+            *reinterpret_cast<u32x4*>(dst) = u32x4{x[0], x[1], z[0], z[1]};
+            *reinterpret_cast<u32x4*>(dst + 16) = u32x4{y[0], y[1], t[0], t[1]};
+        }
+        if (lane < 2) scales[par * 8 + 4 * lane + group] = lane ? raw_s[1] : raw_s[0];
+    };
+
+    // ---- everything that the first tile waits for on its way together: rows of the cos / sin tables, page ids,
+    // queries, then (with the ids) keys and values
+    const int qn = kPQ << (kPWaveShift - log2_heads(a));
+    constexpr int TC = DK / 8, TU = 32 * kPWaves * TC / kPThreads;  // 16-byte chunks of a row, those of a thread at most
+    float4 tc[TU], ts[TU];
+    if (a.cosT)
+    {
+        const __amdgpu_buffer_rsrc_t rc = pf_rsrc(a.cosT, rope_bytes(a, DK / 2)), rs = pf_rsrc(a.sinT, rope_bytes(a, DK / 2));
+        const uint32_t t_at = (uint32_t)(seq.pos0(a) + item.qb * qn) * (uint32_t)(DK * 2) + (uint32_t)tid * 16u;
+#pragma unroll
+        for (int i = 0; i < TU; ++i)
+            if (i * kPThreads < qn * TC)
+            {
+                tc[i] = ld_f4(rc, t_at + (uint32_t)(i * kPThreads * 16));
+                ts[i] = ld_f4(rs, t_at + (uint32_t)(i * kPThreads * 16));
+            }
+    }
+    load_id(k0);
+    PrefillQuery<DK, 8> query;
+    if (w.live) query.load(a, w, seq, h);
+    if (a.cosT)
+    {
+#pragma unroll
+        for (int i = 0; i < TU; ++i)
+        {
+            const int ct = tid + i * kPThreads;
+            if (ct >= qn * TC) break;
+            uint8_t* dst = smem + ct / TC * Tile::kTPitch + 16 * (ct % TC);
+            *reinterpret_cast<float4*>(dst) = tc[i];
+            *reinterpret_cast<float4*>(dst + qn * Tile::kTPitch) = ts[i];
+        }
+    }
+    __syncthreads();
+    load_raw(k0);
+
+    // ---- the lane's rotated query in halves: step c holds dimensions 16c + 8h + 0..7, scaled by 2^eq
+    v8h qh[NC], ql[NC];
+    float f = 0.0f;  // 2^-eq |scale| log2(e), or over the cap
+    if (w.live)
+    {
+        float qv[DK / 2];
+        uint32_t mx = 0;
+        const uint8_t* tab = smem + (min(w.qt, seq.n(a) - 1) - item.qb * qn) * Tile::kTPitch + 32 * h;
+        auto table = [&](const uint8_t* t, int c, int i) { return *reinterpret_cast<const float4*>(t + 64 * c + 16 * i); };
+        query.rotate(a, [&](int c, int i) { return table(tab, c, i); }, [&](int c, int i) { return table(tab + qn * Tile::kTPitch, c, i); },
+                     [&](int c, int e, float y0, float y1) {
+            qv[8 * c + e] = y0;
+            qv[8 * (c + NC / 2) + e] = y1;
+            mx = max(mx, max(__builtin_bit_cast(uint32_t, y0) & 0x7FFFFFFFu, __builtin_bit_cast(uint32_t, y1) & 0x7FFFFFFFu));
+        });
+        mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32, kWave));
+        const int eq = min(f16_exp(mx), 120);  // (infinities and NaN: -114, and they stay what they are)
+        const float sq = a.scale < 0.0f ? -pow2(eq) : pow2(eq);
+        f = pow2(-eq) * (a.cap2 > 0.0f ? a.scale2 * a.capi2 : a.scale2);
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2)
+            {
+                v2h x, y;
+                split2(qv[8 * c + e] * sq, qv[8 * c + e + 1] * sq, x, y);
+                qh[c][e] = x[0], qh[c][e + 1] = x[1];
+                ql[c][e] = y[0], ql[c][e + 1] = y[1];
+            }
+    }
+    v16f o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] = v16f{};
+    float m_ref = -__builtin_inff(), l_run = 0.0f;  // log2 units; l_run: this lane half's keys
+    int unit = 127;                                 // O is in units of 2^(unit - 127)
+    const float slope2 = kShaped && a.slopes ? a.slopes[w.head] * 1.44269504f : 0.0f;
+    __syncthreads();  // the tables have been read
+    convert(0);
+    if (k0 + 2 < k1) load_raw(k0 + 2);
+    const uint32_t k_at = (uint32_t)(l32 * Tile::kKPitch + 16 * h), v_at = (uint32_t)(Tile::kV + l32 * Tile::kVPitch + 16 * h);
+    int par = 0;
+    for (int kb = k0; kb < k1; kb += 2, par ^= 1)
+    {
+        __syncthreads();  // tile kb is in LDS; the other buffer is free
+        const bool more = kb + 2 < k1;
+        if (more && wave < 4)
+        {
+            convert(par ^ 1);
+            if (kb + 4 < k1) load_raw(kb + 4);  // in flight during this tile's products
+        }
+        const uint8_t* const buf = smem + par * Tile::kBuf;
+        const float* const ts4 = scales + par * 8;
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half)
+        {
+            const int key0 = (kb + half) * kPK;
+            if (!w.live || kb + half >= k1 || key0 > seq.to(a, w)) continue;
+            v16f s = v16f{};
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+            {
+                const v8h k = *reinterpret_cast<const v8h*>(buf + k_at + half * kPK * Tile::kKPitch + 32 * c);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[c], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[c], s, 0, 0, 0);
+            }
+            float kf[2], vs[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+            {
+                kf[t] = f * ts4[2 * half + t];
+                vs[t] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, ts4[4 + 2 * half + t])));
+            }
+            const bool masked = key0 + kPK - 1 > seq.from(a, w);
+            if (kShaped || masked)
+            {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) s[v] *= kf[v >> 3];
+                kf[0] = kf[1] = 1.0f;
+            }
+            if constexpr (kShaped)
+            {
+                // scores rarely reach the cap: a polynomial alone where none does
+                float top = 0.0f;  // (a NaN does not show, and stays one in each form)
+                if (a.cap2 > 0.0f)
+                {
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) top = fmaxf(top, fabsf(s[v]));
+                    if (__builtin_amdgcn_ballot_w64(top > 0.25f) == 0)
+                    {
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) s[v] = tanh_below_quarter(s[v]);
+                    }
+                    else if (__builtin_amdgcn_ballot_w64(top > 1.0f) == 0)
+                    {
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) s[v] = tanh_below1(s[v]);
+                    }
+                    else
+                    {
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) s[v] = tanh_any(s[v]);
+                    }
+                }
+                // (the distance of the half's first key and the steps from there apart)
+                const float one = a.cap2 > 0.0f ? a.cap2 : 1.0f, first = (float)(key0 + 4 * h - w.qpos), away = slope2 * first;
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                {
+                    const float step = (float)(8 * (v >> 2) + (v & 3)), bias = __builtin_fmaf(slope2, step, away);
+                    s[v] = __builtin_fmaf(s[v], one, distance && first + step > 0.0f ? -bias : bias);
+                }
+            }
+            if (masked)
+            {
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                    if (key0 + 8 * (v >> 2) + 4 * h + (v & 3) > seq.sight(w)) s[v] = -__builtin_inff();
+            }
+            float top[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+            {
+                top[t] = s[8 * t];
+#pragma unroll
+                for (int v = 1; v < 8; ++v) top[t] = fmaxf(top[t], s[8 * t + v]);
+                top[t] *= kf[t];
+            }
+            const float mx = __builtin_ceilf(max_halves(fmaxf(top[0], top[1])));
+            // the reference of a query moves only when its maximum has grown by 2^8 (or is new)
+            const bool grown = mx > m_ref + kPLazy;
+            if (__builtin_amdgcn_ballot_w64(grown) != 0)
+            {
+                const float m_new = grown ? mx : m_ref;
+                const float corr = grown ? __builtin_amdgcn_exp2f(m_ref - m_new) : 1.0f;
+                l_run *= corr;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) o[d][v] *= corr;
+                m_ref = m_new;
+            }
+            const float base = kI8Up - (m_ref == -__builtin_inff() ? 0.0f : m_ref);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+            {
+                // the scale of the group's values in O's units
+                const uint32_t bits = __builtin_bit_cast(uint32_t, vs[t]);
+                const int e = (int)(bits >> 23);
+                float lv = 0.0f;  // (a scale of 0: all codes are 0)
+                if (e == 255)
+                {
+                    if (key0 + 16 * t <= seq.sight(w)) l_run = __builtin_nanf("");
+                }
+                else if (bits != 0)
+                {
+                    if (e > unit || e < unit - kI8Low)
+                    {
+                        const float by = __builtin_ldexpf(1.0f, unit - e);
+#pragma unroll
+                        for (int d = 0; d < ND; ++d)
+#pragma unroll
+                            for (int v = 0; v < 16; ++v) o[d][v] *= by;
+                        unit = e;
+                    }
+                    lv = e < 64 ? __builtin_amdgcn_logf(vs[t] * 0x1p64f) - (float)(unit - 127 + 64) : __builtin_amdgcn_logf(vs[t]) - (float)(unit - 127);
+                }
+                const float off = base + lv;
+                float sum = 0.0f;
+                v8h pa, pb;
+#pragma unroll
+                for (int v = 0; v < 8; v += 2)
+                {
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * t + v], kf[t], off));
+                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * t + v + 1], kf[t], off));
+                    sum += p0;
+                    sum += p1;
+                    v2h x, y;
+                    split2(p0, p1, x, y);
+                    pa[v] = x[0], pa[v + 1] = x[1];
+                    pb[v] = y[0], pb[v + 1] = y[1];
+                }
+                l_run = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-lv), l_run);
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+                {
+                    const v8h x = *reinterpret_cast<const v8h*>(buf + v_at + 32 * d * Tile::kVPitch + 32 * (2 * half + t));
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pb, o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pa, o[d], 0, 0, 0);
+                }
+            }
+        }
+        if (more && wave >= 4)
+        {
+            convert(par ^ 1);
+            if (kb + 4 < k1) load_raw(kb + 4);
+        }
+    }
+    l_run += __shfl_xor(l_run, 32);
+    const bool any_bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+    if (lane == 0) found_s[wave] = any_bad;
+    __syncthreads();
+    int found = 0;
+#pragma unroll
+    for (int i = 0; i < kPWaves; ++i) found |= found_s[i];
+    if (found) l_run = __builtin_nanf("");
+    const float by = __builtin_ldexpf(1.0f, unit - 127);
+    auto dim = [](int d, int i) { return 32 * d + i; };
+    if (rec)
+    {
+        store_record<DK>(rec, tid, dim, [&](int d, int v) { return o[d][v] * by; }, m_ref, l_run);
+        return;
+    }
+    if (!w.live) return;
+    // (nothing visible above -infinity: 0)
+    const float den = l_run == 0.0f ? 1.0f : l_run;
+    store_out<DK>(a, w, seq, h, dim, [&](int d, int v) { return o[d][v] * by / den; });
+}
+
+// The items of a work-group of a call of packed prompts, one after the other: attend(item, first tile, end, record or
+// null). One item each, heaviest first (the last queries attend over the most keys) and a step further per block of
+// queries, or a long sequence's work-groups, per_qb apart, would all fall on one or two of the 8 XCDs; or spans.
+template <int DK, typename F>
+__device__ __forceinline__ void prompt_items(const PrefillArgs& a, uint8_t* smem, F&& attend)
+{
+    PrefillItem it;
+    const int groups = a.groups, HG = a.Hkv * groups;
+    const int per_qb = a.B * HG, back = (int)blockIdx.x / per_qb;
+    const int bg = ((int)blockIdx.x + back) % per_qb;
+    const int g = blockIdx.x;
+    PromptCut at, end;
+    if (a.spans)
+    {
+        // the span's two cuts by a wave each, while the others look for sequences that do not fit
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        PromptCut* const cuts = reinterpret_cast<PromptCut*>(smem);
+        if (wave < 2)
+        {
+            const PromptCut cut = prompt_cut(a, a.spans, g + wave);
+            if ((threadIdx.x & 63) == 0)
+            {
+                cuts[wave] = cut;
+                if (wave == 0) prompt_cuts<DK>(a, a.spans)[g] = cut;
+            }
+        }
+        else
+            for (int b = g; b < a.B; b += a.spans)
+                if (PrefillSeq<true> any; !packed_seq(a, b, any)) store_nan<DK>(a, b, 0, a.H, (int)threadIdx.x - 2 * kWave, kPThreads - 2 * kWave);
+        __syncthreads();
+        at = uniform(cuts[0]);
+        end = uniform(cuts[1]);
+        __syncthreads();
+    }
+    else
+    {
+        at = {bg % HG, bg / HG, a.nqb - 1 - back, 0};
+        if (!packed_seq(a, at.b, it.seq))
+        {
+            store_nan<DK>(a, at.b, at.gh * a.R, a.R, at.qb * kPThreads + (int)threadIdx.x, a.nqb * kPThreads);
+            return;
+        }
+        if (at.qb >= prompt_blocks(a, it.seq.n_)) return;
+        end = {at.gh, at.b, at.qb + 1, 0};
+    }
+    bool known = a.spans == 0;  // it.seq is at.b's
+    while (cut_before(at, end))
+    {
+        // the next sequence with a block left
+        const bool there = at.b < a.B;
+        if (!there || !(known || packed_seq(a, at.b, it.seq)) || at.qb >= prompt_blocks(a, it.seq.n_))
+        {
+            at = there ? PromptCut{at.gh, at.b + 1, 0, 0} : PromptCut{at.gh + 1, 0, 0, 0};
+            continue;
+        }
+        const int tiles = prompt_tiles(a, it.seq, at.qb), to = cut_same_item(at, end) ? end.t : tiles;
+        it.b = at.b;
+        it.g = at.gh / groups;
+        it.first = at.gh * a.R;
+        it.qb = at.qb;
+        float* rec = at.t == 0 && to == tiles ? nullptr : prompt_record<DK>(a, g, at.t > 0 ? 0 : 1);
+        attend(it, at.t, to, rec);
+        known = false;
+        at = {at.gh, at.b, at.qb + 1, 0};
+    }
+}
+
+template <int DK, bool kShaped>
+__global__ __launch_bounds__(kPThreads) void k_attn_prefill_i8(PrefillArgs a, ScalesI8 sc, int distance)
+{
+    extern __shared__ __align__(16) uint8_t smem[];
+    prompt_items<DK>(a, smem, [&](const PrefillItem& it, int k0, int k1, float* rec) {
+        attend_i8<DK, kShaped>(a, sc, it, smem, k0, k1, rec, distance != 0);
+    });
+}
+
+template <int DK, bool kShaped>
+hipError_t launch_prefill_i8_dk(hipStream_t st, const PrefillArgs& a, const ScalesI8& sc, bool distance)
+{
+    constexpr int lds = TileI8<DK>::kBytes;
+    static std::atomic<uint64_t> set{0};  // a bit per device
+    int device = 0;
+    hipError_t e = hipGetDevice(&device);
+    if (e != hipSuccess) return e;
+    if (device > 63 || !(set.load() >> device & 1))
+    {
+        e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_attn_prefill_i8<DK, kShaped>),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+        if (device <= 63) set.fetch_or(uint64_t(1) << device);
+    }
+    const unsigned blocks = a.spans ? (unsigned)a.spans : (unsigned)(a.nqb * a.B * a.Hkv * a.groups);
+    hipLaunchKernelGGL((k_attn_prefill_i8<DK, kShaped>), dim3(blocks), dim3(kPThreads), lds, st, a, sc, distance ? 1 : 0);
+    if (a.spans > 1)
+    {
+        e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        k_prompt_join<DK><<<dim3((unsigned)a.spans - 1, DK / 16), 32 * kPWaves, 0, st>>>(a);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_pages_prefill_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, const float* q, size_t M, const int32_t* cu,
+                                   const int32_t* pos0, size_t B, size_t t_bound, size_t H, const float* cosT,
+                                   const float* sinT, size_t limit, float scale, float softcap, const float* slopes,
+                                   const int32_t* prefix, bool distance, float* out, void* ws, size_t num_cus)
+{
+    // a KV head's R query heads in work-groups of 8, 4, 2 or 1
+    const size_t heads = H / kv.Hkv, R = heads % 8 == 0 ? 8 : heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
+    const double cap2 = softcap * 1.4426950408889634;
+    PrefillArgs a{q, kv.k, kv.v, cosT, sinT, out, (int)B, (int)t_bound, (int)H, (int)kv.Hkv, (int)R, 0,
+                  (int)limit, (int)std::max<size_t>(1, ceil_div(std::min(t_bound, limit), kPQ * (kPWaves / R))), scale,
+                  (float)(std::fabs(scale) * 1.4426950408889634), 0,
+                  (int)M, (int)(heads / R), kv.table, cu, pos0, prefix, slopes, (int)kv.table_stride, (int)kv.num_pages,
+                  0, (int)limit, (float)cap2, softcap > 0.0f ? (float)(1.0 / cap2) : 0.0f,
+                  static_cast<float*>(ws), (int)pages_prefill_spans(limit, num_cus)};
+    while ((size_t(1) << a.shift) < kv.page_size) ++a.shift;
+    ScalesI8 sc{kv.k_scale, kv.v_scale, 0};
+    while ((size_t(1) << sc.bshift) < kv.block) ++sc.bshift;
+    if (cap2 > 0.0 || slopes)
+        return kv.dk == 64 ? launch_prefill_i8_dk<64, true>(st, a, sc, distance) : launch_prefill_i8_dk<128, true>(st, a, sc, distance);
+    return kv.dk == 64 ? launch_prefill_i8_dk<64, false>(st, a, sc, distance) : launch_prefill_i8_dk<128, false>(st, a, sc, distance);
+}
+
+}  // namespace nnhip

@@ -24,6 +24,25 @@ NNHIP_HD size_t page_row(int id, int g, int slot, int Hkv, int shift)
     return (((size_t)id * (size_t)Hkv + (size_t)g) << shift) + (size_t)slot;
 }
 
+// 8-bit pools hold groups of 16 positions of a head, 16 dk bytes each: row / 16 is the group of a row of page_row.
+// Bytes of dimension d of that row: keys as (dk / 16, 16 positions, 16 dimensions), values as (dk, 16 positions).
+NNHIP_HD size_t key_byte(size_t row, int d, int dk)
+{
+    return (row >> 4) * (size_t)(16 * dk) + (size_t)(((d >> 4) << 8) + (int)((row & 15) << 4) + (d & 15));
+}
+NNHIP_HD size_t value_byte(size_t row, int d, int dk)
+{
+    return (row >> 4) * (size_t)(16 * dk) + (size_t)((d << 4) + (int)(row & 15));
+}
+
+// The column, at most m, from which on a packed call's tokens share the scale of the token at column m: that of
+// its sequence's first token cu0, or of the first position of its block of `block` (a power of two) positions
+NNHIP_HD int block_column(int m, int cu0, int position, int block)
+{
+    const int into = position & (block - 1), t = m - cu0;
+    return m - (into < t ? into : t);
+}
+
 // Position of a chunk (its first position t0, a multiple of 8, n > 0 cached rows) where the decode's tile of
 // rows at, at + 1, ... looks up its page: its own, or the chunk's last one (n == 0: the chunk's first).
 NNHIP_HD int tile_lookup(int t0, int at, int n) { return t0 + (at < n ? at : n > 0 ? n - 1 : 0); }

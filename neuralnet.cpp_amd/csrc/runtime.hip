@@ -242,6 +242,65 @@ nnhip_status check_pages(const char* fn, const nnhip_kv_pages* c, const float* r
     return NNHIP_OK;
 }
 
+// A cache in 8 bits, likewise
+nnhip_status check_pages(const char* fn, const nnhip_kv_pages_i8* c, const float* rope_cos, const float* rope_sin)
+{
+    NNHIP_REQUIRE(c && c->k_scale && c->v_scale, fn, "null cache or scales");
+    NNHIP_REQUIRE(c->page_size >= 16, fn, "page_size must be a power of two in [16, 1024]");
+    NNHIP_REQUIRE(c->block >= 16 && c->block <= 64 && c->block <= c->page_size && (c->block & (c->block - 1)) == 0, fn,
+                  "block must be a power of two in [16, 64], at most page_size");
+    const nnhip_kv_pages p{c->k, c->v, c->table, c->num_pages, c->page_size, c->table_stride, c->Hkv, c->dk, 0};
+    return check_pages(fn, &p, rope_cos, rope_sin);
+}
+
+// The host's checks of a decode attention over pages
+template <typename Pages>
+nnhip_status check_decode(const char* fn, const Pages* cache, size_t B, size_t H, size_t len_bound, const float* rope_cos,
+                          size_t rope_len, float softcap)
+{
+    NNHIP_REQUIRE(H >= cache->Hkv && H % cache->Hkv == 0 && H <= 65535, fn,
+                  "H must be a multiple of Hkv, at most 65535");
+    NNHIP_REQUIRE(B <= 65535 && B * H < (size_t(1) << 22), fn, "B must be at most 65535, B * H below 2^22");
+    NNHIP_REQUIRE(len_bound >= 1 && len_bound <= cache->table_stride * cache->page_size, fn,
+                  "len_bound must be in [1, table_stride * page_size]");
+    NNHIP_REQUIRE(!rope_cos || len_bound <= rope_len, fn, "len_bound must not exceed the rows of the rope tables");
+    NNHIP_REQUIRE(softcap >= 0.0f && softcap <= 1.0e30f && (softcap == 0.0f || softcap >= 1.0e-30f), fn,
+                  "softcap must be 0 or in [1e-30, 1e30]");
+    return NNHIP_OK;
+}
+
+// and of an attention of packed prompts; limit: positions that have a place
+template <typename Pages>
+nnhip_status check_prompts(const char* fn, const Pages* cache, size_t M, size_t B, size_t t_bound, size_t H, const float* rope_cos,
+                           size_t rope_len, float softcap, size_t& limit)
+{
+    NNHIP_REQUIRE(H >= cache->Hkv && H % cache->Hkv == 0 && H <= 65535, fn,
+                  "H must be a multiple of Hkv, at most 65535");
+    NNHIP_REQUIRE(M < (size_t(1) << 29) && H * cache->dk * M < (size_t(1) << 29), fn,
+                  "q / out must be below 2^29 elements");
+    NNHIP_REQUIRE(softcap >= 0.0f && softcap <= 1.0e30f && (softcap == 0.0f || softcap >= 1.0e-30f), fn,
+                  "softcap must be 0 or in [1e-30, 1e30]");
+    NNHIP_REQUIRE(t_bound <= M, fn, "t_bound must not exceed M");
+    limit = cache->table_stride * cache->page_size;
+    if (rope_cos) limit = std::min(limit, rope_len);
+    NNHIP_REQUIRE(!rope_cos || limit * cache->dk < (size_t(1) << 30), fn, "rope tables must be below 2 GiB");
+    NNHIP_REQUIRE(B < (size_t(1) << 22) && B * H < (size_t(1) << 22), fn, "B * H must be below 2^22");
+    return NNHIP_OK;
+}
+
+// The host's checks of a page table
+nnhip_status check_table(const char* fn, const int32_t* table, size_t table_stride, size_t page_size, size_t num_pages, size_t B)
+{
+    NNHIP_REQUIRE(table, fn, "null page table");
+    NNHIP_REQUIRE(page_size >= 8 && page_size <= 1024 && (page_size & (page_size - 1)) == 0, fn,
+                  "page_size must be a power of two in [8, 1024]");
+    NNHIP_REQUIRE(num_pages >= 1 && num_pages <= kMaxDim / page_size, fn, "num_pages * page_size must be in [1, 2^31)");
+    NNHIP_REQUIRE(table_stride >= 1 && table_stride <= (size_t(1) << 30) / page_size, fn,
+                  "table_stride * page_size must be in [1, 2^30]");
+    NNHIP_REQUIRE(B <= 65535, fn, "B must be at most 65535");
+    return NNHIP_OK;
+}
+
 nnhip_status check_matmul_shape(const char* fn, size_t N, size_t K, size_t M)
 {
     NNHIP_REQUIRE(N <= kMaxDim && M <= kMaxDim, fn, "N and M must be below 2^31");
@@ -2075,14 +2134,8 @@ nnhip_status nnhip_attention_pages_decode(nnhip_ctx* ctx, const nnhip_kv_pages* 
     if (st != NNHIP_OK) return st;
     if (B == 0) return NNHIP_OK;
     NNHIP_REQUIRE(q && k && v && pos && out, fn, "null pointer");
-    NNHIP_REQUIRE(H >= cache->Hkv && H % cache->Hkv == 0 && H <= 65535, fn,
-                  "H must be a multiple of Hkv, at most 65535");
-    NNHIP_REQUIRE(B <= 65535 && B * H < (size_t(1) << 22), fn, "B must be at most 65535, B * H below 2^22");
-    NNHIP_REQUIRE(len_bound >= 1 && len_bound <= cache->table_stride * cache->page_size, fn,
-                  "len_bound must be in [1, table_stride * page_size]");
-    NNHIP_REQUIRE(!rope_cos || len_bound <= rope_len, fn, "len_bound must not exceed the rows of the rope tables");
-    NNHIP_REQUIRE(softcap >= 0.0f && softcap <= 1.0e30f && (softcap == 0.0f || softcap >= 1.0e-30f), fn,
-                  "softcap must be 0 or in [1e-30, 1e30]");
+    st = check_decode(fn, cache, B, H, len_bound, rope_cos, rope_len, softcap);
+    if (st != NNHIP_OK) return st;
     void* ws = nullptr;
     st = ensure_stream_ws(ctx, pages_workspace_bytes(B, H, cache->Hkv, cache->dk, len_bound, (size_t)ctx->num_cus), fn, &ws);
     if (st != NNHIP_OK) return st;
@@ -2103,17 +2156,9 @@ static nnhip_status attention_pages_prefill(nnhip_ctx* ctx, const char* fn, cons
     if (!prefill_dk_supported(cache->dk)) return fail(NNHIP_ERR_UNSUPPORTED, fn, "dk must be 64 or 128");
     if (M == 0 || B == 0) return NNHIP_OK;
     NNHIP_REQUIRE(q && cu && out, fn, "null pointer");
-    NNHIP_REQUIRE(H >= cache->Hkv && H % cache->Hkv == 0 && H <= 65535, fn,
-                  "H must be a multiple of Hkv, at most 65535");
-    NNHIP_REQUIRE(M < (size_t(1) << 29) && H * cache->dk * M < (size_t(1) << 29), fn,
-                  "q / out must be below 2^29 elements");
-    NNHIP_REQUIRE(softcap >= 0.0f && softcap <= 1.0e30f && (softcap == 0.0f || softcap >= 1.0e-30f), fn,
-                  "softcap must be 0 or in [1e-30, 1e30]");
-    NNHIP_REQUIRE(t_bound <= M, fn, "t_bound must not exceed M");
-    size_t limit = cache->table_stride * cache->page_size;
-    if (rope_cos) limit = std::min(limit, rope_len);
-    NNHIP_REQUIRE(!rope_cos || limit * cache->dk < (size_t(1) << 30), fn, "rope tables must be below 2 GiB");
-    NNHIP_REQUIRE(B < (size_t(1) << 22) && B * H < (size_t(1) << 22), fn, "B * H must be below 2^22");
+    size_t limit = 0;
+    st = check_prompts(fn, cache, M, B, t_bound, H, rope_cos, rope_len, softcap, limit);
+    if (st != NNHIP_OK) return st;
     void* ws = nullptr;
     st = ensure_stream_ws(ctx, pages_prefill_workspace_bytes(cache->dk, limit, (size_t)ctx->num_cus), fn, &ws);
     if (st != NNHIP_OK) return st;
@@ -2139,6 +2184,153 @@ nnhip_status nnhip_attention_pages_prefill_distance(nnhip_ctx* ctx, const nnhip_
 {
     return attention_pages_prefill(ctx, "nnhip_attention_pages_prefill_distance", cache, q, M, cu, pos0, B, t_bound, H,
                                    rope_cos, rope_sin, rope_len, scale, softcap, slopes, prefix, true, out);
+}
+
+nnhip_status nnhip_kv_pages_fill_i8(nnhip_ctx* ctx, const nnhip_kv_pages_i8* cache, const float* k, const float* v,
+                                    size_t M, const int32_t* cu, const int32_t* pos0, size_t B, const float* rope_cos,
+                                    const float* rope_sin, size_t rope_len)
+{
+    const char* fn = "nnhip_kv_pages_fill_i8";
+    NNHIP_CHECK_CTX(fn);
+    const nnhip_status st = check_pages(fn, cache, rope_cos, rope_sin);
+    if (st != NNHIP_OK) return st;
+    if (M == 0 || B == 0) return NNHIP_OK;
+    NNHIP_REQUIRE(k && v && cu, fn, "null pointer");
+    NNHIP_REQUIRE(B < kMaxDim && M < kMaxDim - 190, fn, "M or B too large");
+    size_t limit = cache->table_stride * cache->page_size;
+    if (rope_cos) limit = std::min(limit, rope_len);
+    NNHIP_LAUNCH(fn, launch_pages_fill_i8(ctx->stream, *cache, k, v, M, cu, pos0, B, rope_cos, rope_sin, limit));
+    return NNHIP_OK;
+}
+
+nnhip_status nnhip_kv_pages_read_i8(nnhip_ctx* ctx, const nnhip_kv_pages_i8* cache, size_t M, const int32_t* cu,
+                                    const int32_t* pos0, size_t B, float* k, float* v)
+{
+    const char* fn = "nnhip_kv_pages_read_i8";
+    NNHIP_CHECK_CTX(fn);
+    const nnhip_status st = check_pages(fn, cache, nullptr, nullptr);
+    if (st != NNHIP_OK) return st;
+    if (M == 0 || B == 0) return NNHIP_OK;
+    NNHIP_REQUIRE(k && v && cu, fn, "null pointer");
+    NNHIP_REQUIRE(B < kMaxDim && M < kMaxDim - 190, fn, "M or B too large");
+    NNHIP_LAUNCH(fn, launch_pages_read_i8(ctx->stream, *cache, M, cu, pos0, B, k, v));
+    return NNHIP_OK;
+}
+
+nnhip_status nnhip_attention_pages_decode_i8(nnhip_ctx* ctx, const nnhip_kv_pages_i8* cache, const float* q, const float* k,
+                                             const float* v, size_t B, size_t H, const int32_t* pos, size_t len_bound,
+                                             const float* rope_cos, const float* rope_sin, size_t rope_len, float scale,
+                                             float softcap, const float* slopes, int tokens, float* out)
+{
+    const char* fn = "nnhip_attention_pages_decode_i8";
+    NNHIP_CHECK_CTX(fn);
+    nnhip_status st = check_pages(fn, cache, rope_cos, rope_sin);
+    if (st != NNHIP_OK) return st;
+    if (B == 0) return NNHIP_OK;
+    NNHIP_REQUIRE(q && pos && out, fn, "null pointer");
+    NNHIP_REQUIRE((k == nullptr) == (v == nullptr), fn, "k and v go together");
+    st = check_decode(fn, cache, B, H, len_bound, rope_cos, rope_len, softcap);
+    if (st != NNHIP_OK) return st;
+    void* ws = nullptr;
+    st = ensure_stream_ws(ctx, pages_workspace_bytes(B, H, cache->Hkv, cache->dk, len_bound, (size_t)ctx->num_cus), fn, &ws);
+    if (st != NNHIP_OK) return st;
+    NNHIP_LAUNCH(fn, launch_pages_attn_i8(ctx->stream, *cache, q, k, v, B, H, pos, len_bound, rope_cos, rope_sin, scale,
+                                          softcap, slopes, tokens != 0, static_cast<float*>(ws), out, (size_t)ctx->num_cus));
+    return NNHIP_OK;
+}
+
+nnhip_status nnhip_attention_pages_prefill_i8(nnhip_ctx* ctx, const nnhip_kv_pages_i8* cache, const float* q, size_t M,
+                                              const int32_t* cu, const int32_t* pos0, size_t B, size_t t_bound, size_t H,
+                                              const float* rope_cos, const float* rope_sin, size_t rope_len, float scale,
+                                              float softcap, const float* slopes, const int32_t* prefix, int distance,
+                                              float* out)
+{
+    const char* fn = "nnhip_attention_pages_prefill_i8";
+    NNHIP_CHECK_CTX(fn);
+    nnhip_status st = check_pages(fn, cache, rope_cos, rope_sin);
+    if (st != NNHIP_OK) return st;
+    if (!prefill_dk_supported(cache->dk)) return fail(NNHIP_ERR_UNSUPPORTED, fn, "dk must be 64 or 128");
+    if (M == 0 || B == 0) return NNHIP_OK;
+    NNHIP_REQUIRE(q && cu && out, fn, "null pointer");
+    size_t limit = 0;
+    st = check_prompts(fn, cache, M, B, t_bound, H, rope_cos, rope_len, softcap, limit);
+    if (st != NNHIP_OK) return st;
+    void* ws = nullptr;
+    st = ensure_stream_ws(ctx, pages_prefill_workspace_bytes(cache->dk, limit, (size_t)ctx->num_cus), fn, &ws);
+    if (st != NNHIP_OK) return st;
+    NNHIP_LAUNCH(fn, launch_pages_prefill_i8(ctx->stream, *cache, q, M, cu, pos0, B, t_bound, H, rope_cos, rope_sin, limit,
+                                             scale, softcap, slopes, prefix, distance != 0, out, ws, (size_t)ctx->num_cus));
+    return NNHIP_OK;
+}
+
+nnhip_status nnhip_qk_norm_rope(nnhip_ctx* ctx, const float* q, const float* k, size_t M, size_t H, size_t Hkv, size_t dk,
+                                const float* gamma_q, const float* gamma_k, float eps, const int32_t* pos,
+                                const float* rope_cos, const float* rope_sin, size_t rope_len, int tokens, float* q_out,
+                                float* k_out)
+{
+    const char* fn = "nnhip_qk_norm_rope";
+    NNHIP_CHECK_CTX(fn);
+    NNHIP_REQUIRE(dk == 64 || dk == 128 || dk == 256, fn, "dk must be 64, 128 or 256");
+    NNHIP_REQUIRE((q == nullptr) == (q_out == nullptr) && (k == nullptr) == (k_out == nullptr), fn,
+                  "q and q_out go together, and k and k_out");
+    NNHIP_REQUIRE((rope_cos == nullptr) == (rope_sin == nullptr), fn, "rope_cos and rope_sin go together");
+    NNHIP_REQUIRE(!rope_cos || pos, fn, "the rotation needs positions");
+    if (M == 0 || (!q && !k)) return NNHIP_OK;
+    NNHIP_REQUIRE((!q || H >= 1) && (!k || Hkv >= 1) && H <= 65535 && Hkv <= 65535, fn, "H and Hkv must be in [1, 65535]");
+    NNHIP_REQUIRE(M < kMaxDim - 64 && M * (H + Hkv) < kMaxDim, fn, "M * (H + Hkv) must be below 2^31");
+    NNHIP_LAUNCH(fn, launch_qk_norm_rope(ctx->stream, q, k, M, H, Hkv, dk, gamma_q, gamma_k, eps, pos, rope_cos, rope_sin,
+                                         rope_len, tokens != 0, q_out, k_out, (size_t)ctx->num_cus));
+    return NNHIP_OK;
+}
+
+nnhip_status nnhip_pages_assign(nnhip_ctx* ctx, int32_t* table, size_t table_stride, size_t page_size, size_t num_pages,
+                                size_t B, int32_t* free_pages, int32_t* free_count, int32_t* lens, const int32_t* add,
+                                int32_t* cu, int32_t* pos0, size_t M, int32_t* pos, int32_t* slots)
+{
+    const char* fn = "nnhip_pages_assign";
+    NNHIP_CHECK_CTX(fn);
+    if (B == 0) return NNHIP_OK;
+    nnhip_status st = check_table(fn, table, table_stride, page_size, num_pages, B);
+    if (st != NNHIP_OK) return st;
+    NNHIP_REQUIRE(free_pages && free_count && lens && add && cu && pos0, fn, "null pointer");
+    NNHIP_REQUIRE(M < kMaxDim - 256, fn, "M too large");
+    void* ws = nullptr;
+    st = ensure_stream_ws(ctx, tables_workspace_bytes(B), fn, &ws);
+    if (st != NNHIP_OK) return st;
+    NNHIP_LAUNCH(fn, launch_pages_assign(ctx->stream, table, table_stride, page_size, num_pages, B, free_pages, free_count, lens,
+                                         add, cu, pos0, M, pos, slots, ws));
+    return NNHIP_OK;
+}
+
+nnhip_status nnhip_pages_slots(nnhip_ctx* ctx, const int32_t* table, size_t table_stride, size_t page_size, size_t num_pages,
+                               const int32_t* cu, const int32_t* pos0, size_t B, size_t M, int32_t* pos, int32_t* slots)
+{
+    const char* fn = "nnhip_pages_slots";
+    NNHIP_CHECK_CTX(fn);
+    if (B == 0 || M == 0) return NNHIP_OK;
+    const nnhip_status st = check_table(fn, table, table_stride, page_size, num_pages, B);
+    if (st != NNHIP_OK) return st;
+    NNHIP_REQUIRE(cu && (pos || slots), fn, "null pointer");
+    NNHIP_REQUIRE(M < kMaxDim - 256, fn, "M too large");
+    NNHIP_LAUNCH(fn, launch_pages_slots(ctx->stream, table, table_stride, page_size, num_pages, cu, pos0, B, M, pos, slots));
+    return NNHIP_OK;
+}
+
+nnhip_status nnhip_pages_release(nnhip_ctx* ctx, const int32_t* table, size_t table_stride, size_t page_size, size_t num_pages,
+                                 size_t B, int32_t* free_pages, int32_t* free_count, int32_t* lens, const int32_t* keep)
+{
+    const char* fn = "nnhip_pages_release";
+    NNHIP_CHECK_CTX(fn);
+    if (B == 0) return NNHIP_OK;
+    nnhip_status st = check_table(fn, table, table_stride, page_size, num_pages, B);
+    if (st != NNHIP_OK) return st;
+    NNHIP_REQUIRE(free_pages && free_count && lens && keep, fn, "null pointer");
+    void* ws = nullptr;
+    st = ensure_stream_ws(ctx, tables_workspace_bytes(B), fn, &ws);
+    if (st != NNHIP_OK) return st;
+    NNHIP_LAUNCH(fn, launch_pages_release(ctx->stream, table, table_stride, page_size, num_pages, B, free_pages, free_count,
+                                          lens, keep, ws));
+    return NNHIP_OK;
 }
 
 size_t nnhip_logits_workspace_bytes(nnhip_ctx* ctx, size_t V, size_t B)
