@@ -24,8 +24,12 @@ last token.
 With paged caches (Decoder(caches=[KVPages, ...]), one per block, which may share a page table) the
 sequences of a batch start, end and grow apart: Decoder.prefill_packed takes prompts of unlike lengths
 packed one behind another (nnhip_kv_pages_fill, nnhip_attention_pages_prefill), and step() runs
-nnhip_attention_pages_decode, for which a position below 0 marks an empty slot. The choice of the next
+nnhip_attention_pages_decode, for which a position below 0 marks an empty slot. The caches may be KVPagesI8 (8 bits) as
+well, and their table one that Context.pages_assign keeps. The choice of the next
 token can go through rules (step(rules=LogitRules), nnhip_logits_adjust_rows).
+
+A block with gains g_q, g_k normalizes the heads of its queries and keys before their rotation (nnhip_qk_norm_rope, in every
+path; its attention and its cache then take them as they are).
 """
 from __future__ import annotations
 
@@ -56,6 +60,8 @@ class Block:
     fc2: Linear
     g_attn_sub: Optional[object] = None
     g_ffn_sub: Optional[object] = None
+    g_q: Optional[object] = None   # (dk): RMSNorm of every head of the queries, and of the keys, before the rotation
+    g_k: Optional[object] = None
 
 
 @dataclass
@@ -114,7 +120,7 @@ class Decoder:
             caches = [(torch.zeros((B, cfg.max_len, Hkv * dk), **cdt), torch.zeros((B, cfg.max_len, Hkv * dk), **cdt))
                       for _ in blocks]
         self.caches = caches
-        self.paged = bool(caches) and isinstance(caches[0], _pkg().KVPages)
+        self.paged = bool(caches) and isinstance(caches[0], (_pkg().KVPages, _pkg().KVPagesI8))
         if cfg.rope:
             c, s = _pkg().rope_table(dk, cfg.max_len)
             self.cos, self.sin = torch.from_numpy(c).to(dev), torch.from_numpy(s).to(dev)
@@ -195,7 +201,7 @@ class Decoder:
             d, Hdk, kv, f32 = cfg.d, cfg.H * cfg.dk, cfg.Hkv * cfg.dk, torch.float32
             self._pf_flat = {name: torch.empty((n * M,), dtype=dt, device=f"cuda:{self.ctx.device}") for name, n, dt in (
                 ("x", d, f32), ("r", d, f32), ("q", Hdk, f32), ("k", kv, f32), ("v", kv, f32), ("a", Hdk, f32),
-                ("s", 1, f32), ("rs", 1, torch.int32), ("xi", _pkg().kp(max(d, Hdk)), torch.int8))}
+                ("s", 1, f32), ("rs", 1, torch.int32), ("pos", 1, torch.int32), ("xi", _pkg().kp(max(d, Hdk)), torch.int8))}
             self._pf_room = M
         if torch.cuda.is_current_stream_capturing():
             self._pf_captured = True
@@ -219,14 +225,35 @@ class Decoder:
         M = B * T
         pf = self._prefill_buffers(M)
 
+        if self._normed and cfg.rope:
+            import torch
+            torch.arange(pos0, pos0 + T, dtype=torch.int32, device=pf["pos"].device, out=pf["pos"][:T])
+            pf["pos"].view(B, T)[1:] = pf["pos"][:T]
+
         def attend(i):
             kc, vc = self.caches[i]
-            ctx.kv_cache_fill(pf["k"], pf["v"], B, T, cfg.Hkv, cfg.dk, pos0, kc, vc, self.cos, self.sin)
-            ctx.attention_prefill(pf["q"], kc, vc, B, T, cfg.H, cfg.Hkv, cfg.dk, pos0, cfg.scale, self.cos, self.sin,
-                                  out=pf["a"])
+            cos, sin = self._qk_norm(i, pf["q"], pf["k"], pf["pos"])
+            ctx.kv_cache_fill(pf["k"], pf["v"], B, T, cfg.Hkv, cfg.dk, pos0, kc, vc, cos, sin)
+            ctx.attention_prefill(pf["q"], kc, vc, B, T, cfg.H, cfg.Hkv, cfg.dk, pos0, cfg.scale, cos, sin, out=pf["a"])
 
         ctx.copy_columns(self._prefill_blocks(ids, M, attend, hook), T - 1, T, B, out=self.x)
         return self._prefill_head(rules)
+
+    @property
+    def _normed(self) -> bool:
+        return any(blk.g_q is not None or blk.g_k is not None for blk in self.blocks)
+
+    def _qk_norm(self, i: int, q, k, pos, tokens: bool = False):
+        """Block i's norms of queries and keys, with their rotation at pos, in place where the block has gains. Returns the
+        tables that its cache and attention still rotate with."""
+        blk, cfg = self.blocks[i], self.cfg
+        if blk.g_q is None and blk.g_k is None:
+            return self.cos, self.sin
+        if blk.g_q is None or blk.g_k is None:
+            raise _pkg().NNHipError(1, "g_q and g_k go together")
+        self.ctx.qk_norm_rope(q, k, cfg.dk, cfg.eps, blk.g_q, blk.g_k, pos=pos if cfg.rope else None, cos=self.cos,
+                              sin=self.sin, q_out=q, k_out=k, tokens=tokens)
+        return None, None
 
     def _prefill_blocks(self, ids, M: int, attend, hook):
         """Every block over the M tokens ids; attend(i) turns block i's q, k, v into its attention output."""
@@ -294,12 +321,17 @@ class Decoder:
             raise _pkg().NNHipError(1, "prefill_packed needs a token")
         pf = self._prefill_buffers(ids.shape[0])
         t_bound = min(t_bound, ids.shape[0])
+        if self._normed and cfg.rope:
+            # (a token without a place keeps its query and key as they are; nothing is written for it)
+            first = self.caches[0]
+            ctx.pages_slots(first.table, first.page_size, first.num_pages, cu, pos0, pos=pf["pos"])
 
         def attend(i):
             cache = self.caches[i]
-            ctx.kv_pages_fill(cache, pf["k"], pf["v"], cu, pos0=pos0, cos=self.cos, sin=self.sin)
-            ctx.attention_pages_prefill(cache, pf["q"], cu, t_bound, cfg.H, cfg.scale, pos0=pos0, cos=self.cos,
-                                        sin=self.sin, out=pf["a"])
+            cos, sin = self._qk_norm(i, pf["q"], pf["k"], pf["pos"])
+            ctx.kv_pages_fill(cache, pf["k"], pf["v"], cu, pos0=pos0, cos=cos, sin=sin)
+            ctx.attention_pages_prefill(cache, pf["q"], cu, t_bound, cfg.H, cfg.scale, pos0=pos0, cos=cos, sin=sin,
+                                        out=pf["a"])
 
         x = self._prefill_blocks(ids, ids.shape[0], attend, hook)
         # (an empty first sequence, or offsets past the tokens, would be an index outside x)
@@ -326,12 +358,15 @@ class Decoder:
     def _attend(self, i: int, q, k, v, pos, len_bound: int, out, tokens: bool = False):
         """Block i's attention of the step's tokens over its cache."""
         cfg, cache = self.cfg, self.caches[i]
+        cos, sin = self._qk_norm(i, q, k, pos, tokens)
+        if self.cos is not None and len_bound > self.cos.shape[0]:
+            raise _pkg().NNHipError(1, "len_bound must not exceed the rows of the rope tables")
         if self.paged:
-            self.ctx.attention_pages_decode(cache, q, k, v, cfg.H, pos, len_bound, cfg.scale, cos=self.cos, sin=self.sin,
+            self.ctx.attention_pages_decode(cache, q, k, v, cfg.H, pos, len_bound, cfg.scale, cos=cos, sin=sin,
                                             out=out, tokens=tokens)
         else:
             self.ctx.attention_decode(q, k, v, cfg.H, cfg.Hkv, cfg.dk, pos, len_bound, cache[0], cache[1], cfg.scale,
-                                      self.cos, self.sin, out=out, tokens=tokens)
+                                      cos, sin, out=out, tokens=tokens)
 
     def _quant(self, x, gamma):
         outs = (self.xi, self.s, self.rs)

@@ -516,3 +516,127 @@ def test_prompt_bad_sequences(ctx, nnhip):
     out = dev(np.full((H * dk, M), 7.0, F32))
     ctx.attention_pages_prefill(c.on_device(nnhip), q, dev(np.array([0, 40, 80], np.int32)), 40, H, 0.125, out=out)
     assert np.all(host(out)[:, 80:] == 7.0) and np.array_equal(host(out)[:, :40], ref[:, :40])
+
+
+@pytest.mark.parametrize("decode", [True, False])
+def test_error_in_norm(ctx, nnhip, decode):
+    """Outputs for normal inputs against 64 bits, in norm. A score of about 1 is off by its sum's roundings (dk = 128 products
+    of values about 1 over sqrt(dk): under 2 u), its scaling and the exponential by 4 u, its weight's parts by 1 u; sums of n
+    weighted values by 0.5 u sqrt(steps) of independent roundings, a step for 8 positions: 8 u + sqrt(n / 8) u / 2 with a margin of 2."""
+    import torch
+    rng = np.random.default_rng(70)
+    n, H, Hkv, dk, page = 3000, 8, 2, 128, 64
+    c = CacheI8(rng, [n], Hkv, page, dk, 32)
+    c.put(0, 0, rng.standard_normal((n, Hkv, dk)).astype(F32), rng.standard_normal((n, Hkv, dk)).astype(F32))
+    T = 1 if decode else 64
+    q = rng.standard_normal((T, H, dk)).astype(F32)
+    scale = float(F32(1 / math.sqrt(dk)))
+    cache = c.on_device(nnhip)
+    if decode:
+        out = host(ctx.attention_pages_decode(cache, dev(columns(q)), None, None, H, dev(np.array([n - 1], np.int32)), n, scale))
+    else:
+        out = host(ctx.attention_pages_prefill(cache, dev(columns(q)), dev(np.array([0, T], np.int32)), T, H, scale,
+                                               pos0=dev(np.array([n - T], np.int32))))
+    out = out.T.reshape(T, H, dk).astype(np.float64)
+    K, V = c.rows(0, n)
+    err = norm = 0.0
+    for t in range(T):
+        m = n - T + t + 1
+        for h in range(H):
+            x = K[:m, h // 4] @ q[t, h].astype(np.float64) * scale
+            p = np.exp(x - x.max())
+            want = p @ V[:m, h // 4] / p.sum()
+            err += float(np.sum((out[t, h] - want) ** 2))
+            norm += float(np.sum(want ** 2))
+    rel = math.sqrt(err / norm)
+    print(f"  {rel / U:.2f} u", flush=True)
+    assert rel <= (8 + 0.5 * math.sqrt(n / 8)) * U * 2
+
+
+def test_captured_and_streams(nnhip):
+    """Fill, decode and prompt captured on a stream of their own and replayed between eager calls of other sizes, the lengths
+    changing on the device: each replay gives what eager calls give, in both pools and outputs."""
+    import torch
+    ctx = nnhip.Context(0)
+    rng = np.random.default_rng(71)
+    H, Hkv, dk, page = 8, 2, 64, 16
+    lens = [700, 500]
+    c = CacheI8(rng, lens, Hkv, page, dk, 16)
+    for b, n in enumerate(lens):
+        c.put(b, 0, tokens_of(rng, n, Hkv, dk), tokens_of(rng, n, Hkv, dk))
+    state = [dev(rng.standard_normal(s).astype(F32)) for s in ((H * dk, 2), (Hkv * dk, 2), (Hkv * dk, 2), (H * dk, 90),
+                                                               (Hkv * dk, 90), (Hkv * dk, 90))]
+    side = torch.cuda.Stream()
+    found = []
+    for captured in (False, True):
+        cache = c.on_device(nnhip)
+        pos, cu, pos0 = dev(np.array([99, 300], np.int32)), dev(np.array([0, 40, 90], np.int32)), dev(np.array([100, 301], np.int32))
+        out, prompt = torch.zeros(H * dk, 2, device="cuda"), torch.zeros(H * dk, 90, device="cuda")
+
+        def call():
+            ctx.attention_pages_decode(cache, state[0], state[1], state[2], H, pos, 700, 0.125, out=out)
+            ctx.kv_pages_fill(cache, state[4], state[5], cu, pos0=pos0)
+            ctx.attention_pages_prefill(cache, state[3], cu, 90, H, 0.125, pos0=pos0, out=prompt)
+
+        with torch.cuda.stream(side):
+            call()
+        torch.cuda.synchronize()
+        trace = []
+        if captured:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                call()
+        for p, split, p0 in (([150, 360], 50, [151, 361]), ([5, -1], 0, [6, 0]), ([600, 400], 90, [601, 2]), ([250, 77], 17, [251, 78])):
+            pos.copy_(dev(np.array(p, np.int32)))
+            cu.copy_(dev(np.array([0, split, 90], np.int32)))
+            pos0.copy_(dev(np.array(p0, np.int32)))
+            torch.cuda.synchronize()
+            if captured:
+                g.replay()
+            else:
+                with torch.cuda.stream(side):
+                    call()
+            torch.cuda.synchronize()
+            ctx.attention_pages_decode(c.on_device(nnhip), state[0], None, None, H, dev(np.array([40, 20], np.int32)), 41, 0.1)
+            trace += [host(x).copy() for x in (out, prompt, cache.k, cache.v, cache.k_scale, cache.v_scale)]
+        found.append(trace)
+    for a, b in zip(*found):
+        assert np.array_equal(a, b, equal_nan=a.dtype.kind == "f")
+    ctx.close()
+
+
+def test_refusals(ctx, nnhip):
+    t = dev(np.zeros((2, 4), np.int32))
+    cache = nnhip.KVPagesI8.empty(4, 2, 16, 64, 16, t)
+    q, k = dev(np.zeros((256, 2), F32)), dev(np.zeros((128, 2), F32))
+    cu, pos = dev(np.array([0, 1, 2], np.int32)), dev(np.zeros(2, np.int32))
+    with pytest.raises(nnhip.NNHipError, match="k and v"):
+        ctx.attention_pages_decode(cache, q, k, None, 4, pos, 8, 0.1)
+    with pytest.raises(nnhip.NNHipError, match="len_bound"):
+        ctx.attention_pages_decode(cache, q, k, k, 4, pos, 65, 0.1)
+    with pytest.raises(nnhip.NNHipError, match="multiple of Hkv"):
+        ctx.attention_pages_decode(cache, dev(np.zeros((192, 2), F32)), k, k, 3, pos, 8, 0.1)
+    with pytest.raises(nnhip.NNHipError, match="softcap"):
+        ctx.attention_pages_prefill(cache, q, cu, 1, 4, 0.1, softcap=-1.0)
+    with pytest.raises(nnhip.NNHipError, match="t_bound"):
+        ctx.attention_pages_prefill(cache, q, cu, 3, 4, 0.1)
+    with pytest.raises(nnhip.NNHipError, match="dtype"):
+        ctx.kv_pages_fill(cache, k.half(), k, cu)
+    with pytest.raises(nnhip.NNHipError, match="shape"):
+        ctx.kv_pages_read(cache, cu, 5, k=k)
+    with pytest.raises(nnhip.NNHipError, match="KVPagesI8"):
+        pool = dev(np.zeros((4, 2, 16, 64), F32))
+        ctx.kv_pages_read(nnhip.KVPages(pool, pool.clone(), t), cu, 2)
+    with pytest.raises(nnhip.NNHipError, match="null"):
+        pool = dev(np.zeros((4, 2, 16, 64), F32))
+        ctx.attention_pages_decode(nnhip.KVPages(pool, pool.clone(), t), q, None, None, 4, pos, 8, 0.1)
+    wide = nnhip.KVPagesI8.empty(4, 1, 32, 256, 16, t)
+    with pytest.raises(nnhip.NNHipError, match="64 or 128"):
+        ctx.attention_pages_prefill(wide, dev(np.zeros((256, 2), F32)), cu, 1, 1, 0.1)
+    for page, dk, block, what in ((128, 64, 128, "block"), (16, 48, 16, "dk must be"), (48, 64, 16, "power of two"), (2048, 64, 16, "power of two")):
+        odd = nnhip.KVPagesI8.empty(2, 1, page, dk, block, t)
+        with pytest.raises(nnhip.NNHipError, match=what):
+            ctx.kv_pages_fill(odd, dev(np.zeros((dk, 2), F32)), dev(np.zeros((dk, 2), F32)), cu)
+    # nothing to do
+    ctx.kv_pages_fill(cache, dev(np.zeros((128, 0), F32)), dev(np.zeros((128, 0), F32)), dev(np.zeros(3, np.int32)))
+    assert ctx.kv_pages_read(cache, dev(np.zeros(1, np.int32)), 2)[0].shape == (128, 2)
