@@ -8,10 +8,11 @@
 //   S^T = K . Q^T  with each query in two f16 parts, q 2^e = hi + lo to 2^-23 of it (and 2^-40 of the query's
 //                  largest): two v_mfma_f32_32x32x16_f16 a step, whose products are exact; a key's scale is a factor of
 //                  the 16 scores that share it, folded into the exponential's argument with the softmax scale;
-//   O^T += V^T . P^T  with the weights in two f16 parts, 2^6 .. 2^15 at their largest, the scale of the values folded into the
-//                  weights by its logarithm in the same argument. Parts hold 22 bits of every weight down to 2^-24 of the largest and
-//                  2^-40 of the largest below. So that no scale costs bits, O is kept in units of a power of two within
-//                  2^-6 .. 2 of the group's scale: where a group's leaves that range, O moves to another unit first.
+//   O^T += V^T . P^T  with the weights in two f16 parts, 2^6 .. 2^15 at their largest: 22 bits of every weight down to 2^-24
+//                  of the largest, and 2^-40 of the largest below. Of the scale of 16 values 2^k, a power of two, goes into their
+//                  codes as they are widened, the rest, in 1 .. 2, into the weights by its logarithm in the same argument. O is in
+//                  units of a power of two that the largest scale of a tile stays within 2^+-5 of: where it leaves that range,
+//                  O moves to another unit first. Groups 2^-14 or more below it are summed apart. So no scale costs the weights bits.
 // O^T stays in the accumulators over all tiles; a query's reference maximum moves when its maximum has grown by
 // 2^8, by a whole power of two. Sums and softmax are f32. The next tile is converted by half of the waves before their
 // products and by the other half behind them, so that every SIMD has one of each.
@@ -37,7 +38,8 @@ struct ScalesI8
 
 constexpr int kI8Keys = 64;      // keys of a tile, two halves of kPK
 constexpr float kI8Up = 6.0f;    // log2 of the largest weight when a reference maximum is new
-constexpr int kI8Low = 6;        // a group's scale of values is at most this many powers of two below O's unit
+constexpr int kI8Near = 5;       // the largest scale of a tile's values is within 2^+-5 of O's unit
+constexpr int kI8Low = -14;      // the least power of two that codes are multiplied by: they stay normal f16 values
 
 template <int DK>
 struct TileI8
@@ -48,12 +50,19 @@ struct TileI8
     static constexpr int kTPitch = DK * 2 + 16;  // rows of the cos / sin tables, before the first tile
     static constexpr int kTables = 2 * 32 * kPWaves * kTPitch;
     static constexpr int kMain = 2 * kBuf > kTables ? 2 * kBuf : kTables;
-    static constexpr int kScales = kMain;          // [2][2][4]: per buffer, of keys and of values
-    static constexpr int kFound = kMain + 64;      // [8]
-    static constexpr int kBytes = kMain + 96;
+    static constexpr int kScales = kMain;          // [4][2][4]: of four tiles' keys and values
+    static constexpr int kFound = kMain + 128;     // [8]
+    static constexpr int kBytes = kMain + 160;
 };
 
-// Four codes as f16: 1024 + 128 + code is the byte code + 128 under the exponent of 1024
+// Four codes times 2^k as f16, f = 2^k, off = -1152 2^k: the byte code + 128 under the exponent of 1024 is 1152 + code
+__device__ __forceinline__ u32x2 widen_codes(uint32_t x, v2h f, v2h off)
+{
+    const uint32_t u = x ^ 0x80808080u;
+    const v2h a = __builtin_elementwise_fma(__builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)), f, off);
+    const v2h b = __builtin_elementwise_fma(__builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)), f, off);
+    return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+}
 __device__ __forceinline__ u32x2 widen_codes(uint32_t x)
 {
     const uint32_t u = x ^ 0x80808080u;
@@ -62,6 +71,12 @@ __device__ __forceinline__ u32x2 widen_codes(uint32_t x)
     const v2h b = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + off;
     return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
 }
+
+// The exponent field of a scale that counts, or 0: zeros, and what is not finite
+__device__ __forceinline__ int scale_field(uint32_t bits) { return (bits >> 23) == 255 ? 0 : (int)(bits >> 23); }
+
+// The power of two that goes into the codes of a group whose scale has that field, where O's unit is `unit`
+__device__ __forceinline__ int code_power(int field, int unit) { return field == 0 ? 0 : min(max(field - unit, kI8Low), kI8Near); }
 
 // Attention of an item over its tiles of 32 keys k0 .. k1 - 1; rec: into a record instead of the output
 template <int DK, bool kShaped>
@@ -95,7 +110,6 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
     auto at_group = [&](int kb) { return min(kb * kPK + 16 * group, end_key & ~15); };
     auto load_id = [&](int kb) { id = a.table[(size_t)w.b * a.table_stride + (at_group(kb) >> a.shift)]; };
     u32x4 raw_k, raw_v;
-    float raw_s[2];
     auto load_raw = [&](int kb) {
         const int page = __builtin_amdgcn_readfirstlane(id);
         const bool in = page_ok(page, a.num_pages);
@@ -104,12 +118,34 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
         const size_t off = (row >> 4) * (size_t)(16 * DK) + (size_t)(16 * piece);
         if (has_k) raw_k = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(a.kc) + off);
         if (has_v) raw_v = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(a.vc) + off);
-        const bool there = kb * kPK + 16 * group <= end_key;  // (behind the last key: whatever is there)
-        raw_s[0] = there ? sc.k[row >> sc.bshift] : 0.0f;
-        raw_s[1] = there ? sc.v[row >> sc.bshift] : 0.0f;
         if (kb + 2 < k1) load_id(kb + 2);
     };
-    auto convert = [&](int par) {
+    // scales: the first four waves read those of a group each, a tile before its codes are widened
+    auto at_scale = [&](int kb) { return min(kb * kPK + 16 * wave, end_key & ~15); };
+    auto scale_id = [&](int kb) { return a.table[(size_t)w.b * a.table_stride + (at_scale(kb) >> a.shift)]; };
+    auto load_scales = [&](int kb, int id, float(&s)[2]) {
+        const int page = __builtin_amdgcn_readfirstlane(id);
+        const size_t row = page_row(page_ok(page, a.num_pages) ? page : 0, w.g, at_scale(kb) & ((1 << a.shift) - 1), a.Hkv, a.shift);
+        const bool there = kb * kPK + 16 * wave <= end_key;  // (behind the last key: whatever is there)
+        s[0] = there ? sc.k[row >> sc.bshift] : 0.0f;
+        s[1] = there ? sc.v[row >> sc.bshift] : 0.0f;
+    };
+    auto slot_of = [&](int kb) { return scales + ((kb - k0) >> 1 & 3) * 8; };
+    auto post_scales = [&](int kb, const float(&s)[2]) {
+        if (lane < 2) slot_of(kb)[4 * lane + wave] = lane ? s[1] : s[0];
+    };
+    // the unit of O for a tile whose scales are posted, where it was `unit` before and `top` at most so far: no more than
+    // 2^80 below that, so that O stays finite
+    auto next_unit = [&](int kb, int unit, int& top) {
+        int field = 0;
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+            field = max(field, scale_field((uint32_t)__builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, slot_of(kb)[4 + n]))));
+        if (field == 0) return unit;
+        top = max(top, field);
+        return field > unit + kI8Near || field < unit - kI8Near ? max(field, top - 80) : unit;
+    };
+    auto convert = [&](int kb, int par, int unit) {
         uint8_t* const buf = smem + par * Tile::kBuf;
         if (has_k)
         {
@@ -122,12 +158,16 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
         if (has_v)
         {
             // 16 positions of dimension `piece`, as S^T's accumulators hold them: 0..3 and 8..11, then 4..7 and 12..15
+            const uint32_t bits = (uint32_t)__builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, slot_of(kb)[4 + group]));
+            const int field = scale_field(bits);  // (0: values below 2^-119, or NaN, which their weights are then)
+            const _Float16 to = field == 0 ? (_Float16)0.0f : (_Float16)pow2(code_power(field, unit)), down = (_Float16)-1152.0f * to;
+            const v2h f = {to, to}, off = {down, down};
             uint8_t* const dst = buf + Tile::kV + piece * Tile::kVPitch + 32 * group;
-            const u32x2 x = widen_codes(raw_v[0]), y = widen_codes(raw_v[1]), z = widen_codes(raw_v[2]), t = widen_codes(raw_v[3]);
+            const u32x2 x = widen_codes(raw_v[0], f, off), y = widen_codes(raw_v[1], f, off), z = widen_codes(raw_v[2], f, off),
+                        t = widen_codes(raw_v[3], f, off);
             *reinterpret_cast<u32x4*>(dst) = u32x4{x[0], x[1], z[0], z[1]};
             *reinterpret_cast<u32x4*>(dst + 16) = u32x4{y[0], y[1], t[0], t[1]};
         }
-        if (lane < 2) scales[par * 8 + 4 * lane + group] = lane ? raw_s[1] : raw_s[0];
     };
 
     // ---- everything that the first tile waits for on its way together: rows of the cos / sin tables, page ids,
@@ -148,6 +188,7 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
             }
     }
     load_id(k0);
+    int sid = wave < 4 ? scale_id(k0) : 0, sid2 = wave < 4 && k0 + 2 < k1 ? scale_id(k0 + 2) : 0;
     PrefillQuery<DK, 8> query;
     if (w.live) query.load(a, w, seq, h);
     if (a.cosT)
@@ -164,6 +205,13 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
     }
     __syncthreads();
     load_raw(k0);
+    float s_now[2], s_next[2];
+    if (wave < 4)
+    {
+        load_scales(k0, sid, s_now);
+        if (k0 + 2 < k1) load_scales(k0 + 2, sid2, s_next);
+        if (k0 + 4 < k1) sid = scale_id(k0 + 4);
+    }
 
     // ---- the lane's rotated query in halves: step c holds dimensions 16c + 8h + 0..7, scaled by 2^eq
     v8h qh[NC], ql[NC];
@@ -199,24 +247,36 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = v16f{};
     float m_ref = -__builtin_inff(), l_run = 0.0f;  // log2 units; l_run: this lane half's keys
-    int unit = 127;                                 // O is in units of 2^(unit - 127)
     const float slope2 = kShaped && a.slopes ? a.slopes[w.head] * 1.44269504f : 0.0f;
-    __syncthreads();  // the tables have been read
-    convert(0);
+    if (wave < 4)
+    {
+        post_scales(k0, s_now);
+        if (k0 + 2 < k1) post_scales(k0 + 2, s_next);
+    }
+    __syncthreads();  // the tables have been read; the first two tiles' scales are there
+    int unit_top = 0, unit = next_unit(k0, 127, unit_top);  // O is in units of 2^(unit - 127)
+    convert(k0, 0, unit);
     if (k0 + 2 < k1) load_raw(k0 + 2);
     const uint32_t k_at = (uint32_t)(l32 * Tile::kKPitch + 16 * h), v_at = (uint32_t)(Tile::kV + l32 * Tile::kVPitch + 16 * h);
     int par = 0;
+    float by = 1.0f;  // from the last tile's unit to this one's
     for (int kb = k0; kb < k1; kb += 2, par ^= 1)
     {
         __syncthreads();  // tile kb is in LDS; the other buffer is free
         const bool more = kb + 2 < k1;
+        const int unit_next = more ? next_unit(kb + 2, unit, unit_top) : unit;
         if (more && wave < 4)
         {
-            convert(par ^ 1);
-            if (kb + 4 < k1) load_raw(kb + 4);  // in flight during this tile's products
+            convert(kb + 2, par ^ 1, unit_next);
+            if (kb + 4 < k1)
+            {
+                load_raw(kb + 4);  // in flight during this tile's products
+                load_scales(kb + 4, sid, s_next);
+                if (kb + 6 < k1) sid = scale_id(kb + 6);
+            }
         }
         const uint8_t* const buf = smem + par * Tile::kBuf;
-        const float* const ts4 = scales + par * 8;
+        const float* const ts4 = slot_of(kb);
 #pragma unroll 1
         for (int half = 0; half < 2; ++half)
         {
@@ -240,6 +300,8 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
             const bool masked = key0 + kPK - 1 > seq.from(a, w);
             if (kShaped || masked)
             {
+                // (an opaque factor: or the products are computed whether the branch is taken or not)
+                if constexpr (!kShaped) asm volatile("" : "+v"(kf[0]), "+v"(kf[1]));
 #pragma unroll
                 for (int v = 0; v < 16; ++v) s[v] *= kf[v >> 3];
                 kf[0] = kf[1] = 1.0f;
@@ -295,11 +357,14 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
             const float mx = __builtin_ceilf(max_halves(fmaxf(top[0], top[1])));
             // the reference of a query moves only when its maximum has grown by 2^8 (or is new)
             const bool grown = mx > m_ref + kPLazy;
-            if (__builtin_amdgcn_ballot_w64(grown) != 0)
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(grown) != 0 || by != 1.0f, 0))
             {
                 const float m_new = grown ? mx : m_ref;
-                const float corr = grown ? __builtin_amdgcn_exp2f(m_ref - m_new) : 1.0f;
+                float corr = grown ? __builtin_amdgcn_exp2f(m_ref - m_new) : 1.0f;
+                asm volatile("" : "+v"(corr));
                 l_run *= corr;
+                corr *= by;
+                by = 1.0f;
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -310,28 +375,13 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
 #pragma unroll
             for (int t = 0; t < 2; ++t)
             {
-                // the scale of the group's values in O's units
+                // what the codes have not got of their scale (0 and what is not finite: nothing)
                 const uint32_t bits = __builtin_bit_cast(uint32_t, vs[t]);
-                const int e = (int)(bits >> 23);
-                float lv = 0.0f;  // (a scale of 0: all codes are 0)
-                if (e == 255)
-                {
-                    if (key0 + 16 * t <= seq.sight(w)) l_run = __builtin_nanf("");
-                }
-                else if (bits != 0)
-                {
-                    if (e > unit || e < unit - kI8Low)
-                    {
-                        const float by = __builtin_ldexpf(1.0f, unit - e);
-#pragma unroll
-                        for (int d = 0; d < ND; ++d)
-#pragma unroll
-                            for (int v = 0; v < 16; ++v) o[d][v] *= by;
-                        unit = e;
-                    }
-                    lv = e < 64 ? __builtin_amdgcn_logf(vs[t] * 0x1p64f) - (float)(unit - 127 + 64) : __builtin_amdgcn_logf(vs[t]) - (float)(unit - 127);
-                }
-                const float off = base + lv;
+                const int e = scale_field(bits);
+                const int power = code_power(e, unit), left = e == 0 ? 0 : e - unit - power;
+                const float lv = e == 0 ? 0.0f : __builtin_amdgcn_logf(vs[t]) - (float)(e - 127);
+                if (__builtin_expect((bits >> 23) == 255, 0) && key0 + 16 * t <= seq.sight(w)) l_run = __builtin_nanf("");
+                const float off = left == 0 ? base + lv : -__builtin_inff();
                 float sum = 0.0f;
                 v8h pa, pb;
 #pragma unroll
@@ -354,12 +404,48 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pb, o[d], 0, 0, 0);
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pa, o[d], 0, 0, 0);
                 }
+                if (__builtin_expect(left != 0, 0))
+                {
+                    // a group whose scale is far below the largest of its tile, which some queries may not see: its
+                    // weights in full, its sums times the power of two that is left
+                    float rest = __builtin_ldexpf(1.0f, left);
+                    asm volatile("" : "+v"(rest));
+                    sum = 0.0f;
+#pragma unroll
+                    for (int v = 0; v < 8; v += 2)
+                    {
+                        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * t + v], kf[t], base + lv));
+                        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * t + v + 1], kf[t], base + lv));
+                        sum += p0;
+                        sum += p1;
+                        v2h x, y;
+                        split2(p0, p1, x, y);
+                        pa[v] = x[0], pa[v + 1] = x[1];
+                        pb[v] = y[0], pb[v + 1] = y[1];
+                    }
+                    l_run = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-lv), l_run);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+                    {
+                        const v8h x = *reinterpret_cast<const v8h*>(buf + v_at + 32 * d * Tile::kVPitch + 32 * (2 * half + t));
+                        v16f y = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pb, v16f{}, 0, 0, 0);
+                        y = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pa, y, 0, 0, 0);
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) o[d][v] = __builtin_fmaf(y[v], rest, o[d][v]);
+                    }
+                }
             }
         }
         if (more && wave >= 4)
         {
-            convert(par ^ 1);
+            convert(kb + 2, par ^ 1, unit_next);
             if (kb + 4 < k1) load_raw(kb + 4);
+        }
+        if (more)
+        {
+            by *= __builtin_ldexpf(1.0f, unit - unit_next);
+            unit = unit_next;
+            if (wave < 4 && kb + 4 < k1) post_scales(kb + 4, s_next);
         }
     }
     l_run += __shfl_xor(l_run, 32);
@@ -370,7 +456,8 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
 #pragma unroll
     for (int i = 0; i < kPWaves; ++i) found |= found_s[i];
     if (found) l_run = __builtin_nanf("");
-    const float by = __builtin_ldexpf(1.0f, unit - 127);
+    // (a unit that no tile of the wave's has taken up yet is still to come off)
+    by = __builtin_ldexpf(by, unit - 127);
     auto dim = [](int d, int i) { return 32 * d + i; };
     if (rec)
     {
