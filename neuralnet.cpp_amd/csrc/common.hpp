@@ -451,7 +451,7 @@ hipError_t launch_pages_fill_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, con
                                 const int32_t* cu, const int32_t* pos0, size_t B, const float* cosT, const float* sinT,
                                 size_t limit);
 hipError_t launch_pages_read_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, size_t M, const int32_t* cu, const int32_t* pos0,
-                                size_t B, float* k, float* v);
+                                size_t B, float* k, float* v, size_t num_cus);
 hipError_t launch_pages_prefill_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, const float* q, size_t M, const int32_t* cu,
                                    const int32_t* pos0, size_t B, size_t t_bound, size_t H, const float* cosT,
                                    const float* sinT, size_t limit, float scale, float softcap, const float* slopes,

@@ -16,6 +16,7 @@
 #include "token_quant.hpp"
 
 #include <cmath>
+#include <type_traits>
 
 namespace nnhip
 {
@@ -36,40 +37,70 @@ typedef int32_t v4i __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v4fu __attribute__((ext_vector_type(4), aligned(4)));
 
-// The old codes of a block again under a larger scale: positions 0 .. n - 1 of the block that begins at row `row`,
-// piece (16 bytes) `at` of every `step`. Of values, only the bytes of those positions are written.
-__device__ __forceinline__ void requantize(int8_t* pool, size_t row, int n, int dk, bool keys, float s_old, float s_new,
-                                           int at, int step)
+// Order between a wave's own LDS accesses of different lanes
+__device__ __forceinline__ void wave_lds_fence()
 {
-    u32x4* const pieces = reinterpret_cast<u32x4*>(pool + (row >> 4) * (size_t)(16 * dk));
-    const int groups = (n + 15) >> 4;
-    for (int i = at; i < groups * dk; i += step)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// A block whose scale has grown: its first row, the positions that it had, and both scales
+struct Regrown
+{
+    int row, n;
+    float before, after;
+};
+
+// The older codes of `count` blocks of `groups` 16s of positions again under their larger scales, of(i) the i-th: thread
+// `at` of `step`, four 16-byte pieces on their way together. Of values, only the bytes of those positions are written.
+template <typename Of>
+__device__ __forceinline__ void requantize(int8_t* pool, int count, int groups, int dk, bool keys, int at, int step, Of&& of)
+{
+    constexpr int U = 4;
+    const int per = groups * dk;
+    for (int i0 = at; i0 < count * per; i0 += U * step)
     {
-        const int first = i / dk * 16;  // position of the piece's group
-        const int live = keys ? (first + (i & 15) < n ? 16 : 0) : min(16, n - first);
-        if (live == 0) continue;
-        u32x4 x = pieces[i];
+        u32x4 x[U];
+        int live[U];
+        u32x4* to[U];
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int u = 0; u < U; ++u)
         {
-            uint32_t y = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-            {
-                const int c = (int8_t)(x[w] >> (8 * e));
-                y |= (uint32_t)(uint8_t)quantize_one(__fmul_rn((float)c, s_old), s_new) << (8 * e);
-            }
-            x[w] = y;
+            const int i = i0 + u * step;
+            live[u] = 0;
+            if (i >= count * per) continue;
+            const Regrown r = of(i / per);
+            const int piece = i % per, first = piece / dk * 16;  // position of the piece's group
+            live[u] = keys ? (first + (piece & 15) < r.n ? 16 : 0) : min(16, r.n - first);
+            to[u] = reinterpret_cast<u32x4*>(pool + ((size_t)r.row >> 4) * (size_t)(16 * dk)) + piece;
+            if (live[u] > 0) x[u] = *to[u];
         }
-        if (live == 16) pieces[i] = x;
-        else
+#pragma unroll 1
+        for (int u = 0; u < U; ++u)
         {
-            int8_t* const b = reinterpret_cast<int8_t*>(pieces + i);
-            for (int e = 0; e < live; ++e)
+            // (one body for the four: the code is fetched once)
+            u32x4 y = u == 0 ? x[0] : u == 1 ? x[1] : u == 2 ? x[2] : x[3];
+            const int n = u == 0 ? live[0] : u == 1 ? live[1] : u == 2 ? live[2] : live[3];
+            u32x4* const out = u == 0 ? to[0] : u == 1 ? to[1] : u == 2 ? to[2] : to[3];
+            if (n <= 0) continue;
+            const Regrown r = of((i0 + u * step) / per);
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
             {
-                const uint32_t w = e < 8 ? (e < 4 ? x[0] : x[1]) : (e < 12 ? x[2] : x[3]);
-                b[e] = (int8_t)(w >> (8 * (e & 3)));
+                uint32_t z = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                {
+                    const int c = (int8_t)(y[w] >> (8 * e));
+                    z |= (uint32_t)(uint8_t)quantize_one(__fmul_rn((float)c, r.before), r.after) << (8 * e);
+                }
+                y[w] = z;
             }
+            if (n == 16) *out = y;
+            else
+                for (int e = 0; e < n; ++e)
+                    reinterpret_cast<int8_t*>(out)[e] = (int8_t)((e < 8 ? (e < 4 ? y[0] : y[1]) : (e < 12 ? y[2] : y[3])) >> (8 * (e & 3)));
         }
     }
 }
@@ -103,6 +134,7 @@ __global__ __launch_bounds__(256) void k_pages_fill_i8(FillI8Args a)
     __shared__ uint32_t top_s[kPfTok];   // by the block's first column: its largest magnitude (bits)
     __shared__ int row_s[kCols];         // row of a column's token, -1 if it is not this work-group's
     __shared__ uint8_t head_s[kCols];    // columns that begin a group of 16 positions, in order
+    __shared__ Regrown grown_s[kPfTok];  // blocks whose scale has grown
     __shared__ __align__(16) uint8_t code_s[DK * kPitch];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = blockIdx.y;
     const bool keys = blockIdx.z == 0;
@@ -156,23 +188,27 @@ __global__ __launch_bounds__(256) void k_pages_fill_i8(FillI8Args a)
             if (page_ok(id, a.num_pages)) row[e] = (int)page_row(id, g, pos[e] & ((1 << a.shift) - 1), a.Hkv, a.shift);
             if (row[e] >= 0 && older[e] > 0) s_old[e] = scales[row[e] >> a.pools.bshift];
         }
+    v4fu cs[2][NP / 4], sn[2][NP / 4];
+    const bool turn = keys && a.cosT;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (turn && any[e])
+#pragma unroll
+            for (int i = 0; i < NP / 4; ++i)
+            {
+                const size_t at = (size_t)max(pos[e], 0) * HALF + (size_t)(w * NP + 4 * i);
+                cs[e][i] = *reinterpret_cast<const v4fu*>(a.cosT + at);
+                sn[e][i] = *reinterpret_cast<const v4fu*>(a.sinT + at);
+            }
     __syncthreads();  // top_s is clear
     float top[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int e = 0; e < 2; ++e)
     {
         if (!any[e]) break;
-        if (keys && a.cosT)
-        {
-            const size_t at = (size_t)max(pos[e], 0) * HALF + (size_t)(w * NP);
+        if (turn)
 #pragma unroll
-            for (int i = 0; i < NP; i += 4)
-            {
-                const v4fu c = *reinterpret_cast<const v4fu*>(a.cosT + at + i), s = *reinterpret_cast<const v4fu*>(a.sinT + at + i);
-#pragma unroll
-                for (int n = 0; n < 4; ++n) pg_rope(x[e][0][i + n], x[e][1][i + n], c[n], s[n], x[e][0][i + n], x[e][1][i + n]);
-            }
-        }
+            for (int i = 0; i < NP; ++i) pg_rope(x[e][0][i], x[e][1][i], cs[e][i / 4][i & 3], sn[e][i / 4][i & 3], x[e][0][i], x[e][1][i]);
 #pragma unroll
         for (int i = 0; i < NP; ++i) top[e] = fmaxf(top[e], fmaxf(fabsf(x[e][0][i]), fabsf(x[e][1][i])));
         if (row[e] >= 0) atomicMax(&top_s[first[e]], __builtin_bit_cast(uint32_t, top[e]));
@@ -192,13 +228,14 @@ __global__ __launch_bounds__(256) void k_pages_fill_i8(FillI8Args a)
     int8_t* const pool = keys ? a.pools.k : a.pools.v;
 
     // ---- older codes of blocks whose scale has grown (each has its first token of this call in the first 64 columns)
-    for (unsigned long long grown = __builtin_amdgcn_ballot_w64(row[0] >= 0 && first[0] == lane && older[0] > 0 && s[0] > s_old[0]);
-         grown != 0; grown &= grown - 1)
+    const bool regrown = row[0] >= 0 && first[0] == lane && older[0] > 0 && s[0] > s_old[0];
+    const unsigned long long grown = __builtin_amdgcn_ballot_w64(regrown);
+    if (grown != 0)
     {
-        const int l = __builtin_ctzll(grown), n = __builtin_amdgcn_readlane(older[0], l);
-        const float before = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s_old[0]), l));
-        const float after = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s[0]), l));
-        requantize(pool, (size_t)(__builtin_amdgcn_readlane(row[0], l) - n), n, DK, keys, before, after, tid, 256);
+        if (w == 0 && regrown)
+            grown_s[__builtin_popcountll(grown & ((1ull << lane) - 1))] = Regrown{row[0] - older[0], older[0], s_old[0], s[0]};
+        __syncthreads();
+        requantize(pool, __builtin_popcountll(grown), block >> 4, DK, keys, tid, 256, [&](int i) { return grown_s[i]; });
     }
 
     // ---- codes: 4 of a quarter's dimensions in a word
@@ -292,7 +329,197 @@ __global__ __launch_bounds__(256) void k_pages_fill_i8(FillI8Args a)
     }
 }
 
+// The window of 64 positions with number `item` of a call, in the order of the sequences: sequence b (-1: none is left), its
+// first position of the window, its column and position of the first token, its tokens that have a place.
+struct FillWindow
+{
+    int b, from, col0, pos0, n;
+};
+
+__device__ __forceinline__ FillWindow find_window(const FillI8Args& a, int item)
+{
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int b0 = 0; b0 < a.B; b0 += kWave)
+    {
+        const int b = b0 + lane;
+        int col0 = 0, p0 = 0, n = 0;
+        if (b < a.B)
+        {
+            col0 = a.cu[b];
+            const int64_t end = min(a.cu[b + 1], a.M);
+            p0 = a.pos0 ? a.pos0[b] : 0;
+            if (col0 >= 0 && p0 >= 0 && p0 < a.limit) n = (int)max((int64_t)0, min(end - col0, (int64_t)(a.limit - p0)));
+        }
+        const int windows = n > 0 ? ((p0 + n - 1) >> 6) - (p0 >> 6) + 1 : 0;
+        int incl = windows;
+        for (int off = 1; off < kWave; off <<= 1)
+        {
+            const int x = __shfl_up(incl, off, kWave);
+            if (lane >= off) incl += x;
+        }
+        const unsigned long long here = __builtin_amdgcn_ballot_w64(before + incl > item);
+        if (here != 0)
+        {
+            const int l = __builtin_ctzll(here);
+            p0 = __builtin_amdgcn_readlane(p0, l);
+            return {b0 + l, ((p0 >> 6) + item - before - __builtin_amdgcn_readlane(incl - windows, l)) << 6,
+                    __builtin_amdgcn_readlane(col0, l), p0, __builtin_amdgcn_readlane(n, l)};
+        }
+        before += __builtin_amdgcn_readlane(incl, 63);
+    }
+    return {-1, 0, 0, 0, 0};
+}
+
+// The same for long prompts: work-group = (window of 64 positions of a sequence, KV head, keys or values), lane = position. A
+// window holds whole blocks and groups, so maxima are those of neighbouring lanes, and the values' bytes are
+// turned 4 x 4 between the lanes of a quad, which leaves words of 4 positions for LDS.
+template <int DK>
+__global__ __launch_bounds__(256) void k_windows_fill_i8(FillI8Args a)
+{
+    constexpr int HALF = DK / 2, NP = DK / 8;  // pairs of a thread
+    constexpr int kPitch = 80;                 // bytes of a dimension's 64 positions in LDS
+    __shared__ float top_s[4][4];
+    __shared__ __align__(16) uint8_t code_s[DK * kPitch];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = blockIdx.y;
+    const bool keys = blockIdx.z == 0;
+    const FillWindow at = find_window(a, xcd_run(blockIdx.x, gridDim.x));
+    if (at.b < 0) return;
+    const int pos = at.from + lane, block = 1 << a.pools.bshift, end = at.pos0 + at.n;
+    const bool in = pos >= at.pos0 && pos < end;
+    const int seen = min(max(pos, at.pos0), end - 1);  // (lanes without a token read another's)
+    const float* const src = (keys ? a.k : a.v) + (size_t)(g * DK + w * NP) * (size_t)a.M + (size_t)(at.col0 + seen - at.pos0);
+    float x[2][NP];
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int i = 0; i < NP; ++i) x[q][i] = src[(size_t)(HALF * q + i) * (size_t)a.M];
+    const bool turn = keys && a.cosT;
+    v4fu cs[NP / 4], sn[NP / 4];
+    if (turn)
+#pragma unroll
+        for (int i = 0; i < NP / 4; ++i)
+        {
+            const size_t r = (size_t)seen * HALF + (size_t)(w * NP + 4 * i);
+            cs[i] = *reinterpret_cast<const v4fu*>(a.cosT + r);
+            sn[i] = *reinterpret_cast<const v4fu*>(a.sinT + r);
+        }
+    // the lane's row: of a block that has older positions, of those, too
+    const int start = pos & -block;  // of the lane's block
+    const bool held = pos < end && start + block > at.pos0;  // the block has a token of the call, or may have
+    int row = -1;
+    if (pos < end)
+    {
+        const int id = a.table[(size_t)at.b * a.table_stride + (pos >> a.shift)];
+        if (page_ok(id, a.num_pages)) row = (int)page_row(id, g, pos & ((1 << a.shift) - 1), a.Hkv, a.shift);
+    }
+    const bool goes_on = held && row >= 0 && start < at.pos0;
+    float* const scales = keys ? a.pools.ks : a.pools.vs;
+    const float s_old = goes_on ? scales[row >> a.pools.bshift] : 0.0f;
+    if (turn)
+#pragma unroll
+        for (int i = 0; i < NP; ++i) pg_rope(x[0][i], x[1][i], cs[i / 4][i & 3], sn[i / 4][i & 3], x[0][i], x[1][i]);
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) top = fmaxf(top, fmaxf(fabsf(x[0][i]), fabsf(x[1][i])));
+    if (!in) top = 0.0f;
+    top = fmaxf(top, dpp<kDppXor1>(top));
+    top = fmaxf(top, dpp<kDppXor2>(top));
+    top = fmaxf(top, dpp<kDppHalfMirror>(top));
+    top = fmaxf(top, dpp<kDppMirror>(top));
+    if (block > 16) top = fmaxf(top, __shfl_xor(top, 16, kWave));
+    if (block > 32) top = fmaxf(top, __shfl_xor(top, 32, kWave));
+    if ((lane & 15) == 0) top_s[w][lane >> 4] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(top_s[0][lane >> 4], top_s[1][lane >> 4]), fmaxf(top_s[2][lane >> 4], top_s[3][lane >> 4]));
+    float s = __fmul_rn(top, 1.0f / 127.0f);
+    if (goes_on) s = fmaxf(s, s_old);
+    const bool begins = in && row >= 0 && (pos == at.pos0 || pos == start);  // the block's first token of the call
+    if (w == 0 && begins) scales[row >> a.pools.bshift] = s;
+    int8_t* const pool = keys ? a.pools.k : a.pools.v;
+    // older codes, of the block that the sequence goes on with
+    const unsigned long long grown = __builtin_amdgcn_ballot_w64(begins && goes_on && s > s_old);
+    if (grown != 0)
+    {
+        const int l = __builtin_ctzll(grown), n = at.pos0 & (block - 1);
+        const Regrown r{__builtin_amdgcn_readlane(row, l) - n, n, __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s_old), l)),
+                        __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s), l))};
+        requantize(pool, 1, (n + 15) >> 4, DK, keys, tid, 256, [&](int) { return r; });
+    }
+    const float rcp = quant_rcp(s);
+    uint32_t code[2][NP / 4];
+    bool amb = false;
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int i = 0; i < NP; i += 4)
+        {
+            uint32_t y = 0;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) y |= (uint32_t)(uint8_t)quantize_code(x[q][i + n], rcp, amb) << (8 * n);
+            code[q][i / 4] = y;
+        }
+    if (amb && in)
+    {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int i = 0; i < NP; i += 4)
+            {
+                uint32_t y = 0;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) y |= (uint32_t)(uint8_t)quantize_one(x[q][i + n], s) << (8 * n);
+                code[q][i / 4] = y;
+            }
+    }
+    if (keys)
+    {
+        if (in && row >= 0)
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int i = 0; i < NP; i += NP < 16 ? NP : 16)
+                {
+                    int8_t* const to = pool + key_byte((size_t)row, HALF * q + w * NP + i, DK);
+                    if constexpr (NP < 16) *reinterpret_cast<uint2*>(to) = make_uint2(code[q][0], code[q][1]);
+                    else
+                        *reinterpret_cast<u32x4*>(to) = u32x4{code[q][i / 4], code[q][i / 4 + 1], code[q][i / 4 + 2], code[q][i / 4 + 3]};
+                }
+        return;
+    }
+    const uint32_t sel1 = lane & 1 ? 0x03070105u : 0x06020400u, sel2 = lane & 2 ? 0x03020706u : 0x05040100u;
+    auto exchanged = [](uint32_t x, auto ctrl) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xF, 0xF, true); };
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int i = 0; i < NP / 4; ++i)
+        {
+            uint32_t y = code[q][i];
+            y = __builtin_amdgcn_perm(exchanged(y, std::integral_constant<int, kDppXor1>{}), y, sel1);
+            y = __builtin_amdgcn_perm(exchanged(y, std::integral_constant<int, kDppXor2>{}), y, sel2);
+            // dimension 4 i + lane % 4 of the quad's positions
+            *reinterpret_cast<uint32_t*>(code_s + (HALF * q + w * NP + 4 * i + (lane & 3)) * kPitch + (lane & ~3)) = y;
+        }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = tid; i < 4 * DK; i += 256)
+    {
+        const int d = i % DK, group = i / DK;  // (a wave's pieces are of one group)
+        const int first = max(at.pos0 - at.from - 16 * group, 0), n = min(end - at.from - 16 * group, 16);
+        // the row of the group's last position, which has a place if any of its positions has
+        const int r = __shfl(row, 16 * group + max(min(n, 16), 1) - 1, kWave);
+        if (first >= n || r < 0) continue;
+        const u32x4 y = *reinterpret_cast<const u32x4*>(code_s + d * kPitch + 16 * group);
+        int8_t* const to = pool + value_byte((size_t)(r & ~15), d, DK);
+        if (n - first == 16) *reinterpret_cast<u32x4*>(to) = y;
+        else
+            for (int e = first; e < n; ++e) to[e] = (int8_t)((e < 8 ? (e < 4 ? y[0] : y[1]) : (e < 12 ? y[2] : y[3])) >> (8 * (e & 3)));
+    }
+}
+
 // ------------------------------------------------------------------ values read back
+
+constexpr int kReadCols = 256;
 
 struct ReadI8Args
 {
@@ -303,50 +530,90 @@ struct ReadI8Args
     float* k;
     float* v;
     int M, B, Hkv, shift, table_stride, num_pages, limit;
+    int parts;  // work-groups that share a head's dimensions
 };
 
-// Work-group = (64 columns, KV head, keys or values), lane = column, wave = a quarter of the dimensions: code * scale,
-// one rounded product. Bound by the f32 columns that it writes.
+// Work-group = (256 columns, KV head and `parts`-th of its dimensions, keys or values), wave = 64 columns, lane = column,
+// 16 dimensions at a time: of keys, the column's piece of them; of values, the pieces (16 positions of a dimension) of the
+// groups that the columns lie in, 8 groups at a time, turned through LDS. (Codes of values taken from the pool one by one, or in words of four columns,
+// are bound by the addresses: 47 and 39 us at 16 x 1111 .. 2048 tokens, 16 x 28 .. 35 tokens 17.) code * scale is one
+// rounded product. Bound by the f32 columns that it writes.
 template <int DK>
 __global__ __launch_bounds__(256) void k_pages_read_i8(ReadI8Args a)
 {
-    constexpr int ND = DK / 4;
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = blockIdx.y;
+    constexpr int kPiece = 16, kGroup = 16 * kPiece + 16;  // bytes of a piece and of a group's 16 in LDS
+    __shared__ __align__(16) uint8_t piece_s[4][8 * kGroup];
+    __shared__ int group_s[4][64];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = blockIdx.y / a.parts, part = blockIdx.y - g * a.parts, d0 = part * (DK / a.parts), d1 = d0 + DK / a.parts;
     const bool keys = blockIdx.z == 0;
-    const int m0 = blockIdx.x * kPfTok, m = m0 + lane;
+    const int m0 = (xcd_run(blockIdx.x, gridDim.x) * 4 + w) * kPfTok, m = m0 + lane;
+    if (m0 >= a.M) return;
     const int b = wave_sequence(a.cu, a.B, a.M, m0, lane);
-    if (b < 0) return;
-    const int pos = packed_position(a.cu, a.pos0, b, m, a.limit);
-    size_t row = 0;
+    const int pos = b < 0 ? -1 : packed_position(a.cu, a.pos0, b, m, a.limit);
+    int row = 0;
     float s = __builtin_nanf("");  // a position that has no place
     if (pos >= 0)
     {
         const int id = a.table[(size_t)b * a.table_stride + (pos >> a.shift)];
         if (page_ok(id, a.num_pages))
         {
-            row = page_row(id, g, pos & ((1 << a.shift) - 1), a.Hkv, a.shift);
+            row = (int)page_row(id, g, pos & ((1 << a.shift) - 1), a.Hkv, a.shift);
             s = (keys ? a.pools.ks : a.pools.vs)[row >> a.pools.bshift];
         }
     }
-    int8_t c[ND];
+    float* const out = (keys ? a.k : a.v) + (size_t)(g * DK) * (size_t)a.M + (size_t)m;
     if (keys)
     {
-#pragma unroll
-        for (int i = 0; i < ND; i += 16)
+        const u32x4* const from = reinterpret_cast<const u32x4*>(a.pools.k + key_byte((size_t)row, 0, DK));
+        u32x4 x = from[d0];  // (256 bytes, 16 pieces, from one 16 dimensions to the next)
+#pragma unroll 1
+        for (int d = d0; d < d1; d += 16)
         {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(a.pools.k + key_byte(row, w * ND + i, DK));
+            const u32x4 y = x;
+            if (d + 16 < d1) x = from[d + 16];
+            if (b >= 0)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) c[i + e] = (int8_t)(x[e / 4] >> (8 * (e & 3)));
+                for (int i = 0; i < 16; ++i)
+                    out[(size_t)(d + i) * (size_t)a.M] = __fmul_rn((float)(int8_t)(y[i / 4] >> (8 * (i & 3))), s);
+        }
+        return;
+    }
+    // the groups of the wave's columns: a column begins one where the one before lies in another
+    const int own = row >> 4;
+    const int before = __shfl_up(own, 1, kWave);  // (every lane takes part: lane 1 reads lane 0's)
+    const bool head = lane == 0 || before != own;
+    const unsigned long long heads = __builtin_amdgcn_ballot_w64(head);
+    const int at = __builtin_popcountll(heads & ((2ull << lane) - 1)) - 1, n = __builtin_popcountll(heads);
+    if (head) group_s[w][at] = own;
+    wave_lds_fence();
+#pragma unroll 1
+    for (int first = 0; first < n; first += 8)
+    {
+        const u32x4* from[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            from[u] = reinterpret_cast<const u32x4*>(a.pools.v) + (size_t)group_s[w][min(first + 4 * u + (lane >> 4), n - 1)] * DK + (lane & 15);
+        const bool mine = at >= first && at < first + 8 && b >= 0;
+        const uint8_t* const code = piece_s[w] + (mine ? (at - first) * kGroup + (row & 15) : 0);
+        uint8_t* const to = piece_s[w] + (lane >> 4) * kGroup + (lane & 15) * kPiece;
+        u32x4 x[2] = {from[0][d0], from[1][d0]};
+#pragma unroll 1
+        for (int d = d0; d < d1; d += 16)
+        {
+            *reinterpret_cast<u32x4*>(to) = x[0];
+            *reinterpret_cast<u32x4*>(to + 4 * kGroup) = x[1];
+            if (d + 16 < d1) x[0] = from[0][d + 16], x[1] = from[1][d + 16];
+            wave_lds_fence();
+            int8_t c[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) c[i] = (int8_t)code[i * kPiece];
+            wave_lds_fence();
+            if (mine)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) out[(size_t)(d + i) * (size_t)a.M] = __fmul_rn((float)c[i], s);
         }
     }
-    else
-    {
-#pragma unroll
-        for (int i = 0; i < ND; ++i) c[i] = a.pools.v[value_byte(row, w * ND + i, DK)];
-    }
-    float* const out = (keys ? a.k : a.v) + (size_t)(g * DK + w * ND) * (size_t)a.M + (size_t)m;
-#pragma unroll
-    for (int i = 0; i < ND; ++i) out[(size_t)i * (size_t)a.M] = __fmul_rn((float)c[i], s);
 }
 
 // ------------------------------------------------------------------ attention of one new token per sequence
@@ -390,7 +657,8 @@ __device__ __forceinline__ void append_i8(const PoolsI8& pools, const float* k, 
         float s = __fmul_rn(__builtin_bit_cast(float, bits), 1.0f / 127.0f);
         if (into > 0) s = fmaxf(s, s_old[q]);
         int8_t* const pool = q ? pools.v : pools.k;
-        if (into > 0 && s > s_old[q]) requantize(pool, row - into, into, DK, q == 0, s_old[q], s, lane, 64);
+        if (into > 0 && s > s_old[q])
+            requantize(pool, 1, (into + 15) >> 4, DK, q == 0, lane, 64, [&](int) { return Regrown{(int)row - into, into, s_old[q], s}; });
         if (lane == 0 && (into == 0 || s > s_old[q])) (q ? pools.vs : pools.ks)[at] = s;
 #pragma unroll
         for (int n = 0; n < N; ++n)
@@ -423,14 +691,6 @@ constexpr int kI8Pitch = 80;      // bytes of a row of weights' digits in LDS (6
 __device__ __forceinline__ uint32_t digits(uint32_t X) { return (X + 0x80808080u) ^ 0x80808080u; }
 
 __device__ __forceinline__ float pow2_field(int field) { return __builtin_bit_cast(float, (uint32_t)field << 23); }
-
-// Order between a wave's own LDS accesses of different lanes
-__device__ __forceinline__ void wave_lds_fence()
-{
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
 
 // Attention of one new token per sequence: work-groups as k_pages_attn's (a chunk of positions of a sequence, a KV head
 // and a group of at most 4 NS of its query heads; four waves take the chunk's tiles in turn), records and join the
@@ -809,6 +1069,16 @@ hipError_t launch_pages_fill_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, con
 {
     const FillI8Args a{k, v, cu, pos0, cosT, sinT, pools_of(kv), kv.table, (int)M, (int)B, (int)kv.Hkv, log2_of(kv.page_size),
                        (int)kv.table_stride, (int)kv.num_pages, (int)limit};
+    // sequences of 64 tokens or more on average: windows of their positions, of which there are at most M / 64 + 2 B
+    if (M >= kPfTok * B)
+    {
+        const dim3 grid((unsigned)(M / kPfTok + 2 * B), (unsigned)kv.Hkv, 2);
+        if (kv.dk == 64) k_windows_fill_i8<64><<<grid, 256, 0, st>>>(a);
+        else if (kv.dk == 128) k_windows_fill_i8<128><<<grid, 256, 0, st>>>(a);
+        else if (kv.dk == 256) k_windows_fill_i8<256><<<grid, 256, 0, st>>>(a);
+        else return hipErrorInvalidValue;
+        return hipGetLastError();
+    }
     const dim3 grid((unsigned)ceil_div(M, kPfTok), (unsigned)kv.Hkv, 2);
     if (kv.dk == 64) k_pages_fill_i8<64><<<grid, 256, 0, st>>>(a);
     else if (kv.dk == 128) k_pages_fill_i8<128><<<grid, 256, 0, st>>>(a);
@@ -818,11 +1088,14 @@ hipError_t launch_pages_fill_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, con
 }
 
 hipError_t launch_pages_read_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, size_t M, const int32_t* cu, const int32_t* pos0,
-                                size_t B, float* k, float* v)
+                                size_t B, float* k, float* v, size_t num_cus)
 {
-    const ReadI8Args a{pools_of(kv), kv.table, cu, pos0, k, v, (int)M, (int)B, (int)kv.Hkv, log2_of(kv.page_size),
-                       (int)kv.table_stride, (int)kv.num_pages, (int)(kv.table_stride * kv.page_size)};
-    const dim3 grid((unsigned)ceil_div(M, kPfTok), (unsigned)kv.Hkv, 2);
+    ReadI8Args a{pools_of(kv), kv.table, cu, pos0, k, v, (int)M, (int)B, (int)kv.Hkv, log2_of(kv.page_size),
+                       (int)kv.table_stride, (int)kv.num_pages, (int)(kv.table_stride * kv.page_size), 1};
+    // few columns: a head's dimensions shared by more work-groups, which do not wait 16 after 16 of them
+    const size_t blocks = ceil_div(M, kReadCols);
+    while ((size_t)a.parts < kv.dk / 16 && blocks * kv.Hkv * 2 * (size_t)a.parts < 2 * num_cus) a.parts *= 2;
+    const dim3 grid((unsigned)blocks, (unsigned)(kv.Hkv * (size_t)a.parts), 2);
     if (kv.dk == 64) k_pages_read_i8<64><<<grid, 256, 0, st>>>(a);
     else if (kv.dk == 128) k_pages_read_i8<128><<<grid, 256, 0, st>>>(a);
     else if (kv.dk == 256) k_pages_read_i8<256><<<grid, 256, 0, st>>>(a);

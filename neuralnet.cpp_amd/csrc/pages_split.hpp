@@ -231,6 +231,14 @@ __device__ __forceinline__ int wave_sequence(const int32_t* cu, int B, int M, in
     return b < B && cu[b] >= 0 && cu[b] <= m && cu[b + 1] > m ? b : -1;
 }
 
+// Block of columns of work-group `at` of `blocks` (issued to the 8 XCDs in turn): an XCD takes a run of them, so that lines
+// of the L2 that two neighbouring blocks share are in one
+__device__ __forceinline__ int xcd_run(int at, int blocks)
+{
+    const int each = blocks >> 3, over = blocks & 7, xcd = at & 7;
+    return xcd * each + min(xcd, over) + (at >> 3);
+}
+
 inline int log2_of(size_t v)
 {
     int n = 0;

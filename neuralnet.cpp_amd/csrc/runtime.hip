@@ -2213,7 +2213,7 @@ nnhip_status nnhip_kv_pages_read_i8(nnhip_ctx* ctx, const nnhip_kv_pages_i8* cac
     if (M == 0 || B == 0) return NNHIP_OK;
     NNHIP_REQUIRE(k && v && cu, fn, "null pointer");
     NNHIP_REQUIRE(B < kMaxDim && M < kMaxDim - 190, fn, "M or B too large");
-    NNHIP_LAUNCH(fn, launch_pages_read_i8(ctx->stream, *cache, M, cu, pos0, B, k, v));
+    NNHIP_LAUNCH(fn, launch_pages_read_i8(ctx->stream, *cache, M, cu, pos0, B, k, v, (size_t)ctx->num_cus));
     return NNHIP_OK;
 }
 
