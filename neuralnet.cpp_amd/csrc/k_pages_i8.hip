@@ -107,6 +107,8 @@ __device__ __forceinline__ void requantize(int8_t* pool, int count, int groups, 
 
 // ------------------------------------------------------------------ fill from packed prompts
 
+constexpr int kFillThreads = 512;  // of a work-group that takes 64 columns
+
 struct FillI8Args
 {
     const float* k;
@@ -122,18 +124,18 @@ struct FillI8Args
 
 // Work-group = (64 columns, KV head, keys or values) and the blocks whose first token of this call lies in them, the
 // last of which may end up to 63 columns further: each block's largest value is known to one work-group, and every
-// element is read once. Lane = column, wave = a quarter of the dimension pairs (j, j + dk / 2); the values stay in
-// registers between the search for the blocks' maxima and their codes. Keys are stored as 16-byte pieces (lanes side
-// by side), values through LDS as bytes, 16 positions of a dimension at a time. Bound by HBM.
+// element is read once. Lane = column, wave = an eighth of the dimension pairs (j, j + dk / 2); the values stay in
+// registers between the search for the blocks' maxima and their codes. Values go through LDS as bytes, up to 16 positions of
+// a dimension at a time. For few tokens of each of many sequences: bound by latency, so by eight waves.
 // Tokens of no sequence, positions outside the table or the rope tables and pages outside the pool are not written.
 template <int DK>
-__global__ __launch_bounds__(256) void k_pages_fill_i8(FillI8Args a)
+__global__ __launch_bounds__(kFillThreads) void k_pages_fill_i8(FillI8Args a)
 {
-    constexpr int HALF = DK / 2, NP = DK / 8;  // pairs of a thread
+    constexpr int HALF = DK / 2, NP = DK / 16;  // pairs of a thread
     constexpr int kCols = 2 * kPfTok, kPitch = kCols + 4;
     __shared__ uint32_t top_s[kPfTok];   // by the block's first column: its largest magnitude (bits)
     __shared__ int row_s[kCols];         // row of a column's token, -1 if it is not this work-group's
-    __shared__ uint8_t head_s[kCols];    // columns that begin a group of 16 positions, in order
+    __shared__ uint8_t head_s[kCols], run_s[kCols];  // columns that begin a group of 16 positions, in order, and the group's
     __shared__ Regrown grown_s[kPfTok];  // blocks whose scale has grown
     __shared__ __align__(16) uint8_t code_s[DK * kPitch];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = blockIdx.y;
@@ -235,7 +237,7 @@ __global__ __launch_bounds__(256) void k_pages_fill_i8(FillI8Args a)
         if (w == 0 && regrown)
             grown_s[__builtin_popcountll(grown & ((1ull << lane) - 1))] = Regrown{row[0] - older[0], older[0], s_old[0], s[0]};
         __syncthreads();
-        requantize(pool, __builtin_popcountll(grown), block >> 4, DK, keys, tid, 256, [&](int i) { return grown_s[i]; });
+        requantize(pool, __builtin_popcountll(grown), block >> 4, DK, keys, tid, kFillThreads, [&](int i) { return grown_s[i]; });
     }
 
     // ---- codes: 4 of a quarter's dimensions in a word
@@ -277,16 +279,13 @@ __global__ __launch_bounds__(256) void k_pages_fill_i8(FillI8Args a)
             if (any[e] && row[e] >= 0)
 #pragma unroll
                 for (int q = 0; q < 2; ++q)
+                {
+                    typedef uint32_t Piece __attribute__((ext_vector_type(NP / 4)));
+                    Piece y;
 #pragma unroll
-                    for (int i = 0; i < NP; i += NP < 16 ? NP : 16)
-                    {
-                        int8_t* const to = pool + key_byte((size_t)row[e], HALF * q + w * NP + i, DK);
-                        if constexpr (NP < 16)
-                            *reinterpret_cast<uint2*>(to) = make_uint2(code[e][q][0], code[e][q][1]);
-                        else
-                            *reinterpret_cast<u32x4*>(to) =
-                                u32x4{code[e][q][i / 4], code[e][q][i / 4 + 1], code[e][q][i / 4 + 2], code[e][q][i / 4 + 3]};
-                    }
+                    for (int i = 0; i < NP / 4; ++i) y[i] = code[e][q][i];
+                    *reinterpret_cast<Piece*>(pool + key_byte((size_t)row[e], HALF * q + w * NP, DK)) = y;
+                }
         return;
     }
 #pragma unroll
@@ -297,25 +296,36 @@ __global__ __launch_bounds__(256) void k_pages_fill_i8(FillI8Args a)
 #pragma unroll
                 for (int i = 0; i < NP; ++i)
                     code_s[(HALF * q + w * NP + i) * kPitch + kPfTok * e + lane] = (uint8_t)(code[e][q][i / 4] >> (8 * (i & 3)));
-    // the columns that begin a group of 16 positions, listed by every wave alike
-    int heads = 0;
+    // the columns that begin a group of 16 positions and how many go on with it, found by every wave alike
+    unsigned long long begins[2], stops[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e)
     {
         const int c = kPfTok * e + lane, before = c > 0 ? row_s[c - 1] : -1;
         const bool head = row[e] >= 0 && !(before >= 0 && before == row[e] - 1 && (row[e] & 15) != 0);
-        const unsigned long long set = __builtin_amdgcn_ballot_w64(head);
-        if (w == 0 && head) head_s[heads + __builtin_popcountll(set & ((1ull << lane) - 1))] = (uint8_t)c;
-        heads += __builtin_popcountll(set);
+        begins[e] = __builtin_amdgcn_ballot_w64(head);
+        stops[e] = begins[e] | __builtin_amdgcn_ballot_w64(row[e] < 0);
     }
+    const int heads = __builtin_popcountll(begins[0]) + __builtin_popcountll(begins[1]);
+    if (w == 0)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (begins[e] >> lane & 1)
+            {
+                const int i = __builtin_popcountll(begins[e] & ((1ull << lane) - 1)) + (e ? __builtin_popcountll(begins[0]) : 0);
+                const unsigned long long own = lane < 63 ? stops[e] >> (lane + 1) : 0;
+                int n = own ? __builtin_ctzll(own) + 1 : 64 - lane;
+                if (!own && e == 0) n += stops[1] ? __builtin_ctzll(stops[1]) : 64;
+                head_s[i] = (uint8_t)(kPfTok * e + lane);
+                run_s[i] = (uint8_t)n;
+            }
     __syncthreads();
-    for (int i = tid; i < heads * DK; i += 256)
+#pragma unroll 2
+    for (int i = tid; i < heads * DK; i += kFillThreads)
     {
-        const int c = head_s[i / DK], d = i % DK, at = row_s[c];
+        const int h = i / DK, d = i % DK, c = head_s[h], n = run_s[h];
         const uint8_t* const from = code_s + d * kPitch + c;
-        int8_t* const to = pool + value_byte((size_t)at, d, DK);
-        int n = 1;
-        while (n < 16 - (at & 15) && c + n < kCols && row_s[c + n] == at + n) ++n;
+        int8_t* const to = pool + value_byte((size_t)row_s[c], d, DK);
         if (n == 16)
         {
             u32x4 y;
@@ -1080,9 +1090,9 @@ hipError_t launch_pages_fill_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, con
         return hipGetLastError();
     }
     const dim3 grid((unsigned)ceil_div(M, kPfTok), (unsigned)kv.Hkv, 2);
-    if (kv.dk == 64) k_pages_fill_i8<64><<<grid, 256, 0, st>>>(a);
-    else if (kv.dk == 128) k_pages_fill_i8<128><<<grid, 256, 0, st>>>(a);
-    else if (kv.dk == 256) k_pages_fill_i8<256><<<grid, 256, 0, st>>>(a);
+    if (kv.dk == 64) k_pages_fill_i8<64><<<grid, kFillThreads, 0, st>>>(a);
+    else if (kv.dk == 128) k_pages_fill_i8<128><<<grid, kFillThreads, 0, st>>>(a);
+    else if (kv.dk == 256) k_pages_fill_i8<256><<<grid, kFillThreads, 0, st>>>(a);
     else return hipErrorInvalidValue;
     return hipGetLastError();
 }
