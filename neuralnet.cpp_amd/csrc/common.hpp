@@ -443,6 +443,7 @@ hipError_t launch_pages_prefill(hipStream_t st, const nnhip_kv_pages& kv, const 
 size_t pages_prefill_spans(size_t limit, size_t num_cus);
 size_t pages_prefill_workspace_bytes(size_t dk, size_t limit, size_t num_cus);
 // the same over pools in 8 bits (k_pages_i8.hip, k_prefill_i8.hip)
+size_t pages_workspace_bytes_i8(size_t B, size_t H, size_t Hkv, size_t dk, size_t len_bound, size_t num_cus);
 hipError_t launch_pages_attn_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, const float* q, const float* k, const float* v,
                                 size_t B, size_t H, const int32_t* pos, size_t len_bound, const float* cosT,
                                 const float* sinT, float scale, float softcap, const float* slopes, bool tokens,

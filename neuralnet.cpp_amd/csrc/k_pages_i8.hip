@@ -628,69 +628,96 @@ __global__ __launch_bounds__(256) void k_pages_read_i8(ReadI8Args a)
 
 // ------------------------------------------------------------------ attention of one new token per sequence
 
-// The new token of a sequence into its page, by one wave: its rotated key and its value (element i at k[i * step]),
-// of KV head g at position p, whose page is `id`. Nothing is written for a page outside the pool.
-template <int DK>
-__device__ __forceinline__ void append_i8(const PoolsI8& pools, const float* k, const float* v, size_t step, const float* cosT,
-                                          const float* sinT, int p, int id, int num_pages, int g, int Hkv, int shift)
+// What the append of a token has left: the scales of its block, and whether older codes have changed
+struct Appended
 {
-    constexpr int HALF = DK / 2, N = (HALF + 63) / 64;
-    const int lane = threadIdx.x & 63, into = p & ((1 << pools.bshift) - 1);
-    float x[2][2][N];  // keys, values; the halves
-#pragma unroll
-    for (int n = 0; n < N; ++n)
+    float s[2];
+    bool regrown;
+};
+
+// The new token of a sequence, by one wave: its rotated key and its value of KV head g at position p. begin() gets its elements
+// (element i at k[i * step]) and its block's scales on their way; end() writes it to its page (row `row`, -1: a page outside
+// the pool, and nothing is written), and its codes, keys' and values', to LDS.
+template <int DK>
+struct Append
+{
+    static constexpr int HALF = DK / 2, N = (HALF + 63) / 64;
+    float x[2][2][N], cs[N], sn[N], s_old[2];  // keys, values; the halves
+    __device__ __forceinline__ void begin(const PoolsI8& pools, const float* k, const float* v, size_t step, const float* cosT,
+                                          const float* sinT, int p, int row)
     {
-        const int i = min(lane + 64 * n, HALF - 1);
-        x[0][0][n] = k[i * step], x[0][1][n] = k[(i + HALF) * step];
-        x[1][0][n] = v[i * step], x[1][1][n] = v[(i + HALF) * step];
-    }
-    if (!page_ok(id, num_pages)) return;
-    const size_t row = page_row(id, g, p & ((1 << shift) - 1), Hkv, shift), at = row >> pools.bshift;
-    float s_old[2] = {0.0f, 0.0f};
-    if (into > 0) s_old[0] = pools.ks[at], s_old[1] = pools.vs[at];
-    if (cosT)
-    {
+        const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int n = 0; n < N; ++n)
         {
-            const size_t r = (size_t)p * HALF + (size_t)min(lane + 64 * n, HALF - 1);
-            pg_rope(x[0][0][n], x[0][1][n], cosT[r], sinT[r], x[0][0][n], x[0][1][n]);
+            const int i = min(lane + 64 * n, HALF - 1);
+            x[0][0][n] = k[i * step], x[0][1][n] = k[(i + HALF) * step];
+            x[1][0][n] = v[i * step], x[1][1][n] = v[(i + HALF) * step];
+            if (cosT) cs[n] = cosT[(size_t)p * HALF + (size_t)i], sn[n] = sinT[(size_t)p * HALF + (size_t)i];
         }
+        const bool goes_on = row >= 0 && (p & ((1 << pools.bshift) - 1)) != 0;
+        s_old[0] = goes_on ? pools.ks[row >> pools.bshift] : 0.0f;
+        s_old[1] = goes_on ? pools.vs[row >> pools.bshift] : 0.0f;
     }
-#pragma unroll
-    for (int q = 0; q < 2; ++q)
+    __device__ __forceinline__ Appended end(const PoolsI8& pools, bool turn, int p, int row, uint8_t (*codes)[DK])
     {
-        float top = 0.0f;
+        const int lane = threadIdx.x & 63, into = p & ((1 << pools.bshift) - 1);
+        if (turn)
 #pragma unroll
-        for (int n = 0; n < N; ++n) top = fmaxf(top, fmaxf(fabsf(x[q][0][n]), fabsf(x[q][1][n])));
-        const uint32_t bits = wave_max(__builtin_bit_cast(uint32_t, top));
-        float s = __fmul_rn(__builtin_bit_cast(float, bits), 1.0f / 127.0f);
-        if (into > 0) s = fmaxf(s, s_old[q]);
-        int8_t* const pool = q ? pools.v : pools.k;
-        if (into > 0 && s > s_old[q])
-            requantize(pool, 1, (into + 15) >> 4, DK, q == 0, lane, 64, [&](int) { return Regrown{(int)row - into, into, s_old[q], s}; });
-        if (lane == 0 && (into == 0 || s > s_old[q])) (q ? pools.vs : pools.ks)[at] = s;
+            for (int n = 0; n < N; ++n) pg_rope(x[0][0][n], x[0][1][n], cs[n], sn[n], x[0][0][n], x[0][1][n]);
+        Appended got{{0.0f, 0.0f}, false};
+#pragma unroll 1
+        for (int q = 0; q < 2; ++q)
+        {
+            float y[2][N];
+            float top = 0.0f;
 #pragma unroll
-        for (int n = 0; n < N; ++n)
-            if (lane + 64 * n < HALF)
+            for (int n = 0; n < N; ++n)
+            {
+                y[0][n] = q ? x[1][0][n] : x[0][0][n], y[1][n] = q ? x[1][1][n] : x[0][1][n];
+                top = fmaxf(top, fmaxf(fabsf(y[0][n]), fabsf(y[1][n])));
+            }
+            const uint32_t bits = wave_max(__builtin_bit_cast(uint32_t, top));
+            const float before = q ? s_old[1] : s_old[0];
+            float s = __fmul_rn(__builtin_bit_cast(float, bits), 1.0f / 127.0f);
+            if (into > 0) s = fmaxf(s, before);
+            (q ? got.s[1] : got.s[0]) = s;
+            int8_t* const pool = q ? pools.v : pools.k;
+            if (row >= 0 && into > 0 && s > before)
+            {
+                got.regrown = true;
+                requantize(pool, 1, (into + 15) >> 4, DK, q == 0, lane, 64, [&](int) { return Regrown{row - into, into, before, s}; });
+            }
+            if (row >= 0 && lane == 0 && (into == 0 || s > before)) (q ? pools.vs : pools.ks)[row >> pools.bshift] = s;
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                {
-                    const int d = lane + 64 * n + HALF * h;
-                    pool[q ? value_byte(row, d, DK) : key_byte(row, d, DK)] = (int8_t)quantize_one(x[q][h][n], s);
-                }
+            for (int n = 0; n < N; ++n)
+                if (lane + 64 * n < HALF)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                    {
+                        const int d = lane + 64 * n + HALF * h;
+                        const int8_t c = (int8_t)quantize_one(y[h][n], s);
+                        if (row >= 0) pool[q ? value_byte((size_t)row, d, DK) : key_byte((size_t)row, d, DK)] = c;
+                        codes[q][d] = (uint8_t)c;
+                    }
+        }
+        return got;
     }
-}
+};
 
 // The append by itself, for calls whose attention reads a KV head by more than one work-group a chunk
 template <int DK>
 __global__ __launch_bounds__(64) void k_pages_append_i8(PagesArgs a, PoolsI8 pools)
 {
+    __shared__ uint8_t codes[2][DK];
     const int g = blockIdx.x, b = blockIdx.y, p = a.pos[b];
     if (p < 0 || p >= a.len_bound) return;
     const size_t at = a.tokens ? ((size_t)b * a.Hkv + g) * DK : (size_t)g * DK * a.B + b;
-    append_i8<DK>(pools, a.k + at, a.v + at, a.tokens ? 1 : (size_t)a.B, a.cosT, a.sinT, p,
-                  a.table[(size_t)b * a.table_stride + (p >> a.shift)], a.num_pages, g, a.Hkv, a.shift);
+    const int id = a.table[(size_t)b * a.table_stride + (p >> a.shift)];
+    const int row = page_ok(id, a.num_pages) ? (int)page_row(id, g, p & ((1 << a.shift) - 1), a.Hkv, a.shift) : -1;
+    Append<DK> append;
+    append.begin(pools, a.k + at, a.v + at, a.tokens ? 1 : (size_t)a.B, a.cosT, a.sinT, p, row);
+    append.end(pools, a.cosT != nullptr, p, row, codes);
 }
 
 constexpr int kI8Tile = 64;       // positions of a wave's tile
@@ -700,10 +727,19 @@ constexpr int kI8Pitch = 80;      // bytes of a row of weights' digits in LDS (6
 // X as four signed base-256 digits, X = sum d_i 256^i, the bytes of the result (|X| < 2^31 - 2^23.01)
 __device__ __forceinline__ uint32_t digits(uint32_t X) { return (X + 0x80808080u) ^ 0x80808080u; }
 
+// The exponent field that scales a query whose largest element has these bits
+__device__ __forceinline__ int query_field(uint32_t top) { return max((int)(top >> 23), 30); }
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_bits(uint32_t x)
+{
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, true);
+}
+
 __device__ __forceinline__ float pow2_field(int field) { return __builtin_bit_cast(float, (uint32_t)field << 23); }
 
 // Attention of one new token per sequence: work-groups as k_pages_attn's (a chunk of positions of a sequence, a KV head
-// and a group of at most 4 NS of its query heads; four waves take the chunk's tiles in turn), records and join the
+// and a group of at most 4 NS of its query heads; its W waves take the chunk's tiles in turn), records and join the
 // same. Both products run on the int8 MFMA with the codes as they lie in the pools:
 //   scores  a head's rotated query as 30-bit fixed point under its largest element, |X| < 2^30, in four
 //           signed base-256 digits: rows 4 h + i of a 16 x 64 operand for four heads, against 16 positions' keys. Every
@@ -716,24 +752,30 @@ __device__ __forceinline__ float pow2_field(int field) { return __builtin_bit_ca
 // positions for 4 heads of 128, where multiply-adds on widened elements would take 1300.
 // A head's reference maximum moves when a score passes it, to 4 above that score (weights are 2^-4 at most then and
 // 1 at most later: none is held to less than 2^-26 of the largest).
-// The chunk that holds the new position first writes its key and value, by the wave that reads them; no other wave
-// reads that block.
+// The chunk that holds the new position writes its key and value, by the wave that reads them (no other wave reads that
+// block), and takes their codes into its operands from LDS: its tile is on its way meanwhile, and is read again only
+// where the block's older codes have changed.
 // A block whose scale is not finite (its tokens had an infinity) stands for NaN, and so does a query with one.
-template <int DK, int NS, bool kFinal>
-__global__ __launch_bounds__(kPgThreads) void k_pages_attn_i8(PagesArgs a, PoolsI8 pools, int append)
+template <int DK, int NS, int W, bool kFinal>
+__global__ __launch_bounds__(64 * W) void k_pages_attn_i8(PagesArgs a, PoolsI8 pools, int append)
 {
-    constexpr int HALF = DK / 2, RT = 4 * NS, KC = DK / 64, ND = DK / 16;
-    constexpr int QI = (RT * HALF + kPgThreads - 1) / kPgThreads;  // query pairs per thread
-    __shared__ __align__(16) float q_s[RT * DK];
-    __shared__ __align__(16) uint8_t w_s[kPgWaves][NS][16 * kI8Pitch];
-    __shared__ float ml_s[2][kPgWaves][RT];
-    __shared__ __align__(16) float red_s[kPgWaves][RT * DK];
-    __shared__ int bad_s[kPgWaves];
+    constexpr int HALF = DK / 2, RT = 4 * NS, KC = DK / 64, ND = DK / 16, T = 64 * W;
+    constexpr int QI = (RT * HALF + T - 1) / T;  // query pairs per thread
+    constexpr int kDigits = DK + 4;              // words of a head's digits in LDS
+    constexpr bool kAhead = DK * NS <= 128;      // the next tile on its way during a tile (its registers are there)
+    __shared__ __align__(16) uint32_t dig_s[RT * kDigits];
+    __shared__ uint32_t top_s[RT];               // each head's largest element (bits)
+    __shared__ __align__(16) uint8_t w_s[W][NS][16 * kI8Pitch];
+    __shared__ __align__(16) uint8_t new_s[2][DK];
+    __shared__ float ml_s[2][W][RT];
+    __shared__ __align__(16) float red_s[W][RT * DK];
+    __shared__ int bad_s[W];
 
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 15, grp = lane >> 4;
     const int HG = a.Hkv * a.groups;
     const int gh = blockIdx.x % HG, item = blockIdx.x / HG;
     const int g = gh / a.groups, hg = gh - g * a.groups;
+    if (tid < RT) top_s[tid] = 0u;
     const PagesItem it = !kFinal && a.even ? find_item(a, item)
                                            : PagesItem{item / a.nchunk, item % a.nchunk, a.chunk, item - item % a.nchunk,
                                                        a.pos[item / a.nchunk]};
@@ -746,7 +788,7 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn_i8(PagesArgs a, Pools
 #pragma unroll
     for (int u = 0; u < QI; ++u)
     {
-        const int e = tid + u * kPgThreads, r = min(e / HALF, R - 1), i = e % HALF;
+        const int e = tid + u * T, r = min(e / HALF, R - 1), i = e % HALF;
         const float* q = a.q + (a.tokens ? ((size_t)b * a.H + h0 + r) * DK : (size_t)(h0 + r) * DK * a.B + b);
         qx[u][0] = q[i * io_step];
         qx[u][1] = q[(i + HALF) * io_step];
@@ -756,7 +798,7 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn_i8(PagesArgs a, Pools
     {
         // no token: zeros; a position past the bound: NaN
         if (c == 0)
-            for (int e = tid; e < R * DK; e += kPgThreads) out[e * io_step] = p < 0 ? 0.0f : __builtin_nanf("");
+            for (int e = tid; e < R * DK; e += T) out[e * io_step] = p < 0 ? 0.0f : __builtin_nanf("");
         return;
     }
     if (!kFinal && a.even && c == 0 && gh == 0 && tid == 0) a.places[b] = make_int2(it.first, it.chunk);
@@ -781,7 +823,7 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn_i8(PagesArgs a, Pools
         ks = pools.ks[row >> (pools.bshift - 4)];
         vs = pools.vs[row >> (pools.bshift - 4)];
         if (at > last) ks = vs = 0.0f;
-        load_id(t + kPgWaves * kI8Tile);
+        load_id(t + W * kI8Tile);
 #pragma unroll
         for (int n = 0; n < 4; ++n)
         {
@@ -793,30 +835,53 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn_i8(PagesArgs a, Pools
 #pragma unroll
         for (int i = 0; i < ND; ++i) vf[i] = __builtin_nontemporal_load(v + 16 * i);
     };
-    const int first = t0 + w * kI8Tile;
+    const int first = t0 + w * kI8Tile, new_tile = p & -kI8Tile;
+    // whether this wave appends the token
+    const bool own = append && p == last && first <= new_tile && (new_tile - first) % (W * kI8Tile) == 0;
     load_id(first);
-    const int new_tile = p & -kI8Tile;
-    if (append && p == last && first <= new_tile && (new_tile - first) % (kPgWaves * kI8Tile) == 0)
+    const int new_id = own ? table[p >> a.shift] : 0;
+    float cs[QI], sn[QI];
+    if (a.cosT)
+#pragma unroll
+        for (int u = 0; u < QI; ++u)
+        {
+            const size_t r = (size_t)p * HALF + (size_t)((tid + u * T) % HALF);
+            cs[u] = a.cosT[r], sn[u] = a.sinT[r];
+        }
+    if (first <= last) load(first);  // on its way during the rest
+    Append<DK> token;
+    Appended done{{0.0f, 0.0f}, false};
+    const int new_row = own && page_ok(new_id, a.num_pages) ? (int)page_row(new_id, g, p & slot_mask, a.Hkv, a.shift) : -1;
+    if (own)
     {
         const size_t at = a.tokens ? ((size_t)b * a.Hkv + g) * DK : (size_t)g * DK * a.B + b;
-        append_i8<DK>(pools, a.k + at, a.v + at, io_step, a.cosT, a.sinT, p, table[p >> a.shift], a.num_pages, g, a.Hkv, a.shift);
-        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
+        token.begin(pools, a.k + at, a.v + at, io_step, a.cosT, a.sinT, p, new_row);
     }
-    if (first <= last) load(first);  // on its way during the rest
 
     // ---- rotated queries, as digits
+    lds_barrier();  // top_s is clear
 #pragma unroll
     for (int u = 0; u < QI; ++u)
     {
-        const int e = tid + u * kPgThreads, r = e / HALF, i = e % HALF;
-        float y0 = qx[u][0], y1 = qx[u][1];
-        if (a.cosT) pg_rope(y0, y1, a.cosT[(size_t)p * HALF + i], a.sinT[(size_t)p * HALF + i], y0, y1);
-        if (e < RT * HALF)
-        {
-            // (heads past R stay 0)
-            q_s[r * DK + i] = r < R ? y0 : 0.0f;
-            q_s[r * DK + i + HALF] = r < R ? y1 : 0.0f;
-        }
+        const int r = (tid + u * T) / HALF;
+        if (a.cosT) pg_rope(qx[u][0], qx[u][1], cs[u], sn[u], qx[u][0], qx[u][1]);
+        uint32_t mx = max(__builtin_bit_cast(uint32_t, qx[u][0]) & 0x7FFFFFFFu, __builtin_bit_cast(uint32_t, qx[u][1]) & 0x7FFFFFFFu);
+        mx = max(mx, dpp_bits<kDppXor1>(mx));
+        mx = max(mx, dpp_bits<kDppXor2>(mx));
+        mx = max(mx, dpp_bits<kDppHalfMirror>(mx));
+        mx = max(mx, dpp_bits<kDppMirror>(mx));
+        if (j == 0 && r < R) atomicMax(&top_s[r], mx);
+    }
+    lds_barrier();
+#pragma unroll
+    for (int u = 0; u < QI; ++u)
+    {
+        const int e = tid + u * T, r = e / HALF, i = e % HALF;
+        if (r >= RT) continue;
+        const float up = pow2_field(283 - query_field(top_s[r]));  // brings the largest below 2^30
+        // (heads past R: 0)
+        dig_s[r * kDigits + i] = r < R ? digits((uint32_t)(int)__builtin_rintf(qx[u][0] * up)) : 0u;
+        dig_s[r * kDigits + i + HALF] = r < R ? digits((uint32_t)(int)__builtin_rintf(qx[u][1] * up)) : 0u;
     }
     lds_barrier();
     u32x4 qd[NS][KC];
@@ -824,40 +889,25 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn_i8(PagesArgs a, Pools
     // (a product past f32's range would make a score of 0 NaN; any other score is past the cap, or the range, with the
     // largest float, too)
     auto held = [](float x) { return fminf(fmaxf(x, -3.40282347e38f), 3.40282347e38f); };
+    const uint32_t sel = (uint32_t)(j & 3) | (uint32_t)((j & 3) + 4) << 8;
 #pragma unroll
     for (int s = 0; s < NS; ++s)
     {
-        const float* const q = q_s + (4 * s + (j >> 2)) * DK + 16 * grp;
-        uint32_t mx = 0;
-#pragma unroll
-        for (int i = 0; i < KC; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) mx = max(mx, __builtin_bit_cast(uint32_t, q[64 * i + e]) & 0x7FFFFFFFu);
-        mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16, kWave));
-        mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32, kWave));
-        const int e0 = max((int)(mx >> 23), 30);  // the largest is below 2^(e0 - 126)
-        const float up = pow2_field(283 - e0);           // brings it below 2^30
+        const uint32_t* const q = dig_s + (4 * s + (j >> 2)) * kDigits + 16 * grp;
 #pragma unroll
         for (int i = 0; i < KC; ++i)
 #pragma unroll
             for (int n = 0; n < 4; ++n)
             {
-                uint32_t y = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                {
-                    const uint32_t d = digits((uint32_t)(int)__builtin_rintf(q[64 * i + 4 * n + e] * up));
-                    y |= (d >> (8 * (j & 3)) & 0xFFu) << (8 * e);
-                }
-                qd[s][i][n] = y;
+                const u32x4 x = *reinterpret_cast<const u32x4*>(q + 64 * i + 4 * n);
+                qd[s][i][n] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(x[3], x[2], sel), __builtin_amdgcn_perm(x[1], x[0], sel), 0x05040100u);
             }
-        // (1 / up is a power of two)
-        float own = mx >= 0x7F800000u ? __builtin_nanf("") : 1.0f / up;
-        own = __shfl(own, 4 * grp, kWave);
-        const float to = a.cap2 > 0.0f ? a.capi : a.scale2;
-        unit[s] = own == own ? held(own * to) : own;
+        const uint32_t mx = top_s[4 * s + grp];
+        const float to = (a.cap2 > 0.0f ? a.capi : a.scale2) * pow2_field(query_field(mx) - 29);
+        unit[s] = mx >= 0x7F800000u ? __builtin_nanf("") : held(to);
         slope2[s] = a.slopes && 4 * s + grp < R ? a.slopes[h0 + 4 * s + grp] * 1.44269504f : 0.0f;
     }
+    if (own) done = token.end(pools, a.cosT != nullptr, p, new_row, new_s);
 
     v4f acc[NS][ND];
     float m[NS], l[NS];
@@ -868,11 +918,50 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn_i8(PagesArgs a, Pools
 #pragma unroll
         for (int i = 0; i < ND; ++i) acc[s][i] = v4f{};
     }
-    auto tile = [&](int t, const u32x4(&kf)[4][KC], const u32x4(&vf)[ND], float ks, float vs) {
+    for (int t = first; t <= last; t += W * kI8Tile)
+    {
+        if (!kAhead && t != first) load(t);
+        if (own && t == new_tile)
+        {
+            if (done.regrown)
+            {
+                __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
+                load_id(t);
+                load(t);
+            }
+            // the token's codes, and its block's scales
+            wave_lds_fence();
+            const int n_new = (p - t) >> 4, at = p & 15;
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+                if (n == n_new && j == at)
+#pragma unroll
+                    for (int i = 0; i < KC; ++i) kf[n][i] = *reinterpret_cast<const u32x4*>(new_s[0] + 64 * i + 16 * grp);
+            const uint32_t keep = ~(0xFFu << (8 * (at & 3)));
+#pragma unroll
+            for (int i = 0; i < ND; ++i)
+            {
+                const uint32_t x = (uint32_t)new_s[1][16 * i + j] << (8 * (at & 3));
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (grp == n_new && e == at >> 2) vf[i][e] = (vf[i][e] & keep) | x;
+            }
+            const int mine = t + 16 * (lane & 3);
+            if (mine >> pools.bshift == p >> pools.bshift && mine <= last) ks = done.s[0], vs = done.s[1];
+        }
+        u32x4 k_now[4][KC], v_now[ND];
+        const float ks_now = ks, vs_now = vs;
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int i = 0; i < KC; ++i) k_now[n][i] = kf[n][i];
+#pragma unroll
+        for (int i = 0; i < ND; ++i) v_now[i] = vf[i];
+        if (kAhead && t + W * kI8Tile <= last) load(t + W * kI8Tile);
         // a power of two above the tile's largest scale of values
-        float top_v = fmaxf(vs, dpp<kDppXor1>(vs));
+        float top_v = fmaxf(vs_now, dpp<kDppXor1>(vs_now));
         top_v = fmaxf(top_v, dpp<kDppXor2>(top_v));
-        const bool odd = __builtin_amdgcn_ballot_w64(!(fabsf(vs) < __builtin_inff())) != 0;
+        const bool odd = __builtin_amdgcn_ballot_w64(!(fabsf(vs_now) < __builtin_inff())) != 0;
         const int ev = min(max(__builtin_amdgcn_readfirstlane((int)(__builtin_bit_cast(uint32_t, top_v) >> 23)), 31), 252);
         const float down = odd ? 0.0f : pow2_field(253 - ev);                  // 2^(126 - ev) times a scale is at most 1
         const float back = odd ? __builtin_nanf("") : pow2_field(ev - 29);     // 2^(ev - 126 - 30)
@@ -880,27 +969,38 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn_i8(PagesArgs a, Pools
 #pragma unroll
         for (int n = 0; n < 4; ++n)
         {
-            kg[n] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), n));
-            vg[n] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs), n)) * down;
+            kg[n] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks_now), n));
+            vg[n] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs_now), n)) * down;
         }
         const bool part = t + kI8Tile - 1 > last;
 #pragma unroll
         for (int s = 0; s < NS; ++s)
         {
             float x[4];
-            float top = -__builtin_inff();
+            float top = -__builtin_inff(), far = 0.0f;
 #pragma unroll
             for (int n = 0; n < 4; ++n)
             {
                 v4i d = v4i{};
 #pragma unroll
                 for (int i = 0; i < KC; ++i)
-                    d = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, qd[s][i]), __builtin_bit_cast(v4i, kf[n][i]), d, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, qd[s][i]), __builtin_bit_cast(v4i, k_now[n][i]), d, 0, 0, 0);
                 const int hi = (int)((uint32_t)d[3] << 8) + d[2], lo = (int)((uint32_t)d[1] << 8) + d[0];
                 float f = unit[s] * kg[n];
                 f = kg[n] < __builtin_inff() && f == f ? held(f) : __builtin_nanf("");
                 x[n] = __builtin_fmaf((float)hi, 65536.0f, (float)lo) * f;
-                if (a.cap2 > 0.0f) x[n] = a.cap2 * tanh_any(x[n]);
+                far = fmaxf(far, fabsf(x[n]));
+            }
+            if (a.cap2 > 0.0f)
+            {
+                // scores rarely reach the cap: a few terms where none does (a NaN does not show, and stays one)
+                const bool near = __builtin_amdgcn_ballot_w64(far > 0.25f) == 0;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) x[n] = a.cap2 * (near ? tanh_below_quarter(x[n]) : tanh_any(x[n]));
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+            {
                 const int at = t + 16 * n + j;
                 if (a.slopes) x[n] = __builtin_fmaf(slope2[s], (float)(at - p), x[n]);
                 if (part && at > last) x[n] = -__builtin_inff();
@@ -910,10 +1010,11 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn_i8(PagesArgs a, Pools
             top = fmaxf(top, dpp<kDppRor4>(top));
             top = fmaxf(top, dpp<kDppXor2>(top));
             top = fmaxf(top, dpp<kDppXor1>(top));
-            if (__builtin_amdgcn_ballot_w64(top > m[s]) != 0)
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > m[s]) != 0, 0))
             {
                 const float to = top > m[s] ? top + kI8Room : m[s];
-                const float corr = m[s] == to ? 1.0f : __builtin_amdgcn_exp2f(m[s] - to);
+                float corr = m[s] == to ? 1.0f : __builtin_amdgcn_exp2f(m[s] - to);
+                asm volatile("" : "+v"(corr));  // (or every product is computed whether the branch is taken or not)
                 l[s] *= corr;
                 m[s] = to;
                 const float f = __shfl(corr, (j >> 2) * 16, kWave);
@@ -940,28 +1041,15 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn_i8(PagesArgs a, Pools
 #pragma unroll
             for (int i = 0; i < ND; ++i)
             {
-                const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, vf[i]), wd, v4i{}, 0, 0, 0);
+                const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, v_now[i]), wd, v4i{}, 0, 0, 0);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[s][i][e] = __builtin_fmaf((float)d[e], back, acc[s][i][e]);
             }
         }
         wave_lds_fence();
-    };
-    for (int t = first; t <= last; t += kPgWaves * kI8Tile)
-    {
-        u32x4 k_now[4][KC], v_now[ND];
-        const float ks_now = ks, vs_now = vs;
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-            for (int i = 0; i < KC; ++i) k_now[n][i] = kf[n][i];
-#pragma unroll
-        for (int i = 0; i < ND; ++i) v_now[i] = vf[i];
-        if (t + kPgWaves * kI8Tile <= last) load(t + kPgWaves * kI8Tile);
-        tile(t, k_now, v_now, ks_now, vs_now);
     }
 
-    // ---- join of the four waves
+    // ---- join of the waves
 #pragma unroll
     for (int s = 0; s < NS; ++s)
     {
@@ -973,14 +1061,20 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn_i8(PagesArgs a, Pools
     }
     const bool any_bad = __builtin_amdgcn_ballot_w64(bad) != 0;
     if (lane == 0) bad_s[w] = any_bad;
-    __syncthreads();
+    lds_barrier();
+    auto top_of = [&](int h) {
+        float top = ml_s[0][0][h];
+#pragma unroll
+        for (int i = 1; i < W; ++i) top = fmaxf(top, ml_s[0][i][h]);
+        return top;
+    };
     const float digit = pow2_field(127 + 8 * (j & 3));
 #pragma unroll
     for (int s = 0; s < NS; ++s)
     {
         const int h = 4 * s + (j >> 2);
-        const float own = ml_s[0][w][h], top = fmaxf(fmaxf(ml_s[0][0][h], ml_s[0][1][h]), fmaxf(ml_s[0][2][h], ml_s[0][3][h]));
-        const float f = (own == top ? 1.0f : __builtin_amdgcn_exp2f(own - top)) * digit;
+        const float mine = ml_s[0][w][h], top = top_of(h);
+        const float f = (mine == top ? 1.0f : __builtin_amdgcn_exp2f(mine - top)) * digit;
 #pragma unroll
         for (int i = 0; i < ND; ++i)
         {
@@ -994,19 +1088,23 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn_i8(PagesArgs a, Pools
             if ((i & 3) == (j & 3)) *reinterpret_cast<v4f*>(&red_s[w][h * DK + 16 * i + 4 * grp]) = y;
         }
     }
-    __syncthreads();
-    const bool lost = (bad_s[0] | bad_s[1] | bad_s[2] | bad_s[3]) != 0;
+    lds_barrier();
+    int lost = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) lost |= bad_s[i];
     float* const rec = a.part + ((size_t)(it.first + c) * HG + gh) * (size_t)(a.RG * DK + kPgRec);
-    for (int e = tid; e < R * DK; e += kPgThreads)
+    for (int e = tid; e < R * DK; e += T)
     {
         const int r = e / DK;
-        const float top = fmaxf(fmaxf(ml_s[0][0][r], ml_s[0][1][r]), fmaxf(ml_s[0][2][r], ml_s[0][3][r]));
-        float sum = 0.0f;
+        const float top = top_of(r);
+        float sum = 0.0f, y = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kPgWaves; ++i)
+        for (int i = 0; i < W; ++i)
+        {
             sum += ml_s[1][i][r] * (ml_s[0][i][r] == top ? 1.0f : __builtin_amdgcn_exp2f(ml_s[0][i][r] - top));
+            y += red_s[i][e];
+        }
         if (lost) sum = __builtin_nanf("");
-        const float y = (red_s[0][e] + red_s[1][e]) + (red_s[2][e] + red_s[3][e]);
         if constexpr (kFinal) out[e * io_step] = sum == 0.0f ? 0.0f : y / sum;
         else
         {
@@ -1018,6 +1116,14 @@ __global__ __launch_bounds__(kPgThreads) void k_pages_attn_i8(PagesArgs a, Pools
             }
         }
     }
+}
+
+// A sequence by one work-group of eight waves up to this many positions: no records, and no join
+constexpr size_t kI8Solo = 1024;
+
+inline PagesCut cut_i8(size_t B, size_t Hkv, size_t R, size_t dk, size_t len_bound, size_t num_cus)
+{
+    return len_bound <= kI8Solo ? PagesCut{round_up(len_bound, kI8Tile), 1, 0} : pages_cut(B, Hkv, R, dk, len_bound, num_cus);
 }
 
 template <int DK, int NS>
@@ -1034,10 +1140,11 @@ hipError_t launch_attn_i8(hipStream_t st, const PagesArgs& a, const PoolsI8& poo
     const dim3 grid((unsigned)(pages_items(a.B, a.len_bound, a.chunk, a.even) * a.Hkv * a.groups));
     if (a.nchunk == 1)
     {
-        k_pages_attn_i8<DK, NS, true><<<grid, kPgThreads, 0, st>>>(a, pools, append);
+        if (a.len_bound <= 4 * kI8Tile) k_pages_attn_i8<DK, NS, 4, true><<<grid, 256, 0, st>>>(a, pools, append);
+        else k_pages_attn_i8<DK, NS, 8, true><<<grid, 512, 0, st>>>(a, pools, append);
         return hipGetLastError();
     }
-    k_pages_attn_i8<DK, NS, false><<<grid, kPgThreads, 0, st>>>(a, pools, append);
+    k_pages_attn_i8<DK, NS, 4, false><<<grid, 256, 0, st>>>(a, pools, append);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     k_pages_join<DK><<<dim3((unsigned)a.H, (unsigned)a.B), kPgThreads, 0, st>>>(a);
@@ -1051,6 +1158,14 @@ PoolsI8 pools_of(const nnhip_kv_pages_i8& kv)
 
 }  // namespace
 
+size_t pages_workspace_bytes_i8(size_t B, size_t H, size_t Hkv, size_t dk, size_t len_bound, size_t num_cus)
+{
+    const size_t R = H / Hkv, groups = pages_groups(R, dk);
+    const PagesCut cut = cut_i8(B, Hkv, R, dk, len_bound, num_cus);
+    if (cut.nchunk == 1) return 0;
+    return pages_records(B, Hkv, groups, ceil_div(R, groups), dk, len_bound, cut) * sizeof(float) + (cut.even ? B * sizeof(int2) : 0);
+}
+
 hipError_t launch_pages_attn_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, const float* q, const float* k, const float* v,
                                 size_t B, size_t H, const int32_t* pos, size_t len_bound, const float* cosT,
                                 const float* sinT, float scale, float softcap, const float* slopes, bool tokens,
@@ -1058,7 +1173,7 @@ hipError_t launch_pages_attn_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, con
 {
     constexpr double kLog2e = 1.4426950408889634;
     const size_t R = H / kv.Hkv, dk = kv.dk, groups = pages_groups(R, dk);
-    const PagesCut cut = pages_cut(B, kv.Hkv, R, dk, len_bound, num_cus);
+    const PagesCut cut = cut_i8(B, kv.Hkv, R, dk, len_bound, num_cus);
     const bool cap = softcap > 0.0f;
     PagesArgs a{q, k, v, pos, cosT, sinT, kv.k, kv.v, kv.table, slopes, part,
                 reinterpret_cast<int2*>(part + (cut.even ? pages_records(B, kv.Hkv, groups, ceil_div(R, groups), dk, len_bound, cut) : 0)),

@@ -2232,7 +2232,7 @@ nnhip_status nnhip_attention_pages_decode_i8(nnhip_ctx* ctx, const nnhip_kv_page
     st = check_decode(fn, cache, B, H, len_bound, rope_cos, rope_len, softcap);
     if (st != NNHIP_OK) return st;
     void* ws = nullptr;
-    st = ensure_stream_ws(ctx, pages_workspace_bytes(B, H, cache->Hkv, cache->dk, len_bound, (size_t)ctx->num_cus), fn, &ws);
+    st = ensure_stream_ws(ctx, pages_workspace_bytes_i8(B, H, cache->Hkv, cache->dk, len_bound, (size_t)ctx->num_cus), fn, &ws);
     if (st != NNHIP_OK) return st;
     NNHIP_LAUNCH(fn, launch_pages_attn_i8(ctx->stream, *cache, q, k, v, B, H, pos, len_bound, rope_cos, rope_sin, scale,
                                           softcap, slopes, tokens != 0, static_cast<float*>(ws), out, (size_t)ctx->num_cus));
