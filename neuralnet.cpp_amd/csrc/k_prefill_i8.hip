@@ -248,6 +248,12 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
     for (int d = 0; d < ND; ++d) o[d] = v16f{};
     float m_ref = -__builtin_inff(), l_run = 0.0f;  // log2 units; l_run: this lane half's keys
     const float slope2 = kShaped && a.slopes ? a.slopes[w.head] * 1.44269504f : 0.0f;
+    float steps[16];  // the bias of a half's keys, from its first on (as many registers, at one work-group to a CU)
+    if constexpr (kShaped)
+    {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) steps[v] = slope2 * (float)(8 * (v >> 2) + (v & 3));
+    }
     if (wave < 4)
     {
         post_scales(k0, s_now);
@@ -298,46 +304,59 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
                 vs[t] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, ts4[4 + 2 * half + t])));
             }
             const bool masked = key0 + kPK - 1 > seq.from(a, w);
-            if (kShaped || masked)
-            {
-                // (an opaque factor: or the products are computed whether the branch is taken or not)
-                if constexpr (!kShaped) asm volatile("" : "+v"(kf[0]), "+v"(kf[1]));
-#pragma unroll
-                for (int v = 0; v < 16; ++v) s[v] *= kf[v >> 3];
-                kf[0] = kf[1] = 1.0f;
-            }
+            float away = 0.0f;  // the bias of the half's first key, the steps from there apart
             if constexpr (kShaped)
             {
-                // scores rarely reach the cap: a polynomial alone where none does
-                float top = 0.0f;  // (a NaN does not show, and stays one in each form)
                 if (a.cap2 > 0.0f)
                 {
+                    // scores rarely reach the cap: a polynomial of few terms where none does
+                    float top = 0.0f;  // (a NaN does not show, and stays one in each form)
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) top = fmaxf(top, fabsf(s[v]));
+                    for (int v = 0; v < 16; ++v)
+                    {
+                        s[v] *= kf[v >> 3];
+                        top = fmaxf(top, fabsf(s[v]));
+                    }
                     if (__builtin_amdgcn_ballot_w64(top > 0.25f) == 0)
                     {
 #pragma unroll
-                        for (int v = 0; v < 16; ++v) s[v] = tanh_below_quarter(s[v]);
+                        for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(tanh_below_quarter(s[v]), a.cap2, steps[v]);
                     }
                     else if (__builtin_amdgcn_ballot_w64(top > 1.0f) == 0)
                     {
 #pragma unroll
-                        for (int v = 0; v < 16; ++v) s[v] = tanh_below1(s[v]);
+                        for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(tanh_below1(s[v]), a.cap2, steps[v]);
                     }
                     else
                     {
 #pragma unroll
-                        for (int v = 0; v < 16; ++v) s[v] = tanh_any(s[v]);
+                        for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(tanh_any(s[v]), a.cap2, steps[v]);
                     }
                 }
-                // (the distance of the half's first key and the steps from there apart)
-                const float one = a.cap2 > 0.0f ? a.cap2 : 1.0f, first = (float)(key0 + 4 * h - w.qpos), away = slope2 * first;
-#pragma unroll
-                for (int v = 0; v < 16; ++v)
+                else
                 {
-                    const float step = (float)(8 * (v >> 2) + (v & 3)), bias = __builtin_fmaf(slope2, step, away);
-                    s[v] = __builtin_fmaf(s[v], one, distance && first + step > 0.0f ? -bias : bias);
+                    // (an opaque factor: or this is computed whether the branch is taken or not)
+                    asm volatile("" : "+v"(kf[0]), "+v"(kf[1]));
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(s[v], kf[v >> 3], steps[v]);
                 }
+                const float first = (float)(key0 + 4 * h - w.qpos);
+                away = slope2 * first;
+                if (distance && key0 + kPK - 1 > seq.pos0(a) + w.t0)
+                {
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        if (first + (float)(8 * (v >> 2) + (v & 3)) > 0.0f) s[v] = __builtin_fmaf(-2.0f, steps[v] + away, s[v]);
+                }
+                kf[0] = kf[1] = 1.0f;
+            }
+            else if (masked)
+            {
+                // (opaque factors here too)
+                asm volatile("" : "+v"(kf[0]), "+v"(kf[1]));
+#pragma unroll
+                for (int v = 0; v < 16; ++v) s[v] *= kf[v >> 3];
+                kf[0] = kf[1] = 1.0f;
             }
             if (masked)
             {
@@ -354,7 +373,7 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
                 for (int v = 1; v < 8; ++v) top[t] = fmaxf(top[t], s[8 * t + v]);
                 top[t] *= kf[t];
             }
-            const float mx = __builtin_ceilf(max_halves(fmaxf(top[0], top[1])));
+            const float mx = __builtin_ceilf(max_halves(fmaxf(top[0], top[1]) + away));
             // the reference of a query moves only when its maximum has grown by 2^8 (or is new)
             const bool grown = mx > m_ref + kPLazy;
             if (__builtin_expect(__builtin_amdgcn_ballot_w64(grown) != 0 || by != 1.0f, 0))
@@ -371,7 +390,7 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
                     for (int v = 0; v < 16; ++v) o[d][v] *= corr;
                 m_ref = m_new;
             }
-            const float base = kI8Up - (m_ref == -__builtin_inff() ? 0.0f : m_ref);
+            const float base = kI8Up + (m_ref == -__builtin_inff() ? 0.0f : away - m_ref);
 #pragma unroll
             for (int t = 0; t < 2; ++t)
             {
@@ -466,8 +485,8 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
     }
     if (!w.live) return;
     // (nothing visible above -infinity: 0)
-    const float den = l_run == 0.0f ? 1.0f : l_run;
-    store_out<DK>(a, w, seq, h, dim, [&](int d, int v) { return o[d][v] * by / den; });
+    const float inv = l_run == 0.0f ? 1.0f : 1.0f / l_run;
+    store_out<DK>(a, w, seq, h, dim, [&](int d, int v) { return o[d][v] * by * inv; });
 }
 
 // The items of a work-group of a call of packed prompts, one after the other: attend(item, first tile, end, record or
