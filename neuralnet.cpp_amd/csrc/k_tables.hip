@@ -26,28 +26,40 @@ __device__ __forceinline__ int64_t shfl_up64(int64_t x, int off)
     return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
 }
 
-// The sum of x over the threads before this one; total: over all
-__device__ __forceinline__ int64_t scan_before(int64_t x, int64_t* wave_s, int64_t& total)
+// The sums of x[k] over the threads before this one; total: over all
+template <int N>
+__device__ __forceinline__ void scan_before(int64_t (&x)[N], int64_t (*wave_s)[N], int64_t (&total)[N])
 {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    int64_t incl = x;
-    for (int off = 1; off < kWave; off <<= 1)
-    {
-        const int64_t y = shfl_up64(incl, off);
-        if (lane >= off) incl += y;
-    }
-    __syncthreads();  // (wave_s may still be read by an earlier scan)
-    if (lane == kWave - 1) wave_s[w] = incl;
-    __syncthreads();
-    int64_t before = 0;
-    total = 0;
+    int64_t incl[N];
 #pragma unroll
-    for (int i = 0; i < kTbWaves; ++i)
+    for (int k = 0; k < N; ++k) incl[k] = x[k];
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1)
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+        {
+            const int64_t y = shfl_up64(incl[k], off);
+            if (lane >= off) incl[k] += y;
+        }
+    if (lane == kWave - 1)
+#pragma unroll
+        for (int k = 0; k < N; ++k) wave_s[w][k] = incl[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k)
     {
-        if (i < w) before += wave_s[i];
-        total += wave_s[i];
+        int64_t before = 0;
+        total[k] = 0;
+#pragma unroll
+        for (int i = 0; i < kTbWaves; ++i)
+        {
+            const int64_t y = wave_s[i][k];
+            if (i < w) before += y;
+            total[k] += y;
+        }
+        x[k] = before + incl[k] - x[k];
     }
-    return before + incl - x;
 }
 
 __device__ __forceinline__ int pages_of(int len, int shift) { return (int)(((int64_t)len + (1 << shift) - 1) >> shift); }
@@ -105,43 +117,56 @@ __device__ __forceinline__ int bisect(const int* x, int n, int at)
     return lo;
 }
 
+// kOne: every sequence in a thread of its own
 template <bool kOne>
 __global__ __launch_bounds__(kTbThreads) void k_pages_assign(AssignArgs a)
 {
-    __shared__ int64_t wave_s[kTbWaves];
+    __shared__ int64_t need_s[kTbWaves][1], given_s[kTbWaves][2];
     __shared__ int cu_s[kOne ? kOneB : 1], page_s[kOne ? kOneB : 1], len_s[kOne ? kOneB : 1];
     const int b0 = min((int)threadIdx.x * a.run, a.B), b1 = min(b0 + a.run, a.B);
     const int64_t count = min(max(*a.free_count, 0), a.num_pages);
-    int64_t need = 0, pages = 0, tokens = 0, total, all_pages, all_tokens;
+    int first_len = 0, first_add = 0, first_n = 0;
+    if (b0 < b1) first_len = a.lens[b0], first_add = wanted(a, first_len, a.add[b0], first_n);
+    // what sequence b asks for: the first one's is in registers
+    auto asks = [&](int b, int& len, int& n) {
+        len = first_len, n = first_n;
+        if (kOne || b == b0) return first_add;
+        len = a.lens[b];
+        return wanted(a, len, a.add[b], n);
+    };
+    // on its way during the sums: the id that this thread will put into the table
+    int64_t at_id = count - 1 - (int)threadIdx.x;
+    const int id = kOne && at_id >= 0 ? a.free_pages[at_id] : 0;
+    int64_t need[1] = {0}, given[2] = {0, 0}, asked[1], all[2];
     for (int b = b0; b < b1; ++b)
     {
-        int n;
-        wanted(a, a.lens[b], a.add[b], n);
-        need += n;
+        int len, n;
+        asks(b, len, n);
+        need[0] += n;
     }
-    const int64_t asked = scan_before(need, wave_s, total);
-    need = asked;
+    scan_before(need, need_s, asked);
+    int64_t so_far = need[0];
     for (int b = b0; b < b1; ++b)
     {
-        int n;
-        const int add = wanted(a, a.lens[b], a.add[b], n);
-        need += n;
-        if (n == 0 || need <= count) pages += n, tokens += add;
+        int len, n;
+        const int add = asks(b, len, n);
+        so_far += n;
+        if (n == 0 || so_far <= count) given[0] += n, given[1] += add;
     }
-    pages = scan_before(pages, wave_s, all_pages);
-    tokens = scan_before(tokens, wave_s, all_tokens);
-    need = asked;
+    scan_before(given, given_s, all);
+    int64_t pages = given[0], tokens = given[1];
+    so_far = need[0];
     if (threadIdx.x == 0)
     {
         a.cu[0] = 0;
-        *a.free_count = (int)(count - all_pages);
+        *a.free_count = (int)(count - all[0]);
     }
     for (int b = b0; b < b1; ++b)
     {
-        int n;
-        const int len = a.lens[b], add = wanted(a, len, a.add[b], n);
-        need += n;
-        const bool given = add > 0 && (n == 0 || need <= count);
+        int len, n;
+        const int add = asks(b, len, n);
+        so_far += n;
+        const bool served = add > 0 && (n == 0 || so_far <= count);
         if (kOne)
         {
             cu_s[b] = (int)tokens;
@@ -149,22 +174,23 @@ __global__ __launch_bounds__(kTbThreads) void k_pages_assign(AssignArgs a)
             len_s[b] = len;
         }
         else a.starts[b] = (int)(count - 1 - pages);
-        if (given)
+        if (served)
         {
             pages += n;
             tokens += add;
             a.lens[b] = len + add;
         }
-        a.pos0[b] = given ? len : -1;
+        a.pos0[b] = served ? len : -1;
         a.cu[b + 1] = (int)tokens;
     }
     if constexpr (kOne)
     {
         __syncthreads();
-        for (int i = threadIdx.x; i < (int)all_pages; i += kTbThreads)
+        for (int i = threadIdx.x; i < (int)all[0]; i += kTbThreads)
         {
             const int b = bisect(page_s, a.B, i);
-            a.table[(size_t)b * a.table_stride + pages_of(len_s[b], a.shift) + (i - page_s[b])] = a.free_pages[count - 1 - i];
+            a.table[(size_t)b * a.table_stride + pages_of(len_s[b], a.shift) + (i - page_s[b])] =
+                i == (int)threadIdx.x ? id : a.free_pages[count - 1 - i];
         }
         if (a.pos || a.slots)
         {
@@ -172,7 +198,7 @@ __global__ __launch_bounds__(kTbThreads) void k_pages_assign(AssignArgs a)
             __syncthreads();  // the table's entries are there
             for (int m = threadIdx.x; m < a.M; m += kTbThreads)
             {
-                const bool there = m < (int)all_tokens;
+                const bool there = m < (int)all[1];
                 const int b = there ? bisect(cu_s, a.B, m) : 0;
                 put_token(a.table, a.table_stride, a.shift, a.num_pages, m, b, there ? len_s[b] + (m - cu_s[b]) : -1, a.pos, a.slots);
             }
@@ -180,15 +206,36 @@ __global__ __launch_bounds__(kTbThreads) void k_pages_assign(AssignArgs a)
     }
 }
 
-// The table's entries, a wave to a sequence
-__global__ __launch_bounds__(256) void k_pages_entries(AssignArgs a)
+// The table's entries, a wave to a sequence in the first `blocks` work-groups, and in the others the tokens, whose new
+// pages come from the free list (the entries may not be there yet)
+__global__ __launch_bounds__(256) void k_pages_entries(AssignArgs a, int blocks)
 {
-    const int b = (int)(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
-    if (b >= a.B) return;
-    const int len = a.pos0[b], start = a.starts[b];
-    if (len < 0) return;
-    const int held = pages_of(len, a.shift), n = pages_of(len + (a.cu[b + 1] - a.cu[b]), a.shift) - held;
-    for (int i = lane; i < n; i += kWave) a.table[(size_t)b * a.table_stride + held + i] = a.free_pages[start - i];
+    const int lane = threadIdx.x & 63;
+    if ((int)blockIdx.x < blocks)
+    {
+        const int b = (int)(blockIdx.x * 4 + (threadIdx.x >> 6));
+        if (b >= a.B) return;
+        const int len = a.pos0[b], start = a.starts[b];
+        if (len < 0) return;
+        const int held = pages_of(len, a.shift), n = pages_of(len + (a.cu[b + 1] - a.cu[b]), a.shift) - held;
+        for (int i = lane; i < n; i += kWave) a.table[(size_t)b * a.table_stride + held + i] = a.free_pages[start - i];
+        return;
+    }
+    const int m0 = (int)((blockIdx.x - blocks) * 256 + (threadIdx.x & ~63u)), m = m0 + lane;
+    if (m0 >= a.M) return;
+    const int b = wave_sequence(a.cu, a.B, a.M, m0, lane);
+    if (m >= a.M) return;
+    int p = -1, slot = -1;
+    if (b >= 0)
+    {
+        const int len = a.pos0[b], held = pages_of(len, a.shift);
+        p = len + (m - a.cu[b]);
+        const int j = p >> a.shift;
+        const int id = j >= held ? a.free_pages[a.starts[b] - (j - held)] : a.table[(size_t)b * a.table_stride + j];
+        if (page_ok(id, a.num_pages)) slot = (id << a.shift) + (p & ((1 << a.shift) - 1));
+    }
+    if (a.pos) a.pos[m] = p;
+    if (a.slots) a.slots[m] = slot;
 }
 
 struct SlotArgs
@@ -235,23 +282,32 @@ __device__ __forceinline__ int behind(const ReleaseArgs& a, int b, int& first, i
 template <bool kOne>
 __global__ __launch_bounds__(kTbThreads) void k_pages_release(ReleaseArgs a)
 {
-    __shared__ int64_t wave_s[kTbWaves];
+    __shared__ int64_t pages_s[kTbWaves][1];
     __shared__ int page_s[kOne ? kOneB : 1], first_s[kOne ? kOneB : 1];
     const int b0 = min((int)threadIdx.x * a.run, a.B), b1 = min(b0 + a.run, a.B);
     const int64_t count = min(max(*a.free_count, 0), a.num_pages);
-    int64_t pages = 0, total;
+    int first_first = 0, first_kept = 0, first_n = 0;
+    if (b0 < b1) first_n = behind(a, b0, first_first, first_kept);
+    // sequence b's: the first one's is in registers
+    auto gives = [&](int b, int& first, int& kept) {
+        first = first_first, kept = first_kept;
+        return kOne || b == b0 ? first_n : behind(a, b, first, kept);
+    };
+    int64_t before[1] = {0}, all[1];
     for (int b = b0; b < b1; ++b)
     {
         int first, kept;
-        pages += behind(a, b, first, kept);
+        before[0] += gives(b, first, kept);
     }
-    pages = scan_before(pages, wave_s, total);
+    scan_before(before, pages_s, all);
+    int64_t pages = before[0];
+    const int64_t total = all[0];
     const int64_t top = min(count + total, (int64_t)a.num_pages);  // (more than the list holds: pages given back twice)
     if (threadIdx.x == 0) *a.free_count = (int)top;
     for (int b = b0; b < b1; ++b)
     {
         int first, kept;
-        const int n = behind(a, b, first, kept);
+        const int n = gives(b, first, kept);
         if (kOne)
         {
             page_s[b] = (int)pages;
@@ -259,7 +315,7 @@ __global__ __launch_bounds__(kTbThreads) void k_pages_release(ReleaseArgs a)
         }
         else a.moves[b] = make_int4(first, n, (int)(count + total - 1 - pages), 0);
         pages += n;
-        if (a.lens[b] >= 0) a.lens[b] = kept;
+        if (kept >= 0) a.lens[b] = kept;
     }
     if constexpr (kOne)
     {
@@ -292,22 +348,23 @@ hipError_t launch_pages_assign(hipStream_t st, int32_t* table, size_t table_stri
 {
     const AssignArgs a{table, free_pages, free_count, lens, add, cu, pos0, pos, slots, static_cast<int32_t*>(ws),
                        (int)table_stride, log2_of(page_size), (int)num_pages, (int)B, (int)M, (int)ceil_div(B, (size_t)kTbThreads)};
-    const bool tokens = M > 0 && (pos || slots), one = B <= (size_t)kOneB;
-    AssignArgs first = a;
-    const bool together = one && tokens && M <= (size_t)kOneM;
-    if (!together) first.pos = first.slots = nullptr;
-    if (one) k_pages_assign<true><<<1, kTbThreads, 0, st>>>(first);
-    else k_pages_assign<false><<<1, kTbThreads, 0, st>>>(first);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    if (!one)
+    const bool tokens = M > 0 && (pos || slots);
+    if (B > (size_t)kOneB)
     {
-        k_pages_entries<<<(unsigned)ceil_div(B, (size_t)4), 256, 0, st>>>(a);
-        e = hipGetLastError();
+        k_pages_assign<false><<<1, kTbThreads, 0, st>>>(a);
+        const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
+        const size_t entries = ceil_div(B, (size_t)4), places = tokens ? ceil_div(M, (size_t)256) : 0;
+        k_pages_entries<<<(unsigned)(entries + places), 256, 0, st>>>(a, (int)entries);
+        return hipGetLastError();
     }
-    return !tokens || together ? hipSuccess
-                               : launch_pages_slots(st, table, table_stride, page_size, num_pages, cu, pos0, B, M, pos, slots);
+    AssignArgs first = a;
+    const bool together = tokens && M <= (size_t)kOneM;
+    if (!together) first.pos = first.slots = nullptr;
+    k_pages_assign<true><<<1, kTbThreads, 0, st>>>(first);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !tokens || together) return e;
+    return launch_pages_slots(st, table, table_stride, page_size, num_pages, cu, pos0, B, M, pos, slots);
 }
 
 hipError_t launch_pages_slots(hipStream_t st, const int32_t* table, size_t table_stride, size_t page_size, size_t num_pages,
