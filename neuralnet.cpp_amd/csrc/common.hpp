@@ -461,7 +461,8 @@ hipError_t launch_pages_prefill_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, 
 hipError_t launch_qk_norm_rope(hipStream_t st, const float* q, const float* k, size_t M, size_t H, size_t Hkv, size_t dk,
                                const float* gq, const float* gk, float eps, const int32_t* pos, const float* cosT,
                                const float* sinT, size_t rope_len, bool tokens, float* q_out, float* k_out, size_t num_cus);
-size_t tables_workspace_bytes(size_t B);
+size_t pages_assign_workspace_bytes(size_t B, size_t M, bool tokens);
+size_t pages_release_workspace_bytes(size_t B);
 hipError_t launch_pages_assign(hipStream_t st, int32_t* table, size_t table_stride, size_t page_size, size_t num_pages, size_t B,
                                int32_t* free_pages, int32_t* free_count, int32_t* lens, const int32_t* add, int32_t* cu,
                                int32_t* pos0, size_t M, int32_t* pos, int32_t* slots, void* ws);

@@ -6,9 +6,11 @@
 // sequence b gets its pages if those of all sequences up to it (that could be served at all) are there, and needs none or
 // gets none otherwise. Sums over the sequences are 64-bit: lengths up to 2^30 of 65535 sequences pass 2^31.
 //
-// One work-group scans the sequences, a run of them to each thread. Latency is what there is to these calls: up to kOneB sequences and
-// kOneM tokens the same work-group also writes the table's entries and the tokens, each found by bisection of
-// the offsets in LDS; beyond that further launches do, a wave to a sequence and a thread to a token.
+// One work-group scans the sequences, a run of them to each thread. Latency is what there is to these calls: the same
+// work-group also writes the table's entries and the tokens, each found by bisection of the offsets in LDS, while they are
+// few; beyond that a second launch does, a wave to a sequence and a thread to a token. Pages for new tokens and their way
+// back, in one launch and in two: 256 sequences of a token 14.8 and 20.8 us, 1000 of 1 .. 30 15.5 and 17.8, of 1 .. 60
+// 19.3 and 17.8, of 900 83 and 22; 16 of 1 .. 2000 15.0 and 18.0, of 1 .. 8000 18.4 and 18.0.
 #include "pages_split.hpp"
 
 namespace nnhip
@@ -17,8 +19,8 @@ namespace
 {
 
 constexpr int kTbThreads = 1024, kTbWaves = kTbThreads / kWave;
-constexpr int kOneB = 256;    // sequences of a call in one launch
-constexpr int kOneM = 4096;   // its tokens at most
+constexpr int kOneB = 256;    // sequences of a call in one launch, whose pages may be any number
+constexpr int kOneT = 1024, kOneM = 16384;  // and where no more than so many tokens ask for pages
 
 __device__ __forceinline__ int64_t shfl_up64(int64_t x, int off)
 {
@@ -122,7 +124,7 @@ template <bool kOne>
 __global__ __launch_bounds__(kTbThreads) void k_pages_assign(AssignArgs a)
 {
     __shared__ int64_t need_s[kTbWaves][1], given_s[kTbWaves][2];
-    __shared__ int cu_s[kOne ? kOneB : 1], page_s[kOne ? kOneB : 1], len_s[kOne ? kOneB : 1];
+    __shared__ int cu_s[kOne ? kOneT : 1], page_s[kOne ? kOneT : 1], len_s[kOne ? kOneT : 1];
     const int b0 = min((int)threadIdx.x * a.run, a.B), b1 = min(b0 + a.run, a.B);
     const int64_t count = min(max(*a.free_count, 0), a.num_pages);
     int first_len = 0, first_add = 0, first_n = 0;
@@ -340,7 +342,12 @@ __global__ __launch_bounds__(256) void k_pages_return(ReleaseArgs a)
 
 }  // namespace
 
-size_t tables_workspace_bytes(size_t B) { return B <= (size_t)kOneB ? 0 : B * sizeof(int4); }
+// Pages for the new tokens in one launch? (tokens: M bounds the pages)
+static bool assign_one(size_t B, size_t M, bool tokens) { return tokens ? B <= (size_t)kOneT && M <= (size_t)kOneM : B <= (size_t)kOneB; }
+
+size_t pages_assign_workspace_bytes(size_t B, size_t M, bool tokens) { return assign_one(B, M, tokens) ? 0 : B * sizeof(int32_t); }
+
+size_t pages_release_workspace_bytes(size_t B) { return B <= (size_t)kOneB ? 0 : B * sizeof(int4); }
 
 hipError_t launch_pages_assign(hipStream_t st, int32_t* table, size_t table_stride, size_t page_size, size_t num_pages, size_t B,
                                int32_t* free_pages, int32_t* free_count, int32_t* lens, const int32_t* add, int32_t* cu,
@@ -349,22 +356,17 @@ hipError_t launch_pages_assign(hipStream_t st, int32_t* table, size_t table_stri
     const AssignArgs a{table, free_pages, free_count, lens, add, cu, pos0, pos, slots, static_cast<int32_t*>(ws),
                        (int)table_stride, log2_of(page_size), (int)num_pages, (int)B, (int)M, (int)ceil_div(B, (size_t)kTbThreads)};
     const bool tokens = M > 0 && (pos || slots);
-    if (B > (size_t)kOneB)
+    if (assign_one(B, M, tokens))
     {
-        k_pages_assign<false><<<1, kTbThreads, 0, st>>>(a);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-        const size_t entries = ceil_div(B, (size_t)4), places = tokens ? ceil_div(M, (size_t)256) : 0;
-        k_pages_entries<<<(unsigned)(entries + places), 256, 0, st>>>(a, (int)entries);
+        k_pages_assign<true><<<1, kTbThreads, 0, st>>>(a);
         return hipGetLastError();
     }
-    AssignArgs first = a;
-    const bool together = tokens && M <= (size_t)kOneM;
-    if (!together) first.pos = first.slots = nullptr;
-    k_pages_assign<true><<<1, kTbThreads, 0, st>>>(first);
+    k_pages_assign<false><<<1, kTbThreads, 0, st>>>(a);
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || !tokens || together) return e;
-    return launch_pages_slots(st, table, table_stride, page_size, num_pages, cu, pos0, B, M, pos, slots);
+    if (e != hipSuccess) return e;
+    const size_t entries = ceil_div(B, (size_t)4), places = tokens ? ceil_div(M, (size_t)256) : 0;
+    k_pages_entries<<<(unsigned)(entries + places), 256, 0, st>>>(a, (int)entries);
+    return hipGetLastError();
 }
 
 hipError_t launch_pages_slots(hipStream_t st, const int32_t* table, size_t table_stride, size_t page_size, size_t num_pages,

@@ -2295,7 +2295,7 @@ nnhip_status nnhip_pages_assign(nnhip_ctx* ctx, int32_t* table, size_t table_str
     NNHIP_REQUIRE(free_pages && free_count && lens && add && cu && pos0, fn, "null pointer");
     NNHIP_REQUIRE(M < kMaxDim - 256, fn, "M too large");
     void* ws = nullptr;
-    st = ensure_stream_ws(ctx, tables_workspace_bytes(B), fn, &ws);
+    st = ensure_stream_ws(ctx, pages_assign_workspace_bytes(B, M, M > 0 && (pos || slots)), fn, &ws);
     if (st != NNHIP_OK) return st;
     NNHIP_LAUNCH(fn, launch_pages_assign(ctx->stream, table, table_stride, page_size, num_pages, B, free_pages, free_count, lens,
                                          add, cu, pos0, M, pos, slots, ws));
@@ -2326,7 +2326,7 @@ nnhip_status nnhip_pages_release(nnhip_ctx* ctx, const int32_t* table, size_t ta
     if (st != NNHIP_OK) return st;
     NNHIP_REQUIRE(free_pages && free_count && lens && keep, fn, "null pointer");
     void* ws = nullptr;
-    st = ensure_stream_ws(ctx, tables_workspace_bytes(B), fn, &ws);
+    st = ensure_stream_ws(ctx, pages_release_workspace_bytes(B), fn, &ws);
     if (st != NNHIP_OK) return st;
     NNHIP_LAUNCH(fn, launch_pages_release(ctx->stream, table, table_stride, page_size, num_pages, B, free_pages, free_count,
                                           lens, keep, ws));

@@ -92,7 +92,8 @@ def step(ctx, m, d, add, M=None):
 
 
 @pytest.mark.parametrize("B,page,most", [(1, 16, 1), (1, 8, 5000), (16, 64, 1), (37, 16, 200), (256, 16, 90), (257, 16, 90),
-                                         (1000, 8, 40), (1025, 32, 70), (3001, 16, 33)])
+                                         (700, 16, 9), (1000, 8, 40), (1024, 16, 15), (1025, 32, 70), (3001, 16, 33), (16, 16, 1900),
+                                         (40, 8, 1100)])
 def test_assign_and_release(ctx, nnhip, B, page, most):
     print(f"tables B={B} page={page} most={most}", flush=True)
     rng = np.random.default_rng(B + page)
