@@ -749,7 +749,8 @@ nnhip_status nnhip_attention_pages_prefill_distance(nnhip_ctx* ctx, const nnhip_
  * and q = round_half_away(clamp(fl(x / s), -127, 127)), 0 for NaN and where s is 0, as nnhip_quantize_i8. Where the block has older
  * tokens (positions before the sequence's first one of the call), its scale is kept if it is at least s;
  * otherwise their codes become those of the values that they stood for under s. An infinity makes a scale infinite, and
- * its block's codes 0: they stand for NaN. */
+ * its block's codes 0: they stand for NaN. Scales from elsewhere must be NaN, or at least 0 and below 2^121 or infinite, as
+ * every write leaves them. */
 typedef struct nnhip_kv_pages_i8
 {
     void* k;
@@ -777,8 +778,8 @@ nnhip_status nnhip_kv_pages_read_i8(nnhip_ctx* ctx, const nnhip_kv_pages_i8* cac
  * The new key and value are written as nnhip_kv_pages_fill_i8 writes one token, and take part as the cache then holds
  * them. k and v both NULL: nothing is written, the cache holds position pos[b] already (several calls may share pages then).
  * Products with the codes are exact, of queries with 30 bits under their head's largest element and weights with 30 bits under
- * the tile's; sums of tiles and softmax are f32. NaN: a head whose rotated query holds an infinity or a NaN, a
- * sequence with a scale that is not finite among its positions. */
+ * the tile's (64 positions; values under scales below 2^-96 lose bits, down to none); sums of tiles and softmax are f32. NaN: a head whose
+ * rotated query holds an infinity or a NaN, a sequence with a scale that is not finite among its positions. */
 nnhip_status nnhip_attention_pages_decode_i8(nnhip_ctx* ctx, const nnhip_kv_pages_i8* cache, const float* q, const float* k,
                                              const float* v, size_t B, size_t H, const int32_t* pos, size_t len_bound,
                                              const float* rope_cos, const float* rope_sin, size_t rope_len, float scale,
@@ -787,7 +788,8 @@ nnhip_status nnhip_attention_pages_decode_i8(nnhip_ctx* ctx, const nnhip_kv_page
 /* nnhip_attention_pages_prefill over a cache in 8 bits: the same arguments and limits, dk in {64, 128}; distance != 0:
  * the bias of nnhip_attention_pages_prefill_distance. The codes go into the products as they are, queries and weights
  * in two f16 parts: queries to 2^-23 of each element and 2^-40 of the query's largest, weights to 2^-22 of each and 2^-31 of the largest
- * before; sums and softmax are f32. NaN: a query that holds an infinity or a NaN, or sees a scale that is not finite. */
+ * before; sums and softmax are f32. Values under a scale below 2^-126 count as 0. NaN: a query that holds an infinity or
+ * a NaN, or sees a scale that is not finite. */
 nnhip_status nnhip_attention_pages_prefill_i8(nnhip_ctx* ctx, const nnhip_kv_pages_i8* cache, const float* q, size_t M,
                                               const int32_t* cu, const int32_t* pos0, size_t B, size_t t_bound, size_t H,
                                               const float* rope_cos, const float* rope_sin, size_t rope_len, float scale,
@@ -831,10 +833,11 @@ nnhip_status nnhip_pages_slots(nnhip_ctx* ctx, const int32_t* table, size_t tabl
 nnhip_status nnhip_pages_release(nnhip_ctx* ctx, const int32_t* table, size_t table_stride, size_t page_size, size_t num_pages,
                                  size_t B, int32_t* free_pages, int32_t* free_count, int32_t* lens, const int32_t* keep);
 
-/* Scratch that nnhip_attention_pages_decode (nnhip_logits_adjust_rows) of these sizes uses, over pages of any type;
+/* Scratch that nnhip_attention_pages_decode (nnhip_logits_adjust_rows) of these sizes uses, over pages in 8 bits at most;
  * nnhip_attention_pages_prefill uses 2 * (dk + 2) KiB and 16 bytes for each CU where the table (and the rope tables) hold
- * more than 128 positions, nnhip_pages_assign and nnhip_pages_release 16 bytes for each of more than 256 sequences. The context keeps one for each stream that it was set to, grown on demand and freed with the context only, so that a
- * captured call stays valid; a call that would have to grow it during a capture fails with
+ * more than 128 positions, nnhip_pages_assign 4 bytes a sequence (none for up to 1024 sequences and 16384 tokens, or 256
+ * sequences without tokens), nnhip_pages_release 16 bytes for each of more than 256 sequences. The context keeps one
+ * for each stream that it was set to, grown on demand and freed with the context only, so that a captured call stays valid; a call that would have to grow it during a capture fails with
  * NNHIP_ERR_UNSUPPORTED (call once before, on the capture's stream). Captured calls of one stream share
  * its scratch, wherever they are replayed: their replays must overlap neither each other nor eager calls
  * on that stream. */

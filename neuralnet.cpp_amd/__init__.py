@@ -1011,14 +1011,14 @@ class Context:
         cs, sn, rows = self._rope(cos, sin, cache.dk)
         shape = (cache.Hkv * cache.dk, M)
         self._bind_stream()
-        fn = "nnhip_kv_pages_fill_i8" if type(cache) is KVPagesI8 else "nnhip_kv_pages_fill"
+        fn = "nnhip_kv_pages_fill_i8" if isinstance(cache, KVPagesI8) else "nnhip_kv_pages_fill"
         _check(getattr(lib(), fn)(self.h, cache.ref, self._arg(k, f32, shape, "k"), self._arg(v, f32, shape, "v"),
                                   M, cu_p, pos0_p, B, cs, sn, rows), fn)
 
     def kv_pages_read(self, cache, cu, M: int, pos0=None, k=None, v=None):
         """The values that cache, a KVPagesI8, holds: k, v (Hkv*dk, M) get in columns cu[b] .. cu[b+1] - 1 those of sequence
         b's positions pos0[b] on. Returns k, v."""
-        if type(cache) is not KVPagesI8:
+        if not isinstance(cache, KVPagesI8):
             raise NNHipError(1, "kv_pages_read takes a KVPagesI8 (the pools of a KVPages are its values)")
         B, cu_p, pos0_p = self._packed(cache, cu, pos0)
         f32, shape = self._torch.float32, (cache.Hkv * cache.dk, M)
@@ -1045,7 +1045,7 @@ class Context:
             out = self._empty(qs, f32)
         cs, sn, rows = self._rope(cos, sin, dk)
         self._bind_stream()
-        fn = "nnhip_attention_pages_decode_i8" if type(cache) is KVPagesI8 else "nnhip_attention_pages_decode"
+        fn = "nnhip_attention_pages_decode_i8" if isinstance(cache, KVPagesI8) else "nnhip_attention_pages_decode"
         _check(getattr(lib(), fn)(
             self.h, cache.ref, self._arg(q, f32, qs, "q"), self._arg(k, f32, ks, "k"), self._arg(v, f32, ks, "v"), B, H,
             self._arg(pos, self._torch.int32, (B,), "pos"), len_bound, cs, sn, rows, scale, softcap,
@@ -1067,7 +1067,7 @@ class Context:
         cs, sn, rows = self._rope(cos, sin, cache.dk)
         self._bind_stream()
         more = ()
-        if type(cache) is KVPagesI8:
+        if isinstance(cache, KVPagesI8):
             fn, more = "nnhip_attention_pages_prefill_i8", (int(distance),)
         else:
             fn = "nnhip_attention_pages_prefill_distance" if distance else "nnhip_attention_pages_prefill"
@@ -1104,12 +1104,20 @@ class Context:
         H, q_p, qo_p, q_out = one(q, q_out, "q")
         Hkv, k_p, ko_p, k_out = one(k, k_out, "k")
         cs, sn, rows = self._rope(cos, sin, dk)
+        if cos is not None and rows == 0:
+            raise NNHipError(1, "the rope tables are empty")
         self._bind_stream()
         _check(lib().nnhip_qk_norm_rope(
             self.h, q_p, k_p, M, H, Hkv, dk, self._arg(gamma_q, f32, (dk,), "gamma_q"),
             self._arg(gamma_k, f32, (dk,), "gamma_k"), eps, self._arg(pos, torch.int32, (M,), "pos"), cs, sn, rows,
             int(tokens), qo_p, ko_p), "nnhip_qk_norm_rope")
         return q_out, k_out
+
+    def _table(self, table):
+        """The address and shape of a page table."""
+        if table.dim() != 2:
+            raise NNHipError(1, f"the page table must be (B, pages), not {tuple(table.shape)}")
+        return self._arg(table, self._torch.int32, table.shape, "table"), table.shape
 
     def _places(self, pos, slots):
         """The capacity M of per-token outputs and their addresses."""
@@ -1122,14 +1130,14 @@ class Context:
         its row of table (B, pages), behind the pages of its lens[b] positions; lens moves on (all int32 device tensors). cu
         (B + 1): offsets of the tokens that got their places; pos0 (B): the first one's position, -1 for none; pos, slots
         (M), when given: every token's position and slot, -1 behind the last. Returns cu, pos0."""
-        i32, (B, width) = self._torch.int32, table.shape
+        i32, (table_p, (B, width)) = self._torch.int32, self._table(table)
         cu = self._empty((B + 1,), i32) if cu is None else cu
         pos0 = self._empty((B,), i32) if pos0 is None else pos0
         num_pages = free_pages.shape[0]
         M, pos_p, slots_p = self._places(pos, slots)
         self._bind_stream()
         _check(lib().nnhip_pages_assign(
-            self.h, self._arg(table, i32, (B, width), "table"), width, page_size, num_pages, B,
+            self.h, table_p, width, page_size, num_pages, B,
             self._arg(free_pages, i32, (num_pages,), "free_pages"), self._arg(free_count, i32, (1,), "free_count"),
             self._arg(lens, i32, (B,), "lens"), self._arg(add, i32, (B,), "add"), self._arg(cu, i32, (B + 1,), "cu"),
             self._arg(pos0, i32, (B,), "pos0"), M, pos_p, slots_p), "nnhip_pages_assign")
@@ -1137,13 +1145,13 @@ class Context:
 
     def pages_slots(self, table, page_size: int, num_pages: int, cu, pos0=None, pos=None, slots=None):
         """Positions pos (M) and slots (M) of packed tokens (cu (B + 1), pos0 (B) or None), either of which may be None."""
-        i32, B = self._torch.int32, cu.shape[0] - 1
-        if B > table.shape[0]:
-            raise NNHipError(1, f"{B} sequences, the page table has {table.shape[0]} rows")
+        i32, B, (table_p, (table_rows, width)) = self._torch.int32, cu.shape[0] - 1, self._table(table)
+        if B < 0 or B > table_rows:
+            raise NNHipError(1, f"cu must hold B + 1 offsets, B at most the page table's {table_rows} rows")
         M, pos_p, slots_p = self._places(pos, slots)
         self._bind_stream()
         _check(lib().nnhip_pages_slots(
-            self.h, self._arg(table, i32, tuple(table.shape), "table"), table.shape[1], page_size, num_pages,
+            self.h, table_p, width, page_size, num_pages,
             self._arg(cu, i32, (B + 1,), "cu"), self._arg(pos0, i32, (B,), "pos0"), B, M, pos_p, slots_p),
             "nnhip_pages_slots")
         return pos, slots
@@ -1151,11 +1159,11 @@ class Context:
     def pages_release(self, table, page_size: int, free_pages, free_count, lens, keep) -> None:
         """Sequence b keeps its first keep[b] positions (0: none): lens[b] becomes that, and the pages behind go back to
         the list, so that a release of what pages_assign has just given leaves the list as it was."""
-        i32, (B, width) = self._torch.int32, table.shape
+        i32, (table_p, (B, width)) = self._torch.int32, self._table(table)
         num_pages = free_pages.shape[0]
         self._bind_stream()
         _check(lib().nnhip_pages_release(
-            self.h, self._arg(table, i32, (B, width), "table"), width, page_size, num_pages, B,
+            self.h, table_p, width, page_size, num_pages, B,
             self._arg(free_pages, i32, (num_pages,), "free_pages"), self._arg(free_count, i32, (1,), "free_count"),
             self._arg(lens, i32, (B,), "lens"), self._arg(keep, i32, (B,), "keep")), "nnhip_pages_release")
 

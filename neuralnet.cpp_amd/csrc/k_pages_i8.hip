@@ -961,7 +961,7 @@ __global__ __launch_bounds__(64 * W) void k_pages_attn_i8(PagesArgs a, PoolsI8 p
         // a power of two above the tile's largest scale of values
         float top_v = fmaxf(vs_now, dpp<kDppXor1>(vs_now));
         top_v = fmaxf(top_v, dpp<kDppXor2>(top_v));
-        const bool odd = __builtin_amdgcn_ballot_w64(!(fabsf(vs_now) < __builtin_inff())) != 0;
+        const bool odd = __builtin_amdgcn_ballot_w64(!(fabsf(vs_now) < 0x1p125f)) != 0;  // (no write makes one from there on)
         const int ev = min(max(__builtin_amdgcn_readfirstlane((int)(__builtin_bit_cast(uint32_t, top_v) >> 23)), 31), 252);
         const float down = odd ? 0.0f : pow2_field(253 - ev);                  // 2^(126 - ev) times a scale is at most 1
         const float back = odd ? __builtin_nanf("") : pow2_field(ev - 29);     // 2^(ev - 126 - 30)

@@ -2199,6 +2199,7 @@ nnhip_status nnhip_kv_pages_fill_i8(nnhip_ctx* ctx, const nnhip_kv_pages_i8* cac
     NNHIP_REQUIRE(B < kMaxDim && M < kMaxDim - 190, fn, "M or B too large");
     size_t limit = cache->table_stride * cache->page_size;
     if (rope_cos) limit = std::min(limit, rope_len);
+    if (limit == 0) return NNHIP_OK;  // (no position has a place)
     NNHIP_LAUNCH(fn, launch_pages_fill_i8(ctx->stream, *cache, k, v, M, cu, pos0, B, rope_cos, rope_sin, limit));
     return NNHIP_OK;
 }
@@ -2274,7 +2275,7 @@ nnhip_status nnhip_qk_norm_rope(nnhip_ctx* ctx, const float* q, const float* k, 
     NNHIP_REQUIRE((q == nullptr) == (q_out == nullptr) && (k == nullptr) == (k_out == nullptr), fn,
                   "q and q_out go together, and k and k_out");
     NNHIP_REQUIRE((rope_cos == nullptr) == (rope_sin == nullptr), fn, "rope_cos and rope_sin go together");
-    NNHIP_REQUIRE(!rope_cos || pos, fn, "the rotation needs positions");
+    NNHIP_REQUIRE(!rope_cos || (pos && rope_len >= 1), fn, "the rotation needs positions, and tables with a row");
     if (M == 0 || (!q && !k)) return NNHIP_OK;
     NNHIP_REQUIRE((!q || H >= 1) && (!k || Hkv >= 1) && H <= 65535 && Hkv <= 65535, fn, "H and Hkv must be in [1, 65535]");
     NNHIP_REQUIRE(M < kMaxDim - 64 && M * (H + Hkv) < kMaxDim, fn, "M * (H + Hkv) must be below 2^31");

@@ -359,7 +359,8 @@ class Decoder:
         """Block i's attention of the step's tokens over its cache."""
         cfg, cache = self.cfg, self.caches[i]
         cos, sin = self._qk_norm(i, q, k, pos, tokens)
-        if self.cos is not None and len_bound > self.cos.shape[0]:
+        if cos is None and self.cos is not None and len_bound > self.cos.shape[0]:
+            # (the attention does not see the tables, which it checks otherwise)
             raise _pkg().NNHipError(1, "len_bound must not exceed the rows of the rope tables")
         if self.paged:
             self.ctx.attention_pages_decode(cache, q, k, v, cfg.H, pos, len_bound, cfg.scale, cos=cos, sin=sin,

@@ -640,3 +640,104 @@ def test_refusals(ctx, nnhip):
     # nothing to do
     ctx.kv_pages_fill(cache, dev(np.zeros((128, 0), F32)), dev(np.zeros((128, 0), F32)), dev(np.zeros(3, np.int32)))
     assert ctx.kv_pages_read(cache, dev(np.zeros(1, np.int32)), 2)[0].shape == (128, 2)
+
+
+def test_rope_tables_without_rows(ctx, nnhip):
+    """No position has a place then: nothing is written, and nothing is read behind the tables' beginning."""
+    t = dev(np.array([[1]], np.int32))
+    cache = nnhip.KVPagesI8.empty(2, 1, 16, 64, 16, t)
+    x, cos, cu = dev(np.ones((64, 9), F32)), dev(np.ones((1, 32), F32)), dev(np.array([0, 9], np.int32))
+    assert nnhip.lib().nnhip_kv_pages_fill_i8(ctx.h, cache.ref, x.data_ptr(), x.data_ptr(), 9, cu.data_ptr(), None, 1,
+                                              cos.data_ptr(), cos.data_ptr(), 0) == 0
+    ctx.sync()
+    assert not host(cache.k).any() and not host(cache.k_scale).any()
+    with pytest.raises(nnhip.NNHipError, match="rope tables are empty"):
+        ctx.qk_norm_rope(x, None, 64, 1e-5, pos=dev(np.zeros(9, np.int32)), cos=cos[:0], sin=cos[:0])
+
+
+def everything(ctx, cache, k, v, cu, q, pos, H, max_len):
+    """A fill, the values read back, attention of the prompts and of a further token."""
+    M = k.shape[1]
+    ctx.kv_pages_fill(cache, k, v, cu)
+    prompt = ctx.attention_pages_prefill(cache, q, cu, M, H, 0.1)
+    B = cu.shape[0] - 1
+    first = q[:, :B].contiguous()
+    one = ctx.attention_pages_decode(cache, first, k[:, :B].contiguous(), v[:, :B].contiguous(), H, pos, max_len, 0.1)
+    return [prompt, one, *ctx.kv_pages_read(cache, cu, M)]
+
+
+@pytest.mark.parametrize("dk", [64, 128])
+def test_large_pool(ctx, nnhip, dk):
+    """Pages past 2^31 bytes of a pool: as in a small one."""
+    import torch
+    rng = np.random.default_rng(90)
+    H, Hkv, page, lens = 8, 4, 128, [300, 1500, 70]
+    need = [-(-(n + 1) // page) for n in lens]
+    total = (2 ** 31 + 2 ** 28) // (Hkv * page * dk)
+    cu = dev(np.concatenate(([0], np.cumsum(lens))).astype(np.int32))
+    k, v, q = (dev(rng.standard_normal((h * dk, sum(lens))).astype(F32)) for h in (Hkv, Hkv, H))
+    pos = dev(np.array(lens, np.int32))
+    found = []
+    for pages in (sum(need), total):
+        table = np.full((3, max(need)), -1, np.int32)
+        at = 0
+        for b, n in enumerate(need):
+            table[b, :n] = pages - 1 - at - np.arange(n)  # from the pool's end
+            at += n
+        cache = nnhip.KVPagesI8.empty(pages, Hkv, page, dk, 32, dev(table))
+        found.append([host(x) for x in everything(ctx, cache, k, v, cu, q, pos, H, max(lens) + 1)])
+        del cache
+    torch.cuda.empty_cache()
+    for a, b in zip(*found):
+        assert np.isfinite(a).all() and np.array_equal(a, b)
+
+
+def test_two_streams_at_once(nnhip):
+    """Calls of unlike sizes on two streams, each over a cache of its own, with records in scratch of their own: as alone."""
+    import torch
+    ctx = nnhip.Context(0)
+    rng = np.random.default_rng(91)
+    H, Hkv, dk, page = 8, 2, 128, 32
+    sets = []
+    for lens in ([1800, 40, 700], [90, 2500]):
+        need = [-(-(n + 1) // page) for n in lens]
+        table = np.zeros((len(lens), max(need)), np.int32)
+        at = 0
+        for b, n in enumerate(need):
+            table[b, :n] = at + np.arange(n)
+            at += n
+        cu = dev(np.concatenate(([0], np.cumsum(lens))).astype(np.int32))
+        k, v, q = (dev(rng.standard_normal((h * dk, sum(lens))).astype(F32)) for h in (Hkv, Hkv, H))
+        cache = nnhip.KVPagesI8.empty(at, Hkv, page, dk, 16, dev(table))
+        sets.append((cache, k, v, cu, q, dev(np.array(lens, np.int32)), H, max(lens) + 1))
+    alone = [[host(x) for x in everything(ctx, *s)] for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        outs = [[], []]
+        for _ in range(3):
+            for i, s in enumerate(sets):
+                with torch.cuda.stream(streams[i]):
+                    outs[i].append(everything(ctx, *s))
+        torch.cuda.synchronize()
+        for i in range(2):
+            for got in outs[i]:
+                for a, b in zip(alone[i], got):
+                    assert np.array_equal(a, host(b))
+    ctx.close()
+
+
+def test_derived_handle(ctx, nnhip):
+    """A class made from KVPagesI8 is one."""
+    class Mine(nnhip.KVPagesI8):
+        pass
+
+    found = []
+    for cls in (nnhip.KVPagesI8, Mine):
+        cache = cls.empty(8, 2, 16, 64, 16, dev(np.arange(8, dtype=np.int32).reshape(2, 4)))
+        r = np.random.default_rng(93)
+        k, v, q = (dev(r.standard_normal((h * 64, 50)).astype(F32)) for h in (2, 2, 4))
+        cu = dev(np.array([0, 20, 50], np.int32))
+        found.append([host(x) for x in everything(ctx, cache, k, v, cu, q, dev(np.array([20, 30], np.int32)), 4, 40)])
+    for a, b in zip(*found):
+        assert np.array_equal(a, b)

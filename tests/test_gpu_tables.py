@@ -230,3 +230,7 @@ def test_table_refusals(ctx, nnhip):
         nnhip._check(nnhip.lib().nnhip_pages_slots(ctx.h, t.data_ptr(), 4, 16, 8, None, None, 2, 5, None, None), "slots")
     with pytest.raises(nnhip.NNHipError, match="rows"):
         ctx.pages_slots(t, 16, 8, dev(np.zeros(4, I32)), pos=b)
+    for call in (lambda x: ctx.pages_assign(x, 16, free, one, b, b), lambda x: ctx.pages_release(x, 16, free, one, b, b),
+                 lambda x: ctx.pages_slots(x, 16, 8, dev(np.zeros(3, I32)), pos=b)):
+        with pytest.raises(nnhip.NNHipError, match="page table must be"):
+            call(dev(np.zeros(8, I32)))
