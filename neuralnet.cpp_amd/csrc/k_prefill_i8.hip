@@ -41,6 +41,8 @@ constexpr float kI8Up = 6.0f;    // log2 of the largest weight when a reference 
 constexpr int kI8Near = 5;       // the largest scale of a tile's values is within 2^+-5 of O's unit
 constexpr int kI8Low = -14;      // the least power of two that codes are multiplied by: they stay normal f16 values
 
+constexpr int kJoin = 8;         // dimensions of a work-group that joins (17 records: 16 25.7 us, 8 24.8, 4 25.0)
+
 template <int DK>
 struct TileI8
 {
@@ -99,6 +101,18 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
     PrefillSeq<true> seq;
     int last_key;
     seat(a, item, tid, w, seq, last_key);
+    // Where at most half of the waves have queries, the others take the second half of each tile for them (6 x 5 .. 30
+    // queries of 16 heads behind 2000 positions, 8 KV heads: 42.5 us without, 37.5)
+    const int pair = kPWaves / 2, queries = kPQ << (kPWaveShift - log2_heads(a));  // of the work-group
+    const bool shared = a.R < kPWaves && seq.n(a) - item.qb * queries <= queries / 2;
+    const bool second = shared && wave >= pair;
+    if (second)
+    {
+        w.t0 -= queries / 2;
+        w.qt -= queries / 2;
+        w.qpos -= queries / 2;
+        w.live = w.t0 < seq.n(a);
+    }
     const int end_key = min(last_key, k1 * kPK - 1);  // the last key of these tiles
 
     // ---- staging: a wave's pieces are of one group of 16 positions
@@ -287,7 +301,7 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
         for (int half = 0; half < 2; ++half)
         {
             const int key0 = (kb + half) * kPK;
-            if (!w.live || kb + half >= k1 || key0 > seq.to(a, w)) continue;
+            if (!w.live || kb + half >= k1 || key0 > seq.to(a, w) || (shared && half != (int)second)) continue;
             v16f s = v16f{};
 #pragma unroll
             for (int c = 0; c < NC; ++c)
@@ -477,13 +491,44 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
     if (found) l_run = __builtin_nanf("");
     // (a unit that no tile of the wave's has taken up yet is still to come off)
     by = __builtin_ldexpf(by, unit - 127);
+    if (shared)
+    {
+        // the second halves' outputs, maxima and sums through LDS (every wave is past its tiles)
+        float* const at = reinterpret_cast<float*>(smem) + (wave & (pair - 1)) * (16 * ND + 2) * kWave + lane;
+        if (second && w.live)
+        {
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) at[(16 * d + v) * kWave] = o[d][v] * by;
+            at[16 * ND * kWave] = m_ref;
+            at[(16 * ND + 1) * kWave] = l_run;
+        }
+        __syncthreads();
+        if (!second && w.live)
+        {
+            const float m = at[16 * ND * kWave], to = fmaxf(m_ref, m);
+            const float own = m_ref == to ? 1.0f : __builtin_amdgcn_exp2f(m_ref - to);
+            const float other = m == to ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+            l_run = __builtin_fmaf(at[(16 * ND + 1) * kWave], other, l_run * own);
+            by *= own;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) o[d][v] = __builtin_fmaf(at[(16 * d + v) * kWave], other, o[d][v] * by);
+            by = 1.0f;
+            m_ref = to;
+        }
+        __syncthreads();  // the next item may write there
+        w.live &= !second;
+    }
     auto dim = [](int d, int i) { return 32 * d + i; };
+    if (!w.live) return;
     if (rec)
     {
         store_record<DK>(rec, tid, dim, [&](int d, int v) { return o[d][v] * by; }, m_ref, l_run);
         return;
     }
-    if (!w.live) return;
     // (nothing visible above -infinity: 0)
     const float inv = l_run == 0.0f ? 1.0f : 1.0f / l_run;
     store_out<DK>(a, w, seq, h, dim, [&](int d, int v) { return o[d][v] * by * inv; });
@@ -508,7 +553,7 @@ __device__ __forceinline__ void prompt_items(const PrefillArgs& a, uint8_t* smem
         PromptCut* const cuts = reinterpret_cast<PromptCut*>(smem);
         if (wave < 2)
         {
-            const PromptCut cut = prompt_cut(a, a.spans, g + wave);
+            const PromptCut cut = prompt_cut<true>(a, a.spans, g + wave);
             if ((threadIdx.x & 63) == 0)
             {
                 cuts[wave] = cut;
@@ -586,7 +631,7 @@ hipError_t launch_prefill_i8_dk(hipStream_t st, const PrefillArgs& a, const Scal
     {
         e = hipGetLastError();
         if (e != hipSuccess) return e;
-        k_prompt_join<DK><<<dim3((unsigned)a.spans - 1, DK / 16), 32 * kPWaves, 0, st>>>(a);
+        k_prompt_join<DK, kJoin, 2><<<dim3((unsigned)a.spans - 1, DK / kJoin), 32 * kPWaves, 0, st>>>(a);
     }
     return hipGetLastError();
 }

@@ -299,28 +299,28 @@ __device__ __forceinline__ int prompt_tiles(const PrefillArgs& a, const PrefillS
     return (max(q.pos0_ + min((qb + 1) << qs, q.n_), q.pre) + kPK - 1) >> kPKShift;
 }
 
-// Tiles of blocks 0 .. qb - 1 with kOver each: A + j u for block j - 1, but at least P, and the last block's own
-__device__ __forceinline__ int64_t prompt_before(const PrefillArgs& a, const PrefillSeq<true>& q, int qb)
+// Tiles of blocks 0 .. qb - 1 with `over` each: A + j u for block j - 1, but at least P, and the last block's own
+__device__ __forceinline__ int64_t prompt_before(const PrefillArgs& a, const PrefillSeq<true>& q, int qb, int over = kOver)
 {
     const int us = kPWaveShift - log2_heads(a);  // log2 of u
     const int nq = prompt_blocks(a, q.n_), A = (q.pos0_ + kPK - 1) >> kPKShift, P = (q.pre + kPK - 1) >> kPKShift;
     const int full = min(qb, nq - 1);
     const int k = max(0, min(full, ((P - A + (1 << us) - 1) >> us) - 1));
-    int64_t f = (int64_t)k * P + (int64_t)(full - k) * (A + kOver) + (int64_t)k * kOver +
+    int64_t f = (int64_t)k * P + (int64_t)(full - k) * (A + over) + (int64_t)k * over +
                 (((int64_t)full * (full + 1) - (int64_t)k * (k + 1)) >> 1 << us);
-    if (qb == nq && nq > 0) f += prompt_tiles(a, q, nq - 1) + kOver;
+    if (qb == nq && nq > 0) f += prompt_tiles(a, q, nq - 1) + over;
     return f;
 }
 
 // Work of sequence b (0 past the last, or if it does not fit)
-__device__ __forceinline__ int64_t prompt_work(const PrefillArgs& a, int b, int& most)
+__device__ __forceinline__ int64_t prompt_work(const PrefillArgs& a, int b, int& most, int over = kOver)
 {
     PrefillSeq<true> q;
     most = 0;
     if (b >= a.B || !packed_seq(a, b, q) || q.n_ <= 0) return 0;
     const int nq = prompt_blocks(a, q.n_);
     most = prompt_tiles(a, q, nq - 1);
-    return prompt_before(a, q, nq);
+    return prompt_before(a, q, nq, over);
 }
 
 __device__ __forceinline__ int64_t read_lane64(int64_t x, int l)
@@ -329,42 +329,65 @@ __device__ __forceinline__ int64_t read_lane64(int64_t x, int l)
     return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)x >> 32), l) << 32) | lo);
 }
 
-// The cut before span `span` of `spans` (or the call's end), found by a wave
+// The cut before span `span` of `spans` (or the call's end), found by a wave. kFew: where two tiles to a span are enough for
+// the whole call, what an item costs beside its tiles is left out, so that the tiles spread over as many work-groups as they
+// can (8-bit pages, 20 heads of 128: 3 x 5 .. 40 queries behind 200 positions 23 us, with it 26; 32 behind 200 18 and 22, behind 1000 25 and 24)
+template <bool kFew = false>
 __device__ __forceinline__ PromptCut prompt_cut(const PrefillArgs& a, int spans, int span)
 {
     const int lane = threadIdx.x & 63;
+    int over = kOver;
     int64_t own = 0, sum = 0;
-    int most = 0;
+    int most = 0, blocks = 0;
     for (int b = lane; b < a.B; b += kWave)
     {
         int m;
         own = prompt_work(a, b, m);
         sum += own;
         most = max(most, m);
+        if constexpr (kFew)
+        {
+            PrefillSeq<true> q;
+            if (packed_seq(a, b, q) && q.n_ > 0) blocks += prompt_blocks(a, q.n_);
+        }
     }
     for (int off = 1; off < min(a.B, kWave); off <<= 1)
     {
         sum += __shfl_xor(sum, off, kWave);
         most = max(most, __shfl_xor(most, off, kWave));
+        if constexpr (kFew) blocks += __shfl_xor(blocks, off, kWave);
     }
-    const int64_t head = read_lane64(sum, 0), total = head * (a.Hkv * a.groups);  // tiles of a head group, of all
+    int64_t head = read_lane64(sum, 0);  // tiles of a head group
+    if constexpr (kFew)
+    {
+        const int64_t bare = head - (int64_t)kOver * __builtin_amdgcn_readfirstlane(blocks);
+        if (bare * (a.Hkv * a.groups) <= (int64_t)kSpanMin * spans)
+        {
+            over = 0;
+            head = bare;
+            int m;
+            if (a.B <= kWave) own = prompt_work(a, lane, m, 0);
+        }
+    }
+    const int64_t total = head * (a.Hkv * a.groups);  // of all
     most = __builtin_amdgcn_readfirstlane(most);
-    int64_t per = (total + spans - 1) / spans;
+    const bool small = total < 0x7FFFFFFF - spans;  // (a 64-bit division is a hundred instructions)
+    int64_t per = small ? (int64_t)((uint32_t)((int)total + spans - 1) / (uint32_t)spans) : (total + spans - 1) / spans;
     int snap = 1 << 30;
     if (most > kShort)
     {
-        per = max(per, (int64_t)max(kSpanMin + kOver, (most + kOver) / 32));  // at most about 32 spans to an item
+        per = max(per, (int64_t)max(kSpanMin + over, (most + over) / 32));  // at most about 32 spans to an item
         snap = kSnap;
     }
     // where tile x of the call lies
     const int64_t x = span * per;
     if (x >= total) return {a.Hkv * a.groups, 0, 0, 0};
-    const int gh = (int)(x / head);
+    const int gh = small ? (int)((uint32_t)x / (uint32_t)head) : (int)(x / head);
     int64_t y = x - gh * head;
     for (int b0 = 0; b0 < a.B; b0 += kWave)
     {
         int m;
-        if (a.B > kWave) own = prompt_work(a, b0 + lane, m);
+        if (a.B > kWave) own = prompt_work(a, b0 + lane, m, over);
         int64_t incl = own;
         const int live = min(a.B - b0, kWave);
         for (int off = 1; off < live; off <<= 1)
@@ -387,13 +410,13 @@ __device__ __forceinline__ PromptCut prompt_cut(const PrefillArgs& a, int spans,
         for (int n = prompt_blocks(a, q.n_); n > 1;)
         {
             const int step = (n + kWave - 1) / kWave;
-            const bool at_or_before = lane * step < n && prompt_before(a, q, qb + lane * step) <= y;
+            const bool at_or_before = lane * step < n && prompt_before(a, q, qb + lane * step, over) <= y;
             const int k = step * (__builtin_popcountll(__builtin_amdgcn_ballot_w64(at_or_before)) - 1);
             qb += k;
             n = min(step, n - k);
         }
         const int tiles = prompt_tiles(a, q, qb);
-        int t = (int)(y - prompt_before(a, q, qb)) - kOver;
+        int t = (int)(y - prompt_before(a, q, qb, over)) - over;
         if (t < snap) t = 0;
         else if (tiles - t < snap) return {gh, b, qb + 1, 0};
         return {gh, b, qb, t};
@@ -433,12 +456,11 @@ __device__ __forceinline__ PromptCut* prompt_cuts(const PrefillArgs& a, int span
 }
 
 // The items that several spans share: work-group g joins the one that the cut before span g is the first to
-// fall into, from its records: sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, 16 dimensions of its 256 queries.
+// fall into, from its records: sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, N dimensions of its 256 queries.
 // Span g - 1 wrote slot 1, those from g on that begin within the item slot 0: fewer than 64 (prompt_cut's per).
-template <int DK>
+template <int DK, int N = 16, int U = 1>
 __global__ __launch_bounds__(32 * kPWaves) void k_prompt_join(PrefillArgs a)
 {
-    constexpr int N = 16;
     const int g = blockIdx.x + 1, d0 = blockIdx.y * N, row = threadIdx.x, lane = row & 63;
     const PromptCut* const cuts = prompt_cuts<DK>(a, a.spans);
     const PromptCut at = cuts[g], last = cuts[g - 1], later = cuts[min(g + lane, a.spans - 1)];
@@ -448,25 +470,37 @@ __global__ __launch_bounds__(32 * kPWaves) void k_prompt_join(PrefillArgs a)
     PrefillSeq<true> q;
     packed_seq(a, at.b, q);
     const int wave = row >> 5, qt = at.qb * kPQ * (kPWaves / a.R) + wave / a.R * kPQ + (row & 31);
+    if (qt >= q.n_) return;
     float top = -__builtin_inff(), den = 0.0f, y[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) y[i] = 0.0f;
-    for (int s = 0; s < n; ++s)
+    // (the records of U spans on their way together, joined in their order: 32 records 9.7 us with 2, 12.4 one by one)
+    for (int s0 = 0; s0 < n; s0 += U)
     {
-        const float* rec = prompt_record<DK>(a, g - 1 + s, s == 0 ? 1 : 0) + row;
-        float x[N];
+        float x[U][N], m[U], l[U];
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = rec[(size_t)(d0 + i) * (32 * kPWaves)];
-        const float m = rec[(size_t)DK * (32 * kPWaves)], l = rec[(size_t)(DK + 1) * (32 * kPWaves)];
-        const float to = fmaxf(top, m);
-        const float old = top == to ? 1.0f : __builtin_amdgcn_exp2f(top - to);
-        const float now = m == to ? 1.0f : __builtin_amdgcn_exp2f(m - to);
-        den = __builtin_fmaf(l, now, den * old);
+        for (int u = 0; u < U; ++u)
+        {
+            const int s = min(s0 + u, n - 1);
+            const float* rec = prompt_record<DK>(a, g - 1 + s, s == 0 ? 1 : 0) + row;
 #pragma unroll
-        for (int i = 0; i < N; ++i) y[i] = __builtin_fmaf(x[i], now, y[i] * old);
-        top = to;
+            for (int i = 0; i < N; ++i) x[u][i] = rec[(size_t)(d0 + i) * (32 * kPWaves)];
+            m[u] = rec[(size_t)DK * (32 * kPWaves)], l[u] = rec[(size_t)(DK + 1) * (32 * kPWaves)];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+        {
+            // (selections, not a branch, which the loads would be moved behind)
+            const bool there = u == 0 || s0 + u < n;
+            const float to = fmaxf(top, m[u]);
+            const float old = top == to ? 1.0f : __builtin_amdgcn_exp2f(top - to);
+            const float now = m[u] == to ? 1.0f : __builtin_amdgcn_exp2f(m[u] - to);
+            den = there ? __builtin_fmaf(l[u], now, den * old) : den;
+#pragma unroll
+            for (int i = 0; i < N; ++i) y[i] = there ? __builtin_fmaf(x[u][i], now, y[i] * old) : y[i];
+            top = there ? to : top;
+        }
     }
-    if (qt >= q.n_) return;
     float* out = a.out + (size_t)((at.gh * a.R + wave % a.R) * DK + d0) * (size_t)a.M + (size_t)(q.col0_ + qt);
 #pragma unroll
     for (int i = 0; i < N; ++i) out[(size_t)i * (size_t)a.M] = den == 0.0f ? 0.0f : y[i] / den;

@@ -439,6 +439,43 @@ def test_prompt(ctx, nnhip, case):
     prompt_case(ctx, nnhip, **case)
 
 
+@pytest.mark.parametrize("case", [
+    dict(lens=[1, 32, 33, 64], pos0=[600, 1000, 90, 64], H=20, Hkv=5, dk=128, page=64, block=32, stride=13),
+    dict(lens=[20], pos0=[3000], H=4, Hkv=1, dk=128, page=32, block=16, cap=20.0, stride=6),
+    dict(lens=[64, 65, 3], pos0=[0, 333, 2000], H=16, Hkv=8, dk=128, page=16, block=16, rope=False, stride=21),
+    dict(lens=[128, 129, 200, 2], pos0=[100, 0, 31, 700], H=4, Hkv=4, dk=64, page=64, block=64, cap=5.0, slopes=True,
+         prefix=[150, 129, 0, 300], distance=True, stride=29),
+    dict(lens=[30, 10], pos0=[0, 40], H=2, Hkv=2, dk=64, page=16, block=16, slopes=True, prefix=[30, 45], stride=4),
+])
+def test_prompt_few_queries(ctx, nnhip, case):
+    """At most half of a work-group's queries: its waves share the keys."""
+    prompt_case(ctx, nnhip, **case)
+
+
+def test_prompt_few_queries_edges(ctx, nnhip):
+    """Scales that differ by any factor from block to block, infinite ones in sight and behind, zeros, over the waves' halves."""
+    base = dict(lens=[20, 9], pos0=[200, 330], H=4, Hkv=1, dk=128, page=32, block=16, stride=3)
+
+    def sizes(c, q):
+        for b, n in ((0, 220), (1, 339)):
+            for i in range(-(-n // 16)):
+                at = (c.table[b, i // 2], slice(None), i % 2)
+                c.scales["v"][at] *= F32(2.0 ** (30 if i % 4 == 1 else -30 if i % 4 == 2 else 0))
+                c.scales["k"][at] *= F32(2.0 ** (1 if i % 3 else -10))
+
+    prompt_case(ctx, nnhip, **base, edit=sizes)
+
+    def odd(c, q):
+        c.scales["v"][c.table[0, 6], 0, 1] = np.inf   # positions 208 .. 223: of some queries
+        c.scales["k"][c.table[1, 10], 0, 1] = np.nan  # 336 .. 351
+        for i in range(0, 10, 2):
+            c.scales["v"][c.table[1, i], 0] = 0.0
+            c.codes["v"][c.table[1, i]] = 0
+        q[25, 2, 7] = np.inf
+
+    prompt_case(ctx, nnhip, **base, edit=odd)
+
+
 def test_prompt_edges(ctx, nnhip):
     base = dict(lens=[60, 50], pos0=[0, 100], H=4, Hkv=2, dk=64, page=16, block=16, rope=False)
 
