@@ -1118,12 +1118,17 @@ __global__ __launch_bounds__(64 * W) void k_pages_attn_i8(PagesArgs a, PoolsI8 p
     }
 }
 
-// A sequence by one work-group of eight waves up to this many positions: no records, and no join
+// A sequence by one work-group, up to so many positions: no records, and no join. Of eight waves from 256 positions on
+// (four of dk = 256, whose tile takes half of a SIMD's registers). With the token read back, alone and split, us: 16 x 400 of
+// 20 heads over 5 of 128 13.4 and 17.1, 16 x 900 17.5 and 19.1, 64 x 900 of 16 over 2 of 64 16.9 and 21.9, 16 x 1500 20.1 and 20.4,
+// 16 x 2500 25.9 and 24.7, 1 x 2000 of 8 over 1 22 and 17. Of 256, which fall behind sooner where there are few: 16 x 400 of 8 over 1 18.9 and 20.4
+// (eight waves 23.2), 16 x 1000 26.1 and 21.2, 64 x 1000 28.8 and 39.5.
 constexpr size_t kI8Solo = 1024;
 
 inline PagesCut cut_i8(size_t B, size_t Hkv, size_t R, size_t dk, size_t len_bound, size_t num_cus)
 {
-    return len_bound <= kI8Solo ? PagesCut{round_up(len_bound, kI8Tile), 1, 0} : pages_cut(B, Hkv, R, dk, len_bound, num_cus);
+    const bool few = dk == 256 && 2 * B * Hkv * pages_groups(R, dk) < num_cus;
+    return len_bound <= (few ? kI8Solo / 2 : kI8Solo) ? PagesCut{round_up(len_bound, kI8Tile), 1, 0} : pages_cut(B, Hkv, R, dk, len_bound, num_cus);
 }
 
 template <int DK, int NS>
@@ -1140,8 +1145,9 @@ hipError_t launch_attn_i8(hipStream_t st, const PagesArgs& a, const PoolsI8& poo
     const dim3 grid((unsigned)(pages_items(a.B, a.len_bound, a.chunk, a.even) * a.Hkv * a.groups));
     if (a.nchunk == 1)
     {
+        constexpr int W = DK == 256 ? 4 : 8;
         if (a.len_bound <= 4 * kI8Tile) k_pages_attn_i8<DK, NS, 4, true><<<grid, 256, 0, st>>>(a, pools, append);
-        else k_pages_attn_i8<DK, NS, 8, true><<<grid, 512, 0, st>>>(a, pools, append);
+        else k_pages_attn_i8<DK, NS, W, true><<<grid, 64 * W, 0, st>>>(a, pools, append);
         return hipGetLastError();
     }
     k_pages_attn_i8<DK, NS, 4, false><<<grid, 256, 0, st>>>(a, pools, append);

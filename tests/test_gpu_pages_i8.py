@@ -295,6 +295,8 @@ def own_bound(q, K, V, scale, n, weights):
     dict(B=2, H=24, Hkv=2, dk=128, page=64, block=32, pos=[129, 400], rope=False),
     dict(B=2, H=16, Hkv=1, dk=256, page=64, block=32, pos=[129, 255]),
     dict(B=3, H=6, Hkv=2, dk=64, page=1024, block=64, pos=[5, 2000, 1023]),
+    dict(B=2, H=4, Hkv=2, dk=256, page=32, block=16, pos=[300, 511], cap=30.0),
+    dict(B=33, H=4, Hkv=4, dk=256, page=128, block=64, pos=[30 * b + 3 for b in range(33)]),
     dict(B=2, H=4, Hkv=1, dk=128, page=64, block=64, pos=[5000, 12345]),
     dict(B=17, H=4, Hkv=2, dk=64, page=16, block=16, pos=list(range(17)), slopes=True),
     dict(B=3, H=20, Hkv=5, dk=128, page=64, block=32, pos=[99, 300, -1], append=False),
