@@ -762,7 +762,6 @@ __global__ __launch_bounds__(64 * W) void k_pages_attn_i8(PagesArgs a, PoolsI8 p
     constexpr int HALF = DK / 2, RT = 4 * NS, KC = DK / 64, ND = DK / 16, T = 64 * W;
     constexpr int QI = (RT * HALF + T - 1) / T;  // query pairs per thread
     constexpr int kDigits = DK + 4;              // words of a head's digits in LDS
-    constexpr bool kAhead = DK * NS <= 128;      // the next tile on its way during a tile (its registers are there)
     __shared__ __align__(16) uint32_t dig_s[RT * kDigits];
     __shared__ uint32_t top_s[RT];               // each head's largest element (bits)
     __shared__ __align__(16) uint8_t w_s[W][NS][16 * kI8Pitch];
@@ -920,7 +919,7 @@ __global__ __launch_bounds__(64 * W) void k_pages_attn_i8(PagesArgs a, PoolsI8 p
     }
     for (int t = first; t <= last; t += W * kI8Tile)
     {
-        if (!kAhead && t != first) load(t);
+        if (t != first) load(t);  // (the next tile's on its way during a tile was up to 4 % slower, its registers there or not)
         if (own && t == new_tile)
         {
             if (done.regrown)
@@ -949,19 +948,10 @@ __global__ __launch_bounds__(64 * W) void k_pages_attn_i8(PagesArgs a, PoolsI8 p
             const int mine = t + 16 * (lane & 3);
             if (mine >> pools.bshift == p >> pools.bshift && mine <= last) ks = done.s[0], vs = done.s[1];
         }
-        u32x4 k_now[4][KC], v_now[ND];
-        const float ks_now = ks, vs_now = vs;
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-            for (int i = 0; i < KC; ++i) k_now[n][i] = kf[n][i];
-#pragma unroll
-        for (int i = 0; i < ND; ++i) v_now[i] = vf[i];
-        if (kAhead && t + W * kI8Tile <= last) load(t + W * kI8Tile);
         // a power of two above the tile's largest scale of values
-        float top_v = fmaxf(vs_now, dpp<kDppXor1>(vs_now));
+        float top_v = fmaxf(vs, dpp<kDppXor1>(vs));
         top_v = fmaxf(top_v, dpp<kDppXor2>(top_v));
-        const bool odd = __builtin_amdgcn_ballot_w64(!(fabsf(vs_now) < 0x1p125f)) != 0;  // (no write makes one from there on)
+        const bool odd = __builtin_amdgcn_ballot_w64(!(fabsf(vs) < 0x1p125f)) != 0;  // (no write makes one from there on)
         const int ev = min(max(__builtin_amdgcn_readfirstlane((int)(__builtin_bit_cast(uint32_t, top_v) >> 23)), 31), 252);
         const float down = odd ? 0.0f : pow2_field(253 - ev);                  // 2^(126 - ev) times a scale is at most 1
         const float back = odd ? __builtin_nanf("") : pow2_field(ev - 29);     // 2^(ev - 126 - 30)
@@ -969,8 +959,8 @@ __global__ __launch_bounds__(64 * W) void k_pages_attn_i8(PagesArgs a, PoolsI8 p
 #pragma unroll
         for (int n = 0; n < 4; ++n)
         {
-            kg[n] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks_now), n));
-            vg[n] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs_now), n)) * down;
+            kg[n] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), n));
+            vg[n] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs), n)) * down;
         }
         const bool part = t + kI8Tile - 1 > last;
 #pragma unroll
@@ -984,7 +974,7 @@ __global__ __launch_bounds__(64 * W) void k_pages_attn_i8(PagesArgs a, PoolsI8 p
                 v4i d = v4i{};
 #pragma unroll
                 for (int i = 0; i < KC; ++i)
-                    d = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, qd[s][i]), __builtin_bit_cast(v4i, k_now[n][i]), d, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, qd[s][i]), __builtin_bit_cast(v4i, kf[n][i]), d, 0, 0, 0);
                 const int hi = (int)((uint32_t)d[3] << 8) + d[2], lo = (int)((uint32_t)d[1] << 8) + d[0];
                 float f = unit[s] * kg[n];
                 f = kg[n] < __builtin_inff() && f == f ? held(f) : __builtin_nanf("");
@@ -1041,7 +1031,7 @@ __global__ __launch_bounds__(64 * W) void k_pages_attn_i8(PagesArgs a, PoolsI8 p
 #pragma unroll
             for (int i = 0; i < ND; ++i)
             {
-                const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, v_now[i]), wd, v4i{}, 0, 0, 0);
+                const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, vf[i]), wd, v4i{}, 0, 0, 0);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[s][i][e] = __builtin_fmaf((float)d[e], back, acc[s][i][e]);
             }
@@ -1200,8 +1190,9 @@ hipError_t launch_pages_fill_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, con
 {
     const FillI8Args a{k, v, cu, pos0, cosT, sinT, pools_of(kv), kv.table, (int)M, (int)B, (int)kv.Hkv, log2_of(kv.page_size),
                        (int)kv.table_stride, (int)kv.num_pages, (int)limit};
-    // sequences of 64 tokens or more on average: windows of their positions, of which there are at most M / 64 + 2 B
-    if (M >= kPfTok * B)
+    // sequences of 128 tokens or more on average: windows of their positions, of which there are at most M / 64 + 2 B (by
+    // windows and by columns, with the values read back, us: 16 x 64 tokens of 5 heads of 128 15.0 and 13.4, x 128 18.9 and 18.5, x 300 22.7 and 27.8)
+    if (M >= 2 * kPfTok * B)
     {
         const dim3 grid((unsigned)(M / kPfTok + 2 * B), (unsigned)kv.Hkv, 2);
         if (kv.dk == 64) k_windows_fill_i8<64><<<grid, 256, 0, st>>>(a);
@@ -1223,7 +1214,8 @@ hipError_t launch_pages_read_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, siz
 {
     ReadI8Args a{pools_of(kv), kv.table, cu, pos0, k, v, (int)M, (int)B, (int)kv.Hkv, log2_of(kv.page_size),
                        (int)kv.table_stride, (int)kv.num_pages, (int)(kv.table_stride * kv.page_size), 1};
-    // few columns: a head's dimensions shared by more work-groups, which do not wait 16 after 16 of them
+    // few columns: a head's dimensions shared by more work-groups, which do not wait 16 after 16 of them (a block of 32
+    // behind 16 sequences: 4.4 us, by whole heads 9.7; from two work-groups to a CU on nothing is gained)
     const size_t blocks = ceil_div(M, kReadCols);
     while ((size_t)a.parts < kv.dk / 16 && blocks * kv.Hkv * 2 * (size_t)a.parts < 2 * num_cus) a.parts *= 2;
     const dim3 grid((unsigned)blocks, (unsigned)(kv.Hkv * (size_t)a.parts), 2);

@@ -123,7 +123,8 @@ def fill(ctx, cache, host_cache, k, v, lens, pos0, tables, skip=0):
 @pytest.mark.parametrize("page,block,lens,pos0", [
     (16, 16, [1], [0]), (16, 16, [100], [0]), (64, 64, [64, 64], [0, 0]), (64, 64, [200, 1, 0, 63, 65], [0, 5, 9, 1, 130]),
     (32, 16, [7, 90, 33], [3, 17, 0]), (128, 32, [1] * 70, list(range(70))), (1024, 64, [130, 127], [63, 64]),
-    (64, 32, [0, 0, 300], [0, 1, 31])])
+    (64, 32, [0, 0, 300], [0, 1, 31]), (16, 16, [150], [13]), (64, 64, [400, 1, 0, 203, 210], [0, 5, 9, 1, 130]),
+    (32, 32, [257], [49]), (128, 32, [0, 0, 500], [0, 1, 31])])
 def test_fill(ctx, nnhip, dk, page, block, lens, pos0):
     print(f"fill dk={dk} page={page} block={block} lens={lens[:6]} pos0={pos0[:6]}", flush=True)
     rng = np.random.default_rng(dk + page + block + len(lens))
@@ -219,6 +220,34 @@ def test_fill_leaves_out(ctx, nnhip):
     assert np.all(got[:, 80:] == 7.0) and np.isnan(got[:, 28:30]).all()           # positions 48, 49: past the table
     assert np.isnan(got[:, 46:62]).all() and np.isnan(got[:, 78:80]).all()        # the bad page; past the table
     assert np.isfinite(got[:, :26]).all() and np.isfinite(got[:, 30:46]).all()
+
+
+@pytest.mark.parametrize("dk,block", [(64, 16), (128, 64), (256, 32)])
+def test_fill_alone_and_among_empty_sequences(ctx, nnhip, dk, block):
+    """A long prompt behind columns of no one, past a bad page and the end of the rope tables, onto older tokens that it
+    outgrows: by windows of positions alone, by columns among empty sequences, the same bits, and the definition's."""
+    rng = np.random.default_rng(8 + dk)
+    Hkv, page, M, p0, n, rows = 2, 64, 330, 37, 300, 320
+    k, v = (tokens_of(rng, M, Hkv, dk) * F32(3.0) for _ in range(2))
+    old = [tokens_of(rng, p0, Hkv, dk) for _ in range(2)]
+    cos, sin = nnhip.rope_table(dk, rows)
+    found = []
+    for empty in (0, 5):
+        c = CacheI8(np.random.default_rng(9), [p0 + n], Hkv, page, dk, block)
+        c.put(0, 0, *old)
+        bad = np.repeat(c.table, 1 + empty, 0)
+        bad[0, 2] = -1  # positions 128 .. 191
+        cache = nnhip.KVPagesI8(*(getattr(c.on_device(nnhip), x) for x in ("k", "v", "k_scale", "v_scale")), dev(bad))
+        cu = dev(np.array([20] + [20 + n] * (1 + empty), np.int32))
+        ctx.kv_pages_fill(cache, dev(columns(k)), dev(columns(v)), cu, pos0=dev(np.array([p0] + [0] * empty, np.int32)),
+                          cos=dev(cos), sin=dev(sin))
+        turned = np.stack([rotate(k[20 + i], cos, sin, p0 + i) for i in range(rows - p0)])
+        c.put(0, p0, turned[:128 - p0], v[20:20 + 128 - p0])
+        c.put(0, 192, turned[192 - p0:], v[20 + 192 - p0:20 + rows - p0])
+        c.check(cache)
+        found.append([host(x) for x in (cache.k, cache.v, cache.k_scale, cache.v_scale)])
+    for a, b in zip(*found):
+        assert np.array_equal(a.view(np.uint8), b.view(np.uint8))
 
 
 def check_decode(ctx, nnhip, B, H, Hkv, dk, page, block, pos, rope=True, cap=0.0, slopes=False, tokens=True, seed=0,
