@@ -151,10 +151,10 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
     // the unit of O for a tile whose scales are posted, where it was `unit` before and `top` at most so far: no more than
     // 2^80 below that, so that O stays finite
     auto next_unit = [&](int kb, int unit, int& top) {
-        int field = 0;
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-            field = max(field, scale_field((uint32_t)__builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, slot_of(kb)[4 + n]))));
+        int field = scale_field(__builtin_bit_cast(uint32_t, slot_of(kb)[4 + (lane & 3)]));
+        field = max(field, __builtin_amdgcn_update_dpp(0, field, 0xB1, 0xF, 0xF, true));  // lane ^ 1
+        field = max(field, __builtin_amdgcn_update_dpp(0, field, 0x4E, 0xF, 0xF, true));  // lane ^ 2
+        field = __builtin_amdgcn_readfirstlane(field);
         if (field == 0) return unit;
         top = max(top, field);
         return field > unit + kI8Near || field < unit - kI8Near ? max(field, top - 80) : unit;
@@ -277,6 +277,43 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
     int unit_top = 0, unit = next_unit(k0, 127, unit_top);  // O is in units of 2^(unit - 127)
     convert(k0, 0, unit);
     if (k0 + 2 < k1) load_raw(k0 + 2);
+    // scores s of a half, with their keys' scales: capped, and their bias from the half's first key on
+    auto shape = [&](v16f& s, float k0, float k1) {
+        float kf[2] = {k0, k1};
+                        if (a.cap2 > 0.0f)
+                        {
+                            // scores rarely reach the cap: a polynomial of few terms where none does
+                            float top = 0.0f;  // (a NaN does not show, and stays one in each form)
+#pragma unroll
+                            for (int v = 0; v < 16; ++v)
+                            {
+                                s[v] *= kf[v >> 3];
+                                top = fmaxf(top, fabsf(s[v]));
+                            }
+                            if (__builtin_amdgcn_ballot_w64(top > 0.25f) == 0)
+                            {
+#pragma unroll
+                                for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(tanh_below_quarter(s[v]), a.cap2, steps[v]);
+                            }
+                            else if (__builtin_amdgcn_ballot_w64(top > 1.0f) == 0)
+                            {
+#pragma unroll
+                                for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(tanh_below1(s[v]), a.cap2, steps[v]);
+                            }
+                            else
+                            {
+#pragma unroll
+                                for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(tanh_any(s[v]), a.cap2, steps[v]);
+                            }
+                        }
+                        else
+                        {
+                            // (an opaque factor: or this is computed whether the branch is taken or not)
+                            asm volatile("" : "+v"(kf[0]), "+v"(kf[1]));
+#pragma unroll
+                            for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(s[v], kf[v >> 3], steps[v]);
+                        }
+    };
     const uint32_t k_at = (uint32_t)(l32 * Tile::kKPitch + 16 * h), v_at = (uint32_t)(Tile::kV + l32 * Tile::kVPitch + 16 * h);
     int par = 0;
     float by = 1.0f;  // from the last tile's unit to this one's
@@ -297,8 +334,118 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
         }
         const uint8_t* const buf = smem + par * Tile::kBuf;
         const float* const ts4 = slot_of(kb);
+        // Where every query sees the whole tile, no unit moves and every scale counts: both halves at once, the second's scores beside
+        // the first one's maximum, its weights beside the first one's products with the values
+        bool whole = !shared && w.live && kb + 1 < k1 && (kb + 2) * kPK - 1 <= (kShaped ? seq.pos0(a) + w.t0 : seq.from(a, w)) &&
+                     __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, by)) == 0x3F800000;
+        float lv4[4];
+        // (keys two steps ahead of their products, of both halves in turn)
+        auto keys = [&](int half, int c) { return *reinterpret_cast<const v8h*>(buf + k_at + half * kPK * Tile::kKPitch + 32 * c); };
+        constexpr int kDeep = 2;
+        v8h k[2][kDeep];
+        if (whole)
+        {
+#pragma unroll
+            for (int i = 0; i < 2 * kDeep; ++i) k[i & 1][i >> 1] = keys(i & 1, i >> 1);
+            const float scale = ts4[4 + (lane & 3)];
+            const int e = scale_field(__builtin_bit_cast(uint32_t, scale));
+            const float lv = __builtin_amdgcn_logf(scale) - (float)(e - 127);
+            whole = __builtin_amdgcn_ballot_w64(e == 0 || e - unit < kI8Low || e - unit > kI8Near) == 0;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) lv4[t] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, lv), t));
+        }
+        if (whole)
+        {
+            v16f s[2] = {v16f{}, v16f{}};
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+            {
+                const v8h x = k[0][c % kDeep], y = k[1][c % kDeep];
+                if (c + kDeep < NC) k[0][c % kDeep] = keys(0, c + kDeep), k[1][c % kDeep] = keys(1, c + kDeep);
+                s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ql[c], s[0], 0, 0, 0);
+                s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, ql[c], s[1], 0, 0, 0);
+                s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[c], s[0], 0, 0, 0);
+                s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, qh[c], s[1], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            float kf[4], away[2] = {0.0f, 0.0f}, top = -__builtin_inff();
+#pragma unroll
+            for (int t = 0; t < 4; ++t) kf[t] = f * ts4[t];
+            if constexpr (kShaped)
+            {
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+                {
+                    shape(s[half], kf[2 * half], kf[2 * half + 1]);
+                    away[half] = slope2 * (float)((kb + half) * kPK + 4 * h - w.qpos);
+                    kf[2 * half] = kf[2 * half + 1] = 1.0f;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+            {
+                float most = s[t >> 1][8 * (t & 1)];
+#pragma unroll
+                for (int v = 1; v < 8; ++v) most = fmaxf(most, s[t >> 1][8 * (t & 1) + v]);
+                top = fmaxf(top, kShaped ? most + away[t >> 1] : most * kf[t]);
+            }
+            const float mx = __builtin_ceilf(max_halves(top));
+            const bool grown = mx > m_ref + kPLazy;
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(grown) != 0, 0))
+            {
+                const float m_new = grown ? mx : m_ref;
+                float corr = grown ? __builtin_amdgcn_exp2f(m_ref - m_new) : 1.0f;
+                asm volatile("" : "+v"(corr));
+                l_run *= corr;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) o[d][v] *= corr;
+                m_ref = m_new;
+            }
+            float base[2];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) base[half] = kI8Up + (m_ref == -__builtin_inff() ? 0.0f : away[half] - m_ref);
+            // weights of group t + 1 between the products of group t: a pair of keys beside 8 / ND products
+            v8h pa[2], pb[2];
+            float sum = 0.0f;
+            auto pair = [&](int t, int v) {
+                const float off = base[t >> 1] + lv4[t];
+                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t >> 1][8 * (t & 1) + v], kf[t], off));
+                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t >> 1][8 * (t & 1) + v + 1], kf[t], off));
+                sum += p0;
+                sum += p1;
+                v2h x, y;
+                split2(p0, p1, x, y);
+                pa[t & 1][v] = x[0], pa[t & 1][v + 1] = x[1];
+                pb[t & 1][v] = y[0], pb[t & 1][v + 1] = y[1];
+                if (v == 6)
+                {
+                    l_run = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-lv4[t]), l_run);
+                    sum = 0.0f;
+                }
+            };
+            auto values = [&](int i) { return *reinterpret_cast<const v8h*>(buf + v_at + 32 * (i % ND) * Tile::kVPitch + 32 * (i / ND)); };
+            v8h x = values(0);
+#pragma unroll
+            for (int v = 0; v < 8; v += 2) pair(0, v);
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+                {
+                    const v8h y = x;
+                    if (t * ND + d + 1 < 4 * ND) x = values(t * ND + d + 1);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, pb[t & 1], o[d], 0, 0, 0);
+                    if (t < 3)
+#pragma unroll
+                        for (int v = 8 / ND * d; v < 8 / ND * (d + 1); v += 2) pair(t + 1, v);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, pa[t & 1], o[d], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        }
 #pragma unroll 1
-        for (int half = 0; half < 2; ++half)
+        for (int half = whole ? 2 : 0; half < 2; ++half)
         {
             const int key0 = (kb + half) * kPK;
             if (!w.live || kb + half >= k1 || key0 > seq.to(a, w) || (shared && half != (int)second)) continue;
@@ -321,39 +468,7 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
             float away = 0.0f;  // the bias of the half's first key, the steps from there apart
             if constexpr (kShaped)
             {
-                if (a.cap2 > 0.0f)
-                {
-                    // scores rarely reach the cap: a polynomial of few terms where none does
-                    float top = 0.0f;  // (a NaN does not show, and stays one in each form)
-#pragma unroll
-                    for (int v = 0; v < 16; ++v)
-                    {
-                        s[v] *= kf[v >> 3];
-                        top = fmaxf(top, fabsf(s[v]));
-                    }
-                    if (__builtin_amdgcn_ballot_w64(top > 0.25f) == 0)
-                    {
-#pragma unroll
-                        for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(tanh_below_quarter(s[v]), a.cap2, steps[v]);
-                    }
-                    else if (__builtin_amdgcn_ballot_w64(top > 1.0f) == 0)
-                    {
-#pragma unroll
-                        for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(tanh_below1(s[v]), a.cap2, steps[v]);
-                    }
-                    else
-                    {
-#pragma unroll
-                        for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(tanh_any(s[v]), a.cap2, steps[v]);
-                    }
-                }
-                else
-                {
-                    // (an opaque factor: or this is computed whether the branch is taken or not)
-                    asm volatile("" : "+v"(kf[0]), "+v"(kf[1]));
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(s[v], kf[v >> 3], steps[v]);
-                }
+                shape(s, kf[0], kf[1]);
                 const float first = (float)(key0 + 4 * h - w.qpos);
                 away = slope2 * first;
                 if (distance && key0 + kPK - 1 > seq.pos0(a) + w.t0)
