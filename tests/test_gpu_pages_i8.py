@@ -477,6 +477,8 @@ def test_prompt(ctx, nnhip, case):
     dict(lens=[128, 129, 200, 2], pos0=[100, 0, 31, 700], H=4, Hkv=4, dk=64, page=64, block=64, cap=5.0, slopes=True,
          prefix=[150, 129, 0, 300], distance=True, stride=29),
     dict(lens=[30, 10], pos0=[0, 40], H=2, Hkv=2, dk=64, page=16, block=16, slopes=True, prefix=[30, 45], stride=4),
+    dict(lens=[b % 4 for b in range(70)], pos0=[37 * b % 190 for b in range(70)], H=4, Hkv=1, dk=64, page=32, block=32),
+    dict(lens=[256], pos0=[64], H=8, Hkv=1, dk=128, page=64, block=64, cap=30.0, slopes=True, stride=51),
 ])
 def test_prompt_few_queries(ctx, nnhip, case):
     """At most half of a work-group's queries: its waves share the keys."""
