@@ -387,7 +387,7 @@ __device__ __forceinline__ FillWindow find_window(const FillI8Args& a, int item)
 // turned 4 x 4 between the lanes of a quad, which leaves words of 4 positions for LDS. 16 x 1111 .. 2048 tokens of 5 heads of
 // 128: 52 us, 3.1 TB/s, bound by HBM and the f32 columns' runs of 256 bytes, which begin anywhere.
 template <int DK>
-__global__ __launch_bounds__(256) void k_windows_fill_i8(FillI8Args a)
+__global__ __launch_bounds__(256, DK == 256 ? 3 : 5) void k_windows_fill_i8(FillI8Args a)
 {
     constexpr int HALF = DK / 2, NP = DK / 8;  // pairs of a thread
     constexpr int kPitch = 80;                 // bytes of a dimension's 64 positions in LDS

@@ -669,13 +669,19 @@ __device__ __forceinline__ void prompt_items(const PrefillArgs& a, uint8_t* smem
     {
         // the span's two cuts by a wave each, while the others look for sequences that do not fit
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        PromptCut* const cuts = reinterpret_cast<PromptCut*>(smem);
+        struct Found
+        {
+            PromptCut cut;
+            PrefillSeq<true> seq;
+        };
+        Found* const cuts = reinterpret_cast<Found*>(smem);
         if (wave < 2)
         {
-            const PromptCut cut = prompt_cut<true>(a, a.spans, g + wave);
+            PrefillSeq<true> seq{};
+            const PromptCut cut = prompt_cut<true>(a, a.spans, g + wave, &seq);
             if ((threadIdx.x & 63) == 0)
             {
-                cuts[wave] = cut;
+                cuts[wave] = {cut, seq};
                 if (wave == 0) prompt_cuts<DK>(a, a.spans)[g] = cut;
             }
         }
@@ -683,8 +689,11 @@ __device__ __forceinline__ void prompt_items(const PrefillArgs& a, uint8_t* smem
             for (int b = g; b < a.B; b += a.spans)
                 if (PrefillSeq<true> any; !packed_seq(a, b, any)) store_nan<DK>(a, b, 0, a.H, (int)threadIdx.x - 2 * kWave, kPThreads - 2 * kWave);
         __syncthreads();
-        at = uniform(cuts[0]);
-        end = uniform(cuts[1]);
+        at = uniform(cuts[0].cut);
+        end = uniform(cuts[1].cut);
+        const PrefillSeq<true> q = cuts[0].seq;
+        it.seq = {__builtin_amdgcn_readfirstlane(q.n_), __builtin_amdgcn_readfirstlane(q.col0_), __builtin_amdgcn_readfirstlane(q.pos0_),
+                  __builtin_amdgcn_readfirstlane(q.pre)};
         __syncthreads();
     }
     else
@@ -698,7 +707,7 @@ __device__ __forceinline__ void prompt_items(const PrefillArgs& a, uint8_t* smem
         if (at.qb >= prompt_blocks(a, it.seq.n_)) return;
         end = {at.gh, at.b, at.qb + 1, 0};
     }
-    bool known = a.spans == 0;  // it.seq is at.b's
+    bool known = true;  // it.seq is at.b's
     while (cut_before(at, end))
     {
         // the next sequence with a block left
@@ -706,6 +715,7 @@ __device__ __forceinline__ void prompt_items(const PrefillArgs& a, uint8_t* smem
         if (!there || !(known || packed_seq(a, at.b, it.seq)) || at.qb >= prompt_blocks(a, it.seq.n_))
         {
             at = there ? PromptCut{at.gh, at.b + 1, 0, 0} : PromptCut{at.gh + 1, 0, 0, 0};
+            known = false;
             continue;
         }
         const int tiles = prompt_tiles(a, it.seq, at.qb), to = cut_same_item(at, end) ? end.t : tiles;
@@ -715,7 +725,7 @@ __device__ __forceinline__ void prompt_items(const PrefillArgs& a, uint8_t* smem
         it.qb = at.qb;
         float* rec = at.t == 0 && to == tiles ? nullptr : prompt_record<DK>(a, g, at.t > 0 ? 0 : 1);
         attend(it, at.t, to, rec);
-        known = false;
+        known = true;
         at = {at.gh, at.b, at.qb + 1, 0};
     }
 }

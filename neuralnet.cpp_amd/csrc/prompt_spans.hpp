@@ -332,13 +332,15 @@ __device__ __forceinline__ int64_t read_lane64(int64_t x, int l)
 // The cut before span `span` of `spans` (or the call's end), found by a wave. kFew: where two tiles to a span are enough for
 // the whole call, what an item costs beside its tiles is left out, so that the tiles spread over as many work-groups as they
 // can (8-bit pages, 20 heads of 128: 3 x 5 .. 40 queries behind 200 positions 23 us, with it 26; 32 behind 200 18 and 22, behind 1000 25 and 24)
+// found, if not null: the cut's sequence, where there is one
 template <bool kFew = false>
-__device__ __forceinline__ PromptCut prompt_cut(const PrefillArgs& a, int spans, int span)
+__device__ __forceinline__ PromptCut prompt_cut(const PrefillArgs& a, int spans, int span, PrefillSeq<true>* found = nullptr)
 {
     const int lane = threadIdx.x & 63;
     int over = kOver;
     int64_t own = 0, sum = 0;
     int most = 0, blocks = 0;
+    PrefillSeq<true> mine{};  // the lane's sequence, of up to 64
     for (int b = lane; b < a.B; b += kWave)
     {
         int m;
@@ -347,8 +349,7 @@ __device__ __forceinline__ PromptCut prompt_cut(const PrefillArgs& a, int spans,
         most = max(most, m);
         if constexpr (kFew)
         {
-            PrefillSeq<true> q;
-            if (packed_seq(a, b, q) && q.n_ > 0) blocks += prompt_blocks(a, q.n_);
+            if (packed_seq(a, b, mine) && mine.n_ > 0) blocks += prompt_blocks(a, mine.n_);
         }
     }
     for (int off = 1; off < min(a.B, kWave); off <<= 1)
@@ -404,7 +405,11 @@ __device__ __forceinline__ PromptCut prompt_cut(const PrefillArgs& a, int spans,
         const int l = __builtin_ctzll(here), b = b0 + l;
         y -= read_lane64(incl - own, l);
         PrefillSeq<true> q;
-        packed_seq(a, b, q);
+        if (kFew && a.B <= kWave)
+            q = {__builtin_amdgcn_readlane(mine.n_, l), __builtin_amdgcn_readlane(mine.col0_, l), __builtin_amdgcn_readlane(mine.pos0_, l),
+                 __builtin_amdgcn_readlane(mine.pre, l)};
+        else packed_seq(a, b, q);
+        if (found) *found = q;
         // the last block whose tiles begin at or before y: of 64 candidates at a time
         int qb = 0;
         for (int n = prompt_blocks(a, q.n_); n > 1;)
