@@ -509,6 +509,41 @@ def test_prompt_few_queries_edges(ctx, nnhip):
     prompt_case(ctx, nnhip, **base, edit=odd)
 
 
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("dk", [64, 128])
+def test_prompt_whole_tiles_edges(ctx, nnhip, dk, cap):
+    """Tiles that every query sees: infinities, NaN and zeros among queries and scales, scales that differ by any factor within
+    a tile and from tile to tile."""
+    base = dict(lens=[40, 33], pos0=[260, 192], H=8, Hkv=1, dk=dk, page=32, block=16, cap=cap, slopes=cap > 0, stride=5)
+
+    def odd(c, q):
+        c.scales["k"][c.table[0, 3], 0, 1] = np.inf   # positions 112 .. 127 of the first
+        c.codes["k"][c.table[0, 3], 0, 16:] = 0
+        q[45, 2, 7] = np.inf
+        q[60, 1, 0] = np.nan
+        q[40] = 0.0
+
+    prompt_case(ctx, nnhip, **base, edit=odd)
+
+    def values(c, q):
+        c.scales["v"][c.table[0, 1], 0, 0] = np.nan
+        for i in range(0, 6, 2):
+            c.scales["v"][c.table[1, i], 0] = 0.0
+            c.codes["v"][c.table[1, i]] = 0
+
+    prompt_case(ctx, nnhip, **base, edit=values)
+
+    def sizes(c, q):
+        for b, n in ((0, 300), (1, 225)):
+            for i in range(-(-n // 16)):
+                at = (c.table[b, i // 2], slice(None), i % 2)
+                c.scales["v"][at] *= F32(2.0 ** (0, 3, -7, 9, 20, -20, 1, 0, 40, 41, 39, 45)[i % 12])
+                c.scales["k"][at] *= F32(2.0 ** (1, 0, -10)[i % 3])
+        q[:20] *= F32(1e-30)
+
+    prompt_case(ctx, nnhip, **base, edit=sizes)
+
+
 def test_prompt_edges(ctx, nnhip):
     base = dict(lens=[60, 50], pos0=[0, 100], H=4, Hkv=2, dk=64, page=16, block=16, rope=False)
 
