@@ -20,7 +20,7 @@
 // Work-groups take equal spans of all tiles and join the items they share (prompt_spans.hpp).
 // 4 x 700 .. 1024 queries at 6144, 20 heads over 5 of 128: 432 us and 20 for the join, 1.06 PFLOP/s of products (a large
 // library product of f16: 1.15), bound by them and the softmax beside them, to which the f32 exponential and the weights' splitting
-// contribute most; 8 x 77 .. 1900 of 16 over 2 of 64, capped and biased: 66 and 9, bound by the VALU (25 instructions a score).
+// contribute most; 8 x 77 .. 1900 of 16 over 2 of 64, capped and biased: 61 and 9, bound by the VALU (25 instructions a score).
 // A query that holds an infinity or a NaN gets NaN, and so does one that sees a block whose scale is not finite.
 #include "prompt_spans.hpp"
 

@@ -285,6 +285,7 @@ struct PromptCut
     int gh, b, qb, t;
 };
 constexpr int kOver = 3, kSnap = 2, kShort = 4, kSpanMin = 2;
+constexpr int kOverI8 = 5;  // over 8-bit pages, whose tiles take less (8 x 77 .. 1900 of 64: 69 us, with 3 73, 8 75; 4 x 700 .. 1024 at 6144 435, 438, 436)
 
 __device__ __forceinline__ int prompt_blocks(const PrefillArgs& a, int n)
 {
@@ -337,14 +338,15 @@ template <bool kFew = false>
 __device__ __forceinline__ PromptCut prompt_cut(const PrefillArgs& a, int spans, int span, PrefillSeq<true>* found = nullptr)
 {
     const int lane = threadIdx.x & 63;
-    int over = kOver;
+    constexpr int kItem = kFew ? kOverI8 : kOver;
+    int over = kItem;
     int64_t own = 0, sum = 0;
     int most = 0, blocks = 0;
     PrefillSeq<true> mine{};  // the lane's sequence, of up to 64
     for (int b = lane; b < a.B; b += kWave)
     {
         int m;
-        own = prompt_work(a, b, m);
+        own = prompt_work(a, b, m, kItem);
         sum += own;
         most = max(most, m);
         if constexpr (kFew)
@@ -361,7 +363,7 @@ __device__ __forceinline__ PromptCut prompt_cut(const PrefillArgs& a, int spans,
     int64_t head = read_lane64(sum, 0);  // tiles of a head group
     if constexpr (kFew)
     {
-        const int64_t bare = head - (int64_t)kOver * __builtin_amdgcn_readfirstlane(blocks);
+        const int64_t bare = head - (int64_t)kItem * __builtin_amdgcn_readfirstlane(blocks);
         if (bare * (a.Hkv * a.groups) <= (int64_t)kSpanMin * spans)
         {
             over = 0;
@@ -377,7 +379,7 @@ __device__ __forceinline__ PromptCut prompt_cut(const PrefillArgs& a, int spans,
     int snap = 1 << 30;
     if (most > kShort)
     {
-        per = max(per, (int64_t)max(kSpanMin + over, (most + over) / 32));  // at most about 32 spans to an item
+        per = max(per, (int64_t)max(kSpanMin + min(over, kOver), (most + over) / 32));  // at most about 32 spans to an item
         snap = kSnap;
     }
     // where tile x of the call lies
