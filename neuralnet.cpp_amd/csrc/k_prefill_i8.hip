@@ -338,8 +338,8 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
         }
         const uint8_t* const buf = smem + par * Tile::kBuf;
         const float* const ts4 = slot_of(kb);
-        // Where every query sees the whole tile, no unit moves and every scale counts: both halves at once, the second's scores beside
-        // the first one's maximum, its weights beside the first one's products with the values
+        // Where every query sees the whole tile, no unit moves and every scale counts: both halves at once, a group's weights beside the
+        // last group's products with the values
         bool whole = !shared && w.live && kb + 1 < k1 && (kb + 2) * kPK - 1 <= (kShaped ? seq.pos0(a) + w.t0 : seq.from(a, w)) &&
                      __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, by)) == 0x3F800000;
         float lv4[4];
