@@ -747,10 +747,10 @@ nnhip_status nnhip_attention_pages_prefill_distance(nnhip_ctx* ctx, const nnhip_
  * token, which is the token at the block's first position.
  * What a write does: s = fl(m * fl(1/127)) with m the largest magnitude (NaN left out) among the call's tokens in the block,
  * and q = round_half_away(clamp(fl(x / s), -127, 127)), 0 for NaN and where s is 0, as nnhip_quantize_i8. Where the block has older
- * tokens (positions before the sequence's first one of the call), its scale is kept if it is at least s;
+ * tokens (positions before the sequence's first one of the call), its scale is kept if it is at least s or NaN;
  * otherwise their codes become those of the values that they stood for under s. An infinity makes a scale infinite, and
- * its block's codes 0: they stand for NaN. Scales from elsewhere must be NaN, or at least 0 and below 2^121 or infinite, as
- * every write leaves them. */
+ * its block's codes 0: they stand for NaN, and so do those of tokens that join a block whose scale is NaN. Scales from
+ * elsewhere must be NaN, or at least 0 and below 2^122 or infinite, as every write leaves them. */
 typedef struct nnhip_kv_pages_i8
 {
     void* k;

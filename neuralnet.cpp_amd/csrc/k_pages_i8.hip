@@ -45,6 +45,10 @@ __device__ __forceinline__ void wave_lds_fence()
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// The scale of a block that goes on: `before` unless the new tokens' s is larger. A NaN stays, as an infinity does (s is never NaN): the
+// block's positions keep standing for NaN, and the new tokens' codes are 0.
+__device__ __forceinline__ float joined_scale(float s, float before) { return s > before ? s : before; }
+
 // A block whose scale has grown: its first row, the positions that it had, and both scales
 struct Regrown
 {
@@ -225,7 +229,7 @@ __global__ __launch_bounds__(kFillThreads) void k_pages_fill_i8(FillI8Args a)
         if (row[e] >= 0)
         {
             s[e] = __fmul_rn(__builtin_bit_cast(float, top_s[first[e]]), 1.0f / 127.0f);
-            if (older[e] > 0) s[e] = fmaxf(s[e], s_old[e]);
+            if (older[e] > 0) s[e] = joined_scale(s[e], s_old[e]);
             if (w == 0 && kPfTok * e + lane == first[e]) scales[row[e] >> a.pools.bshift] = s[e];
         }
     int8_t* const pool = keys ? a.pools.k : a.pools.v;
@@ -445,7 +449,7 @@ __global__ __launch_bounds__(256, DK == 256 ? 3 : 5) void k_windows_fill_i8(Fill
     __syncthreads();
     top = fmaxf(fmaxf(top_s[0][lane >> 4], top_s[1][lane >> 4]), fmaxf(top_s[2][lane >> 4], top_s[3][lane >> 4]));
     float s = __fmul_rn(top, 1.0f / 127.0f);
-    if (goes_on) s = fmaxf(s, s_old);
+    if (goes_on) s = joined_scale(s, s_old);
     const bool begins = in && row >= 0 && (pos == at.pos0 || pos == start);  // the block's first token of the call
     if (w == 0 && begins) scales[row >> a.pools.bshift] = s;
     int8_t* const pool = keys ? a.pools.k : a.pools.v;
@@ -682,7 +686,7 @@ struct Append
             const uint32_t bits = wave_max(__builtin_bit_cast(uint32_t, top));
             const float before = q ? s_old[1] : s_old[0];
             float s = __fmul_rn(__builtin_bit_cast(float, bits), 1.0f / 127.0f);
-            if (into > 0) s = fmaxf(s, before);
+            if (into > 0) s = joined_scale(s, before);
             (q ? got.s[1] : got.s[0]) = s;
             int8_t* const pool = q ? pools.v : pools.k;
             if (row >= 0 && into > 0 && s > before)
