@@ -12,7 +12,9 @@
 //                  of the largest, and 2^-40 of the largest below. Of the scale of 16 values 2^k, a power of two, goes into their
 //                  codes as they are widened, the rest, in 1 .. 2, into the weights by its logarithm in the same argument. O is in
 //                  units of a power of two that the largest scale of a tile stays within 2^+-5 of: where it leaves that range,
-//                  O moves to another unit first. Groups 2^-14 or more below it are summed apart. So no scale costs the weights bits.
+//                  O moves to another unit first. Groups 2^-14 or more below it are summed apart, and so are those of a tile whose unit
+//                  is 2^100 or more above that of a query which does not see the tile's large ones: each query's O has a unit of its
+//                  own then. So no scale costs the weights bits, and none that a query does not see costs it anything.
 // O^T stays in the accumulators over all tiles; a query's reference maximum moves when its maximum has grown by
 // 2^8, by a whole power of two. Sums and softmax are f32. The next tile is converted by half of the waves before their
 // products and by the other half behind them, so that every SIMD has one of each. A tile that every query of the wave sees
@@ -44,6 +46,8 @@ constexpr int kI8Keys = 64;      // keys of a tile, two halves of kPK
 constexpr float kI8Up = 6.0f;    // log2 of the largest weight when a reference maximum is new
 constexpr int kI8Near = 5;       // the largest scale of a tile's values is within 2^+-5 of O's unit
 constexpr int kI8Low = -14;      // the least power of two that codes are multiplied by: they stay normal f16 values
+constexpr int kI8Far = 100;      // O moves up by at most 2^100 to a unit whose scale its query need not see: it stays a normal f32 value
+constexpr int kI8Fall = 60;      // and a unit lies at most 2^60 below the largest: O, below 2^57 in its unit over 2^30 keys, stays finite
 
 constexpr int kJoin = 8;         // dimensions of a work-group that joins (17 records: 16 25.7 us, 8 24.8, 4 25.0)
 
@@ -152,8 +156,7 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
     auto post_scales = [&](int kb, const float(&s)[2]) {
         if (lane < 2) slot_of(kb)[4 * lane + wave] = lane ? s[1] : s[0];
     };
-    // the unit of O for a tile whose scales are posted, where it was `unit` before and `top` at most so far: no more than
-    // 2^80 below that, so that O stays finite
+    // the unit of O for a tile whose scales are posted, where it was `unit` before and `top` at most so far
     auto next_unit = [&](int kb, int unit, int& top) {
         int field = scale_field(__builtin_bit_cast(uint32_t, slot_of(kb)[4 + (lane & 3)]));
         field = max(field, __builtin_amdgcn_update_dpp(0, field, 0xB1, 0xF, 0xF, true));  // lane ^ 1
@@ -161,7 +164,7 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
         field = __builtin_amdgcn_readfirstlane(field);
         if (field == 0) return unit;
         top = max(top, field);
-        return field > unit + kI8Near || field < unit - kI8Near ? max(field, top - 80) : unit;
+        return field > unit + kI8Near || field < unit - kI8Near ? max(field, top - kI8Fall) : unit;
     };
     auto convert = [&](int kb, int par, int unit) {
         uint8_t* const buf = smem + par * Tile::kBuf;
@@ -278,7 +281,9 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
         if (k0 + 2 < k1) post_scales(k0 + 2, s_next);
     }
     __syncthreads();  // the tables have been read; the first two tiles' scales are there
-    int unit_top = 0, unit = next_unit(k0, 127, unit_top);  // O is in units of 2^(unit - 127)
+    int unit_top = 0, unit = next_unit(k0, 127, unit_top);  // tiles are added to O in units of 2^(unit - 127)
+    int lane_unit = unit;                                   // and what the lane has of O is in units of 2^(lane_unit - 127)
+    bool settled = true;                                    // the same in every lane
     convert(k0, 0, unit);
     if (k0 + 2 < k1) load_raw(k0 + 2);
     // scores s of a half, with their keys' scales: capped, and their bias from the half's first key on
@@ -320,7 +325,6 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
     };
     const uint32_t k_at = (uint32_t)(l32 * Tile::kKPitch + 16 * h), v_at = (uint32_t)(Tile::kV + l32 * Tile::kVPitch + 16 * h);
     int par = 0;
-    float by = 1.0f;  // from the last tile's unit to this one's
     for (int kb = k0; kb < k1; kb += 2, par ^= 1)
     {
         __syncthreads();  // tile kb is in LDS; the other buffer is free
@@ -341,7 +345,7 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
         // Where every query sees the whole tile, no unit moves and every scale counts: both halves at once, a group's weights beside the
         // last group's products with the values
         bool whole = !shared && w.live && kb + 1 < k1 && (kb + 2) * kPK - 1 <= (kShaped ? seq.pos0(a) + w.t0 : seq.from(a, w)) &&
-                     __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, by)) == 0x3F800000;
+                     settled;
         float lv4[4];
         // (keys two steps ahead of their products, of both halves in turn)
         auto keys = [&](int half, int c) { return *reinterpret_cast<const v8h*>(buf + k_at + half * kPK * Tile::kKPitch + 32 * c); };
@@ -509,14 +513,12 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
             const float mx = __builtin_ceilf(max_halves(fmaxf(top[0], top[1]) + away));
             // the reference of a query moves only when its maximum has grown by 2^8 (or is new)
             const bool grown = mx > m_ref + kPLazy;
-            if (__builtin_expect(__builtin_amdgcn_ballot_w64(grown) != 0 || by != 1.0f, 0))
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(grown) != 0, 0))
             {
                 const float m_new = grown ? mx : m_ref;
                 float corr = grown ? __builtin_amdgcn_exp2f(m_ref - m_new) : 1.0f;
                 asm volatile("" : "+v"(corr));
                 l_run *= corr;
-                corr *= by;
-                by = 1.0f;
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -524,16 +526,31 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
                 m_ref = m_new;
             }
             const float base = kI8Up + (m_ref == -__builtin_inff() ? 0.0f : away - m_ref);
+            if (__builtin_expect(!settled, 0))
+            {
+                // O to the tile's unit, unless that is far above the lane's: its query may not see what has raised it
+                const bool far = lane_unit - unit < -kI8Far;
+                int by = far ? 0 : lane_unit - unit;
+                asm volatile("" : "+v"(by));
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) o[d][v] = __builtin_ldexpf(o[d][v], by);
+                if (!far) lane_unit = unit;
+                settled = __builtin_amdgcn_ballot_w64(far) == 0;
+            }
+            int apart = 0;  // bit t: group t's sums are not added to O as they are
 #pragma unroll
             for (int t = 0; t < 2; ++t)
             {
                 // what the codes have not got of their scale (0 and what is not finite: nothing)
                 const uint32_t bits = __builtin_bit_cast(uint32_t, vs[t]);
                 const int e = scale_field(bits);
-                const int power = code_power(e, unit), left = e == 0 ? 0 : e - unit - power;
                 const float lv = e == 0 ? 0.0f : __builtin_amdgcn_logf(vs[t]) - (float)(e - 127);
                 if (__builtin_expect((bits >> 23) == 255, 0) && key0 + 16 * t <= seq.sight(w)) l_run = __builtin_nanf("");
-                const float off = left == 0 ? base + lv : -__builtin_inff();
+                const bool here = settled && (e == 0 || e - unit == code_power(e, unit));
+                const float off = here ? base + lv : -__builtin_inff();
+                apart |= here ? 0 : 1 << t;
                 float sum = 0.0f;
                 v8h pa, pb;
 #pragma unroll
@@ -556,35 +573,51 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pb, o[d], 0, 0, 0);
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pa, o[d], 0, 0, 0);
                 }
-                if (__builtin_expect(left != 0, 0))
+            }
+            // A group whose scale is far below the largest of its tile, which some queries may not see, or some lane's unit far below:
+            // its sums, in units of 2^(own - 127), go to each lane's own unit, which becomes the group's where the
+            // query sees that, and it is 2^20 larger or the lane has nothing yet
+#pragma unroll 1
+            for (int t = 0; __builtin_expect(apart >> t != 0, 0); ++t)
+            {
+                if (!(apart >> t & 1)) continue;
+                settled = false;
+                const float scale = t ? vs[1] : vs[0], factor = t ? kf[1] : kf[0];
+                const int e = scale_field(__builtin_bit_cast(uint32_t, scale)), own = e == 0 ? unit : e - code_power(e, unit);
+                const float lv = e == 0 ? 0.0f : __builtin_amdgcn_logf(scale) - (float)(e - 127);
+                uint32_t any = 0;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) any |= __builtin_bit_cast(uint32_t, o[d][v]);
+                int to = own - lane_unit;
+                const int move = (to > 20 || any << 1 == 0) && key0 + 16 * t <= seq.sight(w) ? to : 0;
+                lane_unit += move;
+                to -= move;
+                float sum = 0.0f;
+                v8h pa, pb;
+#pragma unroll
+                for (int v = 0; v < 8; v += 2)
                 {
-                    // a group whose scale is far below the largest of its tile, which some queries may not see: its
-                    // weights in full, its sums times the power of two that is left
-                    float rest = __builtin_ldexpf(1.0f, left);
-                    asm volatile("" : "+v"(rest));
-                    sum = 0.0f;
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(t ? s[8 + v] : s[v], factor, base + lv));
+                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(t ? s[9 + v] : s[v + 1], factor, base + lv));
+                    sum += p0;
+                    sum += p1;
+                    v2h x, y;
+                    split2(p0, p1, x, y);
+                    pa[v] = x[0], pa[v + 1] = x[1];
+                    pb[v] = y[0], pb[v + 1] = y[1];
+                }
+                l_run = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-lv), l_run);
 #pragma unroll
-                    for (int v = 0; v < 8; v += 2)
-                    {
-                        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * t + v], kf[t], base + lv));
-                        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * t + v + 1], kf[t], base + lv));
-                        sum += p0;
-                        sum += p1;
-                        v2h x, y;
-                        split2(p0, p1, x, y);
-                        pa[v] = x[0], pa[v + 1] = x[1];
-                        pb[v] = y[0], pb[v + 1] = y[1];
-                    }
-                    l_run = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-lv), l_run);
+                for (int d = 0; d < ND; ++d)
+                {
+                    const v8h x = *reinterpret_cast<const v8h*>(buf + v_at + 32 * d * Tile::kVPitch + 32 * (2 * half + t));
+                    v16f y = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pb, v16f{}, 0, 0, 0);
+                    y = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pa, y, 0, 0, 0);
 #pragma unroll
-                    for (int d = 0; d < ND; ++d)
-                    {
-                        const v8h x = *reinterpret_cast<const v8h*>(buf + v_at + 32 * d * Tile::kVPitch + 32 * (2 * half + t));
-                        v16f y = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pb, v16f{}, 0, 0, 0);
-                        y = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pa, y, 0, 0, 0);
-#pragma unroll
-                        for (int v = 0; v < 16; ++v) o[d][v] = __builtin_fmaf(y[v], rest, o[d][v]);
-                    }
+                    for (int v = 0; v < 16; ++v) o[d][v] = __builtin_ldexpf(o[d][v], -move) + __builtin_ldexpf(y[v], to);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
@@ -595,7 +628,7 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
         }
         if (more)
         {
-            by *= __builtin_ldexpf(1.0f, unit - unit_next);
+            settled &= unit == unit_next;
             unit = unit_next;
             if (wave < 4 && kb + 4 < k1) post_scales(kb + 4, s_next);
         }
@@ -608,8 +641,7 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
 #pragma unroll
     for (int i = 0; i < kPWaves; ++i) found |= found_s[i];
     if (found) l_run = __builtin_nanf("");
-    // (a unit that no tile of the wave's has taken up yet is still to come off)
-    by = __builtin_ldexpf(by, unit - 127);
+    int power = lane_unit - 127;  // of two, that O is in units of
     if (shared)
     {
         // the second halves' outputs, maxima and sums through LDS (every wave is past its tiles)
@@ -619,7 +651,7 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
 #pragma unroll
             for (int d = 0; d < ND; ++d)
 #pragma unroll
-                for (int v = 0; v < 16; ++v) at[(16 * d + v) * kWave] = o[d][v] * by;
+                for (int v = 0; v < 16; ++v) at[(16 * d + v) * kWave] = __builtin_ldexpf(o[d][v], power);
             at[16 * ND * kWave] = m_ref;
             at[(16 * ND + 1) * kWave] = l_run;
         }
@@ -630,12 +662,12 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
             const float own = m_ref == to ? 1.0f : __builtin_amdgcn_exp2f(m_ref - to);
             const float other = m == to ? 1.0f : __builtin_amdgcn_exp2f(m - to);
             l_run = __builtin_fmaf(at[(16 * ND + 1) * kWave], other, l_run * own);
-            by *= own;
 #pragma unroll
             for (int d = 0; d < ND; ++d)
 #pragma unroll
-                for (int v = 0; v < 16; ++v) o[d][v] = __builtin_fmaf(at[(16 * d + v) * kWave], other, o[d][v] * by);
-            by = 1.0f;
+                for (int v = 0; v < 16; ++v)
+                    o[d][v] = __builtin_fmaf(at[(16 * d + v) * kWave], other, __builtin_ldexpf(o[d][v], power) * own);
+            power = 0;
             m_ref = to;
         }
         __syncthreads();  // the next item may write there
@@ -645,12 +677,12 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
     if (!w.live) return;
     if (rec)
     {
-        store_record<DK>(rec, tid, dim, [&](int d, int v) { return o[d][v] * by; }, m_ref, l_run);
+        store_record<DK>(rec, tid, dim, [&](int d, int v) { return __builtin_ldexpf(o[d][v], power); }, m_ref, l_run);
         return;
     }
     // (nothing visible above -infinity: 0)
     const float inv = l_run == 0.0f ? 1.0f : 1.0f / l_run;
-    store_out<DK>(a, w, seq, h, dim, [&](int d, int v) { return o[d][v] * by * inv; });
+    store_out<DK>(a, w, seq, h, dim, [&](int d, int v) { return __builtin_ldexpf(o[d][v], power) * inv; });
 }
 
 // The items of a work-group of a call of packed prompts, one after the other: attend(item, first tile, end, record or
