@@ -642,6 +642,15 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
     for (int i = 0; i < kPWaves; ++i) found |= found_s[i];
     if (found) l_run = __builtin_nanf("");
     int power = lane_unit - 127;  // of two, that O is in units of
+    if ((rec || shared) && power > 0)
+    {
+        // large values, whose sums would pass f32's range: O and its sum to below 2^-8 of the values, 64 records' to below the
+        // values themselves (where they are joined before the division; small ones would lose bits)
+        const int field = (int)(__builtin_bit_cast(uint32_t, l_run) >> 23), by = l_run > 0.0f && field < 255 ? field - 126 + 8 : 0;
+        l_run = __builtin_ldexpf(l_run, -by);
+        m_ref += (float)by;
+        power -= by;
+    }
     if (shared)
     {
         // the second halves' outputs, maxima and sums through LDS (every wave is past its tiles)
@@ -682,7 +691,7 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
     }
     // (nothing visible above -infinity: 0)
     const float inv = l_run == 0.0f ? 1.0f : 1.0f / l_run;
-    store_out<DK>(a, w, seq, h, dim, [&](int d, int v) { return __builtin_ldexpf(o[d][v], power) * inv; });
+    store_out<DK>(a, w, seq, h, dim, [&](int d, int v) { return __builtin_ldexpf(o[d][v] * inv, power); });
 }
 
 // The items of a work-group of a call of packed prompts, one after the other: attend(item, first tile, end, record or

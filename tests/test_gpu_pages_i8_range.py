@@ -60,3 +60,18 @@ def test_alternating_blocks(ctx, nnhip, cap):
 
     finite_case(ctx, nnhip, lens=[300, 40], pos0=[0, 400], H=4, Hkv=1, dk=128, page=32, block=16, cap=cap, slopes=cap > 0, stride=5,
                 edit=edit)
+
+
+@pytest.mark.parametrize("power", [112, 118, -80])
+@pytest.mark.parametrize("lens,pos0", [([300], [0]), ([256, 100], [700, 0]), ([10], [2000]), ([1, 1], [700, 40]), ([40], [1200])])
+def test_ends_of_the_range(ctx, nnhip, lens, pos0, power):
+    """Values about 2^115 over hundreds of keys, by one work-group, by waves that share keys and by spans that share items: their
+    weighted mean is as large as they are. And small ones."""
+    def edit(c, q):
+        for b in range(len(lens)):
+            n = -(-(lens[b] + pos0[b]) // 16)
+            most = max(float(np.max(c.scales["v"][c.table[b, i // 2], :, i % 2])) for i in range(n))
+            scaled(c, b, 0, n, power - int(np.ceil(np.log2(most))) - 1)  # scales of up to 2^(power - 1), values below 2^(power + 6)
+
+    for H, Hkv, dk in ((4, 4, 64), (8, 1, 128)):
+        finite_case(ctx, nnhip, lens=lens, pos0=pos0, H=H, Hkv=Hkv, dk=dk, page=32, block=16, stride=9, edit=edit)
