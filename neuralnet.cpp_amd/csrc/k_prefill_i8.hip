@@ -323,6 +323,10 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
                             for (int v = 0; v < 16; ++v) s[v] = __builtin_fmaf(s[v], kf[v >> 3], steps[v]);
                         }
     };
+    // a score's factor, of a key's scale: within f32's range, as a score of 0 is 0 under any finite scale (any other is past the
+    // cap, or the range, with the largest float, too). Scales are below 2^122, so only large queries get there
+    auto factor = [&](float scale) { return scale < __builtin_inff() ? fminf(f * scale, 3.40282347e38f) : __builtin_nanf(""); };
+    const bool large = __builtin_amdgcn_ballot_w64(!(f < 32.0f)) != 0;
     const uint32_t k_at = (uint32_t)(l32 * Tile::kKPitch + 16 * h), v_at = (uint32_t)(Tile::kV + l32 * Tile::kVPitch + 16 * h);
     int par = 0;
     for (int kb = k0; kb < k1; kb += 2, par ^= 1)
@@ -342,9 +346,9 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
         }
         const uint8_t* const buf = smem + par * Tile::kBuf;
         const float* const ts4 = slot_of(kb);
-        // Where every query sees the whole tile, no unit moves and every scale counts: both halves at once, a group's weights beside the
+        // Where every query sees the whole tile, no unit moves, every scale counts and no query is large: both halves at once, a group's weights beside the
         // last group's products with the values
-        bool whole = !shared && w.live && kb + 1 < k1 && (kb + 2) * kPK - 1 <= (kShaped ? seq.pos0(a) + w.t0 : seq.from(a, w)) &&
+        bool whole = !shared && !large && w.live && kb + 1 < k1 && (kb + 2) * kPK - 1 <= (kShaped ? seq.pos0(a) + w.t0 : seq.from(a, w)) &&
                      settled;
         float lv4[4];
         // (keys two steps ahead of their products, of both halves in turn)
@@ -469,7 +473,7 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
 #pragma unroll
             for (int t = 0; t < 2; ++t)
             {
-                kf[t] = f * ts4[2 * half + t];
+                kf[t] = factor(ts4[2 * half + t]);
                 vs[t] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, ts4[4 + 2 * half + t])));
             }
             const bool masked = key0 + kPK - 1 > seq.from(a, w);
@@ -582,7 +586,7 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
             {
                 if (!(apart >> t & 1)) continue;
                 settled = false;
-                const float scale = t ? vs[1] : vs[0], factor = t ? kf[1] : kf[0];
+                const float scale = t ? vs[1] : vs[0], by = t ? kf[1] : kf[0];
                 const int e = scale_field(__builtin_bit_cast(uint32_t, scale)), own = e == 0 ? unit : e - code_power(e, unit);
                 const float lv = e == 0 ? 0.0f : __builtin_amdgcn_logf(scale) - (float)(e - 127);
                 uint32_t any = 0;
@@ -599,8 +603,8 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
 #pragma unroll
                 for (int v = 0; v < 8; v += 2)
                 {
-                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(t ? s[8 + v] : s[v], factor, base + lv));
-                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(t ? s[9 + v] : s[v + 1], factor, base + lv));
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(t ? s[8 + v] : s[v], by, base + lv));
+                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(t ? s[9 + v] : s[v + 1], by, base + lv));
                     sum += p0;
                     sum += p1;
                     v2h x, y;

@@ -75,3 +75,15 @@ def test_ends_of_the_range(ctx, nnhip, lens, pos0, power):
 
     for H, Hkv, dk in ((4, 4, 64), (8, 1, 128)):
         finite_case(ctx, nnhip, lens=lens, pos0=pos0, H=H, Hkv=Hkv, dk=dk, page=32, block=16, stride=9, edit=edit)
+
+
+@pytest.mark.parametrize("cap,slopes", [(0.0, False), (20.0, True), (0.0, True)])
+@pytest.mark.parametrize("lens,pos0", [([70], [0]), ([9], [300]), ([200], [200])])
+def test_zero_keys_of_large_scales(ctx, nnhip, lens, pos0, cap, slopes):
+    """Codes of 0 under scales that pass f32's range times the query's size stand for 0, and scores are 0."""
+    def edit(c, q):
+        c.codes["k"][:] = 0
+        c.scales["k"][:] = F32(2.0 ** 100)
+        q *= F32(2.0 ** 90)
+
+    finite_case(ctx, nnhip, lens=lens, pos0=pos0, H=4, Hkv=1, dk=128, page=32, block=16, cap=cap, slopes=slopes, rope=False, stride=7, edit=edit)
