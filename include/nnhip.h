@@ -787,8 +787,8 @@ nnhip_status nnhip_attention_pages_decode_i8(nnhip_ctx* ctx, const nnhip_kv_page
 
 /* nnhip_attention_pages_prefill over a cache in 8 bits: the same arguments and limits, dk in {64, 128}; distance != 0:
  * the bias of nnhip_attention_pages_prefill_distance. The codes go into the products as they are, queries and weights
- * in two f16 parts: queries to 2^-23 of each element and 2^-40 of the query's largest, weights to 2^-22 of each and 2^-31 of the largest
- * before; sums and softmax are f32. Values under a scale below 2^-126 count as 0. NaN: a query that holds an infinity or
+ * in two f16 parts: queries to 2^-23 of each element and 2^-40 of the query's largest, weights to 2^-22 of each and, over up to 8192 keys,
+ * 2^-32 of the largest, over more 2^-25 of the largest in their run of 64; sums and softmax are f32. Values under a scale below 2^-126 count as 0. NaN: a query that holds an infinity or
  * a NaN, or sees a scale that is not finite. */
 nnhip_status nnhip_attention_pages_prefill_i8(nnhip_ctx* ctx, const nnhip_kv_pages_i8* cache, const float* q, size_t M,
                                               const int32_t* cu, const int32_t* pos0, size_t B, size_t t_bound, size_t H,

@@ -8,15 +8,16 @@
 //   S^T = K . Q^T  with each query in two f16 parts, q 2^e = hi + lo to 2^-23 of it (and 2^-40 of the query's
 //                  largest): two v_mfma_f32_32x32x16_f16 a step, whose products are exact; a key's scale is a factor of
 //                  the 16 scores that share it, folded into the exponential's argument with the softmax scale;
-//   O^T += V^T . P^T  with the weights in two f16 parts, 2^6 .. 2^15 at their largest: 22 bits of every weight down to 2^-24
-//                  of the largest, and 2^-40 of the largest below. Of the scale of 16 values 2^k, a power of two, goes into their
+//   O^T += V^T . P^T  with the weights in two f16 parts, 2^8 .. 2^15 at their largest: 2^-22 of every weight down to 2^-10 .. 2^-17
+//                  of the largest, and 2^-33 .. 2^-40 of the largest below; over more than 8192 keys a tile far below the
+//                  largest is weighed under its own. Of the scale of 16 values 2^k, a power of two, goes into their
 //                  codes as they are widened, the rest, in 1 .. 2, into the weights by its logarithm in the same argument. O is in
 //                  units of a power of two that the largest scale of a tile stays within 2^+-5 of: where it leaves that range,
 //                  O moves to another unit first. Groups 2^-14 or more below it are summed apart, and so are those of a tile whose unit
 //                  is 2^100 or more above that of a query which does not see the tile's large ones: each query's O has a unit of its
 //                  own then. So no scale costs the weights bits, and none that a query does not see costs it anything.
 // O^T stays in the accumulators over all tiles; a query's reference maximum moves when its maximum has grown by
-// 2^8, by a whole power of two. Sums and softmax are f32. The next tile is converted by half of the waves before their
+// 2^6, by a whole power of two. Sums and softmax are f32. The next tile is converted by half of the waves before their
 // products and by the other half behind them, so that every SIMD has one of each. A tile that every query of the wave sees
 // goes in one piece, a group's weights between the last group's products (in two halves, each step by itself: 477 us for 446).
 // Work-groups take equal spans of all tiles and join the items they share (prompt_spans.hpp).
@@ -43,7 +44,14 @@ struct ScalesI8
 };
 
 constexpr int kI8Keys = 64;      // keys of a tile, two halves of kPK
-constexpr float kI8Up = 6.0f;    // log2 of the largest weight when a reference maximum is new
+constexpr float kI8Up = 8.0f;    // log2 of the largest weight when a reference maximum is new
+constexpr float kI8Lazy = 6.0f;  // log2 growth of a query's maximum before its sums are rescaled: weights are at most 2^15 then
+// f16 holds a weight to 2^-25, 2^-32 of the largest before: up to kI8Many tiles of 32 keys (8192 keys) all that is lost is 2^-19 of the largest
+// weight at most. Over more of them a tile whose largest weight is more than kI8Deep log2 units below the reference is weighed under that
+// weight. (Where a few queries of one wave do so, all wait for it: 4 x 700 .. 1024 at 6144, which has none with more, 432 us, with
+// every tile looked at 448, from 4 units on 637.)
+constexpr int kI8Many = 256;
+constexpr float kI8Deep = 7.0f;
 constexpr int kI8Near = 5;       // the largest scale of a tile's values is within 2^+-5 of O's unit
 constexpr int kI8Low = -14;      // the least power of two that codes are multiplied by: they stay normal f16 values
 constexpr int kI8Far = 100;      // O moves up by at most 2^100 to a unit whose scale its query need not see: it stays a normal f32 value
@@ -326,6 +334,7 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
     // a score's factor, of a key's scale: within f32's range, as a score of 0 is 0 under any finite scale (any other is past the
     // cap, or the range, with the largest float, too). Scales are below 2^122, so only large queries get there
     auto factor = [&](float scale) { return scale < __builtin_inff() ? fminf(f * scale, 3.40282347e38f) : __builtin_nanf(""); };
+    const bool many = k1 - k0 > kI8Many;
     const bool large = __builtin_amdgcn_ballot_w64(!(f < 32.0f)) != 0;
     const uint32_t k_at = (uint32_t)(l32 * Tile::kKPitch + 16 * h), v_at = (uint32_t)(Tile::kV + l32 * Tile::kVPitch + 16 * h);
     int par = 0;
@@ -402,59 +411,63 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
                 top = fmaxf(top, kShaped ? most + away[t >> 1] : most * kf[t]);
             }
             const float mx = __builtin_ceilf(max_halves(top));
-            const bool grown = mx > m_ref + kPLazy;
-            if (__builtin_expect(__builtin_amdgcn_ballot_w64(grown) != 0, 0))
+            whole = !many || __builtin_amdgcn_ballot_w64(mx < m_ref - kI8Deep) == 0;
+            if (__builtin_expect(whole, 1))
             {
-                const float m_new = grown ? mx : m_ref;
-                float corr = grown ? __builtin_amdgcn_exp2f(m_ref - m_new) : 1.0f;
-                asm volatile("" : "+v"(corr));
-                l_run *= corr;
+                const bool grown = mx > m_ref + kI8Lazy;
+                if (__builtin_expect(__builtin_amdgcn_ballot_w64(grown) != 0, 0))
+                {
+                    const float m_new = grown ? mx : m_ref;
+                    float corr = grown ? __builtin_amdgcn_exp2f(m_ref - m_new) : 1.0f;
+                    asm volatile("" : "+v"(corr));
+                    l_run *= corr;
 #pragma unroll
-                for (int d = 0; d < ND; ++d)
+                    for (int d = 0; d < ND; ++d)
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) o[d][v] *= corr;
-                m_ref = m_new;
+                        for (int v = 0; v < 16; ++v) o[d][v] *= corr;
+                    m_ref = m_new;
+                }
+                float base[2];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) base[half] = kI8Up + (m_ref == -__builtin_inff() ? 0.0f : away[half] - m_ref);
+                // weights of group t + 1 between the products of group t: a pair of keys beside 8 / ND products
+                v8h pa[2], pb[2];
+                float sum = 0.0f;
+                auto pair = [&](int t, int v) {
+                    const float off = base[t >> 1] + lv4[t];
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t >> 1][8 * (t & 1) + v], kf[t], off));
+                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t >> 1][8 * (t & 1) + v + 1], kf[t], off));
+                    sum += p0;
+                    sum += p1;
+                    v2h x, y;
+                    split2(p0, p1, x, y);
+                    pa[t & 1][v] = x[0], pa[t & 1][v + 1] = x[1];
+                    pb[t & 1][v] = y[0], pb[t & 1][v + 1] = y[1];
+                    if (v == 6)
+                    {
+                        l_run = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-lv4[t]), l_run);
+                        sum = 0.0f;
+                    }
+                };
+                auto values = [&](int i) { return *reinterpret_cast<const v8h*>(buf + v_at + 32 * (i % ND) * Tile::kVPitch + 32 * (i / ND)); };
+                v8h x = values(0);
+#pragma unroll
+                for (int v = 0; v < 8; v += 2) pair(0, v);
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+                    {
+                        const v8h y = x;
+                        if (t * ND + d + 1 < 4 * ND) x = values(t * ND + d + 1);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, pb[t & 1], o[d], 0, 0, 0);
+                        if (t < 3)
+#pragma unroll
+                            for (int v = 8 / ND * d; v < 8 / ND * (d + 1); v += 2) pair(t + 1, v);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, pa[t & 1], o[d], 0, 0, 0);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
             }
-            float base[2];
-#pragma unroll
-            for (int half = 0; half < 2; ++half) base[half] = kI8Up + (m_ref == -__builtin_inff() ? 0.0f : away[half] - m_ref);
-            // weights of group t + 1 between the products of group t: a pair of keys beside 8 / ND products
-            v8h pa[2], pb[2];
-            float sum = 0.0f;
-            auto pair = [&](int t, int v) {
-                const float off = base[t >> 1] + lv4[t];
-                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t >> 1][8 * (t & 1) + v], kf[t], off));
-                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t >> 1][8 * (t & 1) + v + 1], kf[t], off));
-                sum += p0;
-                sum += p1;
-                v2h x, y;
-                split2(p0, p1, x, y);
-                pa[t & 1][v] = x[0], pa[t & 1][v + 1] = x[1];
-                pb[t & 1][v] = y[0], pb[t & 1][v + 1] = y[1];
-                if (v == 6)
-                {
-                    l_run = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-lv4[t]), l_run);
-                    sum = 0.0f;
-                }
-            };
-            auto values = [&](int i) { return *reinterpret_cast<const v8h*>(buf + v_at + 32 * (i % ND) * Tile::kVPitch + 32 * (i / ND)); };
-            v8h x = values(0);
-#pragma unroll
-            for (int v = 0; v < 8; v += 2) pair(0, v);
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-                {
-                    const v8h y = x;
-                    if (t * ND + d + 1 < 4 * ND) x = values(t * ND + d + 1);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, pb[t & 1], o[d], 0, 0, 0);
-                    if (t < 3)
-#pragma unroll
-                        for (int v = 8 / ND * d; v < 8 / ND * (d + 1); v += 2) pair(t + 1, v);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, pa[t & 1], o[d], 0, 0, 0);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
         }
 #pragma unroll 1
         for (int half = whole ? 2 : 0; half < 2; ++half)
@@ -515,8 +528,8 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
                 top[t] *= kf[t];
             }
             const float mx = __builtin_ceilf(max_halves(fmaxf(top[0], top[1]) + away));
-            // the reference of a query moves only when its maximum has grown by 2^8 (or is new)
-            const bool grown = mx > m_ref + kPLazy;
+            // the reference of a query moves only when its maximum has grown by 2^6 (or is new)
+            const bool grown = mx > m_ref + kI8Lazy;
             if (__builtin_expect(__builtin_amdgcn_ballot_w64(grown) != 0, 0))
             {
                 const float m_new = grown ? mx : m_ref;
@@ -530,6 +543,7 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
                 m_ref = m_new;
             }
             const float base = kI8Up + (m_ref == -__builtin_inff() ? 0.0f : away - m_ref);
+            const bool deep = many && __builtin_amdgcn_ballot_w64(mx < m_ref - kI8Deep && mx > -__builtin_inff()) != 0;
             if (__builtin_expect(!settled, 0))
             {
                 // O to the tile's unit, unless that is far above the lane's: its query may not see what has raised it
@@ -552,7 +566,7 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
                 const int e = scale_field(bits);
                 const float lv = e == 0 ? 0.0f : __builtin_amdgcn_logf(vs[t]) - (float)(e - 127);
                 if (__builtin_expect((bits >> 23) == 255, 0) && key0 + 16 * t <= seq.sight(w)) l_run = __builtin_nanf("");
-                const bool here = settled && (e == 0 || e - unit == code_power(e, unit));
+                const bool here = settled && !deep && (e == 0 || e - unit == code_power(e, unit));
                 const float off = here ? base + lv : -__builtin_inff();
                 apart |= here ? 0 : 1 << t;
                 float sum = 0.0f;
@@ -578,9 +592,11 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pa, o[d], 0, 0, 0);
                 }
             }
-            // A group whose scale is far below the largest of its tile, which some queries may not see, or some lane's unit far below:
-            // its sums, in units of 2^(own - 127), go to each lane's own unit, which becomes the group's where the
+            // A group whose scale is far below the largest of its tile, which some queries may not see, or some lane's unit far below,
+            // or the largest weight of 32 keys far below the reference, over many keys: weights times 2^up, under a reference of their own,
+            // and their sums, in units of 2^(own - up - 127), to each lane's own unit, which becomes the group's where the
             // query sees that, and it is 2^20 larger or the lane has nothing yet
+            const float up = deep && mx < m_ref - kI8Deep && mx > -__builtin_inff() ? fminf(m_ref - mx, 400.0f) : 0.0f;
 #pragma unroll 1
             for (int t = 0; __builtin_expect(apart >> t != 0, 0); ++t)
             {
@@ -594,7 +610,7 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
                     for (int v = 0; v < 16; ++v) any |= __builtin_bit_cast(uint32_t, o[d][v]);
-                int to = own - lane_unit;
+                int to = own - (int)up - lane_unit;
                 const int move = (to > 20 || any << 1 == 0) && key0 + 16 * t <= seq.sight(w) ? to : 0;
                 lane_unit += move;
                 to -= move;
@@ -603,8 +619,8 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
 #pragma unroll
                 for (int v = 0; v < 8; v += 2)
                 {
-                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(t ? s[8 + v] : s[v], by, base + lv));
-                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(t ? s[9 + v] : s[v + 1], by, base + lv));
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(t ? s[8 + v] : s[v], by, base + up + lv));
+                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(t ? s[9 + v] : s[v + 1], by, base + up + lv));
                     sum += p0;
                     sum += p1;
                     v2h x, y;
@@ -612,7 +628,7 @@ __device__ __forceinline__ void attend_i8(const PrefillArgs& a, const ScalesI8& 
                     pa[v] = x[0], pa[v + 1] = x[1];
                     pb[v] = y[0], pb[v + 1] = y[1];
                 }
-                l_run = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-lv), l_run);
+                l_run = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-lv - up), l_run);
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
                 {
