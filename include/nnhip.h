@@ -777,8 +777,9 @@ nnhip_status nnhip_kv_pages_read_i8(nnhip_ctx* ctx, const nnhip_kv_pages_i8* cac
 /* nnhip_attention_pages_decode over a cache in 8 bits: the same arguments, limits and empty slots; dk in {64, 128, 256}.
  * The new key and value are written as nnhip_kv_pages_fill_i8 writes one token, and take part as the cache then holds
  * them. k and v both NULL: nothing is written, the cache holds position pos[b] already (several calls may share pages then).
- * Products with the codes are exact, of queries with 30 bits under their head's largest element and weights with 30 bits under
- * the tile's (64 positions; values under scales below 2^-96 lose bits, down to none); sums of tiles and softmax are f32. NaN: a head whose
+ * Products with the codes are exact, of queries with 30 bits under their head's largest element and of weights times their blocks'
+ * scales with 30 bits under the largest such product of the head in 64 positions (values under scales below 2^-96 lose bits, down to none);
+ * sums of tiles, before their division by the weights' sum, and softmax are f32. NaN: a head whose
  * rotated query holds an infinity or a NaN, a sequence with a scale that is not finite among its positions. */
 nnhip_status nnhip_attention_pages_decode_i8(nnhip_ctx* ctx, const nnhip_kv_pages_i8* cache, const float* q, const float* k,
                                              const float* v, size_t B, size_t H, const int32_t* pos, size_t len_bound,

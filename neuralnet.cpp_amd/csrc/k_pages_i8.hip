@@ -751,13 +751,15 @@ __device__ __forceinline__ float pow2_field(int field) { return __builtin_bit_ca
 //           signed base-256 digits: rows 4 h + i of a 16 x 64 operand for four heads, against 16 positions' keys. Every
 //           partial sum is exact in int32, and a lane finds the four digit sums of one head and position in its
 //           registers; s = (256 a3 + a2) 2^16 + (256 a1 + a0) is rounded as an f32.
-//   values  the weights of a tile, times their blocks' scales over the tile's largest (a power of two above it), as
-//           30-bit fixed point in the same digits, through LDS to the columns of an operand; the digits' sums over
-//           the tile's 64 positions are exact, and each is added to an f32 sum of its own, joined at the end.
+//   values  the weights of a tile, times their blocks' scales, as 30-bit fixed point under the head's largest such product (a power
+//           of two above it) in the same digits, through LDS to the columns of an operand; the digits' sums over
+//           the tile's 64 positions are exact, and each is added to an f32 sum of its own, joined at the end. (Under the
+//           reference of the whole wave thousands of small weights beside a large one were lost, under the tile's largest
+//           scale those beside a large value without weight.)
 // So neither codes are converted nor multiplied by their scales one by one: 190 VALU instructions a tile of 64
 // positions for 4 heads of 128, where multiply-adds on widened elements would take 1300.
 // A head's reference maximum moves when a score passes it, to 4 above that score (weights are 2^-4 at most then and
-// 1 at most later: none is held to less than 2^-26 of the largest).
+// 1 at most later).
 // The chunk that holds the new position writes its key and value, by the wave that reads them (no other wave reads that
 // block), and takes their codes into its operands from LDS: its tile is on its way meanwhile, and is read again only
 // where the block's older codes have changed.
@@ -962,7 +964,6 @@ __global__ __launch_bounds__(64 * W) void k_pages_attn_i8(PagesArgs a, PoolsI8 p
         const bool odd = __builtin_amdgcn_ballot_w64(!(fabsf(vs) < 0x1p125f)) != 0;  // (no write makes one from there on)
         const int ev = min(max(__builtin_amdgcn_readfirstlane((int)(__builtin_bit_cast(uint32_t, top_v) >> 23)), 31), 252);
         const float down = odd ? 0.0f : pow2_field(253 - ev);                  // 2^(126 - ev) times a scale is at most 1
-        const float back = odd ? __builtin_nanf("") : pow2_field(ev - 29);     // 2^(ev - 126 - 30)
         float kg[4], vg[4];
 #pragma unroll
         for (int n = 0; n < 4; ++n)
@@ -971,6 +972,7 @@ __global__ __launch_bounds__(64 * W) void k_pages_attn_i8(PagesArgs a, PoolsI8 p
             vg[n] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs), n)) * down;
         }
         const bool part = t + kI8Tile - 1 > last;
+        float back[NS];  // of head 4 s + j / 4
 #pragma unroll
         for (int s = 0; s < NS; ++s)
         {
@@ -1019,14 +1021,30 @@ __global__ __launch_bounds__(64 * W) void k_pages_attn_i8(PagesArgs a, PoolsI8 p
 #pragma unroll
                 for (int i = 0; i < ND; ++i) acc[s][i] *= f;
             }
-            uint8_t* const to = w_s[w][s] + 4 * grp * kI8Pitch + j;
+            uint32_t most = 0;  // (bits, of products that are at least 0, or NaN)
 #pragma unroll
             for (int n = 0; n < 4; ++n)
             {
                 // no score above -inf yet: nothing to add (and no -inf - -inf)
                 const float pr = x[n] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x[n] - m[s]);
                 l[s] += pr;
-                const uint32_t d = digits((uint32_t)__builtin_fmaf(pr * vg[n], 0x1p30f, 0.5f));
+                x[n] = pr * vg[n];
+                most = max(most, __builtin_bit_cast(uint32_t, x[n]));
+            }
+            most = max(most, dpp_bits<kDppRor8>(most));
+            most = max(most, dpp_bits<kDppRor4>(most));
+            most = max(most, dpp_bits<kDppXor2>(most));
+            most = max(most, dpp_bits<kDppXor1>(most));
+            const int ew = min(max((int)(most >> 23), 29), 127);
+            const float up = pow2_field(283 - ew);  // brings the largest below 2^30
+            // 2^(ev - 126) 2^(ew - 126) 2^-30
+            back[s] = __shfl(__builtin_ldexpf(1.0f, ew + ev - 282), (j >> 2) * 16, kWave);
+            if (odd) back[s] = __builtin_nanf("");
+            uint8_t* const to = w_s[w][s] + 4 * grp * kI8Pitch + j;
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+            {
+                const uint32_t d = digits((uint32_t)__builtin_fmaf(x[n], up, 0.5f));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) to[i * kI8Pitch + 16 * n] = (uint8_t)(d >> (8 * i));
             }
@@ -1041,7 +1059,7 @@ __global__ __launch_bounds__(64 * W) void k_pages_attn_i8(PagesArgs a, PoolsI8 p
             {
                 const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, vf[i]), wd, v4i{}, 0, 0, 0);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[s][i][e] = __builtin_fmaf((float)d[e], back, acc[s][i][e]);
+                for (int e = 0; e < 4; ++e) acc[s][i][e] = __builtin_fmaf((float)d[e], back[s], acc[s][i][e]);
             }
         }
         wave_lds_fence();

@@ -48,6 +48,51 @@ def expected(K, V, dk, scale, n, run, weight):
     return want, tol + weight * runs.sum() * 127 * 0.5 + 2.0 ** -22 * (p @ np.abs(V[:n]))
 
 
+@pytest.mark.parametrize("H,Hkv,dk", [(1, 1, 64), (8, 1, 128), (4, 1, 256)])
+@pytest.mark.parametrize("n,B,gap,at", [(1024, 2, 28.0, 0), (1024, 2, 40.0, 700), (16384, 600, 31.0, 0), (16384, 600, 31.0, 9000), (4096, 1, 35.0, 5)])
+def test_decode_of_a_sink(ctx, nnhip, H, Hkv, dk, n, B, gap, at):
+    print(f"decode H={H} Hkv={Hkv} dk={dk} n={n} B={B} gap={gap} at={at}", flush=True)
+    cache, K, V, scale = sink(nnhip, n, gap, B, Hkv, dk, at=at)
+    q = dev(np.ones((B, H * dk), F32))
+    out = host(ctx.attention_pages_decode(cache, q, None, None, H, dev(np.full(B, n - 1, np.int32)), n, scale, tokens=True))
+    out = out.reshape(B, H, dk).astype(np.float64)
+    assert np.isfinite(out).all()
+    want, tol = expected(K, V, dk, scale, n, 64, 2.0 ** -31)
+    worst = float(np.max(np.abs(out - want) / tol))
+    print(f"  share {abs(want[0]) / 38.5:.2e}, bound {np.max(tol / np.abs(want)):.2e} of it, worst {worst:.3f} of the bound", flush=True)
+    assert worst <= 1.0
+
+
+def test_decode_of_a_large_value_without_weight(ctx, nnhip):
+    """A block with a value 2^40 times the others' and 2^-60 of their weight: the others' weights keep their bits beside it in a tile."""
+    n, dk = 512, 64
+    cache, K, V, scale = sink(nnhip, n, 0.0, 1, 1, dk, block=16, page=64)
+    # positions 16 .. 31: scores 60 log2 units below the others', values of 100 * 2^40 at position 20 and of 0
+    k = host(cache.k).copy()
+    v = host(cache.v).copy()
+    vs = host(cache.v_scale).copy()
+    ks = host(cache.k_scale).copy()
+    k[0, 0, 1] = -127
+    ks[0, 0, 1] = 60 * math.log(2) / (dk * 127 * scale)
+    v[0, 0, 1] = 0
+    v[0, 0, 1, :, 4] = 100
+    vs[0, 0, 1] = 2.0 ** 40
+    rng = np.random.default_rng(3)
+    for x, y in ((cache.k, k), (cache.v, v), (cache.k_scale, ks), (cache.v_scale, vs)):
+        x.copy_(dev(y))
+    K, V = K.copy(), V.copy()
+    K[16:32], V[16:32] = -127.0 * float(F32(ks[0, 0, 1])), 0.0
+    V[20] = 100 * 2.0 ** 40
+    q = (1 + 0.3 * rng.standard_normal(dk)).astype(F32)
+    out = host(ctx.attention_pages_decode(cache, dev(q[:, None]), None, None, 1, dev(np.array([n - 1], np.int32)), n, scale))[:, 0].astype(np.float64)
+    want, tol = attend64(q.astype(np.float64), K, V, scale, 0.0, 0.0, np.zeros(n), np.ones(n, bool))
+    # of the tile's largest weight times scale, 2^-1 / 496 (2^40 2^-60 / 496 in that block)
+    tol = tol + 2.0 ** -31 * n * 127 * 0.5 / 496
+    worst = float(np.max(np.abs(out - want) / tol))
+    print(f"  worst {worst:.3f} of the bound", flush=True)
+    assert worst <= 1.0
+
+
 @pytest.mark.parametrize("slopes", [False, True])
 @pytest.mark.parametrize("H,Hkv,dk,B,T", [(32, 32, 64, 8, 5), (32, 32, 64, 2, 200), (16, 2, 128, 8, 40), (4, 4, 128, 1, 64)])
 @pytest.mark.parametrize("gap,at", [(32.0, 0), (37.0, 0), (33.0, 20000)])
