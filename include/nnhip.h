@@ -677,7 +677,8 @@ typedef struct nnhip_kv_pages
 /* Write the keys and values of packed prompts: k / v (Hkv*dk, M) feature-major, columns cu[b] ..
  * cu[b+1] - 1 = the new tokens of sequence b (cu: DEVICE (B + 1) int32, not falling, cu[B] <= M), token t at
  * position pos0[b] + t (pos0: DEVICE (B) int32, or NULL for 0). Keys are rotated at their positions with
- * rope_cos / rope_sin (rope_len, dk/2) from nnhip_rope_table (both NULL: no position encoding), bit for
+ * rope_cos / rope_sin (rope_len, dk/2) from nnhip_rope_table (both NULL: no position encoding, and rope_len, where it
+ * is not 0, bounds the positions alone: of keys that were rotated before), bit for
  * bit as nnhip_kv_cache_fill's; f16 pools get the nearest f16. Not written: columns of no sequence
  * (cu[B] and on), positions at or past table_stride * page_size or rope_len, pages outside the pool.
  * Two tokens of one call at one place of the pool leave there, for each element, either's. The paged form of
@@ -719,7 +720,7 @@ nnhip_status nnhip_attention_pages_decode(nnhip_ctx* ctx, const nnhip_kv_pages* 
  * could show take the f32 products). The sums' order depends on all sequences of the call. dk in {64, 128}, any
  * H / Hkv, H <= 65535, B * H < 2^22, H * dk * M < 2^29, with tables min(table_stride * page_size, rope_len) * dk
  * < 2^30. Columns of no sequence are not written. NaN: a sequence with more than t_bound
- * tokens, columns outside [0, M) or positions at or past table_stride * page_size or rope_len; a query that sees
+ * tokens, columns outside [0, M) or positions at or past table_stride * page_size or rope_len (as nnhip_kv_pages_fill's); a query that sees
  * a position whose page is outside the pool (other queries of its sequence may be NaN then, too). The paged form
  * of nnhip_attention_prefill (compute_layer_attention.hpp:1022-1083). */
 nnhip_status nnhip_attention_pages_prefill(nnhip_ctx* ctx, const nnhip_kv_pages* cache, const float* q, size_t M,

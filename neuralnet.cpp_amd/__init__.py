@@ -984,10 +984,14 @@ class Context:
             raise NNHipError(1, f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
         raise NNHipError(1, f"{name} must be contiguous")
 
-    def _rope(self, cos, sin, dk: int):
-        """Addresses and rows of the rope tables (None, None, 0 without)."""
+    def _rope(self, cos, sin, dk: int, limit: int = 0):
+        """Addresses and rows of the rope tables (None, None, limit without)."""
         if cos is None and sin is None:
-            return None, None, 0
+            if limit < 0:
+                raise NNHipError(1, "limit must be at least 0")
+            return None, None, limit
+        if limit:
+            raise NNHipError(1, "limit goes without tables, whose rows bound the positions")
         if cos is None or sin is None:
             raise NNHipError(1, "cos and sin go together")
         shape = (cos.shape[0], dk // 2)
@@ -1003,12 +1007,13 @@ class Context:
             raise NNHipError(1, f"cu must hold B + 1 offsets, B at most the page table's {cache.rows} rows")
         return B, self._arg(cu, i32, (B + 1,), "cu"), self._arg(pos0, i32, (B,), "pos0")
 
-    def kv_pages_fill(self, cache, k, v, cu, pos0=None, cos=None, sin=None) -> None:
+    def kv_pages_fill(self, cache, k, v, cu, pos0=None, cos=None, sin=None, limit: int = 0) -> None:
         """The keys and values k / v (Hkv*dk, M) of packed prompts (sequence b: columns cu[b] .. cu[b+1] - 1,
-        positions pos0[b] on) rotated into the pages of cache, a KVPages or a KVPagesI8 (which holds them quantized)."""
+        positions pos0[b] on) rotated into the pages of cache, a KVPages or a KVPagesI8 (which holds them quantized).
+        Not written: positions at or past the tables' rows, or without tables at or past limit (0: the page table's end)."""
         B, cu_p, pos0_p = self._packed(cache, cu, pos0)
         f32, M = self._torch.float32, k.shape[-1]
-        cs, sn, rows = self._rope(cos, sin, cache.dk)
+        cs, sn, rows = self._rope(cos, sin, cache.dk, limit)
         shape = (cache.Hkv * cache.dk, M)
         self._bind_stream()
         fn = "nnhip_kv_pages_fill_i8" if isinstance(cache, KVPagesI8) else "nnhip_kv_pages_fill"
@@ -1053,18 +1058,20 @@ class Context:
         return out
 
     def attention_pages_prefill(self, cache, q, cu, t_bound: int, H: int, scale: float, pos0=None, cos=None, sin=None,
-                                softcap: float = 0.0, slopes=None, prefix=None, out=None, distance: bool = False):
+                                softcap: float = 0.0, slopes=None, prefix=None, out=None, distance: bool = False,
+                                limit: int = 0):
         """Attention of packed prompts q (H*dk, M) (sequence b: columns cu[b] .. cu[b+1] - 1, at most t_bound <= M of
         them, positions pos0[b] on) over the pages of cache, which hold all their positions: causal, and bidirectional
         over the first prefix[b] positions (prefix (B) int32, or None). slopes (H) bias the scores by
         slopes[h] * (j - i), or with distance by -slopes[h] * |j - i|: for keys ahead of the query, inside a prefix,
-        these differ. Returns out (H*dk, M)."""
+        these differ. A sequence with positions at or past the tables' rows, or without tables at or past limit (0: the
+        page table's end), gets NaN. Returns out (H*dk, M)."""
         B, cu_p, pos0_p = self._packed(cache, cu, pos0)
         f32, M = self._torch.float32, q.shape[-1]
         shape = (H * cache.dk, M)
         if out is None:
             out = self._empty(shape, f32)
-        cs, sn, rows = self._rope(cos, sin, cache.dk)
+        cs, sn, rows = self._rope(cos, sin, cache.dk, limit)
         self._bind_stream()
         more = ()
         if isinstance(cache, KVPagesI8):

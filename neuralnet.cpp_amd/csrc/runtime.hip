@@ -253,6 +253,13 @@ nnhip_status check_pages(const char* fn, const nnhip_kv_pages_i8* c, const float
     return check_pages(fn, &p, rope_cos, rope_sin);
 }
 
+// Positions that have a place, of `places` of a page table: within the rows of the rope tables, or without those within
+// rope_len where it is given (keys that were rotated before)
+size_t position_limit(size_t places, const float* rope_cos, size_t rope_len)
+{
+    return rope_cos || rope_len > 0 ? std::min(places, rope_len) : places;
+}
+
 // The host's checks of a decode attention over pages
 template <typename Pages>
 nnhip_status check_decode(const char* fn, const Pages* cache, size_t B, size_t H, size_t len_bound, const float* rope_cos,
@@ -282,7 +289,7 @@ nnhip_status check_prompts(const char* fn, const Pages* cache, size_t M, size_t 
                   "softcap must be 0 or in [1e-30, 1e30]");
     NNHIP_REQUIRE(t_bound <= M, fn, "t_bound must not exceed M");
     limit = cache->table_stride * cache->page_size;
-    if (rope_cos) limit = std::min(limit, rope_len);
+    limit = position_limit(limit, rope_cos, rope_len);
     NNHIP_REQUIRE(!rope_cos || limit * cache->dk < (size_t(1) << 30), fn, "rope tables must be below 2 GiB");
     NNHIP_REQUIRE(B < (size_t(1) << 22) && B * H < (size_t(1) << 22), fn, "B * H must be below 2^22");
     return NNHIP_OK;
@@ -2112,7 +2119,7 @@ nnhip_status nnhip_kv_pages_fill(nnhip_ctx* ctx, const nnhip_kv_pages* cache, co
     NNHIP_REQUIRE(k && v && cu, fn, "null pointer");
     NNHIP_REQUIRE(B < kMaxDim && M < kMaxDim - 64, fn, "M or B too large");
     size_t limit = cache->table_stride * cache->page_size;
-    if (rope_cos) limit = std::min(limit, rope_len);
+    limit = position_limit(limit, rope_cos, rope_len);
     NNHIP_LAUNCH(fn, launch_pages_fill(ctx->stream, *cache, k, v, M, cu, pos0, B, rope_cos, rope_sin, limit));
     return NNHIP_OK;
 }
@@ -2198,7 +2205,7 @@ nnhip_status nnhip_kv_pages_fill_i8(nnhip_ctx* ctx, const nnhip_kv_pages_i8* cac
     NNHIP_REQUIRE(k && v && cu, fn, "null pointer");
     NNHIP_REQUIRE(B < kMaxDim && M < kMaxDim - 190, fn, "M or B too large");
     size_t limit = cache->table_stride * cache->page_size;
-    if (rope_cos) limit = std::min(limit, rope_len);
+    limit = position_limit(limit, rope_cos, rope_len);
     if (limit == 0) return NNHIP_OK;  // (no position has a place)
     NNHIP_LAUNCH(fn, launch_pages_fill_i8(ctx->stream, *cache, k, v, M, cu, pos0, B, rope_cos, rope_sin, limit));
     return NNHIP_OK;

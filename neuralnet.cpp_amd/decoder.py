@@ -329,9 +329,10 @@ class Decoder:
         def attend(i):
             cache = self.caches[i]
             cos, sin = self._qk_norm(i, pf["q"], pf["k"], pf["pos"])
-            ctx.kv_pages_fill(cache, pf["k"], pf["v"], cu, pos0=pos0, cos=cos, sin=sin)
+            limit = cfg.max_len if cos is None and cfg.rope else 0  # (the tables' rows, with norms as without)
+            ctx.kv_pages_fill(cache, pf["k"], pf["v"], cu, pos0=pos0, cos=cos, sin=sin, limit=limit)
             ctx.attention_pages_prefill(cache, pf["q"], cu, t_bound, cfg.H, cfg.scale, pos0=pos0, cos=cos, sin=sin,
-                                        out=pf["a"])
+                                        out=pf["a"], limit=limit)
 
         x = self._prefill_blocks(ids, ids.shape[0], attend, hook)
         # (an empty first sequence, or offsets past the tokens, would be an index outside x)
