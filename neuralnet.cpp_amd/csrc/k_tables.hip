@@ -161,7 +161,7 @@ __global__ __launch_bounds__(kTbThreads) void k_pages_assign(AssignArgs a)
     if (threadIdx.x == 0)
     {
         a.cu[0] = 0;
-        *a.free_count = (int)(count - all[0]);
+        if (a.B > 0) *a.free_count = (int)(count - all[0]);
     }
     for (int b = b0; b < b1; ++b)
     {

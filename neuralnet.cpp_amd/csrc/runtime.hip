@@ -2297,10 +2297,15 @@ nnhip_status nnhip_pages_assign(nnhip_ctx* ctx, int32_t* table, size_t table_str
 {
     const char* fn = "nnhip_pages_assign";
     NNHIP_CHECK_CTX(fn);
-    if (B == 0) return NNHIP_OK;
-    nnhip_status st = check_table(fn, table, table_stride, page_size, num_pages, B);
-    if (st != NNHIP_OK) return st;
-    NNHIP_REQUIRE(free_pages && free_count && lens && add && cu && pos0, fn, "null pointer");
+    nnhip_status st = NNHIP_OK;
+    if (B > 0)
+    {
+        st = check_table(fn, table, table_stride, page_size, num_pages, B);
+        if (st != NNHIP_OK) return st;
+        NNHIP_REQUIRE(free_pages && free_count && lens && add && cu && pos0, fn, "null pointer");
+    }
+    else if (!cu || !free_count) return NNHIP_OK;
+    else table_stride = 1, page_size = 8, num_pages = 0;  // no sequence: cu[0] and the tokens alone are written, nothing is read
     NNHIP_REQUIRE(M < kMaxDim - 256, fn, "M too large");
     void* ws = nullptr;
     st = ensure_stream_ws(ctx, pages_assign_workspace_bytes(B, M, M > 0 && (pos || slots)), fn, &ws);
@@ -2315,10 +2320,15 @@ nnhip_status nnhip_pages_slots(nnhip_ctx* ctx, const int32_t* table, size_t tabl
 {
     const char* fn = "nnhip_pages_slots";
     NNHIP_CHECK_CTX(fn);
-    if (B == 0 || M == 0) return NNHIP_OK;
-    const nnhip_status st = check_table(fn, table, table_stride, page_size, num_pages, B);
-    if (st != NNHIP_OK) return st;
-    NNHIP_REQUIRE(cu && (pos || slots), fn, "null pointer");
+    if (M == 0) return NNHIP_OK;
+    if (B > 0)
+    {
+        const nnhip_status st = check_table(fn, table, table_stride, page_size, num_pages, B);
+        if (st != NNHIP_OK) return st;
+        NNHIP_REQUIRE(cu && (pos || slots), fn, "null pointer");
+    }
+    else if (!pos && !slots) return NNHIP_OK;
+    else table_stride = 1, page_size = 8, num_pages = 0;  // no sequence: every token is of none
     NNHIP_REQUIRE(M < kMaxDim - 256, fn, "M too large");
     NNHIP_LAUNCH(fn, launch_pages_slots(ctx->stream, table, table_stride, page_size, num_pages, cu, pos0, B, M, pos, slots));
     return NNHIP_OK;
