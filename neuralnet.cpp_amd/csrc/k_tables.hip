@@ -107,7 +107,8 @@ __device__ __forceinline__ void put_token(const int32_t* table, int table_stride
 }
 
 // The last i of n with x[i] <= at (x not falling, x[0] <= at)
-__device__ __forceinline__ int bisect(const int* x, int n, int at)
+template <typename T>
+__device__ __forceinline__ int bisect(const T* x, int n, T at)
 {
     int lo = 0;
     while (n > 1)
@@ -285,7 +286,8 @@ template <bool kOne>
 __global__ __launch_bounds__(kTbThreads) void k_pages_release(ReleaseArgs a)
 {
     __shared__ int64_t pages_s[kTbWaves][1];
-    __shared__ int page_s[kOne ? kOneB : 1], first_s[kOne ? kOneB : 1];
+    __shared__ int64_t page_s[kOne ? kOneB : 1];  // (of pages in more than one row the sums may be anything: past 2^31, too)
+    __shared__ int first_s[kOne ? kOneB : 1];
     const int b0 = min((int)threadIdx.x * a.run, a.B), b1 = min(b0 + a.run, a.B);
     const int64_t count = min(max(*a.free_count, 0), a.num_pages);
     int first_first = 0, first_kept = 0, first_n = 0;
@@ -312,21 +314,20 @@ __global__ __launch_bounds__(kTbThreads) void k_pages_release(ReleaseArgs a)
         const int n = gives(b, first, kept);
         if (kOne)
         {
-            page_s[b] = (int)pages;
+            page_s[b] = pages;
             first_s[b] = first;
         }
-        else a.moves[b] = make_int4(first, n, (int)(count + total - 1 - pages), 0);
+        else a.moves[b] = make_int4(first, n, (int)min(count + total - 1 - pages, (int64_t)0x7FFFFFFF), 0);
         pages += n;
         if (kept >= 0) a.lens[b] = kept;
     }
     if constexpr (kOne)
     {
         __syncthreads();
-        for (int64_t i = threadIdx.x; i < total; i += kTbThreads)
+        for (int64_t i = count + total - top + threadIdx.x; i < total; i += kTbThreads)
         {
-            const int b = bisect(page_s, a.B, (int)i);
-            const int64_t to = count + total - 1 - i;
-            if (to < a.num_pages) a.free_pages[to] = a.table[(size_t)b * a.table_stride + first_s[b] + ((int)i - page_s[b])];
+            const int b = bisect(page_s, a.B, i);
+            a.free_pages[count + total - 1 - i] = a.table[(size_t)b * a.table_stride + first_s[b] + (int)(i - page_s[b])];
         }
     }
 }

@@ -28,3 +28,22 @@ def test_no_sequence(ctx, nnhip, M):
         assert np.all(host(only) == -1)
         ctx.pages_release(table, 16, free, count, none, none)
         assert int(host(count)[0]) == pages
+
+
+@pytest.mark.parametrize("B", [18, 300])
+def test_release_of_too_many(ctx, nnhip, B):
+    """Rows that hold more pages than there are, 2^31 of them in all: the list is full then, of pages that the rows name."""
+    import torch
+    page, width = 8, 2 ** 31 // B + 8000
+    table = (torch.arange(width, dtype=torch.int32, device="cuda") % 40)[None, :].repeat(B, 1)
+    free, count = dev(np.arange(40, dtype=I32)), dev(np.array([10], I32))
+    lens, keep = dev(np.full(B, page * width, I32)), dev(np.zeros(B, I32))
+    assert B * width > 2 ** 31 and page * width <= 2 ** 30
+    ctx.pages_release(table, page, free, count, lens, keep)
+    assert int(host(count)[0]) == 40 and not host(lens).any()
+    got = host(free)
+    assert np.array_equal(got[:10], np.arange(10)) and got.min() >= 0 and got.max() < 40
+    # the last of them were the last to be put down: the last sequence's last pages, upwards
+    assert np.array_equal(got[10:], (width - 1 - np.arange(30)) % 40)
+    del table
+    torch.cuda.empty_cache()
