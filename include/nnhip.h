@@ -764,7 +764,7 @@ typedef struct nnhip_kv_pages_i8
 
 /* nnhip_kv_pages_fill into a cache in 8 bits: the same arguments, the same tokens left out. A sequence's tokens are taken
  * to be new: those at its positions from pos0[b] on and behind are written over, or mean nothing. Two sequences of one
- * call that write into one block of the pool leave anything there. M <= 2^31 - 192. */
+ * call that write into one block of the pool leave anything there. M < 2^29 - 64. */
 nnhip_status nnhip_kv_pages_fill_i8(nnhip_ctx* ctx, const nnhip_kv_pages_i8* cache, const float* k, const float* v,
                                     size_t M, const int32_t* cu, const int32_t* pos0, size_t B, const float* rope_cos,
                                     const float* rope_sin, size_t rope_len);
@@ -803,7 +803,7 @@ nnhip_status nnhip_attention_pages_prefill_i8(nnhip_ctx* ctx, const nnhip_kv_pag
  * nnhip_attention_decode rotates (rope_cos / rope_sin (rope_len, dk/2), both NULL: no rotation). q (H*dk, M), k (Hkv*dk, M)
  * feature-major, or with tokens != 0 (M, H*dk), (M, Hkv*dk); q_out, k_out like them (may be q and k themselves, no other overlap).
  * q or k may be NULL (with its output); gamma_q, gamma_k (dk), NULL: a gain of 1. pos (M) int32, DEVICE, NULL without
- * tables: a token with pos[m] < 0 is left as its output is, one at or past rope_len gets NaN. dk in {64, 128, 256}; M * (H + Hkv) < 2^31.
+ * tables: a token with pos[m] < 0 is left as its output is, one at or past rope_len gets NaN. dk in {64, 128, 256}; M * (H + Hkv) < 2^31, M * (H + Hkv) * dk < 2^35.
  * The attention that follows takes no tables. No counterpart in the reference, whose attention has no such norms; per head the step of
  * RMSNorm::forward (compute_layer_mlp.hpp:686-707) and of RotaryEmbedding (compute_position_encoding.hpp:150-166). */
 nnhip_status nnhip_qk_norm_rope(nnhip_ctx* ctx, const float* q, const float* k, size_t M, size_t H, size_t Hkv, size_t dk,

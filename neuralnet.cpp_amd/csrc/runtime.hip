@@ -2203,7 +2203,8 @@ nnhip_status nnhip_kv_pages_fill_i8(nnhip_ctx* ctx, const nnhip_kv_pages_i8* cac
     if (st != NNHIP_OK) return st;
     if (M == 0 || B == 0) return NNHIP_OK;
     NNHIP_REQUIRE(k && v && cu, fn, "null pointer");
-    NNHIP_REQUIRE(B < kMaxDim && M < kMaxDim - 190, fn, "M or B too large");
+    // (8 threads to a column, of which a launch takes fewer than 2^32)
+    NNHIP_REQUIRE(B < kMaxDim && M < (size_t(1) << 29) - 64, fn, "M or B too large");
     size_t limit = cache->table_stride * cache->page_size;
     limit = position_limit(limit, rope_cos, rope_len);
     if (limit == 0) return NNHIP_OK;  // (no position has a place)
@@ -2285,7 +2286,9 @@ nnhip_status nnhip_qk_norm_rope(nnhip_ctx* ctx, const float* q, const float* k, 
     NNHIP_REQUIRE(!rope_cos || (pos && rope_len >= 1), fn, "the rotation needs positions, and tables with a row");
     if (M == 0 || (!q && !k)) return NNHIP_OK;
     NNHIP_REQUIRE((!q || H >= 1) && (!k || Hkv >= 1) && H <= 65535 && Hkv <= 65535, fn, "H and Hkv must be in [1, 65535]");
-    NNHIP_REQUIRE(M < kMaxDim - 64 && M * (H + Hkv) < kMaxDim, fn, "M * (H + Hkv) must be below 2^31");
+    // (dk / 8 threads to a head of a token, of which a launch takes fewer than 2^32)
+    NNHIP_REQUIRE(M < kMaxDim - 64 && M * (H + Hkv) < kMaxDim && M * (H + Hkv) * dk < (size_t(1) << 35), fn,
+                  "M * (H + Hkv) must be below 2^31, M * (H + Hkv) * dk below 2^35");
     NNHIP_LAUNCH(fn, launch_qk_norm_rope(ctx->stream, q, k, M, H, Hkv, dk, gamma_q, gamma_k, eps, pos, rope_cos, rope_sin,
                                          rope_len, tokens != 0, q_out, k_out, (size_t)ctx->num_cus));
     return NNHIP_OK;
