@@ -110,6 +110,8 @@ class Decoder:
     def __init__(self, ctx, cfg: Config, blocks: List[Block], emb, g_final, head: Linear, B: int, caches=None):
         import torch
 
+        if any((blk.g_q is None) != (blk.g_k is None) for blk in blocks):
+            raise _pkg().NNHipError(1, "g_q and g_k go together")
         self.ctx, self.cfg, self.blocks, self.emb, self.g_final, self.head, self.B = \
             ctx, cfg, blocks, emb, g_final, head, B
         dev = f"cuda:{ctx.device}"

@@ -89,3 +89,14 @@ def test_limit_alone(ctx, nnhip):
             ctx.kv_pages_fill(cache, lay(k), lay(v), cu, **kw)
         with pytest.raises(nnhip.NNHipError, match="limit"):
             ctx.attention_pages_prefill(cache, q, cu, n, H, 0.125, **kw)
+
+
+def test_one_gain_alone(ctx, nnhip):
+    """A block with one of the two gains is refused with the decoder, before any block has run."""
+    from nnhip_py import decoder as dmod
+    cfg = dmod.Config(d=256, H=4, Hkv=2, F=320, vocab=97, max_len=50, act=0, eps=1e-5)
+    base = _gpu_model(ctx, nnhip, cfg, 2, 2, 0x52, subln=True)[0]
+    g = dev(np.ones(cfg.dk, F32))
+    for kw in (dict(g_q=g), dict(g_k=g)):
+        with pytest.raises(nnhip.NNHipError, match="go together"):
+            dmod.Decoder(ctx, cfg, [base.blocks[0], dataclasses.replace(base.blocks[1], **kw)], base.emb, base.g_final, base.head, 2)
