@@ -389,7 +389,9 @@ __device__ __forceinline__ FillWindow find_window(const FillI8Args& a, int item)
 // The same for long prompts: work-group = (window of 64 positions of a sequence, KV head, keys or values), lane = position. A
 // window holds whole blocks and groups, so maxima are those of neighbouring lanes, and the values' bytes are
 // turned 4 x 4 between the lanes of a quad, which leaves words of 4 positions for LDS. 16 x 1111 .. 2048 tokens of 5 heads of
-// 128: 52 us, 3.1 TB/s, bound by HBM and the f32 columns' runs of 256 bytes, which begin anywhere.
+// 128: 51 us, 3.1 TB/s, where a copy's 32 us are the floor. A lane takes one column, so rows are read in runs of 256 bytes that
+// begin anywhere; and the work-groups past the last window lie on the last XCDs, with nothing to do there (a quarter of them at
+// 16 x 300 tokens, 14.2 us, half at 64 x 128, 24.4).
 template <int DK>
 __global__ __launch_bounds__(256, DK == 256 ? 3 : 5) void k_windows_fill_i8(FillI8Args a)
 {
@@ -756,16 +758,18 @@ __device__ __forceinline__ float pow2_field(int field) { return __builtin_bit_ca
 //           the tile's 64 positions are exact, and each is added to an f32 sum of its own, joined at the end. (Under the
 //           reference of the whole wave thousands of small weights beside a large one were lost, under the tile's largest
 //           scale those beside a large value without weight.)
-// So neither codes are converted nor multiplied by their scales one by one: 190 VALU instructions a tile of 64
-// positions for 4 heads of 128, where multiply-adds on widened elements would take 1300.
+// So neither codes are converted nor multiplied by their scales one by one: 330 VALU instructions a tile of 64
+// positions for 4 heads of 128 (counted at 8), where multiply-adds on widened elements would take 1300.
 // A head's reference maximum moves when a score passes it, to 4 above that score (weights are 2^-4 at most then and
 // 1 at most later).
 // The chunk that holds the new position writes its key and value, by the wave that reads them (no other wave reads that
 // block), and takes their codes into its operands from LDS: its tile is on its way meanwhile, and is read again only
-// where the block's older codes have changed.
+// where the block's older codes have changed (16 x 64 .. 4200, alone: 21.7 us where no block's scale is raised, 40.0 where every one is).
 // A block whose scale is not finite (its tokens had an infinity) stands for NaN, and so does a query with one.
-// 6 x 50000 .. 131072 positions, 8 heads to each of 4 KV heads of 128: 100 us, 6.0 TB/s, bound by HBM; 16 x 64 .. 4200, 4 to each of
-// 5: 12.2 us and 3.9 for the join, 1 x 100: 7.3, bound by the chain of round trips from position to page to rows to output.
+// 6 x 50000 .. 131072 positions, 8 heads to each of 4 KV heads of 128: 101 us, 5.9 TB/s, bound by HBM; 16 x 64 .. 4200, 4 to each of
+// 5: 12.0 us and 4.0 for the join, 1 x 100: 7.4, bound by the chain of round trips from position to page to rows to output.
+// Heads of 256 go 4 at a time, for their registers: where a KV head has more, each 4 read all codes again, and the token is
+// appended in a launch of its own (16 x 4000 .. 16000 over 1 KV head, 76 MB: 4 heads 33 us, 8 heads 47).
 template <int DK, int NS, int W, bool kFinal>
 __global__ __launch_bounds__(64 * W) void k_pages_attn_i8(PagesArgs a, PoolsI8 pools, int append)
 {
@@ -1216,7 +1220,8 @@ hipError_t launch_pages_fill_i8(hipStream_t st, const nnhip_kv_pages_i8& kv, con
 {
     const FillI8Args a{k, v, cu, pos0, cosT, sinT, pools_of(kv), kv.table, (int)M, (int)B, (int)kv.Hkv, log2_of(kv.page_size),
                        (int)kv.table_stride, (int)kv.num_pages, (int)limit};
-    // sequences of 128 tokens or more on average: windows of their positions, of which there are at most M / 64 + 2 B (by
+    // sequences of 128 tokens or more on average (the lengths are on the device: one long prompt among many short ones goes by
+    // columns): windows of their positions, of which there are at most M / 64 + 2 B (by
     // windows and by columns, with the values read back, us: 16 x 64 tokens of 5 heads of 128 15.0 and 13.4, x 128 18.9 and 18.5, x 300 22.7 and 27.8)
     if (M >= 2 * kPfTok * B)
     {

@@ -21,9 +21,11 @@
 // products and by the other half behind them, so that every SIMD has one of each. A tile that every query of the wave sees
 // goes in one piece, a group's weights between the last group's products (in two halves, each step by itself: 477 us for 446).
 // Work-groups take equal spans of all tiles and join the items they share (prompt_spans.hpp).
-// 4 x 700 .. 1024 queries at 6144, 20 heads over 5 of 128: 432 us and 20 for the join, 1.06 PFLOP/s of products (a large
-// library product of f16: 1.15), bound by them and the softmax beside them, to which the f32 exponential and the weights' splitting
-// contribute most; 8 x 77 .. 1900 of 16 over 2 of 64, capped and biased: 61 and 9, bound by the VALU (25 instructions a score).
+// 4 x 700 .. 1024 queries at 6144, 20 heads over 5 of 128: 434 us and 20 for the join, 1.06 PFLOP/s of products (a large
+// library product of f16: 1.16); the matrix cores are busy for half of the cycles and the VALU's 10 instructions a score, most of them the f32
+// exponential and the weights' splitting, take most of the rest. 8 x 77 .. 1900 of 16 over 2 of 64, capped and biased: 69 us and 9, of which the
+// VALU (23 instructions a score) takes about half and the matrix cores 15 %: a CU has one work-group, so an item's start, 4 to 5 us
+// before its first product, has nothing beside it, and nearly every span ends in a record.
 // A query that holds an infinity or a NaN gets NaN, and so does one that sees a block whose scale is not finite.
 #include "prompt_spans.hpp"
 
